@@ -592,6 +592,89 @@ typedef struct atk_conv_prepacked_args {
 } atk_conv_prepacked_args;
 int atk_conv_fwd_prepacked_args(const atk_conv_prepacked_args* a);
 
+/* ---------------------------------------------------------------------------
+ * Root-mean-square norm over the last axis, with the residual's addition in front and an 8-bit
+ * output behind (the reference's norms of this kind are Triton and TransformerEngine tiers,
+ * amd_tuned_torch/fused_norm_ops.py, te_ops.py):
+ *   h = x + residual, rounded to `dtype`      (residual NULL: h = x, and h is not written)
+ *   y = h * rstd * weight,  rstd = 1 / sqrt(mean(h^2) + eps)            (weight NULL: ones)
+ * x, residual: M rows of N elements, rows x_stride / residual_stride elements apart; y and h dense.
+ * weight [N] of `dtype` or fp32 (w_dtype).  rstd [M] fp32 is written when given (for the backward).
+ * quant ATK_QUANT_FP8 / ATK_QUANT_INT8: y holds 8-bit values (fp8 e4m3, top 448; int8, top 127) and
+ * scales [M, ceil(N / group)] fp32 what they are multiplied by: max(max|y| / top, 2^-126) over each
+ * run of `group` columns (16..256, a power of two), or over the row where group is 0.  A row of
+ * zeros gives zeros.  N up to 65536 (fp32: 32768), rows of any alignment.
+ * ------------------------------------------------------------------------- */
+enum { ATK_QUANT_NONE = 0, ATK_QUANT_FP8 = 1, ATK_QUANT_INT8 = 2 };
+typedef struct atk_rms_norm_args {
+  const void* x; const void* residual; const void* weight; void* y; void* h; float* rstd; float* scales;
+  int64_t M; int64_t N; int64_t x_stride; int64_t residual_stride;
+  int group; float eps; int dtype; int w_dtype; int quant;
+  atk_stream_t stream;
+} atk_rms_norm_args;
+int atk_rms_norm_fwd(const atk_rms_norm_args* a);
+
+/* Its backward: dx = rstd (w dy - h rstd^2 mean(w dy h)) + dh (the gradient of x and of the residual
+ * alike; dh NULL: none) and dw [N] of w_dtype = sum over rows of dy h rstd (NULL: not wanted).  h, dy,
+ * dh: rows their strides apart; dx dense.  dw needs atk_rms_norm_bwd_workspace_bytes of scratch
+ * (contents ignored) and is summed in a fixed order. */
+size_t atk_rms_norm_bwd_workspace_bytes(int64_t M, int64_t N, int dtype);
+int atk_rms_norm_bwd(const void* h, const void* dy, const void* dh, const void* weight, const float* rstd, void* dx,
+                     void* dw, int64_t M, int64_t N, int64_t h_stride, int64_t dy_stride, int64_t dh_stride, int dtype,
+                     int w_dtype, void* workspace, size_t workspace_bytes, atk_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * The gated delta rule (no counterpart in the reference; the mixer that follows its causal conv1d in
+ * linear-attention blocks).  For each sequence and value head h, with key head h / (Hv / Hk), the
+ * state S [K, V] in fp32:
+ *   S~ = exp(g_t) S;  u = beta_t (v_t - S~^T k_t);  S <- S~ + k_t u^T;  out_t = scale S^T q_t
+ * One token of each of N sequences: q, k (N, Hk, K), v (N, Hv, V) and out (N, Hv, V, dense) of
+ * `dtype`; g (the logarithm of the decay) and beta (N, Hv) of `dtype` or fp32.  The last axis of q, k
+ * and v is dense, the others have strides (in elements).  state (slots, Hv, K, V) is updated in place,
+ * dense but for its first axis' state_stride; state_indices (int32, N) says which slot a sequence has
+ * (NULL: its own number).  A sequence whose index is outside [0, slots) is padding: its output is zero
+ * and no state changes.  No two sequences may share a slot.  K up to 256.
+ * ------------------------------------------------------------------------- */
+typedef struct atk_gated_delta_update_args {
+  const void* q; const void* k; const void* v; const void* g; const void* beta;
+  void* state; void* out; const int* state_indices;
+  int64_t N; int64_t slots; int64_t state_stride;
+  int64_t q_stride_n; int64_t q_stride_h; int64_t k_stride_n; int64_t k_stride_h;
+  int64_t v_stride_n; int64_t v_stride_h; int64_t g_stride_n; int64_t g_stride_h;
+  int64_t beta_stride_n; int64_t beta_stride_h;
+  int Hk; int Hv; int K; int V; int dtype; int g_dtype; int beta_dtype; float scale;
+  atk_stream_t stream;
+} atk_gated_delta_update_args;
+int atk_gated_delta_update(const atk_gated_delta_update_args* a);
+
+/* The same rule over whole sequences: q, k (N, T, Hk, K), v (N, T, Hv, V), g and beta (N, T, Hv), out
+ * (N, T, Hv, V), dense.  Strides are those of the first three axes, in elements; the last axis of q, k
+ * and v is dense.  initial_state (N, Hv, K, V) fp32 or NULL (zeros); final_state likewise is written
+ * when given.  cu_seqlens (int32, N + 1, on the device): the N sequences are packed into one row of T
+ * tokens (first axis 1), sequence n from cu_seqlens[n] to cu_seqlens[n + 1]; offsets must not decrease
+ * and are clamped to the row, and tokens of no sequence get an output of zero.  The workspace (16-byte
+ * aligned, contents ignored) has atk_gated_delta_workspace_bytes of the same arguments. */
+typedef struct atk_gated_delta_args {
+  const void* q; const void* k; const void* v; const void* g; const void* beta;
+  const void* initial_state; void* final_state; void* out; const int* cu_seqlens;
+  int64_t q_stride[3]; int64_t k_stride[3]; int64_t v_stride[3]; int64_t g_stride[3]; int64_t beta_stride[3];
+  int64_t N; int64_t T;
+  int Hk; int Hv; int K; int V; int dtype; int g_dtype; int beta_dtype; float scale;
+  void* workspace; size_t workspace_bytes;
+  atk_stream_t stream;
+} atk_gated_delta_args;
+size_t atk_gated_delta_workspace_bytes(const atk_gated_delta_args* a);
+int atk_gated_delta_fwd(const atk_gated_delta_args* a);
+
+/* Its backward.  The arguments and inputs of the forward (out and final_state are not read, the
+ * workspace has atk_gated_delta_bwd_workspace_bytes), dout (N, T, Hv, V, dense, `dtype`) and
+ * dfinal_state (fp32, like final_state; NULL: zeros).  Writes dq, dk (N, T, Hk, K), dv (N, T, Hv, V),
+ * dg and dbeta (N, T, Hv), all dense and of their tensors' types, and dinitial_state (fp32) when given.
+ * Sums over the value heads of a key head have a fixed order.  Tokens of no sequence are not written. */
+size_t atk_gated_delta_bwd_workspace_bytes(const atk_gated_delta_args* a);
+int atk_gated_delta_bwd(const atk_gated_delta_args* a, const void* dout, const void* dfinal_state, void* dq, void* dk,
+                        void* dv, void* dg, void* dbeta, void* dinitial_state);
+
 #ifdef __cplusplus
 }
 #endif

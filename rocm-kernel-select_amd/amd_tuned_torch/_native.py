@@ -53,6 +53,8 @@ EXPORTED_SYMBOLS = (
     "atk_group_norm_apply", "atk_group_norm_cl_bwd_workspace_bytes", "atk_group_norm_cl_bwd",
     "atk_dwconv1d_fwd_args", "atk_group_norm_fwd_args", "atk_conv_fwd_prepacked_args",
     "atk_causal_conv1d_update_args_fwd",
+    "atk_rms_norm_fwd", "atk_rms_norm_bwd_workspace_bytes", "atk_rms_norm_bwd", "atk_gated_delta_update",
+    "atk_gated_delta_workspace_bytes", "atk_gated_delta_fwd", "atk_gated_delta_bwd_workspace_bytes", "atk_gated_delta_bwd",
 )
 
 
@@ -95,6 +97,32 @@ class _ConvArgs(ctypes.Structure):
                 + [(f, ctypes.c_int) for f in _CONV_GEOM_FIELDS[6:]]
                 + [("dtype", ctypes.c_int), ("variant", ctypes.c_int), ("workspace", ctypes.c_void_p),
                    ("workspace_bytes", ctypes.c_size_t), ("stream", ctypes.c_void_p)])
+
+
+class _RmsArgs(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("x", "residual", "weight", "y", "h", "rstd", "scales")]
+                + [(f, ctypes.c_int64) for f in ("M", "N", "x_stride", "residual_stride")]
+                + [("group", ctypes.c_int), ("eps", ctypes.c_float), ("dtype", ctypes.c_int),
+                   ("w_dtype", ctypes.c_int), ("quant", ctypes.c_int), ("stream", ctypes.c_void_p)])
+
+
+class _DeltaUpdateArgs(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("q", "k", "v", "g", "beta", "state", "out", "state_indices")]
+                + [(f, ctypes.c_int64) for f in ("N", "slots", "state_stride", "q_stride_n", "q_stride_h", "k_stride_n",
+                                                 "k_stride_h", "v_stride_n", "v_stride_h", "g_stride_n", "g_stride_h",
+                                                 "beta_stride_n", "beta_stride_h")]
+                + [(f, ctypes.c_int) for f in ("Hk", "Hv", "K", "V", "dtype", "g_dtype", "beta_dtype")]
+                + [("scale", ctypes.c_float), ("stream", ctypes.c_void_p)])
+
+
+class _DeltaArgs(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("q", "k", "v", "g", "beta", "initial_state", "final_state", "out",
+                                                "cu_seqlens")]
+                + [(f, ctypes.c_int64 * 3) for f in ("q_stride", "k_stride", "v_stride", "g_stride", "beta_stride")]
+                + [("N", ctypes.c_int64), ("T", ctypes.c_int64)]
+                + [(f, ctypes.c_int) for f in ("Hk", "Hv", "K", "V", "dtype", "g_dtype", "beta_dtype")]
+                + [("scale", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+                   ("stream", ctypes.c_void_p)])
 
 
 _tls = threading.local()
@@ -219,13 +247,24 @@ def _declare(lib) -> None:
     lib.atk_dwconv1d_bwd.restype = i32
     lib.atk_group_norm_trace.argtypes = [vp, i64]
     lib.atk_group_norm_trace.restype = i32
+    lib.atk_gated_delta_workspace_bytes.argtypes = [vp]
+    lib.atk_gated_delta_workspace_bytes.restype = sz
+    lib.atk_gated_delta_bwd_workspace_bytes.argtypes = [vp]
+    lib.atk_gated_delta_bwd_workspace_bytes.restype = sz
+    lib.atk_gated_delta_bwd.argtypes = [vp] * 9
+    lib.atk_gated_delta_bwd.restype = i32
+    lib.atk_rms_norm_bwd_workspace_bytes.argtypes = [i64, i64, i32]
+    lib.atk_rms_norm_bwd_workspace_bytes.restype = sz
+    lib.atk_rms_norm_bwd.argtypes = [vp] * 7 + [i64] * 5 + [i32, i32, vp, sz, vp]
+    lib.atk_rms_norm_bwd.restype = i32
     lib.atk_group_norm_noalloc_scratch_bytes.argtypes = []
     lib.atk_group_norm_noalloc_scratch_bytes.restype = sz
     lib.atk_group_norm_fwd_noalloc.argtypes = [vp, vp, vp, vp, i64, i64, i64, i32, c.c_float, i32, i32, i32,
                                                i32, vp]
     lib.atk_group_norm_fwd_noalloc.restype = i32
     for name in ("atk_dwconv1d_fwd_args", "atk_group_norm_fwd_args", "atk_conv_fwd_prepacked_args",
-                 "atk_causal_conv1d_update_args_fwd"):
+                 "atk_causal_conv1d_update_args_fwd", "atk_rms_norm_fwd", "atk_gated_delta_update",
+                 "atk_gated_delta_fwd"):
         getattr(lib, name).argtypes = [vp]
         getattr(lib, name).restype = i32
 
@@ -1492,3 +1531,254 @@ def conv_wgrad(x: torch.Tensor, dy: torch.Tensor, kd: int, *, bias_grad: bool = 
                                  _DTYPE_CODE[x.dtype], _DTYPE_CODE[out_dtype], _ptr(ws), ws.numel(), _stream(x))
     _check(rc, "conv_wgrad")
     return (dw, db) if bias_grad else dw
+
+
+# ---------------------------------------------------------------------------
+# Root-mean-square norm and the gated delta rule
+# ---------------------------------------------------------------------------
+QUANT_DTYPES = {torch.float8_e4m3fn: 1, torch.int8: 2}
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t as the row kernels take it: unit stride along the last axis and one stride between rows (a
+    copy where it has none)."""
+    if t.is_contiguous():
+        return t
+    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+        return t
+    if t.dim() > 2 and t.stride(-1) == 1 and t.stride(-2) >= t.shape[-1]:
+        if all(t.stride(i) == t.stride(i + 1) * t.shape[i + 1] for i in range(t.dim() - 2)):
+            return t
+    return t.contiguous()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(-2) if t.dim() > 1 else t.shape[-1]
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float, residual: Optional[torch.Tensor] = None,
+             *, quant: Optional[torch.dtype] = None, group: int = 0, want_rstd: bool = False):
+    """(y, h, rstd, scales) of the norm over x's last axis: h = x + residual in x's dtype (None without
+    a residual), y in x's dtype or, with `quant`, in that 8-bit dtype with fp32 scales (rows, 1) or
+    (rows, groups); rstd fp32 (rows) with `want_rstd`.  weight (N,) of x's dtype or fp32, or None."""
+    dt = x.dtype
+    N = x.shape[-1] if x.dim() else 0
+    if not x.is_cuda or dt not in _DTYPE_CODE or x.dim() < 1:
+        raise RuntimeError("rms_norm: x must be a GPU tensor of float32, float16 or bfloat16 with at least one axis")
+    if weight is not None and (weight.dtype not in (dt, torch.float32) or weight.shape != (N,)
+                               or weight.device != x.device):
+        raise RuntimeError("rms_norm: weight must be (N,) in x's dtype or float32, on x's device")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != dt or residual.device != x.device):
+        raise RuntimeError("rms_norm: residual must match x")
+    if quant is not None and quant not in QUANT_DTYPES:
+        raise RuntimeError("rms_norm: 8-bit outputs are torch.float8_e4m3fn and torch.int8")
+    if group and (group & (group - 1) or not 16 <= group <= 256):
+        raise RuntimeError("rms_norm: group_size must be a power of two from 16 to 256")
+    x = _rows(x)
+    M = x.numel() // N if N else 0
+    y = torch.empty(x.shape, dtype=quant or dt, device=x.device)
+    h = rstd = scales = None
+    if residual is not None:
+        residual = _rows(residual)
+        h = torch.empty(x.shape, dtype=dt, device=x.device)
+    if want_rstd:
+        rstd = torch.empty(M, dtype=torch.float32, device=x.device)
+    if quant is not None:
+        scales = torch.empty(x.shape[:-1] + (-(-N // group) if group else 1,), dtype=torch.float32, device=x.device)
+    if M == 0:
+        return y, h, rstd, scales
+    if weight is not None and weight.stride(0) != 1:
+        weight = weight.contiguous()
+    blk = _block("rms", _RmsArgs)
+    a = blk[0]
+    xs, rs = _row_stride(x), (_row_stride(residual) if residual is not None else 0)
+    wdt = dt if weight is None else weight.dtype
+    key = (M, N, xs, rs, group, eps, dt, wdt, quant)
+    if blk[2] != key:
+        a.M, a.N, a.x_stride, a.residual_stride, a.group, a.eps = M, N, xs, rs, group, eps
+        a.dtype, a.w_dtype, a.quant = _DTYPE_CODE[dt], _DTYPE_CODE[wdt], QUANT_DTYPES.get(quant, 0)
+        blk[2] = key
+    a.x, a.residual, a.weight, a.y, a.h = x.data_ptr(), _ptr(residual), _ptr(weight), y.data_ptr(), _ptr(h)
+    a.rstd, a.scales, a.stream = _ptr(rstd), _ptr(scales), _stream(x)
+    _check(lib().atk_rms_norm_fwd(blk[1]), "rms_norm")
+    return y, h, rstd, scales
+
+
+def rms_norm_backward(h: torch.Tensor, dy: torch.Tensor, dh: Optional[torch.Tensor], weight: Optional[torch.Tensor],
+                      rstd: torch.Tensor, *, want_dw: bool = True):
+    """(dx, dw) of rms_norm: h what was normalised, rstd (rows) from the forward, dh the gradient of h
+    from elsewhere or None; dw in the weight's dtype, None when not wanted."""
+    _require_cuda(h, dy, dh, weight, rstd)
+    N = h.shape[-1]
+    if dy.shape != h.shape or dy.dtype != h.dtype or (dh is not None and (dh.shape != h.shape or dh.dtype != h.dtype)):
+        raise RuntimeError("rms_norm backward: gradients must match the output")
+    h, dy = _rows(h), _rows(dy)
+    dh = None if dh is None else _rows(dh)
+    dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+    want_dw = want_dw and weight is not None
+    if h.numel() == 0:
+        return dx, (torch.zeros_like(weight) if want_dw else None)
+    dw = torch.empty(N, dtype=weight.dtype, device=h.device) if want_dw else None
+    weight = None if weight is None else weight.contiguous()
+    M, dt = h.numel() // N, _DTYPE_CODE[h.dtype]
+    L = lib()
+    ws = None
+    if want_dw:
+        ws = workspace(h.device, "rms_norm_bwd", _cached_size(L.atk_rms_norm_bwd_workspace_bytes, M, N, dt,
+                                                              device=_device_index(h.device)))
+    rc = L.atk_rms_norm_bwd(_ptr(h), _ptr(dy), _ptr(dh), _ptr(weight), _ptr(rstd), _ptr(dx), _ptr(dw), M, N,
+                            _row_stride(h), _row_stride(dy), 0 if dh is None else _row_stride(dh), dt,
+                            dt if weight is None else _DTYPE_CODE[weight.dtype], _ptr(ws),
+                            0 if ws is None else ws.numel(), _stream(h))
+    _check(rc, "rms_norm backward")
+    return dx, dw
+
+
+def gated_delta_update(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+                       state: torch.Tensor, scale: float, state_indices: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token of the gated delta rule for each sequence; `state` (slots, Hv, K, V) fp32 is updated in
+    place.  q, k (N, Hk, K), v (N, Hv, V) of one dtype, g and beta (N, Hv) of it or fp32; returns
+    (N, Hv, V)."""
+    if q.dim() != 3 or v.dim() != 3 or k.shape != q.shape or state.dim() != 4:
+        raise RuntimeError("gated_delta_rule_update expects q, k (N, Hk, K), v (N, Hv, V), state (slots, Hv, K, V)")
+    N, Hk, K = q.shape
+    _, Hv, V = v.shape
+    dt, gdt, bdt = q.dtype, g.dtype, beta.dtype
+    if v.shape[0] != N or g.shape != (N, Hv) or beta.shape != (N, Hv) or state.shape[1:] != (Hv, K, V):
+        raise RuntimeError("gated_delta_rule_update: sizes of v, g, beta and state must agree with q and k")
+    if Hk == 0 or Hv % Hk:
+        raise RuntimeError("gated_delta_rule_update: value heads must be a multiple of key heads")
+    if dt not in _DTYPE_CODE or k.dtype != dt or v.dtype != dt or gdt not in (dt, torch.float32) \
+            or bdt not in (dt, torch.float32) or state.dtype != torch.float32:
+        raise RuntimeError("gated_delta_rule_update: q, k and v must share a dtype (float32, float16 or bfloat16), "
+                           "g and beta have it or float32, and the state be float32")
+    dev = q.device
+    if not (q.is_cuda and k.device == dev and v.device == dev and g.device == dev and beta.device == dev
+            and state.device == dev):
+        raise RuntimeError("gated_delta_rule_update: all tensors must be on one GPU")
+    if state.stride(3) != 1 or state.stride(2) != V or state.stride(1) != K * V or (
+            state.shape[0] > 1 and state.stride(0) < Hv * K * V):
+        raise RuntimeError("gated_delta_rule_update: each slot of the state must be contiguous (it is updated in place)")
+    if state_indices is not None and (state_indices.dtype != torch.int32 or state_indices.shape != (N,)
+                                      or state_indices.device != dev):
+        raise RuntimeError("gated_delta_rule_update: state_indices must be int32 (N,) on the same GPU")
+    if state_indices is None and state.shape[0] != N:
+        raise RuntimeError("gated_delta_rule_update: without state_indices the state has one slot a sequence")
+    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+    out = torch.empty((N, Hv, V), dtype=dt, device=dev)
+    if out.numel() == 0:
+        return out
+    if state_indices is not None and state_indices.stride(0) != 1:
+        state_indices = state_indices.contiguous()
+    blk = _block("gdu", _DeltaUpdateArgs)
+    a = blk[0]
+    key = (state.shape, state.stride(0), q.shape, V, q.stride(), k.stride(), v.stride(), g.stride(), beta.stride(), dt,
+           gdt, bdt, scale)
+    if blk[2] != key:
+        a.N, a.slots, a.state_stride = N, state.shape[0], state.stride(0)
+        a.q_stride_n, a.q_stride_h = q.stride(0), q.stride(1)
+        a.k_stride_n, a.k_stride_h = k.stride(0), k.stride(1)
+        a.v_stride_n, a.v_stride_h = v.stride(0), v.stride(1)
+        a.g_stride_n, a.g_stride_h = g.stride()
+        a.beta_stride_n, a.beta_stride_h = beta.stride()
+        a.Hk, a.Hv, a.K, a.V, a.scale = Hk, Hv, K, V, scale
+        a.dtype, a.g_dtype, a.beta_dtype = _DTYPE_CODE[dt], _DTYPE_CODE[gdt], _DTYPE_CODE[bdt]
+        blk[2] = key
+    a.q, a.k, a.v, a.g, a.beta = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr()
+    a.state, a.out, a.state_indices, a.stream = state.data_ptr(), out.data_ptr(), _ptr(state_indices), _stream(q)
+    _check(lib().atk_gated_delta_update(blk[1]), "gated_delta_rule_update")
+    return out
+
+
+def _delta_checked(q, k, v, g, beta, initial_state, cu_seqlens):
+    """The tensors of a gated_delta_rule call as the kernels take them, and the number of sequences."""
+    if q.dim() != 4 or v.dim() != 4 or k.shape != q.shape:
+        raise RuntimeError("gated_delta_rule expects q, k (B, T, Hk, K) and v (B, T, Hv, V)")
+    B, T, Hk, K = q.shape
+    Hv, V = v.shape[2:]
+    if v.shape[:2] != (B, T) or g.shape != (B, T, Hv) or beta.shape != (B, T, Hv):
+        raise RuntimeError("gated_delta_rule: sizes of v, g and beta must agree with q and k")
+    if Hk == 0 or K == 0 or V == 0 or Hv == 0 or Hv % Hk:
+        raise RuntimeError("gated_delta_rule: value heads must be a multiple of key heads, and no head empty")
+    dt, dev = q.dtype, q.device
+    if dt not in _DTYPE_CODE or k.dtype != dt or v.dtype != dt or g.dtype not in (dt, torch.float32) \
+            or beta.dtype not in (dt, torch.float32):
+        raise RuntimeError("gated_delta_rule: q, k and v must share a dtype (float32, float16 or bfloat16), g and "
+                           "beta have it or float32")
+    if not (q.is_cuda and k.device == dev and v.device == dev and g.device == dev and beta.device == dev):
+        raise RuntimeError("gated_delta_rule: all tensors must be on one GPU")
+    n = B
+    if cu_seqlens is not None:
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 \
+                or cu_seqlens.device != dev or B != 1:
+            raise RuntimeError("gated_delta_rule: cu_seqlens must be int32 (sequences + 1,) on the same GPU, with a "
+                               "batch of one")
+        n = cu_seqlens.numel() - 1
+        cu_seqlens = cu_seqlens.contiguous()
+    if initial_state is not None:
+        if initial_state.shape != (n, Hv, K, V) or initial_state.dtype != torch.float32 or initial_state.device != dev:
+            raise RuntimeError("gated_delta_rule: initial_state must be float32 (sequences, Hv, K, V) on the same GPU")
+        initial_state = initial_state.contiguous()
+    q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
+    return q, k, v, g, beta, initial_state, cu_seqlens, n
+
+
+def _delta_args(q, k, v, g, beta, scale, initial_state, cu_seqlens, n) -> _DeltaArgs:
+    a = _DeltaArgs()
+    a.q, a.k, a.v, a.g, a.beta = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr()
+    a.initial_state, a.cu_seqlens = _ptr(initial_state), _ptr(cu_seqlens)
+    a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+    a.g_stride[:], a.beta_stride[:] = g.stride(), beta.stride()
+    a.N, a.T, a.Hk, a.Hv, a.K, a.V = n, q.shape[1], q.shape[2], v.shape[2], q.shape[3], v.shape[3]
+    a.dtype, a.g_dtype, a.beta_dtype = _DTYPE_CODE[q.dtype], _DTYPE_CODE[g.dtype], _DTYPE_CODE[beta.dtype]
+    a.scale, a.stream = scale, _stream(q)
+    return a
+
+
+def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, scale: float,
+                initial_state: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None,
+                want_state: bool = False):
+    """The gated delta rule over sequences: (out (B, T, Hv, V), final state fp32 (sequences, Hv, K, V) or
+    None).  q, k (B, T, Hk, K), v (B, T, Hv, V) of one dtype, g and beta (B, T, Hv) of it or fp32."""
+    q, k, v, g, beta, initial_state, cu_seqlens, n = _delta_checked(q, k, v, g, beta, initial_state, cu_seqlens)
+    B, T, Hv, V = v.shape
+    out = torch.empty((B, T, Hv, V), dtype=v.dtype, device=v.device)
+    final = torch.empty((n, Hv, q.shape[3], V), dtype=torch.float32, device=v.device) if want_state else None
+    if n == 0:
+        return out.zero_(), final
+    if out.numel() == 0 and final is None:
+        return out, final
+    a = _delta_args(q, k, v, g, beta, scale, initial_state, cu_seqlens, n)
+    a.out, a.final_state = out.data_ptr(), _ptr(final)
+    L = lib()
+    # scratch of the length of the sequences: from torch's allocator, which gives it back to the stream
+    ws = torch.empty(L.atk_gated_delta_workspace_bytes(ctypes.addressof(a)), dtype=torch.uint8, device=v.device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _check(L.atk_gated_delta_fwd(ctypes.addressof(a)), "gated_delta_rule")
+    return out, final
+
+
+def gated_delta_backward(q, k, v, g, beta, scale: float, initial_state, cu_seqlens, dout: torch.Tensor,
+                         dfinal: Optional[torch.Tensor], want_dstate: bool):
+    """(dq, dk, dv, dg, dbeta, dinitial_state or None) of gated_delta: dout like its output, dfinal (fp32)
+    the gradient of its final state or None."""
+    q, k, v, g, beta, initial_state, cu_seqlens, n = _delta_checked(q, k, v, g, beta, initial_state, cu_seqlens)
+    if dout.shape != v.shape or dout.dtype != v.dtype or dout.device != v.device:
+        raise RuntimeError("gated_delta_rule backward: the gradient must match the output")
+    # tokens that no packed sequence has get a gradient of zero
+    make = torch.empty if cu_seqlens is None else torch.zeros
+    grads = [make(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, g, beta)]
+    dstate = None
+    if want_dstate:
+        dstate = torch.empty((n,) + v.shape[2:3] + (q.shape[3], v.shape[3]), dtype=torch.float32, device=v.device)
+    if n == 0 or (v.numel() == 0 and dstate is None):
+        return (*grads, dstate)
+    dout = dout.contiguous()
+    dfinal = None if dfinal is None else dfinal.contiguous()
+    a = _delta_args(q, k, v, g, beta, scale, initial_state, cu_seqlens, n)
+    L = lib()
+    ws = torch.empty(L.atk_gated_delta_bwd_workspace_bytes(ctypes.addressof(a)), dtype=torch.uint8, device=v.device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    _check(L.atk_gated_delta_bwd(ctypes.addressof(a), _ptr(dout), _ptr(dfinal), *(t.data_ptr() for t in grads),
+                                 _ptr(dstate)), "gated_delta_rule backward")
+    return (*grads, dstate)

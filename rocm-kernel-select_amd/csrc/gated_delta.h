@@ -1,0 +1,127 @@
+// What the kernels of the gated delta rule share: argument structs, limits, and the fragments that
+// their matrix products are fed with.
+//
+// The products run on bf16 MFMA with fp32 accumulators, and the state, the decays and everything
+// that is chained over the sequence are fp32.  So an fp32 operand enters a product as three bf16
+// parts that sum to it (8 bits each, 24 in all), and a product takes the parts' products down to
+// 2^-16 of the largest: 3 MFMAs where the other operand is a bf16 input (exact in one part), 6 where
+// it is fp32 too.  An fp16 input is exact in two parts, an fp32 one in three.
+#pragma once
+#include "atk_common.h"
+
+namespace atk {
+
+constexpr int kGdrMaxK = 256;   // key columns: a state's rows
+constexpr int kGdrC = 64;       // tokens of a chunk
+
+struct GdrStepArgs {
+  const void* q; const void* k; const void* v; const void* g; const void* beta;
+  float* state; void* o; const int* slots;
+  int64_t n, n_slots, state_stride;
+  int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh, g_sb, g_sh, b_sb, b_sh;  // strides in elements: sequence, head
+  int Hv, group, K, V, g_dtype, b_dtype;
+  float scale;
+};
+
+// A whole call on sequences.  Strides in elements: batch, token, head.
+struct GdrArgs {
+  const void* q; const void* k; const void* v; const void* g; const void* beta;
+  void* o; const float* s0; float* s1; const int* cu;
+  int64_t q_s[3], k_s[3], v_s[3], g_s[3], b_s[3];
+  int64_t n, T;          // sequences; tokens of each (of the packed row with cu)
+  int64_t slots;         // chunks, unused ones of packed sequences among them
+  int Hk, Hv, group, K, V, g_dtype, b_dtype;
+  float scale;
+  // workspace: fragments by (slot, key head) and (slot, value head), and each chunk's decays
+  uint4* kf; uint4* qf; uint4* ktf; uint4* tf; uint4* pf;
+  float* row;            // [slot][Hv][3][64]: exp(G_i), exp(G_63 - G_i), beta_i
+  // the backward's: fragments of Q^T, (1 + diag(beta) W)^-T and lower(Q K^T * D)^T; each chunk's G in
+  // 64 bits; the state and the errors that the forward chain had at each chunk, and the gradients of
+  // the state after it and of U: [slot][Hv][KP or 64][VP] fp32, VP = V padded to 32
+  uint4* qtf; uint4* ttf; uint4* ptf;
+  double* gsum;
+  float* sc; float* ec; float* dsc; float* drc;
+  const void* dout; const float* ds1; float* ds0;
+  void* dq; void* dk; void* dv; void* dg; void* dbeta;
+  int VP;
+};
+
+// Host side, shared by the forward and the backward: fragments of all chunks, and the state's chain,
+// which writes the output and final state, or (keep) each chunk's state and errors.
+int gdr_prepare(const GdrArgs& a, int dtype, bool backward, hipStream_t s);
+int gdr_chain(const GdrArgs& a, int dtype, bool keep, hipStream_t s);
+size_t gdr_plan(const atk_gated_delta_args* p, bool backward, GdrArgs* a, int* rc);
+inline int gdr_padded_k(int K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
+
+// Where sequence n's tokens and chunks lie.  A packed sequence has the chunk slots from
+// begin / 64 + n on: the next one's begin at or after its end, whatever the lengths, so no prefix
+// sum over the lengths is needed.  Offsets are clamped to the row, so bad ones stay in bounds.
+struct GdrSeq {
+  int64_t batch, begin, len, slot;
+};
+__device__ __forceinline__ GdrSeq gdr_seq(const int* __restrict__ cu, int64_t T, int64_t n) {
+  if (!cu) return {n, 0, T, n * ((T + kGdrC - 1) / kGdrC)};
+  int64_t b = cu[n], e = cu[n + 1];
+  b = b < 0 ? 0 : b > T ? T : b;
+  e = e < b ? b : e > T ? T : e;
+  return {0, b, e - b, b / kGdrC + n};
+}
+// The sequence that chunk slot `slot` belongs to; a slot that no chunk has gets one past its end.
+__device__ __forceinline__ int64_t gdr_seq_of_slot(const int* __restrict__ cu, int64_t T, int64_t n, int64_t slot) {
+  if (!cu) return slot / ((T + kGdrC - 1) / kGdrC);
+  int64_t lo = 0, hi = n - 1;  // the last sequence whose first slot is not after `slot`
+  while (lo < hi) {
+    const int64_t mid = (lo + hi + 1) / 2;
+    if (gdr_seq(cu, T, mid).slot <= slot) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// bf16 parts that hold an input exactly
+template <typename T> inline constexpr int kParts = sizeof(T) == 4 ? 3 : 2;
+template <> inline constexpr int kParts<__bf16> = 1;
+
+// D[4 g + r][lane & 15] += sum over k < 32 of A[lane & 15][k] B[k][lane & 15], g = lane / 16; a lane
+// holds elements 8 g .. 8 g + 7 of its row of A and of its column of B.
+__device__ __forceinline__ f32x4 mma(const uint4& a, const uint4& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// The same of operands in NA and NB parts, the small products first.
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma_parts(const uint4 (&a)[NA], const uint4 (&b)[NB], f32x4 c) {
+#pragma unroll
+  for (int s = 2; s >= 0; --s)
+#pragma unroll
+    for (int p = 0; p < NA; ++p)
+#pragma unroll
+      for (int q = 0; q < NB; ++q)
+        if (p + q == s) c = mma(a[p], b[q], c);
+  return c;
+}
+
+// v[0..N) as NP parts of N bf16 each
+template <int NP, int N, typename P>
+__device__ __forceinline__ void split_parts(const float* v, P (&out)[NP]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float r = v[i];
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const __bf16 h = static_cast<__bf16>(r);
+      out[p][i] = h;
+      r -= static_cast<float>(h);
+    }
+  }
+}
+
+// fragments of the lower triangle of a 64 x 64 matrix in 16 x 32 tiles (row tile m, column half s)
+constexpr int kTri = 6;
+__device__ __forceinline__ int tri_lower(int m, int s) { return m < 2 ? m : 2 * m - 2 + s; }
+__device__ __forceinline__ int tri_upper(int m, int s) { return m < 2 ? 2 * m + s : m + 2; }
+
+}  // namespace atk

@@ -1,0 +1,165 @@
+// The gated delta rule, one token at a time: the decode step over a cache of states.
+//
+//   S~ = exp(g) S;  u = beta (v - S~^T k);  S' = S~ + k u^T;  o = scale S'^T q
+//
+// S is [K, V] fp32 for each sequence and value head; value head h reads key head h / (Hv / Hk).
+// HBM-bound: the state is read and written once and everything else is small, so the state stays
+// in registers in between.  Both products over K are taken in the same pass over S, since
+// S'^T q = exp(g) S^T q + (k . q) u; the one reduction across the workgroup carries both and k . q.
+#include "gated_delta.h"
+
+namespace atk {
+namespace {
+
+// A workgroup has NV * VW columns of one head's state: NV threads of VW columns side by side, 256 / NV
+// groups of rows, RPT rows a thread.
+template <typename T, int VW, int NV, int RPT>
+__global__ __launch_bounds__(256) void gdr_step_kernel(GdrStepArgs a) {
+  constexpr int RG = 256 / NV, W = 2 * VW;
+  __shared__ float kf[RG * RPT], qf[RG * RPT];
+  __shared__ float red[4][NV][W];
+  __shared__ float red_kq[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int cg = tid % NV, rg = tid / NV;
+  const int64_t n = blockIdx.z;
+  const int h = blockIdx.y, hk = h / a.group;
+  const int c0 = (blockIdx.x * NV + cg) * VW;
+  const int64_t slot = a.slots ? (int64_t)a.slots[n] : n;
+  T* __restrict__ o = static_cast<T*>(a.o) + (n * a.Hv + h) * (int64_t)a.V;
+  if (slot < 0 || slot >= a.n_slots) {  // a row of padding: no state, an output of zeros
+    if (rg == 0)
+#pragma unroll
+      for (int j = 0; j < VW; ++j)
+        if (c0 + j < a.V) o[c0 + j] = from_f32<T>(0.f);
+    return;
+  }
+  float* __restrict__ S = a.state + slot * a.state_stride + (int64_t)h * a.K * a.V;
+  float s[RPT][VW];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = rg + i * RG;
+    const bool in = r < a.K && c0 < a.V;  // V is a multiple of VW (host check)
+    if constexpr (VW == 4) {
+      const float4 t = in ? *reinterpret_cast<const float4*>(S + (int64_t)r * a.V + c0) : make_float4(0.f, 0.f, 0.f, 0.f);
+      s[i][0] = t.x; s[i][1] = t.y; s[i][2] = t.z; s[i][3] = t.w;
+    } else {
+      s[i][0] = in ? S[(int64_t)r * a.V + c0] : 0.f;
+    }
+  }
+  const T* __restrict__ k = static_cast<const T*>(a.k) + n * a.k_sb + hk * a.k_sh;
+  const T* __restrict__ q = static_cast<const T*>(a.q) + n * a.q_sb + hk * a.q_sh;
+  const T* __restrict__ v = static_cast<const T*>(a.v) + n * a.v_sb + h * a.v_sh;
+  for (int r = tid; r < RG * RPT; r += 256) {
+    kf[r] = r < a.K ? to_f32(k[r]) : 0.f;
+    qf[r] = r < a.K ? to_f32(q[r]) : 0.f;
+  }
+  const float decay = expf(load_param(a.g, a.g_dtype, n * a.g_sb + h * a.g_sh));
+  const float beta = load_param(a.beta, a.b_dtype, n * a.b_sb + h * a.b_sh);
+  float vv[VW];
+#pragma unroll
+  for (int j = 0; j < VW; ++j) vv[j] = c0 + j < a.V ? to_f32(v[c0 + j]) : 0.f;
+  __syncthreads();
+  float p[W], kq = 0.f;
+#pragma unroll
+  for (int j = 0; j < W; ++j) p[j] = 0.f;
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const float kr = kf[rg + i * RG], qr = qf[rg + i * RG];
+    kq += kr * qr;
+#pragma unroll
+    for (int j = 0; j < VW; ++j) {
+      p[j] += s[i][j] * kr;
+      p[VW + j] += s[i][j] * qr;
+    }
+  }
+#pragma unroll
+  for (int off = NV; off < 64; off <<= 1) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) p[j] += __shfl_xor(p[j], off, 64);
+    kq += __shfl_xor(kq, off, 64);
+  }
+  if (lane < NV) {
+#pragma unroll
+    for (int j = 0; j < W; ++j) red[wave][cg][j] = p[j];
+    if (lane == 0) red_kq[wave] = kq;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < W; ++j) p[j] = (red[0][cg][j] + red[1][cg][j]) + (red[2][cg][j] + red[3][cg][j]);
+  kq = (red_kq[0] + red_kq[1]) + (red_kq[2] + red_kq[3]);
+  float u[VW];
+#pragma unroll
+  for (int j = 0; j < VW; ++j) u[j] = beta * (vv[j] - decay * p[j]);
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = rg + i * RG;
+    const float kr = kf[r];
+    if (r < a.K && c0 < a.V) {
+      if constexpr (VW == 4) {
+        *reinterpret_cast<float4*>(S + (int64_t)r * a.V + c0) =
+            make_float4(decay * s[i][0] + kr * u[0], decay * s[i][1] + kr * u[1], decay * s[i][2] + kr * u[2],
+                        decay * s[i][3] + kr * u[3]);
+      } else {
+        S[(int64_t)r * a.V + c0] = decay * s[i][0] + kr * u[0];
+      }
+    }
+  }
+  if (rg == 0) {
+#pragma unroll
+    for (int j = 0; j < VW; ++j)
+      if (c0 + j < a.V) o[c0 + j] = from_f32<T>(a.scale * (decay * p[VW + j] + kq * u[j]));
+  }
+}
+
+template <typename T, int VW, int NV, int RPT>
+void launch_step(const GdrStepArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.V + NV * VW - 1) / (NV * VW)), (unsigned)a.Hv, (unsigned)a.n);
+  hipLaunchKernelGGL((gdr_step_kernel<T, VW, NV, RPT>), grid, dim3(256), 0, s, a);
+}
+
+template <typename T>
+void launch_step_typed(const GdrStepArgs& a, hipStream_t s) {
+  const bool vec = a.V % 4 == 0 && aligned16(a.state) && a.state_stride % 4 == 0;
+  if (!vec) {
+    if (a.K <= 64) launch_step<T, 1, 64, 16>(a, s);
+    else if (a.K <= 128) launch_step<T, 1, 64, 32>(a, s);
+    else launch_step<T, 1, 64, 64>(a, s);
+  } else {
+    if (a.K <= 64) launch_step<T, 4, 8, 2>(a, s);
+    else if (a.K <= 128) launch_step<T, 4, 8, 4>(a, s);
+    else launch_step<T, 4, 8, 8>(a, s);
+  }
+}
+
+}  // namespace
+}  // namespace atk
+
+extern "C" int atk_gated_delta_update(const atk_gated_delta_update_args* p) {
+  using namespace atk;
+  if (!p) return fail(ATK_EINVAL, "gated delta update: null arguments");
+  if (!dtype_ok(p->dtype) || !dtype_ok(p->g_dtype) || !dtype_ok(p->beta_dtype))
+    return fail(ATK_EINVAL, "gated delta update: unknown dtype code");
+  if (p->N < 0 || p->Hk <= 0 || p->Hv <= 0 || p->K <= 0 || p->V <= 0 || p->slots < 0)
+    return fail(ATK_EINVAL, "gated delta update: bad sizes");
+  if (p->Hv % p->Hk) return fail(ATK_EINVAL, "gated delta update: value heads must be a multiple of key heads");
+  if (p->K > kGdrMaxK || p->Hv > 65535 || p->N > 65535)
+    return fail(ATK_UNSUPPORTED, "gated delta update: more than %d key columns, 65535 heads or sequences", kGdrMaxK);
+  if (p->N == 0) return ATK_OK;
+  if (!p->q || !p->k || !p->v || !p->g || !p->beta || !p->state || !p->out)
+    return fail(ATK_EINVAL, "gated delta update: null pointer");
+  if (!p->state_indices && p->N > p->slots) return fail(ATK_EINVAL, "gated delta update: fewer states than sequences");
+  GdrStepArgs a;
+  a.q = p->q; a.k = p->k; a.v = p->v; a.g = p->g; a.beta = p->beta;
+  a.state = static_cast<float*>(p->state); a.o = p->out; a.slots = p->state_indices;
+  a.n = p->N; a.n_slots = p->slots; a.state_stride = p->state_stride;
+  a.q_sb = p->q_stride_n; a.q_sh = p->q_stride_h; a.k_sb = p->k_stride_n; a.k_sh = p->k_stride_h;
+  a.v_sb = p->v_stride_n; a.v_sh = p->v_stride_h; a.g_sb = p->g_stride_n; a.g_sh = p->g_stride_h;
+  a.b_sb = p->beta_stride_n; a.b_sh = p->beta_stride_h;
+  a.Hv = p->Hv; a.group = p->Hv / p->Hk; a.K = p->K; a.V = p->V;
+  a.g_dtype = p->g_dtype; a.b_dtype = p->beta_dtype; a.scale = p->scale;
+  hipStream_t s = reinterpret_cast<hipStream_t>(p->stream);
+  if (p->dtype == ATK_F32) launch_step_typed<float>(a, s);
+  else if (p->dtype == ATK_F16) launch_step_typed<_Float16>(a, s);
+  else launch_step_typed<__bf16>(a, s);
+  return check_launch("gdr_step_kernel");
+}

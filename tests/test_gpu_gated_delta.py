@@ -1,0 +1,507 @@
+"""The gated delta rule against its recurrence in 64 bits, one token at a time.
+
+Tolerances.  An output in 16 bits is rounded once (relative 2^-8 for bf16, 2^-11 for fp16).  Before
+that everything is fp32 or finer: every product of the chunked form keeps at least 2^-23 of its
+operands, and its sums run over at most a few hundred terms, chained over the chunks by decays of at
+most one, so 2^-15 (512 roundings of 2^-24) of the tensor's largest value bounds what fp32 leaves."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+ULP = {torch.float32: 0.0, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+F32 = 512 * 2.0 ** -24
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+gpu = pytest.mark.gpu
+
+
+def close(got, want, dtype=None, what=""):
+    assert got.shape == want.shape
+    if not want.numel():
+        return
+    off = (got.double() - want).abs() - ULP[dtype or got.dtype] * want.abs() - F32 * want.abs().max() - 1e-30
+    assert off.max().item() <= 0, (what, off.max().item(), want.abs().max().item())
+
+
+def step64(S, q, k, v, g, beta, scale):
+    """One token of (..., heads, dim) in 64 bits: (S', out)."""
+    rep = v.shape[-2] // k.shape[-2]
+    q, k = (t.double().repeat_interleave(rep, dim=-2) for t in (q, k))
+    S = S.double() * g.double().exp()[..., None, None]
+    u = beta.double()[..., None] * (v.double() - (S * k[..., None]).sum(-2))
+    S = S + k[..., None] * u[..., None, :]
+    return S, scale * (S * q[..., None]).sum(-2)
+
+
+def unit(x):
+    return x / x.norm(dim=-1, keepdim=True).clamp_min(1e-6)
+
+
+def make(lead, hk, hv, dk, dv, dtype, dev, seed=0, gdtype=torch.float32, bdtype=None):
+    gen = torch.Generator().manual_seed(seed)
+    rand = lambda *s: torch.randn(*lead, *s, generator=gen)  # noqa: E731
+    q, k = unit(rand(hk, dk) + 0.3), unit(rand(hk, dk) + 0.3)
+    v, g, beta = rand(hv, dv), -torch.exp(rand(hv) - 1.5), torch.sigmoid(rand(hv))
+    return [t.to(dev) for t in (q.to(dtype), k.to(dtype), v.to(dtype), g.to(gdtype), beta.to(bdtype or dtype))]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,hk,hv,dk,dv", [(1, 1, 1, 1, 1), (3, 2, 4, 128, 128), (2, 1, 3, 64, 100), (2, 2, 2, 130, 36),
+                                           (5, 1, 2, 256, 256), (2, 3, 3, 17, 33), (1, 2, 2, 100, 7), (33, 1, 4, 32, 64)])
+def test_update(dev, n, hk, hv, dk, dv, dtype):
+    import amd_tuned_torch as P
+    args = make((n,), hk, hv, dk, dv, dtype, dev, seed=n + dk)
+    gen = torch.Generator().manual_seed(1)
+    state = torch.randn(n, hv, dk, dv, generator=gen).to(dev)
+    want_s, want = step64(state, *args, dk ** -0.5)
+    got = P.gated_delta_rule_update(*args, state)
+    assert got.dtype == dtype
+    close(got, want)
+    close(state, want_s)
+    want_s, want = step64(state, *args, 0.5)
+    close(P.gated_delta_rule_update(*args, state, 0.5), want)     # from the state it left
+    close(state, want_s)
+
+
+@gpu
+@pytest.mark.parametrize("dv", [64, 66])
+def test_update_slots_strides_and_padding(dev, dv):
+    import amd_tuned_torch as P
+    n, hk, hv, dk = 4, 2, 4, 96
+    q, k, v, g, beta = make((n, 3), hk, hv, dk, dv, torch.bfloat16, dev, gdtype=torch.bfloat16, bdtype=torch.float32)
+    fused = torch.cat([q.flatten(2), k.flatten(2), v.flatten(2)], -1)[:, 1]       # one row of a projection
+    a, b = hk * dk, 2 * hk * dk
+    q, k, v = (fused[:, :a].unflatten(1, (hk, dk)), fused[:, a:b].unflatten(1, (hk, dk)),
+               fused[:, b:].unflatten(1, (hv, dv)))
+    g, beta = g[:, 1], beta[:, 1]
+    cache = torch.randn(9, 2, hv, dk, dv, device=dev)[:, 1]                        # slots apart
+    before = cache.clone()
+    slots = torch.tensor([7, -1, 0, 9], dtype=torch.int32, device=dev)
+    want_s, want = step64(before[[7, 0]], q[[0, 2]], k[[0, 2]], v[[0, 2]], g[[0, 2]], beta[[0, 2]], dk ** -0.5)
+    out = P.gated_delta_rule_update(q, k, v, g, beta, cache, state_indices=slots)
+    close(out[[0, 2]], want)
+    assert out[[1, 3]].eq(0).all()
+    close(cache[[7, 0]], want_s)
+    rest = [1, 2, 3, 4, 5, 6, 8]
+    assert torch.equal(cache[rest], before[rest])
+    twin = before.clone()
+    ref = P.gated_delta.gated_delta_rule_update_ref(q, k, v, g, beta, twin, state_indices=slots)
+    close(ref, out.double())
+    close(twin, cache.double())
+    assert P.gated_delta_rule_update(q[:0], k[:0], v[:0], g[:0], beta[:0], cache, state_indices=slots[:0]).shape == (0, hv, dv)
+
+
+@gpu
+def test_update_forgets_and_passes_nan(dev):
+    import amd_tuned_torch as P
+    q, k, v, g, beta = make((2,), 1, 2, 64, 64, torch.float32, dev)
+    state = torch.randn(2, 2, 64, 64, device=dev)
+    g[0] = float("-inf")
+    v[1, 0, 3] = float("nan")
+    want_s, want = step64(state, q, k, v, g, beta, 0.125)
+    out = P.gated_delta_rule_update(q, k, v, g, beta, state)
+    close(out[0], want[0])
+    close(state[0], want_s[0])
+    assert torch.equal(out[1].isnan(), want[1].isnan()) and torch.equal(state[1].isnan(), want_s[1].isnan())
+
+
+@gpu
+def test_update_in_a_graph_and_on_a_stream(dev):
+    import amd_tuned_torch as P
+    args = make((3,), 2, 4, 128, 128, torch.bfloat16, dev)
+    state = torch.randn(3, 4, 128, 128, device=dev)
+    eager, start = state.clone(), state.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        P.gated_delta_rule_update(*args, state)
+    torch.cuda.current_stream().wait_stream(side)
+    state.copy_(start)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = P.gated_delta_rule_update(*args, state)
+    state.copy_(start)
+    for _ in range(3):
+        graph.replay()
+        want = P.gated_delta_rule_update(*args, eager)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(state, eager)
+
+
+@gpu
+def test_update_refusals(dev):
+    import amd_tuned_torch as P
+    q, k, v, g, beta = make((2,), 2, 4, 32, 16, torch.bfloat16, dev)
+    state = torch.zeros(2, 4, 32, 16, device=dev)
+    idx = torch.zeros(2, dtype=torch.int32, device=dev)
+    bad = [(q[0], k, v, g, beta, state), (q, k[:1], v, g, beta, state), (q, k.half(), v, g, beta, state),
+           (q, k, v[:, :3], g[:, :3], beta[:, :3], state[:, :3]), (q, k, v, g[:1], beta, state),
+           (q, k, v, g.double(), beta, state), (q, k, v, g, beta, state.bfloat16()), (q, k, v, g, beta, state[:1]),
+           (q, k, v, g, beta, state.transpose(2, 3)), (q.cpu(), k, v, g, beta, state), (q, k, v, g, beta, state.cpu())]
+    for a in bad:
+        with pytest.raises(RuntimeError, match="gated_delta_rule_update"):
+            P.gated_delta_rule_update(*a)
+    for i in (idx.long(), idx[:1], idx.cpu()):
+        with pytest.raises(RuntimeError, match="state_indices"):
+            P.gated_delta_rule_update(q, k, v, g, beta, state, state_indices=i)
+    wide = make((1,), 1, 1, 257, 8, torch.bfloat16, dev)
+    with pytest.raises(RuntimeError, match="256"):
+        P.gated_delta_rule_update(*wide, torch.zeros(1, 1, 257, 8, device=dev))
+
+
+# ---------------------------------------------------------------------------------------------
+# whole sequences
+# ---------------------------------------------------------------------------------------------
+def sequence64(q, k, v, g, beta, scale, state, cu=None):
+    """(out, final state) in 64 bits; q, k, v, g, beta (B, T, heads, ...)."""
+    if cu is None:
+        S, out = state.double(), []
+        for t in range(v.shape[1]):
+            S, o = step64(S, q[:, t], k[:, t], v[:, t], g[:, t], beta[:, t], scale)
+            out.append(o)
+        return (torch.stack(out, 1) if out else v.double()), S
+    out, states = torch.zeros_like(v, dtype=torch.float64), []
+    for i, (a, b) in enumerate(zip(cu, cu[1:])):
+        o, S = sequence64(*(x[:, a:b] for x in (q, k, v, g, beta)), scale, state[i:i + 1])
+        out[:, a:b] = o
+        states.append(S)
+    return out, torch.cat(states)
+
+
+SHAPES = [  # batch, tokens, key heads, value heads, key columns, value columns
+    (1, 1, 1, 1, 1, 1), (2, 2, 1, 2, 64, 64), (1, 63, 2, 2, 128, 128), (1, 64, 1, 4, 128, 32), (2, 65, 2, 4, 64, 100),
+    (1, 130, 1, 1, 17, 33), (3, 200, 1, 3, 96, 16), (1, 129, 2, 2, 130, 20), (1, 70, 1, 1, 256, 256), (1, 321, 1, 2, 100, 7)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,t,hk,hv,dk,dv", SHAPES)
+def test_sequences(dev, b, t, hk, hv, dk, dv, dtype):
+    import amd_tuned_torch as P
+    args = make((b, t), hk, hv, dk, dv, dtype, dev, seed=t)
+    state = torch.randn(b, hv, dk, dv, generator=torch.Generator().manual_seed(2)).to(dev)
+    want, want_s = sequence64(*args, dk ** -0.5, state)
+    got, got_s = P.gated_delta_rule(*args, initial_state=state, return_final_state=True)
+    assert got.dtype == dtype and got_s.dtype == torch.float32
+    close(got, want, what="out")
+    close(got_s, want_s, what="state")
+    want, _ = sequence64(*args, 0.3, torch.zeros_like(state))
+    close(P.gated_delta_rule(*args, 0.3), want, what="from nothing")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cu,t", [([0, 5], 5), ([0, 1, 64, 65, 200], 200), ([0, 0, 130, 130, 131, 131], 131),
+                                  ([3, 60, 190], 200), ([0, 63, 126, 189, 252], 256), ([0, 0], 40), ([7], 9)])
+def test_packed_sequences(dev, cu, t, dtype):
+    import amd_tuned_torch as P
+    n = len(cu) - 1
+    args = make((1, t), 2, 4, 64, 48, dtype, dev, seed=t)
+    state = torch.randn(n, 4, 64, 48, generator=torch.Generator().manual_seed(2)).to(dev)
+    offsets = torch.tensor(cu, dtype=torch.int32, device=dev)
+    got, got_s = P.gated_delta_rule(*args, initial_state=state, return_final_state=True, cu_seqlens=offsets)
+    if n:
+        want, want_s = sequence64(*args, 0.125, state, cu)
+        close(got, want, what="out")
+        close(got_s, want_s, what="state")
+        ref, ref_s = P.gated_delta.gated_delta_rule_ref(*args, initial_state=state, return_final_state=True,
+                                                        cu_seqlens=offsets)
+        close(ref, want, what="ref")
+        close(ref_s, want_s, what="ref state")
+    else:
+        assert got.eq(0).all() and got_s.shape == (0, 4, 64, 48)
+
+
+@gpu
+def test_offsets_that_no_row_has(dev):
+    """Offsets past the row or before it are clamped to it; nothing else is read or written."""
+    import amd_tuned_torch as P
+    args = make((1, 100), 1, 2, 64, 64, torch.bfloat16, dev)
+    bad = torch.tensor([-50, 30, 1000], dtype=torch.int32, device=dev)
+    got, got_s = P.gated_delta_rule(*args, return_final_state=True, cu_seqlens=bad)
+    want, want_s = sequence64(*args, 0.125, torch.zeros(2, 2, 64, 64, device=dev), [0, 30, 100])
+    close(got, want)
+    close(got_s, want_s)
+
+
+@gpu
+def test_strided_inputs(dev):
+    import amd_tuned_torch as P
+    b, t, hk, hv, dk, dv = 2, 100, 2, 4, 64, 64
+    q, k, v, g, beta = make((b, t), hk, hv, dk, dv, torch.bfloat16, dev, gdtype=torch.bfloat16, bdtype=torch.float32)
+    want, _ = sequence64(q, k, v, g, beta, 0.125, torch.zeros(b, hv, dk, dv, device=dev))
+    fused = torch.cat([q.flatten(2), k.flatten(2), v.flatten(2), v.flatten(2)[..., :3]], -1)  # odd rows
+    q1, k1, v1 = fused.split([hk * dk, hk * dk, hv * dv, 3], -1)[:3]
+    got = P.gated_delta_rule(q1.unflatten(2, (hk, dk)), k1.unflatten(2, (hk, dk)), v1.unflatten(2, (hv, dv)),
+                             g.transpose(1, 2).contiguous().transpose(1, 2), beta)
+    close(got, want)
+    heads_first = lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    close(P.gated_delta_rule(*(heads_first(x) for x in (q, k, v, g, beta))), want)
+    columns_first = lambda x: x.transpose(2, 3).contiguous().transpose(2, 3)  # noqa: E731
+    close(P.gated_delta_rule(columns_first(q), k, columns_first(v), g, beta), want)
+    one = beta[:, :, :1].expand(b, t, hv)                                      # a broadcast input
+    want, _ = sequence64(q, k, v, g, one, 0.125, torch.zeros(b, hv, dk, dv, device=dev))
+    close(P.gated_delta_rule(q, k, v, g, one), want)
+
+
+@gpu
+def test_offsets_beyond_32_bits(dev):
+    """Rows of a buffer whose elements lie up to 3.3e9 apart."""
+    import amd_tuned_torch as P
+    t, far = 100, 1 << 25
+    q, k, v, g, beta = make((1, t), 1, 1, 64, 64, torch.bfloat16, dev)
+    buffer = torch.empty(t * far, dtype=torch.bfloat16, device=dev)
+    rows = buffer.view(1, t, 1, far)
+    for i, x in enumerate((q, k, v)):
+        rows[..., i * 64:(i + 1) * 64] = x
+    want, _ = sequence64(q, k, v, g, beta, 0.125, torch.zeros(1, 1, 64, 64, device=dev))
+    close(P.gated_delta_rule(*(rows[..., i * 64:(i + 1) * 64] for i in range(3)), g, beta), want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gates_at_their_ends(dev, dtype):
+    """No decay, all forgotten, nothing written, everything replaced, and keys that are all alike."""
+    import amd_tuned_torch as P
+    q, k, v, g, beta = make((1, 150), 1, 6, 64, 64, dtype, dev)
+    g[:, :, 0] = 0
+    g[:, ::7, 1] = float("-inf")
+    g[:, :, 2] = -40
+    g[:, :, 5] = torch.finfo(torch.float32).min
+    beta[:, :, 3] = 0
+    beta[:, 1::2, 2] = 0
+    beta[:, :, 4] = 1
+    state = torch.randn(1, 6, 64, 64, device=dev)
+    want, want_s = sequence64(q, k, v, g, beta, 0.125, state)
+    got, got_s = P.gated_delta_rule(q, k, v, g, beta, initial_state=state, return_final_state=True)
+    for h in range(6):
+        close(got[:, :, h], want[:, :, h], what=h)
+        close(got_s[:, h], want_s[:, h], what=h)
+    k = k[:, :1].expand_as(k).contiguous()
+    k = (k.float() / k.float().norm(dim=-1, keepdim=True)).to(dtype)
+    g = torch.zeros_like(g)
+    want, want_s = sequence64(q, k, v, g, beta.clamp_max(0.96), 0.125, state)
+    got, got_s = P.gated_delta_rule(q, k, v, g, beta.clamp_max(0.96), initial_state=state, return_final_state=True)
+    close(got, want)
+    close(got_s, want_s)
+
+
+@gpu
+def test_nan_stays_behind_its_token(dev):
+    import amd_tuned_torch as P
+    args = make((1, 140), 1, 2, 64, 64, torch.bfloat16, dev)
+    args[2][0, 70, 1, 5] = float("nan")
+    got = P.gated_delta_rule(*args)
+    assert not got[:, :, 0].isnan().any()
+    assert got[:, 70:, 1, 5].isnan().all() and not got[:, :64, 1].isnan().any()
+
+
+@gpu
+def test_continuing_and_decoding_agree_with_one_pass(dev):
+    """A prompt in two parts and then token by token gives what one pass gives."""
+    import amd_tuned_torch as P
+    args = make((2, 150), 2, 4, 128, 64, torch.float32, dev)
+    want, want_s = P.gated_delta_rule(*args, return_final_state=True)
+    part = [x[:, :80] for x in args]
+    out, S = P.gated_delta_rule(*part, return_final_state=True)
+    outs = [out]
+    out, S = P.gated_delta_rule(*(x[:, 80:145] for x in args), initial_state=S, return_final_state=True)
+    outs.append(out)
+    for t in range(145, 150):
+        outs.append(P.gated_delta_rule_update(*(x[:, t] for x in args), S)[:, None])
+    close(torch.cat(outs, 1), want.double())
+    close(S, want_s.double())
+
+
+@gpu
+def test_empty_calls_and_streams(dev):
+    import amd_tuned_torch as P
+    args = make((2, 70), 1, 2, 64, 64, torch.bfloat16, dev)
+    assert P.gated_delta_rule(*(x[:0] for x in args)).shape == (0, 70, 2, 64)
+    state = torch.randn(2, 2, 64, 64, device=dev)
+    out, S = P.gated_delta_rule(*(x[:, :0] for x in args), initial_state=state, return_final_state=True)
+    assert out.shape == (2, 0, 2, 64) and torch.equal(S, state)
+    first = P.gated_delta_rule(*args)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = P.gated_delta_rule(*args)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(first, again)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = P.gated_delta_rule(*args)
+    for _ in range(3):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first)
+        P.gated_delta_rule(*args)
+
+
+@gpu
+def test_sequence_refusals(dev):
+    import amd_tuned_torch as P
+    q, k, v, g, beta = make((2, 5), 2, 4, 32, 16, torch.bfloat16, dev)
+    bad = [(q[0], k, v, g, beta), (q, k[:, :3], v, g, beta), (q, k.half(), v, g, beta), (q, k, v[:, :3], g, beta),
+           (q, k, v[:, :, :3], g[:, :, :3], beta[:, :, :3]), (q, k, v, g.double(), beta), (q, k, v, g, beta[..., :2]),
+           (q.cpu(), k, v, g, beta), tuple(x.double() for x in (q, k, v, g, beta))]
+    for a in bad:
+        with pytest.raises(RuntimeError, match="gated_delta_rule"):
+            P.gated_delta_rule(*a)
+    cu = torch.tensor([0, 5], dtype=torch.int32, device=dev)
+    one = [x[:1] for x in (q, k, v, g, beta)]
+    for c, a in ((cu, (q, k, v, g, beta)), (cu.long(), one), (cu.cpu(), one), (cu[:0], one)):
+        with pytest.raises(RuntimeError, match="cu_seqlens"):
+            P.gated_delta_rule(*a, cu_seqlens=c)
+    for s in (torch.zeros(2, 4, 32, 16, device=dev), torch.zeros(1, 4, 32, 16, device=dev).half(), torch.zeros(1, 4, 32, 16)):
+        with pytest.raises(RuntimeError, match="initial_state"):
+            P.gated_delta_rule(*one, initial_state=s)
+    wide = make((1, 5), 1, 1, 257, 8, torch.bfloat16, dev)
+    with pytest.raises(RuntimeError, match="256"):
+        P.gated_delta_rule(*wide)
+
+
+# ---------------------------------------------------------------------------------------------
+# gradients
+# ---------------------------------------------------------------------------------------------
+NAMES = ("dq", "dk", "dv", "dg", "dbeta", "dstate")
+
+
+def close_grad(got, want, what):
+    """As close(), with four times as much fp32 arithmetic behind it: a gradient goes through the forward's
+    chain and its own, and is a sum of products of both."""
+    assert got.shape == want.shape
+    off = (got.double() - want).abs() - ULP[got.dtype] * want.abs() - 4 * F32 * want.abs().max() - 1e-30
+    assert off.max().item() <= 0, (what, off.max().item(), want.abs().max().item())
+
+
+def gradients64(args, scale, state, dout, dstate, cu=None):
+    """The recurrence's gradients in 64 bits, by torch's autograd on the CPU."""
+    leaves = [x.detach().double().cpu().requires_grad_() for x in (*args, state)]
+    out, S = sequence64(*leaves[:5], scale, leaves[5], cu)
+    loss = (out * dout.double().cpu()).sum() + (S * dstate.double().cpu()).sum()
+    return torch.autograd.grad(loss, leaves)
+
+
+def check_gradients(dev, args, state, cu=None, scale=0.2, seed=7):
+    import amd_tuned_torch as P
+    gen = torch.Generator().manual_seed(seed)
+    dout = torch.randn(args[2].shape, generator=gen).to(args[2].dtype).to(dev)
+    dstate = torch.randn(state.shape, generator=gen).to(dev)
+    leaves = [x.detach().clone().requires_grad_() for x in (*args, state)]
+    offsets = None if cu is None else torch.tensor(cu, dtype=torch.int32, device=dev)
+    out, S = P.gated_delta_rule(*leaves[:5], scale, initial_state=leaves[5], return_final_state=True, cu_seqlens=offsets)
+    got = torch.autograd.grad((out, S), leaves, (dout, dstate))
+    want = gradients64(args, scale, state, dout, dstate, cu)
+    for name, x, y in zip(NAMES, got, want):
+        close_grad(x.cpu(), y, name)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,t,hk,hv,dk,dv", [(1, 1, 1, 1, 1, 1), (2, 3, 1, 2, 64, 64), (1, 64, 1, 1, 128, 32), (2, 65, 2, 4, 64, 100),
+                                             (1, 130, 1, 2, 17, 33), (1, 150, 1, 3, 128, 128), (1, 100, 2, 2, 130, 20),
+                                             (1, 70, 1, 1, 256, 64)])
+def test_gradients(dev, b, t, hk, hv, dk, dv, dtype):
+    args = make((b, t), hk, hv, dk, dv, dtype, dev, seed=t)
+    state = torch.randn(b, hv, dk, dv, generator=torch.Generator().manual_seed(3)).to(dev)
+    check_gradients(dev, args, state)
+
+
+@gpu
+@pytest.mark.parametrize("cu,t", [([0, 5], 5), ([0, 1, 64, 65, 200], 200), ([0, 0, 130, 130, 131], 131), ([3, 60, 190], 200)])
+def test_packed_gradients(dev, cu, t):
+    args = make((1, t), 2, 4, 64, 48, torch.float32, dev, seed=t)
+    state = torch.randn(len(cu) - 1, 4, 64, 48, generator=torch.Generator().manual_seed(3)).to(dev)
+    check_gradients(dev, args, state, cu)
+
+
+@gpu
+def test_gradients_at_the_gates_ends(dev):
+    q, k, v, g, beta = make((1, 150), 1, 5, 64, 64, torch.float32, dev)
+    g[:, :, 0] = 0
+    g[:, ::7, 1] = -200
+    g[:, :, 2] = -40
+    beta[:, :, 3] = 0
+    beta[:, 1::2, 2] = 0
+    beta[:, :, 4] = 1
+    check_gradients(dev, (q, k, v, g, beta), torch.randn(1, 5, 64, 64, device=dev))
+
+
+@gpu
+def test_gradients_of_some_inputs_and_strides(dev):
+    import amd_tuned_torch as P
+    q, k, v, g, beta = make((2, 90), 2, 4, 64, 32, torch.bfloat16, dev, gdtype=torch.bfloat16)
+    dout = torch.randn(2, 4, 90, 32, device=dev).bfloat16().transpose(1, 2)        # heads first
+    state = torch.zeros(2, 4, 64, 32, device=dev)
+    want = gradients64((q, k, v, g, beta), 0.125, state, dout, state)
+    for wanted in ((0,), (2, 4), (3,)):
+        leaves = [x.detach().clone().requires_grad_(i in wanted) for i, x in enumerate((q, k, v, g, beta))]
+        got = torch.autograd.grad(P.gated_delta_rule(*leaves), [leaves[i] for i in wanted], dout)
+        for i, x in zip(wanted, got):
+            close_grad(x.cpu(), want[i], NAMES[i])
+    one = beta[:, :, :1].detach().clone().requires_grad_()                         # a broadcast input
+    got, = torch.autograd.grad(P.gated_delta_rule(q, k, v, g, one.expand(2, 90, 4)), one, dout)
+    full = gradients64((q, k, v, g, one.detach().expand(2, 90, 4)), 0.125, state, dout, state)[4]
+    off = (got.double().cpu() - full.sum(-1, keepdim=True)).abs()                  # four rounded to bf16, then added
+    assert (off <= 2 * ULP[torch.bfloat16] * full.abs().sum(-1, keepdim=True) + 4 * F32 * full.abs().max()).all()
+    # only the final state is used
+    leaves = [x.detach().clone().requires_grad_() for x in (q, k, v, g, beta)]
+    S = P.gated_delta_rule(*leaves, return_final_state=True)[1]
+    got = torch.autograd.grad(S.sum(), leaves, allow_unused=True)
+    want = gradients64((q, k, v, g, beta), 0.125, state, torch.zeros_like(v), torch.ones_like(state))
+    for name, x, y in zip(NAMES, got, want):
+        close_grad(x.cpu(), y, name)
+
+
+@gpu
+def test_gradients_against_differences(dev):
+    """(L(x + e d) - L(x - e d)) / 2e of the kernel's own fp32 forward, e = 2^-7: a cubic term of at most
+    e^2 times a few, and rounding of 2^-20 / e of L, against the gradient's own size."""
+    import amd_tuned_torch as P
+    args = make((1, 100), 1, 2, 32, 32, torch.float32, dev, seed=4)
+    state = torch.randn(1, 2, 32, 32, generator=torch.Generator().manual_seed(3)).to(dev)
+    gen = torch.Generator().manual_seed(5)
+    dout = torch.randn(1, 100, 2, 32, generator=gen).to(dev).double()
+    dstate = torch.randn(1, 2, 32, 32, generator=gen).to(dev).double()
+
+    def loss(a):
+        out, S = P.gated_delta_rule(*a[:5], initial_state=a[5], return_final_state=True)
+        return (out.double() * dout).sum() + (S.double() * dstate).sum()
+
+    leaves = [x.requires_grad_() for x in (*args, state)]
+    grads = torch.autograd.grad(loss(leaves), leaves)
+    e = 2.0 ** -7
+    for i, name in enumerate(NAMES):
+        d = torch.randn(leaves[i].shape, generator=gen).to(dev) * (0.1 if i in (0, 1, 3) else 0.3)
+        ends = []
+        for sign in (1, -1):
+            a = [x.detach() for x in leaves]
+            a[i] = a[i] + sign * e * d
+            ends.append(loss(a))
+        slope = ((ends[0] - ends[1]) / (2 * e)).item()
+        want = (grads[i].double() * d.double()).sum().item()
+        size = (grads[i].double().norm() * d.double().norm()).item()
+        assert abs(slope - want) <= 1e-3 * size, (name, slope, want, size)
+
+
+@gpu
+def test_equal_bits_and_second_derivatives(dev):
+    import amd_tuned_torch as P
+    args = make((2, 200), 1, 4, 64, 64, torch.bfloat16, dev)
+    leaves = [x.requires_grad_() for x in args]
+    dout = torch.randn(2, 200, 4, 64, device=dev).bfloat16()
+    first = torch.autograd.grad(P.gated_delta_rule(*leaves), leaves, dout)
+    again = torch.autograd.grad(P.gated_delta_rule(*leaves), leaves, dout)
+    assert all(torch.equal(x, y) for x, y in zip(first, again))
+    small = [x.requires_grad_() for x in make((1, 9), 1, 2, 8, 8, torch.float32, dev)]
+    twice = []
+    for fn in (P.gated_delta_rule, P.gated_delta.gated_delta_rule_ref):
+        grads = torch.autograd.grad(fn(*small).square().sum(), small, create_graph=True)
+        twice.append(torch.autograd.grad(sum(x.square().sum() for x in grads), small))
+    for x, y in zip(*twice):
+        assert (x - y).abs().max() <= 1e-4 * y.abs().max()
+    with torch.no_grad():
+        assert not P.gated_delta_rule(*small).requires_grad
