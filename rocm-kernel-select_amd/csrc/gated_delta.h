@@ -104,17 +104,25 @@ __device__ __forceinline__ f32x4 mma_parts(const uint4 (&a)[NA], const uint4 (&b
   return c;
 }
 
+// A product's result D has rows 4 g + r in a lane; as the next product's B it needs 8 of 32.  So the 32
+// are taken in the order that gives a lane its own: element i of lane group g is row gdr_at(g, i) of two
+// row tiles, and every A that meets such a B has its columns in that order too.
+__device__ __forceinline__ constexpr int gdr_at(int g, int i) { return i < 4 ? 4 * g + i : 12 + 4 * g + i; }
+
 // v[0..N) as NP parts of N bf16 each
 template <int NP, int N, typename P>
 __device__ __forceinline__ void split_parts(const float* v, P (&out)[NP]) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float r = v[i];
+  for (int i = 0; i < N; i += 2) {
+    f2 r = {v[i], v[i + 1]};
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-      const __bf16 h = static_cast<__bf16>(r);
-      out[p][i] = h;
-      r -= static_cast<float>(h);
+      const b2 h = __builtin_convertvector(r, b2);
+      out[p][i] = h[0];
+      out[p][i + 1] = h[1];
+      if (p + 1 < NP) r -= __builtin_convertvector(h, f2);
     }
   }
 }

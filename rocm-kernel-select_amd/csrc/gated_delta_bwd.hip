@@ -28,6 +28,11 @@ template <typename T, int KP>
 __global__ __launch_bounds__(256) void gdr_bwd_chain_kernel(GdrArgs a) {
   constexpr int NP = kParts<T>, KS = KP / 32, MT = KP / 64, BV = 16;
   constexpr int SP = KP + 8, UP = 64 + 8;
+  // 8 of 32 rows in gdr_at's order
+  auto frag = [](const __bf16* p, int g) {
+    const uint2 lo = *reinterpret_cast<const uint2*>(p + 4 * g), hi = *reinterpret_cast<const uint2*>(p + 16 + 4 * g);
+    return make_uint4(lo.x, lo.y, hi.x, hi.y);
+  };
   __shared__ __align__(16) __bf16 sl[3][BV][SP], dl[NP][BV][UP], gl[3][BV][UP], ul[3][BV][UP], rl[3][BV][UP];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
   const int h = blockIdx.y, hk = h / a.group;
@@ -97,7 +102,7 @@ __global__ __launch_bounds__(256) void gdr_bwd_chain_kernel(GdrArgs a) {
 #pragma unroll
       for (int p = 0; p < NP; ++p) ka[p] = a.kf[kbase + ((s * 4 + wave) * NP + p) * 64 + lane];
 #pragma unroll
-      for (int p = 0; p < 3; ++p) b[p] = *reinterpret_cast<const uint4*>(&sl[p][c][32 * s + 8 * g]);
+      for (int p = 0; p < 3; ++p) b[p] = frag(&sl[p][c][32 * s], g);
       ks = mma_parts<NP, 3>(ka, b, ks);
     }
     for (int s = wave >> 1; s < 2; ++s) {
@@ -105,7 +110,7 @@ __global__ __launch_bounds__(256) void gdr_bwd_chain_kernel(GdrArgs a) {
 #pragma unroll
       for (int p = 0; p < 3; ++p) pa[p] = a.ptf[tbase + (tri_upper(wave, s) * 3 + p) * 64 + lane];
 #pragma unroll
-      for (int p = 0; p < NP; ++p) b[p] = *reinterpret_cast<const uint4*>(&dl[p][c][32 * s + 8 * g]);
+      for (int p = 0; p < NP; ++p) b[p] = frag(&dl[p][c][32 * s], g);
       pd = mma_parts<3, NP>(pa, b, pd);
     }
 #pragma unroll
@@ -118,7 +123,7 @@ __global__ __launch_bounds__(256) void gdr_bwd_chain_kernel(GdrArgs a) {
 #pragma unroll
       for (int p = 0; p < 3; ++p) ta[p] = a.ttf[tbase + (tri_upper(wave, s) * 3 + p) * 64 + lane];
 #pragma unroll
-      for (int p = 0; p < 3; ++p) b[p] = *reinterpret_cast<const uint4*>(&ul[p][c][32 * s + 8 * g]);
+      for (int p = 0; p < 3; ++p) b[p] = frag(&ul[p][c][32 * s], g);
       dr = mma_parts<3, 3>(ta, b, dr);
     }
     float* __restrict__ drc = a.drc + (slot * a.Hv + h) * (int64_t)64 * a.VP;
@@ -136,8 +141,8 @@ __global__ __launch_bounds__(256) void gdr_bwd_chain_kernel(GdrArgs a) {
       uint4 bq[3], bk[3];
 #pragma unroll
       for (int p = 0; p < 3; ++p) {
-        bq[p] = *reinterpret_cast<const uint4*>(&gl[p][c][32 * s + 8 * g]);
-        bk[p] = *reinterpret_cast<const uint4*>(&rl[p][c][32 * s + 8 * g]);
+        bq[p] = frag(&gl[p][c][32 * s], g);
+        bk[p] = frag(&rl[p][c][32 * s], g);
       }
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
@@ -360,11 +365,13 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
         const int ml = f < 2 ? f : f / 2 + 1, sl = f < 2 ? 0 : f & 1, mu = f < 4 ? f / 2 : f - 2, su = f < 4 ? f & 1 : 1;
         float v[8];
         bf16x8 parts[3];
-        split_parts<3, 8>(X + (16 * ml + c) * LD + 32 * sl + 8 * g, parts);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = X[(16 * ml + c) * LD + 32 * sl + gdr_at(g, i)];
+        split_parts<3, 8>(v, parts);
 #pragma unroll
         for (int p = 0; p < 3; ++p) fr[(f * 3 + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = X[(32 * su + 8 * g + i) * LD + 16 * mu + c];
+        for (int i = 0; i < 8; ++i) v[i] = X[(32 * su + gdr_at(g, i)) * LD + 16 * mu + c];
         split_parts<3, 8>(v, parts);
 #pragma unroll
         for (int p = 0; p < 3; ++p) fr[((kTri + f) * 3 + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);

@@ -18,17 +18,17 @@ namespace {
 
 constexpr int LD = 68;  // row pitch of the fp32 64 x 64 tiles in LDS: 16-byte rows, 4 banks apart
 
-// 8 consecutive elements of a row of N, zeros past its end
+// 4 consecutive elements of a row of N, zeros past its end
 template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ p, int c, int N, bool live, float* o) {
-  if (live && c + 8 <= N) {
-    T e[8];
-    __builtin_memcpy(e, p + c, 8 * sizeof(T));  // element alignment only
+__device__ __forceinline__ void load4(const T* __restrict__ p, int c, int N, bool live, float* o) {
+  if (live && c + 4 <= N) {
+    T e[4];
+    __builtin_memcpy(e, p + c, 4 * sizeof(T));  // element alignment only
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = to_f32(e[i]);
+    for (int i = 0; i < 4; ++i) o[i] = to_f32(e[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = live && c + i < N ? to_f32(p[c + i]) : 0.f;
+    for (int i = 0; i < 4; ++i) o[i] = live && c + i < N ? to_f32(p[c + i]) : 0.f;
   }
 }
 
@@ -85,8 +85,11 @@ __device__ __forceinline__ void write_lower(const float* __restrict__ M, uint4* 
   const int c = lane & 15, g = lane >> 4;
   for (int f = wave; f < kTri; f += 4) {
     const int m = f < 2 ? f : f / 2 + 1, s = f < 2 ? 0 : f & 1;
+    float v[8];
     bf16x8 parts[3];
-    split_parts<3, 8>(M + (16 * m + c) * LD + 32 * s + 8 * g, parts);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = M[(16 * m + c) * LD + 32 * s + gdr_at(g, i)];
+    split_parts<3, 8>(v, parts);
 #pragma unroll
     for (int p = 0; p < 3; ++p) out[(f * 3 + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
   }
@@ -99,7 +102,7 @@ __device__ __forceinline__ void write_transposed(const float* __restrict__ M, ui
     const int m = f < 4 ? f / 2 : f - 2, s = f < 4 ? f & 1 : 1;
     float v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = M[(32 * s + 8 * g + i) * LD + 16 * m + c];
+    for (int i = 0; i < 8; ++i) v[i] = M[(32 * s + gdr_at(g, i)) * LD + 16 * m + c];
     bf16x8 parts[3];
     split_parts<3, 8>(v, parts);
 #pragma unroll
@@ -119,8 +122,8 @@ __device__ __forceinline__ void write_columns(const uint4* __restrict__ frags, u
       bf16x8 v;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int tok = 32 * s + 8 * g + i;
-        v[i] = b[((((col >> 5) * 4 + (tok >> 4)) * NP + p) * 64 + (tok & 15) + 16 * ((col >> 3) & 3)) * 8 + (col & 7)];
+        const int tok = 32 * s + gdr_at(g, i);
+        v[i] = b[((((col >> 5) * 4 + (tok >> 4)) * NP + p) * 64 + (tok & 15) + 16 * ((col >> 2) & 3)) * 8 + (col & 3) + 4 * ((col >> 4) & 1)];
       }
       out[(f * NP + p) * 64 + lane] = __builtin_bit_cast(uint4, v);
     }
@@ -180,14 +183,16 @@ __global__ __launch_bounds__(256) void gdr_prepare_kernel(GdrArgs a) {
     for (int s = 0; s < KS; ++s) {
       float v[8];
       bf16x8 parts[NP];
-      load8(q, 32 * s + 8 * g, a.K, live, v);
+      load4(q, 32 * s + 4 * g, a.K, live, v);
+      load4(q, 32 * s + 16 + 4 * g, a.K, live, v + 4);
       split_parts<NP, 8>(v, parts);
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
         qr[s][p] = __builtin_bit_cast(uint4, parts[p]);
         if (owner) a.qf[kbase + ((s * 4 + wave) * NP + p) * 64 + lane] = qr[s][p];
       }
-      load8(k, 32 * s + 8 * g, a.K, live, v);
+      load4(k, 32 * s + 4 * g, a.K, live, v);
+      load4(k, 32 * s + 16 + 4 * g, a.K, live, v + 4);
       split_parts<NP, 8>(v, parts);
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
@@ -255,228 +260,275 @@ __global__ __launch_bounds__(256) void gdr_prepare_kernel(GdrArgs a) {
   }
 }
 
-// The state's chain.  Wave w has the chunk's tokens 16 w .. 16 w + 15, and rows w KP / 4 .. of the
-// state, as fp32 accumulators of 16 NT value columns; what another wave multiplies goes through LDS in
-// three bf16 parts, [column][row].
-template <typename T, int KP, int NT, bool KEEP>
-__global__ __launch_bounds__(256) void gdr_chain_kernel(GdrArgs a) {
-  constexpr int NP = kParts<T>, KS = KP / 32, MT = KP / 64, BV = 16 * NT;
-  constexpr int SP = KP + 8, UP = 64 + 8;  // pitches: 16-byte rows, 4 banks apart
-  __shared__ __align__(16) __bf16 sl[3][BV][SP], xl[3][BV][UP], ul[3][BV][UP], el[3][BV][UP];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-  const int h = blockIdx.y, hk = h / a.group;
-  const int64_t n = blockIdx.z;
-  const int v0 = blockIdx.x * BV;
+// Workgroup -> (value tile, head, sequence).  Workgroups are dealt to the 8 XCDs in turn; all value
+// tiles of a head and sequence get the same one, since they read the same fragments through its L2.
+__device__ __forceinline__ bool chain_place(const GdrArgs& a, int tiles, int* tile, int* h, int64_t* n) {
+  const int64_t j = blockIdx.x / 8, unit = j / tiles * 8 + blockIdx.x % 8;
+  *tile = (int)(j % tiles);
+  *h = (int)(unit % a.Hv);
+  *n = unit / a.Hv;
+  return *n < a.n;
+}
+
+// The state's chain: 16 value columns of one head's state, all of its key rows, from chunk to chunk.
+//
+// What bounds it is the time of one step, since a step needs the one before it: three products that
+// follow each other (K S, T X, K^T E U).  Four waves share them: wave w has the state's row tiles
+// w MT .. in its accumulators, multiplies them as they are (their layout is B's) with the K of all 64
+// tokens, and the four partial sums meet in LDS; then it has the tokens 16 w .. for X and e.  So the
+// state itself never leaves the registers.  Fragments are loaded right after their last use, for the
+// next chunk: a load has most of a step to arrive.  Four more waves make the outputs of the chunk
+// before, off the chain.  A barrier orders LDS only; loads stay in flight across it.
+template <typename T, int KP, bool KEEP>
+__global__ __launch_bounds__(KEEP ? 256 : 512) void gdr_chain_kernel(GdrArgs a) {
+  constexpr int NP = kParts<T>, KS = KP / 32, MT = KP / 64, KW = MT > 1 ? MT / 2 : 1;
+  constexpr int KF = KS * 4 * NP * 64;
+  __shared__ f32x4 kp[4][4][64], qp[KEEP ? 1 : 4][4][64];  // partial sums [state wave][token tile][lane]
+  __shared__ uint2 xl[2][3][64][2], el[2][3][64][2];       // X and E U in parts, as B is read
+  __shared__ f32x4 ul[KEEP ? 1 : 4][64];                   // U, fp32
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int tile, h;
+  int64_t n;
+  if (!chain_place(a, KEEP ? a.VP / 16 : (a.V + 15) / 16, &tile, &h, &n)) return;
+  const int hk = h / a.group, col = tile * 16 + c;
   const GdrSeq seq = gdr_seq(a.cu, a.T, n);
-  T* __restrict__ o = static_cast<T*>(a.o);
-  f32x4 S[MT][NT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int col = v0 + 16 * t + c;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = 16 * (wave * MT + m) + 4 * g + r;
-        S[m][t][r] = a.s0 && row < a.K && col < a.V ? a.s0[((n * a.Hv + h) * a.K + row) * a.V + col] : 0.f;
-      }
-    }
-  auto put_state = [&]() {
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        bf16x4 parts[3];
-        const float x[4] = {S[m][t][0], S[m][t][1], S[m][t][2], S[m][t][3]};
-        split_parts<3, 4>(x, parts);
-#pragma unroll
-        for (int p = 0; p < 3; ++p)
-          *reinterpret_cast<bf16x4*>(&sl[p][16 * t + c][16 * (wave * MT + m) + 4 * g]) = parts[p];
-      }
-  };
-  put_state();
-  __syncthreads();
   const int64_t chunks = (seq.len + kGdrC - 1) / kGdrC;
-  for (int64_t ch = 0; ch < chunks; ++ch) {
-    const int64_t slot = seq.slot + ch;
-    const int64_t left = seq.len - ch * kGdrC;
-    const int rows = (int)(left < kGdrC ? left : kGdrC);
-    const int64_t t0 = seq.begin + ch * kGdrC;
-    const int64_t kbase = (slot * a.Hk + hk) * (int64_t)(KS * 4 * NP * 64);
-    const int64_t tbase = (slot * a.Hv + h) * (int64_t)(kTri * 3 * 64);
-    const float* __restrict__ row = a.row + (slot * a.Hv + h) * 192;
-    float grown[4], rest[4], beta[4], vv[NT][4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = 16 * wave + 4 * g + r;
-      grown[r] = row[i];
-      rest[r] = row[64 + i];
-      beta[r] = row[128 + i];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int col = v0 + 16 * t + c;
-        vv[t][r] = i < rows && col < a.V
-                       ? to_f32(static_cast<const T*>(a.v)[seq.batch * a.v_s[0] + (t0 + i) * a.v_s[1] + h * a.v_s[2] + col])
-                       : 0.f;
-      }
-    }
-    const float all = row[63];
-    if constexpr (KEEP) {
-      float* __restrict__ sc = a.sc + (slot * a.Hv + h) * (int64_t)KP * a.VP;
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sc[(int64_t)(16 * (wave * MT + m) + 4 * g + r) * a.VP + v0 + 16 * t + c] = S[m][t][r];
-    }
-    // K S and Q S of this wave's tokens
-    f32x4 ks[NT], qs[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) ks[t] = qs[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      uint4 ka[NP], qa[NP];
-#pragma unroll
-      for (int p = 0; p < NP; ++p) {
-        ka[p] = a.kf[kbase + ((s * 4 + wave) * NP + p) * 64 + lane];
-        if constexpr (!KEEP) qa[p] = a.qf[kbase + ((s * 4 + wave) * NP + p) * 64 + lane];
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        uint4 b[3];
-#pragma unroll
-        for (int p = 0; p < 3; ++p) b[p] = *reinterpret_cast<const uint4*>(&sl[p][16 * t + c][32 * s + 8 * g]);
-        ks[t] = mma_parts<NP, 3>(ka, b, ks[t]);
-        if constexpr (!KEEP) qs[t] = mma_parts<NP, 3>(qa, b, qs[t]);
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float x[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = vv[t][r] - grown[r] * ks[t][r];
-      bf16x4 parts[3];
-      split_parts<3, 4>(x, parts);
-#pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x4*>(&xl[p][16 * t + c][16 * wave + 4 * g]) = parts[p];
-    }
-    __syncthreads();
-    // the errors, and U
-    f32x4 e[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) e[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s <= wave >> 1; ++s) {
-      uint4 ta[3];
-#pragma unroll
-      for (int p = 0; p < 3; ++p) ta[p] = a.tf[tbase + (tri_lower(wave, s) * 3 + p) * 64 + lane];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        uint4 b[3];
-#pragma unroll
-        for (int p = 0; p < 3; ++p) b[p] = *reinterpret_cast<const uint4*>(&xl[p][16 * t + c][32 * s + 8 * g]);
-        e[t] = mma_parts<3, 3>(ta, b, e[t]);
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      float u[4], eu[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        u[r] = beta[r] * e[t][r];
-        eu[r] = rest[r] * u[r];
-      }
-      bf16x4 parts[3];
-      if constexpr (KEEP) {
-        float* __restrict__ ec = a.ec + (slot * a.Hv + h) * (int64_t)64 * a.VP;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) ec[(int64_t)(16 * wave + 4 * g + r) * a.VP + v0 + 16 * t + c] = e[t][r];
-      } else {
-        split_parts<3, 4>(u, parts);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x4*>(&ul[p][16 * t + c][16 * wave + 4 * g]) = parts[p];
-      }
-      split_parts<3, 4>(eu, parts);
-#pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x4*>(&el[p][16 * t + c][16 * wave + 4 * g]) = parts[p];
-    }
-    __syncthreads();
-    // the state, into LDS for the next chunk
+  const uint4* __restrict__ kf = a.kf + (seq.slot * a.Hk + hk) * KF;
+  const uint4* __restrict__ qf = a.qf + (seq.slot * a.Hk + hk) * KF;
+  const uint4* __restrict__ ktf = a.ktf + (seq.slot * a.Hk + hk) * KF;
+  const uint4* __restrict__ tf = a.tf + (seq.slot * a.Hv + h) * (int64_t)(kTri * 3 * 64);
+  const uint4* __restrict__ pf = a.pf + (seq.slot * a.Hv + h) * (int64_t)(kTri * 3 * 64);
+  const float* __restrict__ row = a.row + (seq.slot * a.Hv + h) * 192;
+  const int64_t kstep = (int64_t)a.Hk * KF, tstep = (int64_t)a.Hv * (kTri * 3 * 64), rstep = (int64_t)a.Hv * 192;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  if (wave < 4) {
+    f32x4 S[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) S[m][t] *= all;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      uint4 ka[MT][NP];
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int p = 0; p < NP; ++p) ka[m][p] = a.ktf[kbase + (((wave * MT + m) * 2 + s) * NP + p) * 64 + lane];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        uint4 b[3];
-#pragma unroll
-        for (int p = 0; p < 3; ++p) b[p] = *reinterpret_cast<const uint4*>(&el[p][16 * t + c][32 * s + 8 * g]);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) S[m][t] = mma_parts<NP, 3>(ka[m], b, S[m][t]);
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * (wave * MT + m) + 4 * g + r;
+        S[m][r] = a.s0 && i < a.K && col < a.V ? a.s0[((n * a.Hv + h) * a.K + i) * a.V + col] : 0.f;
       }
-    }
-    put_state();
-    if constexpr (!KEEP) {  // the output
+    const int s0 = MT == 1 ? wave / 2 : wave * KW;  // this wave's first 32 key columns
+    uint4 ka[KW][4][NP], qa[KW][4][NP], ta[2][3], kta[MT][2][NP];
+    T va[4];
+    f32x4 grown, eb, beta;
+    float all;
+    auto load_k = [&](int64_t ch) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int s = 0; s < KW; ++s)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) qs[t][r] *= grown[r];
-      for (int s = 0; s <= wave >> 1; ++s) {
-        uint4 pa[3];
+        for (int m = 0; m < 4; ++m)
 #pragma unroll
-        for (int p = 0; p < 3; ++p) pa[p] = a.pf[tbase + (tri_lower(wave, s) * 3 + p) * 64 + lane];
+          for (int p = 0; p < NP; ++p) ka[s][m][p] = kf[ch * kstep + (((s0 + s) * 4 + m) * NP + p) * 64 + lane];
+    };
+    auto load_q = [&](int64_t ch) {
+      if constexpr (!KEEP) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          uint4 b[3];
+        for (int s = 0; s < KW; ++s)
 #pragma unroll
-          for (int p = 0; p < 3; ++p) b[p] = *reinterpret_cast<const uint4*>(&ul[p][16 * t + c][32 * s + 8 * g]);
-          qs[t] = mma_parts<3, 3>(pa, b, qs[t]);
-        }
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) qa[s][m][p] = qf[ch * kstep + (((s0 + s) * 4 + m) * NP + p) * 64 + lane];
       }
+    };
+    auto load_rows = [&](int64_t ch) {
+      const float* __restrict__ rw = row + ch * rstep;
+      grown = *reinterpret_cast<const f32x4*>(rw + 16 * wave + 4 * g);
+      const f32x4 rest = *reinterpret_cast<const f32x4*>(rw + 64 + 16 * wave + 4 * g);
+      beta = *reinterpret_cast<const f32x4*>(rw + 128 + 16 * wave + 4 * g);
+      eb = rest * beta;
+      all = rw[63];
+      const int64_t left = seq.len - ch * kGdrC;
+      const int64_t t0 = seq.begin + ch * kGdrC;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = 16 * wave + 4 * g + r;
-        const int64_t at = ((seq.batch * a.T + t0 + i) * a.Hv + h) * (int64_t)a.V;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int col = v0 + 16 * t + c;
-          if (i < rows && col < a.V) o[at + col] = from_f32<T>(a.scale * qs[t][r]);
-        }
+        va[r] = i < left && col < a.V
+                    ? static_cast<const T*>(a.v)[seq.batch * a.v_s[0] + (t0 + i) * a.v_s[1] + h * a.v_s[2] + col]
+                    : from_f32<T>(0.f);
       }
+    };
+    auto load_t = [&](int64_t ch) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s <= wave >> 1)
+#pragma unroll
+          for (int p = 0; p < 3; ++p) ta[s][p] = tf[ch * tstep + (tri_lower(wave, s) * 3 + p) * 64 + lane];
+    };
+    auto load_kt = [&](int64_t ch) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) kta[m][s][p] = ktf[ch * kstep + (((wave * MT + m) * 2 + s) * NP + p) * 64 + lane];
+    };
+    if (chunks > 0) {
+      load_k(0);
+      load_rows(0);
+      load_q(0);
+      load_t(0);
+      load_kt(0);
     }
-    __syncthreads();
-  }
-  if (a.s1) {
+    for (int64_t ch = 0; ch < chunks; ++ch) {
+      const int64_t next = ch + 1 < chunks ? ch + 1 : ch;  // (the last chunk's again at the end)
+      if constexpr (KEEP) {
+        float* __restrict__ sc = a.sc + ((seq.slot + ch) * a.Hv + h) * (int64_t)KP * a.VP;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int col = v0 + 16 * t + c;
+          for (int r = 0; r < 4; ++r) sc[(int64_t)(16 * (wave * MT + m) + 4 * g + r) * a.VP + col] = S[m][r];
+      }
+      uint4 sp[KW][3];
+#pragma unroll
+      for (int s = 0; s < KW; ++s) {
+        float x[8];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int row = 16 * (wave * MT + m) + 4 * g + r;
-          if (row < a.K && col < a.V) a.s1[((n * a.Hv + h) * a.K + row) * a.V + col] = S[m][t][r];
+          x[r] = MT > 1 ? S[MT > 1 ? 2 * s : 0][r] : (wave & 1) ? 0.f : S[0][r];
+          x[4 + r] = MT > 1 ? S[MT > 1 ? 2 * s + 1 : 0][r] : (wave & 1) ? S[0][r] : 0.f;
+        }
+        bf16x8 parts[3];
+        split_parts<3, 8>(x, parts);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) sp[s][p] = __builtin_bit_cast(uint4, parts[p]);
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        f32x4 y = zero;
+#pragma unroll
+        for (int s = 0; s < KW; ++s) y = mma_parts<NP, 3>(ka[s][m], sp[s], y);
+        kp[wave][m][lane] = y;
+      }
+      load_k(next);
+      __syncthreads();
+      const f32x4 y = (kp[0][wave][lane] + kp[1][wave][lane]) + (kp[2][wave][lane] + kp[3][wave][lane]);
+      {
+        float x[4];
+        bf16x4 parts[3];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = to_f32(va[r]) - grown[r] * y[r];
+        split_parts<3, 4>(x, parts);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) xl[wave >> 1][p][lane][wave & 1] = __builtin_bit_cast(uint2, parts[p]);
+      }
+      if constexpr (!KEEP) {
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          f32x4 z = zero;
+#pragma unroll
+          for (int s = 0; s < KW; ++s) z = mma_parts<NP, 3>(qa[s][m], sp[s], z);
+          qp[wave][m][lane] = z;
+        }
+        load_q(next);
+      }
+      __syncthreads();
+      f32x4 e = zero;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s <= wave >> 1) {
+          uint4 b[3];
+#pragma unroll
+          for (int p = 0; p < 3; ++p) b[p] = *reinterpret_cast<const uint4*>(&xl[s][p][lane]);
+          e = mma_parts<3, 3>(ta[s], b, e);
+        }
+      load_t(next);
+      {
+        float x[4];
+        bf16x4 parts[3];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = eb[r] * e[r];
+        split_parts<3, 4>(x, parts);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) el[wave >> 1][p][lane][wave & 1] = __builtin_bit_cast(uint2, parts[p]);
+        if constexpr (KEEP) {
+          float* __restrict__ ec = a.ec + ((seq.slot + ch) * a.Hv + h) * (int64_t)64 * a.VP;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) ec[(int64_t)(16 * wave + 4 * g + r) * a.VP + col] = e[r];
+        } else {
+          ul[wave][lane] = beta * e;
         }
       }
-  }
-  // tokens of a packed row before its first sequence and after its last have an output of zero
-  if (!KEEP && a.cu && (n == 0 || n == a.n - 1)) {
-    const int64_t from[2] = {n == 0 ? 0 : a.T, n == a.n - 1 ? seq.begin + seq.len : a.T};
-    const int64_t to[2] = {n == 0 ? seq.begin : a.T, a.T};
-    for (int z = 0; z < 2; ++z)
-      for (int64_t i = from[z] + (tid >> 4); i < to[z]; i += 16)
+      const float decay = all;
+      load_rows(next);
+      __syncthreads();
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int col = v0 + 16 * t + (tid & 15);
-          if (col < a.V) o[(i * a.Hv + h) * (int64_t)a.V + col] = from_f32<T>(0.f);
+      for (int m = 0; m < MT; ++m) S[m] *= decay;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        uint4 b[3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) b[p] = *reinterpret_cast<const uint4*>(&el[s][p][lane]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) S[m] = mma_parts<NP, 3>(kta[m][s], b, S[m]);
+      }
+      load_kt(next);
+    }
+    if (a.s1) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = 16 * (wave * MT + m) + 4 * g + r;
+          if (i < a.K && col < a.V) a.s1[((n * a.Hv + h) * a.K + i) * a.V + col] = S[m][r];
         }
+    }
+  } else if constexpr (!KEEP) {
+    const int m = wave - 4;
+    T* __restrict__ o = static_cast<T*>(a.o);
+    uint4 pa[2][3];
+    f32x4 grown;
+    auto load = [&](int64_t ch) {
+      grown = *reinterpret_cast<const f32x4*>(row + ch * rstep + 16 * m + 4 * g);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s <= m >> 1)
+#pragma unroll
+          for (int p = 0; p < 3; ++p) pa[s][p] = pf[ch * tstep + (tri_lower(m, s) * 3 + p) * 64 + lane];
+    };
+    if (chunks > 0) load(0);
+    for (int64_t ch = 0; ch < chunks; ++ch) {
+      __syncthreads();
+      __syncthreads();
+      __syncthreads();
+      // from here to the state waves' next barrier but one, qp and ul are this chunk's
+      f32x4 y = (qp[0][m][lane] + qp[1][m][lane]) + (qp[2][m][lane] + qp[3][m][lane]);
+      y *= grown;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (s <= m >> 1) {
+          float x[8];
+          bf16x8 parts[3];
+          uint4 b[3];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            x[r] = ul[2 * s][lane][r];
+            x[4 + r] = ul[2 * s + 1][lane][r];
+          }
+          split_parts<3, 8>(x, parts);
+#pragma unroll
+          for (int p = 0; p < 3; ++p) b[p] = __builtin_bit_cast(uint4, parts[p]);
+          y = mma_parts<3, 3>(pa[s], b, y);
+        }
+      load(ch + 1 < chunks ? ch + 1 : ch);
+      const int64_t left = seq.len - ch * kGdrC, t0 = seq.begin + ch * kGdrC;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int i = 16 * m + 4 * g + r;
+        if (i < left && col < a.V) o[((seq.batch * a.T + t0 + i) * a.Hv + h) * (int64_t)a.V + col] = from_f32<T>(a.scale * y[r]);
+      }
+    }
+    // tokens of a packed row before its first sequence and after its last have an output of zero
+    if (a.cu && (n == 0 || n == a.n - 1)) {
+      const int64_t from[2] = {n == 0 ? 0 : a.T, n == a.n - 1 ? seq.begin + seq.len : a.T};
+      const int64_t to[2] = {n == 0 ? seq.begin : a.T, a.T};
+      for (int z = 0; z < 2; ++z)
+        for (int64_t i = from[z] + 4 * m + g; i < to[z]; i += 16)
+          if (col < a.V) o[(i * a.Hv + h) * (int64_t)a.V + col] = from_f32<T>(0.f);
+    }
   }
 }
 
@@ -489,10 +541,10 @@ int launch_prepare(const GdrArgs& a, bool backward, hipStream_t s) {
 }
 template <typename T, int KP>
 int launch_chain(const GdrArgs& a, bool keep, hipStream_t s) {
-  if (keep)
-    hipLaunchKernelGGL((gdr_chain_kernel<T, KP, 1, true>), dim3((unsigned)(a.VP / 16), (unsigned)a.Hv, (unsigned)a.n), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((gdr_chain_kernel<T, KP, 1, false>), dim3((unsigned)((a.V + 15) / 16), (unsigned)a.Hv, (unsigned)a.n), dim3(256), 0, s, a);
+  const int64_t units = (a.n * a.Hv + 7) / 8 * 8, grid = units * (keep ? a.VP / 16 : (a.V + 15) / 16);
+  if (grid > 0x7fffffff) return fail(ATK_UNSUPPORTED, "gated delta: too many heads, sequences and value columns");
+  if (keep) hipLaunchKernelGGL((gdr_chain_kernel<T, KP, true>), dim3((unsigned)grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((gdr_chain_kernel<T, KP, false>), dim3((unsigned)grid), dim3(512), 0, s, a);
   return check_launch("gdr_chain_kernel");
 }
 
