@@ -32,14 +32,16 @@ struct GdrArgs {
   int64_t slots;         // chunks, unused ones of packed sequences among them
   int Hk, Hv, group, K, V, g_dtype, b_dtype;
   float scale;
-  // workspace: fragments by (slot, key head) and (slot, value head), and each chunk's decays
+  // workspace: fragments by (key head, slot) and (value head, slot), and each chunk's decays; the chunks
+  // of a sequence follow each other, so a chain's next loads are near its last
   uint4* kf; uint4* qf; uint4* ktf; uint4* tf; uint4* pf;
-  float* row;            // [slot][Hv][3][64]: exp(G_i), exp(G_63 - G_i), beta_i
-  // the backward's: fragments of Q^T, (1 + diag(beta) W)^-T and lower(Q K^T * D)^T; each chunk's G in
-  // 64 bits; the state and the errors that the forward chain had at each chunk, and the gradients of
-  // the state after it and of U: [slot][Hv][KP or 64][VP] fp32, VP = V padded to 32
+  void* dump;            // 256 elements that nobody reads
+  float* row;            // [Hv][slot][3][64]: exp(G_i), exp(G_63 - G_i), beta_i
+  // the backward's: fragments of Q^T, (1 + diag(beta) W)^-T and lower(Q K^T * D)^T; each chunk's G / ln 2
+  // as two floats; the state and the errors that the forward chain had at each chunk, and the gradients of
+  // the state after it and of U: [Hv][slot][KP or 64][VP] fp32, VP = V padded to 32
   uint4* qtf; uint4* ttf; uint4* ptf;
-  double* gsum;
+  float2* gsum;
   float* sc; float* ec; float* dsc; float* drc;
   const void* dout; const float* ds1; float* ds0;
   void* dq; void* dk; void* dv; void* dg; void* dbeta;
@@ -125,6 +127,32 @@ __device__ __forceinline__ void split_parts(const float* v, P (&out)[NP]) {
       if (p + 1 < NP) r -= __builtin_convertvector(h, f2);
     }
   }
+}
+
+// The same for N row tiles that meet one B: the tiles take turns, so that no product waits for the one
+// before it.
+template <int N, int NA, int NB>
+__device__ __forceinline__ void mma_tiles(const uint4 (&a)[N][NA], const uint4 (&b)[NB], f32x4 (&c)[N]) {
+#pragma unroll
+  for (int s = 2; s >= 0; --s)
+#pragma unroll
+    for (int p = 0; p < NA; ++p)
+#pragma unroll
+      for (int q = 0; q < NB; ++q)
+        if (p + q == s) {
+#pragma unroll
+          for (int n = 0; n < N; ++n) c[n] = mma(a[n][p], b[q], c[n]);
+          __builtin_amdgcn_sched_barrier(0);  // (the compiler would run each tile's products in a row)
+        }
+}
+
+// parts that an fp32 matrix is multiplied in where the product is only rounded to T: two of bf16 (16
+// bits) are beyond what a 16-bit result shows
+template <typename T> inline constexpr int kOutParts = sizeof(T) == 4 ? 3 : 2;
+
+// exp(G_i - G_j) from G / ln 2 in two floats each: the difference of near sums is exact
+__device__ __forceinline__ float gdr_decay(float2 i, float2 j) {
+  return __builtin_amdgcn_exp2f((i.x - j.x) + (i.y - j.y));
 }
 
 // fragments of the lower triangle of a 64 x 64 matrix in 16 x 32 tiles (row tile m, column half s)

@@ -71,9 +71,9 @@ __global__ __launch_bounds__(256) void gdr_bwd_chain_kernel(GdrArgs a) {
     const int64_t left = seq.len - ch * kGdrC;
     const int rows = (int)(left < kGdrC ? left : kGdrC);
     const int64_t t0 = seq.begin + ch * kGdrC;
-    const int64_t kbase = (slot * a.Hk + hk) * (int64_t)(KS * 4 * NP * 64);
-    const int64_t tbase = (slot * a.Hv + h) * (int64_t)(kTri * 3 * 64);
-    const float* __restrict__ row = a.row + (slot * a.Hv + h) * 192;
+    const int64_t kbase = (hk * a.slots + slot) * (int64_t)(KS * 4 * NP * 64);
+    const int64_t tbase = (h * a.slots + slot) * (int64_t)(kTri * 3 * 64);
+    const float* __restrict__ row = a.row + (h * a.slots + slot) * 192;
     const float all = row[63];
     float rest[4], bg[4], x[4], y[4];
 #pragma unroll
@@ -90,7 +90,7 @@ __global__ __launch_bounds__(256) void gdr_bwd_chain_kernel(GdrArgs a) {
     put_rows(x, dl);
     put_rows(y, gl);
     __syncthreads();
-    float* __restrict__ dsc = a.dsc + (slot * a.Hv + h) * (int64_t)KP * a.VP;
+    float* __restrict__ dsc = a.dsc + (h * a.slots + slot) * (int64_t)KP * a.VP;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(256) void gdr_bwd_chain_kernel(GdrArgs a) {
       for (int p = 0; p < 3; ++p) b[p] = frag(&ul[p][c][32 * s], g);
       dr = mma_parts<3, 3>(ta, b, dr);
     }
-    float* __restrict__ drc = a.drc + (slot * a.Hv + h) * (int64_t)64 * a.VP;
+    float* __restrict__ drc = a.drc + (h * a.slots + slot) * (int64_t)64 * a.VP;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       drc[(int64_t)(16 * wave + 4 * g + r) * a.VP + col] = dr[r];
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
   constexpr int FRAGS = 2 * kTri * 3 * 64;                       // a triangle's and its transpose's
   __shared__ uint4 fr[STAGE > FRAGS ? STAGE : FRAGS];
   __shared__ __align__(16) float nm[64 * LD], mm[64 * LD];
-  __shared__ double gs[64];
+  __shared__ float2 gs[64];
   __shared__ float grown[64], rest[64], beta[64], dg_part[4][64], dots[4];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
   const int64_t slot = blockIdx.x;
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
   if (at < 0 || at >= seq.len) return;
   const int rows = (int)(seq.len - at < kGdrC ? seq.len - at : kGdrC);
   const int64_t t0 = seq.begin + at, token = seq.batch * a.T + t0;
-  const int64_t kbase = (slot * a.Hk + hk) * (int64_t)(KS * 4 * NP * 64);
+  const int64_t kbase = (hk * a.slots + slot) * (int64_t)(KS * 4 * NP * 64);
   const T* __restrict__ qp = static_cast<const T*>(a.q) + seq.batch * a.q_s[0] + t0 * a.q_s[1] + hk * a.q_s[2];
   const T* __restrict__ kp = static_cast<const T*>(a.k) + seq.batch * a.k_s[0] + t0 * a.k_s[1] + hk * a.k_s[2];
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
     for (int t = 0; t < NT; ++t) dqs[m][t] = dks[m][t] = zero;
   for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
-    const int64_t hs = slot * a.Hv + h;
+    const int64_t hs = h * a.slots + slot;
     const float* __restrict__ sc = a.sc + hs * KP * a.VP;
     const float* __restrict__ dsc = a.dsc + hs * KP * a.VP;
     const float* __restrict__ ec = a.ec + hs * 64 * a.VP;
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int i = 16 * it + 4 * g + r;
-          const float d = j <= i ? beta[j] * expf((float)(gs[i] - gs[j])) : 0.f;
+          const float d = j <= i ? beta[j] * gdr_decay(gs[i], gs[j]) : 0.f;
           nm[i * LD + j] = j <= i ? a.scale * d * ne[t][r] : 0.f;
           mm[i * LD + j] = j < i ? -beta[i] * d * me[t][r] : 0.f;
           if (i == j && i < rows) store_param(a.dbeta, a.b_dtype, (token + i) * a.Hv + h, me[t][r]);
