@@ -366,6 +366,9 @@ __device__ __forceinline__ bool chain_place(const GdrArgs& a, int tiles, int* ti
 // state itself never leaves the registers.  Fragments are loaded right after their last use, for the
 // next chunk: a load has most of a step to arrive.  Four more waves bring V into LDS a chunk ahead and
 // make the chunk's outputs, off the chain.  A barrier orders LDS only; loads stay in flight across it.
+// All value tiles of a head read the same fragments, so each brings its share of the lines of the chunk
+// after next into their L2 (a word of each): what the next chunk's loads then find there took a step
+// longer than they have.
 // FULL: no tile of value columns ends in one of fewer than 4, so a lane has 4 columns of a token in one
 // load or store (the last of a tile that V ends in overlap).
 template <typename T, int KP, bool KEEP, bool FULL>
@@ -383,7 +386,8 @@ __global__ __launch_bounds__(512) void gdr_chain_kernel(GdrArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int tile, h;
   int64_t n;
-  if (!chain_place(a, KEEP ? a.VP / 16 : (a.V + 15) / 16, &tile, &h, &n)) return;
+  const int tiles = KEEP ? a.VP / 16 : (a.V + 15) / 16;
+  if (!chain_place(a, tiles, &tile, &h, &n)) return;
   const int hk = h / a.group, col = tile * 16 + c;
   const GdrSeq seq = gdr_seq(a.cu, a.T, n);
   const int64_t chunks = (seq.len + kGdrC - 1) / kGdrC;
@@ -625,6 +629,23 @@ __global__ __launch_bounds__(512) void gdr_chain_kernel(GdrArgs a) {
 #pragma unroll
           for (int p = 0; p < NP; ++p) qa[s][p] = qf[(s * 4 * NP + p) * 64 + lane];
       };
+      // the lines of K, Q, K^T, T and P in turn; this lane's among them, if there is one left for it
+      constexpr int LK = KF / 8, LT = kTri * 3 * 8, LP = kTri * OP * 8, LINES = 3 * LK + LT + LP;
+      int line = (tile * 4 + m) * 64 + lane;
+      line = line < LINES ? line : LINES - 1;
+      const uint4* ahead = line < LK       ? a.kf + (hk * a.slots + seq.slot) * KF + line * 8
+                           : line < 2 * LK ? a.qf + (hk * a.slots + seq.slot) * KF + (line - LK) * 8
+                           : line < 3 * LK ? a.ktf + (hk * a.slots + seq.slot) * KF + (line - 2 * LK) * 8
+                           : line < 3 * LK + LT ? a.tf + (h * a.slots + seq.slot) * (int64_t)(kTri * 3 * 64) + (line - 3 * LK) * 8
+                                                : a.pf + (h * a.slots + seq.slot) * (int64_t)(kTri * OP * 64) + (line - 3 * LK - LT) * 8;
+      const int ahead_step = line < 3 * LK ? KF : line < 3 * LK + LT ? kTri * 3 * 64 : kTri * OP * 64;
+      ahead += (chunks > 2 ? 2 : 0) * ahead_step;
+      uint32_t seen = 0;
+      auto touch = [&](bool another) {
+        asm volatile("" ::"v"(seen));  // (the load before this one has arrived by now)
+        ahead += another ? ahead_step : 0;
+        seen = *reinterpret_cast<const uint32_t*>(ahead);
+      };
       auto load_p = [&]() {
 #pragma unroll
         for (int p = 0; p < OP; ++p) pa[0][p] = pf[p * 64 + lane];
@@ -661,6 +682,7 @@ __global__ __launch_bounds__(512) void gdr_chain_kernel(GdrArgs a) {
         qf += more ? qstep : 0;
         load_q();
         load_next_v(more ? left - kGdrC : left);
+        touch(ch + 3 < chunks);
         __syncthreads();
         // ul is this chunk's for two barriers
         y = (y + z) * grown;
