@@ -80,6 +80,16 @@ __device__ __forceinline__ int64_t gdr_seq_of_slot(const int* __restrict__ cu, i
   return lo;
 }
 
+// Workgroup -> (value tile, head, sequence).  Workgroups are dealt to the 8 XCDs in turn; all value
+// tiles of a head and sequence get the same one, since they read the same fragments through its L2.
+__device__ __forceinline__ bool gdr_chain_place(const GdrArgs& a, int tiles, int* tile, int* h, int64_t* n) {
+  const int64_t j = blockIdx.x / 8, unit = j / tiles * 8 + blockIdx.x % 8;
+  *tile = (int)(j % tiles);
+  *h = (int)(unit % a.Hv);
+  *n = unit / a.Hv;
+  return *n < a.n;
+}
+
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));

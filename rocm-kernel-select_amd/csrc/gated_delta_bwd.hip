@@ -23,150 +23,315 @@ namespace {
 
 constexpr int LD = 68;
 
-// The chain of dS'.  Distribution as in the forward's chain.
-template <typename T, int KP>
-__global__ __launch_bounds__(256) void gdr_bwd_chain_kernel(GdrArgs a) {
-  constexpr int NP = kParts<T>, KS = KP / 32, MT = KP / 64, BV = 16;
-  constexpr int SP = KP + 8, UP = 64 + 8;
-  // 8 of 32 rows in gdr_at's order
-  auto frag = [](const __bf16* p, int g) {
-    const uint2 lo = *reinterpret_cast<const uint2*>(p + 4 * g), hi = *reinterpret_cast<const uint2*>(p + 16 + 4 * g);
-    return make_uint4(lo.x, lo.y, hi.x, hi.y);
-  };
-  __shared__ __align__(16) __bf16 sl[3][BV][SP], dl[NP][BV][UP], gl[3][BV][UP], ul[3][BV][UP], rl[3][BV][UP];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-  const int h = blockIdx.y, hk = h / a.group;
-  const int64_t n = blockIdx.z;
-  const int col = blockIdx.x * BV + c;
+// The chain of dS', built as the forward's: four waves pass the state's gradient on, 16 value columns
+// of it; four more make what needs dO alone, a chunk ahead: scale P^T dO and Q^T (scale exp(G) dO).
+// FULL as there.
+template <typename T, int KP, bool FULL>
+__global__ __launch_bounds__(512) void gdr_bwd_chain_kernel(GdrArgs a) {
+  constexpr int NP = kParts<T>, KS = KP / 32, MT = KP / 64, KW = MT > 1 ? MT / 2 : 1;
+  constexpr int KF = KS * 4 * NP * 64;
+  __shared__ f32x4 kp[4][4][64];                            // partial sums of K dS'
+  __shared__ uint2 ul[2][3][64][2], rl[2][3][64][2];        // dU, and -beta exp(G) dR
+  __shared__ uint2 dl[2][NP][64][2], gl[2][3][64][2];       // dO, and scale exp(G) dO
+  __shared__ f32x4 pl[4][64];                               // scale P^T dO
+  __shared__ f32x4 ql[2][KP / 16][64];                      // Q^T (scale exp(G) dO), two chunks'
+  __shared__ f32x4 tl[4][64];                               // dO on its way from rows to columns
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int tile, h;
+  int64_t n;
+  if (!gdr_chain_place(a, a.VP / 16, &tile, &h, &n)) return;
+  const int hk = h / a.group, col = tile * 16 + c;
   const GdrSeq seq = gdr_seq(a.cu, a.T, n);
-  f32x4 S[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * (wave * MT + m) + 4 * g + r;
-      S[m][r] = a.ds1 && row < a.K && col < a.V ? a.ds1[((n * a.Hv + h) * a.K + row) * a.V + col] : 0.f;
-    }
-  auto put_state = [&]() {
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      bf16x4 parts[3];
-      const float x[4] = {S[m][0], S[m][1], S[m][2], S[m][3]};
-      split_parts<3, 4>(x, parts);
-#pragma unroll
-      for (int p = 0; p < 3; ++p) *reinterpret_cast<bf16x4*>(&sl[p][c][16 * (wave * MT + m) + 4 * g]) = parts[p];
-    }
-  };
-  auto put_rows = [&](const float* x, auto& to) {  // this lane's 4 tokens of one column
-    constexpr int P = sizeof(to) / sizeof(to[0]);
-    bf16x4 parts[P];
-    split_parts<P, 4>(x, parts);
-#pragma unroll
-    for (int p = 0; p < P; ++p) *reinterpret_cast<bf16x4*>(&to[p][c][16 * wave + 4 * g]) = parts[p];
-  };
-  put_state();
-  const int64_t chunks = (seq.len + kGdrC - 1) / kGdrC;
-  for (int64_t ch = chunks - 1; ch >= 0; --ch) {
-    const int64_t slot = seq.slot + ch;
-    const int64_t left = seq.len - ch * kGdrC;
-    const int rows = (int)(left < kGdrC ? left : kGdrC);
-    const int64_t t0 = seq.begin + ch * kGdrC;
-    const int64_t kbase = (hk * a.slots + slot) * (int64_t)(KS * 4 * NP * 64);
-    const int64_t tbase = (h * a.slots + slot) * (int64_t)(kTri * 3 * 64);
-    const float* __restrict__ row = a.row + (h * a.slots + slot) * 192;
-    const float all = row[63];
-    float rest[4], bg[4], x[4], y[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = 16 * wave + 4 * g + r;
-      const float grown = row[i];
-      rest[r] = row[64 + i];
-      bg[r] = -row[128 + i] * grown;
-      x[r] = i < rows && col < a.V
-                 ? to_f32(static_cast<const T*>(a.dout)[((seq.batch * a.T + t0 + i) * a.Hv + h) * (int64_t)a.V + col])
-                 : 0.f;
-      y[r] = a.scale * grown * x[r];
-    }
-    put_rows(x, dl);
-    put_rows(y, gl);
-    __syncthreads();
-    float* __restrict__ dsc = a.dsc + (h * a.slots + slot) * (int64_t)KP * a.VP;
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) dsc[(int64_t)(16 * (wave * MT + m) + 4 * g + r) * a.VP + col] = S[m][r];
-    f32x4 ks = {0.f, 0.f, 0.f, 0.f}, pd = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      uint4 ka[NP], b[3];
-#pragma unroll
-      for (int p = 0; p < NP; ++p) ka[p] = a.kf[kbase + ((s * 4 + wave) * NP + p) * 64 + lane];
-#pragma unroll
-      for (int p = 0; p < 3; ++p) b[p] = frag(&sl[p][c][32 * s], g);
-      ks = mma_parts<NP, 3>(ka, b, ks);
-    }
-    for (int s = wave >> 1; s < 2; ++s) {
-      uint4 pa[3], b[NP];
-#pragma unroll
-      for (int p = 0; p < 3; ++p) pa[p] = a.ptf[tbase + (tri_upper(wave, s) * 3 + p) * 64 + lane];
-#pragma unroll
-      for (int p = 0; p < NP; ++p) b[p] = frag(&dl[p][c][32 * s], g);
-      pd = mma_parts<3, NP>(pa, b, pd);
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = a.scale * pd[r] + rest[r] * ks[r];
-    put_rows(x, ul);
-    __syncthreads();
-    f32x4 dr = {0.f, 0.f, 0.f, 0.f};
-    for (int s = wave >> 1; s < 2; ++s) {
-      uint4 ta[3], b[3];
-#pragma unroll
-      for (int p = 0; p < 3; ++p) ta[p] = a.ttf[tbase + (tri_upper(wave, s) * 3 + p) * 64 + lane];
-#pragma unroll
-      for (int p = 0; p < 3; ++p) b[p] = frag(&ul[p][c][32 * s], g);
-      dr = mma_parts<3, 3>(ta, b, dr);
-    }
-    float* __restrict__ drc = a.drc + (h * a.slots + slot) * (int64_t)64 * a.VP;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      drc[(int64_t)(16 * wave + 4 * g + r) * a.VP + col] = dr[r];
-      x[r] = bg[r] * dr[r];
-    }
-    put_rows(x, rl);
-    __syncthreads();
-#pragma unroll
-    for (int m = 0; m < MT; ++m) S[m] *= all;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      uint4 bq[3], bk[3];
-#pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        bq[p] = frag(&gl[p][c][32 * s], g);
-        bk[p] = frag(&rl[p][c][32 * s], g);
-      }
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        uint4 qa[NP], ka[NP];
-#pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          qa[p] = a.qtf[kbase + (((wave * MT + m) * 2 + s) * NP + p) * 64 + lane];
-          ka[p] = a.ktf[kbase + (((wave * MT + m) * 2 + s) * NP + p) * 64 + lane];
-        }
-        S[m] = mma_parts<NP, 3>(qa, bq, S[m]);
-        S[m] = mma_parts<NP, 3>(ka, bk, S[m]);
-      }
-    }
-    put_state();  // read after the next chunk's first barrier; its last readers are two barriers back
-    __syncthreads();
-  }
-  if (a.ds0) {
+  const int64_t chunks = (seq.len + kGdrC - 1) / kGdrC, end = seq.slot + chunks - 1;  // from the last chunk down
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  if (wave < 4) {
+    const int s0 = MT == 1 ? wave / 2 : wave * KW;
+    const uint4* __restrict__ kf = a.kf + (hk * a.slots + end) * KF + s0 * 4 * NP * 64;
+    const uint4* __restrict__ ktf = a.ktf + (hk * a.slots + end) * KF + wave * MT * 2 * NP * 64;
+    const bool two = wave < 2;  // column halves of this wave's rows of T^T
+    const uint4* __restrict__ tf = a.ttf + (h * a.slots + end) * (int64_t)(kTri * 3 * 64) + tri_upper(wave, wave >> 1) * 3 * 64;
+    const float* __restrict__ row = a.row + (h * a.slots + end) * 192;
+    float* __restrict__ dsc = a.dsc + (h * a.slots + end) * (int64_t)KP * a.VP + col;
+    float* __restrict__ drc = a.drc + (h * a.slots + end) * (int64_t)64 * a.VP + (16 * wave + 4 * g) * (int64_t)a.VP + col;
+    f32x4 S[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int row = 16 * (wave * MT + m) + 4 * g + r;
-        if (row < a.K && col < a.V) a.ds0[((n * a.Hv + h) * a.K + row) * a.V + col] = S[m][r];
+        const int i = 16 * (wave * MT + m) + 4 * g + r;
+        S[m][r] = a.ds1 && i < a.K && col < a.V ? a.ds1[((n * a.Hv + h) * a.K + i) * a.V + col] : 0.f;
       }
+    // here, and not in every pass of the loop, the compiler waits for these loads
+#pragma unroll
+    for (int m = 0; m < MT; ++m) asm volatile("" : "+v"(S[m]));
+    uint4 ka[KW][4][NP], ta[2][3], kta[2][MT][NP];
+    f32x4 grown, rest, beta;
+    float all;
+    int lane63 = 63;
+    asm("" : "+v"(lane63));  // a vector address: a scalar load would be waited for at the next barrier
+    auto load_k = [&]() {
+#pragma unroll
+      for (int s = 0; s < KW; ++s)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) ka[s][m][p] = kf[((s * 4 + m) * NP + p) * 64 + lane];
+    };
+    auto load_t = [&]() {
+#pragma unroll
+      for (int p = 0; p < 3; ++p) ta[0][p] = tf[p * 64 + lane];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) ta[1][p] = tf[((two ? 3 : 0) + p) * 64 + lane];
+    };
+    auto load_kt = [&]() {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) kta[s][m][p] = ktf[((m * 2 + s) * NP + p) * 64 + lane];
+    };
+    auto load_rows = [&]() {
+      grown = *reinterpret_cast<const f32x4*>(row + 16 * wave + 4 * g);
+      rest = *reinterpret_cast<const f32x4*>(row + 64 + 16 * wave + 4 * g);
+      beta = *reinterpret_cast<const f32x4*>(row + 128 + 16 * wave + 4 * g);
+      all = row[lane63];
+    };
+    if (chunks > 0) {
+      load_k();
+      load_rows();
+      load_t();
+      load_kt();
+    }
+    __syncthreads();  // the helpers' dO of the last chunk
+    __syncthreads();  // and what they make of it
+    for (int64_t ch = chunks - 1; ch >= 0; --ch) {
+      const bool more = ch > 0;
+      kf -= more ? KF : 0;
+      ktf -= more ? KF : 0;
+      tf -= more ? kTri * 3 * 64 : 0;
+      row -= more ? 192 : 0;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dsc[(int64_t)(16 * (wave * MT + m) + 4 * g + r) * a.VP] = S[m][r];
+      dsc -= (int64_t)KP * a.VP;
+      f32x4 y[4] = {zero, zero, zero, zero};
+#pragma unroll
+      for (int s = 0; s < KW; ++s) {
+        float x[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[r] = MT > 1 ? S[MT > 1 ? 2 * s : 0][r] : (wave & 1) ? 0.f : S[0][r];
+          x[4 + r] = MT > 1 ? S[MT > 1 ? 2 * s + 1 : 0][r] : (wave & 1) ? S[0][r] : 0.f;
+        }
+        bf16x8 parts[3];
+        uint4 sp[3];
+        split_parts<3, 8>(x, parts);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) sp[p] = __builtin_bit_cast(uint4, parts[p]);
+        mma_tiles<4, NP, 3>(ka[s], sp, y);
+      }
+      load_k();
+#pragma unroll
+      for (int m = 0; m < 4; ++m) kp[wave][m][lane] = y[m];
+      __syncthreads();
+      {
+        const f32x4 y0 = kp[0][wave][lane], y1 = kp[1][wave][lane], y2 = kp[2][wave][lane], y3 = kp[3][wave][lane];
+        const f32x4 z = (y0 + y1) + (y2 + y3), pd = pl[wave][lane];
+        float x[4];
+        bf16x4 parts[3];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = pd[r] + rest[r] * z[r];
+        split_parts<3, 4>(x, parts);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) ul[wave >> 1][p][lane][wave & 1] = __builtin_bit_cast(uint2, parts[p]);
+      }
+      __syncthreads();
+      f32x4 dr;
+      {
+        f32x4 part[3] = {zero, zero, zero};  // three sums, so that no product waits for the one before it
+        uint4 b[2][3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) b[0][p] = *reinterpret_cast<const uint4*>(&ul[wave >> 1][p][lane]);
+        if (two)
+#pragma unroll
+          for (int p = 0; p < 3; ++p) b[1][p] = *reinterpret_cast<const uint4*>(&ul[1][p][lane]);
+        auto half = [&](int s) {
+          part[0] = mma(ta[s][2], b[s][0], part[0]);
+          part[1] = mma(ta[s][1], b[s][1], part[1]);
+          part[2] = mma(ta[s][0], b[s][2], part[2]);
+          __builtin_amdgcn_sched_barrier(0);
+          part[0] = mma(ta[s][1], b[s][0], part[0]);
+          part[1] = mma(ta[s][0], b[s][1], part[1]);
+          part[2] = mma(ta[s][0], b[s][0], part[2]);
+        };
+        half(0);
+        if (two) half(1);
+        dr = (part[0] + part[1]) + part[2];
+      }
+      {
+        float x[4];
+        bf16x4 parts[3];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = -beta[r] * grown[r] * dr[r];
+        split_parts<3, 4>(x, parts);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) rl[wave >> 1][p][lane][wave & 1] = __builtin_bit_cast(uint2, parts[p]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) drc[r * (int64_t)a.VP] = dr[r];
+      drc -= (int64_t)64 * a.VP;
+      load_t();
+      __syncthreads();
+      {
+        f32x4 z[MT];
+        uint4 b[2][3];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int p = 0; p < 3; ++p) b[s][p] = *reinterpret_cast<const uint4*>(&rl[s][p][lane]);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          S[m] = S[m] * all + ql[ch & 1][wave * MT + m][lane];
+          z[m] = zero;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        mma_tiles<MT, NP, 3>(kta[1], b[1], z);
+        mma_tiles<MT, NP, 3>(kta[0], b[0], S);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) S[m] += z[m];
+      }
+      load_rows();
+      load_kt();
+    }
+    if (a.ds0) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = 16 * (wave * MT + m) + 4 * g + r;
+          if (i < a.K && col < a.V) a.ds0[((n * a.Hv + h) * a.K + i) * a.V + col] = S[m][r];
+        }
+    }
+  } else {
+    const int m = wave - 4;
+    const int tok = 16 * m + (lane >> 2);
+    const bool dead = tile * 16 >= a.V;  // a tile of padding: dO of zeros
+    const int c4 = FULL && !dead ? (tile * 16 + 4 * (lane & 3) + 4 <= a.V ? 4 * (lane & 3) : a.V - 4 - tile * 16) : 4 * (lane & 3);
+    const int64_t os = (int64_t)a.Hv * a.V, last = (chunks - 1) * kGdrC;
+    const T* __restrict__ op = static_cast<const T*>(a.dout) + ((seq.batch * a.T + seq.begin + last) * a.Hv + h) * (int64_t)a.V +
+                               (dead ? 0 : tile * 16 + (FULL ? c4 : 0));
+    const bool two = m < 2;
+    const float* __restrict__ row = a.row + (h * a.slots + end) * 192 + 16 * m + 4 * g;
+    const uint4* __restrict__ pf = a.ptf + (h * a.slots + end) * (int64_t)(kTri * 3 * 64) + tri_upper(m, m >> 1) * 3 * 64;
+    const uint4* __restrict__ qtf = a.qtf + (hk * a.slots + end) * KF + m * MT * 2 * NP * 64;
+    T oa[4];
+    bool gone;
+    f32x4 grown;
+    uint4 pa[2][3], qa[2][MT][NP];
+    auto load_o = [&](int64_t left) {
+      gone = dead || tok >= left;
+      const T* __restrict__ p = op + (tok < left ? tok * os : 0);
+      if constexpr (FULL) {
+        __builtin_memcpy(oa, p, 4 * sizeof(T));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) oa[j] = p[tile * 16 + c4 + j < a.V ? c4 + j : 0];
+      }
+      grown = *reinterpret_cast<const f32x4*>(row);
+    };
+    auto load_p = [&]() {
+#pragma unroll
+      for (int p = 0; p < 3; ++p) pa[0][p] = pf[p * 64 + lane];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) pa[1][p] = pf[((two ? 3 : 0) + p) * 64 + lane];
+    };
+    auto load_q = [&]() {
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) qa[s][t][p] = qtf[((t * 2 + s) * NP + p) * 64 + lane];
+    };
+    auto put_o = [&]() {  // this wave's 16 tokens, through LDS from rows to columns
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        tl[m][16 * (lane >> 4) + c4 + j][(lane >> 2) & 3] =
+            gone || (!FULL && tile * 16 + c4 + j >= a.V) ? 0.f : to_f32(oa[j]);
+      __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses keep their order)
+      const f32x4 x = tl[m][lane], y = a.scale * grown * x;
+      bf16x4 exact[NP], parts[3];
+      const float xs[4] = {x[0], x[1], x[2], x[3]}, ys[4] = {y[0], y[1], y[2], y[3]};
+      split_parts<NP, 4>(xs, exact);
+      split_parts<3, 4>(ys, parts);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) dl[m >> 1][p][lane][m & 1] = __builtin_bit_cast(uint2, exact[p]);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) gl[m >> 1][p][lane][m & 1] = __builtin_bit_cast(uint2, parts[p]);
+      __builtin_amdgcn_wave_barrier();
+    };
+    auto products = [&](int buffer) {
+      f32x4 y = zero, z = zero, q[MT];
+      uint4 b[NP], d[2][3];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) b[p] = *reinterpret_cast<const uint4*>(&dl[m >> 1][p][lane]);
+      y = mma_parts<3, NP>(pa[0], b, y);
+      if (two) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) b[p] = *reinterpret_cast<const uint4*>(&dl[1][p][lane]);
+        z = mma_parts<3, NP>(pa[1], b, z);
+      }
+      pl[m][lane] = a.scale * (y + z);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int p = 0; p < 3; ++p) d[s][p] = *reinterpret_cast<const uint4*>(&gl[s][p][lane]);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) q[t] = zero;
+      mma_tiles<MT, NP, 3>(qa[0], d[0], q);
+      mma_tiles<MT, NP, 3>(qa[1], d[1], q);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) ql[buffer][m * MT + t][lane] = q[t];
+    };
+    tl[m][lane] = zero;  // columns past V keep it
+    __builtin_amdgcn_wave_barrier();
+    // Rows past the end of a sequence's last chunk are zeros; the chunks before it are whole.
+    auto next = [&](bool more) {
+      op -= more ? kGdrC * os : 0;
+      row -= more ? 192 : 0;
+      pf -= more ? kTri * 3 * 64 : 0;
+      qtf -= more ? KF : 0;
+    };
+    if (chunks > 0) {
+      load_o(seq.len - last);
+      put_o();
+      load_p();
+      load_q();
+    }
+    __syncthreads();
+    if (chunks > 0) {
+      products((chunks - 1) & 1);
+      next(chunks > 1);
+      load_o(chunks > 1 ? kGdrC : seq.len - last);
+      load_p();
+      load_q();
+    }
+    __syncthreads();
+    for (int64_t ch = chunks - 1; ch >= 0; --ch) {
+      // beside chunk ch: the products of the chunk before it (at the end the first one's again, unread)
+      __syncthreads();
+      put_o();
+      __syncthreads();
+      products((ch - 1) & 1);
+      next(ch > 1);
+      load_o(ch > 0 ? kGdrC : seq.len);
+      load_p();
+      load_q();
+      __syncthreads();
+    }
   }
 }
 
@@ -472,7 +637,10 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
 
 template <typename T, int KP>
 int launch(const GdrArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL((gdr_bwd_chain_kernel<T, KP>), dim3((unsigned)(a.VP / 16), (unsigned)a.Hv, (unsigned)a.n), dim3(256), 0, s, a);
+  const int64_t grid = (a.n * a.Hv + 7) / 8 * 8 * (a.VP / 16);
+  if (grid > 0x7fffffff) return fail(ATK_UNSUPPORTED, "gated delta backward: too many heads, sequences and value columns");
+  if (a.V % 16 == 0 || a.V % 16 >= 4) hipLaunchKernelGGL((gdr_bwd_chain_kernel<T, KP, true>), dim3((unsigned)grid), dim3(512), 0, s, a);
+  else hipLaunchKernelGGL((gdr_bwd_chain_kernel<T, KP, false>), dim3((unsigned)grid), dim3(512), 0, s, a);
   if (int rc = check_launch("gdr_bwd_chain_kernel")) return rc;
   if (a.T == 0) return ATK_OK;
   hipLaunchKernelGGL((gdr_grads_kernel<T, KP>), dim3((unsigned)a.slots, (unsigned)a.Hk), dim3(256), 0, s, a);

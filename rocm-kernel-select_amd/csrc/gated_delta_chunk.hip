@@ -347,16 +347,6 @@ __global__ __launch_bounds__(256) void gdr_prepare_kernel(GdrArgs a) {
   }
 }
 
-// Workgroup -> (value tile, head, sequence).  Workgroups are dealt to the 8 XCDs in turn; all value
-// tiles of a head and sequence get the same one, since they read the same fragments through its L2.
-__device__ __forceinline__ bool chain_place(const GdrArgs& a, int tiles, int* tile, int* h, int64_t* n) {
-  const int64_t j = blockIdx.x / 8, unit = j / tiles * 8 + blockIdx.x % 8;
-  *tile = (int)(j % tiles);
-  *h = (int)(unit % a.Hv);
-  *n = unit / a.Hv;
-  return *n < a.n;
-}
-
 // The state's chain: 16 value columns of one head's state, all of its key rows, from chunk to chunk.
 //
 // What bounds it is the time of one step, since a step needs the one before it: three products that
@@ -387,7 +377,7 @@ __global__ __launch_bounds__(512) void gdr_chain_kernel(GdrArgs a) {
   int tile, h;
   int64_t n;
   const int tiles = KEEP ? a.VP / 16 : (a.V + 15) / 16;
-  if (!chain_place(a, tiles, &tile, &h, &n)) return;
+  if (!gdr_chain_place(a, tiles, &tile, &h, &n)) return;
   const int hk = h / a.group, col = tile * 16 + c;
   const GdrSeq seq = gdr_seq(a.cu, a.T, n);
   const int64_t chunks = (seq.len + kGdrC - 1) / kGdrC;
@@ -600,6 +590,8 @@ __global__ __launch_bounds__(512) void gdr_chain_kernel(GdrArgs a) {
       for (int j = 0; j < 4; ++j) vl[m][16 * (lane >> 4) + c4 + j][(lane >> 2) & 3] = dead ? 0.f : to_f32(va[j]);
       if (m < 3) rl[64 * m + lane] = ra;
     };
+    vl[m][lane] = zero;  // columns past V keep it
+    __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses keep their order)
     if (chunks > 0) {
       load_v(seq.len);
       put_v();
@@ -704,7 +696,7 @@ __global__ __launch_bounds__(512) void gdr_chain_kernel(GdrArgs a) {
         load_p();
 #pragma unroll
         for (int r = 0; r < 4; ++r) ol[m][4 * g + r][c] = from_f32<T>(a.scale * y[r]);
-        __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses keep their order)
+        __builtin_amdgcn_wave_barrier();
         T out[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) out[j] = ol[m][lane >> 2][c4 + j];
