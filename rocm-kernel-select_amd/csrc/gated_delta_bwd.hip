@@ -21,8 +21,6 @@
 namespace atk {
 namespace {
 
-constexpr int LD = 68;
-
 // The chain of dS', built as the forward's: four waves pass the state's gradient on, 16 value columns
 // of it; four more make what needs dO alone, a chunk ahead: scale P^T dO and Q^T (scale exp(G) dO).
 // FULL as there.
@@ -347,20 +345,35 @@ __device__ __forceinline__ void tri_tile(int t, int* i, int* j) {
   *j = t - *i * (*i + 1) / 2;
 }
 
-// What one chunk's gradients need of that chunk, for one key head and all of its value heads.  Wave w
-// has key columns w KP / 4 .. of dq and dk for all 64 tokens.  The value columns are walked 32 at a
-// time: the waves bring 16 tokens each of dO, dR and e into LDS as fragments, and every wave
-// multiplies all of them with its own rows of S and dS', which it splits itself.
+// sum over each 16 lanes, in all of them
+__device__ __forceinline__ float row16_sum(float v) {
+  v += dpp_mov<0xB1>(v);
+  v += dpp_mov<0x4E>(v);
+  v += dpp_mov<0x141>(v);
+  return v + dpp_mov<0x140>(v);
+}
+
+// What one chunk's gradients need of that chunk, for one key head and all of its value heads.  Each of
+// eight waves has 16 NT key columns of dq and dk, for all 64 tokens or (64 columns) for 32.  The value columns are walked 32 at a
+// time: the waves bring dO, dR and e of all tokens into LDS as fragments (the next 32 columns on their
+// way meanwhile), and every wave multiplies them with its own rows of S and dS', which it splits
+// itself.  dO e^T and dR e^T, whose 16 x 16 tiles on and below the diagonal the waves share out, are
+// made both ways round: a result's layout is that of the transpose's rows, so N, M and their
+// transposes go from the accumulators straight into LDS as fragments.  K^T's and Q^T's fragments hold
+// for each lane the elements that its accumulators have, so the row products of dG need no more loads.
 template <typename T, int KP>
-__global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
-  constexpr int NP = kParts<T>, KS = KP / 32, NT = KP / 64;
-  constexpr int STAGE = 4 * (NP + 6) * 64;                       // fragments of 32 value columns
-  constexpr int FRAGS = 2 * kTri * 3 * 64;                       // a triangle's and its transpose's
-  __shared__ uint4 fr[STAGE > FRAGS ? STAGE : FRAGS];
-  __shared__ __align__(16) float nm[64 * LD], mm[64 * LD];
+__global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
+  constexpr int NP = kParts<T>, KS = KP / 32, W = 8, NT = KP > 128 ? KP / 128 : 1;
+  constexpr int CW = KP / 16 / NT, MR = 4 * CW / W;  // waves side by side over the key columns; row tiles of each
+  constexpr int TILES = (20 + W - 1) / W;  // of the twenty, this wave's: wave, wave + W, ..
+  constexpr int UNIT = NP + 6;             // fragments of 16 tokens: dO, dR, e
+  __shared__ uint4 st[4 * UNIT * 64];
+  __shared__ uint2 nf[2][kTri * 3 * 64][2], mf[2][kTri * 3 * 64][2];  // N and M, their transposes
   __shared__ float2 gs[64];
-  __shared__ float grown[64], rest[64], beta[64], dg_part[4][64], dots[4];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+  __shared__ float grown[64], rest[64], beta[64], dg_part[CW][64], dots[W];
+  const int tid = threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int cw = wave % CW, m0 = wave / CW * MR;
   const int64_t slot = blockIdx.x;
   const int hk = blockIdx.y;
   const int64_t n = gdr_seq_of_slot(a.cu, a.T, a.n, slot);
@@ -368,68 +381,117 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
   const int64_t at = (slot - seq.slot) * kGdrC;
   if (at < 0 || at >= seq.len) return;
   const int rows = (int)(seq.len - at < kGdrC ? seq.len - at : kGdrC);
-  const int64_t t0 = seq.begin + at, token = seq.batch * a.T + t0;
+  const int64_t token = seq.batch * a.T + seq.begin + at;
   const int64_t kbase = (hk * a.slots + slot) * (int64_t)(KS * 4 * NP * 64);
-  const T* __restrict__ qp = static_cast<const T*>(a.q) + seq.batch * a.q_s[0] + t0 * a.q_s[1] + hk * a.q_s[2];
-  const T* __restrict__ kp = static_cast<const T*>(a.k) + seq.batch * a.k_s[0] + t0 * a.k_s[1] + hk * a.k_s[2];
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  f32x4 dqs[4][NT], dks[4][NT];  // sums over the group
+  // halves of fragments that lie beyond the diagonal: (row tile, column half, half) of N and of its transpose
+  for (int z = tid; z < 4 * 3 * 64; z += 64 * W) {
+    const int p = z / 64 % 3, l = z % 64, q = z / 192;
+    const int f = q == 0 ? tri_lower(0, 0) : q == 1 ? tri_lower(2, 1) : q == 2 ? tri_upper(1, 0) : tri_upper(3, 1);
+    nf[q >> 1][(f * 3 + p) * 64 + l][q < 2] = mf[q >> 1][(f * 3 + p) * 64 + l][q < 2] = make_uint2(0, 0);
+  }
+  f32x4 dqs[MR][NT], dks[MR][NT];  // sums over the group
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
+  for (int m = 0; m < MR; ++m)
 #pragma unroll
     for (int t = 0; t < NT; ++t) dqs[m][t] = dks[m][t] = zero;
+  // one unit of 16 tokens a wave and turn: 0..3 dO and dR, 4..7 e
+  constexpr int UNITS = 8 / W;
   for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
+    // (opaque to the compiler, which would keep the addresses of every access in registers for the next head)
+    int lane = tid & 63;
+    asm volatile("" : "+v"(lane));
+    const int c = lane & 15, g = lane >> 4;
     const int64_t hs = h * a.slots + slot;
-    const float* __restrict__ sc = a.sc + hs * KP * a.VP;
-    const float* __restrict__ dsc = a.dsc + hs * KP * a.VP;
+    const float* __restrict__ sc = a.sc + hs * KP * a.VP + (16 * cw * NT + c) * (int64_t)a.VP + 8 * g;
+    const float* __restrict__ dsc = a.dsc + hs * KP * a.VP + (16 * cw * NT + c) * (int64_t)a.VP + 8 * g;
     const float* __restrict__ ec = a.ec + hs * 64 * a.VP;
     const float* __restrict__ drc = a.drc + hs * 64 * a.VP;
+    f32x4 rs[NT][2], rd[NT][2], ru[UNITS][2];
+    T ro[8];
+    auto load = [&](int v0) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+          rs[t][z] = *reinterpret_cast<const f32x4*>(sc + 16 * t * (int64_t)a.VP + v0 + 4 * z);
+          rd[t][z] = *reinterpret_cast<const f32x4*>(dsc + 16 * t * (int64_t)a.VP + v0 + 4 * z);
+        }
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int unit = wave + W * u, i = 16 * (unit & 3) + c;
+        const float* __restrict__ p = (unit < 4 ? drc : ec) + (int64_t)i * a.VP + v0 + 8 * g;
+        ru[u][0] = *reinterpret_cast<const f32x4*>(p);
+        ru[u][1] = *reinterpret_cast<const f32x4*>(p + 4);
+      }
+      const int i = 16 * (wave & 3) + c, col = v0 + 8 * g;
+      const T* __restrict__ p = static_cast<const T*>(a.dout) + ((token + (i < rows ? i : 0)) * a.Hv + h) * (int64_t)a.V;
+      if (col + 8 <= a.V) {
+        __builtin_memcpy(ro, p + col, 8 * sizeof(T));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ro[j] = p[col + j < a.V ? col + j : 0];
+      }
+    };
+    load(0);
     if (tid < 64) {
       gs[tid] = a.gsum[hs * 64 + tid];
       grown[tid] = a.row[hs * 192 + tid];
       rest[tid] = a.row[hs * 192 + 64 + tid];
       beta[tid] = a.row[hs * 192 + 128 + tid];
     }
-    f32x4 dq[4][NT], dr[4][NT], dw[4][NT];  // dq, and dk as it is read and as it is written
-    f32x4 ne[3], me[3];                     // dO e^T and dR e^T, tiles wave, wave + 4, wave + 8 of the ten
+    f32x4 dq[MR][NT], dr[MR][NT], dw[MR][NT];  // dq, and dk as it is read and as it is written
+    f32x4 ne[TILES], me[TILES];
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < MR; ++m)
 #pragma unroll
       for (int t = 0; t < NT; ++t) dq[m][t] = dr[m][t] = dw[m][t] = zero;
 #pragma unroll
-    for (int t = 0; t < 3; ++t) ne[t] = me[t] = zero;
+    for (int x = 0; x < TILES; ++x) ne[x] = me[x] = zero;
     float dot = 0.f;  // <S, dS'>
     for (int v0 = 0; v0 < a.VP; v0 += 32) {
-      __syncthreads();  // fr's readers are past it
-      {
-        const int i = 16 * wave + c, col = v0 + 8 * g;  // a token, 8 columns
-        float x[8];
+      __syncthreads();  // st's readers are past it
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        const int unit = wave + W * u, m = unit & 3, i = 16 * m + c, col = v0 + 8 * g;
+        const float x[8] = {ru[u][0][0], ru[u][0][1], ru[u][0][2], ru[u][0][3], ru[u][1][0], ru[u][1][1], ru[u][1][2], ru[u][1][3]};
         bf16x8 parts[3];
-        const T* __restrict__ d = static_cast<const T*>(a.dout) + ((token + (i < rows ? i : 0)) * a.Hv + h) * (int64_t)a.V;
+        split_parts<3, 8>(x, parts);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = i < rows && col + j < a.V ? to_f32(d[col + j]) : 0.f;
-        bf16x8 exact[NP];
-        split_parts<NP, 8>(x, exact);
+        for (int p = 0; p < 3; ++p) st[(m * UNIT + NP + (unit < 4 ? 0 : 3) + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
+        if (unit < 4) {  // dO too, and dV = beta dR
+          float y[8];
+          bf16x8 exact[NP];
 #pragma unroll
-        for (int p = 0; p < NP; ++p) fr[(wave * (NP + 6) + p) * 64 + lane] = __builtin_bit_cast(uint4, exact[p]);
-        split_parts<3, 8>(drc + (int64_t)i * a.VP + col, parts);
+          for (int j = 0; j < 8; ++j) y[j] = i < rows && col + j < a.V ? to_f32(ro[j]) : 0.f;
+          split_parts<NP, 8>(y, exact);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) fr[(wave * (NP + 6) + NP + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
-        split_parts<3, 8>(ec + (int64_t)i * a.VP + col, parts);
+          for (int p = 0; p < NP; ++p) st[(m * UNIT + p) * 64 + lane] = __builtin_bit_cast(uint4, exact[p]);
+          if (i < rows) {
+            const float b = a.row[hs * 192 + 128 + i];
+            T* __restrict__ d = static_cast<T*>(a.dv) + ((token + i) * a.Hv + h) * (int64_t)a.V + col;
+            T z[8];
 #pragma unroll
-        for (int p = 0; p < 3; ++p) fr[(wave * (NP + 6) + NP + 3 + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
+            for (int j = 0; j < 8; ++j) z[j] = from_f32<T>(b * x[j]);
+            if (col + 8 <= a.V) {
+              __builtin_memcpy(d, z, 8 * sizeof(T));
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (col + j < a.V) d[j] = z[j];
+            }
+          }
+        }
       }
-      __syncthreads();
       uint4 sb[NT][3], db[NT][3];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int64_t o = (int64_t)(16 * (wave * NT + t) + c) * a.VP + v0 + 8 * g;
         float x[8], y[8];
         bf16x8 parts[3];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          x[j] = sc[o + j];
-          y[j] = dsc[o + j];
+          x[j] = rs[t][j >> 2][j & 3];
+          y[j] = rd[t][j >> 2][j & 3];
           dot += x[j] * y[j];
         }
         split_parts<3, 8>(x, parts);
@@ -439,15 +501,18 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
 #pragma unroll
         for (int p = 0; p < 3; ++p) db[t][p] = __builtin_bit_cast(uint4, parts[p]);
       }
+      load(v0 + 32 < a.VP ? v0 + 32 : v0);
+      __syncthreads();
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
+      for (int m = 0; m < MR; ++m) {
         uint4 da[NP], ra[3], ea[3];
+        const uint4* from = st + (m0 + m) * UNIT * 64 + lane;
 #pragma unroll
-        for (int p = 0; p < NP; ++p) da[p] = fr[(m * (NP + 6) + p) * 64 + lane];
+        for (int p = 0; p < NP; ++p) da[p] = from[p * 64];
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
-          ra[p] = fr[(m * (NP + 6) + NP + p) * 64 + lane];
-          ea[p] = fr[(m * (NP + 6) + NP + 3 + p) * 64 + lane];
+          ra[p] = from[(NP + p) * 64];
+          ea[p] = from[(NP + 3 + p) * 64];
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -455,159 +520,156 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
           dr[m][t] = mma_parts<3, 3>(ra, sb[t], dr[m][t]);
           dw[m][t] = mma_parts<3, 3>(ea, db[t], dw[m][t]);
         }
+        __builtin_amdgcn_sched_barrier(0);  // (all tiles' operands at once would not fit the registers)
       }
 #pragma unroll
-      for (int t = 0; t < 3; ++t) {
-        if (wave + 4 * t < 10) {
+      for (int x = 0; x < TILES; ++x) {
+        const int u = wave + W * x;
+        if (u < 20) {
           int i, j;
-          tri_tile(wave + 4 * t, &i, &j);
+          tri_tile(u % 10, &i, &j);
           uint4 da[NP], ra[3], ea[3];
 #pragma unroll
-          for (int p = 0; p < NP; ++p) da[p] = fr[(i * (NP + 6) + p) * 64 + lane];
+          for (int p = 0; p < NP; ++p) da[p] = st[(i * UNIT + p) * 64 + lane];
 #pragma unroll
           for (int p = 0; p < 3; ++p) {
-            ra[p] = fr[(i * (NP + 6) + NP + p) * 64 + lane];
-            ea[p] = fr[(j * (NP + 6) + NP + 3 + p) * 64 + lane];
+            ra[p] = st[(i * UNIT + NP + p) * 64 + lane];
+            ea[p] = st[(j * UNIT + NP + 3 + p) * 64 + lane];
           }
-          ne[t] = mma_parts<NP, 3>(da, ea, ne[t]);
-          me[t] = mma_parts<3, 3>(ra, ea, me[t]);
+          if (u < 10) {
+            ne[x] = mma_parts<NP, 3>(da, ea, ne[x]);
+            me[x] = mma_parts<3, 3>(ra, ea, me[x]);
+          } else {
+            ne[x] = mma_parts<3, NP>(ea, da, ne[x]);
+            me[x] = mma_parts<3, 3>(ea, ra, me[x]);
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
-    // N and M, row i, column j
+    // N and M: u < 10 has rows i and columns j, a fragment of the transposes; the others rows j
 #pragma unroll
-    for (int t = 0; t < 3; ++t) {
-      if (wave + 4 * t < 10) {
+    for (int x = 0; x < TILES; ++x) {
+      const int u = wave + W * x;
+      if (u < 20) {
         int it, jt;
-        tri_tile(wave + 4 * t, &it, &jt);
-        const int j = 16 * jt + c;
+        tri_tile(u % 10, &it, &jt);
+        const bool tall = u < 10;
+        float nv[4], mv[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int i = 16 * it + 4 * g + r;
+          const int i = tall ? 16 * it + 4 * g + r : 16 * it + c, j = tall ? 16 * jt + c : 16 * jt + 4 * g + r;
           const float d = j <= i ? beta[j] * gdr_decay(gs[i], gs[j]) : 0.f;
-          nm[i * LD + j] = j <= i ? a.scale * d * ne[t][r] : 0.f;
-          mm[i * LD + j] = j < i ? -beta[i] * d * me[t][r] : 0.f;
-          if (i == j && i < rows) store_param(a.dbeta, a.b_dtype, (token + i) * a.Hv + h, me[t][r]);
+          nv[r] = j <= i ? a.scale * d * ne[x][r] : 0.f;
+          mv[r] = j < i ? -beta[i] * d * me[x][r] : 0.f;
+          if (tall && i == j && i < rows) store_param(a.dbeta, a.b_dtype, (token + i) * a.Hv + h, me[x][r]);
         }
-      }
-    }
-    // tiles above the diagonal that fragments of 32 columns reach into: (0, 1) and (2, 3)
-    for (int z = tid; z < 512; z += 256) {
-      const int i = (z >> 8) * 32 + ((z >> 4) & 15), j = (z >> 8) * 32 + 16 + (z & 15);
-      nm[i * LD + j] = 0.f;
-      mm[i * LD + j] = 0.f;
-    }
-    float last = 0.f;  // sum of k . ((E U) dS'^T): this lane's share
+        const int f = tall ? tri_upper(jt, it >> 1) : tri_lower(it, jt >> 1), half = tall ? it & 1 : jt & 1;
+        bf16x4 parts[3];
+        split_parts<3, 4>(nv, parts);
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+        for (int p = 0; p < 3; ++p) nf[tall][(f * 3 + p) * 64 + lane][half] = __builtin_bit_cast(uint2, parts[p]);
+        split_parts<3, 4>(mv, parts);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) mf[tall][(f * 3 + p) * 64 + lane][half] = __builtin_bit_cast(uint2, parts[p]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    uint4 kb[2][NT][NP], qb[2][NT][NP];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          kb[s][t][p] = a.ktf[kbase + (((cw * NT + t) * 2 + s) * NP + p) * 64 + lane];
+          qb[s][t][p] = a.qtf[kbase + (((cw * NT + t) * 2 + s) * NP + p) * 64 + lane];
+        }
+    auto element = [&](const uint4 (&x)[NP], int i) {  // of a fragment, all parts
+      float v = 0.f;
+#pragma unroll
+      for (int p = NP - 1; p >= 0; --p) v += static_cast<float>(__builtin_bit_cast(bf16x8, x[p])[i]);
+      return v;
+    };
+    float last = m0 ? 0.f : grown[63] * dot;  // and the sum of k . ((E U) dS'^T): this lane's share
+#pragma unroll
+    for (int m = 0; m < MR; ++m)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = 16 * m + 4 * g + r;
+        const int i = 16 * (m0 + m) + 4 * g + r;
         const float sg = a.scale * grown[i], bg = -beta[i] * grown[i], eb = rest[i] * beta[i];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          const int col = 16 * (wave * NT + t) + c;
           dq[m][t][r] *= sg;
           dr[m][t][r] *= bg;
           dw[m][t][r] *= eb;
-          if (i < rows && col < a.K) last += to_f32(kp[i * a.k_s[1] + col]) * dw[m][t][r];
+          last += element(MR == 4 ? kb[m >> 1][t] : m0 ? kb[1][t] : kb[0][t], 4 * (m & 1) + r) * dw[m][t][r];
         }
       }
-    last += grown[63] * dot;
-    last = wave_sum(last);
+    last = wave_sum_rows(last);
     if (lane == 0) dots[wave] = last;
     __syncthreads();
-    // dV = beta dR
-    for (int i = tid >> 5; i < rows; i += 8) {
-      const float b = beta[i];
-      T* __restrict__ d = static_cast<T*>(a.dv) + ((token + i) * a.Hv + h) * (int64_t)a.V;
-      for (int col = tid & 31; col < a.V; col += 32) d[col] = from_f32<T>(b * drc[(int64_t)i * a.VP + col]);
-    }
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {  // N, then M: the products with K and Q
-      const float* __restrict__ X = which ? mm : nm;
-      for (int f = wave; f < kTri; f += 4) {
-        const int ml = f < 2 ? f : f / 2 + 1, sl = f < 2 ? 0 : f & 1, mu = f < 4 ? f / 2 : f - 2, su = f < 4 ? f & 1 : 1;
-        float v[8];
-        bf16x8 parts[3];
+    for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = X[(16 * ml + c) * LD + 32 * sl + gdr_at(g, i)];
-        split_parts<3, 8>(v, parts);
+      for (int m = 0; m < MR; ++m) {
+        const int mt = m0 + m;
+        uint4 xa[3], ya[3];
+        if (s == 0 || mt >= 2) {
+          const int f = tri_lower(mt, s) * 3 * 64 + lane;
 #pragma unroll
-        for (int p = 0; p < 3; ++p) fr[(f * 3 + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = X[(32 * su + gdr_at(g, i)) * LD + 16 * mu + c];
-        split_parts<3, 8>(v, parts);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) fr[((kTri + f) * 3 + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        uint4 kb[NT][NP], qb[NT][NP];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int p = 0; p < NP; ++p) {
-            kb[t][p] = a.ktf[kbase + (((wave * NT + t) * 2 + s) * NP + p) * 64 + lane];
-            if (!which) qb[t][p] = a.qtf[kbase + (((wave * NT + t) * 2 + s) * NP + p) * 64 + lane];
+          for (int p = 0; p < 3; ++p) {
+            xa[p] = *reinterpret_cast<const uint4*>(&nf[0][f + p * 64]);
+            ya[p] = *reinterpret_cast<const uint4*>(&mf[0][f + p * 64]);
           }
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          uint4 xa[3];
-          if (s == 0 || m >= 2) {
-#pragma unroll
-            for (int p = 0; p < 3; ++p) xa[p] = fr[(tri_lower(m, s) * 3 + p) * 64 + lane];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              if (!which) dq[m][t] = mma_parts<3, NP>(xa, kb[t], dq[m][t]);
-              else dr[m][t] = mma_parts<3, NP>(xa, kb[t], dr[m][t]);
-            }
-          }
-          if (s == 1 || m < 2) {
-#pragma unroll
-            for (int p = 0; p < 3; ++p) xa[p] = fr[((kTri + tri_upper(m, s)) * 3 + p) * 64 + lane];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) dw[m][t] = mma_parts<3, NP>(xa, which ? kb[t] : qb[t], dw[m][t]);
+          for (int t = 0; t < NT; ++t) {
+            dq[m][t] = mma_parts<3, NP>(xa, kb[s][t], dq[m][t]);
+            dr[m][t] = mma_parts<3, NP>(ya, kb[s][t], dr[m][t]);
           }
         }
-      }
-      __syncthreads();
-    }
-    // dG, 16 tokens of this wave's columns at a time
+        if (s == 1 || mt < 2) {
+          const int f = tri_upper(mt, s) * 3 * 64 + lane;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      float x[4];
+          for (int p = 0; p < 3; ++p) {
+            xa[p] = *reinterpret_cast<const uint4*>(&nf[1][f + p * 64]);
+            ya[p] = *reinterpret_cast<const uint4*>(&mf[1][f + p * 64]);
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            dw[m][t] = mma_parts<3, NP>(xa, qb[s][t], dw[m][t]);
+            dw[m][t] = mma_parts<3, NP>(ya, kb[s][t], dw[m][t]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    // dG over this wave's columns
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+      float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int half = MR == 4 ? m >> 1 : m0 >> 1;
+          x[r] += element(half ? qb[1][t] : qb[0][t], 4 * (m & 1) + r) * dq[m][t][r] +
+                  element(half ? kb[1][t] : kb[0][t], 4 * (m & 1) + r) * (dr[m][t][r] - dw[m][t][r]);
+          dqs[m][t][r] += dq[m][t][r];
+          dks[m][t][r] += dr[m][t][r] + dw[m][t][r];
+        }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int i = 16 * m + 4 * g + r;
-        x[r] = 0.f;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int col = 16 * (wave * NT + t) + c;
-          if (i < rows && col < a.K)
-            x[r] += to_f32(qp[i * a.q_s[1] + col]) * dq[m][t][r] +
-                    to_f32(kp[i * a.k_s[1] + col]) * (dr[m][t][r] - dw[m][t][r]);
-        }
-      }
-#pragma unroll
-      for (int off = 8; off >= 1; off >>= 1)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] += __shfl_xor(x[r], off, 64);
-      if (c == 0) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) dg_part[wave][16 * m + 4 * g + r] = x[r];
-      }
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        dqs[m][t] += dq[m][t];
-        dks[m][t] += dr[m][t] + dw[m][t];
+        x[r] = row16_sum(x[r]);
+        if (c == 0) dg_part[cw][16 * (m0 + m) + 4 * g + r] = x[r];
       }
     }
     __syncthreads();
     if (wave == 0) {
-      double s = (double)((dg_part[0][lane] + dg_part[1][lane]) + (dg_part[2][lane] + dg_part[3][lane]));
-      if (lane == 63) s += (double)((dots[0] + dots[1]) + (dots[2] + dots[3]));
+      double s = 0.;
+#pragma unroll
+      for (int w = 0; w < CW; ++w) s += (double)dg_part[w][lane];
+#pragma unroll
+      for (int w = 0; w < W; ++w) s += lane == 63 ? (double)dots[w] : 0.;
 #pragma unroll
       for (int off = 1; off < 64; off <<= 1) {
         const double t = __shfl_down(s, off, 64);
@@ -615,18 +677,20 @@ __global__ __launch_bounds__(256) void gdr_grads_kernel(GdrArgs a) {
       }
       if (lane < rows) store_param(a.dg, a.g_dtype, (token + lane) * a.Hv + h, (float)s);
     }
-    // (the next head's first barrier comes before anything that is read here is written)
+    // (the next head's gs, grown .. are wave 0's to write and read after its first barrier; what else is
+    // written then has no readers left, or comes after two barriers)
   }
+  const int c = tid & 15, g = (tid & 63) >> 4;
 #pragma unroll
-  for (int m = 0; m < 4; ++m)
+  for (int m = 0; m < MR; ++m)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * m + 4 * g + r;
+      const int i = 16 * (m0 + m) + 4 * g + r;
       if (i >= rows) continue;
       const int64_t o = ((token + i) * a.Hk + hk) * (int64_t)a.K;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const int col = 16 * (wave * NT + t) + c;
+        const int col = 16 * (cw * NT + t) + c;
         if (col < a.K) {
           static_cast<T*>(a.dq)[o + col] = from_f32<T>(dqs[m][t][r]);
           static_cast<T*>(a.dk)[o + col] = from_f32<T>(dks[m][t][r]);
@@ -643,7 +707,7 @@ int launch(const GdrArgs& a, hipStream_t s) {
   else hipLaunchKernelGGL((gdr_bwd_chain_kernel<T, KP, false>), dim3((unsigned)grid), dim3(512), 0, s, a);
   if (int rc = check_launch("gdr_bwd_chain_kernel")) return rc;
   if (a.T == 0) return ATK_OK;
-  hipLaunchKernelGGL((gdr_grads_kernel<T, KP>), dim3((unsigned)a.slots, (unsigned)a.Hk), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((gdr_grads_kernel<T, KP>), dim3((unsigned)a.slots, (unsigned)a.Hk), dim3(512), 0, s, a);
   return check_launch("gdr_grads_kernel");
 }
 template <typename T>
