@@ -39,7 +39,8 @@ struct GdrArgs {
   float* row;            // [Hv][slot][3][64]: exp(G_i), exp(G_63 - G_i), beta_i
   // the backward's: fragments of Q^T, (1 + diag(beta) W)^-T and lower(Q K^T * D)^T; each chunk's G / ln 2
   // as two floats; the state and the errors that the forward chain had at each chunk, and the gradients of
-  // the state after it and of U: [Hv][slot][KP or 64][VP] fp32, VP = V padded to 32
+  // the state after it and of U: [Hv][slot] matrices
+  // of KP or 64 rows and VP columns in gdr_kept's order, fp32, VP = V padded to 32
   uint4* qtf; uint4* ttf; uint4* ptf;
   float2* gsum;
   float* sc; float* ec; float* dsc; float* drc;
@@ -120,6 +121,13 @@ __device__ __forceinline__ f32x4 mma_parts(const uint4 (&a)[NA], const uint4 (&b
 // are taken in the order that gives a lane its own: element i of lane group g is row gdr_at(g, i) of two
 // row tiles, and every A that meets such a B has its columns in that order too.
 __device__ __forceinline__ constexpr int gdr_at(int g, int i) { return i < 4 ? 4 * g + i : 12 + 4 * g + i; }
+
+// Where a kept matrix has element r of the accumulators of row tile 0 and value tile `tile`, from its
+// start; row tile t is 512 t further.  Read, 32 columns of a row tile are one operand in whole lanes: 8
+// columns of a row each.
+__device__ __forceinline__ int gdr_kept(int tile, int row_tiles, int c, int g) {
+  return (tile >> 1) * row_tiles * 512 + (16 * ((tile & 1) * 2 + (c >> 3)) + 4 * g) * 8 + (c & 7);
+}
 
 // v[0..N) as NP parts of N bf16 each
 template <int NP, int N, typename P>

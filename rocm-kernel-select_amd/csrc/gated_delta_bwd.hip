@@ -50,8 +50,8 @@ __global__ __launch_bounds__(512) void gdr_bwd_chain_kernel(GdrArgs a) {
     const bool two = wave < 2;  // column halves of this wave's rows of T^T
     const uint4* __restrict__ tf = a.ttf + (h * a.slots + end) * (int64_t)(kTri * 3 * 64) + tri_upper(wave, wave >> 1) * 3 * 64;
     const float* __restrict__ row = a.row + (h * a.slots + end) * 192;
-    float* __restrict__ dsc = a.dsc + (h * a.slots + end) * (int64_t)KP * a.VP + col;
-    float* __restrict__ drc = a.drc + (h * a.slots + end) * (int64_t)64 * a.VP + (16 * wave + 4 * g) * (int64_t)a.VP + col;
+    float* __restrict__ dsc = a.dsc + (h * a.slots + end) * (int64_t)KP * a.VP + gdr_kept(tile, KP / 16, c, g);
+    float* __restrict__ drc = a.drc + (h * a.slots + end) * (int64_t)64 * a.VP + gdr_kept(tile, 4, c, g) + wave * 512;
     f32x4 S[MT];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(512) void gdr_bwd_chain_kernel(GdrArgs a) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) dsc[(int64_t)(16 * (wave * MT + m) + 4 * g + r) * a.VP] = S[m][r];
+        for (int r = 0; r < 4; ++r) dsc[(wave * MT + m) * 512 + r * 8] = S[m][r];
       dsc -= (int64_t)KP * a.VP;
       f32x4 y[4] = {zero, zero, zero, zero};
 #pragma unroll
@@ -179,7 +179,7 @@ __global__ __launch_bounds__(512) void gdr_bwd_chain_kernel(GdrArgs a) {
         for (int p = 0; p < 3; ++p) rl[wave >> 1][p][lane][wave & 1] = __builtin_bit_cast(uint2, parts[p]);
       }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) drc[r * (int64_t)a.VP] = dr[r];
+      for (int r = 0; r < 4; ++r) drc[r * 8] = dr[r];
       drc -= (int64_t)64 * a.VP;
       load_t();
       __syncthreads();
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
   for (int m = 0; m < MR; ++m)
 #pragma unroll
     for (int t = 0; t < NT; ++t) dqs[m][t] = dks[m][t] = zero;
-  // one unit of 16 tokens a wave and turn: 0..3 dO and dR, 4..7 e
+  // one unit of 16 tokens a wave and turn: 0..3 dR (and dV), 4..7 e and dO
   constexpr int UNITS = 8 / W;
   for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
     // (opaque to the compiler, which would keep the addresses of every access in registers for the next head)
@@ -403,10 +403,10 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
     asm volatile("" : "+v"(lane));
     const int c = lane & 15, g = lane >> 4;
     const int64_t hs = h * a.slots + slot;
-    const float* __restrict__ sc = a.sc + hs * KP * a.VP + (16 * cw * NT + c) * (int64_t)a.VP + 8 * g;
-    const float* __restrict__ dsc = a.dsc + hs * KP * a.VP + (16 * cw * NT + c) * (int64_t)a.VP + 8 * g;
-    const float* __restrict__ ec = a.ec + hs * 64 * a.VP;
-    const float* __restrict__ drc = a.drc + hs * 64 * a.VP;
+    const float* __restrict__ sc = a.sc + hs * KP * a.VP + cw * NT * 512 + 8 * lane;
+    const float* __restrict__ dsc = a.dsc + hs * KP * a.VP + cw * NT * 512 + 8 * lane;
+    const float* __restrict__ ec = a.ec + hs * 64 * a.VP + 8 * lane;
+    const float* __restrict__ drc = a.drc + hs * 64 * a.VP + 8 * lane;
     f32x4 rs[NT][2], rd[NT][2], ru[UNITS][2];
     T ro[8];
     auto load = [&](int v0) {
@@ -414,13 +414,13 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-          rs[t][z] = *reinterpret_cast<const f32x4*>(sc + 16 * t * (int64_t)a.VP + v0 + 4 * z);
-          rd[t][z] = *reinterpret_cast<const f32x4*>(dsc + 16 * t * (int64_t)a.VP + v0 + 4 * z);
+          rs[t][z] = *reinterpret_cast<const f32x4*>(sc + v0 * KP + t * 512 + 4 * z);
+          rd[t][z] = *reinterpret_cast<const f32x4*>(dsc + v0 * KP + t * 512 + 4 * z);
         }
 #pragma unroll
       for (int u = 0; u < UNITS; ++u) {
-        const int unit = wave + W * u, i = 16 * (unit & 3) + c;
-        const float* __restrict__ p = (unit < 4 ? drc : ec) + (int64_t)i * a.VP + v0 + 8 * g;
+        const int unit = wave + W * u;
+        const float* __restrict__ p = (unit < 4 ? drc : ec) + v0 * 64 + (unit & 3) * 512;
         ru[u][0] = *reinterpret_cast<const f32x4*>(p);
         ru[u][1] = *reinterpret_cast<const f32x4*>(p + 4);
       }
@@ -459,16 +459,9 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
         split_parts<3, 8>(x, parts);
 #pragma unroll
         for (int p = 0; p < 3; ++p) st[(m * UNIT + NP + (unit < 4 ? 0 : 3) + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
-        if (unit < 4) {  // dO too, and dV = beta dR
-          float y[8];
-          bf16x8 exact[NP];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) y[j] = i < rows && col + j < a.V ? to_f32(ro[j]) : 0.f;
-          split_parts<NP, 8>(y, exact);
-#pragma unroll
-          for (int p = 0; p < NP; ++p) st[(m * UNIT + p) * 64 + lane] = __builtin_bit_cast(uint4, exact[p]);
+        if (unit < 4) {  // dV = beta dR
           if (i < rows) {
-            const float b = a.row[hs * 192 + 128 + i];
+            const float b = beta[i];
             T* __restrict__ d = static_cast<T*>(a.dv) + ((token + i) * a.Hv + h) * (int64_t)a.V + col;
             T z[8];
 #pragma unroll
@@ -481,6 +474,14 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
                 if (col + j < a.V) d[j] = z[j];
             }
           }
+        } else {
+          float y[8];
+          bf16x8 exact[NP];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[j] = i < rows && col + j < a.V ? to_f32(ro[j]) : 0.f;
+          split_parts<NP, 8>(y, exact);
+#pragma unroll
+          for (int p = 0; p < NP; ++p) st[(m * UNIT + p) * 64 + lane] = __builtin_bit_cast(uint4, exact[p]);
         }
       }
       uint4 sb[NT][3], db[NT][3];
@@ -515,11 +516,15 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
           ea[p] = from[(NP + 3 + p) * 64];
         }
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          dq[m][t] = mma_parts<NP, 3>(da, sb[t], dq[m][t]);
-          dr[m][t] = mma_parts<3, 3>(ra, sb[t], dr[m][t]);
-          dw[m][t] = mma_parts<3, 3>(ea, db[t], dw[m][t]);
-        }
+        for (int t = 0; t < NT; ++t)  // the three in turn, so that none waits for its own last product
+#pragma unroll
+          for (int z = 2; z >= 0; --z)
+#pragma unroll
+            for (int p = 0; p <= z; ++p) {
+              dr[m][t] = mma(ra[p], sb[t][z - p], dr[m][t]);
+              if (p < NP) dq[m][t] = mma(da[p], sb[t][z - p], dq[m][t]);
+              dw[m][t] = mma(ea[p], db[t][z - p], dw[m][t]);
+            }
         __builtin_amdgcn_sched_barrier(0);  // (all tiles' operands at once would not fit the registers)
       }
 #pragma unroll
@@ -536,13 +541,17 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
             ra[p] = st[(i * UNIT + NP + p) * 64 + lane];
             ea[p] = st[(j * UNIT + NP + 3 + p) * 64 + lane];
           }
-          if (u < 10) {
-            ne[x] = mma_parts<NP, 3>(da, ea, ne[x]);
-            me[x] = mma_parts<3, 3>(ra, ea, me[x]);
-          } else {
-            ne[x] = mma_parts<3, NP>(ea, da, ne[x]);
-            me[x] = mma_parts<3, 3>(ea, ra, me[x]);
-          }
+#pragma unroll
+          for (int z = 2; z >= 0; --z)
+#pragma unroll
+            for (int p = 0; p <= z; ++p)
+              if (u < 10) {
+                me[x] = mma(ra[p], ea[z - p], me[x]);
+                if (p < NP) ne[x] = mma(da[p], ea[z - p], ne[x]);
+              } else {
+                me[x] = mma(ea[z - p], ra[p], me[x]);
+                if (p < NP) ne[x] = mma(ea[z - p], da[p], ne[x]);
+              }
         }
         __builtin_amdgcn_sched_barrier(0);
       }

@@ -438,11 +438,11 @@ __global__ __launch_bounds__(512) void gdr_chain_kernel(GdrArgs a) {
       ktf += more ? kstep : 0;
       tf += more ? tstep : 0;
       if constexpr (KEEP) {
-        float* __restrict__ sc = a.sc + (h * a.slots + seq.slot + ch) * (int64_t)KP * a.VP;
+        float* __restrict__ sc = a.sc + (h * a.slots + seq.slot + ch) * (int64_t)KP * a.VP + gdr_kept(tile, KP / 16, c, g);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) sc[(int64_t)(16 * (wave * MT + m) + 4 * g + r) * a.VP + col] = S[m][r];
+          for (int r = 0; r < 4; ++r) sc[(wave * MT + m) * 512 + r * 8] = S[m][r];
       }
       f32x4 y[4] = {zero, zero, zero, zero};
 #pragma unroll
@@ -518,9 +518,9 @@ __global__ __launch_bounds__(512) void gdr_chain_kernel(GdrArgs a) {
 #pragma unroll
         for (int p = 0; p < 3; ++p) el[wave >> 1][p][lane][wave & 1] = __builtin_bit_cast(uint2, parts[p]);
         if constexpr (KEEP) {
-          float* __restrict__ ec = a.ec + (h * a.slots + seq.slot + ch) * (int64_t)64 * a.VP;
+          float* __restrict__ ec = a.ec + (h * a.slots + seq.slot + ch) * (int64_t)64 * a.VP + gdr_kept(tile, 4, c, g);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) ec[(int64_t)(16 * wave + 4 * g + r) * a.VP + col] = e[r];
+          for (int r = 0; r < 4; ++r) ec[wave * 512 + r * 8] = e[r];
         } else {
           ul[wave][lane] = beta * e;
         }
