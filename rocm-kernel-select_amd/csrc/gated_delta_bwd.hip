@@ -357,15 +357,16 @@ __device__ __forceinline__ float row16_sum(float v) {
 // eight waves has 16 NT key columns of dq and dk, for all 64 tokens or (64 columns) for 32.  The value columns are walked 32 at a
 // time: the waves bring dO, dR and e of all tokens into LDS as fragments (the next 32 columns on their
 // way meanwhile), and every wave multiplies them with its own rows of S and dS', which it splits
-// itself.  dO e^T and dR e^T, whose 16 x 16 tiles on and below the diagonal the waves share out, are
-// made both ways round: a result's layout is that of the transpose's rows, so N, M and their
-// transposes go from the accumulators straight into LDS as fragments.  K^T's and Q^T's fragments hold
-// for each lane the elements that its accumulators have, so the row products of dG need no more loads.
-template <typename T, int KP>
+// itself.  The 16 x 16 tiles of dO e^T and dR e^T on and below the diagonal are shared out among the
+// waves; a result's layout is that of the transpose's rows, so N and M leave the accumulators as
+// fragments of their transposes, and, element by element, as their own.  K^T's and Q^T's fragments
+// hold for each lane the elements that its accumulators have, so the row products of dG need no more
+// loads.  V8: value columns come in eights, so a lane's are all there or all not.
+template <typename T, int KP, bool V8>
 __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
   constexpr int NP = kParts<T>, KS = KP / 32, W = 8, NT = KP > 128 ? KP / 128 : 1;
   constexpr int CW = KP / 16 / NT, MR = 4 * CW / W;  // waves side by side over the key columns; row tiles of each
-  constexpr int TILES = (20 + W - 1) / W;  // of the twenty, this wave's: wave, wave + W, ..
+  constexpr int TILES = 2;                 // of the ten, this wave's: wave, and wave + 8 for the first two
   constexpr int UNIT = NP + 6;             // fragments of 16 tokens: dO, dR, e
   __shared__ uint4 st[4 * UNIT * 64];
   __shared__ uint2 nf[2][kTri * 3 * 64][2], mf[2][kTri * 3 * 64][2];  // N and M, their transposes
@@ -395,6 +396,12 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
   for (int m = 0; m < MR; ++m)
 #pragma unroll
     for (int t = 0; t < NT; ++t) dqs[m][t] = dks[m][t] = zero;
+  int it[TILES], jt[TILES];
+#pragma unroll
+  for (int x = 0; x < TILES; ++x) {
+    tri_tile(wave + W * x < 10 ? wave + W * x : 0, &it[x], &jt[x]);
+    if (wave + W * x >= 10) it[x] = -1;
+  }
   // one unit of 16 tokens a wave and turn: 0..3 dR (and dV), 4..7 e and dO
   constexpr int UNITS = 8 / W;
   for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
@@ -426,8 +433,8 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
       }
       const int i = 16 * (wave & 3) + c, col = v0 + 8 * g;
       const T* __restrict__ p = static_cast<const T*>(a.dout) + ((token + (i < rows ? i : 0)) * a.Hv + h) * (int64_t)a.V;
-      if (col + 8 <= a.V) {
-        __builtin_memcpy(ro, p + col, 8 * sizeof(T));
+      if constexpr (V8) {
+        __builtin_memcpy(ro, p + (col < a.V ? col : 0), 8 * sizeof(T));
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) ro[j] = p[col + j < a.V ? col + j : 0];
@@ -466,8 +473,8 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
             T z[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) z[j] = from_f32<T>(b * x[j]);
-            if (col + 8 <= a.V) {
-              __builtin_memcpy(d, z, 8 * sizeof(T));
+            if constexpr (V8) {
+              if (col < a.V) __builtin_memcpy(d, z, 8 * sizeof(T));
             } else {
 #pragma unroll
               for (int j = 0; j < 8; ++j)
@@ -504,6 +511,11 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
       }
       load(v0 + 32 < a.VP ? v0 + 32 : v0);
       __syncthreads();
+      uint4 et[TILES][3];  // e of this wave's tiles' columns
+#pragma unroll
+      for (int x = 0; x < TILES; ++x)
+#pragma unroll
+        for (int p = 0; p < 3; ++p) et[x][p] = st[(jt[x] * UNIT + NP + 3 + p) * 64 + lane];
 #pragma unroll
       for (int m = 0; m < MR; ++m) {
         uint4 da[NP], ra[3], ea[3];
@@ -525,62 +537,73 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
               if (p < NP) dq[m][t] = mma(da[p], sb[t][z - p], dq[m][t]);
               dw[m][t] = mma(ea[p], db[t][z - p], dw[m][t]);
             }
+        if constexpr (MR == 4) {
+#pragma unroll
+          for (int x = 0; x < TILES; ++x)
+            if (it[x] == m)
+#pragma unroll
+              for (int z = 2; z >= 0; --z)
+#pragma unroll
+                for (int p = 0; p <= z; ++p) {
+                  me[x] = mma(ra[p], et[x][z - p], me[x]);
+                  if (p < NP) ne[x] = mma(da[p], et[x][z - p], ne[x]);
+                }
+        }
         __builtin_amdgcn_sched_barrier(0);  // (all tiles' operands at once would not fit the registers)
       }
+      if constexpr (MR < 4) {
 #pragma unroll
-      for (int x = 0; x < TILES; ++x) {
-        const int u = wave + W * x;
-        if (u < 20) {
-          int i, j;
-          tri_tile(u % 10, &i, &j);
-          uint4 da[NP], ra[3], ea[3];
+        for (int x = 0; x < TILES; ++x)
+          if (it[x] >= 0) {
+            uint4 da[NP], ra[3];
+            const uint4* from = st + it[x] * UNIT * 64 + lane;
 #pragma unroll
-          for (int p = 0; p < NP; ++p) da[p] = st[(i * UNIT + p) * 64 + lane];
+            for (int p = 0; p < NP; ++p) da[p] = from[p * 64];
 #pragma unroll
-          for (int p = 0; p < 3; ++p) {
-            ra[p] = st[(i * UNIT + NP + p) * 64 + lane];
-            ea[p] = st[(j * UNIT + NP + 3 + p) * 64 + lane];
-          }
+            for (int p = 0; p < 3; ++p) ra[p] = from[(NP + p) * 64];
 #pragma unroll
-          for (int z = 2; z >= 0; --z)
+            for (int z = 2; z >= 0; --z)
 #pragma unroll
-            for (int p = 0; p <= z; ++p)
-              if (u < 10) {
-                me[x] = mma(ra[p], ea[z - p], me[x]);
-                if (p < NP) ne[x] = mma(da[p], ea[z - p], ne[x]);
-              } else {
-                me[x] = mma(ea[z - p], ra[p], me[x]);
-                if (p < NP) ne[x] = mma(ea[z - p], da[p], ne[x]);
+              for (int p = 0; p <= z; ++p) {
+                me[x] = mma(ra[p], et[x][z - p], me[x]);
+                if (p < NP) ne[x] = mma(da[p], et[x][z - p], ne[x]);
               }
-        }
-        __builtin_amdgcn_sched_barrier(0);
+          }
       }
     }
-    // N and M: u < 10 has rows i and columns j, a fragment of the transposes; the others rows j
+    // N and M, row i and column j
 #pragma unroll
     for (int x = 0; x < TILES; ++x) {
-      const int u = wave + W * x;
-      if (u < 20) {
-        int it, jt;
-        tri_tile(u % 10, &it, &jt);
-        const bool tall = u < 10;
+      if (it[x] >= 0) {
+        const int j = 16 * jt[x] + c;
+        const float2 gj = gs[j];
+        const float bj = beta[j];
         float nv[4], mv[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int i = tall ? 16 * it + 4 * g + r : 16 * it + c, j = tall ? 16 * jt + c : 16 * jt + 4 * g + r;
-          const float d = j <= i ? beta[j] * gdr_decay(gs[i], gs[j]) : 0.f;
+          const int i = 16 * it[x] + 4 * g + r;
+          const float d = j <= i ? bj * gdr_decay(gs[i], gj) : 0.f;
           nv[r] = j <= i ? a.scale * d * ne[x][r] : 0.f;
           mv[r] = j < i ? -beta[i] * d * me[x][r] : 0.f;
-          if (tall && i == j && i < rows) store_param(a.dbeta, a.b_dtype, (token + i) * a.Hv + h, me[x][r]);
+          if (it[x] == jt[x] && i == j && i < rows) store_param(a.dbeta, a.b_dtype, (token + i) * a.Hv + h, me[x][r]);
         }
-        const int f = tall ? tri_upper(jt, it >> 1) : tri_lower(it, jt >> 1), half = tall ? it & 1 : jt & 1;
+        const int up = tri_upper(jt[x], it[x] >> 1) * 3 * 64 + lane, low = tri_lower(it[x], jt[x] >> 1) * 3 * 64;
+        const int to = 4 * g + 16 * (c >> 2), at = (c & 3) + 4 * (jt[x] & 1);  // of element r = 0 among N's own
         bf16x4 parts[3];
         split_parts<3, 4>(nv, parts);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) nf[tall][(f * 3 + p) * 64 + lane][half] = __builtin_bit_cast(uint2, parts[p]);
+        for (int p = 0; p < 3; ++p) {
+          nf[1][up + p * 64][it[x] & 1] = __builtin_bit_cast(uint2, parts[p]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) reinterpret_cast<__bf16*>(&nf[0][low + p * 64 + to + r])[at] = parts[p][r];
+        }
         split_parts<3, 4>(mv, parts);
 #pragma unroll
-        for (int p = 0; p < 3; ++p) mf[tall][(f * 3 + p) * 64 + lane][half] = __builtin_bit_cast(uint2, parts[p]);
+        for (int p = 0; p < 3; ++p) {
+          mf[1][up + p * 64][it[x] & 1] = __builtin_bit_cast(uint2, parts[p]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) reinterpret_cast<__bf16*>(&mf[0][low + p * 64 + to + r])[at] = parts[p][r];
+        }
       }
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -716,7 +739,9 @@ int launch(const GdrArgs& a, hipStream_t s) {
   else hipLaunchKernelGGL((gdr_bwd_chain_kernel<T, KP, false>), dim3((unsigned)grid), dim3(512), 0, s, a);
   if (int rc = check_launch("gdr_bwd_chain_kernel")) return rc;
   if (a.T == 0) return ATK_OK;
-  hipLaunchKernelGGL((gdr_grads_kernel<T, KP>), dim3((unsigned)a.slots, (unsigned)a.Hk), dim3(512), 0, s, a);
+  const dim3 g((unsigned)a.slots, (unsigned)a.Hk);
+  if (a.V % 8 == 0) hipLaunchKernelGGL((gdr_grads_kernel<T, KP, true>), g, dim3(512), 0, s, a);
+  else hipLaunchKernelGGL((gdr_grads_kernel<T, KP, false>), g, dim3(512), 0, s, a);
   return check_launch("gdr_grads_kernel");
 }
 template <typename T>
