@@ -1765,8 +1765,7 @@ def gated_delta_backward(q, k, v, g, beta, scale: float, initial_state, cu_seqle
     q, k, v, g, beta, initial_state, cu_seqlens, n = _delta_checked(q, k, v, g, beta, initial_state, cu_seqlens)
     if dout.shape != v.shape or dout.dtype != v.dtype or dout.device != v.device:
         raise RuntimeError("gated_delta_rule backward: the gradient must match the output")
-    # tokens that no packed sequence has get a gradient of zero
-    make = torch.empty if cu_seqlens is None else torch.zeros
+    make = torch.empty if n else torch.zeros
     grads = [make(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, g, beta)]
     dstate = None
     if want_dstate:

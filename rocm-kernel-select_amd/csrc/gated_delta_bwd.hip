@@ -21,6 +21,12 @@
 namespace atk {
 namespace {
 
+__device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float v) {
+  if (dtype == ATK_F32) static_cast<float*>(p)[i] = v;
+  else if (dtype == ATK_F16) static_cast<_Float16*>(p)[i] = from_f32<_Float16>(v);
+  else static_cast<__bf16*>(p)[i] = from_f32<__bf16>(v);
+}
+
 // The chain of dS', built as the forward's: four waves pass the state's gradient on, 16 value columns
 // of it; four more make what needs dO alone, a chunk ahead: scale P^T dO and Q^T (scale exp(G) dO).
 // FULL as there.
@@ -330,13 +336,27 @@ __global__ __launch_bounds__(512) void gdr_bwd_chain_kernel(GdrArgs a) {
       load_q();
       __syncthreads();
     }
+    // tokens of a packed row before its first sequence and after its last have gradients of zero
+    if (a.cu && (n == 0 || n == a.n - 1)) {
+      const int64_t from[2] = {n == 0 ? 0 : a.T, n == a.n - 1 ? seq.begin + seq.len : a.T};
+      const int64_t to[2] = {n == 0 ? seq.begin : a.T, a.T};
+      for (int z = 0; z < 2; ++z)
+        for (int64_t i = from[z] + 4 * m + g; i < to[z]; i += 16) {
+          const int64_t at = i * a.Hv + h;
+          if (col < a.V) static_cast<T*>(a.dv)[at * a.V + col] = from_f32<T>(0.f);
+          if (tile > 0) continue;
+          if (c == 0) {
+            store_param(a.dg, a.g_dtype, at, 0.f);
+            store_param(a.dbeta, a.b_dtype, at, 0.f);
+          }
+          if (h % a.group == 0)
+            for (int d = c; d < a.K; d += 16) {
+              static_cast<T*>(a.dq)[(i * a.Hk + hk) * a.K + d] = from_f32<T>(0.f);
+              static_cast<T*>(a.dk)[(i * a.Hk + hk) * a.K + d] = from_f32<T>(0.f);
+            }
+        }
+    }
   }
-}
-
-__device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float v) {
-  if (dtype == ATK_F32) static_cast<float*>(p)[i] = v;
-  else if (dtype == ATK_F16) static_cast<_Float16*>(p)[i] = from_f32<_Float16>(v);
-  else static_cast<__bf16*>(p)[i] = from_f32<__bf16>(v);
 }
 
 // (row, column) tile t of the ten of a lower triangle of 16 x 16 tiles

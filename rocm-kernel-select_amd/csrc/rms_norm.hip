@@ -298,21 +298,28 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwdAr
   for (int j = 0; j < VPT; ++j) store_cols<float, V>(p, (t + j * TPR) * V, a.N, dw[j]);
 }
 
-// dw[c] = sum of part[0..P)[c], rounded once to the weight's type: 16 columns a workgroup, 16
-// threads to a column, joined in a fixed order
+// dw[c] = sum of part[0..P)[c], rounded once to the weight's type: 64 columns a workgroup, 16 threads
+// to 4 columns, joined in a fixed order
 template <typename WT>
 __global__ __launch_bounds__(256) void rms_dw_kernel(const float* __restrict__ part, WT* __restrict__ dw, int P, int N) {
-  __shared__ float s[16][17];
-  const int c = blockIdx.x * 16 + threadIdx.x % 16, k = threadIdx.x / 16;
-  float v = 0.f;
-  if (c < N)
-    for (int p = k; p < P; p += 16) v += part[(int64_t)p * N + c];
-  s[k][threadIdx.x % 16] = v;
-  __syncthreads();
-  if (k == 0 && c < N) {
+  __shared__ float s[16][65];
+  const int c = blockIdx.x * 64 + threadIdx.x % 16 * 4, k = threadIdx.x / 16;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int p = k; p < P; p += 16) {
+    float e[4];
+    load_cols<float, 4>(part + (int64_t)p * N, c, N, e);
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += s[i][threadIdx.x];
-    dw[c] = from_f32<WT>(v);
+    for (int i = 0; i < 4; ++i) v[i] += e[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[k][threadIdx.x % 16 * 4 + i] = v[i];
+  __syncthreads();
+  if (threadIdx.x < 64 && blockIdx.x * 64 + threadIdx.x < N) {
+    float t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += s[i][threadIdx.x];
+    dw[blockIdx.x * 64 + threadIdx.x] = from_f32<WT>(t);
   }
 }
 
@@ -320,9 +327,11 @@ __global__ __launch_bounds__(256) void rms_dw_kernel(const float* __restrict__ p
 struct RmsShape {
   int tpr, vpt;
 };
-RmsShape rms_shape(int64_t nv) {
+// Few rows leave most of the chip without one: there a row of over 64 vectors is a workgroup's.
+RmsShape rms_shape(int64_t nv, int64_t rows) {
   if (nv <= 16) return {16, 1};
   if (nv <= 64) return {64, 1};
+  if (nv <= 256 && rows <= 1024) return {256, 1};
   if (nv <= 128) return {64, 2};
   if (nv <= 256) return {64, 4};
   if (nv <= 512) return {256, 2};
@@ -331,7 +340,7 @@ RmsShape rms_shape(int64_t nv) {
   return {1024, 8};
 }
 
-#define ATK_RMS_SHAPES(X) X(16, 1) X(64, 1) X(64, 2) X(64, 4) X(256, 2) X(256, 4) X(1024, 4) X(1024, 8)
+#define ATK_RMS_SHAPES(X) X(16, 1) X(64, 1) X(64, 2) X(64, 4) X(256, 1) X(256, 2) X(256, 4) X(1024, 4) X(1024, 8)
 
 template <typename T, int Q>
 int launch_fwd(const RmsArgs& a, RmsShape sh, hipStream_t s) {
@@ -383,7 +392,7 @@ int check_rows(const char* what, int64_t M, int64_t N, int dtype, int w_dtype, b
 int bwd_grid(int64_t M, int tpr) {
   const int rpb = tpr < 256 ? 256 / tpr : 1;
   const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  const int64_t most = (int64_t)cus * (tpr > 256 ? 1 : 4), need = (M + rpb - 1) / rpb;
+  const int64_t most = (int64_t)cus * (tpr > 256 ? 1 : 2), need = (M + rpb - 1) / rpb;
   return (int)(need < most ? need : most);
 }
 
@@ -412,7 +421,7 @@ extern "C" int atk_rms_norm_fwd(const atk_rms_norm_args* p) {
   a.x = p->x; a.r = p->residual; a.w = p->weight; a.y = p->y; a.h = p->h; a.rstd = p->rstd; a.scales = p->scales;
   a.M = M; a.x_stride = p->x_stride; a.r_stride = p->residual_stride;
   a.N = (int)N; a.group = group; a.w_f32 = p->w_dtype == ATK_F32; a.eps = p->eps;
-  const RmsShape sh = rms_shape((N + vec - 1) / vec);
+  const RmsShape sh = rms_shape((N + vec - 1) / vec, M);
   hipStream_t s = reinterpret_cast<hipStream_t>(p->stream);
   if (quant == ATK_QUANT_FP8) return launch_fwd_typed<kQFp8>(a, dtype, sh, s);
   if (quant == ATK_QUANT_INT8) return launch_fwd_typed<kQInt8>(a, dtype, sh, s);
@@ -423,7 +432,7 @@ extern "C" size_t atk_rms_norm_bwd_workspace_bytes(int64_t M, int64_t N, int dty
   using namespace atk;
   if (check_rows("rms_norm backward", M, N, dtype, dtype, false) || M == 0 || N == 0) return 0;
   const int vec = 16 / (int)dtype_size(dtype);
-  return (size_t)bwd_grid(M, rms_shape((N + vec - 1) / vec).tpr) * (size_t)N * sizeof(float);
+  return (size_t)bwd_grid(M, rms_shape((N + vec - 1) / vec, M).tpr) * (size_t)N * sizeof(float);
 }
 
 extern "C" int atk_rms_norm_bwd(const void* h, const void* dy, const void* dh, const void* weight, const float* rstd,
@@ -437,7 +446,7 @@ extern "C" int atk_rms_norm_bwd(const void* h, const void* dy, const void* dh, c
   if (M > 1 && (h_stride < N || dy_stride < N || (dh && dh_stride < N)))
     return fail(ATK_EINVAL, "rms_norm backward: rows overlap");
   const int vec = 16 / (int)dtype_size(dtype);
-  const RmsShape sh = rms_shape((N + vec - 1) / vec);
+  const RmsShape sh = rms_shape((N + vec - 1) / vec, M);
   const int grid = bwd_grid(M, sh.tpr);
   if (dw && (!workspace || workspace_bytes < (size_t)grid * (size_t)N * sizeof(float)))
     return fail(ATK_EINVAL, "rms_norm backward: workspace too small");
@@ -450,7 +459,7 @@ extern "C" int atk_rms_norm_bwd(const void* h, const void* dy, const void* dh, c
   int rc = dtype == ATK_F32 ? launch_bwd<float>(a, sh, grid, s)
            : dtype == ATK_F16 ? launch_bwd<_Float16>(a, sh, grid, s) : launch_bwd<__bf16>(a, sh, grid, s);
   if (rc || !dw) return rc;
-  const dim3 g((unsigned)((N + 15) / 16));
+  const dim3 g((unsigned)((N + 63) / 64));
   if (w_dtype == ATK_F32)
     hipLaunchKernelGGL((rms_dw_kernel<float>), g, dim3(256), 0, s, a.dw_part, static_cast<float*>(dw), grid, (int)N);
   else if (w_dtype == ATK_F16)

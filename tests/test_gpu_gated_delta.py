@@ -48,7 +48,8 @@ def make(lead, hk, hv, dk, dv, dtype, dev, seed=0, gdtype=torch.float32, bdtype=
 @gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,hk,hv,dk,dv", [(1, 1, 1, 1, 1), (3, 2, 4, 128, 128), (2, 1, 3, 64, 100), (2, 2, 2, 130, 36),
-                                           (5, 1, 2, 256, 256), (2, 3, 3, 17, 33), (1, 2, 2, 100, 7), (33, 1, 4, 32, 64)])
+                                           (5, 1, 2, 256, 256), (2, 3, 3, 17, 33), (1, 2, 2, 100, 7), (33, 1, 4, 32, 64),
+                                           (64, 1, 4, 128, 100), (86, 1, 3, 200, 132)])
 def test_update(dev, n, hk, hv, dk, dv, dtype):
     import amd_tuned_torch as P
     args = make((n,), hk, hv, dk, dv, dtype, dev, seed=n + dk)
