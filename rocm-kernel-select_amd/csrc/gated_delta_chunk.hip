@@ -72,11 +72,11 @@ __device__ __forceinline__ void substitute_rows(const float (&a)[16], float (&x)
   }
 }
 
-// T = (1 + A)^-1 for the strictly lower A (LDS, 64 x LD; read below the diagonal only), in three steps
-// with a barrier after each.  First the four 16 x 16 diagonal blocks, by one wave: forward
+// T = (1 + A)^-1 in the place of the strictly lower A (LDS, 64 x LD; read below the diagonal only), in
+// three steps with a barrier after each.  First the four 16 x 16 diagonal blocks, by one wave: forward
 // substitution, which is stable whatever A holds; 16 lanes have a block, a column of T each, and a row
 // of A at a time, whose elements a lane takes from its neighbours.
-__device__ __forceinline__ void invert_diagonal(const float* __restrict__ A, float* __restrict__ Tm, int lane) {
+__device__ __forceinline__ void invert_diagonal(float* A, int lane) {
   const int c = lane & 15, g = lane >> 4;
   const int at = 16 * g * LD + 16 * g + c;
   float a[16], x[16];
@@ -84,50 +84,51 @@ __device__ __forceinline__ void invert_diagonal(const float* __restrict__ A, flo
   for (int i = 0; i < 16; ++i) a[i] = A[at + i * LD];
   substitute_rows<0>(a, x, c);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) Tm[at + i * LD] = x[i];
+  for (int i = 0; i < 16; ++i) A[at + i * LD] = x[i];
   if (!(g & 1)) {  // the tiles right of the first and third, which fragments of 32 columns take with them
 #pragma unroll
-    for (int i = 0; i < 16; ++i) Tm[at + i * LD + 16] = 0.f;
+    for (int i = 0; i < 16; ++i) A[at + i * LD + 16] = 0.f;
   }
 }
-// tile (i, k) of A times tile (k, j) of Tm, or (i, k) of Tm times a result already in registers
-__device__ __forceinline__ f32x4 tile_mul(const float* __restrict__ A, const float* __restrict__ B, int i, int k, int j, f32x4 s, int lane) {
+// tile (i, k) times tile (k, j), or times a result already in registers
+__device__ __forceinline__ f32x4 tile_mul(const float* A, int i, int k, int j, f32x4 s, int lane) {
   const int c = lane & 15, g = lane >> 4;
   const f32x4 x = *reinterpret_cast<const f32x4*>(A + (16 * i + c) * LD + 16 * k + 4 * g);
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    s = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], B[(16 * k + 4 * g + r) * LD + 16 * j + c], s, 0, 0, 0);
+    s = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], A[(16 * k + 4 * g + r) * LD + 16 * j + c], s, 0, 0, 0);
   return s;
 }
-__device__ __forceinline__ f32x4 tile_mul(const float* __restrict__ A, int i, int k, f32x4 y, f32x4 s, int lane) {
+__device__ __forceinline__ f32x4 tile_mul(const float* A, int i, int k, f32x4 y, f32x4 s, int lane) {
   const int c = lane & 15, g = lane >> 4;
   const f32x4 x = *reinterpret_cast<const f32x4*>(A + (16 * i + c) * LD + 16 * k + 4 * g);
 #pragma unroll
   for (int r = 0; r < 4; ++r) s = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], y[r], s, 0, 0, 0);
   return s;
 }
-__device__ __forceinline__ void tile_put(float* __restrict__ Tm, int i, int j, f32x4 v, int lane) {
+__device__ __forceinline__ void tile_put(float* Tm, int i, int j, f32x4 v, int lane) {
   const int c = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int r = 0; r < 4; ++r) Tm[(16 * i + 4 * g + r) * LD + 16 * j + c] = -v[r];
 }
 // Then blocks of 32 from blocks of 16, and 64 from 32, on fp32 MFMA: the lower left is
 // -T22 A21 T11.  All four waves call it; barriers inside and at the end.
-__device__ __forceinline__ void invert_below(const float* __restrict__ A, float* __restrict__ Tm, int wave, int lane) {
+__device__ __forceinline__ void invert_below(float* A, int wave, int lane) {
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   if (wave < 2) {
     const int i = 2 * wave + 1, j = 2 * wave;
-    tile_put(Tm, i, j, tile_mul(Tm, i, i, tile_mul(A, Tm, i, j, j, zero, lane), zero, lane), lane);
+    tile_put(A, i, j, tile_mul(A, i, i, tile_mul(A, i, j, j, zero, lane), zero, lane), lane);
   }
   __syncthreads();
   const int i = 2 + (wave >> 1), j = wave & 1;
   f32x4 y = zero, t = zero;
   for (int k = 2; k <= i; ++k) {
-    y = tile_mul(A, Tm, k, 1, j, zero, lane);  // (tile (0, 1) of Tm is zero)
-    if (j == 0) y = tile_mul(A, Tm, k, 0, j, y, lane);
-    t = tile_mul(Tm, i, k, y, t, lane);
+    y = tile_mul(A, k, 1, j, zero, lane);  // (tile (0, 1) of T is zero)
+    if (j == 0) y = tile_mul(A, k, 0, j, y, lane);
+    t = tile_mul(A, i, k, y, t, lane);
   }
-  tile_put(Tm, i, j, t, lane);  // nobody reads these four tiles before the barrier
+  __syncthreads();  // the lower left is still A's until every wave is past it
+  tile_put(A, i, j, t, lane);
   __syncthreads();
 }
 
@@ -198,7 +199,7 @@ template <typename T, int KP, bool BWD>
 __global__ __launch_bounds__(256) void gdr_prepare_kernel(GdrArgs a) {
   constexpr int NP = kParts<T>, KS = KP / 32, PP = BWD ? 3 : kOutParts<T>;
   __shared__ uint4 kl[KS * 4 * NP * 64];  // K's fragments, then Q's
-  __shared__ __align__(16) float wm[64 * LD], tm[64 * LD];
+  __shared__ __align__(16) float wm[64 * LD];
   __shared__ float2 gd[64];
   __shared__ float bs[64];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(256) void gdr_prepare_kernel(GdrArgs a) {
       for (int p = 0; p < NP; ++p) kl[((s * 4 + wave) * NP + p) * 64 + lane] = qr[s][p];
     __syncthreads();
   }
-  if (wave == 0) invert_diagonal(wm, tm, lane);
+  if (wave == 0) invert_diagonal(wm, lane);
   {
     // forward: (Q K^T)^T = K Q^T, columns 16 wave .., row tiles up to the diagonal; backward: Q K^T,
     // columns 16 wave .., row tiles from the diagonal on
@@ -328,9 +329,10 @@ __global__ __launch_bounds__(256) void gdr_prepare_kernel(GdrArgs a) {
       if (owner) write_columns<KP, NP>(kl, a.qtf + kbase, wave, lane);
   }
   __syncthreads();
-  invert_below(wm, tm, wave, lane);
-  write_lower(tm, a.tf + tbase, wave, lane);
+  invert_below(wm, wave, lane);
+  write_lower(wm, a.tf + tbase, wave, lane);
   if constexpr (BWD) {  // and (1 + diag(beta) W)^-1, transposed
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (j <= wave)
@@ -340,10 +342,10 @@ __global__ __launch_bounds__(256) void gdr_prepare_kernel(GdrArgs a) {
           wm[i * LD + 16 * j + c] = bs[i] * w[j][r];
         }
     __syncthreads();
-    if (wave == 0) invert_diagonal(wm, tm, lane);
+    if (wave == 0) invert_diagonal(wm, lane);
     __syncthreads();
-    invert_below(wm, tm, wave, lane);
-    write_transposed(tm, a.ttf + tbase, wave, lane);
+    invert_below(wm, wave, lane);
+    write_transposed(wm, a.ttf + tbase, wave, lane);
   }
 }
 
@@ -692,8 +694,10 @@ __global__ __launch_bounds__(512) void gdr_chain_kernel(GdrArgs a) {
         y = half(0, y);
         if (two) z = half(1, z);
         y += z;
+        // loads before the store: what waits for them would wait for a store in front of them too
         pf += more ? pstep : 0;
         load_p();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int r = 0; r < 4; ++r) ol[m][4 * g + r][c] = from_f32<T>(a.scale * y[r]);
         __builtin_amdgcn_wave_barrier();
