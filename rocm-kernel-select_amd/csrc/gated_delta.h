@@ -53,6 +53,7 @@ struct GdrArgs {
 // which writes the output and final state, or (keep) each chunk's state and errors.
 int gdr_prepare(const GdrArgs& a, int dtype, bool backward, hipStream_t s);
 int gdr_chain(const GdrArgs& a, int dtype, bool keep, hipStream_t s);
+int gdr_tokens(const GdrArgs& a, int dtype, hipStream_t s);  // forward, a token at a time
 size_t gdr_plan(const atk_gated_delta_args* p, bool backward, GdrArgs* a, int* rc);
 inline int gdr_padded_k(int K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
 

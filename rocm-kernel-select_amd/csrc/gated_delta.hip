@@ -1,4 +1,4 @@
-// The gated delta rule, one token at a time: the decode step over a cache of states.
+// The gated delta rule, one token at a time: the decode step over a cache of states, and short sequences.
 //
 //   S~ = exp(g) S;  u = beta (v - S~^T k);  S' = S~ + k u^T;  o = scale S'^T q
 //
@@ -143,7 +143,157 @@ void launch_step_typed(const GdrStepArgs& a, hipStream_t s) {
   }
 }
 
+// A few tokens of each sequence, one after the other, with the state in registers throughout: what
+// short calls take (a chunk's two launches are as long as 10 tokens here).  A workgroup has 32
+// columns (VW 4) or 64 (VW 1) of a head; the next token's inputs are on their way meanwhile.
+template <typename T, int VW, int NV, int RPT>
+__global__ __launch_bounds__(256) void gdr_tokens_kernel(GdrArgs a) {
+  constexpr int RG = 256 / NV, W = 2 * VW, KL = (RG * RPT + 255) / 256;
+  __shared__ float kf[2][RG * RPT], qf[2][RG * RPT];
+  __shared__ float red[2][4][NV][W];
+  __shared__ float red_kq[2][4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int cg = tid % NV, rg = tid / NV;
+  const int64_t n = blockIdx.z;
+  const int h = blockIdx.y, hk = h / a.group;
+  const int c0 = (blockIdx.x * NV + cg) * VW;
+  const bool live = c0 < a.V;  // V is a multiple of VW (host check)
+  const GdrSeq seq = gdr_seq(a.cu, a.T, n);
+  const int64_t at = (n * a.Hv + h) * (int64_t)a.K * a.V + c0;
+  float s[RPT][VW];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = rg + i * RG;
+    if constexpr (VW == 4) {
+      const float4 t = a.s0 && live && r < a.K ? *reinterpret_cast<const float4*>(a.s0 + at + (int64_t)r * a.V) : make_float4(0.f, 0.f, 0.f, 0.f);
+      s[i][0] = t.x; s[i][1] = t.y; s[i][2] = t.z; s[i][3] = t.w;
+    } else {
+      s[i][0] = a.s0 && live && r < a.K ? a.s0[at + (int64_t)r * a.V] : 0.f;
+    }
+  }
+  const T* __restrict__ k = static_cast<const T*>(a.k) + seq.batch * a.k_s[0] + seq.begin * a.k_s[1] + hk * a.k_s[2];
+  const T* __restrict__ q = static_cast<const T*>(a.q) + seq.batch * a.q_s[0] + seq.begin * a.q_s[1] + hk * a.q_s[2];
+  const T* __restrict__ v = static_cast<const T*>(a.v) + seq.batch * a.v_s[0] + seq.begin * a.v_s[1] + h * a.v_s[2];
+  T* __restrict__ o = static_cast<T*>(a.o) + ((seq.batch * a.T + seq.begin) * a.Hv + h) * (int64_t)a.V;
+  float kn[KL], qn[KL], vn[VW], gn, bn;
+  auto load = [&](int64_t t) {
+#pragma unroll
+    for (int z = 0; z < KL; ++z) {
+      const int r = tid + 256 * z;
+      kn[z] = r < a.K ? to_f32(k[t * a.k_s[1] + r]) : 0.f;
+      qn[z] = r < a.K ? to_f32(q[t * a.q_s[1] + r]) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < VW; ++j) vn[j] = live ? to_f32(v[t * a.v_s[1] + c0 + j]) : 0.f;
+    gn = load_param(a.g, a.g_dtype, seq.batch * a.g_s[0] + (seq.begin + t) * a.g_s[1] + h * a.g_s[2]);
+    bn = load_param(a.beta, a.b_dtype, seq.batch * a.b_s[0] + (seq.begin + t) * a.b_s[1] + h * a.b_s[2]);
+  };
+  if (seq.len > 0) load(0);
+  for (int64_t t = 0; t < seq.len; ++t) {
+    const int b = t & 1;
+#pragma unroll
+    for (int z = 0; z < KL; ++z)
+      if (tid + 256 * z < RG * RPT) {
+        kf[b][tid + 256 * z] = kn[z];
+        qf[b][tid + 256 * z] = qn[z];
+      }
+    const float decay = expf(gn), beta = bn;
+    float vv[VW];
+#pragma unroll
+    for (int j = 0; j < VW; ++j) vv[j] = vn[j];
+    if (t + 1 < seq.len) load(t + 1);
+    __syncthreads();
+    float p[W], kq = 0.f;
+#pragma unroll
+    for (int j = 0; j < W; ++j) p[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const float kr = kf[b][rg + i * RG], qr = qf[b][rg + i * RG];
+      kq += kr * qr;
+#pragma unroll
+      for (int j = 0; j < VW; ++j) {
+        p[j] += s[i][j] * kr;
+        p[VW + j] += s[i][j] * qr;
+      }
+    }
+#pragma unroll
+    for (int off = NV; off < 64; off <<= 1) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) p[j] += __shfl_xor(p[j], off, 64);
+      kq += __shfl_xor(kq, off, 64);
+    }
+    if (lane < NV) {
+#pragma unroll
+      for (int j = 0; j < W; ++j) red[b][wave][cg][j] = p[j];
+      if (lane == 0) red_kq[b][wave] = kq;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < W; ++j) p[j] = (red[b][0][cg][j] + red[b][1][cg][j]) + (red[b][2][cg][j] + red[b][3][cg][j]);
+    kq = (red_kq[b][0] + red_kq[b][1]) + (red_kq[b][2] + red_kq[b][3]);
+    float u[VW];
+#pragma unroll
+    for (int j = 0; j < VW; ++j) u[j] = beta * (vv[j] - decay * p[j]);
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const float kr = kf[b][rg + i * RG];
+#pragma unroll
+      for (int j = 0; j < VW; ++j) s[i][j] = decay * s[i][j] + kr * u[j];
+    }
+    if (rg == 0 && live) {
+#pragma unroll
+      for (int j = 0; j < VW; ++j) o[t * a.Hv * (int64_t)a.V + c0 + j] = from_f32<T>(a.scale * (decay * p[VW + j] + kq * u[j]));
+    }
+    // (the buffers of this token are written again two barriers from here at the earliest)
+  }
+  if (a.s1) {
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const int r = rg + i * RG;
+      if (!live || r >= a.K) continue;
+      if constexpr (VW == 4) *reinterpret_cast<float4*>(a.s1 + at + (int64_t)r * a.V) = make_float4(s[i][0], s[i][1], s[i][2], s[i][3]);
+      else a.s1[at + (int64_t)r * a.V] = s[i][0];
+    }
+  }
+  // tokens of a packed row before its first sequence and after its last have an output of zero
+  if (a.cu && live && (n == 0 || n == a.n - 1)) {
+    T* __restrict__ all = static_cast<T*>(a.o);
+    const int64_t from[2] = {n == 0 ? 0 : a.T, n == a.n - 1 ? seq.begin + seq.len : a.T};
+    const int64_t to[2] = {n == 0 ? seq.begin : a.T, a.T};
+    for (int z = 0; z < 2; ++z)
+      for (int64_t i = from[z] + rg; i < to[z]; i += RG)
+#pragma unroll
+        for (int j = 0; j < VW; ++j) all[(i * a.Hv + h) * (int64_t)a.V + c0 + j] = from_f32<T>(0.f);
+  }
+}
+
+template <typename T, int VW, int NV, int RPT>
+void launch_tokens(const GdrArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.V + NV * VW - 1) / (NV * VW)), (unsigned)a.Hv, (unsigned)a.n);
+  hipLaunchKernelGGL((gdr_tokens_kernel<T, VW, NV, RPT>), grid, dim3(256), 0, s, a);
+}
+template <typename T>
+void launch_tokens_typed(const GdrArgs& a, hipStream_t s) {
+  if (a.V % 4 || !aligned16(a.s0) || !aligned16(a.s1)) {
+    if (a.K <= 64) launch_tokens<T, 1, 64, 16>(a, s);
+    else if (a.K <= 128) launch_tokens<T, 1, 64, 32>(a, s);
+    else launch_tokens<T, 1, 64, 64>(a, s);
+  } else {
+    if (a.K <= 64) launch_tokens<T, 4, 8, 2>(a, s);
+    else if (a.K <= 128) launch_tokens<T, 4, 8, 4>(a, s);
+    else launch_tokens<T, 4, 8, 8>(a, s);
+  }
+}
+
 }  // namespace
+
+int gdr_tokens(const GdrArgs& a, int dtype, hipStream_t s) {
+  if (dtype == ATK_F32) launch_tokens_typed<float>(a, s);
+  else if (dtype == ATK_F16) launch_tokens_typed<_Float16>(a, s);
+  else launch_tokens_typed<__bf16>(a, s);
+  return check_launch("gdr_tokens_kernel");
+}
+
 }  // namespace atk
 
 extern "C" int atk_gated_delta_update(const atk_gated_delta_update_args* p) {

@@ -171,7 +171,7 @@ def sequence64(q, k, v, g, beta, scale, state, cu=None):
 
 
 SHAPES = [  # batch, tokens, key heads, value heads, key columns, value columns
-    (1, 1, 1, 1, 1, 1), (2, 2, 1, 2, 64, 64), (1, 63, 2, 2, 128, 128), (1, 64, 1, 4, 128, 32), (2, 65, 2, 4, 64, 100),
+    (1, 1, 1, 1, 1, 1), (2, 2, 1, 2, 64, 64), (3, 5, 2, 4, 128, 100), (1, 8, 1, 2, 200, 33), (2, 7, 1, 1, 130, 64), (2, 9, 1, 2, 128, 128), (1, 63, 2, 2, 128, 128), (1, 64, 1, 4, 128, 32), (2, 65, 2, 4, 64, 100),
     (1, 130, 1, 1, 17, 33), (3, 200, 1, 3, 96, 16), (1, 129, 2, 2, 130, 20), (1, 70, 1, 1, 256, 256), (1, 321, 1, 2, 100, 7)]
 
 
@@ -193,7 +193,7 @@ def test_sequences(dev, b, t, hk, hv, dk, dv, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("cu,t", [([0, 5], 5), ([0, 1, 64, 65, 200], 200), ([0, 0, 130, 130, 131, 131], 131),
+@pytest.mark.parametrize("cu,t", [([0, 5], 5), ([1, 3, 3, 7], 8), ([0, 1, 64, 65, 200], 200), ([0, 0, 130, 130, 131, 131], 131),
                                   ([3, 60, 190], 200), ([0, 63, 126, 189, 252], 256), ([0, 0], 40), ([7], 9)])
 def test_packed_sequences(dev, cu, t, dtype):
     import amd_tuned_torch as P
@@ -412,7 +412,7 @@ def test_gradients(dev, b, t, hk, hv, dk, dv, dtype):
 
 
 @gpu
-@pytest.mark.parametrize("cu,t", [([0, 5], 5), ([0, 1, 64, 65, 200], 200), ([0, 0, 130, 130, 131], 131), ([3, 60, 190], 200)])
+@pytest.mark.parametrize("cu,t", [([0, 5], 5), ([1, 3, 3, 7], 8), ([0, 1, 64, 65, 200], 200), ([0, 0, 130, 130, 131], 131), ([3, 60, 190], 200)])
 def test_packed_gradients(dev, cu, t):
     args = make((1, t), 2, 4, 64, 48, torch.float32, dev, seed=t)
     state = torch.randn(len(cu) - 1, 4, 64, 48, generator=torch.Generator().manual_seed(3)).to(dev)
