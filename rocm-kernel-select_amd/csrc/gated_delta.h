@@ -49,10 +49,8 @@ struct GdrArgs {
   int VP;
 };
 
-// Host side, shared by the forward and the backward: fragments of all chunks, and the state's chain,
-// which writes the output and final state, or (keep) each chunk's state and errors.
+// Host side, shared by the forward and the backward: fragments of all chunks.
 int gdr_prepare(const GdrArgs& a, int dtype, bool backward, hipStream_t s);
-int gdr_chain(const GdrArgs& a, int dtype, bool keep, hipStream_t s);
 int gdr_tokens(const GdrArgs& a, int dtype, hipStream_t s);  // forward, a token at a time
 size_t gdr_plan(const atk_gated_delta_args* p, bool backward, GdrArgs* a, int* rc);
 inline int gdr_padded_k(int K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
@@ -80,16 +78,6 @@ __device__ __forceinline__ int64_t gdr_seq_of_slot(const int* __restrict__ cu, i
     else hi = mid - 1;
   }
   return lo;
-}
-
-// Workgroup -> (value tile, head, sequence).  Workgroups are dealt to the 8 XCDs in turn; all value
-// tiles of a head and sequence get the same one, since they read the same fragments through its L2.
-__device__ __forceinline__ bool gdr_chain_place(const GdrArgs& a, int tiles, int* tile, int* h, int64_t* n) {
-  const int64_t j = blockIdx.x / 8, unit = j / tiles * 8 + blockIdx.x % 8;
-  *tile = (int)(j % tiles);
-  *h = (int)(unit % a.Hv);
-  *n = unit / a.Hv;
-  return *n < a.n;
 }
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));

@@ -16,7 +16,7 @@
 //          exp(G_63) <S, dS'> + sum_j k_j . ((E U) dS'^T)_j;   dg = sums of dG from the chunk's end
 // Key heads that several value heads share get the sum over them in a fixed order: one workgroup has
 // a key head's whole group.
-#include "gated_delta.h"
+#include "gated_delta_chain.h"
 
 namespace atk {
 namespace {
@@ -30,21 +30,34 @@ __device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float
 // The chain of dS', built as the forward's: four waves pass the state's gradient on, 16 value columns
 // of it; four more make what needs dO alone, a chunk ahead: scale P^T dO and Q^T (scale exp(G) dO).
 // FULL as there.
+template <typename T, int KP>
+struct GdrBwdLds {
+  static constexpr int NP = kParts<T>;
+  f32x4 kp[4][4][64];                            // partial sums of K dS'
+  uint2 ul[2][3][64][2], rl[2][3][64][2];        // dU, and -beta exp(G) dR
+  uint2 dl[2][NP][64][2], gl[2][3][64][2];       // dO, and scale exp(G) dO
+  f32x4 pl[4][64];                               // scale P^T dO
+  f32x4 ql[2][KP / 16][64];                      // Q^T (scale exp(G) dO), two chunks'
+  f32x4 tl[4][64];                               // dO on its way from rows to columns
+};
 template <typename T, int KP, bool FULL>
-__global__ __launch_bounds__(512) void gdr_bwd_chain_kernel(GdrArgs a) {
+__device__ __forceinline__ void gdr_bwd_chain(const GdrArgs& a, char* lds, int64_t block) {
   constexpr int NP = kParts<T>, KS = KP / 32, MT = KP / 64, KW = MT > 1 ? MT / 2 : 1;
   constexpr int KF = KS * 4 * NP * 64;
-  __shared__ f32x4 kp[4][4][64];                            // partial sums of K dS'
-  __shared__ uint2 ul[2][3][64][2], rl[2][3][64][2];        // dU, and -beta exp(G) dR
-  __shared__ uint2 dl[2][NP][64][2], gl[2][3][64][2];       // dO, and scale exp(G) dO
-  __shared__ f32x4 pl[4][64];                               // scale P^T dO
-  __shared__ f32x4 ql[2][KP / 16][64];                      // Q^T (scale exp(G) dO), two chunks'
-  __shared__ f32x4 tl[4][64];                               // dO on its way from rows to columns
+  GdrBwdLds<T, KP>& L = *reinterpret_cast<GdrBwdLds<T, KP>*>(lds);
+  auto& kp = L.kp;
+  auto& ul = L.ul;
+  auto& rl = L.rl;
+  auto& dl = L.dl;
+  auto& gl = L.gl;
+  auto& pl = L.pl;
+  auto& ql = L.ql;
+  auto& tl = L.tl;
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   int tile, h;
   int64_t n;
-  if (!gdr_chain_place(a, a.VP / 16, &tile, &h, &n)) return;
+  if (!gdr_chain_place(a, block, a.VP / 16, &tile, &h, &n)) return;
   const int hk = h / a.group, col = tile * 16 + c;
   const GdrSeq seq = gdr_seq(a.cu, a.T, n);
   const int64_t chunks = (seq.len + kGdrC - 1) / kGdrC, end = seq.slot + chunks - 1;  // from the last chunk down
@@ -357,6 +370,19 @@ __global__ __launch_bounds__(512) void gdr_bwd_chain_kernel(GdrArgs a) {
         }
     }
   }
+}
+
+// Both chains in one launch, the longer one's workgroups first: neither needs the other, and where there
+// are fewer tiles than CUs they run side by side (1021 tokens, 4 heads of 64 x 64 fp32: 38 -> 24 us).
+// Two to a CU gained nothing for 256 tiles of 128 x 128 in bf16 (168 us, one after the other 156): their
+// loads then wait for each other.
+template <typename T, int KP, bool FULL>
+__global__ __launch_bounds__(512) void gdr_chains_kernel(GdrArgs a) {
+  constexpr size_t A = sizeof(GdrChainLds<T, KP, true>), B = sizeof(GdrBwdLds<T, KP>);
+  __shared__ __align__(16) char lds[A > B ? A : B];
+  const int64_t half = gridDim.x / 2;
+  if (blockIdx.x >= half) gdr_chain<T, KP, true, FULL>(a, lds, blockIdx.x - half);
+  else gdr_bwd_chain<T, KP, FULL>(a, lds, blockIdx.x);
 }
 
 // (row, column) tile t of the ten of a lower triangle of 16 x 16 tiles
@@ -753,11 +779,11 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
 
 template <typename T, int KP>
 int launch(const GdrArgs& a, hipStream_t s) {
-  const int64_t grid = (a.n * a.Hv + 7) / 8 * 8 * (a.VP / 16);
+  const int64_t grid = (a.n * a.Hv + 7) / 8 * 16 * (a.VP / 16);
   if (grid > 0x7fffffff) return fail(ATK_UNSUPPORTED, "gated delta backward: too many heads, sequences and value columns");
-  if (a.V % 16 == 0 || a.V % 16 >= 4) hipLaunchKernelGGL((gdr_bwd_chain_kernel<T, KP, true>), dim3((unsigned)grid), dim3(512), 0, s, a);
-  else hipLaunchKernelGGL((gdr_bwd_chain_kernel<T, KP, false>), dim3((unsigned)grid), dim3(512), 0, s, a);
-  if (int rc = check_launch("gdr_bwd_chain_kernel")) return rc;
+  if (a.V % 16 == 0 || a.V % 16 >= 4) hipLaunchKernelGGL((gdr_chains_kernel<T, KP, true>), dim3((unsigned)grid), dim3(512), 0, s, a);
+  else hipLaunchKernelGGL((gdr_chains_kernel<T, KP, false>), dim3((unsigned)grid), dim3(512), 0, s, a);
+  if (int rc = check_launch("gdr_chains_kernel")) return rc;
   if (a.T == 0) return ATK_OK;
   const dim3 g((unsigned)a.slots, (unsigned)a.Hk);
   if (a.V % 8 == 0) hipLaunchKernelGGL((gdr_grads_kernel<T, KP, true>), g, dim3(512), 0, s, a);
@@ -798,10 +824,8 @@ extern "C" int atk_gated_delta_bwd(const atk_gated_delta_args* p, const void* do
   a.dout = dout; a.ds1 = static_cast<const float*>(dfinal_state); a.ds0 = static_cast<float*>(dinitial_state);
   a.dq = dq; a.dk = dk; a.dv = dv; a.dg = dg; a.dbeta = dbeta;
   hipStream_t s = reinterpret_cast<hipStream_t>(p->stream);
-  if (p->T > 0) {
+  if (p->T > 0)
     if (int r = gdr_prepare(a, p->dtype, true, s)) return r;
-    if (int r = gdr_chain(a, p->dtype, true, s)) return r;
-  }
   if (p->dtype == ATK_F32) return launch_sized<float>(a, s);
   if (p->dtype == ATK_F16) return launch_sized<_Float16>(a, s);
   return launch_sized<__bf16>(a, s);
