@@ -70,7 +70,7 @@ __device__ __forceinline__ GdrSeq gdr_seq(const int* __restrict__ cu, int64_t T,
 }
 // The sequence that chunk slot `slot` belongs to; a slot that no chunk has gets one past its end.
 __device__ __forceinline__ int64_t gdr_seq_of_slot(const int* __restrict__ cu, int64_t T, int64_t n, int64_t slot) {
-  if (!cu) return slot / ((T + kGdrC - 1) / kGdrC);
+  if (!cu) return (uint32_t)slot / (uint32_t)((T + kGdrC - 1) / kGdrC);  // (both below 2^31)
   int64_t lo = 0, hi = n - 1;  // the last sequence whose first slot is not after `slot`
   while (lo < hi) {
     const int64_t mid = (lo + hi + 1) / 2;

@@ -18,17 +18,22 @@ namespace {
 
 constexpr int LD = 68;  // row pitch of the fp32 64 x 64 tiles in LDS: 16-byte rows, 4 banks apart
 
-// 4 consecutive elements of a row of N, zeros past its end
-template <typename T>
-__device__ __forceinline__ void load4(const T* __restrict__ p, int c, int N, bool live, float* o) {
-  if (live && c + 4 <= N) {
-    T e[4];
-    __builtin_memcpy(e, p + c, 4 * sizeof(T));  // element alignment only
+// This lane's elements of a row of K, in gdr_at's order for each 32, and all of its loads at once: with
+// a branch around each the compiler waits for each (20 000 of a workgroup's 40 000 cycles, when it did).
+template <typename T, int KP, bool FULL>
+__device__ __forceinline__ void load_row(const T* __restrict__ p, int K, int g, T (&o)[KP / 32][8]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = to_f32(e[i]);
-  } else {
+  for (int s = 0; s < KP / 32; ++s) {
+    if constexpr (FULL) {
+      __builtin_memcpy(o[s], p + 32 * s + 4 * g, 4 * sizeof(T));  // element alignment only
+      __builtin_memcpy(o[s] + 4, p + 32 * s + 16 + 4 * g, 4 * sizeof(T));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = live && c + i < N ? to_f32(p[c + i]) : 0.f;
+      for (int i = 0; i < 8; ++i) {
+        const int d = 32 * s + gdr_at(g, i);
+        o[s][i] = p[d < K ? d : 0];
+      }
+    }
   }
 }
 
@@ -192,52 +197,70 @@ __device__ __forceinline__ void write_products(const f32x4& lo, const f32x4& hi,
   for (int p = 0; p < P; ++p) out[p * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
 }
 
-// A workgroup for each (chunk, value head); the first value head of a key head's group also writes
-// that key head's K and K^T (and Q^T).  The masked products leave the registers as fragments: a
-// product's result has the layout of its transpose's rows, so Q K^T comes out of K Q^T.
-template <typename T, int KP, bool BWD>
-__global__ __launch_bounds__(256) void gdr_prepare_kernel(GdrArgs a) {
+// A workgroup for each chunk and `heads` value heads of one key head (one or two); the first of a key
+// head's group also writes that key head's K, Q and K^T (or K, K^T and Q^T).  K K^T and Q K^T are
+// computed once for both.  The masked products leave the registers as fragments: a product's result has
+// the layout of its transpose's rows, so Q K^T comes out of K Q^T.  FULL: K is KP.
+template <typename T, int KP, bool BWD, bool FULL>
+__global__ __launch_bounds__(256) void gdr_prepare_kernel(GdrArgs a, int heads) {
   constexpr int NP = kParts<T>, KS = KP / 32, PP = BWD ? 3 : kOutParts<T>;
   __shared__ uint4 kl[KS * 4 * NP * 64];  // K's fragments, then Q's
   __shared__ __align__(16) float wm[64 * LD];
-  __shared__ float2 gd[64];
-  __shared__ float bs[64];
+  __shared__ float2 gd[2][64];
+  __shared__ float bs[2][64];
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t slot = blockIdx.x;
-  const int h = blockIdx.y, hk = h / a.group;
+  const int h0 = blockIdx.y * heads, hk = h0 / a.group;
   const int64_t n = gdr_seq_of_slot(a.cu, a.T, a.n, slot);
   const GdrSeq seq = gdr_seq(a.cu, a.T, n);
   const int64_t at = (slot - seq.slot) * kGdrC;  // the chunk's first token within the sequence
   if (at < 0 || at >= seq.len) return;
   const int rows = (int)(seq.len - at < kGdrC ? seq.len - at : kGdrC);
   const int64_t t0 = seq.begin + at;
-  const bool owner = h % a.group == 0;
+  const bool owner = h0 % a.group == 0;
   const int64_t kbase = (hk * a.slots + slot) * (int64_t)(KS * 4 * NP * 64);
-  const int64_t tbase = (h * a.slots + slot) * (int64_t)(kTri * 3 * 64);
-  float gv = 0.f, bv = 0.f;
-  if (wave == 0 && lane < rows) {
-    gv = load_param(a.g, a.g_dtype, seq.batch * a.g_s[0] + (t0 + lane) * a.g_s[1] + h * a.g_s[2]);
-    bv = load_param(a.beta, a.b_dtype, seq.batch * a.b_s[0] + (t0 + lane) * a.b_s[1] + h * a.b_s[2]);
-  }
   uint4 qr[KS][NP], kr[KS][NP];  // this wave's 16 tokens
   {
-    const int64_t tok = t0 + 16 * wave + c;
     const bool live = 16 * wave + c < rows;
-    const T* __restrict__ q = static_cast<const T*>(a.q) + (live ? seq.batch * a.q_s[0] + tok * a.q_s[1] + hk * a.q_s[2] : 0);
-    const T* __restrict__ k = static_cast<const T*>(a.k) + (live ? seq.batch * a.k_s[0] + tok * a.k_s[1] + hk * a.k_s[2] : 0);
+    const int64_t tok = t0 + (live ? 16 * wave + c : 0);
+    const T* __restrict__ q = static_cast<const T*>(a.q) + seq.batch * a.q_s[0] + tok * a.q_s[1] + hk * a.q_s[2];
+    const T* __restrict__ k = static_cast<const T*>(a.k) + seq.batch * a.k_s[0] + tok * a.k_s[1] + hk * a.k_s[2];
+    T kv[KS][8], qv[KS][8];
+    load_row<T, KP, FULL>(k, a.K, g, kv);
+    load_row<T, KP, FULL>(q, a.K, g, qv);
+    if (wave < heads) {  // wave w has the decays of head w
+      const int h = h0 + wave;
+      const int64_t i = t0 + (lane < rows ? lane : 0);
+      float gv = load_param(a.g, a.g_dtype, seq.batch * a.g_s[0] + i * a.g_s[1] + h * a.g_s[2]);
+      float bv = load_param(a.beta, a.b_dtype, seq.batch * a.b_s[0] + i * a.b_s[1] + h * a.b_s[2]);
+      gv = lane < rows ? gv : 0.f;
+      bv = lane < rows ? bv : 0.f;
+      float2 last;
+      // below -120 the decay is 0 in fp32 whatever follows, and sums with -inf have no differences
+      const float2 s = running_sum(gv < -120.f ? -120.f : gv, &last);
+      gd[wave][lane] = s;
+      bs[wave][lane] = bv;
+      if constexpr (BWD) a.gsum[(h * a.slots + slot) * 64 + lane] = s;
+      float* __restrict__ row = a.row + (h * a.slots + slot) * 192;
+      row[lane] = gdr_decay(s, make_float2(0.f, 0.f));
+      row[64 + lane] = gdr_decay(last, s);
+      row[128 + lane] = bv;
+    }
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      float v[8];
+      float x[8], y[8];
       bf16x8 parts[NP];
-      load4(k, 32 * s + 4 * g, a.K, live, v);
-      load4(k, 32 * s + 16 + 4 * g, a.K, live, v + 4);
-      split_parts<NP, 8>(v, parts);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool in = live && (FULL || 32 * s + gdr_at(g, i) < a.K);
+        x[i] = in ? to_f32(kv[s][i]) : 0.f;
+        y[i] = in ? to_f32(qv[s][i]) : 0.f;
+      }
+      split_parts<NP, 8>(x, parts);
 #pragma unroll
       for (int p = 0; p < NP; ++p) kr[s][p] = __builtin_bit_cast(uint4, parts[p]);
-      load4(q, 32 * s + 4 * g, a.K, live, v);
-      load4(q, 32 * s + 16 + 4 * g, a.K, live, v + 4);
-      split_parts<NP, 8>(v, parts);
+      split_parts<NP, 8>(y, parts);
 #pragma unroll
       for (int p = 0; p < NP; ++p) qr[s][p] = __builtin_bit_cast(uint4, parts[p]);
     }
@@ -250,102 +273,107 @@ __global__ __launch_bounds__(256) void gdr_prepare_kernel(GdrArgs a) {
         if (!BWD && owner) a.qf[kbase + ((s * 4 + wave) * NP + p) * 64 + lane] = qr[s][p];
       }
   }
-  if (wave == 0) {
-    float2 last;
-    // below -120 the decay is 0 in fp32 whatever follows, and sums with -inf have no differences
-    const float2 s = running_sum(gv < -120.f ? -120.f : gv, &last);
-    gd[lane] = s;
-    bs[lane] = bv;
-    if constexpr (BWD) a.gsum[(h * a.slots + slot) * 64 + lane] = s;
-    float* __restrict__ row = a.row + (h * a.slots + slot) * 192;
-    row[lane] = gdr_decay(s, make_float2(0.f, 0.f));
-    row[64 + lane] = gdr_decay(last, s);
-    row[128 + lane] = bv;
-  }
   __syncthreads();
-  // rows 16 wave .. of W = strictly lower K K^T * D, its columns times beta, into wm
-  f32x4 w[4];
+  // K K^T, rows 16 wave ..
+  f32x4 kk[4], qk[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    w[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    kk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (j <= wave) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         uint4 b[NP];
 #pragma unroll
         for (int p = 0; p < NP; ++p) b[p] = kl[((s * 4 + j) * NP + p) * 64 + lane];
-        w[j] = mma_parts<NP, NP>(kr[s], b, w[j]);
-      }
-      const int cj = 16 * j + c;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int i = 16 * wave + 4 * g + r;
-        w[j][r] = cj < i ? w[j][r] * gdr_decay(gd[i], gd[cj]) : 0.f;
-        wm[i * LD + cj] = w[j][r] * bs[cj];
+        kk[j] = mma_parts<NP, NP>(kr[s], b, kk[j]);
       }
     }
   }
   if (owner) write_columns<KP, NP>(kl, a.ktf + kbase, wave, lane);
-  __syncthreads();
   if constexpr (BWD) {  // Q in K's place
+    __syncthreads();
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int p = 0; p < NP; ++p) kl[((s * 4 + wave) * NP + p) * 64 + lane] = qr[s][p];
     __syncthreads();
   }
-  if (wave == 0) invert_diagonal(wm, lane);
-  {
-    // forward: (Q K^T)^T = K Q^T, columns 16 wave .., row tiles up to the diagonal; backward: Q K^T,
-    // columns 16 wave .., row tiles from the diagonal on
-    const int col = 16 * wave + c;
-    const float2 gc = gd[col];
-    for (int s = BWD ? wave >> 1 : 0; s < (BWD ? 2 : (wave >> 1) + 1); ++s) {
-      f32x4 y[2];
+  // forward: (Q K^T)^T = K Q^T, columns 16 wave .., row tiles up to the diagonal; backward: Q K^T,
+  // columns 16 wave .., row tiles from the diagonal on
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int j = 2 * s + u;
-        y[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (BWD ? j >= wave : j <= wave) {
+  for (int j = 0; j < 4; ++j) {
+    qk[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (BWD ? j >= wave : j <= wave) {
 #pragma unroll
-          for (int z = 0; z < KS; ++z) {
-            uint4 b[NP];
+      for (int s = 0; s < KS; ++s) {
+        uint4 b[NP];
 #pragma unroll
-            for (int p = 0; p < NP; ++p) b[p] = kl[((z * 4 + j) * NP + p) * 64 + lane];
-            y[u] = mma_parts<NP, NP>(b, BWD ? kr[z] : qr[z], y[u]);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int i = 16 * j + 4 * g + r;
-            if constexpr (BWD) y[u][r] = i >= col ? y[u][r] * gdr_decay(gd[i], gc) : 0.f;
-            else y[u][r] = i <= col ? y[u][r] * gdr_decay(gc, gd[i]) : 0.f;
-          }
-        }
+        for (int p = 0; p < NP; ++p) b[p] = kl[((s * 4 + j) * NP + p) * 64 + lane];
+        qk[j] = mma_parts<NP, NP>(b, BWD ? kr[s] : qr[s], qk[j]);
       }
-      write_products<PP>(y[0], y[1], (BWD ? a.ptf + tbase + tri_upper(wave, s) * PP * 64
-                                          : a.pf + (h * a.slots + slot) * (int64_t)(kTri * PP * 64) + tri_lower(wave, s) * PP * 64), lane);
     }
-    if constexpr (BWD)
-      if (owner) write_columns<KP, NP>(kl, a.qtf + kbase, wave, lane);
   }
-  __syncthreads();
-  invert_below(wm, wave, lane);
-  write_lower(wm, a.tf + tbase, wave, lane);
-  if constexpr (BWD) {  // and (1 + diag(beta) W)^-1, transposed
-    __syncthreads();
+  if constexpr (BWD)
+    if (owner) write_columns<KP, NP>(kl, a.qtf + kbase, wave, lane);
+  for (int x = 0; x < heads; ++x) {
+    const int h = h0 + x;
+    const int64_t tbase = (h * a.slots + slot) * (int64_t)(kTri * 3 * 64);
+    // W = strictly lower K K^T * D, its columns times beta
+    f32x4 w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (j <= wave)
+      if (j <= wave) {
+        const int cj = 16 * j + c;
+        const float2 gj = gd[x][cj];
+        const float bj = bs[x][cj];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int i = 16 * wave + 4 * g + r;
-          wm[i * LD + 16 * j + c] = bs[i] * w[j][r];
+          w[j][r] = cj < i ? kk[j][r] * gdr_decay(gd[x][i], gj) : 0.f;
+          wm[i * LD + cj] = w[j][r] * bj;
         }
+      }
     __syncthreads();
     if (wave == 0) invert_diagonal(wm, lane);
+    {
+      const int col = 16 * wave + c;
+      const float2 gc = gd[x][col];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        if (BWD ? s >= wave >> 1 : s <= wave >> 1) {
+          f32x4 y[2];
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int i = 16 * (2 * s + u) + 4 * g + r;
+              if constexpr (BWD) y[u][r] = i >= col ? qk[2 * s + u][r] * gdr_decay(gd[x][i], gc) : 0.f;
+              else y[u][r] = i <= col ? qk[2 * s + u][r] * gdr_decay(gc, gd[x][i]) : 0.f;
+            }
+          write_products<PP>(y[0], y[1], (BWD ? a.ptf + tbase + tri_upper(wave, s) * PP * 64
+                                              : a.pf + (h * a.slots + slot) * (int64_t)(kTri * PP * 64) + tri_lower(wave, s) * PP * 64), lane);
+        }
+    }
     __syncthreads();
     invert_below(wm, wave, lane);
-    write_transposed(wm, a.ttf + tbase, wave, lane);
+    write_lower(wm, a.tf + tbase, wave, lane);
+    __syncthreads();
+    if constexpr (BWD) {  // and (1 + diag(beta) W)^-1, transposed
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j <= wave)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int i = 16 * wave + 4 * g + r;
+            wm[i * LD + 16 * j + c] = bs[x][i] * w[j][r];
+          }
+      __syncthreads();
+      if (wave == 0) invert_diagonal(wm, lane);
+      __syncthreads();
+      invert_below(wm, wave, lane);
+      write_transposed(wm, a.ttf + tbase, wave, lane);
+      __syncthreads();
+    }
   }
 }
 
@@ -357,9 +385,16 @@ __global__ __launch_bounds__(512, (kChainWaves<T, KP>)) void gdr_chain_kernel(Gd
 
 template <typename T, int KP>
 int launch_prepare(const GdrArgs& a, bool backward, hipStream_t s) {
-  const dim3 grid((unsigned)a.slots, (unsigned)a.Hv);
-  if (backward) hipLaunchKernelGGL((gdr_prepare_kernel<T, KP, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((gdr_prepare_kernel<T, KP, false>), grid, dim3(256), 0, s, a);
+  // Two heads of a group to a workgroup where that still leaves four for each CU; one, for their latency,
+  // where it does not.
+  const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
+  const int heads = a.group % 2 == 0 && a.slots * a.Hv >= 8 * cus ? 2 : 1;
+  const dim3 grid((unsigned)a.slots, (unsigned)(a.Hv / heads)), b(256);
+  const bool full = a.K == KP;
+  if (backward && full) hipLaunchKernelGGL((gdr_prepare_kernel<T, KP, true, true>), grid, b, 0, s, a, heads);
+  else if (backward) hipLaunchKernelGGL((gdr_prepare_kernel<T, KP, true, false>), grid, b, 0, s, a, heads);
+  else if (full) hipLaunchKernelGGL((gdr_prepare_kernel<T, KP, false, true>), grid, b, 0, s, a, heads);
+  else hipLaunchKernelGGL((gdr_prepare_kernel<T, KP, false, false>), grid, b, 0, s, a, heads);
   return check_launch("gdr_prepare_kernel");
 }
 template <typename T, int KP>
