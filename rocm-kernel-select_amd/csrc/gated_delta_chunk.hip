@@ -202,7 +202,7 @@ __device__ __forceinline__ void write_products(const f32x4& lo, const f32x4& hi,
 // computed once for both.  The masked products leave the registers as fragments: a product's result has
 // the layout of its transpose's rows, so Q K^T comes out of K Q^T.  FULL: K is KP.
 template <typename T, int KP, bool BWD, bool FULL>
-__global__ __launch_bounds__(256) void gdr_prepare_kernel(GdrArgs a, int heads) {
+__global__ __launch_bounds__(256, (KP * kParts<T> <= 128 ? 4 : 1)) void gdr_prepare_kernel(GdrArgs a, int heads) {
   constexpr int NP = kParts<T>, KS = KP / 32, PP = BWD ? 3 : kOutParts<T>;
   __shared__ uint4 kl[KS * 4 * NP * 64];  // K's fragments, then Q's
   __shared__ __align__(16) float wm[64 * LD];
