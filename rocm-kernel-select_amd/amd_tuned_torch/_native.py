@@ -1595,6 +1595,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float, residu
     wdt = dt if weight is None else weight.dtype
     key = (M, N, xs, rs, group, eps, dt, wdt, quant)
     if blk[2] != key:
+        blk[2] = None  # until all fields are set
         a.M, a.N, a.x_stride, a.residual_stride, a.group, a.eps = M, N, xs, rs, group, eps
         a.dtype, a.w_dtype, a.quant = _DTYPE_CODE[dt], _DTYPE_CODE[wdt], QUANT_DTYPES.get(quant, 0)
         blk[2] = key
@@ -1639,6 +1640,41 @@ def gated_delta_update(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: tor
     """One token of the gated delta rule for each sequence; `state` (slots, Hv, K, V) fp32 is updated in
     place.  q, k (N, Hk, K), v (N, Hv, V) of one dtype, g and beta (N, Hv) of it or fp32; returns
     (N, Hv, V)."""
+    blk = _block("gdu", _DeltaUpdateArgs)
+    a = blk[0]
+    key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), g.shape, g.stride(), beta.shape, beta.stride(),
+           state.shape, state.stride(), q.dtype, k.dtype, v.dtype, g.dtype, beta.dtype, state.dtype, q.device, k.device,
+           v.device, g.device, beta.device, state.device, scale,
+           None if state_indices is None else (state_indices.shape, state_indices.stride(), state_indices.dtype,
+                                               state_indices.device))
+    if blk[2] != key:
+        _delta_update_check(q, k, v, g, beta, state, state_indices)
+        if q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1 or (
+                state_indices is not None and not state_indices.is_contiguous()):
+            q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+            state_indices = None if state_indices is None else state_indices.contiguous()
+            key = None
+        blk[2] = None  # until all fields are set
+        N, Hk, K = q.shape
+        a.N, a.slots, a.state_stride = N, state.shape[0], state.stride(0)
+        a.q_stride_n, a.q_stride_h = q.stride(0), q.stride(1)
+        a.k_stride_n, a.k_stride_h = k.stride(0), k.stride(1)
+        a.v_stride_n, a.v_stride_h = v.stride(0), v.stride(1)
+        a.g_stride_n, a.g_stride_h = g.stride()
+        a.beta_stride_n, a.beta_stride_h = beta.stride()
+        a.Hk, a.Hv, a.K, a.V, a.scale = Hk, v.shape[1], K, v.shape[2], scale
+        a.dtype, a.g_dtype, a.beta_dtype = _DTYPE_CODE[q.dtype], _DTYPE_CODE[g.dtype], _DTYPE_CODE[beta.dtype]
+        blk[2] = key
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    if a.N == 0:
+        return out
+    a.q, a.k, a.v, a.g, a.beta = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr()
+    a.state, a.out, a.state_indices, a.stream = state.data_ptr(), out.data_ptr(), _ptr(state_indices), _stream(q)
+    _check(lib().atk_gated_delta_update(blk[1]), "gated_delta_rule_update")
+    return out
+
+
+def _delta_update_check(q, k, v, g, beta, state, state_indices) -> None:
     if q.dim() != 3 or v.dim() != 3 or k.shape != q.shape or state.dim() != 4:
         raise RuntimeError("gated_delta_rule_update expects q, k (N, Hk, K), v (N, Hv, V), state (slots, Hv, K, V)")
     N, Hk, K = q.shape
@@ -1646,8 +1682,8 @@ def gated_delta_update(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: tor
     dt, gdt, bdt = q.dtype, g.dtype, beta.dtype
     if v.shape[0] != N or g.shape != (N, Hv) or beta.shape != (N, Hv) or state.shape[1:] != (Hv, K, V):
         raise RuntimeError("gated_delta_rule_update: sizes of v, g, beta and state must agree with q and k")
-    if Hk == 0 or Hv % Hk:
-        raise RuntimeError("gated_delta_rule_update: value heads must be a multiple of key heads")
+    if Hk == 0 or K == 0 or V == 0 or Hv == 0 or Hv % Hk:
+        raise RuntimeError("gated_delta_rule_update: value heads must be a multiple of key heads, and no head empty")
     if dt not in _DTYPE_CODE or k.dtype != dt or v.dtype != dt or gdt not in (dt, torch.float32) \
             or bdt not in (dt, torch.float32) or state.dtype != torch.float32:
         raise RuntimeError("gated_delta_rule_update: q, k and v must share a dtype (float32, float16 or bfloat16), "
@@ -1664,34 +1700,10 @@ def gated_delta_update(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: tor
         raise RuntimeError("gated_delta_rule_update: state_indices must be int32 (N,) on the same GPU")
     if state_indices is None and state.shape[0] != N:
         raise RuntimeError("gated_delta_rule_update: without state_indices the state has one slot a sequence")
-    q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
-    out = torch.empty((N, Hv, V), dtype=dt, device=dev)
-    if out.numel() == 0:
-        return out
-    if state_indices is not None and state_indices.stride(0) != 1:
-        state_indices = state_indices.contiguous()
-    blk = _block("gdu", _DeltaUpdateArgs)
-    a = blk[0]
-    key = (state.shape, state.stride(0), q.shape, V, q.stride(), k.stride(), v.stride(), g.stride(), beta.stride(), dt,
-           gdt, bdt, scale)
-    if blk[2] != key:
-        a.N, a.slots, a.state_stride = N, state.shape[0], state.stride(0)
-        a.q_stride_n, a.q_stride_h = q.stride(0), q.stride(1)
-        a.k_stride_n, a.k_stride_h = k.stride(0), k.stride(1)
-        a.v_stride_n, a.v_stride_h = v.stride(0), v.stride(1)
-        a.g_stride_n, a.g_stride_h = g.stride()
-        a.beta_stride_n, a.beta_stride_h = beta.stride()
-        a.Hk, a.Hv, a.K, a.V, a.scale = Hk, Hv, K, V, scale
-        a.dtype, a.g_dtype, a.beta_dtype = _DTYPE_CODE[dt], _DTYPE_CODE[gdt], _DTYPE_CODE[bdt]
-        blk[2] = key
-    a.q, a.k, a.v, a.g, a.beta = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr()
-    a.state, a.out, a.state_indices, a.stream = state.data_ptr(), out.data_ptr(), _ptr(state_indices), _stream(q)
-    _check(lib().atk_gated_delta_update(blk[1]), "gated_delta_rule_update")
-    return out
 
 
-def _delta_checked(q, k, v, g, beta, initial_state, cu_seqlens):
-    """The tensors of a gated_delta_rule call as the kernels take them, and the number of sequences."""
+def _delta_check(q, k, v, g, beta, initial_state, cu_seqlens) -> int:
+    """Refuses what the kernels do not take; the number of sequences."""
     if q.dim() != 4 or v.dim() != 4 or k.shape != q.shape:
         raise RuntimeError("gated_delta_rule expects q, k (B, T, Hk, K) and v (B, T, Hv, V)")
     B, T, Hk, K = q.shape
@@ -1714,25 +1726,48 @@ def _delta_checked(q, k, v, g, beta, initial_state, cu_seqlens):
             raise RuntimeError("gated_delta_rule: cu_seqlens must be int32 (sequences + 1,) on the same GPU, with a "
                                "batch of one")
         n = cu_seqlens.numel() - 1
-        cu_seqlens = cu_seqlens.contiguous()
-    if initial_state is not None:
-        if initial_state.shape != (n, Hv, K, V) or initial_state.dtype != torch.float32 or initial_state.device != dev:
-            raise RuntimeError("gated_delta_rule: initial_state must be float32 (sequences, Hv, K, V) on the same GPU")
-        initial_state = initial_state.contiguous()
-    q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
-    return q, k, v, g, beta, initial_state, cu_seqlens, n
+    if initial_state is not None and (initial_state.shape != (n, Hv, K, V) or initial_state.dtype != torch.float32
+                                      or initial_state.device != dev):
+        raise RuntimeError("gated_delta_rule: initial_state must be float32 (sequences, Hv, K, V) on the same GPU")
+    return n
 
 
-def _delta_args(q, k, v, g, beta, scale, initial_state, cu_seqlens, n) -> _DeltaArgs:
-    a = _DeltaArgs()
+def _delta_block(q, k, v, g, beta, scale, initial_state, cu_seqlens):
+    """This thread's argument block of a call on sequences, its pointers to the inputs and its stream set:
+    [struct, address, key, sequences, workspace bytes, the backward's, inputs that had to be copied].  What
+    the key holds is checked, and the rest of the struct filled, where it differs from the last call's."""
+    blk = getattr(_tls, "gdr", None)
+    if blk is None:
+        st = _DeltaArgs()
+        blk = _tls.gdr = [st, ctypes.addressof(st), None, 0, 0, 0, None]
+    key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), g.shape, g.stride(), beta.shape, beta.stride(),
+           q.dtype, k.dtype, v.dtype, g.dtype, beta.dtype, q.device, k.device, v.device, g.device, beta.device, scale,
+           None if initial_state is None else (initial_state.shape, initial_state.stride(), initial_state.dtype,
+                                               initial_state.device),
+           None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.stride(), cu_seqlens.dtype, cu_seqlens.device))
+    a = blk[0]
+    blk[6] = None
+    if blk[2] != key:
+        n = _delta_check(q, k, v, g, beta, initial_state, cu_seqlens)
+        if q.stride(3) != 1 or k.stride(3) != 1 or v.stride(3) != 1 or not (
+                (initial_state is None or initial_state.is_contiguous()) and (cu_seqlens is None or cu_seqlens.is_contiguous())):
+            q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
+            initial_state = None if initial_state is None else initial_state.contiguous()
+            cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
+            blk[6] = (q, k, v, initial_state, cu_seqlens)
+            key = None
+        blk[2] = None  # until all fields are set
+        a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+        a.g_stride[:], a.beta_stride[:] = g.stride(), beta.stride()
+        a.N, a.T, a.Hk, a.Hv, a.K, a.V = n, q.shape[1], q.shape[2], v.shape[2], q.shape[3], v.shape[3]
+        a.dtype, a.g_dtype, a.beta_dtype = _DTYPE_CODE[q.dtype], _DTYPE_CODE[g.dtype], _DTYPE_CODE[beta.dtype]
+        a.scale = scale
+        a.cu_seqlens = _ptr(cu_seqlens)  # the sizes below ask whether there are any
+        L = lib()
+        blk[2:6] = [key, n, L.atk_gated_delta_workspace_bytes(blk[1]), L.atk_gated_delta_bwd_workspace_bytes(blk[1])]
     a.q, a.k, a.v, a.g, a.beta = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr()
-    a.initial_state, a.cu_seqlens = _ptr(initial_state), _ptr(cu_seqlens)
-    a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
-    a.g_stride[:], a.beta_stride[:] = g.stride(), beta.stride()
-    a.N, a.T, a.Hk, a.Hv, a.K, a.V = n, q.shape[1], q.shape[2], v.shape[2], q.shape[3], v.shape[3]
-    a.dtype, a.g_dtype, a.beta_dtype = _DTYPE_CODE[q.dtype], _DTYPE_CODE[g.dtype], _DTYPE_CODE[beta.dtype]
-    a.scale, a.stream = scale, _stream(q)
-    return a
+    a.initial_state, a.cu_seqlens, a.stream = _ptr(initial_state), _ptr(cu_seqlens), _stream(q)
+    return blk
 
 
 def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor, scale: float,
@@ -1740,21 +1775,20 @@ def gated_delta(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
                 want_state: bool = False):
     """The gated delta rule over sequences: (out (B, T, Hv, V), final state fp32 (sequences, Hv, K, V) or
     None).  q, k (B, T, Hk, K), v (B, T, Hv, V) of one dtype, g and beta (B, T, Hv) of it or fp32."""
-    q, k, v, g, beta, initial_state, cu_seqlens, n = _delta_checked(q, k, v, g, beta, initial_state, cu_seqlens)
-    B, T, Hv, V = v.shape
-    out = torch.empty((B, T, Hv, V), dtype=v.dtype, device=v.device)
-    final = torch.empty((n, Hv, q.shape[3], V), dtype=torch.float32, device=v.device) if want_state else None
+    blk = _delta_block(q, k, v, g, beta, scale, initial_state, cu_seqlens)
+    a, n, device = blk[0], blk[3], v.device
+    out = torch.empty(v.shape, dtype=v.dtype, device=device)
+    final = torch.empty((n, v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=device) if want_state else None
     if n == 0:
         return out.zero_(), final
     if out.numel() == 0 and final is None:
         return out, final
-    a = _delta_args(q, k, v, g, beta, scale, initial_state, cu_seqlens, n)
-    a.out, a.final_state = out.data_ptr(), _ptr(final)
-    L = lib()
     # scratch of the length of the sequences: from torch's allocator, which gives it back to the stream
-    ws = torch.empty(L.atk_gated_delta_workspace_bytes(ctypes.addressof(a)), dtype=torch.uint8, device=v.device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    _check(L.atk_gated_delta_fwd(ctypes.addressof(a)), "gated_delta_rule")
+    ws = torch.empty(blk[4], dtype=torch.uint8, device=device)
+    a.out, a.final_state, a.workspace, a.workspace_bytes = out.data_ptr(), _ptr(final), ws.data_ptr(), blk[4]
+    rc = lib().atk_gated_delta_fwd(blk[1])
+    blk[6] = None
+    _check(rc, "gated_delta_rule")
     return out, final
 
 
@@ -1762,22 +1796,22 @@ def gated_delta_backward(q, k, v, g, beta, scale: float, initial_state, cu_seqle
                          dfinal: Optional[torch.Tensor], want_dstate: bool):
     """(dq, dk, dv, dg, dbeta, dinitial_state or None) of gated_delta: dout like its output, dfinal (fp32)
     the gradient of its final state or None."""
-    q, k, v, g, beta, initial_state, cu_seqlens, n = _delta_checked(q, k, v, g, beta, initial_state, cu_seqlens)
     if dout.shape != v.shape or dout.dtype != v.dtype or dout.device != v.device:
         raise RuntimeError("gated_delta_rule backward: the gradient must match the output")
+    blk = _delta_block(q, k, v, g, beta, scale, initial_state, cu_seqlens)
+    a, n, device = blk[0], blk[3], v.device
     make = torch.empty if n else torch.zeros
-    grads = [make(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v, g, beta)]
+    grads = [make(t.shape, dtype=t.dtype, device=device) for t in (q, k, v, g, beta)]
     dstate = None
     if want_dstate:
-        dstate = torch.empty((n,) + v.shape[2:3] + (q.shape[3], v.shape[3]), dtype=torch.float32, device=v.device)
+        dstate = torch.empty((n, v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=device)
     if n == 0 or (v.numel() == 0 and dstate is None):
         return (*grads, dstate)
     dout = dout.contiguous()
     dfinal = None if dfinal is None else dfinal.contiguous()
-    a = _delta_args(q, k, v, g, beta, scale, initial_state, cu_seqlens, n)
-    L = lib()
-    ws = torch.empty(L.atk_gated_delta_bwd_workspace_bytes(ctypes.addressof(a)), dtype=torch.uint8, device=v.device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-    _check(L.atk_gated_delta_bwd(ctypes.addressof(a), _ptr(dout), _ptr(dfinal), *(t.data_ptr() for t in grads),
-                                 _ptr(dstate)), "gated_delta_rule backward")
+    ws = torch.empty(blk[5], dtype=torch.uint8, device=device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), blk[5]
+    rc = lib().atk_gated_delta_bwd(blk[1], dout.data_ptr(), _ptr(dfinal), *[t.data_ptr() for t in grads], _ptr(dstate))
+    blk[6] = None
+    _check(rc, "gated_delta_rule backward")
     return (*grads, dstate)
