@@ -201,6 +201,9 @@ __device__ __forceinline__ void write_products(const f32x4& lo, const f32x4& hi,
 // head's group also writes that key head's K, Q and K^T (or K, K^T and Q^T).  K K^T and Q K^T are
 // computed once for both.  The masked products leave the registers as fragments: a product's result has
 // the layout of its transpose's rows, so Q K^T comes out of K Q^T.  FULL: K is KP.
+// Bound by latency: loads, then the products, then the inverse's three dependent steps, then stores
+// (bf16, 8192 tokens, 16 and 32 heads of 128: 65 to 70 us for 224 MB written and 69 read, 4.3 TB/s; one
+// chunk each of 16 heads: 11 us).
 template <typename T, int KP, bool BWD, bool FULL>
 __global__ __launch_bounds__(256, (KP * kParts<T> <= 128 ? 4 : 1)) void gdr_prepare_kernel(GdrArgs a, int heads) {
   constexpr int NP = kParts<T>, KS = KP / 32, PP = BWD ? 3 : kOutParts<T>;
@@ -386,7 +389,8 @@ __global__ __launch_bounds__(512, (kChainWaves<T, KP>)) void gdr_chain_kernel(Gd
 template <typename T, int KP>
 int launch_prepare(const GdrArgs& a, bool backward, hipStream_t s) {
   // Two heads of a group to a workgroup where that still leaves four for each CU; one, for their latency,
-  // where it does not.
+  // where it does not (bf16, K 128, one and two: 16 chunks of 16 heads 15.9 and 19.4 us, 32 of 32 22.0
+  // and 21.0, 64 of 32 36.9 and 32.0, 128 of 32 74.8 and 68.6).
   const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
   const int heads = a.group % 2 == 0 && a.slots * a.Hv >= 8 * cus ? 2 : 1;
   const dim3 grid((unsigned)a.slots, (unsigned)(a.Hv / heads)), b(256);

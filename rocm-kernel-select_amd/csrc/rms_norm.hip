@@ -10,7 +10,9 @@
 // HBM-bound: every input is read and every output written once.  A row stays in registers as fp32
 // between its loads and its stores, so the statistics need no second read; sums and maxima are fp32.
 // TPR threads share a row, VPT vectors of 16 input bytes each: a quarter wave for a head's 128
-// columns (four rows to a wave), one wave up to 2048, a workgroup above.
+// columns (four rows to a wave), one wave up to 2048, a workgroup above.  Measured, bf16: 262144 x 128
+// 20.5 us, 6.5 TB/s; 8192 x 2048 with a residual 22 us (134 MB) and into fp8 by groups of 128 19 to 27
+// (118 MB, part of it from the last-level cache), its backward 24 to 28 us for 134 MB.
 #include "atk_common.h"
 
 namespace atk {
@@ -33,19 +35,42 @@ struct RmsBwdArgs {
   int N, w_f32;
 };
 
-// V elements at p (element alignment only: rows of any width), fp32; zeros from column N on
+// V columns of a row of N from c on, as they are in memory (element alignment only: rows of any width).
+// No branch and no conversion, so a thread's loads are all in flight together: with a branch around each,
+// every load waited for the one before it (8192 x 2048, residual, fp8, 33 us).  What would pass the row's
+// end is loaded from further left.  TINY: rows shorter than V.
 template <typename T, int V>
-__device__ __forceinline__ void load_cols(const T* __restrict__ p, int c, int N, float* o) {
-  if (c + V <= N) {
-    T e[V];
-    __builtin_memcpy(e, p + c, V * sizeof(T));
+struct Cols {
+  T e[V];
+};
+template <typename T, int V, bool TINY>
+__device__ __forceinline__ Cols<T, V> load_raw(const T* __restrict__ p, int c, int N) {
+  Cols<T, V> o;
+  if constexpr (TINY) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = to_f32(e[i]);
+    for (int i = 0; i < V; ++i) o.e[i] = c + i < N ? p[c + i] : static_cast<T>(0.f);
   } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = c + i < N ? to_f32(p[c + i]) : 0.f;
+    __builtin_memcpy(o.e, p + (c < N - V ? c : N - V), V * sizeof(T));
   }
+  return o;
 }
+// In their places, fp32, zeros from column N on.
+template <typename T, int V, bool TINY>
+__device__ __forceinline__ void to_cols(Cols<T, V> r, int c, int N, float* o) {
+  if constexpr (!TINY) {
+    const int past = c + V - N;
+    if (past > 0) {
+      unsigned __int128 u;
+      __builtin_memcpy(&u, r.e, sizeof(u));
+      u = past < V ? u >> (past * (int)sizeof(T) * 8) : 0;
+      __builtin_memcpy(r.e, &u, sizeof(u));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = to_f32(r.e[i]);
+}
+// Loads before this are issued before anything after it.
+__device__ __forceinline__ void loads_issued() { asm volatile("" ::: "memory"); }
 
 template <typename T, int V>
 __device__ __forceinline__ void store_cols(T* __restrict__ p, int c, int N, const float* v) {
@@ -61,17 +86,43 @@ __device__ __forceinline__ void store_cols(T* __restrict__ p, int c, int N, cons
   }
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void load_weight(const void* w, int w_f32, int c, int N, float* o) {
+// The weight's columns of a thread's vectors: of the rows' type they come with the loads of the rows
+// (raw), as fp32 later, for vectors j0 .. j0 + J - 1 at once; ones without a weight.
+template <typename T, int V, bool TINY, int TPR, int J>
+__device__ __forceinline__ void weight_raw(const void* w, int w_f32, int t, int j0, int N, Cols<T, V> (&r)[J]) {
+  if (!w || w_f32) return;
+#pragma unroll
+  for (int j = 0; j < J; ++j) r[j] = load_raw<T, V, TINY>(static_cast<const T*>(w), (t + (j0 + j) * TPR) * V, N);
+}
+template <typename T, int V, bool TINY, int TPR, int J>
+__device__ __forceinline__ void to_weight(const Cols<T, V> (&r)[J], const void* w, int w_f32, int t, int j0, int N,
+                                          float (&o)[J][V]) {
   if (!w) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = 1.f;
-  } else if (w_f32) {
-    load_cols<float, V>(static_cast<const float*>(w), c, N, o);
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[j][i] = 1.f;
+  } else if (!w_f32) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) to_cols<T, V, TINY>(r[j], (t + (j0 + j) * TPR) * V, N, o[j]);
   } else {
-    load_cols<T, V>(static_cast<const T*>(w), c, N, o);
+    Cols<float, 4> e[J][V / 4];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i)
+        e[j][i] = load_raw<float, 4, TINY>(static_cast<const float*>(w), (t + (j0 + j) * TPR) * V + 4 * i, N);
+    loads_issued();
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i)
+        to_cols<float, 4, TINY>(e[j][i], (t + (j0 + j) * TPR) * V + 4 * i, N, o[j] + 4 * i);
   }
 }
+// How many vectors at once: a workgroup of 1024 has 128 registers a thread.
+template <int TPR, int VPT>
+inline constexpr int kTogether = TPR == 1024 ? 1 : VPT;
 
 // Sum over the TPR threads of a row, the same in each of them.  Order fixed.  TPR > 64 uses `red`
 // (one float a wave) and has two barriers.
@@ -141,28 +192,49 @@ __device__ __forceinline__ void store_q(uint8_t* __restrict__ p, int c, int N, c
   }
 }
 
-template <typename T, int Q, int TPR, int VPT>
+template <typename T, int Q, int TPR, int VPT, bool RES>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsArgs a) {
   constexpr int V = 16 / sizeof(T), NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
+  constexpr bool TINY = TPR == 8;
   __shared__ float red[NT / 64];
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
   const bool live = row < a.M;  // a dead row takes part in its wave's reductions, and stores nothing
   const T* __restrict__ x = static_cast<const T*>(a.x) + (live ? row : 0) * a.x_stride;
+  constexpr int J = kTogether<TPR, VPT>;
+  // (opaque where vectors take turns: the compiler would keep all of their addresses in registers)
+  const auto lane = [&] {
+    int u = t;
+    if constexpr (J < VPT) asm volatile("" : "+v"(u));
+    return u;
+  };
   float f[VPT][V];
+  Cols<T, V> wr[J];
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) load_cols<T, V>(x, (t + j * TPR) * V, a.N, f[j]);
-  if (a.r) {
-    const T* __restrict__ r = static_cast<const T*>(a.r) + (live ? row : 0) * a.r_stride;
-    T* __restrict__ h = static_cast<T*>(a.h) + row * a.N;
+  for (int j0 = 0; j0 < VPT; j0 += J) {
+    const int t = lane();
+    Cols<T, V> xr[J], rr[J];
 #pragma unroll
-    for (int j = 0; j < VPT; ++j) {
-      float g[V];
-      load_cols<T, V>(r, (t + j * TPR) * V, a.N, g);
-      // the norm is of h as it is stored: one rounding, the stream's own
+    for (int j = 0; j < J; ++j) xr[j] = load_raw<T, V, TINY>(x, (t + (j0 + j) * TPR) * V, a.N);
+    if constexpr (RES) {
+      const T* __restrict__ r = static_cast<const T*>(a.r) + (live ? row : 0) * a.r_stride;
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[j][i] = to_f32(from_f32<T>(f[j][i] + g[i]));
-      if (live) store_cols<T, V>(h, (t + j * TPR) * V, a.N, f[j]);
+      for (int j = 0; j < J; ++j) rr[j] = load_raw<T, V, TINY>(r, (t + (j0 + j) * TPR) * V, a.N);
+    }
+    if constexpr (J == VPT) weight_raw<T, V, TINY, TPR>(a.w, a.w_f32, t, 0, a.N, wr);
+    loads_issued();
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int c = (t + (j0 + j) * TPR) * V;
+      to_cols<T, V, TINY>(xr[j], c, a.N, f[j0 + j]);
+      if constexpr (RES) {
+        float g[V];
+        to_cols<T, V, TINY>(rr[j], c, a.N, g);
+        // the norm is of h as it is stored: one rounding, the stream's own
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[j0 + j][i] = to_f32(from_f32<T>(f[j0 + j][i] + g[i]));
+        if (live) store_cols<T, V>(static_cast<T*>(a.h) + row * a.N, c, a.N, f[j0 + j]);
+      }
     }
   }
   float ss = 0.f;
@@ -173,18 +245,22 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsArgs 
   ss = row_sum<TPR>(ss, red);
   const float rstd = rsqrtf(ss / (float)a.N + a.eps);
   if (a.rstd && live && t == 0) a.rstd[row] = rstd;
+  #pragma unroll
+  for (int j0 = 0; j0 < VPT; j0 += J) {
+    const int t = lane();
+    float w[J][V];
+    if constexpr (J < VPT) weight_raw<T, V, TINY, TPR>(a.w, a.w_f32, t, j0, a.N, wr);
+    to_weight<T, V, TINY, TPR>(wr, a.w, a.w_f32, t, j0, a.N, w);
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    float w[V];
-    load_weight<T, V>(a.w, a.w_f32, (t + j * TPR) * V, a.N, w);
+    for (int j = 0; j < J; ++j)
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[j][i] = f[j][i] * rstd * w[i];
+      for (int i = 0; i < V; ++i) f[j0 + j][i] = f[j0 + j][i] * rstd * w[j][i];
   }
   if constexpr (Q == kQNone) {
     T* __restrict__ y = static_cast<T*>(a.y) + row * a.N;
     if (live) {
 #pragma unroll
-      for (int j = 0; j < VPT; ++j) store_cols<T, V>(y, (t + j * TPR) * V, a.N, f[j]);
+      for (int j = 0; j < VPT; ++j) store_cols<T, V>(y, (lane() + j * TPR) * V, a.N, f[j]);
     }
   } else {
     constexpr float top = Q == kQFp8 ? 448.f : 127.f;
@@ -203,7 +279,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsArgs 
       if (!live) return;
       if (t == 0) a.scales[row] = scale;
 #pragma unroll
-      for (int j = 0; j < VPT; ++j) store_q<Q, V>(y, (t + j * TPR) * V, a.N, f[j], inv);
+      for (int j = 0; j < VPT; ++j) store_q<Q, V>(y, (lane() + j * TPR) * V, a.N, f[j], inv);
     } else {
       // a group is a run of group / V lanes (both powers of two, at most TPR and 64; host check)
       const int lanes = a.group / V;
@@ -211,7 +287,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsArgs 
       for (int j = 0; j < VPT; ++j) {
         for (int off = lanes >> 1; off >= 1; off >>= 1) amax[j] = fmaxf(amax[j], __shfl_xor(amax[j], off, 64));
         const float scale = fmaxf(amax[j] / top, 0x1p-126f), inv = 1.f / scale;
-        const int c = (t + j * TPR) * V;
+        const int c = (lane() + j * TPR) * V;
         if (live && c < a.N) {
           if (t % lanes == 0) a.scales[row * a.groups + c / a.group] = scale;
           store_q<Q, V>(y, c, a.N, f[j], inv);
@@ -223,20 +299,24 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsArgs 
 
 // dx for every row, and the sum of dy h rstd over this workgroup's rows (every gridDim.x-th row
 // group) in dw_part[workgroup][N].  The rows of a workgroup are summed in a fixed order, so equal
-// inputs give equal bits.
+// inputs give equal bits.  HBM-bound as the forward.
 template <typename T, int TPR, int VPT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwdArgs a) {
   constexpr int V = 16 / sizeof(T), NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
+  constexpr bool TINY = TPR == 8;
   __shared__ float red[NT / 64];
   __shared__ float acc[RPB > 1 ? (RPB - 1) * TPR * VPT * V : 1];
   const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
   float w[VPT][V], dw[VPT][V];
+  {
+    Cols<T, V> wr[VPT];
+    weight_raw<T, V, TINY, TPR>(a.w, a.w_f32, t, 0, a.N, wr);
+    to_weight<T, V, TINY, TPR>(wr, a.w, a.w_f32, t, 0, a.N, w);
+  }
 #pragma unroll
-  for (int j = 0; j < VPT; ++j) {
-    load_weight<T, V>(a.w, a.w_f32, (t + j * TPR) * V, a.N, w[j]);
+  for (int j = 0; j < VPT; ++j)
 #pragma unroll
     for (int i = 0; i < V; ++i) dw[j][i] = 0.f;
-  }
   for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < a.M; row0 += (int64_t)gridDim.x * RPB) {
     const int64_t row = row0 + slot;
     const bool live = row < a.M;
@@ -244,14 +324,23 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwdAr
     const T* __restrict__ h = static_cast<const T*>(a.h) + rl * a.h_stride;
     const T* __restrict__ dy = static_cast<const T*>(a.dy) + rl * a.dy_stride;
     float f[VPT][V], g[VPT][V], s = 0.f;
+    Cols<T, V> hr[VPT], yr[VPT], er[VPT];
 #pragma unroll
     for (int j = 0; j < VPT; ++j) {
-      load_cols<T, V>(h, (t + j * TPR) * V, a.N, f[j]);
-      load_cols<T, V>(dy, (t + j * TPR) * V, a.N, g[j]);
+      hr[j] = load_raw<T, V, TINY>(h, (t + j * TPR) * V, a.N);
+      yr[j] = load_raw<T, V, TINY>(dy, (t + j * TPR) * V, a.N);
     }
     const float rstd = a.rstd[rl];
+    const T* __restrict__ dh = static_cast<const T*>(a.dh) + rl * a.dh_stride;
+    if (TPR < 512 && a.dh) {  // (late where a workgroup's size leaves few registers)
 #pragma unroll
-    for (int j = 0; j < VPT; ++j)
+      for (int j = 0; j < VPT; ++j) er[j] = load_raw<T, V, TINY>(dh, (t + j * TPR) * V, a.N);
+    }
+    loads_issued();
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+      to_cols<T, V, TINY>(hr[j], (t + j * TPR) * V, a.N, f[j]);
+      to_cols<T, V, TINY>(yr[j], (t + j * TPR) * V, a.N, g[j]);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
         f[j][i] *= rstd;
@@ -259,6 +348,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwdAr
         g[j][i] *= w[j][i];
         s += g[j][i] * f[j][i];
       }
+    }
     s = row_sum<TPR>(s, red) / (float)a.N;
     if (live) {
       T* __restrict__ dx = static_cast<T*>(a.dx) + row * a.N;
@@ -266,7 +356,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwdAr
       for (int j = 0; j < VPT; ++j) {
         float e[V];
         if (a.dh) {
-          load_cols<T, V>(static_cast<const T*>(a.dh) + row * a.dh_stride, (t + j * TPR) * V, a.N, e);
+          if (TPR >= 512) er[j] = load_raw<T, V, TINY>(dh, (t + j * TPR) * V, a.N);
+          to_cols<T, V, TINY>(er[j], (t + j * TPR) * V, a.N, e);
         } else {
 #pragma unroll
           for (int i = 0; i < V; ++i) e[i] = 0.f;
@@ -299,19 +390,20 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwdAr
 }
 
 // dw[c] = sum of part[0..P)[c], rounded once to the weight's type: 64 columns a workgroup, 16 threads
-// to 4 columns, joined in a fixed order
-template <typename WT>
+// to 4 columns, joined in a fixed order (512 parts of 2048 columns: 4.1 us; 20 with a thread to a column)
+template <typename WT, bool TINY>
 __global__ __launch_bounds__(256) void rms_dw_kernel(const float* __restrict__ part, WT* __restrict__ dw, int P, int N) {
   __shared__ float s[16][65];
   const int c = blockIdx.x * 64 + threadIdx.x % 16 * 4, k = threadIdx.x / 16;
-  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  Cols<float, 4> sum = {};
 #pragma unroll 8
   for (int p = k; p < P; p += 16) {
-    float e[4];
-    load_cols<float, 4>(part + (int64_t)p * N, c, N, e);
+    const Cols<float, 4> e = load_raw<float, 4, TINY>(part + (int64_t)p * N, c, N);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] += e[i];
+    for (int i = 0; i < 4; ++i) sum.e[i] += e.e[i];
   }
+  float v[4];
+  to_cols<float, 4, TINY>(sum, c, N, v);
 #pragma unroll
   for (int i = 0; i < 4; ++i) s[k][threadIdx.x % 16 * 4 + i] = v[i];
   __syncthreads();
@@ -323,31 +415,38 @@ __global__ __launch_bounds__(256) void rms_dw_kernel(const float* __restrict__ p
   }
 }
 
-// Threads to a row and vectors to a thread for rows of nv vectors.
+// Threads to a row and vectors to a thread.
 struct RmsShape {
   int tpr, vpt;
 };
-// Few rows leave most of the chip without one: there a row of over 64 vectors is a workgroup's.
-RmsShape rms_shape(int64_t nv, int64_t rows) {
+// Few rows leave most of the chip without one: there a row of over 128 vectors is a workgroup's (bf16,
+// residual, fp8; a wave's against a workgroup's.  2048 columns: 64 rows 4.8 and 3.6 us, 1024 rows 5.8
+// and 5.5, 2048 rows 7.4 and 7.7; 1024 columns: 64 rows 3.7 and 3.8, 1024 rows 4.4 and 5.3).
+RmsShape rms_shape(int64_t N, int vec, int64_t rows) {
+  if (N < vec) return {8, 1};
+  const int64_t nv = (N + vec - 1) / vec;
   if (nv <= 16) return {16, 1};
   if (nv <= 64) return {64, 1};
-  if (nv <= 256 && rows <= 1024) return {256, 1};
   if (nv <= 128) return {64, 2};
+  if (nv <= 256 && rows <= 1024) return {256, 1};
   if (nv <= 256) return {64, 4};
   if (nv <= 512) return {256, 2};
   if (nv <= 1024) return {256, 4};
-  if (nv <= 4096) return {1024, 4};
+  if (nv <= 2048) return {256, 8};
+  if (nv <= 4096) return {512, 8};
   return {1024, 8};
 }
 
-#define ATK_RMS_SHAPES(X) X(16, 1) X(64, 1) X(64, 2) X(64, 4) X(256, 1) X(256, 2) X(256, 4) X(1024, 4) X(1024, 8)
+#define ATK_RMS_SHAPES(X) X(8, 1) X(16, 1) X(64, 1) X(64, 2) X(64, 4) X(256, 1) X(256, 2) X(256, 4) X(256, 8) X(512, 8) X(1024, 8)
 
 template <typename T, int Q>
 int launch_fwd(const RmsArgs& a, RmsShape sh, hipStream_t s) {
 #define X(TPR, VPT)                                                                                     \
   if (sh.tpr == TPR && sh.vpt == VPT) {                                                                 \
     constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;                                           \
-    hipLaunchKernelGGL((rms_fwd_kernel<T, Q, TPR, VPT>), dim3((unsigned)((a.M + RPB - 1) / RPB)), dim3(NT), 0, s, a); \
+    const dim3 grid((unsigned)((a.M + RPB - 1) / RPB));                                                 \
+    if (a.r) hipLaunchKernelGGL((rms_fwd_kernel<T, Q, TPR, VPT, true>), grid, dim3(NT), 0, s, a);       \
+    else hipLaunchKernelGGL((rms_fwd_kernel<T, Q, TPR, VPT, false>), grid, dim3(NT), 0, s, a);          \
     return check_launch("rms_fwd_kernel");                                                              \
   }
   ATK_RMS_SHAPES(X)
@@ -365,6 +464,13 @@ int launch_bwd(const RmsBwdArgs& a, RmsShape sh, int grid, hipStream_t s) {
   ATK_RMS_SHAPES(X)
 #undef X
   return fail(ATK_UNSUPPORTED, "rms_norm backward: no kernel for this row width");
+}
+
+template <typename WT>
+void launch_dw(const float* part, void* dw, int P, int N, hipStream_t s) {
+  const dim3 g((unsigned)((N + 63) / 64));
+  if (N >= 4) hipLaunchKernelGGL((rms_dw_kernel<WT, false>), g, dim3(256), 0, s, part, static_cast<WT*>(dw), P, N);
+  else hipLaunchKernelGGL((rms_dw_kernel<WT, true>), g, dim3(256), 0, s, part, static_cast<WT*>(dw), P, N);
 }
 
 template <int Q>
@@ -388,11 +494,13 @@ int check_rows(const char* what, int64_t M, int64_t N, int dtype, int w_dtype, b
 }
 
 // Workgroups of the backward: enough to fill the chip, few enough that the partial sums of dw stay
-// small beside the rows (each workgroup writes one row of fp32).
-int bwd_grid(int64_t M, int tpr) {
-  const int rpb = tpr < 256 ? 256 / tpr : 1;
+// small beside the rows (each workgroup writes one row of fp32).  With dw's sum, at one, two and four to a
+// CU, bf16: 8192 x 2048 26.5, 22.7 and 25.4 us; 8192 x 8192 93.9, 75.0 and 80.3; 65536 x 128 20.4, 15.7
+// and 15.4; where one fills a CU's registers, 1024 x 16384, 30.9, 37.0 and 49.6.
+int bwd_grid(int64_t M, RmsShape sh) {
+  const int rpb = sh.tpr < 256 ? 256 / sh.tpr : 1;
   const int cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  const int64_t most = (int64_t)cus * (tpr > 256 ? 1 : 2), need = (M + rpb - 1) / rpb;
+  const int64_t most = (int64_t)cus * (sh.vpt >= 8 ? 1 : 2), need = (M + rpb - 1) / rpb;
   return (int)(need < most ? need : most);
 }
 
@@ -421,7 +529,7 @@ extern "C" int atk_rms_norm_fwd(const atk_rms_norm_args* p) {
   a.x = p->x; a.r = p->residual; a.w = p->weight; a.y = p->y; a.h = p->h; a.rstd = p->rstd; a.scales = p->scales;
   a.M = M; a.x_stride = p->x_stride; a.r_stride = p->residual_stride;
   a.N = (int)N; a.group = group; a.w_f32 = p->w_dtype == ATK_F32; a.eps = p->eps;
-  const RmsShape sh = rms_shape((N + vec - 1) / vec, M);
+  const RmsShape sh = rms_shape(N, vec, M);
   hipStream_t s = reinterpret_cast<hipStream_t>(p->stream);
   if (quant == ATK_QUANT_FP8) return launch_fwd_typed<kQFp8>(a, dtype, sh, s);
   if (quant == ATK_QUANT_INT8) return launch_fwd_typed<kQInt8>(a, dtype, sh, s);
@@ -432,7 +540,7 @@ extern "C" size_t atk_rms_norm_bwd_workspace_bytes(int64_t M, int64_t N, int dty
   using namespace atk;
   if (check_rows("rms_norm backward", M, N, dtype, dtype, false) || M == 0 || N == 0) return 0;
   const int vec = 16 / (int)dtype_size(dtype);
-  return (size_t)bwd_grid(M, rms_shape((N + vec - 1) / vec, M).tpr) * (size_t)N * sizeof(float);
+  return (size_t)bwd_grid(M, rms_shape(N, vec, M)) * (size_t)N * sizeof(float);
 }
 
 extern "C" int atk_rms_norm_bwd(const void* h, const void* dy, const void* dh, const void* weight, const float* rstd,
@@ -446,8 +554,8 @@ extern "C" int atk_rms_norm_bwd(const void* h, const void* dy, const void* dh, c
   if (M > 1 && (h_stride < N || dy_stride < N || (dh && dh_stride < N)))
     return fail(ATK_EINVAL, "rms_norm backward: rows overlap");
   const int vec = 16 / (int)dtype_size(dtype);
-  const RmsShape sh = rms_shape((N + vec - 1) / vec, M);
-  const int grid = bwd_grid(M, sh.tpr);
+  const RmsShape sh = rms_shape(N, vec, M);
+  const int grid = bwd_grid(M, sh);
   if (dw && (!workspace || workspace_bytes < (size_t)grid * (size_t)N * sizeof(float)))
     return fail(ATK_EINVAL, "rms_norm backward: workspace too small");
   RmsBwdArgs a;
@@ -459,12 +567,8 @@ extern "C" int atk_rms_norm_bwd(const void* h, const void* dy, const void* dh, c
   int rc = dtype == ATK_F32 ? launch_bwd<float>(a, sh, grid, s)
            : dtype == ATK_F16 ? launch_bwd<_Float16>(a, sh, grid, s) : launch_bwd<__bf16>(a, sh, grid, s);
   if (rc || !dw) return rc;
-  const dim3 g((unsigned)((N + 63) / 64));
-  if (w_dtype == ATK_F32)
-    hipLaunchKernelGGL((rms_dw_kernel<float>), g, dim3(256), 0, s, a.dw_part, static_cast<float*>(dw), grid, (int)N);
-  else if (w_dtype == ATK_F16)
-    hipLaunchKernelGGL((rms_dw_kernel<_Float16>), g, dim3(256), 0, s, a.dw_part, static_cast<_Float16*>(dw), grid, (int)N);
-  else
-    hipLaunchKernelGGL((rms_dw_kernel<__bf16>), g, dim3(256), 0, s, a.dw_part, static_cast<__bf16*>(dw), grid, (int)N);
+  if (w_dtype == ATK_F32) launch_dw<float>(a.dw_part, dw, grid, (int)N, s);
+  else if (w_dtype == ATK_F16) launch_dw<_Float16>(a.dw_part, dw, grid, (int)N, s);
+  else launch_dw<__bf16>(a.dw_part, dw, grid, (int)N, s);
   return check_launch("rms_dw_kernel");
 }
