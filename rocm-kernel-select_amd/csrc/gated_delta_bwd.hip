@@ -29,8 +29,8 @@ __device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float
 
 // The chain of dS', built as the forward's: four waves pass the state's gradient on, 16 value columns
 // of it; four more make what needs dO alone, a chunk ahead: scale P^T dO and Q^T (scale exp(G) dO).
-// Bound by a step's time too: 2048 tokens, 2 x 16 heads of 128 x 128 bf16, 32 steps in 95 us, 3 us each
-// (it writes dS' and dR of every chunk, 50 KB a step and workgroup less than it reads).
+// Bound by a step's time too, with the forward chain after it: 2048 tokens, 2 x 16 heads of 128 x 128 bf16,
+// twice 32 steps in 160 us, matrix units 12 % busy, 84 MB read and 197 MB written.
 // FULL as there.
 template <typename T, int KP>
 struct GdrBwdLds {
@@ -410,9 +410,9 @@ __device__ __forceinline__ float row16_sum(float v) {
 // fragments of their transposes, and, element by element, as their own.  K^T's and Q^T's fragments
 // hold for each lane the elements that its accumulators have, so the row products of dG need no more
 // loads.  V8: value columns come in eights, so a lane's are all there or all not.
-// Bound by LDS and its own splitting into parts, one workgroup a CU: 64 chunks of 16 heads of 128 x 128
-// bf16 in 92 us, 200 MB read (2.2 TB/s), 19 GFLOP of the six-product kind.  With four waves and S and
-// dS' through LDS it took 257.
+// Bound by latency, one workgroup a CU and waves that wait about half of their time: 64 chunks, 8 and 16
+// heads of 128 x 128, bf16, in 93 us, 126 MB read and 39 MB written, matrix units 24 % busy.  (With four
+// waves, and S and dS' through LDS, 257 us.)
 template <typename T, int KP, bool V8>
 __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
   constexpr int NP = kParts<T>, KS = KP / 32, W = 8, NT = KP > 128 ? KP / 128 : 1;

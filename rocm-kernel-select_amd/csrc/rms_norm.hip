@@ -10,9 +10,9 @@
 // HBM-bound: every input is read and every output written once.  A row stays in registers as fp32
 // between its loads and its stores, so the statistics need no second read; sums and maxima are fp32.
 // TPR threads share a row, VPT vectors of 16 input bytes each: a quarter wave for a head's 128
-// columns (four rows to a wave), one wave up to 2048, a workgroup above.  Measured, bf16: 262144 x 128
-// 20.5 us, 6.5 TB/s; 8192 x 2048 with a residual 22 us (134 MB) and into fp8 by groups of 128 19 to 27
-// (118 MB, part of it from the last-level cache), its backward 24 to 28 us for 134 MB.
+// columns (four rows to a wave), one wave up to 2048, a workgroup above.  Measured, bf16, no input in any
+// cache: 8192 x 2048 with a residual 25 us for 134 MB, into fp8 by groups of 128 27 us for 118 MB, the
+// backward with dw 32 us for 134 MB; 262144 x 128 23 us for 134 MB, 5.8 TB/s.
 #include "atk_common.h"
 
 namespace atk {
@@ -124,32 +124,58 @@ __device__ __forceinline__ void to_weight(const Cols<T, V> (&r)[J], const void* 
 template <int TPR, int VPT>
 inline constexpr int kTogether = TPR == 1024 ? 1 : VPT;
 
-// Sum over the TPR threads of a row, the same in each of them.  Order fixed.  TPR > 64 uses `red`
-// (one float a wave) and has two barriers.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-  if constexpr (TPR == 64) return wave_sum_rows(v);
-  if constexpr (TPR < 64) {
-#pragma unroll
-    for (int off = TPR / 2; off >= 1; off >>= 1) v += __shfl_xor(v, off, 64);
-    return v;
-  }
-  return block_sum<TPR>(v, red);
+// Over each run of L lanes (a power of two up to 64), the same in each of them, order fixed; lane
+// exchanges up to 16 lanes need no LDS.  Every lane of the wave takes part.
+template <int L, typename F>
+__device__ __forceinline__ float lanes_reduce(float v, F f) {
+  if constexpr (L >= 2) v = f(v, dpp_mov<0xB1>(v));   // lane ^ 1
+  if constexpr (L >= 4) v = f(v, dpp_mov<0x4E>(v));   // lane ^ 2
+  if constexpr (L >= 8) v = f(v, dpp_mov<0x141>(v));  // mirrored in 8, whose fours have one value each
+  if constexpr (L >= 16) v = f(v, dpp_mov<0x140>(v));
+  if constexpr (L >= 32) v = f(v, __shfl_xor(v, 16, 64));
+  if constexpr (L >= 64) v = f(v, __shfl_xor(v, 32, 64));
+  return v;
 }
-
-template <int TPR>
-__device__ __forceinline__ float row_max(float v, float* red) {
-#pragma unroll
-  for (int off = (TPR < 64 ? TPR : 64) / 2; off >= 1; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+struct Max {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct Add {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+// Over the TPR threads of a row.  TPR > 64 uses `red` (one float a wave), which the next call but one may
+// use again, and has one barrier.
+template <int TPR, typename F>
+__device__ __forceinline__ float row_reduce(float v, float* red, F f) {
+  v = lanes_reduce<TPR < 64 ? TPR : 64>(v, f);
   if constexpr (TPR > 64) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int i = 1; i < TPR / 64; ++i) v = fmaxf(v, red[i]);
-    __syncthreads();
+    for (int i = 1; i < TPR / 64; ++i) v = f(v, red[i]);
   }
   return v;
+}
+// v[0..N) each over runs of `lanes` lanes
+template <int N>
+__device__ __forceinline__ void group_max(float (&v)[N], int lanes) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = lanes_reduce<2>(v[j], Max());
+  if (lanes >= 4)
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], dpp_mov<0x4E>(v[j]));
+  if (lanes >= 8)
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], dpp_mov<0x141>(v[j]));
+  if (lanes >= 16)
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], dpp_mov<0x140>(v[j]));
+  if (lanes >= 32)
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], __shfl_xor(v[j], 16, 64));
+  if (lanes >= 64)
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], __shfl_xor(v[j], 32, 64));
 }
 
 // two values into the low or high half of `old` as fp8 e4m3, nearest even; beyond +-448 saturates,
@@ -196,7 +222,7 @@ template <typename T, int Q, int TPR, int VPT, bool RES>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsArgs a) {
   constexpr int V = 16 / sizeof(T), NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
   constexpr bool TINY = TPR == 8;
-  __shared__ float red[NT / 64];
+  __shared__ float red[2][NT / 64];
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / TPR;
   const bool live = row < a.M;  // a dead row takes part in its wave's reductions, and stores nothing
@@ -242,7 +268,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsArgs 
   for (int j = 0; j < VPT; ++j)
 #pragma unroll
     for (int i = 0; i < V; ++i) ss += f[j][i] * f[j][i];
-  ss = row_sum<TPR>(ss, red);
+  ss = row_reduce<TPR>(ss, red[0], Add());
   const float rstd = rsqrtf(ss / (float)a.N + a.eps);
   if (a.rstd && live && t == 0) a.rstd[row] = rstd;
   #pragma unroll
@@ -275,7 +301,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsArgs 
     if (a.groups == 1) {
 #pragma unroll
       for (int j = 1; j < VPT; ++j) amax[0] = fmaxf(amax[0], amax[j]);
-      const float scale = fmaxf(row_max<TPR>(amax[0], red) / top, 0x1p-126f), inv = 1.f / scale;
+      const float scale = fmaxf(row_reduce<TPR>(amax[0], red[1], Max()) / top, 0x1p-126f), inv = 1.f / scale;
       if (!live) return;
       if (t == 0) a.scales[row] = scale;
 #pragma unroll
@@ -283,9 +309,9 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsArgs 
     } else {
       // a group is a run of group / V lanes (both powers of two, at most TPR and 64; host check)
       const int lanes = a.group / V;
+      group_max(amax, lanes);
 #pragma unroll
       for (int j = 0; j < VPT; ++j) {
-        for (int off = lanes >> 1; off >= 1; off >>= 1) amax[j] = fmaxf(amax[j], __shfl_xor(amax[j], off, 64));
         const float scale = fmaxf(amax[j] / top, 0x1p-126f), inv = 1.f / scale;
         const int c = (lane() + j * TPR) * V;
         if (live && c < a.N) {
@@ -304,7 +330,7 @@ template <typename T, int TPR, int VPT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwdArgs a) {
   constexpr int V = 16 / sizeof(T), NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;
   constexpr bool TINY = TPR == 8;
-  __shared__ float red[NT / 64];
+  __shared__ float red[2][NT / 64];
   __shared__ float acc[RPB > 1 ? (RPB - 1) * TPR * VPT * V : 1];
   const int t = threadIdx.x % TPR, slot = threadIdx.x / TPR;
   float w[VPT][V], dw[VPT][V];
@@ -317,6 +343,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwdAr
   for (int j = 0; j < VPT; ++j)
 #pragma unroll
     for (int i = 0; i < V; ++i) dw[j][i] = 0.f;
+  int turn = 0;
   for (int64_t row0 = (int64_t)blockIdx.x * RPB; row0 < a.M; row0 += (int64_t)gridDim.x * RPB) {
     const int64_t row = row0 + slot;
     const bool live = row < a.M;
@@ -349,7 +376,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_bwd_kernel(RmsBwdAr
         s += g[j][i] * f[j][i];
       }
     }
-    s = row_sum<TPR>(s, red) / (float)a.N;
+    s = row_reduce<TPR>(s, red[turn], Add()) / (float)a.N;
+    turn ^= 1;
     if (live) {
       T* __restrict__ dx = static_cast<T*>(a.dx) + row * a.N;
 #pragma unroll
