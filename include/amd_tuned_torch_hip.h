@@ -594,8 +594,7 @@ int atk_conv_fwd_prepacked_args(const atk_conv_prepacked_args* a);
 
 /* ---------------------------------------------------------------------------
  * Root-mean-square norm over the last axis, with the residual's addition in front and an 8-bit
- * output behind (the reference's norms of this kind are Triton and TransformerEngine tiers,
- * amd_tuned_torch/fused_norm_ops.py, te_ops.py):
+ * output behind:
  *   h = x + residual, rounded to `dtype`      (residual NULL: h = x, and h is not written)
  *   y = h * rstd * weight,  rstd = 1 / sqrt(mean(h^2) + eps)            (weight NULL: ones)
  * x, residual: M rows of N elements, rows x_stride / residual_stride elements apart; y and h dense.

@@ -7,10 +7,8 @@
 
 h = x + residual, rounded to x's dtype: the residual stream as the next layers read it, and what
 is normalised.  y = h / sqrt(mean(h^2) + eps) * weight.  q * scales stands for y: fp8 e4m3 or
-int8, a scale for each row (its last axis 1) or for each run of `group_size` columns.  The norms
-of this kind in the reference are Triton and TransformerEngine tiers (amd_tuned_torch/
-fused_norm_ops.py, te_ops.py); here they are the library's kernels, on CUDA tensors of any row
-width up to 65536 (float32: 32768) and any row alignment.  `rms_norm` is differentiable;
+int8, a scale for each row (its last axis 1) or for each run of `group_size` columns.  GPU tensors
+of any row width up to 65536 (float32: 32768) and any row alignment.  `rms_norm` is differentiable;
 `rms_norm_quant` is for inference and records no gradient.
 """
 from __future__ import annotations

@@ -202,7 +202,7 @@ __device__ __forceinline__ void write_products(const f32x4& lo, const f32x4& hi,
 // computed once for both.  The masked products leave the registers as fragments: a product's result has
 // the layout of its transpose's rows, so Q K^T comes out of K Q^T.  FULL: K is KP.
 // Bound by latency: loads, then the products, then the inverse's three dependent steps, then stores
-// (bf16, 8192 tokens, 16 and 32 heads of 128: 65 to 70 us for 224 MB written and 69 read, 4.3 TB/s; one
+// (bf16, 8192 tokens, 16 and 32 heads of 128: 65 to 70 us for 224 MB written and 67 read, 4.3 TB/s; one
 // chunk each of 16 heads: 11 us).
 template <typename T, int KP, bool BWD, bool FULL>
 __global__ __launch_bounds__(256, (KP * kParts<T> <= 128 ? 4 : 1)) void gdr_prepare_kernel(GdrArgs a, int heads) {
