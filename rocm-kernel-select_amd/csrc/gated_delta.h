@@ -84,6 +84,23 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// A gate or strength, of T or fp32, as two halves of 16 bits (an fp32 one's low and high): no branch on
+// the type around the load, which would make the loads before and after it wait for each other.
+struct GdrGate {
+  unsigned short lo, hi;
+};
+__device__ __forceinline__ GdrGate gdr_gate_load(const void* p, int dtype, int64_t i) {
+  const int wide = dtype == ATK_F32;
+  const unsigned short* at = static_cast<const unsigned short*>(p) + (i << wide);
+  return {at[0], at[wide]};
+}
+template <typename T>
+__device__ __forceinline__ float gdr_gate(GdrGate v, int dtype) {
+  if constexpr (sizeof(T) == 2)
+    if (dtype != ATK_F32) return to_f32(__builtin_bit_cast(T, v.lo));
+  return __uint_as_float((unsigned)v.hi << 16 | v.lo);
+}
+
 // bf16 parts that hold an input exactly
 template <typename T> inline constexpr int kParts = sizeof(T) == 4 ? 3 : 2;
 template <> inline constexpr int kParts<__bf16> = 1;

@@ -7,8 +7,8 @@
 // in registers in between.  Both products over K are taken in the same pass over S, since
 // S'^T q = exp(g) S^T q + (k . q) u; the one reduction across the workgroup carries both and k . q.
 // The state is loaded and stored past the caches' replacement (nontemporal): by the next step every
-// other layer has gone through them.  64 sequences, 32 heads, 128 x 128: 50.2 us for 268 MB, 5.3 TB/s
-// (58.2 us with plain accesses).
+// other layer has gone through them.  64 sequences, 32 heads, 128 x 128: 46 to 48 us for 268 MB, 5.7 TB/s
+// (50.2 us with small loads that waited for each other, 58.2 with plain state accesses as well).
 #include "gated_delta.h"
 
 namespace atk {
@@ -37,11 +37,26 @@ __global__ __launch_bounds__(256) void gdr_step_kernel(GdrStepArgs a) {
     return;
   }
   float* __restrict__ S = a.state + slot * a.state_stride + (int64_t)h * a.K * a.V;
+  // All loads at once, none in a branch that converts: the small ones first, the state while they arrive.
+  const T* __restrict__ k = static_cast<const T*>(a.k) + n * a.k_sb + hk * a.k_sh;
+  const T* __restrict__ q = static_cast<const T*>(a.q) + n * a.q_sb + hk * a.q_sh;
+  const T* __restrict__ v = static_cast<const T*>(a.v) + n * a.v_sb + h * a.v_sh;
+  const GdrGate gr = gdr_gate_load(a.g, a.g_dtype, n * a.g_sb + h * a.g_sh);
+  const GdrGate br = gdr_gate_load(a.beta, a.b_dtype, n * a.b_sb + h * a.b_sh);
+  constexpr int KL = (RG * RPT + 255) / 256;
+  T kr0[KL], qr0[KL], vr[VW];
+#pragma unroll
+  for (int z = 0; z < KL; ++z) {
+    const int r = tid + 256 * z < a.K ? tid + 256 * z : 0;
+    kr0[z] = k[r];
+    qr0[z] = q[r];
+  }
+  __builtin_memcpy(vr, v + (c0 < a.V ? c0 : 0), VW * sizeof(T));  // V is a multiple of VW (host check)
   float s[RPT][VW];
 #pragma unroll
   for (int i = 0; i < RPT; ++i) {
     const int r = rg + i * RG;
-    const bool in = r < a.K && c0 < a.V;  // V is a multiple of VW (host check)
+    const bool in = r < a.K && c0 < a.V;
     if constexpr (VW == 4) {
       const uint4 t = in ? ld16<true>(S + (int64_t)r * a.V + c0) : make_uint4(0, 0, 0, 0);
       s[i][0] = __uint_as_float(t.x); s[i][1] = __uint_as_float(t.y);
@@ -50,18 +65,18 @@ __global__ __launch_bounds__(256) void gdr_step_kernel(GdrStepArgs a) {
       s[i][0] = in ? S[(int64_t)r * a.V + c0] : 0.f;
     }
   }
-  const T* __restrict__ k = static_cast<const T*>(a.k) + n * a.k_sb + hk * a.k_sh;
-  const T* __restrict__ q = static_cast<const T*>(a.q) + n * a.q_sb + hk * a.q_sh;
-  const T* __restrict__ v = static_cast<const T*>(a.v) + n * a.v_sb + h * a.v_sh;
-  for (int r = tid; r < RG * RPT; r += 256) {
-    kf[r] = r < a.K ? to_f32(k[r]) : 0.f;
-    qf[r] = r < a.K ? to_f32(q[r]) : 0.f;
+#pragma unroll
+  for (int z = 0; z < KL; ++z) {
+    const int r = tid + 256 * z;
+    if (r < RG * RPT) {
+      kf[r] = r < a.K ? to_f32(kr0[z]) : 0.f;
+      qf[r] = r < a.K ? to_f32(qr0[z]) : 0.f;
+    }
   }
-  const float decay = expf(load_param(a.g, a.g_dtype, n * a.g_sb + h * a.g_sh));
-  const float beta = load_param(a.beta, a.b_dtype, n * a.b_sb + h * a.b_sh);
+  const float decay = expf(gdr_gate<T>(gr, a.g_dtype)), beta = gdr_gate<T>(br, a.b_dtype);
   float vv[VW];
 #pragma unroll
-  for (int j = 0; j < VW; ++j) vv[j] = c0 + j < a.V ? to_f32(v[c0 + j]) : 0.f;
+  for (int j = 0; j < VW; ++j) vv[j] = c0 < a.V ? to_f32(vr[j]) : 0.f;
   __syncthreads();
   float p[W], kq = 0.f;
 #pragma unroll
@@ -126,7 +141,7 @@ void launch_step_typed(const GdrStepArgs& a, hipStream_t s) {
   const bool vec = a.V % 4 == 0 && aligned16(a.state) && a.state_stride % 4 == 0;
   // 128 columns a workgroup (its waves then read whole rows) where that is one for each CU at least; 32
   // below, to spread the state over the chip.  32 heads of 128 x 128, states not in any cache: 16
-  // sequences 12.5 us against 16.1, 64 sequences 50.2 against 52.7; 4 sequences 6.0 against 5.6.
+  // sequences 11.6 us against 15.0, 64 sequences 45.8 against 50.7; 4 sequences 5.8 against 5.2.
   const bool wide = (a.V + 127) / 128 * (int64_t)a.Hv * a.n >= (device_cu_count() > 0 ? device_cu_count() : 256);
   if (!vec) {
     if (a.K <= 64) launch_step<T, 1, 64, 16>(a, s);
@@ -175,18 +190,18 @@ __global__ __launch_bounds__(256) void gdr_tokens_kernel(GdrArgs a) {
   const T* __restrict__ q = static_cast<const T*>(a.q) + seq.batch * a.q_s[0] + seq.begin * a.q_s[1] + hk * a.q_s[2];
   const T* __restrict__ v = static_cast<const T*>(a.v) + seq.batch * a.v_s[0] + seq.begin * a.v_s[1] + h * a.v_s[2];
   T* __restrict__ o = static_cast<T*>(a.o) + ((seq.batch * a.T + seq.begin) * a.Hv + h) * (int64_t)a.V;
-  float kn[KL], qn[KL], vn[VW], gn, bn;
+  T kn[KL], qn[KL], vn[VW];  // as they are in memory: a conversion would wait for its load
+  GdrGate gn, bn;
   auto load = [&](int64_t t) {
+    gn = gdr_gate_load(a.g, a.g_dtype, seq.batch * a.g_s[0] + (seq.begin + t) * a.g_s[1] + h * a.g_s[2]);
+    bn = gdr_gate_load(a.beta, a.b_dtype, seq.batch * a.b_s[0] + (seq.begin + t) * a.b_s[1] + h * a.b_s[2]);
 #pragma unroll
     for (int z = 0; z < KL; ++z) {
-      const int r = tid + 256 * z;
-      kn[z] = r < a.K ? to_f32(k[t * a.k_s[1] + r]) : 0.f;
-      qn[z] = r < a.K ? to_f32(q[t * a.q_s[1] + r]) : 0.f;
+      const int r = tid + 256 * z < a.K ? tid + 256 * z : 0;
+      kn[z] = k[t * a.k_s[1] + r];
+      qn[z] = q[t * a.q_s[1] + r];
     }
-#pragma unroll
-    for (int j = 0; j < VW; ++j) vn[j] = live ? to_f32(v[t * a.v_s[1] + c0 + j]) : 0.f;
-    gn = load_param(a.g, a.g_dtype, seq.batch * a.g_s[0] + (seq.begin + t) * a.g_s[1] + h * a.g_s[2]);
-    bn = load_param(a.beta, a.b_dtype, seq.batch * a.b_s[0] + (seq.begin + t) * a.b_s[1] + h * a.b_s[2]);
+    __builtin_memcpy(vn, v + t * a.v_s[1] + (live ? c0 : 0), VW * sizeof(T));
   };
   if (seq.len > 0) load(0);
   for (int64_t t = 0; t < seq.len; ++t) {
@@ -194,14 +209,14 @@ __global__ __launch_bounds__(256) void gdr_tokens_kernel(GdrArgs a) {
 #pragma unroll
     for (int z = 0; z < KL; ++z)
       if (tid + 256 * z < RG * RPT) {
-        kf[b][tid + 256 * z] = kn[z];
-        qf[b][tid + 256 * z] = qn[z];
+        kf[b][tid + 256 * z] = tid + 256 * z < a.K ? to_f32(kn[z]) : 0.f;
+        qf[b][tid + 256 * z] = tid + 256 * z < a.K ? to_f32(qn[z]) : 0.f;
       }
-    const float decay = expf(gn), beta = bn;
+    const float decay = expf(gdr_gate<T>(gn, a.g_dtype)), beta = gdr_gate<T>(bn, a.b_dtype);
     float vv[VW];
 #pragma unroll
-    for (int j = 0; j < VW; ++j) vv[j] = vn[j];
-    if (t + 1 < seq.len) load(t + 1);
+    for (int j = 0; j < VW; ++j) vv[j] = live ? to_f32(vn[j]) : 0.f;
+    load(t + 1 < seq.len ? t + 1 : t);
     __syncthreads();
     float p[W], kq = 0.f;
 #pragma unroll

@@ -229,16 +229,17 @@ __global__ __launch_bounds__(256, (KP * kParts<T> <= 128 ? 4 : 1)) void gdr_prep
     const int64_t tok = t0 + (live ? 16 * wave + c : 0);
     const T* __restrict__ q = static_cast<const T*>(a.q) + seq.batch * a.q_s[0] + tok * a.q_s[1] + hk * a.q_s[2];
     const T* __restrict__ k = static_cast<const T*>(a.k) + seq.batch * a.k_s[0] + tok * a.k_s[1] + hk * a.k_s[2];
+    // wave w has the decays of head w
+    const int h = h0 + (wave < heads ? wave : 0);
+    const int64_t i = t0 + (lane < rows ? lane : 0);
+    const GdrGate gr = gdr_gate_load(a.g, a.g_dtype, seq.batch * a.g_s[0] + i * a.g_s[1] + h * a.g_s[2]);
+    const GdrGate br = gdr_gate_load(a.beta, a.b_dtype, seq.batch * a.b_s[0] + i * a.b_s[1] + h * a.b_s[2]);
     T kv[KS][8], qv[KS][8];
     load_row<T, KP, FULL>(k, a.K, g, kv);
     load_row<T, KP, FULL>(q, a.K, g, qv);
-    if (wave < heads) {  // wave w has the decays of head w
-      const int h = h0 + wave;
-      const int64_t i = t0 + (lane < rows ? lane : 0);
-      float gv = load_param(a.g, a.g_dtype, seq.batch * a.g_s[0] + i * a.g_s[1] + h * a.g_s[2]);
-      float bv = load_param(a.beta, a.b_dtype, seq.batch * a.b_s[0] + i * a.b_s[1] + h * a.b_s[2]);
-      gv = lane < rows ? gv : 0.f;
-      bv = lane < rows ? bv : 0.f;
+    if (wave < heads) {
+      const float gv = lane < rows ? gdr_gate<T>(gr, a.g_dtype) : 0.f;
+      const float bv = lane < rows ? gdr_gate<T>(br, a.b_dtype) : 0.f;
       float2 last;
       // below -120 the decay is 0 in fp32 whatever follows, and sums with -inf have no differences
       const float2 s = running_sum(gv < -120.f ? -120.f : gv, &last);
@@ -493,10 +494,11 @@ extern "C" int atk_gated_delta_fwd(const atk_gated_delta_args* p) {
   if (need && (!p->workspace || p->workspace_bytes < need || !aligned16(p->workspace)))
     return fail(ATK_EINVAL, "gated delta: workspace too small or not 16-byte aligned");
   hipStream_t s = reinterpret_cast<hipStream_t>(p->stream);
-  // A token at a time takes 1.4 us for each, two launches on a chunk 13 to 20 us whatever it holds (1
-  // sequence, 16 heads, 128 x 128: 8 tokens 14.0 us against 15.9, 16 tokens 25.3 against 15.1; 16
-  // sequences, 32 heads: 8 tokens 43.7 us against 82.0, 16 tokens 80.2 against 81.0).
-  if (p->T <= 8) return gdr_tokens(a, p->dtype, s);
+  // A token at a time takes 1.1 us for each where few heads run, two launches on a chunk 12 to 18 us
+  // whatever it holds (128 x 128, bf16, the one against the other.  1 sequence, 16 heads: 8 tokens 11.9 us
+  // and 13.6, 10 tokens 14.2 and 13.6, 12 tokens 16.6 and 13.7; 4 sequences: 10 tokens 14.8 and 16.9, 12
+  // tokens 16.9 and 17.0; 16 sequences, 32 heads: 10 tokens 44.8 and 59.4, 16 tokens 67.8 and 58.5).
+  if (p->T <= 10) return gdr_tokens(a, p->dtype, s);
   if (int r = gdr_prepare(a, p->dtype, false, s)) return r;
   const int dtype = p->dtype;
   return ATK_GDR_TYPED(launch_chain, a, s);
