@@ -228,3 +228,32 @@ def test_refusals(dev):
                  lambda: P.rms_norm_quant(x, group_size=-16)):
         with pytest.raises(RuntimeError, match="rms_norm"):
             call()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [2, 3, 4, 5, 9, 15, 63, 127, 511, 513, 1023, 1025, 2047, 2049, 8191, 8193, 16383, 16385,
+                               32767])
+def test_rows_that_end_inside_a_vector(dev, n, dtype):
+    """Rows amid NaN, from an odd element on, with an fp32 weight: nothing beyond a row is taken for part
+    of it, and nothing beyond the output is written."""
+    import amd_tuned_torch as P
+    m = 3
+    x, r, w = inputs((m, n), dtype, dev, seed=n, wdtype=torch.float32)
+    wide = [torch.full((m, n + 4), float("nan"), dtype=dtype, device=dev) for _ in range(2)]
+    for b, t in zip(wide, (x, r)):
+        b[:, 1:n + 1] = t
+    xv, rv = (b[:, 1:n + 1] for b in wide)
+    y, h = P.rms_norm(xv, w, 1e-6, residual=rv)
+    assert torch.equal(h, (x.float() + r.float()).to(dtype))
+    want = formula(h, w)
+    close(y, want, dtype, want.abs() + 1)
+    xv, wg = xv.detach().requires_grad_(), w.detach().requires_grad_()
+    dy = wide[1][:, 1:n + 1]
+    dx, dw = torch.autograd.grad(P.rms_norm(xv, wg, 1e-6), (xv, wg), dy)
+    x64, w64 = x.double().requires_grad_(), w.double().requires_grad_()
+    ex, ew = torch.autograd.grad(formula(x64, w64), (x64, w64), r.double())
+    # dx: a term of the row's mean besides its own; dw: a sum over the rows
+    rstd = (x.double().square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    g = (r.double() * w.double()).abs()
+    close(dx, ex, dtype, rstd * (g + (x.double() * rstd).abs() * (g * (x.double() * rstd).abs()).mean(-1, keepdim=True)))
+    close(dw, ew, torch.float32, (r.double() * x.double() * rstd).abs().sum(0))
