@@ -1553,7 +1553,9 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _row_stride(t: torch.Tensor) -> int:
-    return t.stride(-2) if t.dim() > 1 else t.shape[-1]
+    """Elements from row to row of what _rows returned.  A contiguous tensor's is its width: the stride
+    that it states for an axis of length 1 may be anything."""
+    return t.shape[-1] if t.is_contiguous() else t.stride(-2)
 
 
 def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float, residual: Optional[torch.Tensor] = None,
