@@ -92,8 +92,10 @@ class GatedDeltaFn(torch.autograd.Function):
 
 def _backward_ops(inputs, scale, cu_seqlens, dout, dstate, need):
     """The gradients from torch operations, for those that are to be differentiated again or that come
-    batched (the kernels record nothing)."""
+    batched (the kernels record nothing).  They are taken at views made here: an input may be computed
+    from another, or be the same tensor, and the way between them is the outer backward's."""
     with torch.enable_grad():
+        inputs = [None if x is None else x.view_as(x) for x in inputs]
         out, state = gated_delta_rule_ref(*inputs[:5], scale, inputs[5], True, cu_seqlens)
         ends = [(y, dy) for y, dy in ((out, dout), (state, dstate)) if dy is not None]
         wanted = [x for x, wants in zip(inputs, need) if wants]

@@ -42,3 +42,44 @@ def test_row_strides(nat, name):
     flat = torch.empty(0).set_(rows.untyped_storage(), 0, (held,), (1,))
     seen = torch.stack([flat[rows.storage_offset() + i * stride:][:n] for i in range(m)])
     assert torch.equal(seen, t.reshape(m, n))
+
+
+def dependent_inputs(name, leaf):
+    """(q, k, v, g, beta, state) in 64 bits, computed from one leaf in part."""
+    gen = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=gen, dtype=torch.float64)  # noqa: E731
+    q, k, v, g, beta, state = leaf, r(1, 5, 2, 4), r(1, 5, 2, 4), -r(1, 5, 2).abs(), r(1, 5, 2).sigmoid(), r(1, 2, 4, 4)
+    if name == "v from q":
+        v = 2 * q
+    elif name == "q is k":
+        k = q
+    elif name == "gates and state from q":
+        g, beta, state = -q.square().sum(-1), q.sum(-1).sigmoid(), q[:, 0, :, :, None] * k[:, 1, :, None]
+    return q, k, v, g, beta, state
+
+
+@pytest.mark.parametrize("name", ["v from q", "q is k", "gates and state from q"])
+def test_gradients_in_torch_operations_of_dependent_inputs(name):
+    """The backward that is taken for a second derivative, inside autograd, against autograd of the
+    statement itself: both are the same operations in 64 bits, so 1e-12 is thousands of roundings."""
+    from amd_tuned_torch import gated_delta as gd
+
+    class Statement(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, *inputs):
+            ctx.save_for_backward(*inputs)
+            return gd.gated_delta_rule_ref(*inputs[:5], 0.3, inputs[5], True)
+
+        @staticmethod
+        def backward(ctx, dout, dstate):
+            return tuple(gd._backward_ops(ctx.saved_tensors, 0.3, None, dout, dstate, list(ctx.needs_input_grad)))
+
+    leaf = torch.randn(1, 5, 2, 4, generator=torch.Generator().manual_seed(0), dtype=torch.float64).requires_grad_()
+    got = []
+    for fn in (Statement.apply, lambda *a: gd.gated_delta_rule_ref(*a[:5], 0.3, a[5], True)):
+        out, state = fn(*dependent_inputs(name, leaf))
+        first, = torch.autograd.grad(out.square().sum() + state.square().sum(), leaf, create_graph=True)
+        second, = torch.autograd.grad(first.pow(3).sum(), leaf)
+        got.append((first.detach(), second))
+    for a, b in zip(*got):
+        assert (a - b).abs().max() <= 1e-12 * b.abs().max()
