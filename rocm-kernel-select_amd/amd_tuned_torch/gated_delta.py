@@ -97,7 +97,10 @@ def _backward_ops(inputs, scale, cu_seqlens, dout, dstate, need):
     with torch.enable_grad():
         inputs = [None if x is None else x.view_as(x) for x in inputs]
         out, state = gated_delta_rule_ref(*inputs[:5], scale, inputs[5], True, cu_seqlens)
-        ends = [(y, dy) for y, dy in ((out, dout), (state, dstate)) if dy is not None]
+        # (the final state does not depend on q, so without other gradients it has none)
+        ends = [(y, dy) for y, dy in ((out, dout), (state, dstate)) if dy is not None and y.requires_grad]
+        if not ends:
+            return [None] * len(inputs)
         wanted = [x for x, wants in zip(inputs, need) if wants]
         grads = iter(torch.autograd.grad([y for y, _ in ends], wanted, [dy for _, dy in ends], create_graph=True,
                                          allow_unused=True))

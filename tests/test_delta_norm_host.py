@@ -58,28 +58,45 @@ def dependent_inputs(name, leaf):
     return q, k, v, g, beta, state
 
 
-@pytest.mark.parametrize("name", ["v from q", "q is k", "gates and state from q"])
-def test_gradients_in_torch_operations_of_dependent_inputs(name):
-    """The backward that is taken for a second derivative, inside autograd, against autograd of the
-    statement itself: both are the same operations in 64 bits, so 1e-12 is thousands of roundings."""
-    from amd_tuned_torch import gated_delta as gd
-
+def statement(gd):
+    """The operator as an autograd function whose backward is the one in torch operations."""
     class Statement(torch.autograd.Function):
         @staticmethod
         def forward(ctx, *inputs):
+            ctx.set_materialize_grads(False)
             ctx.save_for_backward(*inputs)
             return gd.gated_delta_rule_ref(*inputs[:5], 0.3, inputs[5], True)
 
         @staticmethod
         def backward(ctx, dout, dstate):
             return tuple(gd._backward_ops(ctx.saved_tensors, 0.3, None, dout, dstate, list(ctx.needs_input_grad)))
+    return Statement
 
+
+@pytest.mark.parametrize("name", ["v from q", "q is k", "gates and state from q"])
+def test_gradients_in_torch_operations_of_dependent_inputs(name):
+    """The backward that is taken for a second derivative, inside autograd, against autograd of the
+    statement itself: both are the same operations in 64 bits, so 1e-12 is thousands of roundings."""
+    from amd_tuned_torch import gated_delta as gd
     leaf = torch.randn(1, 5, 2, 4, generator=torch.Generator().manual_seed(0), dtype=torch.float64).requires_grad_()
     got = []
-    for fn in (Statement.apply, lambda *a: gd.gated_delta_rule_ref(*a[:5], 0.3, a[5], True)):
+    for fn in (statement(gd).apply, lambda *a: gd.gated_delta_rule_ref(*a[:5], 0.3, a[5], True)):
         out, state = fn(*dependent_inputs(name, leaf))
         first, = torch.autograd.grad(out.square().sum() + state.square().sum(), leaf, create_graph=True)
         second, = torch.autograd.grad(first.pow(3).sum(), leaf)
         got.append((first.detach(), second))
     for a, b in zip(*got):
         assert (a - b).abs().max() <= 1e-12 * b.abs().max()
+
+
+def test_gradients_in_torch_operations_of_q_alone():
+    """The final state takes no part of q: asked for its gradient, the backward has zeros, or nothing."""
+    from amd_tuned_torch import gated_delta as gd
+    leaf = torch.randn(1, 5, 2, 4, generator=torch.Generator().manual_seed(0), dtype=torch.float64).requires_grad_()
+    inputs = dependent_inputs("apart", leaf)
+    out, state = statement(gd).apply(*inputs)
+    got, = torch.autograd.grad(out.square().sum() + state.square().sum(), leaf, create_graph=True)
+    want, = torch.autograd.grad(gd.gated_delta_rule_ref(*inputs[:5], 0.3, inputs[5]).square().sum(), leaf)
+    assert (got - want).abs().max() <= 1e-12 * want.abs().max()
+    out, state = statement(gd).apply(*inputs)
+    assert torch.autograd.grad(state.square().sum(), leaf, create_graph=True, allow_unused=True)[0] is None
