@@ -1627,8 +1627,9 @@ def rms_norm_backward(h: torch.Tensor, dy: torch.Tensor, dh: Optional[torch.Tens
     L = lib()
     ws = None
     if want_dw:
-        ws = workspace(h.device, "rms_norm_bwd", _cached_size(L.atk_rms_norm_bwd_workspace_bytes, M, N, dt,
-                                                              device=_device_index(h.device)))
+        # of this call alone: graphs are captured on one stream and may be replayed on several at once
+        ws = torch.empty(_cached_size(L.atk_rms_norm_bwd_workspace_bytes, M, N, dt, device=_device_index(h.device)),
+                         dtype=torch.uint8, device=h.device)
     rc = L.atk_rms_norm_bwd(_ptr(h), _ptr(dy), _ptr(dh), _ptr(weight), _ptr(rstd), _ptr(dx), _ptr(dw), M, N,
                             _row_stride(h), _row_stride(dy), 0 if dh is None else _row_stride(dh), dt,
                             dt if weight is None else _DTYPE_CODE[weight.dtype], _ptr(ws),

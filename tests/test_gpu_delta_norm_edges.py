@@ -40,3 +40,36 @@ def test_rms_norm_of_axes_of_one(dev, n, dtype):
             grads[-1] += torch.autograd.grad(P.rms_norm(leaves[0], leaves[2]), (leaves[0], leaves[2]), c)  # h is x itself
         for got, want in zip(*grads):
             assert torch.equal(got.reshape(want.shape), want)
+
+
+def test_weight_gradients_of_graphs_that_run_side_by_side(dev):
+    """Two captured backward passes, replayed on two streams at once: each has scratch of its own."""
+    import amd_tuned_torch as P
+    from amd_tuned_torch import _native
+    before = set(_native.workspace_keys())
+    sets, graphs = [], []
+    for seed in (0, 1):
+        gen = torch.Generator().manual_seed(seed)
+        x, dy = (torch.randn(4096, 512, generator=gen).bfloat16().to(dev) for _ in range(2))
+        w = torch.ones(512, dtype=torch.bfloat16, device=dev)
+        _, _, rstd, _ = _native.rms_norm(x, w, 1e-6, want_rstd=True)
+        want = _native.rms_norm_backward(x, dy, None, w, rstd)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = _native.rms_norm_backward(x, dy, None, w, rstd)
+        sets.append((got, want, (x, dy, w, rstd)))  # (a graph reads its inputs where they were)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for got, _, _ in sets:
+            for t in got:
+                t.zero_()
+        torch.cuda.synchronize()
+        for _ in range(4):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        for got, want, _ in sets:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert not [k for k in set(_native.workspace_keys()) - before if "rms" in k[2]]
