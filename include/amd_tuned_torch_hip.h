@@ -602,7 +602,7 @@ int atk_conv_fwd_prepacked_args(const atk_conv_prepacked_args* a);
  * quant ATK_QUANT_FP8 / ATK_QUANT_INT8: y holds 8-bit values (fp8 e4m3, top 448; int8, top 127) and
  * scales [M, ceil(N / group)] fp32 what they are multiplied by: max(max|y| / top, 2^-126) over each
  * run of `group` columns (16..256, a power of two), or over the row where group is 0.  A row of
- * zeros gives zeros.  N up to 65536 (fp32: 32768), rows of any alignment.
+ * zeros gives zeros; a row or run with a NaN has a scale of NaN.  N up to 65536 (fp32: 32768), rows of any alignment.
  * ------------------------------------------------------------------------- */
 enum { ATK_QUANT_NONE = 0, ATK_QUANT_FP8 = 1, ATK_QUANT_INT8 = 2 };
 typedef struct atk_rms_norm_args {

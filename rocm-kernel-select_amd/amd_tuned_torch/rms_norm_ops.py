@@ -7,7 +7,8 @@
 
 h = x + residual, rounded to x's dtype: the residual stream as the next layers read it, and what
 is normalised.  y = h / sqrt(mean(h^2) + eps) * weight.  q * scales stands for y: fp8 e4m3 or
-int8, a scale for each row (its last axis 1) or for each run of `group_size` columns.  GPU tensors
+int8, a scale for each row (its last axis 1) or for each run of `group_size` columns, NaN where y has
+one there.  GPU tensors
 of any row width up to 65536 (float32: 32768) and any row alignment.  `rms_norm` is differentiable;
 `rms_norm_quant` is for inference and records no gradient.
 """

@@ -136,8 +136,13 @@ __device__ __forceinline__ float lanes_reduce(float v, F f) {
   if constexpr (L >= 64) v = f(v, __shfl_xor(v, 32, 64));
   return v;
 }
+// The larger of two magnitudes, a NaN above all: their bits are in that order.
+__device__ __forceinline__ float max_abs(float a, float b) {
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+  return __uint_as_float(x > y ? x : y);
+}
 struct Max {
-  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+  __device__ __forceinline__ float operator()(float a, float b) const { return max_abs(a, b); }
 };
 struct Add {
   __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
@@ -156,26 +161,26 @@ __device__ __forceinline__ float row_reduce(float v, float* red, F f) {
   }
   return v;
 }
-// v[0..N) each over runs of `lanes` lanes
+// magnitudes v[0..N) each over runs of `lanes` lanes
 template <int N>
 __device__ __forceinline__ void group_max(float (&v)[N], int lanes) {
 #pragma unroll
   for (int j = 0; j < N; ++j) v[j] = lanes_reduce<2>(v[j], Max());
   if (lanes >= 4)
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], dpp_mov<0x4E>(v[j]));
+    for (int j = 0; j < N; ++j) v[j] = max_abs(v[j], dpp_mov<0x4E>(v[j]));
   if (lanes >= 8)
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], dpp_mov<0x141>(v[j]));
+    for (int j = 0; j < N; ++j) v[j] = max_abs(v[j], dpp_mov<0x141>(v[j]));
   if (lanes >= 16)
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], dpp_mov<0x140>(v[j]));
+    for (int j = 0; j < N; ++j) v[j] = max_abs(v[j], dpp_mov<0x140>(v[j]));
   if (lanes >= 32)
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], __shfl_xor(v[j], 16, 64));
+    for (int j = 0; j < N; ++j) v[j] = max_abs(v[j], __shfl_xor(v[j], 16, 64));
   if (lanes >= 64)
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = fmaxf(v[j], __shfl_xor(v[j], 32, 64));
+    for (int j = 0; j < N; ++j) v[j] = max_abs(v[j], __shfl_xor(v[j], 32, 64));
 }
 
 // two values into the low or high half of `old` as fp8 e4m3, nearest even; beyond +-448 saturates,
@@ -183,6 +188,12 @@ __device__ __forceinline__ void group_max(float (&v)[N], int lanes) {
 __device__ __forceinline__ float clamp_keep_nan(float v, float top) {
   const float c = fminf(fmaxf(v, -top), top);
   return v != v ? v : c;
+}
+// What 8-bit values of at most `top` are multiplied by; a NaN stays one, so a row or group that holds
+// one reads back as NaN in int8 too.
+__device__ __forceinline__ float scale_of(float amax, float top) {
+  const float s = amax / top;
+  return s < 0x1p-126f ? 0x1p-126f : s;
 }
 template <int Q, int V>
 __device__ __forceinline__ void store_q(uint8_t* __restrict__ p, int c, int N, const float* v, float inv) {
@@ -296,12 +307,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsArgs 
     for (int j = 0; j < VPT; ++j) {
       amax[j] = 0.f;
 #pragma unroll
-      for (int i = 0; i < V; ++i) amax[j] = fmaxf(amax[j], fabsf(f[j][i]));
+      for (int i = 0; i < V; ++i) amax[j] = max_abs(amax[j], fabsf(f[j][i]));
     }
     if (a.groups == 1) {
 #pragma unroll
-      for (int j = 1; j < VPT; ++j) amax[0] = fmaxf(amax[0], amax[j]);
-      const float scale = fmaxf(row_reduce<TPR>(amax[0], red[1], Max()) / top, 0x1p-126f), inv = 1.f / scale;
+      for (int j = 1; j < VPT; ++j) amax[0] = max_abs(amax[0], amax[j]);
+      const float scale = scale_of(row_reduce<TPR>(amax[0], red[1], Max()), top), inv = 1.f / scale;
       if (!live) return;
       if (t == 0) a.scales[row] = scale;
 #pragma unroll
@@ -312,7 +323,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_fwd_kernel(RmsArgs 
       group_max(amax, lanes);
 #pragma unroll
       for (int j = 0; j < VPT; ++j) {
-        const float scale = fmaxf(amax[j] / top, 0x1p-126f), inv = 1.f / scale;
+        const float scale = scale_of(amax[j], top), inv = 1.f / scale;
         const int c = (lane() + j * TPR) * V;
         if (live && c < a.N) {
           if (t % lanes == 0) a.scales[row * a.groups + c / a.group] = scale;

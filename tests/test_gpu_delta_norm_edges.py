@@ -73,3 +73,29 @@ def test_weight_gradients_of_graphs_that_run_side_by_side(dev):
         for got, want, _ in sets:
             assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert not [k for k in set(_native.workspace_keys()) - before if "rms" in k[2]]
+
+
+@pytest.mark.parametrize("out", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [5, 100, 200, 1021, 2048, 4100, 20000])
+def test_eight_bits_keep_nan(dev, n, dtype, out):
+    """A scale is NaN where its row or group holds one, and there alone, so the values it stands for are."""
+    import amd_tuned_torch as P
+    x = torch.randn(6, n, generator=torch.Generator().manual_seed(n)).to(dtype).to(dev)
+    x[1, n // 2] = float("nan")
+    x[3, n - 1] = float("inf")        # the row's own value is inf / inf, the others are 0
+    x[4] = 0
+    w = torch.ones(n, dtype=dtype, device=dev)
+    spoilt = w.clone()
+    spoilt[n // 3] = float("nan")     # a column of every row
+    for weight in (None, w, spoilt):
+        for group in (None, 16, 64, 256):
+            q, s = P.rms_norm_quant(x, weight, 1e-6, dtype=out, group_size=group)
+            h = x.double()
+            y = h / (h.square().mean(-1, keepdim=True) + 1e-6).sqrt() * (1 if weight is None else weight.double())
+            width = group or n
+            bad = torch.stack([y[:, a:a + width].isnan().any(-1) for a in range(0, n, width)], -1)
+            assert torch.equal(s.isnan(), bad) and (s[~bad] >= 2.0 ** -126).all() and s[~bad].isfinite().all()
+            wide = s.repeat_interleave(width, -1)[:, :n] if group else s
+            assert torch.equal((q.float() * wide).isnan(), bad.repeat_interleave(width, -1)[:, :n])
+            assert q[4].float()[~bad.repeat_interleave(width, -1)[4, :n]].eq(0).all()
