@@ -1588,7 +1588,7 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float, residu
     if quant is not None:
         scales = torch.empty(x.shape[:-1] + (-(-N // group) if group else 1,), dtype=torch.float32, device=x.device)
     if M == 0:
-        return y, h, rstd, scales
+        return y, h, rstd, scales if scales is None else scales.fill_(2.0 ** -126)  # (rows of no columns have one)
     if weight is not None and weight.stride(0) != 1:
         weight = weight.contiguous()
     blk = _block("rms", _RmsArgs)

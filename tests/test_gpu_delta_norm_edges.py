@@ -99,3 +99,12 @@ def test_eight_bits_keep_nan(dev, n, dtype, out):
             wide = s.repeat_interleave(width, -1)[:, :n] if group else s
             assert torch.equal((q.float() * wide).isnan(), bad.repeat_interleave(width, -1)[:, :n])
             assert q[4].float()[~bad.repeat_interleave(width, -1)[4, :n]].eq(0).all()
+
+
+def test_eight_bits_of_no_columns(dev):
+    import amd_tuned_torch as P
+    torch.full((4096,), float("nan"), device=dev)  # what a fresh tensor may hold
+    q, s = P.rms_norm_quant(torch.empty(4096, 0, device=dev))
+    assert q.shape == (4096, 0) and s.shape == (4096, 1) and s.eq(2.0 ** -126).all()
+    q, s, h = P.rms_norm_quant(torch.empty(3, 0, device=dev), residual=torch.empty(3, 0, device=dev), group_size=32)
+    assert s.shape == (3, 0) and h.shape == (3, 0)
