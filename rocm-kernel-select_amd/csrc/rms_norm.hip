@@ -478,15 +478,34 @@ RmsShape rms_shape(int64_t N, int vec, int64_t rows) {
 
 #define ATK_RMS_SHAPES(X) X(8, 1) X(16, 1) X(64, 1) X(64, 2) X(64, 4) X(256, 1) X(256, 2) X(256, 4) X(256, 8) X(512, 8) X(1024, 8)
 
+// `rows` rows from `row` on
+template <typename T, int Q>
+RmsArgs rows_from(RmsArgs a, int64_t row, int64_t rows) {
+  a.x = static_cast<const T*>(a.x) + row * a.x_stride;
+  if (a.r) a.r = static_cast<const T*>(a.r) + row * a.r_stride;
+  if (a.h) a.h = static_cast<T*>(a.h) + row * a.N;
+  a.y = static_cast<char*>(a.y) + row * a.N * (Q == kQNone ? sizeof(T) : 1);
+  if (a.rstd) a.rstd += row;
+  if (a.scales) a.scales += row * a.groups;
+  a.M = rows;
+  return a;
+}
+
+// A launch has fewer than 2^32 threads, so a call of very many rows takes several.
 template <typename T, int Q>
 int launch_fwd(const RmsArgs& a, RmsShape sh, hipStream_t s) {
 #define X(TPR, VPT)                                                                                     \
   if (sh.tpr == TPR && sh.vpt == VPT) {                                                                 \
     constexpr int NT = TPR < 256 ? 256 : TPR, RPB = NT / TPR;                                           \
-    const dim3 grid((unsigned)((a.M + RPB - 1) / RPB));                                                 \
-    if (a.r) hipLaunchKernelGGL((rms_fwd_kernel<T, Q, TPR, VPT, true>), grid, dim3(NT), 0, s, a);       \
-    else hipLaunchKernelGGL((rms_fwd_kernel<T, Q, TPR, VPT, false>), grid, dim3(NT), 0, s, a);          \
-    return check_launch("rms_fwd_kernel");                                                              \
+    constexpr int64_t most = ((int64_t)1 << 31) / TPR;                                                  \
+    for (int64_t row = 0; row < a.M; row += most) {                                                     \
+      const RmsArgs b = rows_from<T, Q>(a, row, a.M - row < most ? a.M - row : most);                   \
+      const dim3 grid((unsigned)((b.M + RPB - 1) / RPB));                                               \
+      if (a.r) hipLaunchKernelGGL((rms_fwd_kernel<T, Q, TPR, VPT, true>), grid, dim3(NT), 0, s, b);     \
+      else hipLaunchKernelGGL((rms_fwd_kernel<T, Q, TPR, VPT, false>), grid, dim3(NT), 0, s, b);        \
+      if (int rc = check_launch("rms_fwd_kernel")) return rc;                                           \
+    }                                                                                                   \
+    return ATK_OK;                                                                                      \
   }
   ATK_RMS_SHAPES(X)
 #undef X

@@ -108,3 +108,28 @@ def test_eight_bits_of_no_columns(dev):
     assert q.shape == (4096, 0) and s.shape == (4096, 1) and s.eq(2.0 ** -126).all()
     q, s, h = P.rms_norm_quant(torch.empty(3, 0, device=dev), residual=torch.empty(3, 0, device=dev), group_size=32)
     assert s.shape == (3, 0) and h.shape == (3, 0)
+
+
+@pytest.mark.parametrize("m,n", [((1 << 26) + 3, 130), ((1 << 28) + 5, 12)])
+def test_rows_beyond_2_to_the_32_threads(dev, m, n):
+    """More rows than one launch has threads for: the rows around the seam and at the ends, against the
+    same rows alone."""
+    import amd_tuned_torch as P
+    if torch.cuda.mem_get_info(dev)[0] < 5 * m * n * 2:
+        pytest.skip("not enough memory")
+    x = torch.empty(m, n, dtype=torch.bfloat16, device=dev)
+    part = torch.randn(1 << 20, n, device=dev).bfloat16()
+    for at in range(0, m, 1 << 20):
+        x[at:at + (1 << 20)] = part[:m - at]
+        part = part.roll(1, 0)
+    seam = 1 << 25 if n > 128 else 1 << 27
+    y = P.rms_norm(x)
+    for rows in (slice(0, 9), slice(seam - 9, seam + 9), slice(2 * seam - 9, 2 * seam + 2), slice(m - 3, m)):
+        assert torch.equal(y[rows], P.rms_norm(x[rows])), rows
+    del y
+    q, s, h = P.rms_norm_quant(x, residual=x, dtype=torch.int8)
+    for rows in (slice(seam - 9, seam + 9), slice(m - 3, m)):
+        for got, want in zip((q, s, h), P.rms_norm_quant(x[rows], residual=x[rows], dtype=torch.int8)):
+            assert torch.equal(got[rows], want), rows
+    del x, q, s, h, got
+    torch.cuda.empty_cache()
