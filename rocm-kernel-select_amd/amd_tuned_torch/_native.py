@@ -1695,8 +1695,7 @@ def _delta_update_check(q, k, v, g, beta, state, state_indices) -> None:
     if not (q.is_cuda and k.device == dev and v.device == dev and g.device == dev and beta.device == dev
             and state.device == dev):
         raise RuntimeError("gated_delta_rule_update: all tensors must be on one GPU")
-    if state.stride(3) != 1 or state.stride(2) != V or state.stride(1) != K * V or (
-            state.shape[0] > 1 and state.stride(0) < Hv * K * V):
+    if not state[:1].is_contiguous() or (state.shape[0] > 1 and state.stride(0) < Hv * K * V):
         raise RuntimeError("gated_delta_rule_update: each slot of the state must be contiguous (it is updated in place)")
     if state_indices is not None and (state_indices.dtype != torch.int32 or state_indices.shape != (N,)
                                       or state_indices.device != dev):

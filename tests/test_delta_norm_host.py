@@ -100,3 +100,37 @@ def test_gradients_in_torch_operations_of_q_alone():
     assert (got - want).abs().max() <= 1e-12 * want.abs().max()
     out, state = statement(gd).apply(*inputs)
     assert torch.autograd.grad(state.square().sum(), leaf, create_graph=True, allow_unused=True)[0] is None
+
+
+class OnDevice:
+    """A CPU tensor that says it is on the GPU: for the checks, which look at sizes and strides alone."""
+
+    def __init__(self, t):
+        self.t, self.is_cuda, self.device = t, True, torch.device("cuda", 0)
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def __getitem__(self, at):
+        return OnDevice(self.t[at])
+
+
+def test_states_with_an_axis_of_one(nat):
+    """Slots that are contiguous pass, whatever strides their axes of length 1 state; others do not."""
+    def check(state, n=2):
+        hv, dk, dv = state.shape[1:]
+        r = lambda *s: OnDevice(torch.zeros(s))  # noqa: E731
+        nat._delta_update_check(r(n, 1, dk), r(n, 1, dk), r(n, hv, dv), r(n, hv), r(n, hv), OnDevice(state),
+                                OnDevice(torch.zeros(n, dtype=torch.int32)))
+
+    base = torch.zeros(4096)
+    for state in (base[:768].view(3, 4, 8, 8).contiguous(), base[:192].view(1, 3, 8, 8).transpose(0, 1),  # one head
+                  base.view(8, 8, 8, 8)[:, 2:3], base.as_strided((3, 1, 8, 8), (64, 5, 8, 1)),
+                  base.as_strided((3, 2, 1, 8), (16, 8, 3, 1)), base.as_strided((3, 2, 8, 1), (16, 8, 1, 9)),
+                  base.as_strided((1, 2, 8, 8), (7, 64, 8, 1)), base.view(2, 2, 4, 16, 16)[:, 1]):
+        check(state)
+    for state in (base.view(1, 8, 8, 64)[..., :8], base[:256].view(2, 2, 8, 8).transpose(2, 3),
+                  base.view(8, 8, 8, 8).transpose(1, 2), base.as_strided((3, 1, 8, 8), (32, 64, 8, 1)),
+                  base.as_strided((3, 2, 8, 8), (0, 64, 8, 1))):
+        with pytest.raises(RuntimeError, match="contiguous"):
+            check(state)

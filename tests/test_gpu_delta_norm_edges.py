@@ -133,3 +133,16 @@ def test_rows_beyond_2_to_the_32_threads(dev, m, n):
             assert torch.equal(got[rows], want), rows
     del x, q, s, h, got
     torch.cuda.empty_cache()
+
+
+def test_update_of_one_head(dev):
+    """A cache of one value head that was laid out heads first: equal bits to the same states copied."""
+    import amd_tuned_torch as P
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen).to(dev)  # noqa: E731
+    q, k, v, g, beta = r(3, 1, 64) / 8, r(3, 1, 64) / 8, r(3, 1, 36), -r(3, 1).abs(), r(3, 1).sigmoid()
+    state = r(1, 5, 64, 36).transpose(0, 1)
+    copy = state.reshape(5, 64 * 36).clone().view(5, 1, 64, 36)
+    slots = torch.tensor([4, 0, 2], dtype=torch.int32, device=dev)
+    got, want = (P.gated_delta_rule_update(q, k, v, g, beta, s, state_indices=slots) for s in (state, copy))
+    assert torch.equal(got, want) and torch.equal(state, copy)
