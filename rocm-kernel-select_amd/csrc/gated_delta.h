@@ -53,6 +53,7 @@ struct GdrArgs {
 int gdr_prepare(const GdrArgs& a, int dtype, bool backward, hipStream_t s);
 int gdr_tokens(const GdrArgs& a, int dtype, hipStream_t s);  // forward, a token at a time
 size_t gdr_plan(const atk_gated_delta_args* p, bool backward, GdrArgs* a, int* rc);
+inline bool gdr_gate_ok(int gate, int dtype) { return gate == dtype || gate == ATK_F32; }  // what gdr_gate reads
 inline int gdr_padded_k(int K) { return K <= 64 ? 64 : K <= 128 ? 128 : 256; }
 
 // Where sequence n's tokens and chunks lie.  A packed sequence has the chunk slots from

@@ -316,6 +316,8 @@ extern "C" int atk_gated_delta_update(const atk_gated_delta_update_args* p) {
   if (!p) return fail(ATK_EINVAL, "gated delta update: null arguments");
   if (!dtype_ok(p->dtype) || !dtype_ok(p->g_dtype) || !dtype_ok(p->beta_dtype))
     return fail(ATK_EINVAL, "gated delta update: unknown dtype code");
+  if (!gdr_gate_ok(p->g_dtype, p->dtype) || !gdr_gate_ok(p->beta_dtype, p->dtype))
+    return fail(ATK_EINVAL, "gated delta update: g and beta must be of the inputs' type or fp32");
   if (p->N < 0 || p->Hk <= 0 || p->Hv <= 0 || p->K <= 0 || p->V <= 0 || p->slots < 0)
     return fail(ATK_EINVAL, "gated delta update: bad sizes");
   if (p->Hv % p->Hk) return fail(ATK_EINVAL, "gated delta update: value heads must be a multiple of key heads");

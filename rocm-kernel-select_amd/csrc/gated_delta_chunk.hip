@@ -432,6 +432,8 @@ size_t gdr_plan(const atk_gated_delta_args* p, bool backward, GdrArgs* a, int* r
   if (!p) return *rc = fail(ATK_EINVAL, "gated delta: null arguments"), 0;
   if (!dtype_ok(p->dtype) || !dtype_ok(p->g_dtype) || !dtype_ok(p->beta_dtype))
     return *rc = fail(ATK_EINVAL, "gated delta: unknown dtype code"), 0;
+  if (!gdr_gate_ok(p->g_dtype, p->dtype) || !gdr_gate_ok(p->beta_dtype, p->dtype))
+    return *rc = fail(ATK_EINVAL, "gated delta: g and beta must be of the inputs' type or fp32"), 0;
   if (p->N < 0 || p->T < 0 || p->Hk <= 0 || p->Hv <= 0 || p->K <= 0 || p->V <= 0)
     return *rc = fail(ATK_EINVAL, "gated delta: bad sizes"), 0;
   if (p->Hv % p->Hk) return *rc = fail(ATK_EINVAL, "gated delta: value heads must be a multiple of key heads"), 0;

@@ -134,3 +134,39 @@ def test_states_with_an_axis_of_one(nat):
                   base.as_strided((3, 2, 8, 8), (0, 64, 8, 1))):
         with pytest.raises(RuntimeError, match="contiguous"):
             check(state)
+
+
+P = 1 << 20  # a pointer that no refusal may follow
+
+
+def sequences(nat, fn, **kw):
+    import ctypes
+    a = nat._DeltaArgs()
+    for f in ("q", "k", "v", "g", "beta", "out"):
+        setattr(a, f, P)
+    a.N, a.T, a.Hk, a.Hv, a.K, a.V, a.dtype = 2, 100, 2, 4, 64, 64, nat.ATK_BF16
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return fn(ctypes.addressof(a))
+
+
+def test_gates_of_a_type_that_the_kernels_do_not_read(nat):
+    import ctypes
+    lib = nat.lib()
+    bwd = lambda p: lib.atk_gated_delta_bwd(p, P, None, P, P, P, P, P, None)  # noqa: E731
+    pairs = [(nat.ATK_BF16, nat.ATK_F16), (nat.ATK_F16, nat.ATK_BF16), (nat.ATK_F32, nat.ATK_F16),
+             (nat.ATK_F32, nat.ATK_BF16)]
+    for dtype, gate in pairs:
+        for name, other in (("g_dtype", "beta_dtype"), ("beta_dtype", "g_dtype")):
+            kw = {"dtype": dtype, name: gate, other: dtype}
+            for size in (lib.atk_gated_delta_workspace_bytes, lib.atk_gated_delta_bwd_workspace_bytes):
+                assert sequences(nat, size, **kw) == 0, kw
+            for fn in (lib.atk_gated_delta_fwd, bwd):
+                assert sequences(nat, fn, workspace=P, workspace_bytes=1 << 40, **kw) == nat.ATK_EINVAL, kw
+            a = nat._DeltaUpdateArgs()
+            for f in ("q", "k", "v", "g", "beta", "state", "out"):
+                setattr(a, f, P)
+            a.N, a.slots, a.Hk, a.Hv, a.K, a.V = 2, 2, 2, 4, 64, 64
+            for f, value in kw.items():
+                setattr(a, f, value)
+            assert lib.atk_gated_delta_update(ctypes.addressof(a)) == nat.ATK_EINVAL, kw
