@@ -652,7 +652,8 @@ int atk_gated_delta_update(const atk_gated_delta_update_args* a);
  * when given.  cu_seqlens (int32, N + 1, on the device): the N sequences are packed into one row of T
  * tokens (first axis 1), sequence n from cu_seqlens[n] to cu_seqlens[n + 1]; offsets must not decrease
  * and are clamped to the row, and tokens of no sequence get an output of zero.  The workspace (16-byte
- * aligned, contents ignored) has atk_gated_delta_workspace_bytes of the same arguments. */
+ * aligned, contents ignored) has atk_gated_delta_workspace_bytes of the same arguments: 0 for rows of a
+ * few tokens, which need none. */
 typedef struct atk_gated_delta_args {
   const void* q; const void* k; const void* v; const void* g; const void* beta;
   const void* initial_state; void* final_state; void* out; const int* cu_seqlens;

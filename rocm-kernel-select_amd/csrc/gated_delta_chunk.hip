@@ -426,6 +426,13 @@ int gdr_prepare(const GdrArgs& a, int dtype, bool backward, hipStream_t s) {
   return ATK_GDR_TYPED(launch_prepare, a, backward, s);
 }
 
+// A token at a time takes 1.1 us for each where few heads run, two launches on a chunk 12 to 18 us
+// whatever it holds (128 x 128, bf16, the one against the other.  1 sequence, 16 heads: 8 tokens 11.9 us
+// and 13.6, 10 tokens 14.2 and 13.6, 12 tokens 16.6 and 13.7; 4 sequences: 10 tokens 14.8 and 16.9, 12
+// tokens 16.9 and 17.0; 16 sequences, 32 heads: 10 tokens 44.8 and 59.4, 16 tokens 67.8 and 58.5).  Such
+// calls keep the state in registers and need no workspace.
+static bool gdr_by_token(int64_t tokens) { return tokens <= 10; }
+
 // Checks a call and lays out its workspace: the bytes it takes, or 0 with *rc set.
 size_t gdr_plan(const atk_gated_delta_args* p, bool backward, GdrArgs* a, int* rc) {
   *rc = ATK_OK;
@@ -452,6 +459,7 @@ size_t gdr_plan(const atk_gated_delta_args* p, bool backward, GdrArgs* a, int* r
   a->Hk = p->Hk; a->Hv = p->Hv; a->group = p->Hv / p->Hk; a->K = p->K; a->V = p->V;
   a->VP = (a->V + 31) / 32 * 32;
   a->g_dtype = p->g_dtype; a->b_dtype = p->beta_dtype; a->scale = p->scale;
+  if (!backward && gdr_by_token(p->T)) return 0;
   // (16-byte pieces throughout, so each part of the workspace is aligned as its start is)
   const int np = p->dtype == ATK_F32 ? 3 : p->dtype == ATK_F16 ? 2 : 1;
   const size_t kb = (size_t)a->slots * a->Hk * gdr_padded_k(a->K) * 64 * 2 * np, tb = (size_t)a->slots * a->Hv * kTri * 3 * 1024;
@@ -496,11 +504,7 @@ extern "C" int atk_gated_delta_fwd(const atk_gated_delta_args* p) {
   if (need && (!p->workspace || p->workspace_bytes < need || !aligned16(p->workspace)))
     return fail(ATK_EINVAL, "gated delta: workspace too small or not 16-byte aligned");
   hipStream_t s = reinterpret_cast<hipStream_t>(p->stream);
-  // A token at a time takes 1.1 us for each where few heads run, two launches on a chunk 12 to 18 us
-  // whatever it holds (128 x 128, bf16, the one against the other.  1 sequence, 16 heads: 8 tokens 11.9 us
-  // and 13.6, 10 tokens 14.2 and 13.6, 12 tokens 16.6 and 13.7; 4 sequences: 10 tokens 14.8 and 16.9, 12
-  // tokens 16.9 and 17.0; 16 sequences, 32 heads: 10 tokens 44.8 and 59.4, 16 tokens 67.8 and 58.5).
-  if (p->T <= 10) return gdr_tokens(a, p->dtype, s);
+  if (gdr_by_token(p->T)) return gdr_tokens(a, p->dtype, s);
   if (int r = gdr_prepare(a, p->dtype, false, s)) return r;
   const int dtype = p->dtype;
   return ATK_GDR_TYPED(launch_chain, a, s);

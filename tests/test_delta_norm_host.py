@@ -170,3 +170,14 @@ def test_gates_of_a_type_that_the_kernels_do_not_read(nat):
             for f, value in kw.items():
                 setattr(a, f, value)
             assert lib.atk_gated_delta_update(ctypes.addressof(a)) == nat.ATK_EINVAL, kw
+
+
+def test_short_calls_need_no_workspace(nat):
+    """Ten tokens go one after the other with the state in registers; the backward has chunks all the same."""
+    lib = nat.lib()
+    size, size_b = lib.atk_gated_delta_workspace_bytes, lib.atk_gated_delta_bwd_workspace_bytes
+    for n in (1, 1024):
+        for t in (0, 1, 10):
+            assert sequences(nat, size, N=n, T=t) == 0
+            assert sequences(nat, size, N=n, T=t, cu_seqlens=P) == 0
+        assert sequences(nat, size, N=n, T=11) > 0 and sequences(nat, size_b, N=n, T=10) > 0
