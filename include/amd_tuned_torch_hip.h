@@ -670,7 +670,8 @@ int atk_gated_delta_fwd(const atk_gated_delta_args* a);
  * workspace has atk_gated_delta_bwd_workspace_bytes), dout (N, T, Hv, V, dense, `dtype`) and
  * dfinal_state (fp32, like final_state; NULL: zeros).  Writes dq, dk (N, T, Hk, K), dv (N, T, Hv, V),
  * dg and dbeta (N, T, Hv), all dense and of their tensors' types, and dinitial_state (fp32) when given.
- * Sums over the value heads of a key head have a fixed order.  Tokens of no sequence get zeros. */
+ * Sums over the value heads of a key head have a fixed order.  Tokens of no sequence get zeros.  One
+ * state, of K padded to 64, 128 or 256 and V to 32, must have fewer than 2^31 elements. */
 size_t atk_gated_delta_bwd_workspace_bytes(const atk_gated_delta_args* a);
 int atk_gated_delta_bwd(const atk_gated_delta_args* a, const void* dout, const void* dfinal_state, void* dq, void* dk,
                         void* dv, void* dg, void* dbeta, void* dinitial_state);

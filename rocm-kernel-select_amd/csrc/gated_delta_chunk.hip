@@ -448,6 +448,9 @@ size_t gdr_plan(const atk_gated_delta_args* p, bool backward, GdrArgs* a, int* r
   if (p->K > kGdrMaxK || p->Hv > 65535 || p->N > 65535 || p->T >= ((int64_t)1 << 31) - 64 ||
       (double)per * (double)p->N >= 2147483648.0 || p->V > (1 << 24))
     return *rc = fail(ATK_UNSUPPORTED, "gated delta: more than %d key columns, 65535 heads or sequences, or 2^31 tokens", kGdrMaxK), 0;
+  // a chunk's states are indexed in 32 bits by the backward, columns padded to its tiles
+  if (backward && ((int64_t)p->V + 31) / 32 * 32 * gdr_padded_k(p->K) > 0x7fffffff)
+    return *rc = fail(ATK_UNSUPPORTED, "gated delta backward: states of more than 2^31 elements"), 0;
   *a = GdrArgs{};
   a->q = p->q; a->k = p->k; a->v = p->v; a->g = p->g; a->beta = p->beta; a->o = p->out;
   a->s0 = static_cast<const float*>(p->initial_state); a->s1 = static_cast<float*>(p->final_state); a->cu = p->cu_seqlens;

@@ -181,3 +181,15 @@ def test_short_calls_need_no_workspace(nat):
             assert sequences(nat, size, N=n, T=t) == 0
             assert sequences(nat, size, N=n, T=t, cu_seqlens=P) == 0
         assert sequences(nat, size, N=n, T=11) > 0 and sequences(nat, size_b, N=n, T=10) > 0
+
+
+def test_states_that_32_bits_cannot_index(nat):
+    lib = nat.lib()
+    bwd = lambda p: lib.atk_gated_delta_bwd(p, P, None, P, P, P, P, P, None)  # noqa: E731
+    size, size_b = lib.atk_gated_delta_workspace_bytes, lib.atk_gated_delta_bwd_workspace_bytes
+    for k, v in ((129, 1 << 23), (256, (1 << 23) - 31), (128, 1 << 24)):
+        kw = dict(N=1, Hk=1, Hv=1, K=k, V=v, workspace=P, workspace_bytes=1 << 60)
+        assert sequences(nat, bwd, **kw) == nat.ATK_UNSUPPORTED and sequences(nat, size_b, **kw) == 0
+        assert sequences(nat, size, **kw) > 0    # the forward has no such index
+    for k, v in ((256, (1 << 23) - 32), (64, 1 << 24)):
+        assert sequences(nat, size_b, N=1, Hk=1, Hv=1, K=k, V=v) > 0
