@@ -444,9 +444,10 @@ size_t gdr_plan(const atk_gated_delta_args* p, bool backward, GdrArgs* a, int* r
   if (p->N < 0 || p->T < 0 || p->Hk <= 0 || p->Hv <= 0 || p->K <= 0 || p->V <= 0)
     return *rc = fail(ATK_EINVAL, "gated delta: bad sizes"), 0;
   if (p->Hv % p->Hk) return *rc = fail(ATK_EINVAL, "gated delta: value heads must be a multiple of key heads"), 0;
-  const int64_t per = (p->T + kGdrC - 1) / kGdrC;
+  // chunks; in doubles, since N and T may be anything yet
+  const double slots = p->cu_seqlens ? (double)(p->T / kGdrC) + (double)p->N : (double)((p->T + kGdrC - 1) / kGdrC) * (double)p->N;
   if (p->K > kGdrMaxK || p->Hv > 65535 || p->N > 65535 || p->T >= ((int64_t)1 << 31) - 64 ||
-      (double)per * (double)p->N >= 2147483648.0 || p->V > (1 << 24))
+      p->V > (1 << 24) || slots > 2147483647.0)
     return *rc = fail(ATK_UNSUPPORTED, "gated delta: more than %d key columns, 65535 heads or sequences, or 2^31 tokens", kGdrMaxK), 0;
   // a chunk's states are indexed in 32 bits by the backward, columns padded to its tiles
   if (backward && ((int64_t)p->V + 31) / 32 * 32 * gdr_padded_k(p->K) > 0x7fffffff)
@@ -458,7 +459,7 @@ size_t gdr_plan(const atk_gated_delta_args* p, bool backward, GdrArgs* a, int* r
     a->q_s[i] = p->q_stride[i]; a->k_s[i] = p->k_stride[i]; a->v_s[i] = p->v_stride[i];
     a->g_s[i] = p->g_stride[i]; a->b_s[i] = p->beta_stride[i];
   }
-  a->n = p->N; a->T = p->T; a->slots = p->cu_seqlens ? p->T / kGdrC + p->N : p->N * per;
+  a->n = p->N; a->T = p->T; a->slots = (int64_t)slots;
   a->Hk = p->Hk; a->Hv = p->Hv; a->group = p->Hv / p->Hk; a->K = p->K; a->V = p->V;
   a->VP = (a->V + 31) / 32 * 32;
   a->g_dtype = p->g_dtype; a->b_dtype = p->beta_dtype; a->scale = p->scale;

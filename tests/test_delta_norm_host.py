@@ -193,3 +193,13 @@ def test_states_that_32_bits_cannot_index(nat):
         assert sequences(nat, size, **kw) > 0    # the forward has no such index
     for k, v in ((256, (1 << 23) - 32), (64, 1 << 24)):
         assert sequences(nat, size_b, N=1, Hk=1, Hv=1, K=k, V=v) > 0
+
+
+def test_many_sequences_in_one_long_row(nat):
+    """A packed row has a chunk for each 64 tokens and one a sequence, not the row's for every sequence."""
+    size = nat.lib().atk_gated_delta_workspace_bytes
+    chunk = sequences(nat, size, N=2, T=64) - sequences(nat, size, N=1, T=64)
+    base = sequences(nat, size, N=1, T=64) - chunk
+    for n, t in ((40000, 1 << 22), (65535, (1 << 31) - 128)):
+        assert sequences(nat, size, N=n, T=t, cu_seqlens=P) == base + chunk * (t // 64 + n)
+    assert sequences(nat, nat.lib().atk_gated_delta_fwd, N=40000, T=1 << 22) == nat.ATK_UNSUPPORTED
