@@ -13,6 +13,9 @@ namespace atk {
 
 constexpr int kGdrMaxK = 256;   // key columns: a state's rows
 constexpr int kGdrC = 64;       // tokens of a chunk
+// workgroups of 512 that one launch of a chain has at most: with fewer than 2^32 threads in a launch, a
+// call of more heads, sequences and value tiles takes several (a multiple of the 8 XCDs each)
+constexpr int64_t kGdrBlocks = (int64_t)1 << 21;
 
 struct GdrStepArgs {
   const void* q; const void* k; const void* v; const void* g; const void* beta;

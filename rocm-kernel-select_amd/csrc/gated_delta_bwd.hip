@@ -379,12 +379,12 @@ __device__ __forceinline__ void gdr_bwd_chain(const GdrArgs& a, char* lds, int64
 // Two to a CU gained nothing for 256 tiles of 128 x 128 in bf16 (168 us, one after the other 156): their
 // loads then wait for each other.
 template <typename T, int KP, bool FULL>
-__global__ __launch_bounds__(512) void gdr_chains_kernel(GdrArgs a) {
+__global__ __launch_bounds__(512) void gdr_chains_kernel(GdrArgs a, int64_t first) {
   constexpr size_t A = sizeof(GdrChainLds<T, KP, true>), B = sizeof(GdrBwdLds<T, KP>);
   __shared__ __align__(16) char lds[A > B ? A : B];
   const int64_t half = gridDim.x / 2;
-  if (blockIdx.x >= half) gdr_chain<T, KP, true, FULL>(a, lds, blockIdx.x - half);
-  else gdr_bwd_chain<T, KP, FULL>(a, lds, blockIdx.x);
+  if (blockIdx.x >= half) gdr_chain<T, KP, true, FULL>(a, lds, first + blockIdx.x - half);
+  else gdr_bwd_chain<T, KP, FULL>(a, lds, first + blockIdx.x);
 }
 
 // (row, column) tile t of the ten of a lower triangle of 16 x 16 tiles
@@ -784,11 +784,13 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
 
 template <typename T, int KP>
 int launch(const GdrArgs& a, hipStream_t s) {
-  const int64_t grid = (a.n * a.Hv + 7) / 8 * 16 * (a.VP / 16);
-  if (grid > 0x7fffffff) return fail(ATK_UNSUPPORTED, "gated delta backward: too many heads, sequences and value columns");
-  if (a.V % 16 == 0 || a.V % 16 >= 4) hipLaunchKernelGGL((gdr_chains_kernel<T, KP, true>), dim3((unsigned)grid), dim3(512), 0, s, a);
-  else hipLaunchKernelGGL((gdr_chains_kernel<T, KP, false>), dim3((unsigned)grid), dim3(512), 0, s, a);
-  if (int rc = check_launch("gdr_chains_kernel")) return rc;
+  const int64_t grid = (a.n * a.Hv + 7) / 8 * 8 * (a.VP / 16);  // of each chain
+  for (int64_t first = 0; first < grid; first += kGdrBlocks) {
+    const dim3 c(2 * (unsigned)(grid - first < kGdrBlocks ? grid - first : kGdrBlocks));
+    if (a.V % 16 == 0 || a.V % 16 >= 4) hipLaunchKernelGGL((gdr_chains_kernel<T, KP, true>), c, dim3(512), 0, s, a, first);
+    else hipLaunchKernelGGL((gdr_chains_kernel<T, KP, false>), c, dim3(512), 0, s, a, first);
+    if (int rc = check_launch("gdr_chains_kernel")) return rc;
+  }
   if (a.T == 0) return ATK_OK;
   const dim3 g((unsigned)a.slots, (unsigned)a.Hk);
   if (a.V % 8 == 0) hipLaunchKernelGGL((gdr_grads_kernel<T, KP, true>), g, dim3(512), 0, s, a);

@@ -382,9 +382,9 @@ __global__ __launch_bounds__(256, (KP * kParts<T> <= 128 ? 4 : 1)) void gdr_prep
 }
 
 template <typename T, int KP, bool FULL>
-__global__ __launch_bounds__(512, (kChainWaves<T, KP>)) void gdr_chain_kernel(GdrArgs a) {
+__global__ __launch_bounds__(512, (kChainWaves<T, KP>)) void gdr_chain_kernel(GdrArgs a, int64_t first) {
   __shared__ __align__(16) char lds[sizeof(GdrChainLds<T, KP, false>)];
-  gdr_chain<T, KP, false, FULL>(a, lds, blockIdx.x);
+  gdr_chain<T, KP, false, FULL>(a, lds, first + blockIdx.x);
 }
 
 template <typename T, int KP>
@@ -405,11 +405,13 @@ int launch_prepare(const GdrArgs& a, bool backward, hipStream_t s) {
 template <typename T, int KP>
 int launch_chain(const GdrArgs& a, hipStream_t s) {
   const int64_t grid = (a.n * a.Hv + 7) / 8 * 8 * ((a.V + 15) / 16);
-  if (grid > 0x7fffffff) return fail(ATK_UNSUPPORTED, "gated delta: too many heads, sequences and value columns");
-  const dim3 g((unsigned)grid), b(512);
-  if (a.V % 16 == 0 || a.V % 16 >= 4) hipLaunchKernelGGL((gdr_chain_kernel<T, KP, true>), g, b, 0, s, a);
-  else hipLaunchKernelGGL((gdr_chain_kernel<T, KP, false>), g, b, 0, s, a);
-  return check_launch("gdr_chain_kernel");
+  for (int64_t first = 0; first < grid; first += kGdrBlocks) {
+    const dim3 g((unsigned)(grid - first < kGdrBlocks ? grid - first : kGdrBlocks)), b(512);
+    if (a.V % 16 == 0 || a.V % 16 >= 4) hipLaunchKernelGGL((gdr_chain_kernel<T, KP, true>), g, b, 0, s, a, first);
+    else hipLaunchKernelGGL((gdr_chain_kernel<T, KP, false>), g, b, 0, s, a, first);
+    if (int rc = check_launch("gdr_chain_kernel")) return rc;
+  }
+  return ATK_OK;
 }
 
 }  // namespace

@@ -146,3 +146,38 @@ def test_update_of_one_head(dev):
     slots = torch.tensor([4, 0, 2], dtype=torch.int32, device=dev)
     got, want = (P.gated_delta_rule_update(q, k, v, g, beta, s, state_indices=slots) for s in (state, copy))
     assert torch.equal(got, want) and torch.equal(state, copy)
+
+
+@pytest.mark.parametrize("n,hv,gradients", [(64, 64, False), (64, 34, True)])
+def test_chains_beyond_one_launch(dev, n, hv, gradients):
+    """More heads, sequences and value tiles than one launch has threads for.  A value column depends on no
+    other, so columns from here and there have equal bits to a call on them alone."""
+    import amd_tuned_torch as P
+    t, dk, dv = 11, 16, 32768
+    if torch.cuda.mem_get_info(dev)[0] < (200 << 30):
+        pytest.skip("not enough memory")
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    q, k = (torch.nn.functional.normalize(r(n, t, 1, dk), dim=-1).bfloat16().to(dev) for _ in range(2))
+    g, beta = -r(n, t, hv).abs().to(dev), r(n, t, hv).sigmoid().bfloat16().to(dev)
+    v = torch.empty(n, t, hv, dv, dtype=torch.bfloat16, device=dev)
+    for i in range(n):
+        v[i].normal_(generator=torch.Generator(device=dev).manual_seed(i))
+    parts = [slice(0, 64), slice(16384, 16448), slice(dv - 64, dv)]
+    if not gradients:
+        out = P.gated_delta_rule(q, k, v, g, beta)
+        for at in parts:
+            assert torch.equal(out[..., at], P.gated_delta_rule(q, k, v[..., at], g, beta)), at
+    else:
+        dout = torch.empty_like(v)
+        for i in range(n):
+            dout[i].normal_(generator=torch.Generator(device=dev).manual_seed(n + i))
+        v.requires_grad_()
+        dv_all, = torch.autograd.grad(P.gated_delta_rule(q, k, v, g, beta), v, dout)
+        for at in parts:
+            some = v.detach()[..., at].clone().requires_grad_()
+            want, = torch.autograd.grad(P.gated_delta_rule(q, k, some, g, beta), some, dout[..., at])
+            assert torch.equal(dv_all[..., at], want), at
+        del dout, dv_all
+    del v
+    torch.cuda.empty_cache()
