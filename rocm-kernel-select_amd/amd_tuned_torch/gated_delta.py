@@ -37,8 +37,8 @@ def gated_delta_rule_ref(q, k, v, g, beta, scale=None, initial_state=None, retur
     if cu_seqlens is None:
         parts = [(slice(None), 0, v.shape[1])]
     else:
-        ends = cu_seqlens.tolist()
-        parts = [(slice(0, 1), a, b) for a, b in zip(ends, ends[1:])]
+        ends = cu_seqlens.clamp(0, v.shape[1]).tolist()
+        parts = [(slice(0, 1), a, max(a, b)) for a, b in zip(ends, ends[1:])]
     outs, states = [], []
     for i, (row, a, b) in enumerate(parts):
         if initial_state is None:

@@ -203,3 +203,14 @@ def test_many_sequences_in_one_long_row(nat):
     for n, t in ((40000, 1 << 22), (65535, (1 << 31) - 128)):
         assert sequences(nat, size, N=n, T=t, cu_seqlens=P) == base + chunk * (t // 64 + n)
     assert sequences(nat, nat.lib().atk_gated_delta_fwd, N=40000, T=1 << 22) == nat.ATK_UNSUPPORTED
+
+
+def test_statement_clamps_offsets():
+    """As the kernels do: what offsets beyond the row leave of it, in the result and the gradients."""
+    from amd_tuned_torch import gated_delta as gd
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen, dtype=torch.float64)  # noqa: E731
+    args = r(1, 9, 1, 4), r(1, 9, 1, 4), r(1, 9, 2, 3), -r(1, 9, 2).abs(), r(1, 9, 2).sigmoid()
+    for bad, good in (([-5, 3, 40], [0, 3, 9]), ([2, 4, 12], [2, 4, 9]), ([11, 12], [9, 9])):
+        got, want = (gd.gated_delta_rule_ref(*args, 0.3, None, True, torch.tensor(cu, dtype=torch.int32)) for cu in (bad, good))
+        assert got[0].shape == args[2].shape and all(torch.equal(a, b) for a, b in zip(got, want))
