@@ -129,6 +129,19 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     return (out, state) if return_final_state else out
 
 
+class GatedDeltaUpdateFn(torch.autograd.Function):
+    """The decode step where autograd is watching: the states it overwrites are gone, so it has no gradient
+    and says so when asked for one."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, state, scale, state_indices):
+        return _native.gated_delta_update(q, k, v, g, beta, state, scale, state_indices)
+
+    @staticmethod
+    def backward(ctx, dout):
+        raise RuntimeError("gated_delta_rule_update overwrites its states and has no gradient; gated_delta_rule has one")
+
+
 def gated_delta_rule_update(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
                             state: torch.Tensor, scale: Optional[float] = None,
                             state_indices: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -136,9 +149,14 @@ def gated_delta_rule_update(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g
     (batch, heads_v), state float32 (slots, heads_v, dim_k, dim_v) updated in place ->
     out (batch, heads_v, dim_v).  state_indices int32 (batch,): the slot of each sequence, all
     different; one outside [0, slots) marks a row of padding, whose output is zero.  Without it the
-    state has one slot a sequence.  scale: dim_k ** -0.5 by default."""
-    return _native.gated_delta_update(q, k, v, g, beta, state, q.shape[-1] ** -0.5 if scale is None else scale,
-                                      state_indices)
+    state has one slot a sequence.  scale: dim_k ** -0.5 by default.  For decoding: it has no gradient,
+    and a backward that comes to it, or a tangent, is an error."""
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
+                                    or beta.requires_grad or state.requires_grad) \
+            or autograd_state.transformed(q, k, v, g, beta, state):
+        return GatedDeltaUpdateFn.apply(q, k, v, g, beta, state, scale, state_indices)
+    return _native.gated_delta_update(q, k, v, g, beta, state, scale, state_indices)
 
 
 def gated_delta_rule_update_ref(q, k, v, g, beta, state, scale=None, state_indices=None):

@@ -214,3 +214,36 @@ def test_statement_clamps_offsets():
     for bad, good in (([-5, 3, 40], [0, 3, 9]), ([2, 4, 12], [2, 4, 9]), ([11, 12], [9, 9])):
         got, want = (gd.gated_delta_rule_ref(*args, 0.3, None, True, torch.tensor(cu, dtype=torch.int32)) for cu in (bad, good))
         assert got[0].shape == args[2].shape and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_decode_step_has_no_gradient_and_says_so(nat, monkeypatch):
+    """With the torch statement, under no_grad as a kernel is, in the kernel's place."""
+    from amd_tuned_torch import gated_delta as gd
+
+    def kernel(*a):
+        with torch.no_grad():
+            return gd.gated_delta_rule_update_ref(*a)
+
+    monkeypatch.setattr(nat, "gated_delta_update", kernel)
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    args = [r(2, 1, 4), r(2, 1, 4), r(2, 2, 3), -r(2, 2).abs(), r(2, 2).sigmoid(), r(2, 2, 4, 3)]
+    plain = gd.gated_delta_rule_update(*(x.clone() for x in args))
+    assert not plain.requires_grad
+    for i in range(6):
+        a = [x.clone() for x in args]
+        with torch.no_grad():
+            assert not gd.gated_delta_rule_update(*a[:i], a[i].requires_grad_(), *a[i + 1:]).requires_grad
+        a = [x.clone().requires_grad_(j == i) for j, x in enumerate(args)]
+        out = gd.gated_delta_rule_update(*a)
+        assert torch.equal(out, plain)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            out.sum().backward()
+    for i in range(5):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(lambda x: gd.gated_delta_rule_update(*args[:i], x, *args[i + 1:]), (args[i],), (args[i],))
+        with pytest.raises(RuntimeError):
+            with torch.autograd.forward_ad.dual_level():
+                a = list(args)
+                a[i] = torch.autograd.forward_ad.make_dual(a[i], a[i])
+                gd.gated_delta_rule_update(*a)
