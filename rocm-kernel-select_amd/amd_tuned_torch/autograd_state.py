@@ -27,6 +27,12 @@ def transformed(*tensors) -> bool:
     return _forward_ad._current_level >= 0 and _dual(tensors)
 
 
+def recorded(*tensors) -> bool:
+    """transformed(), or torch.jit.trace is recording: a kernel's work is in no trace, which would return
+    memory that nothing wrote."""
+    return torch._C._is_tracing() or transformed(*tensors)
+
+
 def graph_wanted(grad_output, *saved) -> bool:
     """In a backward: True when the gradients must come from differentiable ops -- they are to be
     differentiated again (create_graph=True), or the incoming gradient is batched

@@ -120,10 +120,12 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     cu_seqlens[n + 1] (not decreasing); tokens of no sequence get an output, and a gradient, of zero.
     scale: dim_k ** -0.5 by default.  Keys are used as they come: with unit length and beta in [0, 1]
     the state cannot grow."""
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)  # (a trace has sizes as tensors)
     if autograd_state.transformed(q, k, v, g, beta, initial_state):
         return gated_delta_rule_ref(q, k, v, g, beta, scale, initial_state, return_final_state, cu_seqlens)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state)):
+    # (a trace records the function, to be called with whatever lengths come; the kernels' own work it cannot)
+    if torch._C._is_tracing() or torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state)):
         return GatedDeltaFn.apply(q, k, v, g, beta, scale, initial_state, return_final_state, cu_seqlens)
     out, state = _native.gated_delta(q, k, v, g, beta, scale, initial_state, cu_seqlens, return_final_state)
     return (out, state) if return_final_state else out
@@ -151,10 +153,10 @@ def gated_delta_rule_update(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g
     different; one outside [0, slots) marks a row of padding, whose output is zero.  Without it the
     state has one slot a sequence.  scale: dim_k ** -0.5 by default.  For decoding: it has no gradient,
     and a backward that comes to it, or a tangent, is an error."""
-    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
                                     or beta.requires_grad or state.requires_grad) \
-            or autograd_state.transformed(q, k, v, g, beta, state):
+            or autograd_state.recorded(q, k, v, g, beta, state):
         return GatedDeltaUpdateFn.apply(q, k, v, g, beta, state, scale, state_indices)
     return _native.gated_delta_update(q, k, v, g, beta, state, scale, state_indices)
 

@@ -75,13 +75,35 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
              residual: Optional[torch.Tensor] = None):
     """x (..., N), weight (N,) of x's dtype or float32, residual like x; returns y, or (y, h) with a
     residual, h = x + residual."""
-    if autograd_state.transformed(x, weight, residual):
+    if autograd_state.recorded(x, weight, residual):
         return rms_norm_ref(x, weight, eps, residual)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
                                     or (residual is not None and residual.requires_grad)):
         return RmsNormFn.apply(x, weight, eps, residual)
     y, h, _, _ = _native.rms_norm(x, weight, eps, residual)
     return y if residual is None else (y, h)
+
+
+_TOP = {torch.float8_e4m3fn: 448.0, torch.int8: 127.0}
+
+
+def rms_norm_quant_ref(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       residual: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float8_e4m3fn,
+                       group_size: Optional[int] = None):
+    """rms_norm_quant in torch operations."""
+    acc = torch.promote_types(x.dtype, torch.float32)
+    h = x if residual is None else (x.to(acc) + residual.to(acc)).to(x.dtype)
+    y = rms_norm_ref(h.to(acc), weight, eps)
+    n, top = x.shape[-1], _TOP[dtype]
+    width = group_size or max(n, 1)
+    y = torch.nn.functional.pad(y, (0, -n % width)).unflatten(-1, (-1, width)) if n else y[..., None, :]
+    amax = y.abs().amax(-1, keepdim=True) if n else y.new_zeros(y.shape[:-1] + (1,))
+    scales = (amax / top).clamp_min(2.0 ** -126)
+    q = (y * (1 / scales)).clamp(-top, top).flatten(-2)[..., :n]
+    if dtype == torch.int8:
+        q = torch.where(q.isnan(), -top, q.round())  # (what the kernel stores; the scale is NaN)
+    q, scales = q.to(dtype), scales.squeeze(-1)
+    return (q, scales) if residual is None else (q, scales, h)
 
 
 def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
@@ -92,5 +114,7 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: 
     group_size (a power of two from 16 to 256)."""
     if dtype is None:
         raise RuntimeError("rms_norm: 8-bit outputs are torch.float8_e4m3fn and torch.int8")
+    if torch._C._is_tracing():
+        return rms_norm_quant_ref(x, weight, eps, residual, dtype, group_size)
     y, h, _, scales = _native.rms_norm(x, weight, eps, residual, quant=dtype, group=group_size or 0)
     return (y, scales) if residual is None else (y, scales, h)

@@ -247,3 +247,87 @@ def test_decode_step_has_no_gradient_and_says_so(nat, monkeypatch):
                 a = list(args)
                 a[i] = torch.autograd.forward_ad.make_dual(a[i], a[i])
                 gd.gated_delta_rule_update(*a)
+
+
+def unrecorded(fn):
+    """`fn` as a kernel is to autograd and to traces: its results appear in fresh memory."""
+    def kernel(*a, **kw):
+        arrays = [x.detach().numpy() if isinstance(x, torch.Tensor) else x for x in a]
+        out = []
+
+        def work():
+            with torch.no_grad():
+                out.append(fn(*[torch.from_numpy(x) if hasattr(x, "ctypes") else x for x in arrays], **kw))
+
+        import threading
+        thread = threading.Thread(target=work)     # (a trace records its own thread)
+        thread.start()
+        thread.join()
+        got = out[0] if isinstance(out[0], tuple) else (out[0],)
+        fresh = [None if x is None else torch.empty(x.shape, dtype=x.dtype) for x in got]
+        for to, x in zip(fresh, got):
+            if x is not None:
+                import ctypes
+                ctypes.memmove(to.data_ptr(), x.contiguous().data_ptr(), x.numel() * x.element_size())
+        return tuple(fresh) if isinstance(out[0], tuple) else fresh[0]
+    return kernel
+
+
+def test_traces(nat, monkeypatch):
+    """What torch.jit.trace records computes the operators on other inputs, of other lengths too."""
+    import amd_tuned_torch as att
+    from amd_tuned_torch import gated_delta as gd
+
+    def rule(q, k, v, g, beta, scale, initial_state=None, cu_seqlens=None, want_state=False):
+        out, state = gd.gated_delta_rule_ref(q, k, v, g, beta, scale, initial_state, True, cu_seqlens)
+        return out, state if want_state else None
+
+    monkeypatch.setattr(nat, "gated_delta", unrecorded(rule))
+    monkeypatch.setattr(nat, "gated_delta_update", unrecorded(gd.gated_delta_rule_update_ref))
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    seqs = lambda t: (r(1, t, 1, 4), r(1, t, 1, 4), r(1, t, 2, 3), -r(1, t, 2).abs(), r(1, t, 2).sigmoid())  # noqa: E731
+    token = lambda: (r(2, 1, 4), r(2, 1, 4), r(2, 2, 3), -r(2, 2).abs(), r(2, 2).sigmoid(), r(2, 2, 4, 3))  # noqa: E731
+    rows = lambda m: (r(m, 40), r(40), r(m, 40))  # noqa: E731
+    cases = [(lambda *a: att.gated_delta_rule(*a), seqs(5), seqs(7)),
+             (lambda *a: att.gated_delta_rule(*a, return_final_state=True), seqs(5), seqs(3)),
+             (lambda *a: att.gated_delta_rule_update(*a), token(), token()),
+             (lambda x, w, h: att.rms_norm(x, w, residual=h), rows(3), rows(5)),
+             (lambda x, w, h: att.rms_norm(x, w), rows(3), rows(5)),
+             (lambda x, w, h: att.rms_norm_quant(x, w, residual=h), rows(3), rows(5)),
+             (lambda x, w, h: att.rms_norm_quant(x, w, dtype=torch.int8, group_size=16), rows(3), rows(5))]
+    refs = {"rms_norm": att.rms_norm_ops.rms_norm_ref, "rms_norm_quant": att.rms_norm_ops.rms_norm_quant_ref}
+    for i, (fn, first, other) in enumerate(cases):
+        with torch.no_grad():
+            traced = torch.jit.trace(fn, tuple(x.clone() for x in first), check_trace=False)
+            got = traced(*(x.clone() for x in other))
+            with monkeypatch.context() as m:
+                for name, ref in refs.items():
+                    m.setattr(att, name, ref)
+                want = fn(*(x.clone() for x in other))
+        for a, b in zip(*(x if isinstance(x, tuple) else (x,) for x in (got, want))):
+            assert torch.equal(a.float(), b.float()), i
+
+
+@pytest.mark.parametrize("out", [torch.float8_e4m3fn, torch.int8])
+@pytest.mark.parametrize("n,group", [(0, None), (1, None), (40, None), (40, 16), (64, 32), (7, 16)])
+def test_statement_in_8_bits(n, group, out):
+    """Half a step of int8 or of fp8's 3 bits, and the scales of the definition; a NaN spoils its run."""
+    from amd_tuned_torch.rms_norm_ops import rms_norm_quant_ref
+    gen = torch.Generator().manual_seed(n)
+    x, w, res = (torch.randn(*s, generator=gen) for s in ((3, n), (n,), (3, n)))
+    top = 448.0 if out == torch.float8_e4m3fn else 127.0
+    q, s, h = rms_norm_quant_ref(x, w, 1e-6, res, out, group)
+    assert torch.equal(h, x + res) and q.dtype == out and q.shape == x.shape
+    assert s.shape == (3, -(-n // group) if group else 1)
+    y = h.double() / (h.double().square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+    wide = (s.repeat_interleave(group, -1)[:, :n] if group else s).double()
+    if n:
+        v = y / wide
+        half = 0.5 if out == torch.int8 else torch.maximum(v.abs() * 2.0 ** -4, torch.full_like(v, 2.0 ** -10))
+        assert ((q.double() - v).abs() <= half + 1e-4).all() and q.float().abs().max() <= top
+        x[1, 0] = float("nan")
+        q, s = rms_norm_quant_ref(x, w, 1e-6, None, out, group)
+        assert s[1].isnan().all() and s[[0, 2]].isfinite().all()
+    else:
+        assert s.eq(2.0 ** -126).all()

@@ -181,3 +181,50 @@ def test_chains_beyond_one_launch(dev, n, hv, gradients):
         del dout, dv_all
     del v
     torch.cuda.empty_cache()
+
+
+def programs(dev):
+    """(operator, inputs, other inputs), the others of another length."""
+    import amd_tuned_torch as P
+    gen = torch.Generator().manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen).to(dev)  # noqa: E731
+    seqs = lambda t: (r(1, t, 1, 32) / 6, r(1, t, 1, 32) / 6, r(1, t, 2, 36), -r(1, t, 2).abs(), r(1, t, 2).sigmoid())  # noqa: E731
+    token = lambda: (r(2, 1, 32) / 6, r(2, 1, 32) / 6, r(2, 2, 36), -r(2, 2).abs(), r(2, 2).sigmoid(), r(2, 2, 32, 36))  # noqa: E731
+    rows = lambda m: (r(m, 140), r(140), r(m, 140))  # noqa: E731
+    return [(lambda *a: P.gated_delta_rule(*a), seqs(70), seqs(133)),
+            (lambda *a: P.gated_delta_rule(*a, return_final_state=True), seqs(5), seqs(80)),
+            (lambda *a: P.gated_delta_rule_update(*a), token(), token()),
+            (lambda x, w, h: P.rms_norm(x, w, residual=h), rows(3), rows(5)),
+            (lambda x, w, h: P.rms_norm(x, w), rows(3), rows(5)),
+            (lambda x, w, h: P.rms_norm_quant(x, w, residual=h, dtype=torch.int8), rows(3), rows(5))]
+
+
+def check_program(fn, recorded, inputs):
+    """Outputs, and the state that a step overwrites, as the call's own: fp32 sums in another order at most,
+    64 roundings of 2^-24 of the largest value; 8-bit values a step apart at most."""
+    with torch.no_grad():
+        a, b = [x.clone() for x in inputs], [x.clone() for x in inputs]
+        want, got = fn(*a), recorded(*b)
+    want, got = (list(x) if isinstance(x, tuple) else [x] for x in (want, got))
+    for x, y in zip(got + b, want + a):
+        assert x.dtype == y.dtype and x.shape == y.shape
+        off = (x.double() - y.double()).abs().max()
+        assert off <= (1 if x.dtype == torch.int8 else 64 * 2.0 ** -24 * y.double().abs().max())
+
+
+def test_traces_on_the_device(dev):
+    for fn, first, other in programs(dev):
+        with torch.no_grad():
+            traced = torch.jit.trace(fn, tuple(x.clone() for x in first), check_trace=False)
+        check_program(fn, traced, first)
+        check_program(fn, traced, other)
+
+
+def test_compiled_functions(dev):
+    """Inside torch.compile the operators run as they are, between graphs."""
+    for fn, first, other in programs(dev):
+        torch._dynamo.reset()
+        compiled = torch.compile(lambda *a, fn=fn: fn(*[x + 0 for x in a[:5]], *a[5:]), backend="eager")
+        check_program(fn, compiled, first)
+        check_program(fn, compiled, other)
+    torch._dynamo.reset()
