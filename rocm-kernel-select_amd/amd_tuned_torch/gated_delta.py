@@ -119,7 +119,8 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     device, packs sequences into a batch of one: sequence n has tokens cu_seqlens[n] to
     cu_seqlens[n + 1] (not decreasing); tokens of no sequence get an output, and a gradient, of zero.
     scale: dim_k ** -0.5 by default.  Keys are used as they come: with unit length and beta in [0, 1]
-    the state cannot grow."""
+    the state cannot grow.  A value that is not finite spoils no token before its own; gradients it may
+    spoil throughout its 64 tokens, counted from the sequence's start."""
     scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)  # (a trace has sizes as tensors)
     if autograd_state.transformed(q, k, v, g, beta, initial_state):
         return gated_delta_rule_ref(q, k, v, g, beta, scale, initial_state, return_final_state, cu_seqlens)

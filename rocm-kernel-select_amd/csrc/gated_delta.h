@@ -178,6 +178,35 @@ __device__ __forceinline__ void mma_tiles(const uint4 (&a)[N][NA], const uint4 (
 // bits) are beyond what a 16-bit result shows
 template <typename T> inline constexpr int kOutParts = sizeof(T) == 4 ? 3 : 2;
 
+// A zero of a triangular factor times a NaN or an infinity is NaN, and would carry it to the tokens before
+// its own.  So what such a factor is multiplied with is clamped to numbers that bf16 has (a NaN too), and
+// the rows that the recurrence spoils, those from the first such one on, are made NaN afterwards.
+__device__ __forceinline__ float gdr_finite(float v) {
+  float most = 0x1.fep127f;
+  asm("" : "+s"(most));  // (a scalar register's, both signs)
+  return __builtin_amdgcn_fmed3f(v, -most, most);
+}
+// Whether any of N values is a NaN or an infinity.
+template <int N, typename V>
+__device__ __forceinline__ bool gdr_spoilt(const V& v) {
+  float z[2] = {0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) z[i & 1] = fmaf(v[i], 0.f, z[i & 1]);
+  return z[0] + z[1] != 0.f;
+}
+// The lane, computed here, and not kept in a register from before a loop for a branch that is hardly
+// ever taken.
+__device__ __forceinline__ int gdr_lane() {
+  int zero = 0;
+  asm volatile("" : "+v"(zero));
+  return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+}
+__device__ __forceinline__ float gdr_nan() {
+  int nan = 0x7fc00000;
+  asm volatile("" : "+v"(nan));
+  return __int_as_float(nan);
+}
+
 // exp(G_i - G_j) from G / ln 2 in two floats each: the difference of near sums is exact
 __device__ __forceinline__ float gdr_decay(float2 i, float2 j) {
   return __builtin_amdgcn_exp2f((i.x - j.x) + (i.y - j.y));

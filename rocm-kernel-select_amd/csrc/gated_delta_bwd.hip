@@ -14,7 +14,8 @@
 //   dK = [M K - beta exp(G) dR S^T] + [M^T K + N^T Q + (E U) dS'^T]      (k_t read, and written)
 //   dG_i = q_i . dq_i + k_i . (read part - written part)_i, and for the chunk's last token also
 //          exp(G_63) <S, dS'> + sum_j k_j . ((E U) dS'^T)_j;   dg = sums of dG from the chunk's end
-// Key heads that several value heads share get the sum over them in a fixed order: one workgroup has
+// What is not finite leaves no gradient finite that the recurrence spoils, but may spoil others of its chunk
+// (dg is a sum from the chunk's end).  Key heads that several value heads share get the sum over them in a fixed order: one workgroup has
 // a key head's whole group.
 #include "gated_delta_chain.h"
 
@@ -423,6 +424,7 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
   __shared__ uint2 nf[2][kTri * 3 * 64][2], mf[2][kTri * 3 * 64][2];  // N and M, their transposes
   __shared__ float2 gs[64];
   __shared__ float grown[64], rest[64], beta[64], dg_part[CW][64], dots[W];
+  __shared__ int spoilt;  // the first token whose e is not finite
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cw = wave % CW, m0 = wave / CW * MR;
@@ -492,6 +494,7 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
       }
     };
     load(0);
+    if (tid == 0) spoilt = kGdrC;
     if (tid < 64) {
       gs[tid] = a.gsum[hs * 64 + tid];
       grown[tid] = a.row[hs * 192 + tid];
@@ -514,6 +517,7 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
         const int unit = wave + W * u, m = unit & 3, i = 16 * m + c, col = v0 + 8 * g;
         const float x[8] = {ru[u][0][0], ru[u][0][1], ru[u][0][2], ru[u][0][3], ru[u][1][0], ru[u][1][1], ru[u][1][2], ru[u][1][3]};
         bf16x8 parts[3];
+        if (unit >= 4 && gdr_spoilt<8>(x)) atomicMin(&spoilt, i);
         split_parts<3, 8>(x, parts);
 #pragma unroll
         for (int p = 0; p < 3; ++p) st[(m * UNIT + NP + (unit < 4 ? 0 : 3) + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
@@ -636,7 +640,9 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
           const float d = j <= i ? bj * gdr_decay(gs[i], gj) : 0.f;
           nv[r] = j <= i ? a.scale * d * ne[x][r] : 0.f;
           mv[r] = j < i ? -beta[i] * d * me[x][r] : 0.f;
-          if (it[x] == jt[x] && i == j && i < rows) store_param(a.dbeta, a.b_dtype, (token + i) * a.Hv + h, me[x][r]);
+          // (e of later tokens may be finite all the same, where the recurrence's is not)
+          if (it[x] == jt[x] && i == j && i < rows)
+            store_param(a.dbeta, a.b_dtype, (token + i) * a.Hv + h, i > spoilt ? gdr_nan() : me[x][r]);
         }
         const int up = tri_upper(jt[x], it[x] >> 1) * 3 * 64 + lane, low = tri_lower(it[x], jt[x] >> 1) * 3 * 64;
         const int to = 4 * g + 16 * (c >> 2), at = (c & 3) + 4 * (jt[x] & 1);  // of element r = 0 among N's own

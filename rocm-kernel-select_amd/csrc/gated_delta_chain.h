@@ -162,6 +162,8 @@ __device__ __forceinline__ void gdr_chain(const GdrArgs& a, char* lds, int64_t b
 #pragma unroll
       for (int m = 0; m < 4; ++m) kp[wave][m][lane] = y[m];
       __syncthreads();
+      f32x4 rest, beta, spoilt;  // NaN where X is not finite, else 0
+      float all;
       {
         const f32x4 v = vl[wave][lane], y0 = kp[0][wave][lane], y1 = kp[1][wave][lane], y2 = kp[2][wave][lane], y3 = kp[3][wave][lane];
         const f32x4 grown = *reinterpret_cast<const f32x4*>(&rl[16 * wave + 4 * g]);
@@ -170,13 +172,24 @@ __device__ __forceinline__ void gdr_chain(const GdrArgs& a, char* lds, int64_t b
         bf16x4 parts[3];
 #pragma unroll
         for (int r = 0; r < 4; ++r) x[r] = v[r] - grown[r] * z[r];
+        __builtin_amdgcn_sched_barrier(0);  // (what follows would not fit the registers beside the partial sums)
+        rest = *reinterpret_cast<const f32x4*>(&rl[64 + 16 * wave + 4 * g]);
+        beta = *reinterpret_cast<const f32x4*>(&rl[128 + 16 * wave + 4 * g]);
+        all = rl[63];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          spoilt[r] = x[r] * 0.f;
+          x[r] = gdr_finite(x[r]);
+        }
         split_parts<3, 4>(x, parts);
 #pragma unroll
         for (int p = 0; p < 3; ++p) xl[wave >> 1][p][lane][wave & 1] = __builtin_bit_cast(uint2, parts[p]);
+        // U is not finite where X is not, so neither is the state after the chunk
+        if constexpr (!KEEP) {
+          beta += spoilt;
+          asm volatile("" : "+v"(beta));
+        }
       }
-      const f32x4 rest = *reinterpret_cast<const f32x4*>(&rl[64 + 16 * wave + 4 * g]);
-      const f32x4 beta = *reinterpret_cast<const f32x4*>(&rl[128 + 16 * wave + 4 * g]);
-      const float all = rl[63];
       __syncthreads();
       f32x4 e;
       {
@@ -199,6 +212,7 @@ __device__ __forceinline__ void gdr_chain(const GdrArgs& a, char* lds, int64_t b
         half(0);
         if (two) half(1);
         e = (part[0] + part[1]) + part[2];
+        if constexpr (KEEP) e += spoilt;
       }
       {
         float x[4];
@@ -370,11 +384,17 @@ __device__ __forceinline__ void gdr_chain(const GdrArgs& a, char* lds, int64_t b
         // ul is this chunk's for two barriers
         y = (y + z) * grown;
         z = zero;
+        float spoilt = 0.f;
         auto half = [&](int s, f32x4 w) {
           bf16x8 parts[OP];
           uint4 b[OP];
           const f32x4 lo = ul[2 * s][lane], hi = ul[2 * s + 1][lane];
-          const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            spoilt = fmaf(x[i], 0.f, spoilt);
+            x[i] = gdr_finite(x[i]);
+          }
           split_parts<OP, 8>(x, parts);
 #pragma unroll
           for (int p = 0; p < OP; ++p) b[p] = __builtin_bit_cast(uint4, parts[p]);
@@ -383,6 +403,15 @@ __device__ __forceinline__ void gdr_chain(const GdrArgs& a, char* lds, int64_t b
         y = half(0, y);
         if (two) z = half(1, z);
         y += z;
+        if (__any(spoilt != 0.f)) {  // rows from the first of this column's tokens on whose U is not finite
+          const int l = gdr_lane();
+          int first = kGdrC;
+#pragma nounroll
+          for (int i = 16 * m + 15; i >= 0; --i)
+            first = gdr_spoilt<1>(&reinterpret_cast<const float*>(&ul[i >> 4][16 * ((i >> 2) & 3) + (l & 15)])[i & 3]) ? i : first;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[r] = 16 * m + 4 * (l >> 4) + r < first ? y[r] : gdr_nan();
+        }
         // loads before the store: what waits for them would wait for a store in front of them too
         pf += more ? pstep : 0;
         load_p();

@@ -137,19 +137,37 @@ __device__ __forceinline__ void invert_below(float* A, int wave, int lane) {
   __syncthreads();
 }
 
-// The rows of a lower triangular 64 x 64 matrix (LDS) as fragments in three parts.
-__device__ __forceinline__ void write_lower(const float* __restrict__ M, uint4* __restrict__ out, int wave, int lane) {
+// The same row by row, a column of T a lane, for an A that is not finite or whose T is not: there the blocks
+// would multiply zeros with what is not, and spoil rows before the first.  One wave; slow, and hardly ever run.
+__device__ __forceinline__ void invert_by_rows(float* A) {
+  const int lane = gdr_lane();
+#pragma nounroll
+  for (int i = 0; i < kGdrC; ++i) {
+    float t = lane == i ? 1.f : 0.f;
+#pragma nounroll
+    for (int j = 0; j < i; ++j) t -= A[i * LD + j] * A[j * LD + lane];
+    __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses keep their order)
+    A[i * LD + lane] = t;
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// The rows of a lower triangular 64 x 64 matrix (LDS) as fragments in three parts; whether any is not finite.
+__device__ __forceinline__ bool write_lower(const float* __restrict__ M, uint4* __restrict__ out, int wave, int lane) {
   const int c = lane & 15, g = lane >> 4;
+  bool spoilt = false;
   for (int f = wave; f < kTri; f += 4) {
     const int m = f < 2 ? f : f / 2 + 1, s = f < 2 ? 0 : f & 1;
     float v[8];
     bf16x8 parts[3];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = M[(16 * m + c) * LD + 32 * s + gdr_at(g, i)];
+    spoilt |= gdr_spoilt<8>(v);
     split_parts<3, 8>(v, parts);
 #pragma unroll
     for (int p = 0; p < 3; ++p) out[(f * 3 + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
   }
+  return spoilt;
 }
 
 // Its columns: the rows of the transpose, an upper triangular matrix.
@@ -211,6 +229,7 @@ __global__ __launch_bounds__(256, (KP * kParts<T> <= 128 ? 4 : 1)) void gdr_prep
   __shared__ __align__(16) float wm[64 * LD];
   __shared__ float2 gd[2][64];
   __shared__ float bs[2][64];
+  __shared__ int spoilt[2];  // whether a head's T is not finite
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t slot = blockIdx.x;
@@ -223,6 +242,7 @@ __global__ __launch_bounds__(256, (KP * kParts<T> <= 128 ? 4 : 1)) void gdr_prep
   const int64_t t0 = seq.begin + at;
   const bool owner = h0 % a.group == 0;
   const int64_t kbase = (hk * a.slots + slot) * (int64_t)(KS * 4 * NP * 64);
+  if (tid < 2) spoilt[tid] = 0;
   uint4 qr[KS][NP], kr[KS][NP];  // this wave's 16 tokens
   {
     const bool live = 16 * wave + c < rows;
@@ -360,8 +380,24 @@ __global__ __launch_bounds__(256, (KP * kParts<T> <= 128 ? 4 : 1)) void gdr_prep
     }
     __syncthreads();
     invert_below(wm, wave, lane);
-    write_lower(wm, a.tf + tbase, wave, lane);
+    if (write_lower(wm, a.tf + tbase, wave, lane)) spoilt[x] = 1;
     __syncthreads();
+    if (spoilt[x]) {
+      const int l = gdr_lane(), cl = l & 15, gl = l >> 4;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j <= wave)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int i = 16 * wave + 4 * gl + r, cj = 16 * j + cl;
+            if (cj < i) wm[i * LD + cj] = kk[j][r] * gdr_decay(gd[x][i], gd[x][cj]) * bs[x][cj];
+          }
+      __syncthreads();
+      if (wave == 0) invert_by_rows(wm);
+      __syncthreads();
+      write_lower(wm, a.tf + tbase, wave, l);
+      __syncthreads();
+    }
     if constexpr (BWD) {  // and (1 + diag(beta) W)^-1, transposed
 #pragma unroll
       for (int j = 0; j < 4; ++j)

@@ -228,3 +228,137 @@ def test_compiled_functions(dev):
         check_program(fn, compiled, first)
         check_program(fn, compiled, other)
     torch._dynamo.reset()
+
+
+# ---------------------------------------------------------------------------------------------
+# what is not finite, in the chunked form
+# ---------------------------------------------------------------------------------------------
+def sequences(lead, hk, hv, dk, dv, dtype, dev, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*lead, *s, generator=gen)  # noqa: E731
+    q, k = (torch.nn.functional.normalize(r(hk, dk) + 0.3, dim=-1).to(dtype) for _ in range(2))
+    return [t.to(dev) for t in (q, k, r(hv, dv).to(dtype), -torch.exp(r(hv) - 1.5), torch.sigmoid(r(hv)).to(dtype))]
+
+
+def recurrence(args, scale, state):
+    """(out, final state) in 64 bits, token by token."""
+    q, k, v, g, beta = (t.double() for t in args)
+    rep = v.shape[2] // q.shape[2]
+    q, k = (t.repeat_interleave(rep, dim=2) for t in (q, k))
+    S, out = state.double(), []
+    for t in range(v.shape[1]):
+        S = S * g[:, t].exp()[..., None, None]
+        u = beta[:, t][..., None] * (v[:, t] - (S * k[:, t][..., None]).sum(-2))
+        S = S + k[:, t][..., None] * u[..., None, :]
+        out.append(scale * (S * q[:, t][..., None]).sum(-2))
+    return torch.stack(out, 1), S
+
+
+def finite_alike(got, want, what):
+    """Finite where the recurrence is, and there as near to it as any call: one rounding of the type, and
+    512 of 2^-24 of the largest value."""
+    ok = want.isfinite()
+    assert torch.equal(got.isfinite(), ok), what
+    ulp = {torch.float32: 0.0, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[got.dtype]
+    off = (got.double() - want).abs()[ok] - ulp * want.abs()[ok]
+    assert not off.numel() or off.max() <= 512 * 2.0 ** -24 * want[ok].abs().max(), what
+
+
+SPOILT = [(i, x) for i in range(5) for x in (float("nan"), float("inf"), float("-inf")) if (i, x) != (3, float("-inf"))]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 36), (200, 7)])
+def test_what_is_not_finite_stays_behind_its_token(dev, dk, dv, dtype):
+    """A value of q, k, v, g or beta spoils what the recurrence says it does: no earlier token, no other
+    column, head or sequence."""
+    import amd_tuned_torch as P
+    clean = sequences((2, 140), 2, 4, dk, dv, dtype, dev, seed=dk)
+    state = torch.randn(2, 4, dk, dv, generator=torch.Generator().manual_seed(1)).to(dev)
+    for t in (0, 1, 15, 16, 38, 63, 64, 70, 111, 139):
+        for i, value in SPOILT:
+            args = [x.clone() for x in clean]
+            args[i][(1, t, 1, 3) if i < 3 else (1, t, 1)] = value
+            want, want_s = recurrence(args, 0.2, state)
+            got, got_s = P.gated_delta_rule(*args, 0.2, initial_state=state, return_final_state=True)
+            finite_alike(got, want, (t, "qkvgb"[i], value))
+            finite_alike(got_s, want_s, (t, "qkvgb"[i], value, "state"))
+
+
+def test_several_that_are_not_finite(dev):
+    """In several columns, heads and chunks, in tokens out of order."""
+    import amd_tuned_torch as P
+    args = sequences((1, 200), 1, 3, 64, 48, torch.bfloat16, dev)
+    for t, h, c in ((50, 0, 3), (10, 0, 4), (20, 0, 3), (63, 0, 20), (130, 0, 47), (64, 1, 0), (100, 1, 17), (99, 1, 16)):
+        args[2][0, t, h, c] = float("inf") if t % 2 else float("nan")
+    args[4][0, 180, 1] = float("nan")
+    state = torch.zeros(1, 3, 64, 48, device=dev)
+    want, want_s = recurrence(args, 0.2, state)
+    got, got_s = P.gated_delta_rule(*args, 0.2, return_final_state=True)
+    finite_alike(got, want, "out")
+    finite_alike(got_s, want_s, "state")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_growth_beyond_fp32_stays_behind(dev, dtype):
+    """Keys so long that errors grow by 1e3 a token from token 70 on: tokens before the overflow are finite,
+    those long after it are not."""
+    import amd_tuned_torch as P
+    args = sequences((1, 140), 1, 2, 64, 32, dtype, dev)
+    args[1][:, 70:] *= 40
+    state = torch.zeros(1, 2, 64, 32, device=dev)
+    want, _ = recurrence(args, 0.2, state)
+    got = P.gated_delta_rule(*args, 0.2)
+    size = want.abs().amax((0, 2, 3)).cummax(0).values
+    assert size[70] < 1e3 and size[-1] > 1e60
+    assert got[:, size < 1e25].isfinite().all() and not got[:, size > 1e45].isfinite().any()
+    assert (got[:, :70].double() - want[:, :70]).abs().max() <= 2.0 ** -7 * want[:, :70].abs().max()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_other_sequences_know_nothing_of_it(dev, dtype):
+    """Packed sequences beside a spoilt one have equal bits to those beside a clean one, gradients too."""
+    import amd_tuned_torch as P
+    clean = sequences((1, 200), 1, 2, 64, 36, dtype, dev)
+    cu = torch.tensor([0, 30, 95, 200], dtype=torch.int32, device=dev)
+    dout = torch.randn(1, 200, 2, 36, generator=torch.Generator().manual_seed(3)).to(dtype).to(dev)
+    results = []
+    for i in (None, 0, 1, 2, 3, 4):
+        args = [x.clone() for x in clean]
+        if i is not None:
+            args[i][0, 30:95:9] = float("nan")
+        leaves = [x.requires_grad_() for x in args]
+        out, state = P.gated_delta_rule(*leaves, return_final_state=True, cu_seqlens=cu)
+        results.append([x[:, at] for x in (out, *torch.autograd.grad(out, leaves, dout))
+                        for at in (slice(0, 30), slice(95, 200))] + [state[[0, 2]]])
+    for other in results[1:]:
+        assert all(torch.equal(a, b) and b.isfinite().all() for a, b in zip(other, results[0]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradients_hide_nothing(dev, dtype):
+    """Where the recurrence's gradients are not finite, neither are the kernels'.  Within the chunk of what is
+    not finite they may have more of it; where they are finite they are as near as any gradient, and those of
+    other heads and sequences are all finite."""
+    import amd_tuned_torch as P
+    clean = sequences((2, 140), 1, 2, 64, 36, dtype, dev)
+    dout = torch.randn(2, 140, 2, 36, generator=torch.Generator().manual_seed(3)).to(dtype).to(dev)
+    ulp = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8}
+    for t in (0, 20, 64, 77, 139):
+        for i in range(5):
+            args = [x.clone() for x in clean]
+            args[i][(1, t, 0, 3) if i < 3 else (1, t, 0)] = float("nan")
+            leaves = [x.clone().requires_grad_() for x in args]
+            got = torch.autograd.grad(P.gated_delta_rule(*leaves, 0.2), leaves, dout)
+            wide = [x.detach().double().cpu().requires_grad_() for x in args]
+            out, _ = recurrence(wide, 0.2, torch.zeros(2, 2, 64, 36, dtype=torch.float64))
+            want = torch.autograd.grad((out * dout.double().cpu()).sum(), wide)
+            for name, a, b in zip("qkvgb", got, want):
+                a = a.cpu()
+                assert not (a.isfinite() & ~b.isfinite()).any(), (t, i, name)
+                assert a[0].isfinite().all() and (name in "qk" or a[1, :, 1].isfinite().all() or i < 2), (t, i, name)
+                ok = a.isfinite() & b.isfinite()
+                off = (a.double() - b).abs()[ok] - ulp[a.dtype] * b.abs()[ok]
+                assert off.max() <= 4 * 512 * 2.0 ** -24 * b[ok].abs().max(), (t, i, name)
+                if i == 2 and t >= 64:
+                    assert a[1, :t // 64 * 64].isfinite().all(), (t, name)
