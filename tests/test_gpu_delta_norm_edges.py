@@ -362,3 +362,54 @@ def test_gradients_hide_nothing(dev, dtype):
                 assert off.max() <= 4 * 512 * 2.0 ** -24 * b[ok].abs().max(), (t, i, name)
                 if i == 2 and t >= 64:
                     assert a[1, :t // 64 * 64].isfinite().all(), (t, name)
+
+
+# ---------------------------------------------------------------------------------------------
+# forms that programs use together: packed, in 16 bits, as views of one projection
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hk,hv,dk,dv", [(2, 4, 64, 48), (1, 3, 128, 100), (1, 1, 200, 33)])
+def test_packed_views_of_a_projection_in_16_bits(dev, hk, hv, dk, dv, dtype):
+    """q, k and v are slices of one row of a projection, sequences of unequal lengths (none, one, a chunk, more)
+    are packed with states; the result and every gradient, the projection's among them, against the recurrence
+    in 64 bits.  An output is rounded once (relative 2^-8 or 2^-11) after fp32 sums of a few hundred terms, 512
+    roundings of 2^-24 of the largest; a gradient has four times as much fp32 arithmetic behind it."""
+    import amd_tuned_torch as P
+    cu = [2, 2, 3, 67, 200, 231]
+    t, n, cols = 233, len(cu) - 1, 2 * hk * dk + hv * dv
+    gen = torch.Generator().manual_seed(dk)
+    r = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    q, k = (torch.nn.functional.normalize(r(1, t, hk, dk), dim=-1) for _ in range(2))
+    fused = torch.cat([q.flatten(2), k.flatten(2), r(1, t, hv * dv), r(1, t, 5)], -1).to(dtype).to(dev).requires_grad_()
+    g, beta = -torch.exp(r(1, t, hv) - 1.5).to(dev).requires_grad_(), r(1, t, hv).sigmoid().to(dtype).to(dev).requires_grad_()
+    state = r(n, hv, dk, dv).to(dev).requires_grad_()
+    dout, dstate = r(1, t, hv, dv).to(dtype).to(dev), r(n, hv, dk, dv).to(dev)
+    leaves = (fused, g, beta, state)
+
+    def split(x):
+        a, b, c, _ = x.split([hk * dk, hk * dk, hv * dv, 5], -1)
+        return a.unflatten(2, (hk, dk)), b.unflatten(2, (hk, dk)), c.unflatten(2, (hv, dv))
+
+    out, final = P.gated_delta_rule(*split(fused), g, beta, 0.2, state, True,
+                                    torch.tensor(cu, dtype=torch.int32, device=dev))
+    grads = torch.autograd.grad((out, final), leaves, (dout, dstate))
+    wide = [x.detach().double().cpu().requires_grad_() for x in leaves]
+    parts = split(wide[0])
+    want, finals = torch.zeros(1, t, hv, dv, dtype=torch.float64), []
+    for i, (a, b) in enumerate(zip(cu, cu[1:])):
+        if a == b:
+            finals.append(wide[3][i:i + 1])
+            continue
+        o, S = recurrence([x[:, a:b] for x in (*parts, wide[1], wide[2])], 0.2, wide[3][i:i + 1])
+        want = torch.cat([want[:, :a], o, want[:, b:]], 1)
+        finals.append(S)
+    want_s = torch.cat(finals)
+    want_g = torch.autograd.grad((want * dout.double().cpu()).sum() + (want_s * dstate.double().cpu()).sum(), wide)
+    assert cols + 5 == fused.shape[-1]
+    ulp = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 0.0}
+    regions = [slice(0, hk * dk), slice(hk * dk, 2 * hk * dk), slice(2 * hk * dk, cols), slice(cols, None)]
+    pairs = [(out, want, 1), (final, want_s, 1)] + [(a, b, 4) for a, b in zip(grads[1:], want_g[1:])] + \
+            [(grads[0][..., c], want_g[0][..., c], 4) for c in regions]
+    for i, (a, b, times) in enumerate(pairs):
+        off = (a.detach().double().cpu() - b).abs() - ulp[a.dtype] * b.abs()
+        assert off.max() <= times * 512 * 2.0 ** -24 * b.abs().max() + 1e-30, i
