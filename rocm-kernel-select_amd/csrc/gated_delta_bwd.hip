@@ -423,8 +423,7 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
   __shared__ uint4 st[4 * UNIT * 64];
   __shared__ uint2 nf[2][kTri * 3 * 64][2], mf[2][kTri * 3 * 64][2];  // N and M, their transposes
   __shared__ float2 gs[64];
-  __shared__ float grown[64], rest[64], beta[64], dg_part[CW][64], dots[W];
-  __shared__ int spoilt;  // the first token whose e is not finite
+  __shared__ float grown[64], rest[64], beta[64], dg_part[CW][64], dots[W], db[64];
   const int tid = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int cw = wave % CW, m0 = wave / CW * MR;
@@ -494,7 +493,6 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
       }
     };
     load(0);
-    if (tid == 0) spoilt = kGdrC;
     if (tid < 64) {
       gs[tid] = a.gsum[hs * 64 + tid];
       grown[tid] = a.row[hs * 192 + tid];
@@ -517,7 +515,6 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
         const int unit = wave + W * u, m = unit & 3, i = 16 * m + c, col = v0 + 8 * g;
         const float x[8] = {ru[u][0][0], ru[u][0][1], ru[u][0][2], ru[u][0][3], ru[u][1][0], ru[u][1][1], ru[u][1][2], ru[u][1][3]};
         bf16x8 parts[3];
-        if (unit >= 4 && gdr_spoilt<8>(x)) atomicMin(&spoilt, i);
         split_parts<3, 8>(x, parts);
 #pragma unroll
         for (int p = 0; p < 3; ++p) st[(m * UNIT + NP + (unit < 4 ? 0 : 3) + p) * 64 + lane] = __builtin_bit_cast(uint4, parts[p]);
@@ -640,9 +637,7 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
           const float d = j <= i ? bj * gdr_decay(gs[i], gj) : 0.f;
           nv[r] = j <= i ? a.scale * d * ne[x][r] : 0.f;
           mv[r] = j < i ? -beta[i] * d * me[x][r] : 0.f;
-          // (e of later tokens may be finite all the same, where the recurrence's is not)
-          if (it[x] == jt[x] && i == j && i < rows)
-            store_param(a.dbeta, a.b_dtype, (token + i) * a.Hv + h, i > spoilt ? gdr_nan() : me[x][r]);
+          if (it[x] == jt[x] && i == j) db[i] = me[x][r];
         }
         const int up = tri_upper(jt[x], it[x] >> 1) * 3 * 64 + lane, low = tri_lower(it[x], jt[x] >> 1) * 3 * 64;
         const int to = 4 * g + 16 * (c >> 2), at = (c & 3) + 4 * (jt[x] & 1);  // of element r = 0 among N's own
@@ -757,6 +752,9 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
       double s = 0.;
 #pragma unroll
       for (int w = 0; w < CW; ++w) s += (double)dg_part[w][lane];
+      // after a token whose e is not finite later ones may be finite here, where the recurrence's are not; their
+      // dq is not, so neither is dG
+      const float dbeta = db[lane] + (float)s * 0.f;
 #pragma unroll
       for (int w = 0; w < W; ++w) s += lane == 63 ? (double)dots[w] : 0.;
 #pragma unroll
@@ -764,7 +762,10 @@ __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {
         const double t = __shfl_down(s, off, 64);
         if (lane + off < 64) s += t;
       }
-      if (lane < rows) store_param(a.dg, a.g_dtype, (token + lane) * a.Hv + h, (float)s);
+      if (lane < rows) {
+        store_param(a.dg, a.g_dtype, (token + lane) * a.Hv + h, (float)s);
+        store_param(a.dbeta, a.b_dtype, (token + lane) * a.Hv + h, dbeta);
+      }
     }
     // (the next head's gs, grown .. are wave 0's to write and read after its first barrier; what else is
     // written then has no readers left, or comes after two barriers)

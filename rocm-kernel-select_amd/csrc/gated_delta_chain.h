@@ -384,38 +384,45 @@ __device__ __forceinline__ void gdr_chain(const GdrArgs& a, char* lds, int64_t b
         // ul is this chunk's for two barriers
         y = (y + z) * grown;
         z = zero;
-        float spoilt = 0.f;
-        auto half = [&](int s, f32x4 w) {
+        const f32x4 before = y;
+        auto half = [&](const uint4 (&p)[OP], int s, f32x4 w, bool clean) {
           bf16x8 parts[OP];
           uint4 b[OP];
           const f32x4 lo = ul[2 * s][lane], hi = ul[2 * s + 1][lane];
           float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          if (clean)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            spoilt = fmaf(x[i], 0.f, spoilt);
-            x[i] = gdr_finite(x[i]);
-          }
+            for (int i = 0; i < 8; ++i) x[i] = gdr_finite(x[i]);
           split_parts<OP, 8>(x, parts);
 #pragma unroll
-          for (int p = 0; p < OP; ++p) b[p] = __builtin_bit_cast(uint4, parts[p]);
-          return mma_parts<OP, OP>(pa[s], b, w);
+          for (int i = 0; i < OP; ++i) b[i] = __builtin_bit_cast(uint4, parts[i]);
+          return mma_parts<OP, OP>(p, b, w);
         };
-        y = half(0, y);
-        if (two) z = half(1, z);
+        y = half(pa[0], 0, y, false);
+        if (two) z = half(pa[1], 1, z, false);
         y += z;
-        if (__any(spoilt != 0.f)) {  // rows from the first of this column's tokens on whose U is not finite
+        // loads before the store: what waits for them would wait for a store in front of them too
+        const uint4* __restrict__ now = pf;
+        pf += more ? pstep : 0;
+        load_p();
+        __builtin_amdgcn_sched_barrier(0);
+        if (__any(gdr_spoilt<4>(y))) {  // again, without what is not finite
+          y = before;
           const int l = gdr_lane();
-          int first = kGdrC;
+#pragma nounroll
+          for (int s = 0; s <= (two ? 1 : 0); ++s) {
+            uint4 p[OP];
+#pragma unroll
+            for (int i = 0; i < OP; ++i) p[i] = now[(s * OP + i) * 64 + l];
+            y = half(p, s, y, true);
+          }
+          int first = kGdrC;  // of this column's tokens whose U is not finite
 #pragma nounroll
           for (int i = 16 * m + 15; i >= 0; --i)
             first = gdr_spoilt<1>(&reinterpret_cast<const float*>(&ul[i >> 4][16 * ((i >> 2) & 3) + (l & 15)])[i & 3]) ? i : first;
 #pragma unroll
           for (int r = 0; r < 4; ++r) y[r] = 16 * m + 4 * (l >> 4) + r < first ? y[r] : gdr_nan();
         }
-        // loads before the store: what waits for them would wait for a store in front of them too
-        pf += more ? pstep : 0;
-        load_p();
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int r = 0; r < 4; ++r) ol[m][4 * g + r][c] = from_f32<T>(a.scale * y[r]);
         __builtin_amdgcn_wave_barrier();

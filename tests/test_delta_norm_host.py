@@ -273,6 +273,7 @@ def unrecorded(fn):
     return kernel
 
 
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
 def test_traces(nat, monkeypatch):
     """What torch.jit.trace records computes the operators on other inputs, of other lengths too."""
     import amd_tuned_torch as att

@@ -212,6 +212,7 @@ def check_program(fn, recorded, inputs):
         assert off <= (1 if x.dtype == torch.int8 else 64 * 2.0 ** -24 * y.double().abs().max())
 
 
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
 def test_traces_on_the_device(dev):
     for fn, first, other in programs(dev):
         with torch.no_grad():
