@@ -31,7 +31,7 @@ __device__ __forceinline__ void store_param(void* p, int dtype, int64_t i, float
 // The chain of dS', built as the forward's: four waves pass the state's gradient on, 16 value columns
 // of it; four more make what needs dO alone, a chunk ahead: scale P^T dO and Q^T (scale exp(G) dO).
 // Bound by a step's time too, with the forward chain after it: 2048 tokens, 2 x 16 heads of 128 x 128 bf16,
-// twice 32 steps in 160 us, matrix units 12 % busy, 84 MB read and 197 MB written.
+// twice 32 steps in 160 to 166 us, matrix units 12 % busy, 84 MB read and 197 MB written.
 // FULL as there.
 template <typename T, int KP>
 struct GdrBwdLds {
@@ -412,7 +412,7 @@ __device__ __forceinline__ float row16_sum(float v) {
 // hold for each lane the elements that its accumulators have, so the row products of dG need no more
 // loads.  V8: value columns come in eights, so a lane's are all there or all not.
 // Bound by latency, one workgroup a CU and waves that wait about half of their time: 64 chunks, 8 and 16
-// heads of 128 x 128, bf16, in 93 us, 126 MB read and 39 MB written, matrix units 24 % busy.  (With four
+// heads of 128 x 128, bf16, in 93 to 96 us, 126 MB read and 40 MB written, matrix units 24 % busy.  (With four
 // waves, and S and dS' through LDS, 257 us.)
 template <typename T, int KP, bool V8>
 __global__ __launch_bounds__(512) void gdr_grads_kernel(GdrArgs a) {

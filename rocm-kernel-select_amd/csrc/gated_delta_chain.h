@@ -43,7 +43,7 @@ struct GdrChainLds {
 // make the chunk's outputs, off the chain.  A barrier orders LDS only; loads stay in flight across it.
 // All value tiles of a head read the same fragments, so each brings its share of the lines of the chunk
 // after next into their L2 (a word of each): what the next chunk's loads then find there took a step
-// longer than they have.  bf16, 8192 tokens, 32 heads of 128 x 128: 128 steps in 237 to 248 us, 1.9 us
+// longer than they have.  bf16, 8192 tokens, 32 heads of 128 x 128: 128 steps in 236 to 253 us, 1.9 us
 // each, the matrix units 22 % busy; a CU issues about 105 vector loads and stores a step, which is what
 // the step waits for beside the three products.  (All four waves on both the state and the outputs,
 // loads after each barrier: 943 us.)

@@ -220,7 +220,7 @@ __device__ __forceinline__ void write_products(const f32x4& lo, const f32x4& hi,
 // computed once for both.  The masked products leave the registers as fragments: a product's result has
 // the layout of its transpose's rows, so Q K^T comes out of K Q^T.  FULL: K is KP.
 // Bound by latency: loads, then the products, then the inverse's three dependent steps, then stores
-// (bf16, 8192 tokens, 16 and 32 heads of 128: 65 to 70 us for 224 MB written and 67 read, 4.3 TB/s; one
+// (bf16, 8192 tokens, 16 and 32 heads of 128: 69 to 74 us for 224 MB written and 35 read, 3.6 TB/s; one
 // chunk each of 16 heads: 11 us).
 template <typename T, int KP, bool BWD, bool FULL>
 __global__ __launch_bounds__(256, (KP * kParts<T> <= 128 ? 4 : 1)) void gdr_prepare_kernel(GdrArgs a, int heads) {
@@ -468,7 +468,8 @@ int gdr_prepare(const GdrArgs& a, int dtype, bool backward, hipStream_t s) {
 // whatever it holds (128 x 128, bf16, the one against the other.  1 sequence, 16 heads: 8 tokens 11.9 us
 // and 13.6, 10 tokens 14.2 and 13.6, 12 tokens 16.6 and 13.7; 4 sequences: 10 tokens 14.8 and 16.9, 12
 // tokens 16.9 and 17.0; 16 sequences, 32 heads: 10 tokens 44.8 and 59.4, 16 tokens 67.8 and 58.5).  Such
-// calls keep the state in registers and need no workspace.
+// calls keep the state in registers and need no workspace.  A packed row counts by its own length: those of
+// its sequences are on the device.
 static bool gdr_by_token(int64_t tokens) { return tokens <= 10; }
 
 // Checks a call and lays out its workspace: the bytes it takes, or 0 with *rc set.

@@ -11,7 +11,7 @@
 // between its loads and its stores, so the statistics need no second read; sums and maxima are fp32.
 // TPR threads share a row, VPT vectors of 16 input bytes each: a quarter wave for a head's 128
 // columns (four rows to a wave), one wave up to 2048, a workgroup above.  Measured, bf16, no input in any
-// cache: 8192 x 2048 with a residual 25 us for 134 MB, into fp8 by groups of 128 27 us for 118 MB, the
+// cache: 8192 x 2048 with a residual 25 us for 134 MB, into fp8 by groups of 128 27 to 31 us for 118 MB, the
 // backward with dw 32 us for 134 MB; 262144 x 128 23 us for 134 MB, 5.8 TB/s.
 #include "atk_common.h"
 
