@@ -121,7 +121,7 @@ def gated_delta_rule(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch
     scale: dim_k ** -0.5 by default.  Keys are used as they come: with unit length and beta in [0, 1]
     the state cannot grow.  A value that is not finite spoils no token before its own; gradients it may
     spoil throughout its 64 tokens, counted from the sequence's start."""
-    scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)  # (a trace has sizes as tensors)
+    scale = float(max(q.shape[-1], 1)) ** -0.5 if scale is None else float(scale)  # (a trace has sizes as tensors)
     if autograd_state.transformed(q, k, v, g, beta, initial_state):
         return gated_delta_rule_ref(q, k, v, g, beta, scale, initial_state, return_final_state, cu_seqlens)
     # (a trace records the function, to be called with whatever lengths come; the kernels' own work it cannot)
@@ -154,7 +154,7 @@ def gated_delta_rule_update(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g
     different; one outside [0, slots) marks a row of padding, whose output is zero.  Without it the
     state has one slot a sequence.  scale: dim_k ** -0.5 by default.  For decoding: it has no gradient,
     and a backward that comes to it, or a tangent, is an error."""
-    scale = float(q.shape[-1]) ** -0.5 if scale is None else float(scale)
+    scale = float(max(q.shape[-1], 1)) ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or g.requires_grad
                                     or beta.requires_grad or state.requires_grad) \
             or autograd_state.recorded(q, k, v, g, beta, state):

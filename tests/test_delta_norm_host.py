@@ -332,3 +332,14 @@ def test_statement_in_8_bits(n, group, out):
         assert s[1].isnan().all() and s[[0, 2]].isfinite().all()
     else:
         assert s.eq(2.0 ** -126).all()
+
+
+def test_heads_without_columns_are_refused(nat):
+    """By the operators' own checks, with the default scale too."""
+    import amd_tuned_torch as att
+    z = lambda *s: torch.zeros(s)  # noqa: E731
+    for dk, dv in ((0, 4), (4, 0)):
+        with pytest.raises(RuntimeError, match="no head empty"):
+            att.gated_delta_rule(z(1, 3, 1, dk), z(1, 3, 1, dk), z(1, 3, 2, dv), z(1, 3, 2), z(1, 3, 2))
+        with pytest.raises(RuntimeError, match="no head empty"):
+            att.gated_delta_rule_update(z(1, 1, dk), z(1, 1, dk), z(1, 2, dv), z(1, 2), z(1, 2), z(1, 2, dk, dv))
