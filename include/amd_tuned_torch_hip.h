@@ -676,6 +676,91 @@ size_t atk_gated_delta_bwd_workspace_bytes(const atk_gated_delta_args* a);
 int atk_gated_delta_bwd(const atk_gated_delta_args* a, const void* dout, const void* dfinal_state, void* dq, void* dk,
                         void* dv, void* dg, void* dbeta, void* dinitial_state);
 
+/* ---------------------------------------------------------------------------
+ * Root-mean-square norm with a gate (no counterpart in the reference; it stands between the mixer of a
+ * linear-attention block and the block's output projection), over each run of `group` columns:
+ *   y = x rstd weight act(gate),  rstd = 1 / sqrt(mean(x^2) + eps)
+ *   gate_first: u = x act(gate), y = u rstd weight, rstd = 1 / sqrt(mean(u^2) + eps)
+ * act ATK_GATE_SILU: z / (1 + exp(-z)); ATK_GATE_SIGMOID: 1 / (1 + exp(-z)).  x, gate: M rows of N
+ * elements of `dtype`, rows x_stride / gate_stride elements apart, any alignment; y dense.  weight [N] of
+ * `dtype` or fp32, NULL: ones.  N a multiple of group; group up to 16384 (fp32: 8192), up to 65535 groups.
+ * The backward reads the same arguments (not y) and dy, rows dy_stride apart; it writes dx, dgate (dense,
+ * `dtype`) and dw [N] of w_dtype, when given, which needs atk_rms_norm_gated_bwd_workspace_bytes of scratch
+ * (contents ignored) and is summed in a fixed order.
+ * ------------------------------------------------------------------------- */
+enum { ATK_GATE_SILU = 0, ATK_GATE_SIGMOID = 1 };
+typedef struct atk_rms_norm_gated_args {
+  const void* x; const void* gate; const void* weight; void* y;
+  int64_t M; int64_t N; int64_t group; int64_t x_stride; int64_t gate_stride;
+  float eps; int activation; int gate_first; int dtype; int w_dtype;
+  atk_stream_t stream;
+} atk_rms_norm_gated_args;
+int atk_rms_norm_gated_fwd(const atk_rms_norm_gated_args* a);
+size_t atk_rms_norm_gated_bwd_workspace_bytes(int64_t M, int64_t N, int64_t group, int dtype);
+int atk_rms_norm_gated_bwd(const atk_rms_norm_gated_args* a, const void* dy, int64_t dy_stride, void* dx, void* dgate,
+                           void* dw, void* workspace, size_t workspace_bytes);
+
+/* ---------------------------------------------------------------------------
+ * Rotary positions (no counterpart in the reference; in front of the mixers of attention blocks):
+ * queries q (N, T, Hq, D) and keys k (N, T, Hk, D) of `dtype`, each token's pairs of columns turned by
+ * angle = position * inv_freq[i], i < rot / 2, and scaled:
+ *   (a, b) -> scale (a cos - b sin, a sin + b cos)
+ * Pair i is columns i and i + rot / 2, or 2 i and 2 i + 1 where interleaved; columns from rot on are
+ * copied.  inverse: by the opposite angle (the gradient).  positions (N, T) of int32, or int64 with pos64,
+ * its strides in elements (0 shares an axis); NULL: offset + t.  inv_freq [rot / 2] fp32, or fp64 with
+ * freq64.  The strides of q and k are those of their first three axes, in elements, the last axis dense;
+ * q_out and k_out are dense.  Hq or Hk may be 0.  D up to 4096.
+ * ------------------------------------------------------------------------- */
+typedef struct atk_rotary_args {
+  const void* q; const void* k; void* q_out; void* k_out; const void* positions; const void* inv_freq;
+  int64_t q_stride[3]; int64_t k_stride[3]; int64_t pos_stride[2];
+  int64_t offset; int64_t N; int64_t T;
+  int Hq; int Hk; int D; int rot; int pos64; int freq64; int interleaved; int inverse; int dtype; float scale;
+  atk_stream_t stream;
+} atk_rotary_args;
+int atk_rotary(const atk_rotary_args* a);
+
+/* ---------------------------------------------------------------------------
+ * Linear attention with a decay for each head (no counterpart in the reference; a mixer of linear-attention
+ * blocks beside the gated delta rule).  For each sequence and value head h, with key head h / (Hv / Hk),
+ * the state S [K, V] in fp32:
+ *   S <- exp(g_t) S + k_t v_t^T;  out_t = scale S^T q_t
+ * One token of each of N sequences; arguments as for atk_gated_delta_update.  g (N, Hv), or one decay a
+ * head with g_stride_n 0.
+ * ------------------------------------------------------------------------- */
+typedef struct atk_linear_attn_update_args {
+  const void* q; const void* k; const void* v; const void* g;
+  void* state; void* out; const int* state_indices;
+  int64_t N; int64_t slots; int64_t state_stride;
+  int64_t q_stride_n; int64_t q_stride_h; int64_t k_stride_n; int64_t k_stride_h;
+  int64_t v_stride_n; int64_t v_stride_h; int64_t g_stride_n; int64_t g_stride_h;
+  int Hk; int Hv; int K; int V; int dtype; int g_dtype; float scale;
+  atk_stream_t stream;
+} atk_linear_attn_update_args;
+int atk_linear_attn_update(const atk_linear_attn_update_args* a);
+
+/* The same over whole sequences; arguments as for atk_gated_delta_fwd.  g (N, T, Hv), or with fixed_decay
+ * one decay a head (its strides of the first two axes 0).  The workspace (16-byte aligned, contents
+ * ignored) has atk_linear_attn_workspace_bytes of the same arguments: 0 for sequences that one workgroup a
+ * head goes through. */
+typedef struct atk_linear_attn_args {
+  const void* q; const void* k; const void* v; const void* g;
+  const void* initial_state; void* final_state; void* out; const int* cu_seqlens;
+  int64_t q_stride[3]; int64_t k_stride[3]; int64_t v_stride[3]; int64_t g_stride[3];
+  int64_t N; int64_t T;
+  int Hk; int Hv; int K; int V; int dtype; int g_dtype; int fixed_decay; float scale;
+  void* workspace; size_t workspace_bytes;
+  atk_stream_t stream;
+} atk_linear_attn_args;
+size_t atk_linear_attn_workspace_bytes(const atk_linear_attn_args* a);
+int atk_linear_attn_fwd(const atk_linear_attn_args* a);
+
+/* Its backward, arguments as for atk_gated_delta_bwd.  dg (NULL: not wanted) is (N, T, Hv), or [Hv] with
+ * fixed_decay; where a decay is below exp(-120) it is 0.  Sums over heads, columns and tokens have a fixed order. */
+size_t atk_linear_attn_bwd_workspace_bytes(const atk_linear_attn_args* a);
+int atk_linear_attn_bwd(const atk_linear_attn_args* a, const void* dout, const void* dfinal_state, void* dq, void* dk,
+                        void* dv, void* dg, void* dinitial_state);
+
 #ifdef __cplusplus
 }
 #endif

@@ -36,14 +36,18 @@ from . import compile_ops  # noqa: E402
 from . import depthwise_conv1d_ops  # noqa: E402
 from . import causal_conv1d  # noqa: E402
 from . import gated_delta  # noqa: E402
+from . import linear_attention_ops  # noqa: E402
 from . import rms_norm_ops  # noqa: E402
+from . import rotary_ops  # noqa: E402
 from . import miopen_fallback  # noqa: E402  (installs the F.conv1d wrapper at import)
 from . import _dispatch  # noqa: E402
 from ._dispatch import *  # noqa: E402,F401,F403
 from ._dispatch import enable, disable, is_enabled, ops  # noqa: E402
 from .conv_fusion_ops import group_norm_silu, replace_conv_blocks, unfuse_conv_blocks  # noqa: E402
 from .gated_delta import gated_delta_rule, gated_delta_rule_update  # noqa: E402
-from .rms_norm_ops import rms_norm, rms_norm_quant  # noqa: E402
+from .linear_attention_ops import linear_attention, linear_attention_update  # noqa: E402
+from .rms_norm_ops import rms_norm, rms_norm_gated, rms_norm_quant  # noqa: E402
+from .rotary_ops import rotary_embedding, rotary_frequencies  # noqa: E402
 
 __version__ = "0.1.0"
 

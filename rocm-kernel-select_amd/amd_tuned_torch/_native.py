@@ -55,6 +55,9 @@ EXPORTED_SYMBOLS = (
     "atk_causal_conv1d_update_args_fwd",
     "atk_rms_norm_fwd", "atk_rms_norm_bwd_workspace_bytes", "atk_rms_norm_bwd", "atk_gated_delta_update",
     "atk_gated_delta_workspace_bytes", "atk_gated_delta_fwd", "atk_gated_delta_bwd_workspace_bytes", "atk_gated_delta_bwd",
+    "atk_rms_norm_gated_fwd", "atk_rms_norm_gated_bwd_workspace_bytes", "atk_rms_norm_gated_bwd", "atk_rotary",
+    "atk_linear_attn_update", "atk_linear_attn_workspace_bytes", "atk_linear_attn_fwd",
+    "atk_linear_attn_bwd_workspace_bytes", "atk_linear_attn_bwd",
 )
 
 
@@ -121,6 +124,39 @@ class _DeltaArgs(ctypes.Structure):
                 + [(f, ctypes.c_int64 * 3) for f in ("q_stride", "k_stride", "v_stride", "g_stride", "beta_stride")]
                 + [("N", ctypes.c_int64), ("T", ctypes.c_int64)]
                 + [(f, ctypes.c_int) for f in ("Hk", "Hv", "K", "V", "dtype", "g_dtype", "beta_dtype")]
+                + [("scale", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
+                   ("stream", ctypes.c_void_p)])
+
+
+class _GatedArgs(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("x", "gate", "weight", "y")]
+                + [(f, ctypes.c_int64) for f in ("M", "N", "group", "x_stride", "gate_stride")]
+                + [("eps", ctypes.c_float)]
+                + [(f, ctypes.c_int) for f in ("activation", "gate_first", "dtype", "w_dtype")]
+                + [("stream", ctypes.c_void_p)])
+
+
+class _RotaryArgs(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("q", "k", "q_out", "k_out", "positions", "inv_freq")]
+                + [("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3), ("pos_stride", ctypes.c_int64 * 2)]
+                + [(f, ctypes.c_int64) for f in ("offset", "N", "T")]
+                + [(f, ctypes.c_int) for f in ("Hq", "Hk", "D", "rot", "pos64", "freq64", "interleaved", "inverse", "dtype")]
+                + [("scale", ctypes.c_float), ("stream", ctypes.c_void_p)])
+
+
+class _LinearUpdateArgs(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("q", "k", "v", "g", "state", "out", "state_indices")]
+                + [(f, ctypes.c_int64) for f in ("N", "slots", "state_stride", "q_stride_n", "q_stride_h", "k_stride_n",
+                                                 "k_stride_h", "v_stride_n", "v_stride_h", "g_stride_n", "g_stride_h")]
+                + [(f, ctypes.c_int) for f in ("Hk", "Hv", "K", "V", "dtype", "g_dtype")]
+                + [("scale", ctypes.c_float), ("stream", ctypes.c_void_p)])
+
+
+class _LinearArgs(ctypes.Structure):
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("q", "k", "v", "g", "initial_state", "final_state", "out", "cu_seqlens")]
+                + [(f, ctypes.c_int64 * 3) for f in ("q_stride", "k_stride", "v_stride", "g_stride")]
+                + [("N", ctypes.c_int64), ("T", ctypes.c_int64)]
+                + [(f, ctypes.c_int) for f in ("Hk", "Hv", "K", "V", "dtype", "g_dtype", "fixed_decay")]
                 + [("scale", ctypes.c_float), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t),
                    ("stream", ctypes.c_void_p)])
 
@@ -257,6 +293,16 @@ def _declare(lib) -> None:
     lib.atk_rms_norm_bwd_workspace_bytes.restype = sz
     lib.atk_rms_norm_bwd.argtypes = [vp] * 7 + [i64] * 5 + [i32, i32, vp, sz, vp]
     lib.atk_rms_norm_bwd.restype = i32
+    lib.atk_rms_norm_gated_bwd_workspace_bytes.argtypes = [i64, i64, i64, i32]
+    lib.atk_rms_norm_gated_bwd_workspace_bytes.restype = sz
+    lib.atk_rms_norm_gated_bwd.argtypes = [vp, vp, i64, vp, vp, vp, vp, sz]
+    lib.atk_rms_norm_gated_bwd.restype = i32
+    lib.atk_linear_attn_workspace_bytes.argtypes = [vp]
+    lib.atk_linear_attn_workspace_bytes.restype = sz
+    lib.atk_linear_attn_bwd_workspace_bytes.argtypes = [vp]
+    lib.atk_linear_attn_bwd_workspace_bytes.restype = sz
+    lib.atk_linear_attn_bwd.argtypes = [vp] * 8
+    lib.atk_linear_attn_bwd.restype = i32
     lib.atk_group_norm_noalloc_scratch_bytes.argtypes = []
     lib.atk_group_norm_noalloc_scratch_bytes.restype = sz
     lib.atk_group_norm_fwd_noalloc.argtypes = [vp, vp, vp, vp, i64, i64, i64, i32, c.c_float, i32, i32, i32,
@@ -264,7 +310,8 @@ def _declare(lib) -> None:
     lib.atk_group_norm_fwd_noalloc.restype = i32
     for name in ("atk_dwconv1d_fwd_args", "atk_group_norm_fwd_args", "atk_conv_fwd_prepacked_args",
                  "atk_causal_conv1d_update_args_fwd", "atk_rms_norm_fwd", "atk_gated_delta_update",
-                 "atk_gated_delta_fwd"):
+                 "atk_gated_delta_fwd", "atk_rms_norm_gated_fwd", "atk_rotary", "atk_linear_attn_update",
+                 "atk_linear_attn_fwd"):
         getattr(lib, name).argtypes = [vp]
         getattr(lib, name).restype = i32
 
@@ -1817,3 +1864,361 @@ def gated_delta_backward(q, k, v, g, beta, scale: float, initial_state, cu_seqle
     blk[6] = None
     _check(rc, "gated_delta_rule backward")
     return (*grads, dstate)
+
+
+# ---------------------------------------------------------------------------
+# The gated norm, rotary positions and linear attention with a decay for each head
+# ---------------------------------------------------------------------------
+GATES = {"silu": 0, "sigmoid": 1}
+
+
+def _on(device: torch.device, fn, *args):
+    """fn(*args) with `device` the current one: a launch goes to the current device, whatever stream it names."""
+    if device.index == torch._C._cuda_getDevice():
+        return fn(*args)
+    with torch.cuda.device(device):
+        return fn(*args)
+
+
+def _gated_block(x, gate, weight, eps: float, group: int, activation: str, gate_first: bool):
+    """(struct, its address, x and gate as rows, weight), checked and filled but for the outputs."""
+    dt = x.dtype
+    if not x.is_cuda or dt not in _DTYPE_CODE or x.dim() < 1:
+        raise RuntimeError("rms_norm_gated: x must be a GPU tensor of float32, float16 or bfloat16 with at least one axis")
+    N = x.shape[-1]
+    if gate.shape != x.shape or gate.dtype != dt or gate.device != x.device:
+        raise RuntimeError("rms_norm_gated: gate must match x")
+    if weight is not None and (weight.dtype not in (dt, torch.float32) or weight.shape != (N,) or weight.device != x.device):
+        raise RuntimeError("rms_norm_gated: weight must be (N,) in x's dtype or float32, on x's device")
+    if activation not in GATES:
+        raise RuntimeError("rms_norm_gated: activation must be 'silu' or 'sigmoid'")
+    if group < 0 or (group and N % group):
+        raise RuntimeError("rms_norm_gated: group_size must divide the columns")
+    x, gate = _rows(x), _rows(gate)
+    if weight is not None and weight.stride(0) != 1:
+        weight = weight.contiguous()
+    blk = _block("gated", _GatedArgs)
+    a = blk[0]
+    xs, zs, wdt = _row_stride(x), _row_stride(gate), dt if weight is None else weight.dtype
+    M = x.numel() // N if N else 0
+    key = (M, N, xs, zs, group, eps, activation, gate_first, dt, wdt)
+    if blk[2] != key:
+        blk[2] = None  # until all fields are set
+        a.M, a.N, a.group, a.x_stride, a.gate_stride, a.eps = M, N, group or N, xs, zs, eps
+        a.activation, a.gate_first, a.dtype, a.w_dtype = GATES[activation], int(gate_first), _DTYPE_CODE[dt], _DTYPE_CODE[wdt]
+        blk[2] = key
+    a.x, a.gate, a.weight, a.stream = x.data_ptr(), gate.data_ptr(), _ptr(weight), _stream(x)
+    return a, blk[1], x, gate, weight
+
+
+def rms_norm_gated(x: torch.Tensor, gate: torch.Tensor, weight: Optional[torch.Tensor], eps: float, group: int = 0,
+                   activation: str = "silu", gate_first: bool = False) -> torch.Tensor:
+    """The norm over each run of `group` columns of x's last axis (0: all of it), times weight and the gate's
+    activation, which gate_first puts in front of the norm."""
+    a, at, x, gate, weight = _gated_block(x, gate, weight, eps, group, activation, gate_first)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if a.M == 0 or a.N == 0:
+        return y
+    a.y = y.data_ptr()
+    _check(_on(x.device, lib().atk_rms_norm_gated_fwd, at), "rms_norm_gated")
+    return y
+
+
+def rms_norm_gated_backward(dy: torch.Tensor, x: torch.Tensor, gate: torch.Tensor, weight: Optional[torch.Tensor], eps: float,
+                            group: int, activation: str, gate_first: bool, *, want_dw: bool = True):
+    """(dx, dgate, dw) of rms_norm_gated; dw in the weight's dtype, None when not wanted."""
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise RuntimeError("rms_norm_gated backward: the gradient must match the output")
+    a, at, x, gate, weight = _gated_block(x, gate, weight, eps, group, activation, gate_first)
+    dx, dz = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
+    want_dw = want_dw and weight is not None
+    if a.M == 0 or a.N == 0:
+        return dx, dz, (torch.zeros_like(weight) if want_dw else None)
+    dy = _rows(dy)
+    dw = torch.empty(a.N, dtype=weight.dtype, device=x.device) if want_dw else None
+    L, ws = lib(), None
+
+    def call():
+        nonlocal ws
+        if want_dw:
+            # of this call alone: graphs are captured on one stream and may be replayed on several at once
+            ws = torch.empty(_cached_size(L.atk_rms_norm_gated_bwd_workspace_bytes, a.M, a.N, a.group, a.dtype,
+                                          device=x.device.index), dtype=torch.uint8, device=x.device)
+        return L.atk_rms_norm_gated_bwd(at, dy.data_ptr(), _row_stride(dy), dx.data_ptr(), dz.data_ptr(), _ptr(dw), _ptr(ws),
+                                        0 if ws is None else ws.numel())
+
+    _check(_on(x.device, call), "rms_norm_gated backward")
+    return dx, dz, dw
+
+
+def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, positions, interleaved: bool, scale: float,
+           inverse: bool = False):
+    """(q, k) with their pairs of columns turned, k None where it is.  q (B, T, Hq, D), k (B, T, Hk, D), or without
+    the first axis; positions an int (the first token's) or an int32 / int64 tensor that broadcasts to (B, T)."""
+    blk = _block("rotary", _RotaryArgs)
+    a = blk[0]
+    tensor = isinstance(positions, torch.Tensor)
+    key = (q.shape, q.stride(), q.dtype, q.device, None if k is None else (k.shape, k.stride(), k.dtype, k.device),
+           inv_freq.shape, inv_freq.stride(), inv_freq.dtype, inv_freq.device,
+           (positions.shape, positions.stride(), positions.dtype, positions.device) if tensor else None, interleaved, scale, inverse)
+    if blk[2] != key:
+        _rotary_check(q, k, inv_freq, positions)
+        if q.stride(-1) != 1 or (k is not None and k.stride(-1) != 1) or (inv_freq.numel() > 1 and inv_freq.stride(0) != 1):
+            q = q if q.stride(-1) == 1 else q.contiguous()
+            k = k if k is None or k.stride(-1) == 1 else k.contiguous()
+            inv_freq = inv_freq.contiguous()
+            key = None
+        blk[2] = None  # until all fields are set
+        lead = q.dim() - 3
+        B, T = (q.shape[0], q.shape[1]) if lead else (1, q.shape[0])
+        for t, s in ((q, a.q_stride), (k, a.k_stride)):
+            if t is not None:
+                s[:] = (t.stride(0) if lead else 0, t.stride(lead), t.stride(lead + 1))
+        if tensor:
+            e = positions.expand(q.shape[:-2])
+            a.pos_stride[:] = (e.stride(0) if lead else 0, e.stride(lead))
+            a.pos64 = int(positions.dtype == torch.int64)
+        a.N, a.T, a.Hq, a.D = B, T, q.shape[-2], q.shape[-1]
+        a.Hk = 0 if k is None else k.shape[-2]
+        a.rot, a.freq64, a.interleaved, a.inverse = 2 * inv_freq.numel(), int(inv_freq.dtype == torch.float64), interleaved, inverse
+        a.dtype, a.scale = _DTYPE_CODE[q.dtype], scale
+        blk[2] = key
+    oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ok = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    if oq.numel() == 0 and (ok is None or ok.numel() == 0):
+        return oq, ok
+    a.q, a.k, a.q_out, a.k_out, a.inv_freq = q.data_ptr(), _ptr(k), oq.data_ptr(), _ptr(ok), inv_freq.data_ptr()
+    a.positions, a.offset, a.stream = (positions.data_ptr(), 0, _stream(q)) if tensor else (None, positions, _stream(q))
+    _check(_on(q.device, lib().atk_rotary, blk[1]), "rotary_embedding")
+    return oq, ok
+
+
+def _rotary_check(q, k, inv_freq, positions) -> None:
+    if not q.is_cuda or q.dtype not in _DTYPE_CODE or q.dim() not in (3, 4):
+        raise RuntimeError("rotary_embedding: q must be a GPU tensor (batch, seqlen, heads, dim) or (tokens, heads, dim) of "
+                           "float32, float16 or bfloat16")
+    if k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2] or k.shape[-1] != q.shape[-1]
+                          or k.dtype != q.dtype or k.device != q.device):
+        raise RuntimeError("rotary_embedding: k must match q in all but its heads")
+    if inv_freq.dim() != 1 or inv_freq.dtype not in (torch.float32, torch.float64) or inv_freq.device != q.device \
+            or 2 * inv_freq.numel() > q.shape[-1]:
+        raise RuntimeError("rotary_embedding: inv_freq must be (rot / 2,) of float32 or float64 on the same GPU, rot at most dim")
+    if isinstance(positions, torch.Tensor):
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
+            raise RuntimeError("rotary_embedding: positions must be int32 or int64 on the same GPU")
+        lead = q.shape[:-2]
+        fits = positions.dim() <= len(lead) and all(p in (1, n) for p, n in zip(reversed(positions.shape), reversed(lead)))
+        if not fits:
+            raise RuntimeError("rotary_embedding: positions must have an element for each token")
+    elif not isinstance(positions, int):
+        raise RuntimeError("rotary_embedding: positions must be an int or a tensor")
+
+
+def linear_attn_update(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, state: torch.Tensor, scale: float,
+                       state_indices: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token of linear attention for each sequence; `state` (slots, Hv, K, V) fp32 is updated in place.  q, k
+    (N, Hk, K), v (N, Hv, V) of one dtype, g (N, Hv) or (Hv,) of it or fp32; returns (N, Hv, V)."""
+    blk = _block("lau", _LinearUpdateArgs)
+    a = blk[0]
+    key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), g.shape, g.stride(), state.shape, state.stride(),
+           q.dtype, k.dtype, v.dtype, g.dtype, state.dtype, q.device, k.device, v.device, g.device, state.device, scale,
+           None if state_indices is None else (state_indices.shape, state_indices.stride(), state_indices.dtype,
+                                               state_indices.device))
+    if blk[2] != key:
+        _linear_update_check(q, k, v, g, state, state_indices)
+        if q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1 or (
+                state_indices is not None and not state_indices.is_contiguous()):
+            q, k, v = (t if t.stride(2) == 1 else t.contiguous() for t in (q, k, v))
+            state_indices = None if state_indices is None else state_indices.contiguous()
+            key = None
+        blk[2] = None  # until all fields are set
+        N, Hk, K = q.shape
+        a.N, a.slots, a.state_stride = N, state.shape[0], state.stride(0)
+        a.q_stride_n, a.q_stride_h = q.stride(0), q.stride(1)
+        a.k_stride_n, a.k_stride_h = k.stride(0), k.stride(1)
+        a.v_stride_n, a.v_stride_h = v.stride(0), v.stride(1)
+        a.g_stride_n, a.g_stride_h = g.stride() if g.dim() == 2 else (0, g.stride(0))
+        a.Hk, a.Hv, a.K, a.V, a.scale = Hk, v.shape[1], K, v.shape[2], scale
+        a.dtype, a.g_dtype = _DTYPE_CODE[q.dtype], _DTYPE_CODE[g.dtype]
+        blk[2] = key
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    if a.N == 0:
+        return out
+    a.q, a.k, a.v, a.g = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr()
+    a.state, a.out, a.state_indices, a.stream = state.data_ptr(), out.data_ptr(), _ptr(state_indices), _stream(q)
+    _check(_on(q.device, lib().atk_linear_attn_update, blk[1]), "linear_attention_update")
+    return out
+
+
+def _linear_update_check(q, k, v, g, state, state_indices) -> None:
+    if q.dim() != 3 or v.dim() != 3 or k.shape != q.shape or state.dim() != 4:
+        raise RuntimeError("linear_attention_update expects q, k (N, Hk, K), v (N, Hv, V), state (slots, Hv, K, V)")
+    N, Hk, K = q.shape
+    _, Hv, V = v.shape
+    dt, dev = q.dtype, q.device
+    if v.shape[0] != N or g.shape not in ((N, Hv), (Hv,)) or state.shape[1:] != (Hv, K, V):
+        raise RuntimeError("linear_attention_update: sizes of v, g and state must agree with q and k")
+    if Hk == 0 or K == 0 or V == 0 or Hv == 0 or Hv % Hk:
+        raise RuntimeError("linear_attention_update: value heads must be a multiple of key heads, and no head empty")
+    if dt not in _DTYPE_CODE or k.dtype != dt or v.dtype != dt or g.dtype not in (dt, torch.float32) \
+            or state.dtype != torch.float32:
+        raise RuntimeError("linear_attention_update: q, k and v must share a dtype (float32, float16 or bfloat16), "
+                           "g have it or float32, and the state be float32")
+    if not (q.is_cuda and k.device == dev and v.device == dev and g.device == dev and state.device == dev):
+        raise RuntimeError("linear_attention_update: all tensors must be on one GPU")
+    if not state[:1].is_contiguous() or (state.shape[0] > 1 and state.stride(0) < Hv * K * V):
+        raise RuntimeError("linear_attention_update: each slot of the state must be contiguous (it is updated in place)")
+    if state_indices is not None and (state_indices.dtype != torch.int32 or state_indices.shape != (N,)
+                                      or state_indices.device != dev):
+        raise RuntimeError("linear_attention_update: state_indices must be int32 (N,) on the same GPU")
+    if state_indices is None and state.shape[0] != N:
+        raise RuntimeError("linear_attention_update: without state_indices the state has one slot a sequence")
+
+
+def _linear_check(q, k, v, g, initial_state, cu_seqlens) -> int:
+    """Refuses what the kernels do not take; the number of sequences."""
+    if q.dim() != 4 or v.dim() != 4 or k.shape != q.shape:
+        raise RuntimeError("linear_attention expects q, k (B, T, Hk, K) and v (B, T, Hv, V)")
+    B, T, Hk, K = q.shape
+    Hv, V = v.shape[2:]
+    if v.shape[:2] != (B, T) or g.shape not in ((B, T, Hv), (Hv,)):
+        raise RuntimeError("linear_attention: sizes of v and g must agree with q and k")
+    if Hk == 0 or K == 0 or V == 0 or Hv == 0 or Hv % Hk:
+        raise RuntimeError("linear_attention: value heads must be a multiple of key heads, and no head empty")
+    dt, dev = q.dtype, q.device
+    if dt not in _DTYPE_CODE or k.dtype != dt or v.dtype != dt or g.dtype not in (dt, torch.float32):
+        raise RuntimeError("linear_attention: q, k and v must share a dtype (float32, float16 or bfloat16), and g have it "
+                           "or float32")
+    if not (q.is_cuda and k.device == dev and v.device == dev and g.device == dev):
+        raise RuntimeError("linear_attention: all tensors must be on one GPU")
+    n = B
+    if cu_seqlens is not None:
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 \
+                or cu_seqlens.device != dev or B != 1:
+            raise RuntimeError("linear_attention: cu_seqlens must be int32 (sequences + 1,) on the same GPU, with a "
+                               "batch of one")
+        n = cu_seqlens.numel() - 1
+    if initial_state is not None and (initial_state.shape != (n, Hv, K, V) or initial_state.dtype != torch.float32
+                                      or initial_state.device != dev):
+        raise RuntimeError("linear_attention: initial_state must be float32 (sequences, Hv, K, V) on the same GPU")
+    return n
+
+
+def _linear_block(q, k, v, g, scale, initial_state, cu_seqlens):
+    """This thread's argument block of a call on sequences, its pointers to the inputs and its stream set:
+    [struct, address, key, sequences, workspace bytes, the backward's, inputs that had to be copied].  What
+    the key holds is checked, and the rest of the struct filled, where it differs from the last call's."""
+    blk = getattr(_tls, "la", None)
+    if blk is None:
+        st = _LinearArgs()
+        blk = _tls.la = [st, ctypes.addressof(st), None, 0, 0, 0, None]
+    key = (q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), g.shape, g.stride(), q.dtype, k.dtype, v.dtype,
+           g.dtype, q.device, k.device, v.device, g.device, scale,
+           None if initial_state is None else (initial_state.shape, initial_state.stride(), initial_state.dtype,
+                                               initial_state.device),
+           None if cu_seqlens is None else (cu_seqlens.shape, cu_seqlens.stride(), cu_seqlens.dtype, cu_seqlens.device))
+    a = blk[0]
+    blk[6] = None
+    if blk[2] != key:
+        n = _linear_check(q, k, v, g, initial_state, cu_seqlens)
+        if q.stride(3) != 1 or k.stride(3) != 1 or v.stride(3) != 1 or not (
+                (initial_state is None or initial_state.is_contiguous()) and (cu_seqlens is None or cu_seqlens.is_contiguous())):
+            q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
+            initial_state = None if initial_state is None else initial_state.contiguous()
+            cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
+            blk[6] = (q, k, v, initial_state, cu_seqlens)
+            key = None
+        blk[2] = None  # until all fields are set
+        a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
+        a.fixed_decay = int(g.dim() == 1)
+        a.g_stride[:] = (0, 0, g.stride(0)) if g.dim() == 1 else g.stride()
+        a.N, a.T, a.Hk, a.Hv, a.K, a.V = n, q.shape[1], q.shape[2], v.shape[2], q.shape[3], v.shape[3]
+        a.dtype, a.g_dtype = _DTYPE_CODE[q.dtype], _DTYPE_CODE[g.dtype]
+        a.scale = scale
+        a.cu_seqlens = _ptr(cu_seqlens)  # the sizes below ask whether there are any
+        L = lib()
+        blk[2:6] = [key, n, _on(q.device, L.atk_linear_attn_workspace_bytes, blk[1]),
+                    _on(q.device, L.atk_linear_attn_bwd_workspace_bytes, blk[1])]
+    a.q, a.k, a.v, a.g = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr()
+    a.initial_state, a.cu_seqlens, a.stream = _ptr(initial_state), _ptr(cu_seqlens), _stream(q)
+    return blk
+
+
+def _narrow(q, v) -> int:
+    """Columns that heads of fewer than 16 bytes are padded to, or 0: the kernels load vectors."""
+    if q.dim() != 4 or v.dim() != 4 or not q.is_cuda:
+        return 0  # (refused later)
+    vec = 16 // q.element_size()
+    return vec if 0 < q.shape[3] < vec or 0 < v.shape[3] < vec else 0
+
+
+def _widen(vec, q, k, v, state):
+    K, V = max(vec, q.shape[3]), max(vec, v.shape[3])
+    pad = torch.nn.functional.pad
+    return (pad(q, (0, K - q.shape[3])), pad(k, (0, K - k.shape[3])), pad(v, (0, V - v.shape[3])),
+            None if state is None else pad(state, (0, V - state.shape[3], 0, K - state.shape[2])))
+
+
+def linear_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, scale: float,
+                initial_state: Optional[torch.Tensor] = None, cu_seqlens: Optional[torch.Tensor] = None,
+                want_state: bool = False):
+    """Linear attention over sequences: (out (B, T, Hv, V), final state fp32 (sequences, Hv, K, V) or None).
+    q, k (B, T, Hk, K), v (B, T, Hv, V) of one dtype, g (B, T, Hv) or (Hv,) of it or fp32."""
+    vec = _narrow(q, v)
+    if vec:
+        _linear_check(q, k, v, g, initial_state, cu_seqlens)
+        out, final = linear_attn(*_widen(vec, q, k, v, None)[:3], g, scale, _widen(vec, q, k, v, initial_state)[3], cu_seqlens,
+                                 want_state)
+        K, V = q.shape[3], v.shape[3]
+        return out[..., :V].contiguous(), None if final is None else final[:, :, :K, :V].contiguous()
+    blk = _linear_block(q, k, v, g, scale, initial_state, cu_seqlens)
+    a, n, device = blk[0], blk[3], v.device
+    out = torch.empty(v.shape, dtype=v.dtype, device=device)
+    final = torch.empty((n, v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=device) if want_state else None
+    if n == 0:
+        return out.zero_(), final
+    if out.numel() == 0 and final is None:
+        return out, final
+    # scratch of the length of the sequences: from torch's allocator, which gives it back to the stream
+    ws = torch.empty(blk[4], dtype=torch.uint8, device=device) if blk[4] else None
+    a.out, a.final_state, a.workspace, a.workspace_bytes = out.data_ptr(), _ptr(final), _ptr(ws), blk[4]
+    rc = _on(device, lib().atk_linear_attn_fwd, blk[1])
+    blk[6] = None
+    _check(rc, "linear_attention")
+    return out, final
+
+
+def linear_attn_backward(q, k, v, g, scale: float, initial_state, cu_seqlens, dout: torch.Tensor,
+                         dfinal: Optional[torch.Tensor], want_dstate: bool, want_dg: bool = True):
+    """(dq, dk, dv, dg or None, dinitial_state or None) of linear_attn: dout like its output, dfinal (fp32) the
+    gradient of its final state or None."""
+    if dout.shape != v.shape or dout.dtype != v.dtype or dout.device != v.device:
+        raise RuntimeError("linear_attention backward: the gradient must match the output")
+    vec = _narrow(q, v)
+    if vec:
+        _linear_check(q, k, v, g, initial_state, cu_seqlens)
+        K, V = q.shape[3], v.shape[3]
+        wq, wk, wv, ws0 = _widen(vec, q, k, v, initial_state)
+        dq, dk, dv, dg, ds = linear_attn_backward(wq, wk, wv, g, scale, ws0, cu_seqlens, _widen(vec, q, k, dout, None)[2],
+                                                  _widen(vec, q, k, v, dfinal)[3], want_dstate, want_dg)
+        return (dq[..., :K].contiguous(), dk[..., :K].contiguous(), dv[..., :V].contiguous(), dg,
+                None if ds is None else ds[:, :, :K, :V].contiguous())
+    blk = _linear_block(q, k, v, g, scale, initial_state, cu_seqlens)
+    a, n, device = blk[0], blk[3], v.device
+    make = torch.empty if n and v.numel() else torch.zeros
+    grads = [make(t.shape, dtype=t.dtype, device=device) for t in (q, k, v)]
+    dg = make(g.shape, dtype=g.dtype, device=device) if want_dg else None
+    dstate = None
+    if want_dstate:
+        dstate = torch.empty((n, v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=device)
+    if n == 0 or (v.numel() == 0 and dstate is None):
+        return (*grads, dg, dstate)
+    dout = dout.contiguous()
+    dfinal = None if dfinal is None else dfinal.contiguous()
+    ws = torch.empty(blk[5], dtype=torch.uint8, device=device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), blk[5]
+    rc = _on(device, lib().atk_linear_attn_bwd, blk[1], dout.data_ptr(), _ptr(dfinal), *[t.data_ptr() for t in grads],
+             _ptr(dg), _ptr(dstate))
+    blk[6] = None
+    _check(rc, "linear_attention backward")
+    return (*grads, dg, dstate)

@@ -4,6 +4,8 @@
     rms_norm(x, weight=None, eps=1e-6, residual=None) -> y, or (y, h) with a residual
     rms_norm_quant(x, weight=None, eps=1e-6, residual=None, dtype=torch.float8_e4m3fn,
                    group_size=None) -> (q, scales), or (q, scales, h)
+    rms_norm_gated(x, gate, weight=None, eps=1e-6, gate_first=False, activation="silu",
+                   group_size=None) -> y
 
 h = x + residual, rounded to x's dtype: the residual stream as the next layers read it, and what
 is normalised.  y = h / sqrt(mean(h^2) + eps) * weight.  q * scales stands for y: fp8 e4m3 or
@@ -11,6 +13,11 @@ int8, a scale for each row (its last axis 1) or for each run of `group_size` col
 one there.  GPU tensors
 of any row width up to 65536 (float32: 32768) and any row alignment.  `rms_norm` is differentiable;
 `rms_norm_quant` is for inference and records no gradient.
+
+rms_norm_gated is the norm between a linear-attention mixer and the block's output projection:
+y = x / sqrt(mean(x^2) + eps) * weight * act(gate), or with gate_first the norm of x * act(gate) times
+weight, over the whole last axis or over each run of `group_size` columns of it (up to 16384, float32:
+8192).  It is differentiable.
 """
 from __future__ import annotations
 
@@ -118,3 +125,54 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: 
         return rms_norm_quant_ref(x, weight, eps, residual, dtype, group_size)
     y, h, _, scales = _native.rms_norm(x, weight, eps, residual, quant=dtype, group=group_size or 0)
     return (y, scales) if residual is None else (y, scales, h)
+
+
+def rms_norm_gated_ref(x: torch.Tensor, gate: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       gate_first: bool = False, activation: str = "silu", group_size: Optional[int] = None):
+    """rms_norm_gated in torch operations (fp32 or wider, rounded once), differentiable any number of times."""
+    acc = torch.promote_types(x.dtype, torch.float32)
+    z = gate.to(acc)
+    act = torch.sigmoid(z) if activation == "sigmoid" else z * torch.sigmoid(z)
+    u = x.to(acc) * act if gate_first else x.to(acc)
+    if x.shape[-1]:
+        u = u.unflatten(-1, (-1, group_size or x.shape[-1]))
+        u = (u * torch.rsqrt(u.square().mean(-1, keepdim=True) + eps)).flatten(-2)
+    if weight is not None:
+        u = u * weight.to(acc)
+    return (u if gate_first else u * act).to(x.dtype)
+
+
+class RmsNormGatedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, weight, eps, gate_first, activation, group_size):
+        ctx.how = eps, gate_first, activation, group_size
+        ctx.save_for_backward(x, gate, weight)
+        return _native.rms_norm_gated(x, gate, weight, eps, group_size or 0, activation, gate_first)
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, gate, weight = ctx.saved_tensors
+        eps, gate_first, activation, group_size = ctx.how
+        if autograd_state.graph_wanted(dy, x, gate, weight):
+            need = ctx.needs_input_grad[:3]
+            with torch.enable_grad():  # at views: an input may be computed from another, or be the same tensor
+                inputs = [None if t is None else t.view_as(t) for t in (x, gate, weight)]
+                y = rms_norm_gated_ref(*inputs, eps, gate_first, activation, group_size)
+                wanted = [t for t, n in zip(inputs, need) if n]
+                grads = iter(torch.autograd.grad(y, wanted, dy, create_graph=True))
+            dx, dz, dw = (next(grads) if n else None for n in need)
+        else:
+            dx, dz, dw = _native.rms_norm_gated_backward(dy, x, gate, weight, eps, group_size or 0, activation, gate_first,
+                                                         want_dw=ctx.needs_input_grad[2])
+        return dx, dz, dw, None, None, None, None
+
+
+def rms_norm_gated(x: torch.Tensor, gate: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                   gate_first: bool = False, activation: str = "silu", group_size: Optional[int] = None) -> torch.Tensor:
+    """x (..., N), gate like x, weight (N,) of x's dtype or float32; activation "silu" (z * sigmoid(z)) or
+    "sigmoid"; group_size divides N."""
+    if autograd_state.recorded(x, gate, weight):
+        return rms_norm_gated_ref(x, gate, weight, eps, gate_first, activation, group_size)
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (weight is not None and weight.requires_grad)):
+        return RmsNormGatedFn.apply(x, gate, weight, eps, gate_first, activation, group_size)
+    return _native.rms_norm_gated(x, gate, weight, eps, group_size or 0, activation, gate_first)

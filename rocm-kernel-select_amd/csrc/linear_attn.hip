@@ -1,0 +1,552 @@
+// Linear attention with a decay for each head: the decode step over a cache of states, what joins the
+// segments of sequences, and the C entries.
+//
+//   S' = exp(g) S + k v^T;  o = scale S'^T q
+#include "linear_attn.h"
+
+namespace atk {
+namespace {
+
+struct LaStepArgs {
+  const void* q; const void* k; const void* v; const void* g;
+  float* state; void* o; const int* slots;
+  int64_t n, n_slots, state_stride;
+  int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh, g_sb, g_sh;  // strides in elements: sequence, head
+  int Hv, group, K, V, g_dtype;
+  float scale;
+};
+
+// The decode step is HBM-bound: the state is read and written once, past the caches' replacement
+// (nontemporal), since every other layer has gone through them by the next step.  A new element is stored
+// as soon as its old one is there; only o waits for a reduction over the rows.
+// A workgroup has NV * VW columns of one head's state: NV threads of VW columns side by side, 256 / NV
+// groups of rows, RPT rows a thread.
+template <typename T, int VW, int NV, int RPT>
+__global__ __launch_bounds__(256) void la_step_kernel(LaStepArgs a) {
+  constexpr int RG = 256 / NV, KL = (RG * RPT + 255) / 256;
+  __shared__ float kf[RG * RPT], qf[RG * RPT];
+  __shared__ float red[4][NV][VW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int cg = tid % NV, rg = tid / NV;
+  const int64_t n = blockIdx.z;
+  const int h = blockIdx.y, hk = h / a.group;
+  const int c0 = (blockIdx.x * NV + cg) * VW;
+  const int64_t slot = a.slots ? (int64_t)a.slots[n] : n;
+  T* __restrict__ o = static_cast<T*>(a.o) + (n * a.Hv + h) * (int64_t)a.V;
+  if (slot < 0 || slot >= a.n_slots) {  // a row of padding: no state, an output of zeros
+    if (rg == 0)
+#pragma unroll
+      for (int j = 0; j < VW; ++j)
+        if (c0 + j < a.V) o[c0 + j] = from_f32<T>(0.f);
+    return;
+  }
+  float* __restrict__ S = a.state + slot * a.state_stride + (int64_t)h * a.K * a.V;
+  const T* __restrict__ q = static_cast<const T*>(a.q) + n * a.q_sb + hk * a.q_sh;
+  const T* __restrict__ k = static_cast<const T*>(a.k) + n * a.k_sb + hk * a.k_sh;
+  const T* __restrict__ v = static_cast<const T*>(a.v) + n * a.v_sb + h * a.v_sh;
+  // every load before the first conversion, so that they are in flight together
+  T kr[KL], qr[KL], vr[VW];
+#pragma unroll
+  for (int z = 0; z < KL; ++z) {
+    const int r = tid + 256 * z, at = r < a.K ? r : 0;
+    kr[z] = k[at];
+    qr[z] = q[at];
+  }
+#pragma unroll
+  for (int j = 0; j < VW; ++j) vr[j] = v[c0 + j < a.V ? c0 + j : 0];
+  const GdrGate gr = gdr_gate_load(a.g, a.g_dtype, n * a.g_sb + h * a.g_sh);
+  float s[RPT][VW];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = rg + i * RG;
+    const bool in = r < a.K && c0 < a.V;
+    if constexpr (VW == 4) {
+      const uint4 t = in ? ld16<true>(S + (int64_t)r * a.V + c0) : make_uint4(0, 0, 0, 0);
+      s[i][0] = __uint_as_float(t.x); s[i][1] = __uint_as_float(t.y);
+      s[i][2] = __uint_as_float(t.z); s[i][3] = __uint_as_float(t.w);
+    } else {
+      s[i][0] = in ? S[(int64_t)r * a.V + c0] : 0.f;
+    }
+  }
+#pragma unroll
+  for (int z = 0; z < KL; ++z) {
+    const int r = tid + 256 * z;
+    if (r < RG * RPT) {
+      kf[r] = r < a.K ? to_f32(kr[z]) : 0.f;
+      qf[r] = r < a.K ? to_f32(qr[z]) : 0.f;
+    }
+  }
+  const float decay = expf(gdr_gate<T>(gr, a.g_dtype));
+  float vv[VW], p[VW];
+#pragma unroll
+  for (int j = 0; j < VW; ++j) {
+    vv[j] = to_f32(vr[j]);
+    p[j] = 0.f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = rg + i * RG;
+    const float kk = kf[r], qq = qf[r];
+    if (r < a.K && c0 < a.V) {
+      float x[VW];
+#pragma unroll
+      for (int j = 0; j < VW; ++j) {
+        x[j] = fmaf(decay, s[i][j], kk * vv[j]);
+        p[j] += x[j] * qq;
+      }
+      if constexpr (VW == 4) st16<true>(S + (int64_t)r * a.V + c0, pack16<float>(x));
+      else S[(int64_t)r * a.V + c0] = x[0];
+    }
+  }
+#pragma unroll
+  for (int off = NV; off < 64; off <<= 1)
+#pragma unroll
+    for (int j = 0; j < VW; ++j) p[j] += __shfl_xor(p[j], off, 64);
+  if (lane < NV)
+#pragma unroll
+    for (int j = 0; j < VW; ++j) red[wave][cg][j] = p[j];
+  __syncthreads();
+  if (rg == 0)
+#pragma unroll
+    for (int j = 0; j < VW; ++j)
+      if (c0 + j < a.V)
+        o[c0 + j] = from_f32<T>(a.scale * ((red[0][cg][j] + red[1][cg][j]) + (red[2][cg][j] + red[3][cg][j])));
+}
+
+template <typename T, int VW, int NV, int RPT>
+void launch_step(const LaStepArgs& a, hipStream_t s) {
+  const dim3 grid((unsigned)((a.V + NV * VW - 1) / (NV * VW)), (unsigned)a.Hv, (unsigned)a.n);
+  hipLaunchKernelGGL((la_step_kernel<T, VW, NV, RPT>), grid, dim3(256), 0, s, a);
+}
+template <typename T>
+void launch_step_typed(const LaStepArgs& a, hipStream_t s) {
+  const bool vec = a.V % 4 == 0 && aligned16(a.state) && a.state_stride % 4 == 0;
+  // 128 columns a workgroup where that is one for each CU at least; 32 below, to spread the state over the
+  // chip (as for the gated delta rule's step, whose traffic this has)
+  const bool wide = (a.V + 127) / 128 * (int64_t)a.Hv * a.n >= (device_cu_count() > 0 ? device_cu_count() : 256);
+  if (!vec) {
+    if (a.K <= 64) launch_step<T, 1, 64, 16>(a, s);
+    else if (a.K <= 128) launch_step<T, 1, 64, 32>(a, s);
+    else launch_step<T, 1, 64, 64>(a, s);
+  } else if (wide) {
+    if (a.K <= 64) launch_step<T, 4, 32, 8>(a, s);
+    else if (a.K <= 128) launch_step<T, 4, 32, 16>(a, s);
+    else launch_step<T, 4, 32, 32>(a, s);
+  } else {
+    if (a.K <= 64) launch_step<T, 4, 8, 2>(a, s);
+    else if (a.K <= 128) launch_step<T, 4, 8, 4>(a, s);
+    else launch_step<T, 4, 8, 8>(a, s);
+  }
+}
+
+// Segments joined: what each adds to the state becomes the state after it (in reverse, the gradient of the
+// state before it), in place.  A thread has VW elements of a state, all segments of a sequence.
+template <int VW>
+__global__ __launch_bounds__(256) void la_scan_kernel(LaArgs a, float* s0, float* s1, const float* decays, int per, int64_t first) {
+  const int64_t block = first + blockIdx.x;
+  const int64_t unit = block / per, n = unit / a.Hv;
+  const int h = (int)(unit - n * a.Hv);
+  const int64_t kv = (int64_t)a.K * a.V, i = ((block - unit * per) * 256 + threadIdx.x) * VW;
+  const bool rev = blockIdx.y;
+  if (i >= kv) return;
+  const LaSeq seq = la_seq(a, n);
+  const int64_t segs = la_segments(seq, a.seg);
+  const float* init = a.role[rev ? 2 : 0].s_first;
+  float run[VW];
+#pragma unroll
+  for (int j = 0; j < VW; ++j) run[j] = init ? init[(n * a.Hv + h) * kv + i + j] : 0.f;
+  const int64_t step = a.Hv * kv;
+  float* __restrict__ p = (rev ? s1 : s0) + (seq.slot + (rev ? segs - 1 : 0)) * step + h * kv + i;
+  const float* __restrict__ d = decays + ((rev ? a.slots : 0) + seq.slot + (rev ? segs - 1 : 0)) * a.Hv + h;
+  const int64_t ps = rev ? -step : step, ds = rev ? -a.Hv : a.Hv;
+  constexpr int U = 8;  // segments whose loads are in flight together
+  for (int64_t z = 0; z + 1 < segs; z += U) {
+    float t[U][VW], f[U];
+    const int64_t left = segs - 1 - z;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = u < left ? u : 0;
+      __builtin_memcpy(t[u], p + at * ps, 4 * VW);
+      f[u] = d[at * ds];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u < left) {
+#pragma unroll
+        for (int j = 0; j < VW; ++j) run[j] = fmaf(f[u], run[j], t[u][j]);
+        __builtin_memcpy(p + u * ps, run, 4 * VW);
+      }
+    p += U * ps;
+    d += U * ds;
+  }
+}
+
+// Sums of a gradient's parts, over value heads of a key head and tiles of value columns, rounded once.
+struct LaSumArgs {
+  const float* parts[2]; void* out[2];
+  int64_t count;  // elements of the gradient
+  int n;          // parts
+};
+template <typename T, int VW>
+__global__ __launch_bounds__(256) void la_sum_kernel(LaSumArgs a) {
+  const float* __restrict__ p = a.parts[blockIdx.y];
+  T* __restrict__ o = static_cast<T*>(a.out[blockIdx.y]);
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VW; i < a.count; i += (int64_t)gridDim.x * 256 * VW) {
+    float s[VW];
+    __builtin_memcpy(s, p + i, 4 * VW);
+    for (int k = 1; k < a.n; ++k) {
+      float t[VW];
+      __builtin_memcpy(t, p + k * a.count + i, 4 * VW);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) s[j] += t[j];
+    }
+    T e[VW];
+#pragma unroll
+    for (int j = 0; j < VW; ++j) e[j] = from_f32<T>(s[j]);
+    __builtin_memcpy(o + i, e, VW * sizeof(T));
+  }
+}
+
+// The gradient of a log decay: with q_t . dq_t - k_t . dk_t summed from t to the end of the segment, and the
+// inner product of the state there with its gradient.  A wave for each segment and head.  The sums cancel
+// where the decay is strong, so they are in 64 bits.
+struct LaGateArgs {
+  const float* qd; const float* kd; const float* x; void* dg; float* seg_sums;
+  int tiles;
+};
+template <typename G>
+__global__ __launch_bounds__(256) void la_gate_kernel(LaArgs a, LaGateArgs b) {
+  const int lane = threadIdx.x & 63;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t slot = unit / a.Hv;
+  const int h = (int)(unit - slot * a.Hv);
+  if (slot >= a.slots) return;
+  const int64_t n = la_seq_of_slot(a, slot);
+  const LaSeq seq = la_seq(a, n);
+  const int64_t z = slot - seq.slot, segs = la_segments(seq, a.seg);
+  const bool live = z >= 0 && z < segs;
+  const int64_t BT = a.B * a.T;
+  double carry = 0, all = 0;
+  if (live) {
+    const int64_t t0 = z * a.seg, left = seq.len - t0, len = left < a.seg ? left : a.seg;
+    const int64_t first = seq.batch * a.T + seq.begin + t0;
+    for (int t = 0; t < b.tiles; ++t) carry += (double)b.x[((int64_t)t * a.slots + slot) * a.Hv + h];
+    for (int64_t end = len; end > 0; end -= 64) {
+      const int64_t t = end - 1 - lane;  // the lane's token, from the end
+      const int64_t at = first + (t > 0 ? t : 0);
+      double v = 0;
+      for (int i = 0; i < b.tiles; ++i) {
+        const int64_t j = ((int64_t)i * a.Hv + h) * BT + at;
+        v += (double)b.qd[j] - (double)b.kd[j];
+      }
+      if (t < 0) v = 0;
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) {
+        const double o = __shfl_up(v, off, 64);
+        if (lane >= off) v += o;
+      }
+      const GdrGate gr = gdr_gate_load(a.g, a.g_dtype, seq.batch * a.g_s[0] + (seq.begin + t0 + (t > 0 ? t : 0)) * a.g_s[1] + h * a.g_s[2]);
+      const double dg = gdr_gate<G>(gr, a.g_dtype) < -120.f ? 0.0 : carry + v;
+      if (t >= 0) {
+        if (!a.fixed) static_cast<G*>(b.dg)[at * a.Hv + h] = from_f32<G>((float)dg);
+        all += dg;
+      }
+      carry += __shfl(v, 63, 64);
+    }
+  }
+  if (a.fixed) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off, 64);
+    if (lane == 0) b.seg_sums[h * a.slots + slot] = (float)all;
+  } else if (live && a.cu) {  // tokens of no sequence
+    if (n == 0 && z == 0)
+      for (int64_t t = lane; t < seq.begin; t += 64) static_cast<G*>(b.dg)[t * a.Hv + h] = from_f32<G>(0.f);
+    if (n == a.n - 1 && z == segs - 1)
+      for (int64_t t = seq.begin + seq.len + lane; t < a.T; t += 64) static_cast<G*>(b.dg)[t * a.Hv + h] = from_f32<G>(0.f);
+  }
+}
+// one decay a head: its gradient is the sum over all segments
+template <typename G>
+__global__ __launch_bounds__(256) void la_gate_sum_kernel(const float* __restrict__ sums, G* __restrict__ dg, int64_t slots) {
+  __shared__ double red[256];
+  double s = 0;
+  for (int64_t i = threadIdx.x; i < slots; i += 256) s += (double)sums[blockIdx.x * slots + i];
+  red[threadIdx.x] = s;
+  __syncthreads();
+  for (int k = 128; k >= 1; k >>= 1) {
+    if ((int)threadIdx.x < k) red[threadIdx.x] += red[threadIdx.x + k];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) dg[blockIdx.x] = from_f32<G>((float)red[0]);
+}
+
+struct LaPlan {
+  float* s_fwd; float* s_rev; float* decays; float* parts[2]; float* dots[2]; float* x; float* seg_sums;
+  int n_parts, k_tiles, a_tiles;
+  bool split;   // more than one segment
+  size_t bytes;
+};
+
+// Tokens of a segment.  A workgroup goes through one chunk after the other; segments of a sequence run at
+// once, for the price of their states.
+int64_t la_segment_tokens(const atk_linear_attn_args* p) {
+  const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
+  const double chunks = ((double)p->T / 64 + 1) * (p->cu_seqlens ? 1.0 : (double)p->N);
+  const double tiles = (p->V + 127) / 128;
+  int64_t per = (int64_t)(chunks * p->Hv * tiles / (double)(2 * cus)) + 1;
+  per = per < 4 ? 4 : per > 1024 ? 1024 : per;
+  return per * 64;
+}
+
+// Checks a call and lays out its workspace; *rc says why where it is refused.
+LaPlan la_plan(const atk_linear_attn_args* p, bool backward, LaArgs* a, int* rc) {
+  LaPlan L = {};
+  *rc = ATK_OK;
+  if (!p) return *rc = fail(ATK_EINVAL, "linear attention: null arguments"), L;
+  if (!dtype_ok(p->dtype) || !dtype_ok(p->g_dtype)) return *rc = fail(ATK_EINVAL, "linear attention: unknown dtype code"), L;
+  if (!gdr_gate_ok(p->g_dtype, p->dtype))
+    return *rc = fail(ATK_EINVAL, "linear attention: g must be of the inputs' type or fp32"), L;
+  if (p->N < 0 || p->T < 0 || p->Hk <= 0 || p->Hv <= 0 || p->K <= 0 || p->V <= 0)
+    return *rc = fail(ATK_EINVAL, "linear attention: bad sizes"), L;
+  if (p->Hv % p->Hk) return *rc = fail(ATK_EINVAL, "linear attention: value heads must be a multiple of key heads"), L;
+  const int vec = 16 / (int)dtype_size(p->dtype);
+  if (p->K > kLaMaxK || p->K < vec || p->V < vec || p->V > (1 << 24) || p->Hv > 65535 || p->N > 65535 ||
+      p->T >= ((int64_t)1 << 31) - 64)
+    return *rc = fail(ATK_UNSUPPORTED, "linear attention: heads of fewer than 16 bytes or more than %d key columns, more than "
+                      "65535 heads or sequences, or 2^31 tokens", kLaMaxK), L;
+  const int64_t seg = la_segment_tokens(p);
+  const double slots = p->cu_seqlens ? (double)(p->T / seg) + (double)p->N
+                                     : (double)(p->T > seg ? (p->T + seg - 1) / seg : 1) * (double)p->N;
+  if (slots * p->Hv > 2147483647.0 || (double)p->N * (double)p->T > 1e15)
+    return *rc = fail(ATK_UNSUPPORTED, "linear attention: too many sequences and heads"), L;
+  *a = LaArgs{};
+  a->g = p->g; a->cu = p->cu_seqlens; a->n = p->N; a->T = p->T; a->B = p->cu_seqlens ? 1 : p->N;
+  for (int i = 0; i < 3; ++i) a->g_s[i] = p->g_stride[i];
+  a->slots = (int64_t)slots; a->seg = seg;
+  a->Hk = p->Hk; a->Hv = p->Hv; a->group = p->Hv / p->Hk; a->K = p->K; a->V = p->V;
+  a->g_dtype = p->g_dtype; a->fixed = p->fixed_decay; a->scale = p->scale;
+  L.split = p->T > seg;
+  char* w = static_cast<char*>(p->workspace);
+  auto take = [&](size_t floats) {
+    float* q = w ? reinterpret_cast<float*>(w + L.bytes) : nullptr;
+    L.bytes += (floats * 4 + 15) / 16 * 16;
+    return q;
+  };
+  const size_t state = (size_t)a->slots * a->Hv * a->K * a->V, tokens = (size_t)a->B * a->T;
+  if (L.split) {
+    L.s_fwd = take(state);
+    L.decays = take((size_t)a->slots * a->Hv * (backward ? 2 : 1));
+    if (backward) L.s_rev = take(state);
+  }
+  if (backward) {
+    const int da = la_padded(a->V);
+    L.a_tiles = (a->V + da - 1) / da;
+    L.k_tiles = (a->K + 64 * la_wide(da, a->K) - 1) / (64 * la_wide(da, a->K));
+    L.n_parts = a->group * L.a_tiles;
+    if (L.n_parts > 1)
+      for (int i = 0; i < 2; ++i) L.parts[i] = take((size_t)L.n_parts * tokens * a->Hk * a->K);
+    for (int i = 0; i < 2; ++i) L.dots[i] = take((size_t)L.a_tiles * L.k_tiles * a->Hv * tokens);
+    L.x = take((size_t)L.a_tiles * L.k_tiles * a->slots * a->Hv);
+    if (a->fixed) L.seg_sums = take((size_t)a->slots * a->Hv);
+  }
+  return L;
+}
+
+void la_copy3(int64_t (&to)[3], const int64_t* from) {
+  for (int i = 0; i < 3; ++i) to[i] = from[i];
+}
+
+template <typename T>
+int la_scan(const LaArgs& a, float* s0, float* s1, const float* decays, int roles, hipStream_t s) {
+  const int64_t kv = (int64_t)a.K * a.V;
+  const bool vec = kv % 4 == 0 && (!a.role[0].s_first || aligned16(a.role[0].s_first)) && (roles < 2 || !a.role[2].s_first || aligned16(a.role[2].s_first));
+  const int64_t per = (kv + (vec ? 1023 : 255)) / (vec ? 1024 : 256), grid = per * a.Hv * a.n;
+  for (int64_t b = 0; b < grid; b += kLaBlocks / 2) {
+    const dim3 g((unsigned)(grid - b < kLaBlocks / 2 ? grid - b : kLaBlocks / 2), (unsigned)roles);
+    if (vec) hipLaunchKernelGGL((la_scan_kernel<4>), g, dim3(256), 0, s, a, s0, s1, decays, (int)per, b);
+    else hipLaunchKernelGGL((la_scan_kernel<1>), g, dim3(256), 0, s, a, s0, s1, decays, (int)per, b);
+    if (int rc = check_launch("la_scan_kernel")) return rc;
+  }
+  return ATK_OK;
+}
+
+template <typename T>
+int la_forward(const atk_linear_attn_args* p, LaArgs& a, const LaPlan& L, hipStream_t s) {
+  LaRole& r = a.role[0];
+  r = LaRole{};
+  r.a = p->q; r.b = p->k; r.c = p->v; r.a_key = r.b_key = 1;
+  la_copy3(r.a_s, p->q_stride); la_copy3(r.b_s, p->k_stride); la_copy3(r.c_s, p->v_stride);
+  r.AD = a.K; r.CD = a.V; r.a_tiles = 1; r.guard = 1;
+  r.s_first = static_cast<const float*>(p->initial_state); r.s_last = static_cast<float*>(p->final_state);
+  r.out = p->out;
+  if (L.split) {
+    r.s_between = L.s_fwd;
+    float* to[1] = {L.s_fwd};
+    if (int rc = la_launch_states<T>(a, 1, to, L.decays, s)) return rc;
+    if (int rc = la_scan<T>(a, L.s_fwd, nullptr, L.decays, 1, s)) return rc;
+  }
+  return la_launch_out<T>(a, 0, 1, false, s);
+}
+
+template <typename T, typename G>
+int la_gates(const LaArgs& a, const LaPlan& L, void* dg, hipStream_t s) {
+  LaGateArgs b = {L.dots[0], L.dots[1], L.x, dg, L.seg_sums, L.a_tiles * L.k_tiles};
+  hipLaunchKernelGGL((la_gate_kernel<G>), dim3((unsigned)((a.slots * a.Hv + 3) / 4)), dim3(256), 0, s, a, b);
+  if (int rc = check_launch("la_gate_kernel")) return rc;
+  if (!a.fixed) return ATK_OK;
+  hipLaunchKernelGGL((la_gate_sum_kernel<G>), dim3((unsigned)a.Hv), dim3(256), 0, s, L.seg_sums, static_cast<G*>(dg), a.slots);
+  return check_launch("la_gate_sum_kernel");
+}
+
+template <typename T>
+int la_backward(const atk_linear_attn_args* p, LaArgs& a, const LaPlan& L, const void* dout, const float* ds1, void* dq,
+                void* dk, void* dv, void* dg, float* ds0, hipStream_t s) {
+  const int64_t vs[3] = {a.T * a.Hv * a.V, (int64_t)a.Hv * a.V, a.V};  // dout's strides
+  // roles 0 and 1: dq and dk; role 2: dv
+  LaRole& q = a.role[0];
+  LaRole& k = a.role[1];
+  LaRole& v = a.role[2];
+  q = k = v = LaRole{};
+  q.a = dout; q.b = p->v; q.c = p->k; q.e = p->q; q.c_key = 1;
+  la_copy3(q.a_s, vs); la_copy3(q.b_s, p->v_stride); la_copy3(q.c_s, p->k_stride); la_copy3(q.e_s, p->q_stride);
+  k.a = p->v; k.b = dout; k.c = p->q; k.e = p->k; k.c_key = 1; k.reverse = 1;
+  la_copy3(k.a_s, p->v_stride); la_copy3(k.b_s, vs); la_copy3(k.c_s, p->q_stride); la_copy3(k.e_s, p->k_stride);
+  v.a = p->k; v.b = p->q; v.c = dout; v.a_key = v.b_key = 1; v.reverse = 1;
+  la_copy3(v.a_s, p->k_stride); la_copy3(v.b_s, p->q_stride); la_copy3(v.c_s, vs);
+  q.AD = k.AD = a.V; q.CD = k.CD = a.K; v.AD = a.K; v.CD = a.V;
+  q.a_tiles = k.a_tiles = L.a_tiles; v.a_tiles = 1;
+  q.transposed = k.transposed = 1;
+  q.s_first = static_cast<const float*>(p->initial_state);
+  k.s_first = v.s_first = ds1;
+  v.s_last = ds0;
+  q.out = dq; k.out = dk; v.out = dv;
+  q.parts = L.parts[0]; k.parts = L.parts[1];
+  if (dg) {
+    q.dots = L.dots[0]; k.dots = L.dots[1];
+    q.x_last = ds1; q.x_between = L.s_rev; q.x_out = L.x;
+  }
+  if (L.split) {
+    q.s_between = L.s_fwd; k.s_between = v.s_between = L.s_rev;
+    // states of segments: k, v forward and q, dO in reverse
+    LaArgs b = a;
+    LaRole& f = b.role[0];
+    f = LaRole{};
+    f.b = p->k; f.c = p->v; f.b_key = 1; la_copy3(f.b_s, p->k_stride); la_copy3(f.c_s, p->v_stride);
+    f.AD = a.K; f.CD = a.V; f.s_first = q.s_first;
+    float* to[2] = {L.s_fwd, L.s_rev};
+    if (int rc = la_launch_states<T>(b, 2, to, L.decays, s)) return rc;
+    if (int rc = la_scan<T>(b, L.s_fwd, L.s_rev, L.decays, 2, s)) return rc;
+  }
+  if (int rc = la_launch_out<T>(a, 0, 2, dg != nullptr, s)) return rc;
+  if (int rc = la_launch_out<T>(a, 2, 1, false, s)) return rc;
+  if (L.n_parts > 1 && a.T > 0) {
+    LaSumArgs m = {{L.parts[0], L.parts[1]}, {dq, dk}, a.B * a.T * a.Hk * (int64_t)a.K, L.n_parts};
+    const bool vec = m.count % 4 == 0;
+    int64_t blocks = (m.count + (vec ? 1023 : 255)) / (vec ? 1024 : 256);
+    blocks = blocks < 16384 ? blocks : 16384;
+    const dim3 g((unsigned)blocks, 2);
+    if (vec) hipLaunchKernelGGL((la_sum_kernel<T, 4>), g, dim3(256), 0, s, m);
+    else hipLaunchKernelGGL((la_sum_kernel<T, 1>), g, dim3(256), 0, s, m);
+    if (int rc = check_launch("la_sum_kernel")) return rc;
+  }
+  if (!dg) return ATK_OK;
+  return a.g_dtype == ATK_F32 ? la_gates<T, float>(a, L, dg, s) : la_gates<T, T>(a, L, dg, s);
+}
+
+}  // namespace
+}  // namespace atk
+
+extern "C" int atk_linear_attn_update(const atk_linear_attn_update_args* p) {
+  using namespace atk;
+  if (!p) return fail(ATK_EINVAL, "linear attention update: null arguments");
+  if (!dtype_ok(p->dtype) || !dtype_ok(p->g_dtype)) return fail(ATK_EINVAL, "linear attention update: unknown dtype code");
+  if (!gdr_gate_ok(p->g_dtype, p->dtype))
+    return fail(ATK_EINVAL, "linear attention update: g must be of the inputs' type or fp32");
+  if (p->N < 0 || p->slots < 0 || p->Hk <= 0 || p->Hv <= 0 || p->K <= 0 || p->V <= 0)
+    return fail(ATK_EINVAL, "linear attention update: bad sizes");
+  if (p->Hv % p->Hk) return fail(ATK_EINVAL, "linear attention update: value heads must be a multiple of key heads");
+  if (p->K > kLaMaxK || p->Hv > 65535 || p->N > 65535 || p->V > (1 << 24))
+    return fail(ATK_UNSUPPORTED, "linear attention update: more than %d key columns, or more than 65535 heads or sequences", kLaMaxK);
+  if (p->N == 0) return ATK_OK;
+  if (!p->q || !p->k || !p->v || !p->g || !p->state || !p->out) return fail(ATK_EINVAL, "linear attention update: null pointer");
+  if (!p->state_indices && p->slots < p->N) return fail(ATK_EINVAL, "linear attention update: fewer slots than sequences");
+  LaStepArgs a = {};
+  a.q = p->q; a.k = p->k; a.v = p->v; a.g = p->g;
+  a.state = static_cast<float*>(p->state); a.o = p->out; a.slots = p->state_indices;
+  a.n = p->N; a.n_slots = p->slots; a.state_stride = p->state_stride;
+  a.q_sb = p->q_stride_n; a.q_sh = p->q_stride_h; a.k_sb = p->k_stride_n; a.k_sh = p->k_stride_h;
+  a.v_sb = p->v_stride_n; a.v_sh = p->v_stride_h; a.g_sb = p->g_stride_n; a.g_sh = p->g_stride_h;
+  a.Hv = p->Hv; a.group = p->Hv / p->Hk; a.K = p->K; a.V = p->V; a.g_dtype = p->g_dtype; a.scale = p->scale;
+  hipStream_t s = reinterpret_cast<hipStream_t>(p->stream);
+  // a launch has fewer than 2^32 threads: so many sequences at a time
+  const int64_t blocks = (int64_t)((a.V + 31) / 32) * a.Hv, most = kLaBlocks / blocks > 0 ? kLaBlocks / blocks : 1;
+  for (int64_t n = 0; n < p->N; n += most) {
+    LaStepArgs b = a;
+    const size_t e = dtype_size(p->dtype);
+    b.n = p->N - n < most ? p->N - n : most;
+    b.q = static_cast<const char*>(a.q) + n * a.q_sb * (int64_t)e;
+    b.k = static_cast<const char*>(a.k) + n * a.k_sb * (int64_t)e;
+    b.v = static_cast<const char*>(a.v) + n * a.v_sb * (int64_t)e;
+    b.g = static_cast<const char*>(a.g) + n * a.g_sb * (int64_t)dtype_size(p->g_dtype);
+    b.o = static_cast<char*>(a.o) + n * a.Hv * a.V * (int64_t)e;
+    if (a.slots) b.slots = a.slots + n;
+    else {
+      b.state = a.state + n * a.state_stride;
+      b.n_slots = a.n_slots - n;
+    }
+    if (p->dtype == ATK_F32) launch_step_typed<float>(b, s);
+    else if (p->dtype == ATK_F16) launch_step_typed<_Float16>(b, s);
+    else launch_step_typed<__bf16>(b, s);
+    if (int rc = check_launch("la_step_kernel")) return rc;
+  }
+  return ATK_OK;
+}
+
+extern "C" size_t atk_linear_attn_workspace_bytes(const atk_linear_attn_args* p) {
+  atk::LaArgs a;
+  int rc;
+  return atk::la_plan(p, false, &a, &rc).bytes;
+}
+
+extern "C" int atk_linear_attn_fwd(const atk_linear_attn_args* p) {
+  using namespace atk;
+  LaArgs a;
+  int rc;
+  const LaPlan L = la_plan(p, false, &a, &rc);
+  if (rc) return rc;
+  if (p->N == 0 || (p->T == 0 && !p->final_state)) return ATK_OK;
+  if (p->T > 0 && (!p->q || !p->k || !p->v || !p->g || !p->out)) return fail(ATK_EINVAL, "linear attention: null pointer");
+  if (L.bytes && (!p->workspace || p->workspace_bytes < L.bytes || !aligned16(p->workspace)))
+    return fail(ATK_EINVAL, "linear attention: workspace too small or not 16-byte aligned");
+  hipStream_t s = reinterpret_cast<hipStream_t>(p->stream);
+  if (p->dtype == ATK_F32) return la_forward<float>(p, a, L, s);
+  if (p->dtype == ATK_F16) return la_forward<_Float16>(p, a, L, s);
+  return la_forward<__bf16>(p, a, L, s);
+}
+
+extern "C" size_t atk_linear_attn_bwd_workspace_bytes(const atk_linear_attn_args* p) {
+  atk::LaArgs a;
+  int rc;
+  return atk::la_plan(p, true, &a, &rc).bytes;
+}
+
+extern "C" int atk_linear_attn_bwd(const atk_linear_attn_args* p, const void* dout, const void* dfinal_state, void* dq, void* dk,
+                                   void* dv, void* dg, void* dinitial_state) {
+  using namespace atk;
+  LaArgs a;
+  int rc;
+  const LaPlan L = la_plan(p, true, &a, &rc);
+  if (rc) return rc;
+  if (p->N == 0) return ATK_OK;
+  if (p->T > 0 && (!p->q || !p->k || !p->v || !p->g || !dout || !dq || !dk || !dv))
+    return fail(ATK_EINVAL, "linear attention backward: null pointer");
+  if (L.bytes && (!p->workspace || p->workspace_bytes < L.bytes || !aligned16(p->workspace)))
+    return fail(ATK_EINVAL, "linear attention backward: workspace too small or not 16-byte aligned");
+  hipStream_t s = reinterpret_cast<hipStream_t>(p->stream);
+  const float* ds1 = static_cast<const float*>(dfinal_state);
+  float* ds0 = static_cast<float*>(dinitial_state);
+  if (p->dtype == ATK_F32) return la_backward<float>(p, a, L, dout, ds1, dq, dk, dv, dg, ds0, s);
+  if (p->dtype == ATK_F16) return la_backward<_Float16>(p, a, L, dout, ds1, dq, dk, dv, dg, ds0, s);
+  return la_backward<__bf16>(p, a, L, dout, ds1, dq, dk, dv, dg, ds0, s);
+}

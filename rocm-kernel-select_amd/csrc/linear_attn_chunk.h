@@ -1,0 +1,726 @@
+// Linear attention over sequences in chunks of CT tokens: the kernels, one set for each type.
+//
+// With G the running sum of the log decays within a chunk, D_ij = exp(G_i - G_j) and S the state before it:
+//   O  = scale (exp(G) (Q S) + lower(Q K^T * D) V)
+//   S' = exp(G_last) S + K^T (exp(G_last - G) V)
+// A workgroup of four waves has one head's segment of a sequence and a tile of V's columns, each wave 16 NT
+// of them.  The state stays in the accumulators from chunk to chunk: as it is, it is the next product's
+// second operand.  Rows of a, b and c are staged in LDS in bf16 parts, the next chunk's loads in flight
+// meanwhile; products over tokens read them transposed (ds_read_tr).
+#pragma once
+#include "linear_attn.h"
+
+namespace atk {
+namespace {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Tokens of a chunk: 64, or 32 where the parts of 64 rows would not fit LDS twice.
+template <typename T, int DA> inline constexpr int kLaC = kParts<T> * DA <= 256 && sizeof(T) == 2 ? 64 : 32;
+// parts of what is multiplied towards outputs of T; gradients of decays are fp32, from three
+template <typename T, bool DOTS> inline constexpr int kLaOut = DOTS || sizeof(T) == 4 ? 3 : 2;
+
+// Running sum over the wave of v / ln 2 in 64 bits, as two floats each; lane 63's sum in *last.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double la_dpp(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ float2 la_running(float v, float2* last) {
+  double s = (double)v * 1.4426950408889634;
+  s += la_dpp<0x111, 0xF>(s);  // row_shr 1, 2, 4, 8: sums within 16 lanes
+  s += la_dpp<0x112, 0xF>(s);
+  s += la_dpp<0x114, 0xF>(s);
+  s += la_dpp<0x118, 0xF>(s);
+  s += la_dpp<0x142, 0xA>(s);  // row_bcast 15 into rows 1 and 3
+  s += la_dpp<0x143, 0xC>(s);  // row_bcast 31 into rows 2 and 3
+  const float2 r = make_float2((float)s, (float)(s - (double)(float)s));
+  last->x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, r.x), 63));
+  last->y = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, r.y), 63));
+  return r;
+}
+
+// ROWS x W elements in registers on their way to LDS, vectors of 16 bytes: a thread's loads all in flight at
+// once, without branches.  Rows and columns that are not there are loaded from where there are some, and
+// become zeros when they are put down.
+template <typename T, int ROWS, int W>
+struct LaTile {
+  static constexpr int V = 16 / sizeof(T), PER = W / V, N = ROWS * PER / 256;
+  static_assert(ROWS * PER % 256 == 0, "whole vectors a thread");
+  uint4 r[N];
+  __device__ __forceinline__ void load(const T* __restrict__ p, int64_t stride, int rows, int cols) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = threadIdx.x + 256 * i, row = at / PER, c = at % PER * V;
+      const T* __restrict__ from = p + (row < rows ? row : 0) * stride + (c + V <= cols ? c : cols - V);
+      __builtin_memcpy(&r[i], from, 16);  // element alignment only
+    }
+  }
+  // as bf16 parts, `pitch` elements from row to row
+  template <int NP>
+  __device__ __forceinline__ void put(__bf16* lds, int pitch, int part, int rows, int cols) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = threadIdx.x + 256 * i, row = at / PER, c = at % PER * V;
+      uint4 v = r[i];
+      const int past = c + V - cols;
+      if (past > 0) {
+        unsigned __int128 u = __builtin_bit_cast(unsigned __int128, v);
+        u = past < V ? u >> (past * (int)sizeof(T) * 8) : 0;
+        v = __builtin_bit_cast(uint4, u);
+      }
+      if (row >= rows) v = make_uint4(0, 0, 0, 0);
+      __bf16* to = lds + row * pitch + c;
+      if constexpr (NP == 1) {
+        *reinterpret_cast<uint4*>(to) = v;
+      } else {
+        T e[V];
+        float f[V];
+        typedef __bf16 part_t __attribute__((ext_vector_type(V)));
+        part_t parts[NP];
+        __builtin_memcpy(e, &v, 16);
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = to_f32(e[j]);
+        split_parts<NP, V>(f, parts);
+#pragma unroll
+        for (int q = 0; q < NP; ++q) __builtin_memcpy(to + q * part, &parts[q], V * 2);
+      }
+    }
+  }
+};
+
+// 8 of 32 columns of a staged row, in gdr_at's order
+__device__ __forceinline__ uint4 la_row(const __bf16* p, int g) {
+  const uint2 lo = *reinterpret_cast<const uint2*>(p + 4 * g), hi = *reinterpret_cast<const uint2*>(p + 16 + 4 * g);
+  return make_uint4(lo.x, lo.y, hi.x, hi.y);
+}
+// 8 of 32 staged rows (tokens) of column lane & 15, in gdr_at's order: 16 lanes read four rows of 16
+// columns, four columns a lane, and each gets a column of them.
+__device__ __forceinline__ uint4 la_col(const __bf16* p, int pitch, int lane) {
+  typedef __attribute__((address_space(3))) s16x4 lds_t;
+  const __bf16* at = p + (4 * (lane >> 4) + ((lane >> 2) & 3)) * pitch + 4 * (lane & 3);
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(at));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(at + 16 * pitch));
+  const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
+  return make_uint4(x.x, x.y, y.x, y.y);
+}
+__device__ __forceinline__ float la_bf(uint32_t pair, int i) { return __uint_as_float(i ? pair & 0xffff0000u : pair << 16); }
+// the 8 values that a fragment's parts stand for
+template <int NP>
+__device__ __forceinline__ void la_values(const uint4 (&f)[NP], float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    v[i] = 0.f;
+#pragma unroll
+    for (int p = NP - 1; p >= 0; --p) {
+      const uint32_t w[4] = {f[p].x, f[p].y, f[p].z, f[p].w};
+      v[i] += la_bf(w[i / 2], i & 1);
+    }
+  }
+}
+template <int NP>
+__device__ __forceinline__ void la_split(const float (&v)[8], uint4 (&f)[NP]) {
+  bf16x8 parts[NP];
+  split_parts<NP, 8>(v, parts);
+#pragma unroll
+  for (int p = 0; p < NP; ++p) f[p] = __builtin_bit_cast(uint4, parts[p]);
+}
+
+// M x N accumulators, from M first and N second operands: none waits for the one before it.
+template <int M, int N, int NA, int NB>
+__device__ __forceinline__ void la_mma(const uint4 (&a)[M][NA], const uint4 (&b)[N][NB], f32x4 (&c)[M][N]) {
+#pragma unroll
+  for (int s = 2; s >= 0; --s)
+#pragma unroll
+    for (int p = 0; p < NA; ++p)
+#pragma unroll
+      for (int q = 0; q < NB; ++q)
+        if (p + q == s) {
+#pragma unroll
+          for (int m = 0; m < M; ++m)
+#pragma unroll
+            for (int n = 0; n < N; ++n) c[m][n] = mma(a[m][p], b[n][q], c[m][n]);
+        }
+}
+
+// A chunk's decays, by one wave: G / ln 2 in two floats, exp(G), exp(G_last - G), exp(G_last).
+template <int CT>
+struct LaDecays {
+  float2 gd[CT];
+  float grown[CT], rest[CT];
+  float all, pad[3];
+  __device__ __forceinline__ void put(float g, int lane, int rows) {
+    float2 last;
+    // below -120 the decay is 0 in fp32 whatever follows, and sums with -inf have no differences
+    const float v = lane < rows ? g : 0.f;
+    const float2 s = la_running(v < -120.f ? -120.f : v, &last);
+    if (lane < CT) {
+      gd[lane] = s;
+      grown[lane] = gdr_decay(s, make_float2(0.f, 0.f));
+      rest[lane] = gdr_decay(last, s);
+    }
+    if (lane == 0) all = gdr_decay(last, make_float2(0.f, 0.f));
+  }
+};
+
+// S (or another matrix of its layout) between registers and memory: rows 16 t + 4 g + r from row i0 on,
+// columns col + 16 n.
+template <int RT, int NT, typename F>
+__device__ __forceinline__ void la_each(const LaArgs& a, const LaRole& r, int i0, int col, int g, F f) {
+  const int64_t si = r.transposed ? 1 : a.V, sj = r.transposed ? a.V : 1;
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = i0 + 16 * t + 4 * g + e, j = col + 16 * n;
+        f(t, n, e, i < r.AD && j < r.CD, i * si + j * sj);
+      }
+}
+
+template <typename T, int DA, int NT, bool DOTS>
+struct LaLds {
+  static constexpr int NP = kParts<T>, CT = kLaC<T, DA>, W = 64 * NT, PA = DA + 8, PC = W + 8, PO = 16 * NT + 4;
+  static constexpr int PF = CT == 64 ? kTri : 2;
+  __bf16 a[NP][CT][PA];
+  __bf16 b[NP][CT][PA];
+  __bf16 c[NP][CT][PC];
+  uint4 p[PF][kLaOut<T, DOTS>][64];
+  float o[4][16][PO];
+  LaDecays<CT> d;
+  float dots[DOTS ? 4 : 1][CT];
+};
+
+// The outputs of one segment, and its last state.
+template <typename T, int DA, int NT, bool DOTS>
+__device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, char* lds, int64_t block) {
+  using Lds = LaLds<T, DA, NT, DOTS>;
+  constexpr int NP = Lds::NP, CT = Lds::CT, W = Lds::W, RT = DA / 16, KS = DA / 32, MT = CT / 16, HS = CT / 32;
+  constexpr int OP = kLaOut<T, DOTS>, OW = 4 * NT;
+  Lds& L = *reinterpret_cast<Lds*>(lds);
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c_tiles = (r.CD + W - 1) / W;
+  int tile, h;
+  int64_t slot;
+  if (!la_place(a, block, c_tiles * r.a_tiles, &tile, &h, &slot)) return;
+  const int hk = h / a.group, c_tile = tile % c_tiles, a_tile = tile / c_tiles;
+  const int64_t n = la_seq_of_slot(a, slot);
+  const LaSeq seq = la_seq(a, n);
+  const int64_t z = slot - seq.slot, segs = la_segments(seq, a.seg);
+  if (z < 0 || z >= segs) return;
+  const int64_t t0 = z * a.seg, left = seq.len - t0;
+  const int len = (int)(left < a.seg ? left : a.seg);  // tokens of this segment
+  const int chunks = (len + CT - 1) / CT;
+  const int a0 = a_tile * DA, col0 = c_tile * W, col = col0 + wave * 16 * NT + c;
+  const int acols = r.AD - a0 < DA ? r.AD - a0 : DA, ccols = r.CD - col0 < W ? r.CD - col0 : W;
+  const bool rev = r.reverse;
+  const int64_t first = seq.begin + t0;
+  const T* __restrict__ pa = static_cast<const T*>(r.a) + seq.batch * r.a_s[0] + first * r.a_s[1] + (r.a_key ? hk : h) * r.a_s[2] + a0;
+  const T* __restrict__ pb = static_cast<const T*>(r.b) + seq.batch * r.b_s[0] + first * r.b_s[1] + (r.b_key ? hk : h) * r.b_s[2] + a0;
+  const T* __restrict__ pc = static_cast<const T*>(r.c) + seq.batch * r.c_s[0] + first * r.c_s[1] + (r.c_key ? hk : h) * r.c_s[2] + col0;
+  const T* __restrict__ pe = DOTS ? static_cast<const T*>(r.e) + seq.batch * r.e_s[0] + first * r.e_s[1] + hk * r.e_s[2] + col0 : nullptr;
+  const int64_t pg = seq.batch * a.g_s[0] + first * a.g_s[1] + h * a.g_s[2];
+
+  f32x4 S[RT][NT];
+  const float* from = (rev ? z == segs - 1 : z == 0) ? r.s_first : r.s_between;
+  bool have = from != nullptr;
+  if (from) {
+    const int64_t at = from == r.s_first ? n * a.Hv + h : (slot + (rev ? 1 : -1)) * a.Hv + h;
+    from += at * a.K * a.V;
+    la_each<RT, NT>(a, r, a0, col, g, [&](int t, int m, int e, bool in, int64_t i) { S[t][m][e] = in ? from[i] : 0.f; });
+  } else {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int m = 0; m < NT; ++m) S[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  LaTile<T, CT, DA> ta, tb;
+  LaTile<T, CT, W> tc;
+  GdrGate tg;
+  auto load = [&](int ch) {
+    const int at = ch * CT, rows = len - at < CT ? len - at : CT;
+    ta.load(pa + at * r.a_s[1], r.a_s[1], rows, acols);
+    tb.load(pb + at * r.b_s[1], r.b_s[1], rows, acols);
+    tc.load(pc + at * r.c_s[1], r.c_s[1], rows, ccols);
+    tg = gdr_gate_load(a.g, a.g_dtype, pg + (at + (lane < rows ? lane : 0)) * a.g_s[1]);
+  };
+  if (chunks > 0) load(rev ? chunks - 1 : 0);
+  for (int k = 0; k < chunks; ++k) {
+    const int ch = rev ? chunks - 1 - k : k, at = ch * CT, rows = len - at < CT ? len - at : CT;
+    ta.template put<NP>(&L.a[0][0][0], Lds::PA, CT * Lds::PA, rows, acols);
+    tb.template put<NP>(&L.b[0][0][0], Lds::PA, CT * Lds::PA, rows, acols);
+    tc.template put<NP>(&L.c[0][0][0], Lds::PC, CT * Lds::PC, rows, ccols);
+    if (wave == 0) L.d.put(gdr_gate<T>(tg, a.g_dtype), lane, rows);
+    __syncthreads();
+    load(k + 1 < chunks ? (rev ? ch - 1 : ch + 1) : ch);  // (at the end the last one's again)
+    // lower(A B^T * D), or upper in reverse, in the layout of a first operand: as the results of its transpose
+    if (wave < MT) {
+      uint4 af[KS][NP];
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) af[s][p] = la_row(&L.a[p][16 * wave + c][32 * s], g);
+      const float2 go = L.d.gd[16 * wave + c];
+#pragma unroll
+      for (int s = 0; s < HS; ++s) {
+        if (HS > 1 && (rev ? s < wave >> 1 : s > wave >> 1)) continue;
+        f32x4 y[2][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}, {f32x4{0.f, 0.f, 0.f, 0.f}}};
+#pragma unroll
+        for (int q = 0; q < KS; ++q) {
+          uint4 bf[2][NP], ao[1][NP];
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            ao[0][p] = af[q][p];
+            bf[0][p] = la_row(&L.b[p][32 * s + c][32 * q], g);
+            bf[1][p] = la_row(&L.b[p][32 * s + 16 + c][32 * q], g);
+          }
+          la_mma<2, 1, NP, NP>(bf, ao, y);
+        }
+        float v[8];
+        const int out = 16 * wave + c;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int in = 32 * s + 16 * u + 4 * g + e;
+            const float2 gi = L.d.gd[in];
+            const float decay = gdr_decay(rev ? gi : go, rev ? go : gi);
+            v[4 * u + e] = (rev ? in >= out : in <= out) ? y[u][0][e] * decay * a.scale : 0.f;
+          }
+        uint4 f[OP];
+        la_split<OP>(v, f);
+        const int at_p = HS == 1 ? wave : rev ? tri_upper(wave, s) : tri_lower(wave, s);
+#pragma unroll
+        for (int p = 0; p < OP; ++p) L.p[at_p][p][lane] = f[p];
+      }
+    }
+    __syncthreads();
+    uint4 cf[HS][NT][NP];
+#pragma unroll
+    for (int s = 0; s < HS; ++s)
+#pragma unroll
+      for (int m = 0; m < NT; ++m)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) cf[s][m][p] = la_col(&L.c[p][32 * s][wave * 16 * NT + 16 * m], Lds::PC, lane);
+    f32x4 acc[MT][NT];
+    for (bool clean = false;; clean = true) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int x = 0; x < NT; ++x) acc[m][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (have) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          uint4 sf[NT][OP], af[MT][NP];
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int p = 0; p < NP; ++p) af[m][p] = la_row(&L.a[p][16 * m + c][32 * s], g);
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = S[2 * s + e / 4][x][e & 3];
+            la_split<OP>(v, sf[x]);
+          }
+          la_mma<MT, NT, NP, OP>(af, sf, acc);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const f32x4 f = rev ? *reinterpret_cast<const f32x4*>(&L.d.rest[16 * m + 4 * g])
+                              : *reinterpret_cast<const f32x4*>(&L.d.grown[16 * m + 4 * g]) * a.scale;
+#pragma unroll
+          for (int x = 0; x < NT; ++x) acc[m][x] *= f;
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < HS; ++s) {
+        uint4 b[NT][NP];
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+#pragma unroll
+          for (int p = 0; p < NP; ++p) b[x][p] = cf[s][x][p];
+          if (clean) {
+            float v[8];
+            la_values<NP>(b[x], v);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = gdr_finite(v[e]);
+            la_split<NP>(v, b[x]);
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if (HS > 1 && (rev ? s < m >> 1 : s > m >> 1)) continue;
+          uint4 f[1][OP];
+          const int at_p = HS == 1 ? m : rev ? tri_upper(m, s) : tri_lower(m, s);
+#pragma unroll
+          for (int p = 0; p < OP; ++p) f[0][p] = L.p[at_p][p][lane];
+          f32x4 y[1][NT];
+#pragma unroll
+          for (int x = 0; x < NT; ++x) y[0][x] = acc[m][x];
+          la_mma<1, NT, OP, NP>(f, b, y);
+#pragma unroll
+          for (int x = 0; x < NT; ++x) acc[m][x] = y[0][x];
+        }
+      }
+      if (clean || !r.guard) break;
+      bool spoilt = false;
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int x = 0; x < NT; ++x) spoilt |= gdr_spoilt<4>(acc[m][x]);
+      if (!__any(spoilt)) break;
+    }
+    if (r.guard) {
+      // (only after a second pass can outputs that are not finite be owed to c: those from the first such row on)
+      bool spoilt = false;
+#pragma unroll
+      for (int s = 0; s < HS; ++s)
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          float v[8];
+          la_values<NP>(cf[s][x], v);
+          spoilt |= gdr_spoilt<8>(v);
+        }
+      if (__any(spoilt)) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          int bad = CT;  // this column's first token that is not finite
+#pragma unroll
+          for (int s = 0; s < HS; ++s) {
+            float v[8];
+            la_values<NP>(cf[s][x], v);
+#pragma unroll
+            for (int e = 7; e >= 0; --e) {
+              const int tok = 32 * s + gdr_at(g, e);
+              if (gdr_spoilt<1>(&v[e]) && tok < bad) bad = tok;
+            }
+          }
+          int other = __shfl_xor(bad, 16, 64);
+          bad = other < bad ? other : bad;
+          other = __shfl_xor(bad, 32, 64);
+          bad = other < bad ? other : bad;
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (16 * m + 4 * g + e >= bad) acc[m][x][e] = gdr_nan();
+        }
+      }
+    }
+    // the state after the chunk (in reverse: before it)
+    {
+      const float all = L.d.all;
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int x = 0; x < NT; ++x) S[t][x] *= all;
+#pragma unroll
+      for (int s = 0; s < HS; ++s) {
+        uint4 cw[NT][3];
+        float f[8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const f32x4 t = rev ? *reinterpret_cast<const f32x4*>(&L.d.grown[32 * s + 16 * u + 4 * g]) * a.scale
+                              : *reinterpret_cast<const f32x4*>(&L.d.rest[32 * s + 16 * u + 4 * g]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f[4 * u + e] = t[e];
+        }
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+          float v[8];
+          la_values<NP>(cf[s][x], v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= f[e];
+          la_split<3>(v, cw[x]);
+        }
+#pragma unroll
+        for (int t = 0; t < RT; t += 4) {
+          uint4 bf[4][NP];
+          f32x4 y[4][NT];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+#pragma unroll
+            for (int p = 0; p < NP; ++p) bf[u][p] = la_col(&L.b[p][32 * s][16 * (t + u)], Lds::PA, lane);
+#pragma unroll
+            for (int x = 0; x < NT; ++x) y[u][x] = S[t + u][x];
+          }
+          la_mma<4, NT, NP, 3>(bf, cw, y);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int x = 0; x < NT; ++x) S[t + u][x] = y[u][x];
+        }
+      }
+      have = true;
+    }
+    // rows of 16 tokens through LDS: OW columns of one a lane
+    const int orow = lane >> 2, oc = wave * 16 * NT + (lane & 3) * OW;
+    const bool whole = col0 + oc + OW <= r.CD;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses keep their order)
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) L.o[wave][4 * g + e][16 * x + c] = acc[m][x][e];
+      __builtin_amdgcn_wave_barrier();
+      float o[OW];
+#pragma unroll
+      for (int e = 0; e < OW; e += 4) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(&L.o[wave][orow][(lane & 3) * OW + e]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[e + q] = t[q];
+      }
+      const int row = 16 * m + orow;
+      if constexpr (DOTS) {
+        float dot = 0.f;
+        if (row < rows) {
+          const T* __restrict__ e = pe + (at + row) * r.e_s[1] + oc;
+#pragma unroll
+          for (int q = 0; q < OW; ++q)
+            if (whole || col0 + oc + q < r.CD) dot += o[q] * to_f32(e[q]);
+        }
+        dot += dpp_mov<0xB1>(dot);
+        dot += dpp_mov<0x4E>(dot);
+        if ((lane & 3) == 0) L.dots[wave][row] = dot;
+      }
+      if (row < rows) {
+        const int64_t tok = seq.batch * a.T + first + at + row;
+        if (r.parts) {
+          float* __restrict__ to = r.parts + ((((int64_t)(h % a.group) * r.a_tiles + a_tile) * a.B * a.T + tok) * a.Hk + hk) * r.CD + col0 + oc;
+#pragma unroll
+          for (int q = 0; q < OW; ++q)
+            if (whole || col0 + oc + q < r.CD) to[q] = o[q];
+        } else {
+          T* __restrict__ to = static_cast<T*>(r.out) + (tok * (r.e ? a.Hk : a.Hv) + (r.e ? hk : h)) * r.CD + col0 + oc;
+          T v[OW];
+#pragma unroll
+          for (int q = 0; q < OW; ++q) v[q] = from_f32<T>(o[q]);
+          if (whole) {
+            __builtin_memcpy(to, v, OW * sizeof(T));
+          } else {
+#pragma unroll
+            for (int q = 0; q < OW; ++q)
+              if (col0 + oc + q < r.CD) to[q] = v[q];
+          }
+        }
+      }
+    }
+    __syncthreads();  // the chunk's LDS is free
+    if constexpr (DOTS) {
+      if (tid < rows)
+        r.dots[((int64_t)tile * a.Hv + h) * a.B * a.T + seq.batch * a.T + first + at + tid] =
+            (L.dots[0][tid] + L.dots[1][tid]) + (L.dots[2][tid] + L.dots[3][tid]);
+    }
+  }
+  if (r.s_last && (rev ? z == 0 : z == segs - 1)) {
+    float* __restrict__ to = r.s_last + (n * a.Hv + h) * a.K * a.V;
+    la_each<RT, NT>(a, r, a0, col, g, [&](int t, int m, int e, bool in, int64_t i) { if (in) to[i] = S[t][m][e]; });
+  }
+  if constexpr (DOTS) {
+    if (r.x_out) {  // the state at the segment's end, and the gradient of it from what follows
+      float x = 0.f;
+      const float* d = z == segs - 1 ? r.x_last : r.x_between;
+      if (d) {
+        d += (z == segs - 1 ? n * a.Hv + h : (slot + 1) * a.Hv + h) * a.K * a.V;
+        la_each<RT, NT>(a, r, a0, col, g, [&](int t, int m, int e, bool in, int64_t i) { x += in ? S[t][m][e] * d[i] : 0.f; });
+      }
+      x = wave_sum(x);
+      __syncthreads();
+      if (lane == 0) L.o[0][0][wave] = x;
+      __syncthreads();
+      if (tid == 0) r.x_out[((int64_t)tile * a.slots + slot) * a.Hv + h] = (L.o[0][0][0] + L.o[0][0][1]) + (L.o[0][0][2] + L.o[0][0][3]);
+    }
+  }
+  // tokens of a packed row before its first sequence and after its last have zeros
+  if (a.cu && a_tile == 0) {
+    const int heads = r.e ? a.Hk : a.Hv, ho = r.e ? hk : h;
+    for (int w = 0; w < 2; ++w) {
+      if (w == 0 ? n != 0 || z != 0 : n != a.n - 1 || z != segs - 1) continue;
+      const int64_t b = w == 0 ? 0 : seq.begin + seq.len, end = w == 0 ? seq.begin : a.T;
+      for (int64_t t = b; t < end; ++t)
+        for (int j = tid; j < ccols; j += 256) {
+          if (r.parts) {
+            for (int q = 0; q < r.a_tiles; ++q)
+              r.parts[((((int64_t)(h % a.group) * r.a_tiles + q) * a.B * a.T + t) * a.Hk + hk) * r.CD + col0 + j] = 0.f;
+          } else {
+            static_cast<T*>(r.out)[(t * heads + ho) * r.CD + col0 + j] = from_f32<T>(0.f);
+          }
+        }
+    }
+  }
+}
+
+template <typename T, int DA, int NT, bool DOTS>
+__global__ __launch_bounds__(256, 2) void la_out_kernel(LaArgs a, int role, int64_t first) {
+  __shared__ __align__(16) char lds[sizeof(LaLds<T, DA, NT, DOTS>)];
+  la_segment<T, DA, NT, DOTS>(a, a.role[role + blockIdx.y], lds, first + blockIdx.x);
+}
+
+template <typename T, int DA, int NT>
+struct LaStateLds {
+  static constexpr int NP = kParts<T>, CT = kLaC<T, DA>, W = 64 * NT, PA = DA + 8, PC = W + 8;
+  __bf16 b[NP][CT][PA];
+  __bf16 c[NP][CT][PC];
+  LaDecays<CT> d;
+};
+
+// What a segment adds to the state, and its decay: b and c alone.  The last segment's (in reverse the
+// first's) nobody asks for.
+template <typename T, int DA, int NT>
+__global__ __launch_bounds__(256, 2) void la_state_kernel(LaArgs a, float* to0, float* to1, float* decays, int64_t block0) {
+  using Lds = LaStateLds<T, DA, NT>;
+  constexpr int NP = Lds::NP, CT = Lds::CT, W = Lds::W, RT = DA / 16, HS = CT / 32;
+  __shared__ __align__(16) char lds[sizeof(Lds)];
+  Lds& L = *reinterpret_cast<Lds*>(lds);
+  const LaRole& r = a.role[blockIdx.y ? 2 : 0];  // k, v; in reverse q, dO
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int tile, h;
+  int64_t slot;
+  if (!la_place(a, block0 + blockIdx.x, (r.CD + W - 1) / W, &tile, &h, &slot)) return;
+  const int hk = h / a.group;
+  const int64_t n = la_seq_of_slot(a, slot);
+  const LaSeq seq = la_seq(a, n);
+  const int64_t z = slot - seq.slot, segs = la_segments(seq, a.seg);
+  const bool rev = r.reverse;
+  if (z < 0 || z >= segs || z == (rev ? 0 : segs - 1)) return;
+  const int64_t t0 = z * a.seg, left = seq.len - t0;
+  const int len = (int)(left < a.seg ? left : a.seg), chunks = (len + CT - 1) / CT;
+  const int col0 = tile * W, col = col0 + wave * 16 * NT + c;
+  const int acols = r.AD, ccols = r.CD - col0 < W ? r.CD - col0 : W;
+  const int64_t first = seq.begin + t0;
+  const T* __restrict__ pb = static_cast<const T*>(r.b) + seq.batch * r.b_s[0] + first * r.b_s[1] + (r.b_key ? hk : h) * r.b_s[2];
+  const T* __restrict__ pc = static_cast<const T*>(r.c) + seq.batch * r.c_s[0] + first * r.c_s[1] + (r.c_key ? hk : h) * r.c_s[2] + col0;
+  const int64_t pg = seq.batch * a.g_s[0] + first * a.g_s[1] + h * a.g_s[2];
+  f32x4 S[RT][NT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int x = 0; x < NT; ++x) S[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float2 total = make_float2(0.f, 0.f);
+  LaTile<T, CT, DA> tb;
+  LaTile<T, CT, W> tc;
+  GdrGate tg;
+  auto load = [&](int ch) {
+    const int at = ch * CT, rows = len - at < CT ? len - at : CT;
+    tb.load(pb + at * r.b_s[1], r.b_s[1], rows, acols);
+    tc.load(pc + at * r.c_s[1], r.c_s[1], rows, ccols);
+    tg = gdr_gate_load(a.g, a.g_dtype, pg + (at + (lane < rows ? lane : 0)) * a.g_s[1]);
+  };
+  load(rev ? chunks - 1 : 0);
+  for (int k = 0; k < chunks; ++k) {
+    const int ch = rev ? chunks - 1 - k : k, at = ch * CT, rows = len - at < CT ? len - at : CT;
+    tb.template put<NP>(&L.b[0][0][0], Lds::PA, CT * Lds::PA, rows, acols);
+    tc.template put<NP>(&L.c[0][0][0], Lds::PC, CT * Lds::PC, rows, ccols);
+    if (wave == 0) L.d.put(gdr_gate<T>(tg, a.g_dtype), lane, rows);
+    __syncthreads();
+    load(k + 1 < chunks ? (rev ? ch - 1 : ch + 1) : ch);
+    const float all = L.d.all;
+    const float2 last = L.d.gd[CT - 1];
+    total.x += last.x;
+    total.y += last.y;
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int x = 0; x < NT; ++x) S[t][x] *= all;
+#pragma unroll
+    for (int s = 0; s < HS; ++s) {
+      uint4 cw[NT][3];
+      float f[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const f32x4 t = rev ? *reinterpret_cast<const f32x4*>(&L.d.grown[32 * s + 16 * u + 4 * g]) * a.scale
+                            : *reinterpret_cast<const f32x4*>(&L.d.rest[32 * s + 16 * u + 4 * g]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[4 * u + e] = t[e];
+      }
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        uint4 cf[NP];
+        float v[8];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) cf[p] = la_col(&L.c[p][32 * s][wave * 16 * NT + 16 * x], Lds::PC, lane);
+        la_values<NP>(cf, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= f[e];
+        la_split<3>(v, cw[x]);
+      }
+#pragma unroll
+      for (int t = 0; t < RT; t += 4) {
+        uint4 bf[4][NP];
+        f32x4 y[4][NT];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+#pragma unroll
+          for (int p = 0; p < NP; ++p) bf[u][p] = la_col(&L.b[p][32 * s][16 * (t + u)], Lds::PA, lane);
+#pragma unroll
+          for (int x = 0; x < NT; ++x) y[u][x] = S[t + u][x];
+        }
+        la_mma<4, NT, NP, 3>(bf, cw, y);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int x = 0; x < NT; ++x) S[t + u][x] = y[u][x];
+      }
+    }
+    __syncthreads();
+  }
+  float* __restrict__ to = (blockIdx.y ? to1 : to0) + (slot * a.Hv + h) * a.K * a.V;
+  la_each<RT, NT>(a, r, 0, col, g, [&](int t, int m, int e, bool in, int64_t i) { if (in) to[i] = S[t][m][e]; });
+  if (tile == 0 && tid == 0) decays[(blockIdx.y * a.slots + slot) * a.Hv + h] = gdr_decay(total, make_float2(0.f, 0.f));
+}
+
+template <typename T, int DA, int NT, bool DOTS>
+int la_run_out(const LaArgs& a, int first, int roles, hipStream_t s) {
+  const LaRole& r = a.role[first];
+  const int64_t grid = la_grid(a, (r.CD + 64 * NT - 1) / (64 * NT) * r.a_tiles);
+  for (int64_t b = 0; b < grid; b += kLaBlocks / 4) {
+    const dim3 gr((unsigned)(grid - b < kLaBlocks / 4 ? grid - b : kLaBlocks / 4), (unsigned)roles);
+    hipLaunchKernelGGL((la_out_kernel<T, DA, NT, DOTS>), gr, dim3(256), 0, s, a, first, b);
+    if (int rc = check_launch("la_out_kernel")) return rc;
+  }
+  return ATK_OK;
+}
+template <typename T, int DA, int NT>
+int la_run_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s) {
+  const int64_t grid = la_grid(a, (a.V + 64 * NT - 1) / (64 * NT));
+  for (int64_t b = 0; b < grid; b += kLaBlocks / 4) {
+    const dim3 gr((unsigned)(grid - b < kLaBlocks / 4 ? grid - b : kLaBlocks / 4), (unsigned)roles);
+    hipLaunchKernelGGL((la_state_kernel<T, DA, NT>), gr, dim3(256), 0, s, a, to[0], roles > 1 ? to[1] : nullptr, decays, b);
+    if (int rc = check_launch("la_state_kernel")) return rc;
+  }
+  return ATK_OK;
+}
+
+}  // namespace
+
+template <typename T>
+int la_launch_out(const LaArgs& a, int first, int roles, bool dots, hipStream_t s) {
+  const LaRole& r = a.role[first];
+  const int da = la_padded(r.AD), nt = la_wide(da, r.CD);
+#define ATK_LA(DA, NT) return dots ? la_run_out<T, DA, NT, true>(a, first, roles, s) : la_run_out<T, DA, NT, false>(a, first, roles, s)
+  if (da == 256) ATK_LA(256, 1);
+  if (da == 128 && nt == 2) ATK_LA(128, 2);
+  if (da == 128) ATK_LA(128, 1);
+  if (nt == 2) ATK_LA(64, 2);
+  ATK_LA(64, 1);
+#undef ATK_LA
+}
+template <typename T>
+int la_launch_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s) {
+  const int da = la_padded(a.K), nt = la_wide(da, a.V);
+  if (da == 256) return la_run_states<T, 256, 1>(a, roles, to, decays, s);
+  if (da == 128 && nt == 2) return la_run_states<T, 128, 2>(a, roles, to, decays, s);
+  if (da == 128) return la_run_states<T, 128, 1>(a, roles, to, decays, s);
+  if (nt == 2) return la_run_states<T, 64, 2>(a, roles, to, decays, s);
+  return la_run_states<T, 64, 1>(a, roles, to, decays, s);
+}
+
+}  // namespace atk

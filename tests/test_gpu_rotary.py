@@ -1,0 +1,205 @@
+"""Rotary positions against the turn of complex numbers in 64 bits.
+
+Tolerance: an angle is brought to a part of a turn in 64 bits and rounded to fp32 there (2^-25 of a turn, 2 pi 2^-25
+of the angle), sine and cosine have errors of 2^-23, products, the scale and the sum one rounding of 2^-24 each: in
+all below 2^-20 of scale (|a| + |b|).  Then the result is rounded once to its type."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+ULP = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+gpu = pytest.mark.gpu
+
+
+def turned64(x, inv_freq, positions, interleaved, scale, sign=1):
+    """(x with its pairs turned, scale (|a| + |b|) in each element's place)."""
+    x = x.double()
+    rot = 2 * inv_freq.numel()
+    angle = sign * positions.expand(x.shape[:-2]).double()[..., None, None] * inv_freq.double()
+    i = torch.arange(rot // 2, device=x.device)
+    a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + rot // 2)
+    z = torch.complex(x[..., a], x[..., b]) * torch.polar(torch.full_like(angle, scale), angle)
+    out, size = x.clone(), torch.zeros_like(x)
+    out[..., a], out[..., b] = z.real, z.imag
+    size[..., a] = size[..., b] = scale * (x[..., a].abs() + x[..., b].abs())
+    return out, size
+
+
+def close(got, want, size, what=""):
+    floor = 2.0 ** -24 if got.dtype == torch.float16 else 1e-30
+    off = (got.double() - want).abs() - ULP[got.dtype] * want.abs() - 2.0 ** -20 * size - floor
+    assert got.shape == want.shape and (not off.numel() or off.max().item() <= 0), (what, off.max().item())
+
+
+def freqs(rot, dev, dtype=torch.float64):
+    return (10000.0 ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)).to(dev, dtype) if rot else \
+        torch.zeros(0, dtype=dtype, device=dev)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("b,t,hq,hk,d,rot", [(1, 1, 1, 0, 2, 2), (2, 7, 3, 1, 64, 64), (1, 33, 2, 2, 128, 64), (3, 5, 4, 2, 90, 34),
+                                             (2, 9, 1, 1, 17, 6), (1, 300, 8, 2, 256, 256), (1, 3, 2, 1, 16, 0),
+                                             (2, 2, 1, 1, 5, 4), (1, 2, 1, 3, 130, 128), (1, 1100, 1, 1, 32, 30)])
+def test_forward(dev, b, t, hq, hk, d, rot, interleaved, dtype):
+    import amd_tuned_torch as P
+    gen = torch.Generator().manual_seed(d + t)
+    q, k = (torch.randn(b, t, h, d, generator=gen).to(dev, dtype) for h in (hq, max(hk, 1)))
+    pos = torch.randint(-5, 1 << 20, (b, t), generator=gen).to(dev)
+    for p, f, scale in ((pos, torch.float64, 1.25), (pos.int(), torch.float32, 1.0), (pos[:1], torch.float64, 0.5),
+                        (pos[0, :], torch.float64, 1.0), (12345, torch.float64, 1.0), (0, torch.float32, 1.0)):
+        inv = freqs(rot, dev, f)
+        at = p if isinstance(p, torch.Tensor) else p + torch.arange(t, device=dev)
+        got = P.rotary_embedding(q, k if hk else None, inv, p, interleaved, scale)
+        got_q, got_k = got if hk else (got, None)
+        assert got_q.dtype == dtype and got_q.is_contiguous()
+        close(got_q, *turned64(q, inv, at, interleaved, scale), "q")
+        assert torch.equal(got_q[..., rot:], q[..., rot:])
+        if hk:
+            close(got_k, *turned64(k, inv, at, interleaved, scale), "k")
+        ref = P.rotary_ops.rotary_embedding_ref(q, None, inv, p, interleaved, scale)
+        close(ref, *turned64(q, inv, at, interleaved, scale), "statement")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_far_positions_and_strides(dev, dtype):
+    """Heads of one projection, tokens of a packed row, positions of 10^9; the last axis strided."""
+    import amd_tuned_torch as P
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(11, 3 * 5 * 48 + 1, generator=gen).to(dev, dtype)[:, 1:].unflatten(1, (15, 48))
+    q, k = x[:, :5], x[:, 5:10]
+    pos = torch.tensor([0, 10 ** 9, 3, 1 << 30, 5, 6, 999999937, 8, 9, 10, -10 ** 9], device=dev)
+    inv = freqs(48, dev)
+    for a, b, p in ((q, k, pos), (q[::2], k[::2], pos[::2]), (q[:, :, ::2], k[:, :, ::2], pos)):
+        f = inv[:a.shape[-1] // 2]
+        gq, gk = P.rotary_embedding(a, b, f, p)
+        close(gq, *turned64(a, f, p, False, 1.0))
+        close(gk, *turned64(b, f, p, False, 1.0))
+    strided = torch.stack((inv, inv), 1).flatten()[::2]
+    assert torch.equal(P.rotary_embedding(q, None, strided, pos), P.rotary_embedding(q, None, inv, pos))
+    one = x[:1, :5].expand(11, 5, 48)                                      # broadcast tokens
+    close(P.rotary_embedding(one, None, inv, pos), *turned64(one, inv, pos, False, 1.0))
+    assert P.rotary_embedding(q[:0], k[:0], inv, pos[:0])[1].shape == (0, 5, 48)
+    assert P.rotary_embedding(q, k[:, :0], inv, pos)[1].shape == (11, 0, 48)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_backward(dev, interleaved, dtype):
+    import amd_tuned_torch as P
+    gen = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=gen).to(dev, dtype)  # noqa: E731
+    q, k, dq, dk = r(2, 9, 4, 40), r(2, 9, 1, 40), r(2, 9, 4, 40), r(2, 9, 1, 40)
+    inv, pos = freqs(24, dev), torch.randint(0, 50000, (2, 9), generator=gen).to(dev)
+    q.requires_grad_()
+    k.requires_grad_()
+    oq, ok = P.rotary_embedding(q, k, inv, pos, interleaved, 1.5)
+    gq, gk = torch.autograd.grad((oq, ok), (q, k), (dq, dk), retain_graph=True)
+    close(gq, *turned64(dq, inv, pos, interleaved, 1.5, -1))
+    close(gk, *turned64(dk, inv, pos, interleaved, 1.5, -1))
+    only, = torch.autograd.grad(ok, k, dk, retain_graph=True)              # one output has a gradient
+    assert torch.equal(only, gk)
+    one, = torch.autograd.grad(P.rotary_embedding(q, None, inv, pos, interleaved, 1.5), q, dq)
+    assert torch.equal(one, gq)
+    # twice: the gradient of the gradient in its own direction is the operator again
+    d = dq.clone().requires_grad_()
+    first, = torch.autograd.grad(oq, q, d, create_graph=True, retain_graph=True)
+    second, = torch.autograd.grad(first, d, dq)
+    close(second, *turned64(dq, inv, pos, interleaved, 1.5))
+    # batched gradients
+    both, = torch.autograd.grad(oq, q, torch.stack((dq, 2 * dq)), is_grads_batched=True)
+    close(both[0], *turned64(dq, inv, pos, interleaved, 1.5, -1))
+    # differences: the operator is linear, so a step of any length gives the derivative
+    f = lambda x: (P.rotary_embedding(x, None, inv, pos, interleaved, 1.5).double() * dq.double()).sum()  # noqa: E731
+    with torch.no_grad():
+        step = r(2, 9, 4, 40)
+        want = (gq.double() * step.double()).sum()
+        got = f(step) - f(torch.zeros_like(step))
+        size = (turned64(step, inv, pos, interleaved, 1.5)[1] + step.abs().double()) * dq.double().abs()
+        size = size + turned64(dq, inv, pos, interleaved, 1.5)[1] * step.double().abs()
+        assert (got - want).abs() <= (2 * ULP[dtype] + 2.0 ** -19) * size.sum()
+
+
+@gpu
+def test_refusals(dev):
+    import amd_tuned_torch as P
+    q = torch.randn(2, 3, 4, 16, device=dev)
+    inv = freqs(16, dev)
+    bad = [(q[0, 0], None, inv, 0), (q, q[:1], inv, 0), (q, q.half(), inv, 0), (q.double(), None, inv, 0),
+           (q, None, freqs(18, dev), 0), (q, None, inv.half(), 0), (q, None, inv.cpu(), 0), (q, None, inv, 0.5),
+           (q, None, inv, torch.zeros(2, 3, device=dev)), (q, None, inv, torch.zeros(2, 4, dtype=torch.int64, device=dev)),
+           (q, None, inv, torch.zeros(2, 3, dtype=torch.int64)), (q, None, inv, torch.zeros(1, 2, 3, dtype=torch.int64, device=dev)),
+           (q, None, inv[None], 0), (q, None, inv.clone().requires_grad_(), 0)]
+    for args in bad:
+        with pytest.raises(RuntimeError):
+            P.rotary_embedding(*args)
+
+
+@gpu
+def test_other_stream_and_graph(dev):
+    """A captured call, replayed with inputs and positions changed between."""
+    import amd_tuned_torch as P
+    gen = torch.Generator().manual_seed(2)
+    q, k = (torch.randn(3, 1, h, 64, generator=gen).to(dev, torch.bfloat16) for h in (4, 2))
+    inv, pos = freqs(64, dev), torch.zeros(3, 1, dtype=torch.int64, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        P.rotary_embedding(q, k, inv, pos)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        oq, ok = P.rotary_embedding(q, k, inv, pos)
+    for step in range(4):
+        q.normal_()
+        pos.add_(1000 * step + 1)
+        graph.replay()
+        torch.cuda.synchronize()
+        eq, ek = P.rotary_embedding(q, k, inv, pos)
+        assert torch.equal(oq, eq) and torch.equal(ok, ek), step
+
+
+def test_frequencies():
+    import amd_tuned_torch as P
+    plain, one = P.rotary_frequencies(64, 10000.0)
+    assert plain.dtype == torch.float64 and plain.shape == (32,) and one == 1.0
+    assert plain[0] == 1.0 and abs(plain[31].item() - 10000.0 ** (-62 / 64)) < 1e-18
+    linear, _ = P.rotary_frequencies(64, scaling="linear", factor=4.0)
+    assert torch.equal(linear, plain / 4)
+    ntk, s = P.rotary_frequencies(64, scaling="base", factor=4.0)
+    assert s == 1.0 and ntk[0] == 1.0 and abs(ntk[31] / plain[31] - 0.25) < 1e-12
+    parts, s = P.rotary_frequencies(64, scaling="parts", factor=8.0, original_length=4096)
+    assert abs(s - (1 + 0.1 * math.log(8))) < 1e-15
+    turns = 4096 * plain / (2 * math.pi)
+    assert torch.equal(parts[turns >= 32], plain[turns >= 32])
+    assert torch.allclose(parts[turns <= 1], plain[turns <= 1] / 8, rtol=1e-15)
+    between = (turns > 1) & (turns < 32)
+    assert ((parts < plain) & (parts > plain / 8))[between].all() and between.any()
+    assert P.rotary_frequencies(64, scaling="parts", factor=1.0)[1] == 1.0
+    for kw in (dict(dim=7), dict(dim=0), dict(dim=8, scaling="other"), dict(dim=8, factor=0.0), dict(dim=8, base=-1.0),
+               dict(dim=8, original_length=0), dict(dim=8, fast_turns=1.0)):
+        with pytest.raises(ValueError):
+            P.rotary_frequencies(**kw)
+
+
+def test_statement_on_the_cpu():
+    """In 64 bits against complex numbers, and its gradient against differences."""
+    from amd_tuned_torch import rotary_ops as R
+    gen = torch.Generator().manual_seed(0)
+    q = torch.randn(2, 3, 2, 10, generator=gen, dtype=torch.float64)
+    inv, pos = freqs(6, "cpu"), torch.randint(0, 100, (2, 3), generator=gen)
+    for interleaved in (False, True):
+        want, size = turned64(q, inv, pos, interleaved, 1.5)
+        got = R.rotary_embedding_ref(q, None, inv, pos, interleaved, 1.5)
+        assert ((got - want).abs() <= 1e-14 * (1 + size)).all()
+        back = R.rotary_embedding_ref(got, None, inv, pos, interleaved, 1 / 1.5, inverse=True)
+        assert (back - q).abs().max() < 1e-13
+        assert torch.autograd.gradcheck(lambda x: R.rotary_embedding_ref(x, None, inv, pos, interleaved, 1.5),
+                                        q.clone().requires_grad_())
