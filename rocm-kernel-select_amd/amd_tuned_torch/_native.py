@@ -2121,12 +2121,14 @@ def _linear_block(q, k, v, g, scale, initial_state, cu_seqlens):
     blk[6] = None
     if blk[2] != key:
         n = _linear_check(q, k, v, g, initial_state, cu_seqlens)
-        if q.stride(3) != 1 or k.stride(3) != 1 or v.stride(3) != 1 or not (
+        fits = [t.stride(3) == 1 and t.stride(1) < 1 << 22 for t in (q, k, v)]  # (the kernels' offsets within 64 tokens)
+        if not all(fits) or (g.dim() == 3 and g.stride(1) >= 1 << 22) or not (
                 (initial_state is None or initial_state.is_contiguous()) and (cu_seqlens is None or cu_seqlens.is_contiguous())):
-            q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
+            q, k, v = (t if ok else t.contiguous() for t, ok in zip((q, k, v), fits))
+            g = g.contiguous()
             initial_state = None if initial_state is None else initial_state.contiguous()
             cu_seqlens = None if cu_seqlens is None else cu_seqlens.contiguous()
-            blk[6] = (q, k, v, initial_state, cu_seqlens)
+            blk[6] = (q, k, v, g, initial_state, cu_seqlens)
             key = None
         blk[2] = None  # until all fields are set
         a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]

@@ -6,22 +6,25 @@
 namespace atk {
 
 constexpr int kLaMaxK = 256;                      // key columns: a state's rows
-constexpr int64_t kLaBlocks = (int64_t)1 << 23;   // workgroups of 256 in a launch of fewer than 2^32 threads
+constexpr int kLaBlocks = 1 << 22;                // workgroups of 256 in a launch: fewer than 2^32 threads, with two roles too
 
-// One chunked product over the sequences:
-//   out_i = sum over j of D_ij (a_i . b_j) c_j + f_i S^T a_i
-// with j up to i (or, in reverse, from i on), D_ij the decay between the two, f_i the one between i and the
-// chunk's first end that S stands at, and S the sum of decayed b c^T so far.  The forward has a, b, c = q, k, v;
-// the gradients: dq from dO, v, k; dk from v, dO, q in reverse; dv from k, q, dO in reverse.
+// One chunked product over the sequences, of which the forward and the gradients are four:
+//   out_i = scale sum over j of D_ij (a_i . b_j) c_j + f_i S^T a_i
+// with j up to i (or, in reverse, from i on), D_ij the decay between the two, S the sum of decayed b c^T of the
+// chunks before (in reverse: after), f_i the decay between i and where S stands.
+//   a, b, c        forward: q, k, v;  dv: k, q, dO in reverse;  dq: dO, v, k;  dk: v, dO, q in reverse
+// In reverse b c^T is scaled where it enters S, else where S is read.
+enum LaMode { kLaFwd = 0, kLaDv = 1, kLaDq = 2, kLaDk = 3 };
+constexpr bool la_reverse(int mode) { return mode == kLaDv || mode == kLaDk; }
+// whether a and b are of the value heads, c and out of the key heads, and S as stored has its rows over c's columns
+constexpr bool la_swapped(int mode) { return mode >= kLaDq; }
+
 struct LaRole {
-  const void* a; const void* b; const void* c; const void* e;
+  const void* a; const void* b; const void* c;
+  const void* e;                           // dots: the rows that out is multiplied with (of the key heads)
   int64_t a_s[3], b_s[3], c_s[3], e_s[3];  // strides in elements: batch, token, head
-  int a_key, b_key, c_key;                 // whether the head is the key head (e's is c's other side: the key head)
   int AD, CD;                              // columns of a and b, and of c, in all
   int a_tiles;                             // tiles of a's columns, each a sum of its own
-  int reverse;
-  int transposed;                          // whether S as stored has its rows over c's columns
-  int guard;                               // whether rows before the first non-finite c stay clean
   const float* s_first;                    // state that the first segment starts from, or null (zeros)
   const float* s_between;                  // [slot][Hv] states at the ends (in reverse: the starts) of segments, or null
   float* s_last;                           // where the last segment's state goes, or null
@@ -32,12 +35,13 @@ struct LaRole {
 };
 
 struct LaArgs {
-  LaRole role[3];
+  LaRole role[2];
   const void* g; int64_t g_s[3];
   const int* cu;
-  int64_t n, T, B;          // sequences; tokens of each (of the packed row with cu); first axis of the tensors
-  int64_t slots, seg;       // segments (unused ones of packed sequences among them), tokens of one
+  int64_t T, B;             // tokens of a sequence (of the packed row with cu); first axis of the tensors
+  int n, slots, seg;        // sequences; segments (unused ones of packed sequences among them), tokens of one
   int Hk, Hv, group, K, V, g_dtype, fixed;
+  FastDiv by_hk, by_hv, by_seg, by_segs;  // segments of a sequence where all have as many
   float scale;
 };
 
@@ -45,43 +49,49 @@ struct LaArgs {
 // on: the next one's begin at or after its end, so no prefix sum over the lengths is needed.  Offsets are
 // clamped to the row.
 struct LaSeq {
-  int64_t batch, begin, len, slot;
+  int batch, begin, len, slot, segs;
 };
-__device__ __forceinline__ LaSeq la_seq(const LaArgs& a, int64_t n) {
-  if (!a.cu) return {n, 0, a.T, n * (a.T > a.seg ? (a.T + a.seg - 1) / a.seg : 1)};
-  int64_t b = a.cu[n], e = a.cu[n + 1];
-  b = b < 0 ? 0 : b > a.T ? a.T : b;
-  e = e < b ? b : e > a.T ? a.T : e;
-  return {0, b, e - b, b / a.seg + n};
+__device__ __forceinline__ int la_segments(const LaArgs& a, int len) {
+  return len > a.seg ? (int)fdiv((uint32_t)(len - 1), a.by_seg) + 1 : 1;
 }
-__device__ __forceinline__ int64_t la_seq_of_slot(const LaArgs& a, int64_t slot) {
-  if (!a.cu) return slot / (a.T > a.seg ? (a.T + a.seg - 1) / a.seg : 1);
-  int64_t lo = 0, hi = a.n - 1;  // the last sequence whose first slot is not after `slot`
+__device__ __forceinline__ LaSeq la_seq(const LaArgs& a, int n) {
+  const int T = (int)a.T;
+  if (!a.cu) return {n, 0, T, n * (int)a.by_segs.d, (int)a.by_segs.d};
+  int b = a.cu[n], e = a.cu[n + 1];
+  b = b < 0 ? 0 : b > T ? T : b;
+  e = e < b ? b : e > T ? T : e;
+  return {0, b, e - b, (int)fdiv((uint32_t)b, a.by_seg) + n, la_segments(a, e - b)};
+}
+__device__ __forceinline__ int la_seq_of_slot(const LaArgs& a, int slot) {
+  if (!a.cu) return (int)fdiv((uint32_t)slot, a.by_segs);
+  int lo = 0, hi = a.n - 1;  // the last sequence whose first slot is not after `slot`
   while (lo < hi) {
-    const int64_t mid = (lo + hi + 1) / 2;
+    const int mid = (lo + hi + 1) / 2;
     if (la_seq(a, mid).slot <= slot) lo = mid;
     else hi = mid - 1;
   }
   return lo;
 }
-__device__ __forceinline__ int64_t la_segments(const LaSeq& s, int64_t seg) { return s.len > seg ? (s.len + seg - 1) / seg : 1; }
 
 // Workgroup -> (tile, value head, slot).  Workgroups are dealt to the 8 XCDs in turn; the tiles and value
-// heads of a key head get the same one, since they read the same rows through its L2.
-__device__ __forceinline__ bool la_place(const LaArgs& a, int64_t block, int tiles, int* tile, int* h, int64_t* slot) {
-  const int per = tiles * a.group;
-  const int64_t j = block / 8, unit = j / per * 8 + block % 8;
-  const int in = (int)(j % per);
-  *tile = in % tiles;
-  *h = (int)(unit % a.Hk) * a.group + in / tiles;
-  *slot = unit / a.Hk;
-  return *slot < a.slots;
+// heads of a key head get the same one, since they read the same rows through its L2.  A launch begins with
+// the first workgroup of unit `unit0`, a multiple of 8.
+struct LaGrid {
+  FastDiv per, tiles;  // workgroups of a unit (tiles of the value heads of a key head); tiles of a head
+  int unit0;
+};
+__device__ __forceinline__ bool la_place(const LaArgs& a, const LaGrid& gr, int* tile, int* h, int* slot) {
+  const uint32_t j = blockIdx.x / 8, u = fdiv(j, gr.per), unit = gr.unit0 + u * 8 + blockIdx.x % 8;
+  const uint32_t in = j - u * gr.per.d, head = fdiv(in, gr.tiles), s = fdiv(unit, a.by_hk);
+  *tile = (int)(in - head * gr.tiles.d);
+  *h = (int)((unit - s * a.by_hk.d) * a.group + head);
+  *slot = (int)s;
+  return s < (uint32_t)a.slots;
 }
-inline int64_t la_grid(const LaArgs& a, int tiles) { return (a.slots * a.Hk + 7) / 8 * 8 * tiles * a.group; }
 
-// Launchers, each for one type: outputs of roles first .. first + roles - 1, which share AD's padding and dots;
-// states of segments alone (roles 0 .. roles - 1, forward and reverse).
-template <typename T> int la_launch_out(const LaArgs& a, int first, int roles, bool dots, hipStream_t s);
+// Launchers, each for one type: the outputs of role 0, or of roles 0 and 1 for kLaDq (dq and dk); what segments
+// add to the states, forward and, with roles 2, in reverse.
+template <typename T> int la_launch_out(const LaArgs& a, int mode, bool dots, hipStream_t s);
 template <typename T> int la_launch_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s);
 
 inline int la_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }

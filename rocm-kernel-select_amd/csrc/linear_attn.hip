@@ -143,30 +143,29 @@ void launch_step_typed(const LaStepArgs& a, hipStream_t s) {
 // Segments joined: what each adds to the state becomes the state after it (in reverse, the gradient of the
 // state before it), in place.  A thread has VW elements of a state, all segments of a sequence.
 template <int VW>
-__global__ __launch_bounds__(256) void la_scan_kernel(LaArgs a, float* s0, float* s1, const float* decays, int per, int64_t first) {
-  const int64_t block = first + blockIdx.x;
-  const int64_t unit = block / per, n = unit / a.Hv;
-  const int h = (int)(unit - n * a.Hv);
-  const int64_t kv = (int64_t)a.K * a.V, i = ((block - unit * per) * 256 + threadIdx.x) * VW;
+__global__ __launch_bounds__(256) void la_scan_kernel(LaArgs a, float* s0, float* s1, const float* decays, FastDiv per, int first) {
+  const uint32_t unit = fdiv(blockIdx.x, per), nh = first + unit, n = fdiv(nh, a.by_hv);
+  const int h = (int)(nh - n * a.by_hv.d);
+  const int kv = a.K * a.V, i = (int)((blockIdx.x - unit * per.d) * 256 + threadIdx.x) * VW;
   const bool rev = blockIdx.y;
   if (i >= kv) return;
-  const LaSeq seq = la_seq(a, n);
-  const int64_t segs = la_segments(seq, a.seg);
-  const float* init = a.role[rev ? 2 : 0].s_first;
+  const LaSeq seq = la_seq(a, (int)n);
+  const int segs = seq.segs;
+  const float* init = a.role[rev].s_first;
   float run[VW];
 #pragma unroll
-  for (int j = 0; j < VW; ++j) run[j] = init ? init[(n * a.Hv + h) * kv + i + j] : 0.f;
-  const int64_t step = a.Hv * kv;
-  float* __restrict__ p = (rev ? s1 : s0) + (seq.slot + (rev ? segs - 1 : 0)) * step + h * kv + i;
-  const float* __restrict__ d = decays + ((rev ? a.slots : 0) + seq.slot + (rev ? segs - 1 : 0)) * a.Hv + h;
+  for (int j = 0; j < VW; ++j) run[j] = init ? init[(int64_t)nh * kv + i + j] : 0.f;
+  const int64_t step = (int64_t)a.Hv * kv;
+  float* __restrict__ p = (rev ? s1 : s0) + (seq.slot + (rev ? segs - 1 : 0)) * step + (int64_t)h * kv + i;
+  const float* __restrict__ d = decays + ((int64_t)(rev ? a.slots : 0) + seq.slot + (rev ? segs - 1 : 0)) * a.Hv + h;
   const int64_t ps = rev ? -step : step, ds = rev ? -a.Hv : a.Hv;
   constexpr int U = 8;  // segments whose loads are in flight together
-  for (int64_t z = 0; z + 1 < segs; z += U) {
+  for (int z = 0; z + 1 < segs; z += U) {
     float t[U][VW], f[U];
-    const int64_t left = segs - 1 - z;
+    const int left = segs - 1 - z;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t at = u < left ? u : 0;
+      const int at = u < left ? u : 0;
       __builtin_memcpy(t[u], p + at * ps, 4 * VW);
       f[u] = d[at * ds];
     }
@@ -218,22 +217,21 @@ struct LaGateArgs {
 template <typename G>
 __global__ __launch_bounds__(256) void la_gate_kernel(LaArgs a, LaGateArgs b) {
   const int lane = threadIdx.x & 63;
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int64_t slot = unit / a.Hv;
-  const int h = (int)(unit - slot * a.Hv);
+  const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int slot = (int)fdiv(unit, a.by_hv), h = (int)unit - slot * a.Hv;
   if (slot >= a.slots) return;
-  const int64_t n = la_seq_of_slot(a, slot);
+  const int n = la_seq_of_slot(a, slot);
   const LaSeq seq = la_seq(a, n);
-  const int64_t z = slot - seq.slot, segs = la_segments(seq, a.seg);
+  const int z = slot - seq.slot, segs = seq.segs;
   const bool live = z >= 0 && z < segs;
   const int64_t BT = a.B * a.T;
   double carry = 0, all = 0;
   if (live) {
-    const int64_t t0 = z * a.seg, left = seq.len - t0, len = left < a.seg ? left : a.seg;
-    const int64_t first = seq.batch * a.T + seq.begin + t0;
+    const int t0 = z * a.seg, left = seq.len - t0, len = left < a.seg ? left : a.seg;
+    const int64_t first = (int64_t)seq.batch * a.T + seq.begin + t0;
     for (int t = 0; t < b.tiles; ++t) carry += (double)b.x[((int64_t)t * a.slots + slot) * a.Hv + h];
-    for (int64_t end = len; end > 0; end -= 64) {
-      const int64_t t = end - 1 - lane;  // the lane's token, from the end
+    for (int end = len; end > 0; end -= 64) {
+      const int t = end - 1 - lane;  // the lane's token, from the end
       const int64_t at = first + (t > 0 ? t : 0);
       double v = 0;
       for (int i = 0; i < b.tiles; ++i) {
@@ -246,7 +244,7 @@ __global__ __launch_bounds__(256) void la_gate_kernel(LaArgs a, LaGateArgs b) {
         const double o = __shfl_up(v, off, 64);
         if (lane >= off) v += o;
       }
-      const GdrGate gr = gdr_gate_load(a.g, a.g_dtype, seq.batch * a.g_s[0] + (seq.begin + t0 + (t > 0 ? t : 0)) * a.g_s[1] + h * a.g_s[2]);
+      const GdrGate gr = gdr_gate_load(a.g, a.g_dtype, seq.batch * a.g_s[0] + (int64_t)(seq.begin + t0 + (t > 0 ? t : 0)) * a.g_s[1] + h * a.g_s[2]);
       const double dg = gdr_gate<G>(gr, a.g_dtype) < -120.f ? 0.0 : carry + v;
       if (t >= 0) {
         if (!a.fixed) static_cast<G*>(b.dg)[at * a.Hv + h] = from_f32<G>((float)dg);
@@ -258,7 +256,7 @@ __global__ __launch_bounds__(256) void la_gate_kernel(LaArgs a, LaGateArgs b) {
   if (a.fixed) {
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off, 64);
-    if (lane == 0) b.seg_sums[h * a.slots + slot] = (float)all;
+    if (lane == 0) b.seg_sums[(int64_t)h * a.slots + slot] = (float)all;
   } else if (live && a.cu) {  // tokens of no sequence
     if (n == 0 && z == 0)
       for (int64_t t = lane; t < seq.begin; t += 64) static_cast<G*>(b.dg)[t * a.Hv + h] = from_f32<G>(0.f);
@@ -318,14 +316,20 @@ LaPlan la_plan(const atk_linear_attn_args* p, bool backward, LaArgs* a, int* rc)
   const int64_t seg = la_segment_tokens(p);
   const double slots = p->cu_seqlens ? (double)(p->T / seg) + (double)p->N
                                      : (double)(p->T > seg ? (p->T + seg - 1) / seg : 1) * (double)p->N;
-  if (slots * p->Hv > 2147483647.0 || (double)p->N * (double)p->T > 1e15)
-    return *rc = fail(ATK_UNSUPPORTED, "linear attention: too many sequences and heads"), L;
+  if ((double)p->K * p->V >= (double)(1 << 29) || slots * p->Hv > 2147483000.0 || slots > 2147483000.0 || (double)p->N * (double)p->T > 1e15)
+    return *rc = fail(ATK_UNSUPPORTED, "linear attention: a state of 2^29 elements or more, or too many sequences and heads"), L;
   *a = LaArgs{};
-  a->g = p->g; a->cu = p->cu_seqlens; a->n = p->N; a->T = p->T; a->B = p->cu_seqlens ? 1 : p->N;
+  // the kernels' loads of 64 tokens have offsets of 32 bits
+  for (const int64_t* st : {p->q_stride, p->k_stride, p->v_stride, p->g_stride})
+    if (st[1] < 0 || st[1] >= (1 << 22)) return *rc = fail(ATK_UNSUPPORTED, "linear attention: tokens of 2^22 elements or more apart"), L;
+  if ((int64_t)p->Hv * p->V >= (1 << 22) && backward) return *rc = fail(ATK_UNSUPPORTED, "linear attention backward: 2^22 value columns or more"), L;
+  a->g = p->g; a->cu = p->cu_seqlens; a->n = (int)p->N; a->T = p->T; a->B = p->cu_seqlens ? 1 : p->N;
   for (int i = 0; i < 3; ++i) a->g_s[i] = p->g_stride[i];
-  a->slots = (int64_t)slots; a->seg = seg;
+  a->slots = (int)slots; a->seg = (int)seg;
   a->Hk = p->Hk; a->Hv = p->Hv; a->group = p->Hv / p->Hk; a->K = p->K; a->V = p->V;
   a->g_dtype = p->g_dtype; a->fixed = p->fixed_decay; a->scale = p->scale;
+  a->by_hk = make_fastdiv((uint32_t)p->Hk); a->by_hv = make_fastdiv((uint32_t)p->Hv); a->by_seg = make_fastdiv((uint32_t)seg);
+  a->by_segs = make_fastdiv((uint32_t)(p->T > seg ? (p->T + seg - 1) / seg : 1));
   L.split = p->T > seg;
   char* w = static_cast<char*>(p->workspace);
   auto take = [&](size_t floats) {
@@ -357,15 +361,16 @@ void la_copy3(int64_t (&to)[3], const int64_t* from) {
   for (int i = 0; i < 3; ++i) to[i] = from[i];
 }
 
-template <typename T>
 int la_scan(const LaArgs& a, float* s0, float* s1, const float* decays, int roles, hipStream_t s) {
   const int64_t kv = (int64_t)a.K * a.V;
-  const bool vec = kv % 4 == 0 && (!a.role[0].s_first || aligned16(a.role[0].s_first)) && (roles < 2 || !a.role[2].s_first || aligned16(a.role[2].s_first));
-  const int64_t per = (kv + (vec ? 1023 : 255)) / (vec ? 1024 : 256), grid = per * a.Hv * a.n;
-  for (int64_t b = 0; b < grid; b += kLaBlocks / 2) {
-    const dim3 g((unsigned)(grid - b < kLaBlocks / 2 ? grid - b : kLaBlocks / 2), (unsigned)roles);
-    if (vec) hipLaunchKernelGGL((la_scan_kernel<4>), g, dim3(256), 0, s, a, s0, s1, decays, (int)per, b);
-    else hipLaunchKernelGGL((la_scan_kernel<1>), g, dim3(256), 0, s, a, s0, s1, decays, (int)per, b);
+  bool vec = kv % 4 == 0;
+  for (int i = 0; i < roles; ++i) vec = vec && aligned16(a.role[i].s_first);
+  const int64_t per = (kv + (vec ? 1023 : 255)) / (vec ? 1024 : 256), units = (int64_t)a.n * a.Hv;
+  const int64_t most = kLaBlocks / per > 0 ? kLaBlocks / per : 1;
+  for (int64_t u = 0; u < units; u += most) {
+    const dim3 g((unsigned)((units - u < most ? units - u : most) * per), (unsigned)roles);
+    if (vec) hipLaunchKernelGGL((la_scan_kernel<4>), g, dim3(256), 0, s, a, s0, s1, decays, make_fastdiv((uint32_t)per), (int)u);
+    else hipLaunchKernelGGL((la_scan_kernel<1>), g, dim3(256), 0, s, a, s0, s1, decays, make_fastdiv((uint32_t)per), (int)u);
     if (int rc = check_launch("la_scan_kernel")) return rc;
   }
   return ATK_OK;
@@ -375,24 +380,24 @@ template <typename T>
 int la_forward(const atk_linear_attn_args* p, LaArgs& a, const LaPlan& L, hipStream_t s) {
   LaRole& r = a.role[0];
   r = LaRole{};
-  r.a = p->q; r.b = p->k; r.c = p->v; r.a_key = r.b_key = 1;
+  r.a = p->q; r.b = p->k; r.c = p->v;
   la_copy3(r.a_s, p->q_stride); la_copy3(r.b_s, p->k_stride); la_copy3(r.c_s, p->v_stride);
-  r.AD = a.K; r.CD = a.V; r.a_tiles = 1; r.guard = 1;
+  r.AD = a.K; r.CD = a.V; r.a_tiles = 1;
   r.s_first = static_cast<const float*>(p->initial_state); r.s_last = static_cast<float*>(p->final_state);
   r.out = p->out;
   if (L.split) {
     r.s_between = L.s_fwd;
     float* to[1] = {L.s_fwd};
     if (int rc = la_launch_states<T>(a, 1, to, L.decays, s)) return rc;
-    if (int rc = la_scan<T>(a, L.s_fwd, nullptr, L.decays, 1, s)) return rc;
+    if (int rc = la_scan(a, L.s_fwd, nullptr, L.decays, 1, s)) return rc;
   }
-  return la_launch_out<T>(a, 0, 1, false, s);
+  return la_launch_out<T>(a, kLaFwd, false, s);
 }
 
 template <typename T, typename G>
 int la_gates(const LaArgs& a, const LaPlan& L, void* dg, hipStream_t s) {
   LaGateArgs b = {L.dots[0], L.dots[1], L.x, dg, L.seg_sums, L.a_tiles * L.k_tiles};
-  hipLaunchKernelGGL((la_gate_kernel<G>), dim3((unsigned)((a.slots * a.Hv + 3) / 4)), dim3(256), 0, s, a, b);
+  hipLaunchKernelGGL((la_gate_kernel<G>), dim3((unsigned)(((int64_t)a.slots * a.Hv + 3) / 4)), dim3(256), 0, s, a, b);
   if (int rc = check_launch("la_gate_kernel")) return rc;
   if (!a.fixed) return ATK_OK;
   hipLaunchKernelGGL((la_gate_sum_kernel<G>), dim3((unsigned)a.Hv), dim3(256), 0, s, L.seg_sums, static_cast<G*>(dg), a.slots);
@@ -403,43 +408,39 @@ template <typename T>
 int la_backward(const atk_linear_attn_args* p, LaArgs& a, const LaPlan& L, const void* dout, const float* ds1, void* dq,
                 void* dk, void* dv, void* dg, float* ds0, hipStream_t s) {
   const int64_t vs[3] = {a.T * a.Hv * a.V, (int64_t)a.Hv * a.V, a.V};  // dout's strides
-  // roles 0 and 1: dq and dk; role 2: dv
-  LaRole& q = a.role[0];
-  LaRole& k = a.role[1];
-  LaRole& v = a.role[2];
-  q = k = v = LaRole{};
-  q.a = dout; q.b = p->v; q.c = p->k; q.e = p->q; q.c_key = 1;
-  la_copy3(q.a_s, vs); la_copy3(q.b_s, p->v_stride); la_copy3(q.c_s, p->k_stride); la_copy3(q.e_s, p->q_stride);
-  k.a = p->v; k.b = dout; k.c = p->q; k.e = p->k; k.c_key = 1; k.reverse = 1;
-  la_copy3(k.a_s, p->v_stride); la_copy3(k.b_s, vs); la_copy3(k.c_s, p->q_stride); la_copy3(k.e_s, p->k_stride);
-  v.a = p->k; v.b = p->q; v.c = dout; v.a_key = v.b_key = 1; v.reverse = 1;
+  LaArgs b = a;  // states of segments: k, v forward and q, dO in reverse, which is also dv's (k, q, dO)
+  LaRole& f = b.role[0];
+  LaRole& v = b.role[1];
+  f = v = LaRole{};
+  f.b = p->k; f.c = p->v;
+  la_copy3(f.b_s, p->k_stride); la_copy3(f.c_s, p->v_stride);
+  v.a = p->k; v.b = p->q; v.c = dout; v.out = dv;
   la_copy3(v.a_s, p->k_stride); la_copy3(v.b_s, p->q_stride); la_copy3(v.c_s, vs);
-  q.AD = k.AD = a.V; q.CD = k.CD = a.K; v.AD = a.K; v.CD = a.V;
-  q.a_tiles = k.a_tiles = L.a_tiles; v.a_tiles = 1;
-  q.transposed = k.transposed = 1;
-  q.s_first = static_cast<const float*>(p->initial_state);
-  k.s_first = v.s_first = ds1;
-  v.s_last = ds0;
-  q.out = dq; k.out = dk; v.out = dv;
-  q.parts = L.parts[0]; k.parts = L.parts[1];
-  if (dg) {
-    q.dots = L.dots[0]; k.dots = L.dots[1];
-    q.x_last = ds1; q.x_between = L.s_rev; q.x_out = L.x;
-  }
+  f.AD = v.AD = a.K; f.CD = v.CD = a.V; v.a_tiles = 1;
+  f.s_first = static_cast<const float*>(p->initial_state);
+  v.s_first = ds1; v.s_between = L.s_rev; v.s_last = ds0;
   if (L.split) {
-    q.s_between = L.s_fwd; k.s_between = v.s_between = L.s_rev;
-    // states of segments: k, v forward and q, dO in reverse
-    LaArgs b = a;
-    LaRole& f = b.role[0];
-    f = LaRole{};
-    f.b = p->k; f.c = p->v; f.b_key = 1; la_copy3(f.b_s, p->k_stride); la_copy3(f.c_s, p->v_stride);
-    f.AD = a.K; f.CD = a.V; f.s_first = q.s_first;
     float* to[2] = {L.s_fwd, L.s_rev};
     if (int rc = la_launch_states<T>(b, 2, to, L.decays, s)) return rc;
-    if (int rc = la_scan<T>(b, L.s_fwd, L.s_rev, L.decays, 2, s)) return rc;
+    if (int rc = la_scan(b, L.s_fwd, L.s_rev, L.decays, 2, s)) return rc;
   }
-  if (int rc = la_launch_out<T>(a, 0, 2, dg != nullptr, s)) return rc;
-  if (int rc = la_launch_out<T>(a, 2, 1, false, s)) return rc;
+  LaRole& q = a.role[0];
+  LaRole& k = a.role[1];
+  q = k = LaRole{};
+  q.a = dout; q.b = p->v; q.c = p->k; q.e = p->q; q.out = dq;
+  la_copy3(q.a_s, vs); la_copy3(q.b_s, p->v_stride); la_copy3(q.c_s, p->k_stride); la_copy3(q.e_s, p->q_stride);
+  k.a = p->v; k.b = dout; k.c = p->q; k.e = p->k; k.out = dk;
+  la_copy3(k.a_s, p->v_stride); la_copy3(k.b_s, vs); la_copy3(k.c_s, p->q_stride); la_copy3(k.e_s, p->k_stride);
+  q.AD = k.AD = a.V; q.CD = k.CD = a.K;
+  q.a_tiles = k.a_tiles = L.a_tiles;
+  q.s_first = f.s_first; q.s_between = L.s_fwd;
+  k.s_first = ds1; k.s_between = L.s_rev;
+  q.parts = L.parts[0]; k.parts = L.parts[1];
+  q.dots = L.dots[0]; k.dots = L.dots[1];
+  q.x_last = ds1; q.x_between = L.s_rev; q.x_out = L.x;
+  if (int rc = la_launch_out<T>(a, kLaDq, dg != nullptr, s)) return rc;
+  b.role[0] = v;
+  if (int rc = la_launch_out<T>(b, kLaDv, false, s)) return rc;
   if (L.n_parts > 1 && a.T > 0) {
     LaSumArgs m = {{L.parts[0], L.parts[1]}, {dq, dk}, a.B * a.T * a.Hk * (int64_t)a.K, L.n_parts};
     const bool vec = m.count % 4 == 0;

@@ -8,6 +8,8 @@
 // second operand.  Rows of a, b and c are staged in LDS in bf16 parts, the next chunk's loads in flight
 // meanwhile; products over tokens read them transposed (ds_read_tr).
 #pragma once
+#include <limits.h>
+
 #include "linear_attn.h"
 
 namespace atk {
@@ -50,17 +52,24 @@ struct LaTile {
   static constexpr int V = 16 / sizeof(T), PER = W / V, N = ROWS * PER / 256;
   static_assert(ROWS * PER % 256 == 0, "whole vectors a thread");
   uint4 r[N];
-  __device__ __forceinline__ void load(const T* __restrict__ p, int64_t stride, int rows, int cols) {
+  // `p` the same in all lanes; 64 rows are within 2^31 bytes (host check).  A tile that is not a row's first may
+  // have fewer columns than a vector: its loads begin in the tile before it, offsets stay positive.
+  __device__ __forceinline__ void load(const T* __restrict__ p, int stride, int rows, int cols) {
+    const int back = cols < V ? V - cols : 0;
+    const char* __restrict__ base = reinterpret_cast<const char*>(p - back);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int at = threadIdx.x + 256 * i, row = at / PER, c = at % PER * V;
-      const T* __restrict__ from = p + (row < rows ? row : 0) * stride + (c + V <= cols ? c : cols - V);
-      __builtin_memcpy(&r[i], from, 16);  // element alignment only
+      const uint32_t off = (uint32_t)(row < rows ? row : rows - 1) * (uint32_t)stride + (uint32_t)((c + V <= cols ? c : cols - V) + back);
+      __builtin_memcpy(&r[i], base + (size_t)(off * (uint32_t)sizeof(T)), 16);  // element alignment only
     }
   }
-  // as bf16 parts, `pitch` elements from row to row
-  template <int NP>
-  __device__ __forceinline__ void put(__bf16* lds, int pitch, int part, int rows, int cols) const {
+  // as bf16 parts, `pitch` elements from row to row.  GUARD: a zero of the triangular factor times a NaN or an
+  // infinity is NaN and would carry it to the tokens before its own, so such elements become zeros
+  // here; `bad` learns of each column's first one (at `from` + row), and *spoilt that there is any.
+  template <int NP, bool GUARD = false>
+  __device__ __forceinline__ void put(__bf16* lds, int pitch, int part, int rows, int cols, int from = 0, int* bad = nullptr,
+                                      int* spoilt = nullptr) const {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int at = threadIdx.x + 256 * i, row = at / PER, c = at % PER * V;
@@ -72,15 +81,36 @@ struct LaTile {
         v = __builtin_bit_cast(uint4, u);
       }
       if (row >= rows) v = make_uint4(0, 0, 0, 0);
+      T e[V];
+      __builtin_memcpy(e, &v, 16);
+      if constexpr (GUARD) {
+        float z = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) z = fmaf(to_f32(e[j]), 0.f, z);
+        if (__any(z != 0.f)) {
+#pragma nounroll
+          for (int j = 0; j < V; ++j) {
+            float f = 0.f;
+#pragma unroll
+            for (int q = 0; q < V; ++q) f = q == j ? to_f32(e[q]) : f;
+            if (f * 0.f != 0.f) {
+              atomicMin(&bad[c + j], from + row);
+              *spoilt = 1;
+#pragma unroll
+              for (int q = 0; q < V; ++q)
+                if (q == j) e[q] = from_f32<T>(0.f);
+            }
+          }
+          __builtin_memcpy(&v, e, 16);
+        }
+      }
       __bf16* to = lds + row * pitch + c;
       if constexpr (NP == 1) {
         *reinterpret_cast<uint4*>(to) = v;
       } else {
-        T e[V];
         float f[V];
         typedef __bf16 part_t __attribute__((ext_vector_type(V)));
         part_t parts[NP];
-        __builtin_memcpy(e, &v, 16);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[j] = to_f32(e[j]);
         split_parts<NP, V>(f, parts);
@@ -165,20 +195,40 @@ struct LaDecays {
   }
 };
 
-// S (or another matrix of its layout) between registers and memory: rows 16 t + 4 g + r from row i0 on,
-// columns col + 16 n.
-template <int RT, int NT, typename F>
-__device__ __forceinline__ void la_each(const LaArgs& a, const LaRole& r, int i0, int col, int g, F f) {
-  const int64_t si = r.transposed ? 1 : a.V, sj = r.transposed ? a.V : 1;
+// Where S (or another matrix of its layout) has element (16 t + 4 g + e, 16 x + c) of a tile: f(t, x, e, whether
+// it is there, its address, or another element's where it is not).  No branch around what f loads.  (A state has
+// fewer than 2^29 elements: host check.)
+template <int RT, int NT, bool SWAP, typename P, typename F>
+__device__ __forceinline__ void la_each(const LaArgs& a, const LaRole& r, int i0, int col, int g, P* p, F f) {
+  const int si = SWAP ? 1 : a.V, sj = SWAP ? a.V : 1;
+  uint32_t at[NT];
+#pragma unroll
+  for (int x = 0; x < NT; ++x) at[x] = (uint32_t)((col + 16 * x < r.CD ? col + 16 * x : 0) * sj);
 #pragma unroll
   for (int t = 0; t < RT; ++t)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int e = 0; e < 4; ++e) {
+      const int i = i0 + 16 * t + 4 * g + e;
+      const uint32_t row = (uint32_t)((i < r.AD ? i : 0) * si);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = i0 + 16 * t + 4 * g + e, j = col + 16 * n;
-        f(t, n, e, i < r.AD && j < r.CD, i * si + j * sj);
-      }
+      for (int x = 0; x < NT; ++x) f(t, x, e, i < r.AD && col + 16 * x < r.CD, p + (at[x] + row));
+    }
+}
+
+// full: the tile has no rows or columns past the state's
+template <int RT, int NT>
+__device__ __forceinline__ void la_store(const LaArgs& a, const LaRole& r, bool full, int col, int g, float* to, const f32x4 (&S)[RT][NT]) {
+  if (full) {
+    float* __restrict__ at = to + (uint32_t)(4 * g * a.V + col);
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int x = 0; x < NT; ++x) at[(uint32_t)((16 * t + e) * a.V) + 16 * x] = S[t][x][e];
+  } else {
+    la_each<RT, NT, false>(a, r, 0, col, g, to, [&](int t, int x, int e, bool in, float* p) { if (in) *p = S[t][x][e]; });
+  }
 }
 
 template <typename T, int DA, int NT, bool DOTS>
@@ -191,47 +241,51 @@ struct LaLds {
   uint4 p[PF][kLaOut<T, DOTS>][64];
   float o[4][16][PO];
   LaDecays<CT> d;
-  float dots[DOTS ? 4 : 1][CT];
+  union {
+    float dots[DOTS ? 4 : 1][CT];
+    int bad[W];  // (forward) each column's first token whose c is not finite
+  };
+  int spoilt;
 };
 
 // The outputs of one segment, and its last state.
-template <typename T, int DA, int NT, bool DOTS>
-__device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, char* lds, int64_t block) {
+template <typename T, int DA, int NT, int MODE, bool DOTS>
+__device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, const LaGrid& gr, char* lds) {
   using Lds = LaLds<T, DA, NT, DOTS>;
   constexpr int NP = Lds::NP, CT = Lds::CT, W = Lds::W, RT = DA / 16, KS = DA / 32, MT = CT / 16, HS = CT / 32;
   constexpr int OP = kLaOut<T, DOTS>, OW = 4 * NT;
   Lds& L = *reinterpret_cast<Lds*>(lds);
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c_tiles = (r.CD + W - 1) / W;
-  int tile, h;
-  int64_t slot;
-  if (!la_place(a, block, c_tiles * r.a_tiles, &tile, &h, &slot)) return;
-  const int hk = h / a.group, c_tile = tile % c_tiles, a_tile = tile / c_tiles;
-  const int64_t n = la_seq_of_slot(a, slot);
+  constexpr bool rev = la_reverse(MODE), swapped = la_swapped(MODE);
+  int tile, h, slot;
+  if (!la_place(a, gr, &tile, &h, &slot)) return;
+  const int hk = h / a.group, c_tiles = (r.CD + W - 1) / W, c_tile = swapped ? tile % c_tiles : tile, a_tile = swapped ? tile / c_tiles : 0;
+  const int n = la_seq_of_slot(a, slot);
   const LaSeq seq = la_seq(a, n);
-  const int64_t z = slot - seq.slot, segs = la_segments(seq, a.seg);
-  if (z < 0 || z >= segs) return;
-  const int64_t t0 = z * a.seg, left = seq.len - t0;
-  const int len = (int)(left < a.seg ? left : a.seg);  // tokens of this segment
+  const int z = slot - seq.slot;
+  if (z < 0 || z >= seq.segs) return;
+  const int t0 = z * a.seg, len = seq.len - t0 < a.seg ? seq.len - t0 : a.seg;  // tokens of this segment
   const int chunks = (len + CT - 1) / CT;
   const int a0 = a_tile * DA, col0 = c_tile * W, col = col0 + wave * 16 * NT + c;
   const int acols = r.AD - a0 < DA ? r.AD - a0 : DA, ccols = r.CD - col0 < W ? r.CD - col0 : W;
-  const bool rev = r.reverse;
+  const int ha = swapped ? h : hk, hc = MODE == kLaFwd || MODE == kLaDv ? h : hk;
   const int64_t first = seq.begin + t0;
-  const T* __restrict__ pa = static_cast<const T*>(r.a) + seq.batch * r.a_s[0] + first * r.a_s[1] + (r.a_key ? hk : h) * r.a_s[2] + a0;
-  const T* __restrict__ pb = static_cast<const T*>(r.b) + seq.batch * r.b_s[0] + first * r.b_s[1] + (r.b_key ? hk : h) * r.b_s[2] + a0;
-  const T* __restrict__ pc = static_cast<const T*>(r.c) + seq.batch * r.c_s[0] + first * r.c_s[1] + (r.c_key ? hk : h) * r.c_s[2] + col0;
+  const T* __restrict__ pa = static_cast<const T*>(r.a) + seq.batch * r.a_s[0] + first * r.a_s[1] + ha * r.a_s[2] + a0;
+  const T* __restrict__ pb = static_cast<const T*>(r.b) + seq.batch * r.b_s[0] + first * r.b_s[1] + ha * r.b_s[2] + a0;
+  const T* __restrict__ pc = static_cast<const T*>(r.c) + seq.batch * r.c_s[0] + first * r.c_s[1] + hc * r.c_s[2] + col0;
   const T* __restrict__ pe = DOTS ? static_cast<const T*>(r.e) + seq.batch * r.e_s[0] + first * r.e_s[1] + hk * r.e_s[2] + col0 : nullptr;
   const int64_t pg = seq.batch * a.g_s[0] + first * a.g_s[1] + h * a.g_s[2];
 
   f32x4 S[RT][NT];
-  const float* from = (rev ? z == segs - 1 : z == 0) ? r.s_first : r.s_between;
+  const float* from = (rev ? z == seq.segs - 1 : z == 0) ? r.s_first : r.s_between;
   bool have = from != nullptr;
   if (from) {
-    const int64_t at = from == r.s_first ? n * a.Hv + h : (slot + (rev ? 1 : -1)) * a.Hv + h;
-    from += at * a.K * a.V;
-    la_each<RT, NT>(a, r, a0, col, g, [&](int t, int m, int e, bool in, int64_t i) { S[t][m][e] = in ? from[i] : 0.f; });
+    const int64_t at = (int64_t)((rev ? z == seq.segs - 1 : z == 0) ? n : slot + (rev ? 1 : -1)) * a.Hv + h;
+    la_each<RT, NT, swapped>(a, r, a0, col, g, from + at * a.K * a.V, [&](int t, int x, int e, bool in, const float* p) {
+      const float v = *p;
+      S[t][x][e] = in ? v : 0.f;
+    });
   } else {
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -244,17 +298,22 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, cha
   GdrGate tg;
   auto load = [&](int ch) {
     const int at = ch * CT, rows = len - at < CT ? len - at : CT;
-    ta.load(pa + at * r.a_s[1], r.a_s[1], rows, acols);
-    tb.load(pb + at * r.b_s[1], r.b_s[1], rows, acols);
-    tc.load(pc + at * r.c_s[1], r.c_s[1], rows, ccols);
+    ta.load(pa + at * r.a_s[1], (int)r.a_s[1], rows, acols);
+    tb.load(pb + at * r.b_s[1], (int)r.b_s[1], rows, acols);
+    tc.load(pc + at * r.c_s[1], (int)r.c_s[1], rows, ccols);
     tg = gdr_gate_load(a.g, a.g_dtype, pg + (at + (lane < rows ? lane : 0)) * a.g_s[1]);
   };
   if (chunks > 0) load(rev ? chunks - 1 : 0);
+  if constexpr (MODE == kLaFwd) {
+    for (int i = tid; i < W; i += 256) L.bad[i] = INT_MAX;
+    if (tid == 0) L.spoilt = 0;
+    __syncthreads();
+  }
   for (int k = 0; k < chunks; ++k) {
     const int ch = rev ? chunks - 1 - k : k, at = ch * CT, rows = len - at < CT ? len - at : CT;
     ta.template put<NP>(&L.a[0][0][0], Lds::PA, CT * Lds::PA, rows, acols);
     tb.template put<NP>(&L.b[0][0][0], Lds::PA, CT * Lds::PA, rows, acols);
-    tc.template put<NP>(&L.c[0][0][0], Lds::PC, CT * Lds::PC, rows, ccols);
+    tc.template put<NP, MODE == kLaFwd>(&L.c[0][0][0], Lds::PC, CT * Lds::PC, rows, ccols, at, L.bad, &L.spoilt);
     if (wave == 0) L.d.put(gdr_gate<T>(tg, a.g_dtype), lane, rows);
     __syncthreads();
     load(k + 1 < chunks ? (rev ? ch - 1 : ch + 1) : ch);  // (at the end the last one's again)
@@ -300,15 +359,23 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, cha
       }
     }
     __syncthreads();
-    uint4 cf[HS][NT][NP];
+    // 32 tokens of this wave's columns of c
+    auto load_c = [&](int s, uint4 (&f)[NT][NP]) {
 #pragma unroll
-    for (int s = 0; s < HS; ++s)
+      for (int x = 0; x < NT; ++x)
 #pragma unroll
-      for (int m = 0; m < NT; ++m)
+        for (int p = 0; p < NP; ++p) f[x][p] = la_col(&L.c[p][32 * s][wave * 16 * NT + 16 * x], Lds::PC, lane);
+    };
+    T ev[DOTS ? MT : 1][OW];
+    const int orow = lane >> 2, oc = wave * 16 * NT + (lane & 3) * OW;  // a lane's row of 16 and first column of a result
+    const bool whole = col0 + oc + OW <= r.CD;
+    if constexpr (DOTS) {
 #pragma unroll
-        for (int p = 0; p < NP; ++p) cf[s][m][p] = la_col(&L.c[p][32 * s][wave * 16 * NT + 16 * m], Lds::PC, lane);
+      for (int m = 0; m < MT; ++m)
+        __builtin_memcpy(ev[m], pe + (at + (16 * m + orow < rows ? 16 * m + orow : 0)) * r.e_s[1] + (whole ? oc : -col0), OW * sizeof(T));
+    }
     f32x4 acc[MT][NT];
-    for (bool clean = false;; clean = true) {
+    {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -341,18 +408,7 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, cha
 #pragma unroll
       for (int s = 0; s < HS; ++s) {
         uint4 b[NT][NP];
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-#pragma unroll
-          for (int p = 0; p < NP; ++p) b[x][p] = cf[s][x][p];
-          if (clean) {
-            float v[8];
-            la_values<NP>(b[x], v);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = gdr_finite(v[e]);
-            la_split<NP>(v, b[x]);
-          }
-        }
+        load_c(s, b);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           if (HS > 1 && (rev ? s < m >> 1 : s > m >> 1)) continue;
@@ -368,48 +424,71 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, cha
           for (int x = 0; x < NT; ++x) acc[m][x] = y[0][x];
         }
       }
-      if (clean || !r.guard) break;
-      bool spoilt = false;
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int x = 0; x < NT; ++x) spoilt |= gdr_spoilt<4>(acc[m][x]);
-      if (!__any(spoilt)) break;
     }
-    if (r.guard) {
-      // (only after a second pass can outputs that are not finite be owed to c: those from the first such row on)
-      bool spoilt = false;
-#pragma unroll
-      for (int s = 0; s < HS; ++s)
+    if constexpr (MODE == kLaFwd) {
+      if (L.spoilt) {  // outputs from a column's first c on that is not finite are not either
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-          float v[8];
-          la_values<NP>(cf[s][x], v);
-          spoilt |= gdr_spoilt<8>(v);
-        }
-      if (__any(spoilt)) {
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          int bad = CT;  // this column's first token that is not finite
-#pragma unroll
-          for (int s = 0; s < HS; ++s) {
-            float v[8];
-            la_values<NP>(cf[s][x], v);
-#pragma unroll
-            for (int e = 7; e >= 0; --e) {
-              const int tok = 32 * s + gdr_at(g, e);
-              if (gdr_spoilt<1>(&v[e]) && tok < bad) bad = tok;
-            }
-          }
-          int other = __shfl_xor(bad, 16, 64);
-          bad = other < bad ? other : bad;
-          other = __shfl_xor(bad, 32, 64);
-          bad = other < bad ? other : bad;
+          const int bad = L.bad[wave * 16 * NT + 16 * x + c];
 #pragma unroll
           for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (16 * m + 4 * g + e >= bad) acc[m][x][e] = gdr_nan();
+              if (at + 16 * m + 4 * g + e >= bad) acc[m][x][e] = gdr_nan();
+        }
+      }
+    }
+    // rows of 16 tokens through LDS: OW columns of one a lane
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses keep their order)
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) L.o[wave][4 * g + e][16 * x + c] = acc[m][x][e];
+      __builtin_amdgcn_wave_barrier();
+      float o[OW];
+#pragma unroll
+      for (int e = 0; e < OW; e += 4) {
+        const f32x4 t = *reinterpret_cast<const f32x4*>(&L.o[wave][orow][(lane & 3) * OW + e]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[e + q] = t[q];
+      }
+      const int row = 16 * m + orow;
+      if constexpr (DOTS) {
+        float dot = 0.f;
+        if (whole) {
+#pragma unroll
+          for (int q = 0; q < OW; ++q) dot += o[q] * to_f32(ev[m][q]);
+        } else if (row < rows) {
+          const T* __restrict__ e = pe + (at + row) * r.e_s[1] + oc;
+#pragma unroll
+          for (int q = 0; q < OW; ++q)
+            if (col0 + oc + q < r.CD) dot += o[q] * to_f32(e[q]);
+        }
+        dot += dpp_mov<0xB1>(dot);
+        dot += dpp_mov<0x4E>(dot);
+        if ((lane & 3) == 0) L.dots[wave][row] = dot;
+      }
+      if (row < rows) {
+        const int64_t tok = seq.batch * a.T + first + at + row;
+        if (swapped && r.parts) {
+          float* __restrict__ to = r.parts + ((((int64_t)(h % a.group) * r.a_tiles + a_tile) * a.B * a.T + tok) * a.Hk + hk) * r.CD + col0 + oc;
+#pragma unroll
+          for (int q = 0; q < OW; ++q)
+            if (whole || col0 + oc + q < r.CD) to[q] = o[q];
+        } else {
+          T* __restrict__ to = static_cast<T*>(r.out) + (tok * (swapped ? a.Hk : a.Hv) + hc) * r.CD + col0 + oc;
+          T v[OW];
+#pragma unroll
+          for (int q = 0; q < OW; ++q) v[q] = from_f32<T>(o[q]);
+          if (whole) {
+            __builtin_memcpy(to, v, OW * sizeof(T));
+          } else {
+#pragma unroll
+            for (int q = 0; q < OW; ++q)
+              if (col0 + oc + q < r.CD) to[q] = v[q];
+          }
         }
       }
     }
@@ -431,10 +510,12 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, cha
 #pragma unroll
           for (int e = 0; e < 4; ++e) f[4 * u + e] = t[e];
         }
+        uint4 cf[NT][NP];
+        load_c(s, cf);
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
           float v[8];
-          la_values<NP>(cf[s][x], v);
+          la_values<NP>(cf[x], v);
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] *= f[e];
           la_split<3>(v, cw[x]);
@@ -459,59 +540,6 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, cha
       }
       have = true;
     }
-    // rows of 16 tokens through LDS: OW columns of one a lane
-    const int orow = lane >> 2, oc = wave * 16 * NT + (lane & 3) * OW;
-    const bool whole = col0 + oc + OW <= r.CD;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses keep their order)
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) L.o[wave][4 * g + e][16 * x + c] = acc[m][x][e];
-      __builtin_amdgcn_wave_barrier();
-      float o[OW];
-#pragma unroll
-      for (int e = 0; e < OW; e += 4) {
-        const f32x4 t = *reinterpret_cast<const f32x4*>(&L.o[wave][orow][(lane & 3) * OW + e]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) o[e + q] = t[q];
-      }
-      const int row = 16 * m + orow;
-      if constexpr (DOTS) {
-        float dot = 0.f;
-        if (row < rows) {
-          const T* __restrict__ e = pe + (at + row) * r.e_s[1] + oc;
-#pragma unroll
-          for (int q = 0; q < OW; ++q)
-            if (whole || col0 + oc + q < r.CD) dot += o[q] * to_f32(e[q]);
-        }
-        dot += dpp_mov<0xB1>(dot);
-        dot += dpp_mov<0x4E>(dot);
-        if ((lane & 3) == 0) L.dots[wave][row] = dot;
-      }
-      if (row < rows) {
-        const int64_t tok = seq.batch * a.T + first + at + row;
-        if (r.parts) {
-          float* __restrict__ to = r.parts + ((((int64_t)(h % a.group) * r.a_tiles + a_tile) * a.B * a.T + tok) * a.Hk + hk) * r.CD + col0 + oc;
-#pragma unroll
-          for (int q = 0; q < OW; ++q)
-            if (whole || col0 + oc + q < r.CD) to[q] = o[q];
-        } else {
-          T* __restrict__ to = static_cast<T*>(r.out) + (tok * (r.e ? a.Hk : a.Hv) + (r.e ? hk : h)) * r.CD + col0 + oc;
-          T v[OW];
-#pragma unroll
-          for (int q = 0; q < OW; ++q) v[q] = from_f32<T>(o[q]);
-          if (whole) {
-            __builtin_memcpy(to, v, OW * sizeof(T));
-          } else {
-#pragma unroll
-            for (int q = 0; q < OW; ++q)
-              if (col0 + oc + q < r.CD) to[q] = v[q];
-          }
-        }
-      }
-    }
     __syncthreads();  // the chunk's LDS is free
     if constexpr (DOTS) {
       if (tid < rows)
@@ -519,17 +547,30 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, cha
             (L.dots[0][tid] + L.dots[1][tid]) + (L.dots[2][tid] + L.dots[3][tid]);
     }
   }
-  if (r.s_last && (rev ? z == 0 : z == segs - 1)) {
-    float* __restrict__ to = r.s_last + (n * a.Hv + h) * a.K * a.V;
-    la_each<RT, NT>(a, r, a0, col, g, [&](int t, int m, int e, bool in, int64_t i) { if (in) to[i] = S[t][m][e]; });
+  if (!swapped && r.s_last && (rev ? z == 0 : z == seq.segs - 1)) {
+    if constexpr (MODE == kLaFwd) {
+      if (L.spoilt) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+          if (L.bad[wave * 16 * NT + 16 * x + c] != INT_MAX)
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) S[t][x][e] = gdr_nan();
+      }
+    }
+    la_store<RT, NT>(a, r, acols == DA && ccols == W, col, g, r.s_last + ((int64_t)n * a.Hv + h) * a.K * a.V, S);
   }
   if constexpr (DOTS) {
-    if (r.x_out) {  // the state at the segment's end, and the gradient of it from what follows
+    if (MODE == kLaDq) {  // the state at the segment's end, and the gradient of it from what follows
       float x = 0.f;
-      const float* d = z == segs - 1 ? r.x_last : r.x_between;
+      const float* d = z == seq.segs - 1 ? r.x_last : r.x_between;
       if (d) {
-        d += (z == segs - 1 ? n * a.Hv + h : (slot + 1) * a.Hv + h) * a.K * a.V;
-        la_each<RT, NT>(a, r, a0, col, g, [&](int t, int m, int e, bool in, int64_t i) { x += in ? S[t][m][e] * d[i] : 0.f; });
+        d += ((int64_t)(z == seq.segs - 1 ? n : slot + 1) * a.Hv + h) * a.K * a.V;
+        la_each<RT, NT, swapped>(a, r, a0, col, g, d, [&](int t, int m, int e, bool in, const float* p) {
+          const float v = *p;
+          x += in ? S[t][m][e] * v : 0.f;
+        });
       }
       x = wave_sum(x);
       __syncthreads();
@@ -540,27 +581,35 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, cha
   }
   // tokens of a packed row before its first sequence and after its last have zeros
   if (a.cu && a_tile == 0) {
-    const int heads = r.e ? a.Hk : a.Hv, ho = r.e ? hk : h;
     for (int w = 0; w < 2; ++w) {
-      if (w == 0 ? n != 0 || z != 0 : n != a.n - 1 || z != segs - 1) continue;
+      if (w == 0 ? n != 0 || z != 0 : n != a.n - 1 || z != seq.segs - 1) continue;
       const int64_t b = w == 0 ? 0 : seq.begin + seq.len, end = w == 0 ? seq.begin : a.T;
       for (int64_t t = b; t < end; ++t)
         for (int j = tid; j < ccols; j += 256) {
-          if (r.parts) {
+          if (swapped && r.parts) {
             for (int q = 0; q < r.a_tiles; ++q)
               r.parts[((((int64_t)(h % a.group) * r.a_tiles + q) * a.B * a.T + t) * a.Hk + hk) * r.CD + col0 + j] = 0.f;
           } else {
-            static_cast<T*>(r.out)[(t * heads + ho) * r.CD + col0 + j] = from_f32<T>(0.f);
+            static_cast<T*>(r.out)[(t * (swapped ? a.Hk : a.Hv) + hc) * r.CD + col0 + j] = from_f32<T>(0.f);
           }
         }
     }
   }
 }
 
+// Waves of a SIMD that a kernel is compiled for: two workgroups share a CU where their LDS lets them.
+template <typename Lds> inline constexpr int kLaWaves = 2 * sizeof(Lds) <= 163840 ? 2 : 1;
+
+template <typename T, int DA, int NT, int MODE>
+__global__ __launch_bounds__(256, (kLaWaves<LaLds<T, DA, NT, false>>)) void la_out_kernel(LaArgs a, LaGrid gr) {
+  __shared__ __align__(16) char lds[sizeof(LaLds<T, DA, NT, false>)];
+  la_segment<T, DA, NT, MODE, false>(a, a.role[0], gr, lds);
+}
 template <typename T, int DA, int NT, bool DOTS>
-__global__ __launch_bounds__(256, 2) void la_out_kernel(LaArgs a, int role, int64_t first) {
+__global__ __launch_bounds__(256, (kLaWaves<LaLds<T, DA, NT, DOTS>>)) void la_dqk_kernel(LaArgs a, LaGrid gr) {
   __shared__ __align__(16) char lds[sizeof(LaLds<T, DA, NT, DOTS>)];
-  la_segment<T, DA, NT, DOTS>(a, a.role[role + blockIdx.y], lds, first + blockIdx.x);
+  if (blockIdx.y == 0) la_segment<T, DA, NT, kLaDq, DOTS>(a, a.role[0], gr, lds);
+  else la_segment<T, DA, NT, kLaDk, DOTS>(a, a.role[1], gr, lds);
 }
 
 template <typename T, int DA, int NT>
@@ -573,31 +622,26 @@ struct LaStateLds {
 
 // What a segment adds to the state, and its decay: b and c alone.  The last segment's (in reverse the
 // first's) nobody asks for.
-template <typename T, int DA, int NT>
-__global__ __launch_bounds__(256, 2) void la_state_kernel(LaArgs a, float* to0, float* to1, float* decays, int64_t block0) {
+template <typename T, int DA, int NT, bool rev>
+__device__ __forceinline__ void la_state(const LaArgs& a, const LaRole& r, const LaGrid& gr, char* lds, float* to, float* decays) {
   using Lds = LaStateLds<T, DA, NT>;
   constexpr int NP = Lds::NP, CT = Lds::CT, W = Lds::W, RT = DA / 16, HS = CT / 32;
-  __shared__ __align__(16) char lds[sizeof(Lds)];
   Lds& L = *reinterpret_cast<Lds*>(lds);
-  const LaRole& r = a.role[blockIdx.y ? 2 : 0];  // k, v; in reverse q, dO
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  int tile, h;
-  int64_t slot;
-  if (!la_place(a, block0 + blockIdx.x, (r.CD + W - 1) / W, &tile, &h, &slot)) return;
+  int tile, h, slot;
+  if (!la_place(a, gr, &tile, &h, &slot)) return;
   const int hk = h / a.group;
-  const int64_t n = la_seq_of_slot(a, slot);
+  const int n = la_seq_of_slot(a, slot);
   const LaSeq seq = la_seq(a, n);
-  const int64_t z = slot - seq.slot, segs = la_segments(seq, a.seg);
-  const bool rev = r.reverse;
-  if (z < 0 || z >= segs || z == (rev ? 0 : segs - 1)) return;
-  const int64_t t0 = z * a.seg, left = seq.len - t0;
-  const int len = (int)(left < a.seg ? left : a.seg), chunks = (len + CT - 1) / CT;
+  const int z = slot - seq.slot;
+  if (z < 0 || z >= seq.segs || z == (rev ? 0 : seq.segs - 1)) return;
+  const int t0 = z * a.seg, len = seq.len - t0 < a.seg ? seq.len - t0 : a.seg, chunks = (len + CT - 1) / CT;
   const int col0 = tile * W, col = col0 + wave * 16 * NT + c;
   const int acols = r.AD, ccols = r.CD - col0 < W ? r.CD - col0 : W;
   const int64_t first = seq.begin + t0;
-  const T* __restrict__ pb = static_cast<const T*>(r.b) + seq.batch * r.b_s[0] + first * r.b_s[1] + (r.b_key ? hk : h) * r.b_s[2];
-  const T* __restrict__ pc = static_cast<const T*>(r.c) + seq.batch * r.c_s[0] + first * r.c_s[1] + (r.c_key ? hk : h) * r.c_s[2] + col0;
+  const T* __restrict__ pb = static_cast<const T*>(r.b) + seq.batch * r.b_s[0] + first * r.b_s[1] + hk * r.b_s[2];
+  const T* __restrict__ pc = static_cast<const T*>(r.c) + seq.batch * r.c_s[0] + first * r.c_s[1] + h * r.c_s[2] + col0;
   const int64_t pg = seq.batch * a.g_s[0] + first * a.g_s[1] + h * a.g_s[2];
   f32x4 S[RT][NT];
 #pragma unroll
@@ -610,8 +654,8 @@ __global__ __launch_bounds__(256, 2) void la_state_kernel(LaArgs a, float* to0, 
   GdrGate tg;
   auto load = [&](int ch) {
     const int at = ch * CT, rows = len - at < CT ? len - at : CT;
-    tb.load(pb + at * r.b_s[1], r.b_s[1], rows, acols);
-    tc.load(pc + at * r.c_s[1], r.c_s[1], rows, ccols);
+    tb.load(pb + at * r.b_s[1], (int)r.b_s[1], rows, acols);
+    tc.load(pc + at * r.c_s[1], (int)r.c_s[1], rows, ccols);
     tg = gdr_gate_load(a.g, a.g_dtype, pg + (at + (lane < rows ? lane : 0)) * a.g_s[1]);
   };
   load(rev ? chunks - 1 : 0);
@@ -672,46 +716,57 @@ __global__ __launch_bounds__(256, 2) void la_state_kernel(LaArgs a, float* to0, 
     }
     __syncthreads();
   }
-  float* __restrict__ to = (blockIdx.y ? to1 : to0) + (slot * a.Hv + h) * a.K * a.V;
-  la_each<RT, NT>(a, r, 0, col, g, [&](int t, int m, int e, bool in, int64_t i) { if (in) to[i] = S[t][m][e]; });
-  if (tile == 0 && tid == 0) decays[(blockIdx.y * a.slots + slot) * a.Hv + h] = gdr_decay(total, make_float2(0.f, 0.f));
+  la_store<RT, NT>(a, r, acols == DA && ccols == W, col, g, to + ((int64_t)slot * a.Hv + h) * a.K * a.V, S);
+  if (tile == 0 && tid == 0) decays[(int64_t)slot * a.Hv + h] = gdr_decay(total, make_float2(0.f, 0.f));
+}
+// Roles 0 and, where there is a second row of workgroups, 1 in reverse.
+template <typename T, int DA, int NT>
+__global__ __launch_bounds__(256, 2) void la_state_kernel(LaArgs a, LaGrid gr, float* to0, float* to1, float* decays) {
+  __shared__ __align__(16) char lds[sizeof(LaStateLds<T, DA, NT>)];
+  if (blockIdx.y == 0) la_state<T, DA, NT, false>(a, a.role[0], gr, lds, to0, decays);
+  else la_state<T, DA, NT, true>(a, a.role[1], gr, lds, to1, decays + (int64_t)a.slots * a.Hv);
 }
 
-template <typename T, int DA, int NT, bool DOTS>
-int la_run_out(const LaArgs& a, int first, int roles, hipStream_t s) {
-  const LaRole& r = a.role[first];
-  const int64_t grid = la_grid(a, (r.CD + 64 * NT - 1) / (64 * NT) * r.a_tiles);
-  for (int64_t b = 0; b < grid; b += kLaBlocks / 4) {
-    const dim3 gr((unsigned)(grid - b < kLaBlocks / 4 ? grid - b : kLaBlocks / 4), (unsigned)roles);
-    hipLaunchKernelGGL((la_out_kernel<T, DA, NT, DOTS>), gr, dim3(256), 0, s, a, first, b);
-    if (int rc = check_launch("la_out_kernel")) return rc;
+// launch(grid, its place) for workgroups of all tiles, heads and segments, in as many launches as it takes
+template <typename F>
+int la_launches(const LaArgs& a, int64_t tiles, const char* what, F launch) {
+  const int64_t per = tiles * a.group, units = ((int64_t)a.slots * a.Hk + 7) / 8 * 8;
+  if (per > kLaBlocks / 8) return fail(ATK_UNSUPPORTED, "linear attention: too many value heads and columns of a key head");
+  const int64_t most = kLaBlocks / 8 / per * 8;
+  for (int64_t u = 0; u < units; u += most) {
+    launch((unsigned)((units - u < most ? units - u : most) * per),
+           LaGrid{make_fastdiv((uint32_t)per), make_fastdiv((uint32_t)tiles), (int)u});
+    if (int rc = check_launch(what)) return rc;
   }
   return ATK_OK;
 }
 template <typename T, int DA, int NT>
+int la_run_out(const LaArgs& a, int mode, bool dots, hipStream_t s) {
+  const LaRole& r = a.role[0];
+  return la_launches(a, (int64_t)((r.CD + 64 * NT - 1) / (64 * NT)) * r.a_tiles, "la_out_kernel", [&](unsigned n, LaGrid g) {
+    if (mode == kLaFwd) hipLaunchKernelGGL((la_out_kernel<T, DA, NT, kLaFwd>), dim3(n), dim3(256), 0, s, a, g);
+    else if (mode == kLaDv) hipLaunchKernelGGL((la_out_kernel<T, DA, NT, kLaDv>), dim3(n), dim3(256), 0, s, a, g);
+    else if (dots) hipLaunchKernelGGL((la_dqk_kernel<T, DA, NT, true>), dim3(n, 2), dim3(256), 0, s, a, g);
+    else hipLaunchKernelGGL((la_dqk_kernel<T, DA, NT, false>), dim3(n, 2), dim3(256), 0, s, a, g);
+  });
+}
+template <typename T, int DA, int NT>
 int la_run_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s) {
-  const int64_t grid = la_grid(a, (a.V + 64 * NT - 1) / (64 * NT));
-  for (int64_t b = 0; b < grid; b += kLaBlocks / 4) {
-    const dim3 gr((unsigned)(grid - b < kLaBlocks / 4 ? grid - b : kLaBlocks / 4), (unsigned)roles);
-    hipLaunchKernelGGL((la_state_kernel<T, DA, NT>), gr, dim3(256), 0, s, a, to[0], roles > 1 ? to[1] : nullptr, decays, b);
-    if (int rc = check_launch("la_state_kernel")) return rc;
-  }
-  return ATK_OK;
+  return la_launches(a, (a.V + 64 * NT - 1) / (64 * NT), "la_state_kernel", [&](unsigned n, LaGrid g) {
+    hipLaunchKernelGGL((la_state_kernel<T, DA, NT>), dim3(n, (unsigned)roles), dim3(256), 0, s, a, g, to[0], roles > 1 ? to[1] : nullptr, decays);
+  });
 }
 
 }  // namespace
 
 template <typename T>
-int la_launch_out(const LaArgs& a, int first, int roles, bool dots, hipStream_t s) {
-  const LaRole& r = a.role[first];
-  const int da = la_padded(r.AD), nt = la_wide(da, r.CD);
-#define ATK_LA(DA, NT) return dots ? la_run_out<T, DA, NT, true>(a, first, roles, s) : la_run_out<T, DA, NT, false>(a, first, roles, s)
-  if (da == 256) ATK_LA(256, 1);
-  if (da == 128 && nt == 2) ATK_LA(128, 2);
-  if (da == 128) ATK_LA(128, 1);
-  if (nt == 2) ATK_LA(64, 2);
-  ATK_LA(64, 1);
-#undef ATK_LA
+int la_launch_out(const LaArgs& a, int mode, bool dots, hipStream_t s) {
+  const int da = la_padded(a.role[0].AD), nt = la_wide(da, a.role[0].CD);
+  if (da == 256) return la_run_out<T, 256, 1>(a, mode, dots, s);
+  if (da == 128 && nt == 2) return la_run_out<T, 128, 2>(a, mode, dots, s);
+  if (da == 128) return la_run_out<T, 128, 1>(a, mode, dots, s);
+  if (nt == 2) return la_run_out<T, 64, 2>(a, mode, dots, s);
+  return la_run_out<T, 64, 1>(a, mode, dots, s);
 }
 template <typename T>
 int la_launch_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s) {
