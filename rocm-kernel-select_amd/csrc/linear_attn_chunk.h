@@ -55,67 +55,93 @@ struct LaTile {
   // `p` the same in all lanes; 64 rows are within 2^31 bytes (host check).  A tile that is not a row's first may
   // have fewer columns than a vector: its loads begin in the tile before it, offsets stay positive.
   __device__ __forceinline__ void load(const T* __restrict__ p, int stride, int rows, int cols) {
-    const int back = cols < V ? V - cols : 0;
-    const char* __restrict__ base = reinterpret_cast<const char*>(p - back);
+    const int back = cols < V ? V - cols : 0, row0 = threadIdx.x / PER, c = threadIdx.x % PER * V;
+    const uint32_t col = (uint32_t)((c + V <= cols ? c : cols - V) + back);
+    constexpr int STEP = 256 / PER;  // rows from one vector of a thread to its next
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + 256 * i, row = at / PER, c = at % PER * V;
-      const uint32_t off = (uint32_t)(row < rows ? row : rows - 1) * (uint32_t)stride + (uint32_t)((c + V <= cols ? c : cols - V) + back);
-      __builtin_memcpy(&r[i], base + (size_t)(off * (uint32_t)sizeof(T)), 16);  // element alignment only
+      // row0 + i STEP, or the last row
+      const int row = row0 < rows - 1 - i * STEP ? row0 : rows - 1 - i * STEP;
+      const uint32_t off = ((uint32_t)(row + i * STEP) * (uint32_t)stride + col) * (uint32_t)sizeof(T);
+      __builtin_memcpy(&r[i], reinterpret_cast<const char*>(p - back) + (size_t)off, 16);  // element alignment only
     }
+  }
+  // NaN or not zero where one of a vector's elements is not finite
+  static __device__ __forceinline__ float spoilt_by(uint4 v) {
+    float z = 0.f;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        z = fmaf(__uint_as_float(w[j]), 0.f, z);
+      } else if constexpr (__is_same(T, __bf16)) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        z = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w[j]), b2{0, 0}, z, false);
+      } else {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        z = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w[j]), h2{0, 0}, z, false);
+      }
+    }
+    return z;
   }
   // as bf16 parts, `pitch` elements from row to row.  GUARD: a zero of the triangular factor times a NaN or an
   // infinity is NaN and would carry it to the tokens before its own, so such elements become zeros
   // here; `bad` learns of each column's first one (at `from` + row), and *spoilt that there is any.
   template <int NP, bool GUARD = false>
   __device__ __forceinline__ void put(__bf16* lds, int pitch, int part, int rows, int cols, int from = 0, int* bad = nullptr,
-                                      int* spoilt = nullptr) const {
+                                      int* spoilt = nullptr) {
+    const int row0 = threadIdx.x / PER, c = threadIdx.x % PER * V;
+    constexpr int STEP = 256 / PER;
+    if (rows < ROWS || cols < W) {  // (no branch for each lane where all is there)
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = threadIdx.x + 256 * i, row = at / PER, c = at % PER * V;
-      uint4 v = r[i];
-      const int past = c + V - cols;
-      if (past > 0) {
-        unsigned __int128 u = __builtin_bit_cast(unsigned __int128, v);
-        u = past < V ? u >> (past * (int)sizeof(T) * 8) : 0;
-        v = __builtin_bit_cast(uint4, u);
+      for (int i = 0; i < N; ++i) {
+        const int past = c + V - cols;
+        if (past > 0) {
+          unsigned __int128 u = __builtin_bit_cast(unsigned __int128, r[i]);
+          u = past < V ? u >> (past * (int)sizeof(T) * 8) : 0;
+          r[i] = __builtin_bit_cast(uint4, u);
+        }
+        if (row0 + i * STEP >= rows) r[i] = make_uint4(0, 0, 0, 0);
       }
-      if (row >= rows) v = make_uint4(0, 0, 0, 0);
-      T e[V];
-      __builtin_memcpy(e, &v, 16);
-      if constexpr (GUARD) {
-        float z = 0.f;
+    }
+    if constexpr (GUARD) {
+      float z = 0.f;
 #pragma unroll
-        for (int j = 0; j < V; ++j) z = fmaf(to_f32(e[j]), 0.f, z);
-        if (__any(z != 0.f)) {
-#pragma nounroll
+      for (int i = 0; i < N; ++i) z += spoilt_by(r[i]);
+      if (__any(z != 0.f)) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          T e[V];
+          __builtin_memcpy(e, &r[i], 16);
+#pragma unroll
           for (int j = 0; j < V; ++j) {
-            float f = 0.f;
-#pragma unroll
-            for (int q = 0; q < V; ++q) f = q == j ? to_f32(e[q]) : f;
+            const float f = to_f32(e[j]);
             if (f * 0.f != 0.f) {
-              atomicMin(&bad[c + j], from + row);
+              atomicMin(&bad[c + j], from + row0 + i * STEP);
               *spoilt = 1;
-#pragma unroll
-              for (int q = 0; q < V; ++q)
-                if (q == j) e[q] = from_f32<T>(0.f);
+              e[j] = from_f32<T>(0.f);
             }
           }
-          __builtin_memcpy(&v, e, 16);
+          __builtin_memcpy(&r[i], e, 16);
         }
       }
-      __bf16* to = lds + row * pitch + c;
+    }
+    __bf16* const to = lds + row0 * pitch + c;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
       if constexpr (NP == 1) {
-        *reinterpret_cast<uint4*>(to) = v;
+        *reinterpret_cast<uint4*>(to + i * STEP * pitch) = r[i];
       } else {
+        T e[V];
         float f[V];
         typedef __bf16 part_t __attribute__((ext_vector_type(V)));
         part_t parts[NP];
+        __builtin_memcpy(e, &r[i], 16);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[j] = to_f32(e[j]);
         split_parts<NP, V>(f, parts);
 #pragma unroll
-        for (int q = 0; q < NP; ++q) __builtin_memcpy(to + q * part, &parts[q], V * 2);
+        for (int q = 0; q < NP; ++q) __builtin_memcpy(to + i * STEP * pitch + q * part, &parts[q], V * 2);
       }
     }
   }
