@@ -6,7 +6,7 @@
 namespace atk {
 
 constexpr int kLaMaxK = 256;                      // key columns: a state's rows
-constexpr int kLaBlocks = 1 << 22;                // workgroups of 256 in a launch: fewer than 2^32 threads, with two roles too
+constexpr int kLaBlocks = 1 << 21;                // workgroups of 256 in a launch: fewer than 2^32 threads, with two roles too
 
 // One chunked product over the sequences, of which the forward and the gradients are four:
 //   out_i = scale sum over j of D_ij (a_i . b_j) c_j + f_i S^T a_i
@@ -95,7 +95,7 @@ template <typename T> int la_launch_out(const LaArgs& a, int mode, bool dots, hi
 template <typename T> int la_launch_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s);
 
 inline int la_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-// columns of c that a workgroup has: 128 (32 a wave) where the state's rows leave the registers for it
+// 16 columns of c that each wave of a workgroup has, times: two where the state's rows leave the registers for it
 inline int la_wide(int rows, int cols) { return rows <= 128 && cols > 64 ? 2 : 1; }
 
 }  // namespace atk

@@ -3,8 +3,8 @@
 // With G the running sum of the log decays within a chunk, D_ij = exp(G_i - G_j) and S the state before it:
 //   O  = scale (exp(G) (Q S) + lower(Q K^T * D) V)
 //   S' = exp(G_last) S + K^T (exp(G_last - G) V)
-// A workgroup of four waves has one head's segment of a sequence and a tile of V's columns, each wave 16 NT
-// of them.  The state stays in the accumulators from chunk to chunk: as it is, it is the next product's
+// A workgroup of four waves has one head's segment of a sequence and a tile of V's columns, each wave NT times
+// 16 of them.  The state stays in the accumulators from chunk to chunk: as it is, it is the next product's
 // second operand.  Rows of a, b and c are staged in LDS in bf16 parts, the next chunk's loads in flight
 // meanwhile; products over tokens read them transposed (ds_read_tr).
 #pragma once
@@ -152,16 +152,21 @@ __device__ __forceinline__ uint4 la_row(const __bf16* p, int g) {
   const uint2 lo = *reinterpret_cast<const uint2*>(p + 4 * g), hi = *reinterpret_cast<const uint2*>(p + 16 + 4 * g);
   return make_uint4(lo.x, lo.y, hi.x, hi.y);
 }
-// 8 of 32 staged rows (tokens) of column lane & 15, in gdr_at's order: 16 lanes read four rows of 16
-// columns, four columns a lane, and each gets a column of them.
+// 8 of 32 staged rows (tokens) of a column, in gdr_at's order: 16 lanes read four rows of four times four
+// columns, JUMP columns apart, and each gets a column of them.
+template <int JUMP = 4>
 __device__ __forceinline__ uint4 la_col(const __bf16* p, int pitch, int lane) {
   typedef __attribute__((address_space(3))) s16x4 lds_t;
-  const __bf16* at = p + (4 * (lane >> 4) + ((lane >> 2) & 3)) * pitch + 4 * (lane & 3);
+  const __bf16* at = p + (4 * (lane >> 4) + ((lane >> 2) & 3)) * pitch + JUMP * (lane & 3);
   const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(at));
   const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(at + 16 * pitch));
   const uint2 x = __builtin_bit_cast(uint2, lo), y = __builtin_bit_cast(uint2, hi);
   return make_uint4(x.x, x.y, y.x, y.y);
 }
+// The wave's column of c and S that lane index c of tile x has: with two tiles a lane that holds rows 4 g .. of
+// both as results has 8 columns in a row.
+template <int NT>
+__device__ __forceinline__ int la_at(int c, int x) { return NT == 2 ? 8 * (c >> 2) + 4 * x + (c & 3) : c; }
 __device__ __forceinline__ float la_bf(uint32_t pair, int i) { return __uint_as_float(i ? pair & 0xffff0000u : pair << 16); }
 // the 8 values that a fragment's parts stand for
 template <int NP>
@@ -221,51 +226,121 @@ struct LaDecays {
   }
 };
 
-// Where S (or another matrix of its layout) has element (16 t + 4 g + e, 16 x + c) of a tile: f(t, x, e, whether
+// Where S (or another matrix of its layout) has element (16 t + 4 g + e, la_at(c, x)) of a tile: f(t, x, e, whether
 // it is there, its address, or another element's where it is not).  No branch around what f loads.  (A state has
 // fewer than 2^29 elements: host check.)
 template <int RT, int NT, bool SWAP, typename P, typename F>
-__device__ __forceinline__ void la_each(const LaArgs& a, const LaRole& r, int i0, int col, int g, P* p, F f) {
+__device__ __forceinline__ void la_each(const LaArgs& a, const LaRole& r, int i0, int col, int c, int g, P* p, F f) {
   const int si = SWAP ? 1 : a.V, sj = SWAP ? a.V : 1;
-  uint32_t at[NT];
 #pragma unroll
-  for (int x = 0; x < NT; ++x) at[x] = (uint32_t)((col + 16 * x < r.CD ? col + 16 * x : 0) * sj);
-#pragma unroll
-  for (int t = 0; t < RT; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = i0 + 16 * t + 4 * g + e;
-      const uint32_t row = (uint32_t)((i < r.AD ? i : 0) * si);
-#pragma unroll
-      for (int x = 0; x < NT; ++x) f(t, x, e, i < r.AD && col + 16 * x < r.CD, p + (at[x] + row));
-    }
-}
-
-// full: the tile has no rows or columns past the state's
-template <int RT, int NT>
-__device__ __forceinline__ void la_store(const LaArgs& a, const LaRole& r, bool full, int col, int g, float* to, const f32x4 (&S)[RT][NT]) {
-  if (full) {
-    float* __restrict__ at = to + (uint32_t)(4 * g * a.V + col);
+  for (int x = 0; x < NT; ++x) {
+    const int j = col + la_at<NT>(c, x);
+    const uint32_t at = (uint32_t)((j < r.CD ? j : 0) * sj);
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) {
+        const int i = i0 + 16 * t + 4 * g + e;
+        f(t, x, e, i < r.AD && j < r.CD, p + (at + (uint32_t)((i < r.AD ? i : 0) * si)));
+      }
+  }
+}
+// full: the tile has no rows or columns past the state's.  `col`: the wave's first column.
+template <int RT, int NT, bool SWAP>
+__device__ __forceinline__ void la_load(const LaArgs& a, const LaRole& r, bool full, int i0, int col, int c, int g, const float* from,
+                                        f32x4 (&S)[RT][NT]) {
+  if (full && (!SWAP || a.V % 4 == 0)) {
 #pragma unroll
-        for (int x = 0; x < NT; ++x) at[(uint32_t)((16 * t + e) * a.V) + 16 * x] = S[t][x][e];
+    for (int x = 0; x < NT; ++x) {
+      const int j = col + la_at<NT>(c, x);
+      const float* __restrict__ at = from + (SWAP ? (uint32_t)(j * a.V + i0 + 4 * g) : (uint32_t)(4 * g * a.V + j));
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        if constexpr (SWAP) {
+          S[t][x] = *reinterpret_cast<const f32x4*>(at + 16 * t);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) S[t][x][e] = at[(uint32_t)((16 * t + e) * a.V)];
+        }
+      }
+    }
   } else {
-    la_each<RT, NT, false>(a, r, 0, col, g, to, [&](int t, int x, int e, bool in, float* p) { if (in) *p = S[t][x][e]; });
+    la_each<RT, NT, SWAP>(a, r, i0, col, c, g, from, [&](int t, int x, int e, bool in, const float* p) {
+      const float v = *p;
+      S[t][x][e] = in ? v : 0.f;
+    });
+  }
+}
+template <int RT, int NT>
+__device__ __forceinline__ void la_store(const LaArgs& a, const LaRole& r, bool full, int col, int c, int g, float* to,
+                                         const f32x4 (&S)[RT][NT]) {
+  if (full) {
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      float* __restrict__ at = to + (uint32_t)(4 * g * a.V + col + la_at<NT>(c, x));
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) at[(uint32_t)((16 * t + e) * a.V)] = S[t][x][e];
+    }
+  } else {
+    la_each<RT, NT, false>(a, r, 0, col, c, g, to, [&](int t, int x, int e, bool in, float* p) { if (in) *p = S[t][x][e]; });
+  }
+}
+// S after a chunk (in reverse: before it): S all + B^T (C f), 32 staged tokens at a time
+template <int RT, int NT, int HS, int NP>
+__device__ __forceinline__ void la_update(const __bf16* b, int b_pitch, int b_part, const __bf16* c, int c_pitch, int c_part, const float* f,
+                                          float factor, float all, int lane, f32x4 (&S)[RT][NT]) {
+  const int g = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int x = 0; x < NT; ++x) S[t][x] *= all;
+#pragma unroll
+  for (int s = 0; s < HS; ++s) {
+    uint4 cw[NT][3];
+    f32x4 w[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) w[u] = *reinterpret_cast<const f32x4*>(f + 32 * s + 16 * u + 4 * g) * factor;
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      uint4 cf[NP];
+      float v[8];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) cf[p] = la_col<4 * NT>(c + p * c_part + 32 * s * c_pitch + 4 * x, c_pitch, lane);
+      la_values<NP>(cf, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] *= w[e / 4][e & 3];
+      la_split<3>(v, cw[x]);
+    }
+#pragma unroll
+    for (int t = 0; t < RT; t += 4) {
+      uint4 bf[4][NP];
+      f32x4 y[4][NT];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) bf[u][p] = la_col(b + p * b_part + 32 * s * b_pitch + 16 * (t + u), b_pitch, lane);
+#pragma unroll
+        for (int x = 0; x < NT; ++x) y[u][x] = S[t + u][x];
+      }
+      la_mma<4, NT, NP, 3>(bf, cw, y);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int x = 0; x < NT; ++x) S[t + u][x] = y[u][x];
+    }
   }
 }
 
 template <typename T, int DA, int NT, bool DOTS>
 struct LaLds {
-  static constexpr int NP = kParts<T>, CT = kLaC<T, DA>, W = 64 * NT, PA = DA + 8, PC = W + 8, PO = 16 * NT + 4;
+  static constexpr int NP = kParts<T>, CT = kLaC<T, DA>, W = 64 * NT, PA = DA + 8, PC = W + 8;
   static constexpr int PF = CT == 64 ? kTri : 2;
   __bf16 a[NP][CT][PA];
   __bf16 b[NP][CT][PA];
   __bf16 c[NP][CT][PC];
   uint4 p[PF][kLaOut<T, DOTS>][64];
-  float o[4][16][PO];
   LaDecays<CT> d;
   union {
     float dots[DOTS ? 4 : 1][CT];
@@ -274,16 +349,17 @@ struct LaLds {
   int spoilt;
 };
 
-// The outputs of one segment, and its last state.
+// The outputs of one segment, and its last state.  Products that make outputs are taken transposed, so that a
+// lane has 4 NT columns of one token.
 template <typename T, int DA, int NT, int MODE, bool DOTS>
 __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, const LaGrid& gr, char* lds) {
   using Lds = LaLds<T, DA, NT, DOTS>;
   constexpr int NP = Lds::NP, CT = Lds::CT, W = Lds::W, RT = DA / 16, KS = DA / 32, MT = CT / 16, HS = CT / 32;
   constexpr int OP = kLaOut<T, DOTS>, OW = 4 * NT;
+  constexpr bool rev = la_reverse(MODE), swapped = la_swapped(MODE);
   Lds& L = *reinterpret_cast<Lds*>(lds);
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  constexpr bool rev = la_reverse(MODE), swapped = la_swapped(MODE);
   int tile, h, slot;
   if (!la_place(a, gr, &tile, &h, &slot)) return;
   const int hk = h / a.group, c_tiles = (r.CD + W - 1) / W, c_tile = swapped ? tile % c_tiles : tile, a_tile = swapped ? tile / c_tiles : 0;
@@ -293,31 +369,19 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
   if (z < 0 || z >= seq.segs) return;
   const int t0 = z * a.seg, len = seq.len - t0 < a.seg ? seq.len - t0 : a.seg;  // tokens of this segment
   const int chunks = (len + CT - 1) / CT;
-  const int a0 = a_tile * DA, col0 = c_tile * W, col = col0 + wave * 16 * NT + c;
+  const int a0 = a_tile * DA, col0 = c_tile * W, col = col0 + wave * 16 * NT;
   const int acols = r.AD - a0 < DA ? r.AD - a0 : DA, ccols = r.CD - col0 < W ? r.CD - col0 : W;
-  const int ha = swapped ? h : hk, hc = MODE == kLaFwd || MODE == kLaDv ? h : hk;
+  const bool full = acols == DA && ccols == W;
+  const int ha = swapped ? h : hk, hc = swapped ? hk : h;
   const int64_t first = seq.begin + t0;
   const T* __restrict__ pa = static_cast<const T*>(r.a) + seq.batch * r.a_s[0] + first * r.a_s[1] + ha * r.a_s[2] + a0;
   const T* __restrict__ pb = static_cast<const T*>(r.b) + seq.batch * r.b_s[0] + first * r.b_s[1] + ha * r.b_s[2] + a0;
   const T* __restrict__ pc = static_cast<const T*>(r.c) + seq.batch * r.c_s[0] + first * r.c_s[1] + hc * r.c_s[2] + col0;
-  const T* __restrict__ pe = DOTS ? static_cast<const T*>(r.e) + seq.batch * r.e_s[0] + first * r.e_s[1] + hk * r.e_s[2] + col0 : nullptr;
   const int64_t pg = seq.batch * a.g_s[0] + first * a.g_s[1] + h * a.g_s[2];
-
-  f32x4 S[RT][NT];
-  const float* from = (rev ? z == seq.segs - 1 : z == 0) ? r.s_first : r.s_between;
-  bool have = from != nullptr;
-  if (from) {
-    const int64_t at = (int64_t)((rev ? z == seq.segs - 1 : z == 0) ? n : slot + (rev ? 1 : -1)) * a.Hv + h;
-    la_each<RT, NT, swapped>(a, r, a0, col, g, from + at * a.K * a.V, [&](int t, int x, int e, bool in, const float* p) {
-      const float v = *p;
-      S[t][x][e] = in ? v : 0.f;
-    });
-  } else {
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int m = 0; m < NT; ++m) S[t][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
+  // a lane's columns of a result, and of e's rows where they are all there
+  const int oc = wave * 16 * NT + OW * g;
+  const bool whole = col0 + oc + OW <= r.CD;
+  const T* __restrict__ pe = DOTS ? static_cast<const T*>(r.e) + seq.batch * r.e_s[0] + first * r.e_s[1] + hk * r.e_s[2] + (whole ? col0 + oc : 0) : nullptr;
 
   LaTile<T, CT, DA> ta, tb;
   LaTile<T, CT, W> tc;
@@ -330,6 +394,18 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
     tg = gdr_gate_load(a.g, a.g_dtype, pg + (at + (lane < rows ? lane : 0)) * a.g_s[1]);
   };
   if (chunks > 0) load(rev ? chunks - 1 : 0);
+  f32x4 S[RT][NT];
+  const float* from = (rev ? z == seq.segs - 1 : z == 0) ? r.s_first : r.s_between;
+  bool have = from != nullptr;
+  if (have) {
+    const int64_t at = (int64_t)((rev ? z == seq.segs - 1 : z == 0) ? n : slot + (rev ? 1 : -1)) * a.Hv + h;
+    la_load<RT, NT, swapped>(a, r, full, a0, col, c, g, from + at * a.K * a.V, S);
+  } else {
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int x = 0; x < NT; ++x) S[t][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   if constexpr (MODE == kLaFwd) {
     for (int i = tid; i < W; i += 256) L.bad[i] = INT_MAX;
     if (tid == 0) L.spoilt = 0;
@@ -340,169 +416,165 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
     ta.template put<NP>(&L.a[0][0][0], Lds::PA, CT * Lds::PA, rows, acols);
     tb.template put<NP>(&L.b[0][0][0], Lds::PA, CT * Lds::PA, rows, acols);
     tc.template put<NP, MODE == kLaFwd>(&L.c[0][0][0], Lds::PC, CT * Lds::PC, rows, ccols, at, L.bad, &L.spoilt);
-    if (wave == 0) L.d.put(gdr_gate<T>(tg, a.g_dtype), lane, rows);
+    if (wave == 3) L.d.put(gdr_gate<T>(tg, a.g_dtype), lane, rows);
     __syncthreads();
     load(k + 1 < chunks ? (rev ? ch - 1 : ch + 1) : ch);  // (at the end the last one's again)
-    // lower(A B^T * D), or upper in reverse, in the layout of a first operand: as the results of its transpose
-    if (wave < MT) {
-      uint4 af[KS][NP];
+    // scale lower(A B^T * D), or upper in reverse, as the results of its transpose: a lane has 8 of 32 columns
+    // of a row, one fragment.  The fragments within the triangle are shared out to the waves.
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
-#pragma unroll
-        for (int p = 0; p < NP; ++p) af[s][p] = la_row(&L.a[p][16 * wave + c][32 * s], g);
-      const float2 go = L.d.gd[16 * wave + c];
-#pragma unroll
-      for (int s = 0; s < HS; ++s) {
-        if (HS > 1 && (rev ? s < wave >> 1 : s > wave >> 1)) continue;
-        f32x4 y[2][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}, {f32x4{0.f, 0.f, 0.f, 0.f}}};
-#pragma unroll
-        for (int q = 0; q < KS; ++q) {
-          uint4 bf[2][NP], ao[1][NP];
-#pragma unroll
-          for (int p = 0; p < NP; ++p) {
-            ao[0][p] = af[q][p];
-            bf[0][p] = la_row(&L.b[p][32 * s + c][32 * q], g);
-            bf[1][p] = la_row(&L.b[p][32 * s + 16 + c][32 * q], g);
-          }
-          la_mma<2, 1, NP, NP>(bf, ao, y);
-        }
-        float v[8];
-        const int out = 16 * wave + c;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int in = 32 * s + 16 * u + 4 * g + e;
-            const float2 gi = L.d.gd[in];
-            const float decay = gdr_decay(rev ? gi : go, rev ? go : gi);
-            v[4 * u + e] = (rev ? in >= out : in <= out) ? y[u][0][e] * decay * a.scale : 0.f;
-          }
-        uint4 f[OP];
-        la_split<OP>(v, f);
-        const int at_p = HS == 1 ? wave : rev ? tri_upper(wave, s) : tri_lower(wave, s);
-#pragma unroll
-        for (int p = 0; p < OP; ++p) L.p[at_p][p][lane] = f[p];
+    for (int f0 = 0; f0 < Lds::PF; f0 += 4) {
+      const int f = f0 + wave;
+      if (f >= Lds::PF) continue;
+      int m = f, s = 0;  // row tile, half of the columns
+      if constexpr (HS > 1) {
+        m = rev ? (f < 4 ? f >> 1 : f - 2) : f < 2 ? f : 1 + (f >> 1);
+        s = rev ? (f < 4 ? f & 1 : 1) : f < 2 ? 0 : f & 1;
       }
+      f32x4 y[2][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}, {f32x4{0.f, 0.f, 0.f, 0.f}}};
+#pragma unroll
+      for (int q = 0; q < KS; ++q) {
+        uint4 bf[2][NP], af[1][NP];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          af[0][p] = la_row(&L.a[p][16 * m + c][32 * q], g);
+          bf[0][p] = la_row(&L.b[p][32 * s + c][32 * q], g);
+          bf[1][p] = la_row(&L.b[p][32 * s + 16 + c][32 * q], g);
+        }
+        la_mma<2, 1, NP, NP>(bf, af, y);
+      }
+      const int out = 16 * m + c;
+      const float2 go = L.d.gd[out];
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float4 gi[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) gi[e] = *reinterpret_cast<const float4*>(&L.d.gd[32 * s + 16 * u + 4 * g + 2 * e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 i = e & 1 ? make_float2(gi[e / 2].z, gi[e / 2].w) : make_float2(gi[e / 2].x, gi[e / 2].y);
+          float p = y[u][0][e] * gdr_decay(rev ? i : go, rev ? go : i) * a.scale;
+          asm("" : "+v"(p));  // (else a branch for each)
+          const int in = 32 * s + 16 * u + 4 * g + e;
+          v[4 * u + e] = (rev ? in >= out : in <= out) ? p : 0.f;
+        }
+      }
+      uint4 w[OP];
+      la_split<OP>(v, w);
+#pragma unroll
+      for (int p = 0; p < OP; ++p) L.p[f][p][lane] = w[p];
     }
-    __syncthreads();
-    // 32 tokens of this wave's columns of c
-    auto load_c = [&](int s, uint4 (&f)[NT][NP]) {
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int p = 0; p < NP; ++p) f[x][p] = la_col(&L.c[p][32 * s][wave * 16 * NT + 16 * x], Lds::PC, lane);
-    };
     T ev[DOTS ? MT : 1][OW];
-    const int orow = lane >> 2, oc = wave * 16 * NT + (lane & 3) * OW;  // a lane's row of 16 and first column of a result
-    const bool whole = col0 + oc + OW <= r.CD;
     if constexpr (DOTS) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
-        __builtin_memcpy(ev[m], pe + (at + (16 * m + orow < rows ? 16 * m + orow : 0)) * r.e_s[1] + (whole ? oc : -col0), OW * sizeof(T));
+        __builtin_memcpy(ev[m], pe + (at + (16 * m + c < rows ? 16 * m + c : 0)) * r.e_s[1], OW * sizeof(T));
     }
-    f32x4 acc[MT][NT];
-    {
+    __syncthreads();
+    f32x4 acc[NT][MT];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int x = 0; x < NT; ++x) acc[m][x] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (have) {
+      for (int x = 0; x < NT; ++x) acc[x][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (have) {
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          uint4 sf[NT][OP], af[MT][NP];
+      for (int s = 0; s < KS; ++s) {
+        uint4 sf[NT][OP], af[MT][NP];
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int p = 0; p < NP; ++p) af[m][p] = la_row(&L.a[p][16 * m + c][32 * s], g);
+          for (int p = 0; p < NP; ++p) af[m][p] = la_row(&L.a[p][16 * m + c][32 * s], g);
 #pragma unroll
-          for (int x = 0; x < NT; ++x) {
-            float v[8];
+        for (int x = 0; x < NT; ++x) {
+          float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = S[2 * s + e / 4][x][e & 3];
-            la_split<OP>(v, sf[x]);
-          }
-          la_mma<MT, NT, NP, OP>(af, sf, acc);
+          for (int e = 0; e < 8; ++e) v[e] = S[2 * s + e / 4][x][e & 3];
+          la_split<OP>(v, sf[x]);
         }
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const f32x4 f = rev ? *reinterpret_cast<const f32x4*>(&L.d.rest[16 * m + 4 * g])
-                              : *reinterpret_cast<const f32x4*>(&L.d.grown[16 * m + 4 * g]) * a.scale;
-#pragma unroll
-          for (int x = 0; x < NT; ++x) acc[m][x] *= f;
-        }
+        la_mma<NT, MT, OP, NP>(sf, af, acc);
       }
 #pragma unroll
-      for (int s = 0; s < HS; ++s) {
-        uint4 b[NT][NP];
-        load_c(s, b);
+      for (int m = 0; m < MT; ++m) {
+        const float f = rev ? L.d.rest[16 * m + c] : L.d.grown[16 * m + c] * a.scale;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          if (HS > 1 && (rev ? s < m >> 1 : s > m >> 1)) continue;
-          uint4 f[1][OP];
-          const int at_p = HS == 1 ? m : rev ? tri_upper(m, s) : tri_lower(m, s);
-#pragma unroll
-          for (int p = 0; p < OP; ++p) f[0][p] = L.p[at_p][p][lane];
-          f32x4 y[1][NT];
-#pragma unroll
-          for (int x = 0; x < NT; ++x) y[0][x] = acc[m][x];
-          la_mma<1, NT, OP, NP>(f, b, y);
-#pragma unroll
-          for (int x = 0; x < NT; ++x) acc[m][x] = y[0][x];
-        }
+        for (int x = 0; x < NT; ++x) acc[x][m] *= f;
       }
+    }
+#pragma unroll
+    for (int s = 0; s < HS; ++s) {
+      uint4 cf[NT][NP], pf[MT][OP];
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int p = 0; p < NP; ++p) cf[x][p] = la_col<4 * NT>(&L.c[p][32 * s][wave * 16 * NT + 4 * x], Lds::PC, lane);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (HS > 1 && (rev ? s < m >> 1 : s > m >> 1)) continue;
+        const int f = HS == 1 ? m : rev ? tri_upper(m, s) : tri_lower(m, s);
+#pragma unroll
+        for (int p = 0; p < OP; ++p) pf[m][p] = L.p[f][p][lane];
+      }
+#pragma unroll
+      for (int z = 2; z >= 0; --z)
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+          for (int q = 0; q < OP; ++q)
+            if (p + q == z) {
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                if (HS > 1 && (rev ? s < m >> 1 : s > m >> 1)) continue;
+#pragma unroll
+                for (int x = 0; x < NT; ++x) acc[x][m] = mma(cf[x][p], pf[m][q], acc[x][m]);
+              }
+            }
     }
     if constexpr (MODE == kLaFwd) {
       if (L.spoilt) {  // outputs from a column's first c on that is not finite are not either
 #pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          const int bad = L.bad[wave * 16 * NT + 16 * x + c];
+        for (int x = 0; x < NT; ++x)
 #pragma unroll
-          for (int m = 0; m < MT; ++m)
+          for (int e = 0; e < 4; ++e) {
+            const int bad = L.bad[oc + 4 * x + e];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (at + 16 * m + 4 * g + e >= bad) acc[m][x][e] = gdr_nan();
-        }
+            for (int m = 0; m < MT; ++m) acc[x][m][e] = at + 16 * m + c >= bad ? gdr_nan() : acc[x][m][e];
+          }
       }
     }
-    // rows of 16 tokens through LDS: OW columns of one a lane
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      __builtin_amdgcn_wave_barrier();  // (a wave's LDS accesses keep their order)
+      const int row = 16 * m + c;
+      float o[OW];
 #pragma unroll
       for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) L.o[wave][4 * g + e][16 * x + c] = acc[m][x][e];
-      __builtin_amdgcn_wave_barrier();
-      float o[OW];
-#pragma unroll
-      for (int e = 0; e < OW; e += 4) {
-        const f32x4 t = *reinterpret_cast<const f32x4*>(&L.o[wave][orow][(lane & 3) * OW + e]);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) o[e + q] = t[q];
-      }
-      const int row = 16 * m + orow;
+        for (int e = 0; e < 4; ++e) o[4 * x + e] = acc[x][m][e];
       if constexpr (DOTS) {
         float dot = 0.f;
         if (whole) {
 #pragma unroll
           for (int q = 0; q < OW; ++q) dot += o[q] * to_f32(ev[m][q]);
         } else if (row < rows) {
-          const T* __restrict__ e = pe + (at + row) * r.e_s[1] + oc;
+          const T* __restrict__ e = pe + (at + row) * r.e_s[1];
 #pragma unroll
           for (int q = 0; q < OW; ++q)
-            if (col0 + oc + q < r.CD) dot += o[q] * to_f32(e[q]);
+            if (col0 + oc + q < r.CD) dot += o[q] * to_f32(e[col0 + oc + q]);
         }
-        dot += dpp_mov<0xB1>(dot);
-        dot += dpp_mov<0x4E>(dot);
-        if ((lane & 3) == 0) L.dots[wave][row] = dot;
+        dot += __shfl_xor(dot, 16, 64);
+        dot += __shfl_xor(dot, 32, 64);
+        if (g == 0) L.dots[wave][row] = dot;
       }
       if (row < rows) {
         const int64_t tok = seq.batch * a.T + first + at + row;
         if (swapped && r.parts) {
           float* __restrict__ to = r.parts + ((((int64_t)(h % a.group) * r.a_tiles + a_tile) * a.B * a.T + tok) * a.Hk + hk) * r.CD + col0 + oc;
+          if (whole) {
+            __builtin_memcpy(to, o, OW * 4);
+          } else {
 #pragma unroll
-          for (int q = 0; q < OW; ++q)
-            if (whole || col0 + oc + q < r.CD) to[q] = o[q];
+            for (int q = 0; q < OW; ++q)
+              if (col0 + oc + q < r.CD) to[q] = o[q];
+          }
         } else {
           T* __restrict__ to = static_cast<T*>(r.out) + (tok * (swapped ? a.Hk : a.Hv) + hc) * r.CD + col0 + oc;
           T v[OW];
@@ -518,54 +590,9 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
         }
       }
     }
-    // the state after the chunk (in reverse: before it)
-    {
-      const float all = L.d.all;
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int x = 0; x < NT; ++x) S[t][x] *= all;
-#pragma unroll
-      for (int s = 0; s < HS; ++s) {
-        uint4 cw[NT][3];
-        float f[8];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const f32x4 t = rev ? *reinterpret_cast<const f32x4*>(&L.d.grown[32 * s + 16 * u + 4 * g]) * a.scale
-                              : *reinterpret_cast<const f32x4*>(&L.d.rest[32 * s + 16 * u + 4 * g]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) f[4 * u + e] = t[e];
-        }
-        uint4 cf[NT][NP];
-        load_c(s, cf);
-#pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          float v[8];
-          la_values<NP>(cf[x], v);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] *= f[e];
-          la_split<3>(v, cw[x]);
-        }
-#pragma unroll
-        for (int t = 0; t < RT; t += 4) {
-          uint4 bf[4][NP];
-          f32x4 y[4][NT];
-#pragma unroll
-          for (int u = 0; u < 4; ++u) {
-#pragma unroll
-            for (int p = 0; p < NP; ++p) bf[u][p] = la_col(&L.b[p][32 * s][16 * (t + u)], Lds::PA, lane);
-#pragma unroll
-            for (int x = 0; x < NT; ++x) y[u][x] = S[t + u][x];
-          }
-          la_mma<4, NT, NP, 3>(bf, cw, y);
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int x = 0; x < NT; ++x) S[t + u][x] = y[u][x];
-        }
-      }
-      have = true;
-    }
+    la_update<RT, NT, HS, NP>(&L.b[0][0][0], Lds::PA, CT * Lds::PA, &L.c[0][0][wave * 16 * NT], Lds::PC, CT * Lds::PC,
+                              rev ? L.d.grown : L.d.rest, rev ? a.scale : 1.f, L.d.all, lane, S);
+    have = true;
     __syncthreads();  // the chunk's LDS is free
     if constexpr (DOTS) {
       if (tid < rows)
@@ -577,32 +604,37 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
     if constexpr (MODE == kLaFwd) {
       if (L.spoilt) {
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
-          if (L.bad[wave * 16 * NT + 16 * x + c] != INT_MAX)
+        for (int x = 0; x < NT; ++x) {
+          const bool bad = L.bad[wave * 16 * NT + la_at<NT>(c, x)] != INT_MAX;
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
+          for (int t = 0; t < RT; ++t)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) S[t][x][e] = gdr_nan();
+            for (int e = 0; e < 4; ++e) S[t][x][e] = bad ? gdr_nan() : S[t][x][e];
+        }
       }
     }
-    la_store<RT, NT>(a, r, acols == DA && ccols == W, col, g, r.s_last + ((int64_t)n * a.Hv + h) * a.K * a.V, S);
+    la_store<RT, NT>(a, r, full, col, c, g, r.s_last + ((int64_t)n * a.Hv + h) * a.K * a.V, S);
   }
   if constexpr (DOTS) {
     if (MODE == kLaDq) {  // the state at the segment's end, and the gradient of it from what follows
       float x = 0.f;
       const float* d = z == seq.segs - 1 ? r.x_last : r.x_between;
       if (d) {
-        d += ((int64_t)(z == seq.segs - 1 ? n : slot + 1) * a.Hv + h) * a.K * a.V;
-        la_each<RT, NT, swapped>(a, r, a0, col, g, d, [&](int t, int m, int e, bool in, const float* p) {
-          const float v = *p;
-          x += in ? S[t][m][e] * v : 0.f;
-        });
+        f32x4 D[RT][NT];
+        la_load<RT, NT, true>(a, r, full, a0, col, c, g, d + ((int64_t)(z == seq.segs - 1 ? n : slot + 1) * a.Hv + h) * a.K * a.V, D);
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+          for (int y = 0; y < NT; ++y)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x += S[t][y][e] * D[t][y][e];
       }
       x = wave_sum(x);
       __syncthreads();
-      if (lane == 0) L.o[0][0][wave] = x;
+      if (lane == 0) L.dots[wave][0] = x;
       __syncthreads();
-      if (tid == 0) r.x_out[((int64_t)tile * a.slots + slot) * a.Hv + h] = (L.o[0][0][0] + L.o[0][0][1]) + (L.o[0][0][2] + L.o[0][0][3]);
+      if (tid == 0)
+        r.x_out[((int64_t)tile * a.slots + slot) * a.Hv + h] = (L.dots[0][0] + L.dots[1][0]) + (L.dots[2][0] + L.dots[3][0]);
     }
   }
   // tokens of a packed row before its first sequence and after its last have zeros
@@ -663,7 +695,7 @@ __device__ __forceinline__ void la_state(const LaArgs& a, const LaRole& r, const
   const int z = slot - seq.slot;
   if (z < 0 || z >= seq.segs || z == (rev ? 0 : seq.segs - 1)) return;
   const int t0 = z * a.seg, len = seq.len - t0 < a.seg ? seq.len - t0 : a.seg, chunks = (len + CT - 1) / CT;
-  const int col0 = tile * W, col = col0 + wave * 16 * NT + c;
+  const int col0 = tile * W, col = col0 + wave * 16 * NT;
   const int acols = r.AD, ccols = r.CD - col0 < W ? r.CD - col0 : W;
   const int64_t first = seq.begin + t0;
   const T* __restrict__ pb = static_cast<const T*>(r.b) + seq.batch * r.b_s[0] + first * r.b_s[1] + hk * r.b_s[2];
@@ -689,60 +721,17 @@ __device__ __forceinline__ void la_state(const LaArgs& a, const LaRole& r, const
     const int ch = rev ? chunks - 1 - k : k, at = ch * CT, rows = len - at < CT ? len - at : CT;
     tb.template put<NP>(&L.b[0][0][0], Lds::PA, CT * Lds::PA, rows, acols);
     tc.template put<NP>(&L.c[0][0][0], Lds::PC, CT * Lds::PC, rows, ccols);
-    if (wave == 0) L.d.put(gdr_gate<T>(tg, a.g_dtype), lane, rows);
+    if (wave == 3) L.d.put(gdr_gate<T>(tg, a.g_dtype), lane, rows);
     __syncthreads();
     load(k + 1 < chunks ? (rev ? ch - 1 : ch + 1) : ch);
-    const float all = L.d.all;
     const float2 last = L.d.gd[CT - 1];
     total.x += last.x;
     total.y += last.y;
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int x = 0; x < NT; ++x) S[t][x] *= all;
-#pragma unroll
-    for (int s = 0; s < HS; ++s) {
-      uint4 cw[NT][3];
-      float f[8];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const f32x4 t = rev ? *reinterpret_cast<const f32x4*>(&L.d.grown[32 * s + 16 * u + 4 * g]) * a.scale
-                            : *reinterpret_cast<const f32x4*>(&L.d.rest[32 * s + 16 * u + 4 * g]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[4 * u + e] = t[e];
-      }
-#pragma unroll
-      for (int x = 0; x < NT; ++x) {
-        uint4 cf[NP];
-        float v[8];
-#pragma unroll
-        for (int p = 0; p < NP; ++p) cf[p] = la_col(&L.c[p][32 * s][wave * 16 * NT + 16 * x], Lds::PC, lane);
-        la_values<NP>(cf, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] *= f[e];
-        la_split<3>(v, cw[x]);
-      }
-#pragma unroll
-      for (int t = 0; t < RT; t += 4) {
-        uint4 bf[4][NP];
-        f32x4 y[4][NT];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-#pragma unroll
-          for (int p = 0; p < NP; ++p) bf[u][p] = la_col(&L.b[p][32 * s][16 * (t + u)], Lds::PA, lane);
-#pragma unroll
-          for (int x = 0; x < NT; ++x) y[u][x] = S[t + u][x];
-        }
-        la_mma<4, NT, NP, 3>(bf, cw, y);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-          for (int x = 0; x < NT; ++x) S[t + u][x] = y[u][x];
-      }
-    }
+    la_update<RT, NT, HS, NP>(&L.b[0][0][0], Lds::PA, CT * Lds::PA, &L.c[0][0][wave * 16 * NT], Lds::PC, CT * Lds::PC,
+                              rev ? L.d.grown : L.d.rest, rev ? a.scale : 1.f, L.d.all, lane, S);
     __syncthreads();
   }
-  la_store<RT, NT>(a, r, acols == DA && ccols == W, col, g, to + ((int64_t)slot * a.Hv + h) * a.K * a.V, S);
+  la_store<RT, NT>(a, r, acols == DA && ccols == W, col, c, g, to + ((int64_t)slot * a.Hv + h) * a.K * a.V, S);
   if (tile == 0 && tid == 0) decays[(int64_t)slot * a.Hv + h] = gdr_decay(total, make_float2(0.f, 0.f));
 }
 // Roles 0 and, where there is a second row of workgroups, 1 in reverse.
@@ -769,11 +758,12 @@ int la_launches(const LaArgs& a, int64_t tiles, const char* what, F launch) {
 template <typename T, int DA, int NT>
 int la_run_out(const LaArgs& a, int mode, bool dots, hipStream_t s) {
   const LaRole& r = a.role[0];
+  const dim3 b(256);
   return la_launches(a, (int64_t)((r.CD + 64 * NT - 1) / (64 * NT)) * r.a_tiles, "la_out_kernel", [&](unsigned n, LaGrid g) {
-    if (mode == kLaFwd) hipLaunchKernelGGL((la_out_kernel<T, DA, NT, kLaFwd>), dim3(n), dim3(256), 0, s, a, g);
-    else if (mode == kLaDv) hipLaunchKernelGGL((la_out_kernel<T, DA, NT, kLaDv>), dim3(n), dim3(256), 0, s, a, g);
-    else if (dots) hipLaunchKernelGGL((la_dqk_kernel<T, DA, NT, true>), dim3(n, 2), dim3(256), 0, s, a, g);
-    else hipLaunchKernelGGL((la_dqk_kernel<T, DA, NT, false>), dim3(n, 2), dim3(256), 0, s, a, g);
+    if (mode == kLaFwd) hipLaunchKernelGGL((la_out_kernel<T, DA, NT, kLaFwd>), dim3(n), b, 0, s, a, g);
+    else if (mode == kLaDv) hipLaunchKernelGGL((la_out_kernel<T, DA, NT, kLaDv>), dim3(n), b, 0, s, a, g);
+    else if (dots) hipLaunchKernelGGL((la_dqk_kernel<T, DA, NT, true>), dim3(n, 2), b, 0, s, a, g);
+    else hipLaunchKernelGGL((la_dqk_kernel<T, DA, NT, false>), dim3(n, 2), b, 0, s, a, g);
   });
 }
 template <typename T, int DA, int NT>
@@ -785,23 +775,19 @@ int la_run_states(const LaArgs& a, int roles, float* const* to, float* decays, h
 
 }  // namespace
 
+#define ATK_LA_SHAPED(FN, ROWS, COLS, ...)                                                  \
+  [&]() {                                                                                   \
+    const int da = la_padded(ROWS);                                                         \
+    if (la_wide(da, COLS) == 2) return da == 128 ? FN<T, 128, 2>(__VA_ARGS__) : FN<T, 64, 2>(__VA_ARGS__); \
+    return da == 256 ? FN<T, 256, 1>(__VA_ARGS__) : da == 128 ? FN<T, 128, 1>(__VA_ARGS__) : FN<T, 64, 1>(__VA_ARGS__); \
+  }()
 template <typename T>
 int la_launch_out(const LaArgs& a, int mode, bool dots, hipStream_t s) {
-  const int da = la_padded(a.role[0].AD), nt = la_wide(da, a.role[0].CD);
-  if (da == 256) return la_run_out<T, 256, 1>(a, mode, dots, s);
-  if (da == 128 && nt == 2) return la_run_out<T, 128, 2>(a, mode, dots, s);
-  if (da == 128) return la_run_out<T, 128, 1>(a, mode, dots, s);
-  if (nt == 2) return la_run_out<T, 64, 2>(a, mode, dots, s);
-  return la_run_out<T, 64, 1>(a, mode, dots, s);
+  return ATK_LA_SHAPED(la_run_out, a.role[0].AD, a.role[0].CD, a, mode, dots, s);
 }
 template <typename T>
 int la_launch_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s) {
-  const int da = la_padded(a.K), nt = la_wide(da, a.V);
-  if (da == 256) return la_run_states<T, 256, 1>(a, roles, to, decays, s);
-  if (da == 128 && nt == 2) return la_run_states<T, 128, 2>(a, roles, to, decays, s);
-  if (da == 128) return la_run_states<T, 128, 1>(a, roles, to, decays, s);
-  if (nt == 2) return la_run_states<T, 64, 2>(a, roles, to, decays, s);
-  return la_run_states<T, 64, 1>(a, roles, to, decays, s);
+  return ATK_LA_SHAPED(la_run_states, a.K, a.V, a, roles, to, decays, s);
 }
 
 }  // namespace atk
