@@ -2,6 +2,8 @@
 // segments of sequences, and the C entries.
 //
 //   S' = exp(g) S + k v^T;  o = scale S'^T q
+#include <math.h>
+
 #include "linear_attn.h"
 
 namespace atk {
@@ -290,9 +292,9 @@ struct LaPlan {
 // once, for the price of their states.
 int64_t la_segment_tokens(const atk_linear_attn_args* p) {
   const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  const double chunks = ((double)p->T / 64 + 1) * (p->cu_seqlens ? 1.0 : (double)p->N);
+  const double chunks = p->cu_seqlens ? (double)p->T / 64 + 1 : (double)((p->T + 63) / 64) * (double)p->N;
   const double tiles = (p->V + 127) / 128;
-  int64_t per = (int64_t)(chunks * p->Hv * tiles / (double)(2 * cus)) + 1;
+  int64_t per = (int64_t)ceil(chunks * p->Hv * tiles / (double)(2 * cus));
   per = per < 4 ? 4 : per > 1024 ? 1024 : per;
   return per * 64;
 }

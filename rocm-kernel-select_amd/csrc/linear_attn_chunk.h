@@ -18,7 +18,7 @@ namespace {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // Tokens of a chunk: 64, or 32 where the parts of 64 rows would not fit LDS twice.
-template <typename T, int DA> inline constexpr int kLaC = kParts<T> * DA <= 256 && sizeof(T) == 2 ? 64 : 32;
+template <typename T, int DA> inline constexpr int kLaC = kParts<T> == 1 ? 64 : 32;
 // parts of what is multiplied towards outputs of T; gradients of decays are fp32, from three
 template <typename T, bool DOTS> inline constexpr int kLaOut = DOTS || sizeof(T) == 4 ? 3 : 2;
 
@@ -349,6 +349,18 @@ struct LaLds {
   int spoilt;
 };
 
+// the first n of N values, one at a time
+template <int N, typename T>
+__device__ __forceinline__ void la_tail(T* to, const float* v, int n) {
+#pragma nounroll
+  for (int i = 0; i < n; ++i) {
+    float x = v[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) x = i == j ? v[j] : x;
+    to[i] = from_f32<T>(x);
+  }
+}
+
 // The outputs of one segment, and its last state.  Products that make outputs are taken transposed, so that a
 // lane has 4 NT columns of one token.
 template <typename T, int DA, int NT, int MODE, bool DOTS>
@@ -418,7 +430,6 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
     tc.template put<NP, MODE == kLaFwd>(&L.c[0][0][0], Lds::PC, CT * Lds::PC, rows, ccols, at, L.bad, &L.spoilt);
     if (wave == 3) L.d.put(gdr_gate<T>(tg, a.g_dtype), lane, rows);
     __syncthreads();
-    load(k + 1 < chunks ? (rev ? ch - 1 : ch + 1) : ch);  // (at the end the last one's again)
     // scale lower(A B^T * D), or upper in reverse, as the results of its transpose: a lane has 8 of 32 columns
     // of a row, one fragment.  The fragments within the triangle are shared out to the waves.
 #pragma unroll
@@ -431,16 +442,21 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
         s = rev ? (f < 4 ? f & 1 : 1) : f < 2 ? 0 : f & 1;
       }
       f32x4 y[2][1] = {{f32x4{0.f, 0.f, 0.f, 0.f}}, {f32x4{0.f, 0.f, 0.f, 0.f}}};
+      constexpr int Q = KS * NP <= 4 ? KS : 1;  // products whose operands are on their way together
 #pragma unroll
-      for (int q = 0; q < KS; ++q) {
-        uint4 bf[2][NP], af[1][NP];
+      for (int q0 = 0; q0 < KS; q0 += Q) {
+        uint4 bf[Q][2][NP], af[Q][1][NP];
 #pragma unroll
-        for (int p = 0; p < NP; ++p) {
-          af[0][p] = la_row(&L.a[p][16 * m + c][32 * q], g);
-          bf[0][p] = la_row(&L.b[p][32 * s + c][32 * q], g);
-          bf[1][p] = la_row(&L.b[p][32 * s + 16 + c][32 * q], g);
-        }
-        la_mma<2, 1, NP, NP>(bf, af, y);
+        for (int q = 0; q < Q; ++q)
+#pragma unroll
+          for (int p = 0; p < NP; ++p) {
+            af[q][0][p] = la_row(&L.a[p][16 * m + c][32 * (q0 + q)], g);
+            bf[q][0][p] = la_row(&L.b[p][32 * s + c][32 * (q0 + q)], g);
+            bf[q][1][p] = la_row(&L.b[p][32 * s + 16 + c][32 * (q0 + q)], g);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) la_mma<2, 1, NP, NP>(bf[q], af[q], y);
       }
       const int out = 16 * m + c;
       const float2 go = L.d.gd[out];
@@ -463,12 +479,6 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
       la_split<OP>(v, w);
 #pragma unroll
       for (int p = 0; p < OP; ++p) L.p[f][p][lane] = w[p];
-    }
-    T ev[DOTS ? MT : 1][OW];
-    if constexpr (DOTS) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        __builtin_memcpy(ev[m], pe + (at + (16 * m + c < rows ? 16 * m + c : 0)) * r.e_s[1], OW * sizeof(T));
     }
     __syncthreads();
     f32x4 acc[NT][MT];
@@ -500,6 +510,12 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
         for (int x = 0; x < NT; ++x) acc[x][m] *= f;
       }
     }
+    T ev[DOTS ? MT : 1][OW];
+    if constexpr (DOTS) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        __builtin_memcpy(ev[m], pe + (at + (16 * m + c < rows ? 16 * m + c : 0)) * r.e_s[1], OW * sizeof(T));
+    }
 #pragma unroll
     for (int s = 0; s < HS; ++s) {
       uint4 cf[NT][NP], pf[MT][OP];
@@ -514,6 +530,7 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
 #pragma unroll
         for (int p = 0; p < OP; ++p) pf[m][p] = L.p[f][p][lane];
       }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int z = 2; z >= 0; --z)
 #pragma unroll
@@ -557,8 +574,10 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
         } else if (row < rows) {
           const T* __restrict__ e = pe + (at + row) * r.e_s[1];
 #pragma unroll
-          for (int q = 0; q < OW; ++q)
-            if (col0 + oc + q < r.CD) dot += o[q] * to_f32(e[col0 + oc + q]);
+          for (int q = 0; q < OW; ++q) {
+            const int j = col0 + oc + q;
+            dot += j < r.CD ? o[q] * to_f32(e[j < r.CD ? j : 0]) : 0.f;
+          }
         }
         dot += __shfl_xor(dot, 16, 64);
         dot += __shfl_xor(dot, 32, 64);
@@ -568,28 +587,20 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
         const int64_t tok = seq.batch * a.T + first + at + row;
         if (swapped && r.parts) {
           float* __restrict__ to = r.parts + ((((int64_t)(h % a.group) * r.a_tiles + a_tile) * a.B * a.T + tok) * a.Hk + hk) * r.CD + col0 + oc;
-          if (whole) {
-            __builtin_memcpy(to, o, OW * 4);
-          } else {
-#pragma unroll
-            for (int q = 0; q < OW; ++q)
-              if (col0 + oc + q < r.CD) to[q] = o[q];
-          }
+          if (whole) __builtin_memcpy(to, o, OW * 4);
+          else la_tail<OW>(to, o, r.CD - col0 - oc);
         } else {
           T* __restrict__ to = static_cast<T*>(r.out) + (tok * (swapped ? a.Hk : a.Hv) + hc) * r.CD + col0 + oc;
           T v[OW];
 #pragma unroll
           for (int q = 0; q < OW; ++q) v[q] = from_f32<T>(o[q]);
-          if (whole) {
-            __builtin_memcpy(to, v, OW * sizeof(T));
-          } else {
-#pragma unroll
-            for (int q = 0; q < OW; ++q)
-              if (col0 + oc + q < r.CD) to[q] = v[q];
-          }
+          if (whole) __builtin_memcpy(to, v, OW * sizeof(T));
+          else la_tail<OW>(to, o, r.CD - col0 - oc);
         }
       }
     }
+    // here the outputs' registers are free (at the end the last chunk's again)
+    load(k + 1 < chunks ? (rev ? ch - 1 : ch + 1) : ch);
     la_update<RT, NT, HS, NP>(&L.b[0][0][0], Lds::PA, CT * Lds::PA, &L.c[0][0][wave * 16 * NT], Lds::PC, CT * Lds::PC,
                               rev ? L.d.grown : L.d.rest, rev ? a.scale : 1.f, L.d.all, lane, S);
     have = true;
@@ -670,20 +681,22 @@ __global__ __launch_bounds__(256, (kLaWaves<LaLds<T, DA, NT, DOTS>>)) void la_dq
   else la_segment<T, DA, NT, kLaDk, DOTS>(a, a.role[1], gr, lds);
 }
 
-template <typename T, int DA, int NT>
+template <typename T, int DA>
 struct LaStateLds {
-  static constexpr int NP = kParts<T>, CT = kLaC<T, DA>, W = 64 * NT, PA = DA + 8, PC = W + 8;
+  static constexpr int NP = kParts<T>, CT = kLaC<T, DA>, W = 64, PA = DA + 8, PC = W + 8;
   __bf16 b[NP][CT][PA];
   __bf16 c[NP][CT][PC];
   LaDecays<CT> d;
 };
 
+// (64 columns a workgroup, also where there are more: it is bound by loads on their way, and twice as many
+// workgroups have more of them; 8192 tokens, 32 heads of 128 x 128: 139 us a call against 145.)
 // What a segment adds to the state, and its decay: b and c alone.  The last segment's (in reverse the
 // first's) nobody asks for.
-template <typename T, int DA, int NT, bool rev>
+template <typename T, int DA, bool rev>
 __device__ __forceinline__ void la_state(const LaArgs& a, const LaRole& r, const LaGrid& gr, char* lds, float* to, float* decays) {
-  using Lds = LaStateLds<T, DA, NT>;
-  constexpr int NP = Lds::NP, CT = Lds::CT, W = Lds::W, RT = DA / 16, HS = CT / 32;
+  using Lds = LaStateLds<T, DA>;
+  constexpr int NP = Lds::NP, CT = Lds::CT, W = Lds::W, RT = DA / 16, NT = 1, HS = CT / 32;
   Lds& L = *reinterpret_cast<Lds*>(lds);
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -735,11 +748,11 @@ __device__ __forceinline__ void la_state(const LaArgs& a, const LaRole& r, const
   if (tile == 0 && tid == 0) decays[(int64_t)slot * a.Hv + h] = gdr_decay(total, make_float2(0.f, 0.f));
 }
 // Roles 0 and, where there is a second row of workgroups, 1 in reverse.
-template <typename T, int DA, int NT>
+template <typename T, int DA>
 __global__ __launch_bounds__(256, 2) void la_state_kernel(LaArgs a, LaGrid gr, float* to0, float* to1, float* decays) {
-  __shared__ __align__(16) char lds[sizeof(LaStateLds<T, DA, NT>)];
-  if (blockIdx.y == 0) la_state<T, DA, NT, false>(a, a.role[0], gr, lds, to0, decays);
-  else la_state<T, DA, NT, true>(a, a.role[1], gr, lds, to1, decays + (int64_t)a.slots * a.Hv);
+  __shared__ __align__(16) char lds[sizeof(LaStateLds<T, DA>)];
+  if (blockIdx.y == 0) la_state<T, DA, false>(a, a.role[0], gr, lds, to0, decays);
+  else la_state<T, DA, true>(a, a.role[1], gr, lds, to1, decays + (int64_t)a.slots * a.Hv);
 }
 
 // launch(grid, its place) for workgroups of all tiles, heads and segments, in as many launches as it takes
@@ -766,28 +779,27 @@ int la_run_out(const LaArgs& a, int mode, bool dots, hipStream_t s) {
     else hipLaunchKernelGGL((la_dqk_kernel<T, DA, NT, false>), dim3(n, 2), b, 0, s, a, g);
   });
 }
-template <typename T, int DA, int NT>
+template <typename T, int DA>
 int la_run_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s) {
-  return la_launches(a, (a.V + 64 * NT - 1) / (64 * NT), "la_state_kernel", [&](unsigned n, LaGrid g) {
-    hipLaunchKernelGGL((la_state_kernel<T, DA, NT>), dim3(n, (unsigned)roles), dim3(256), 0, s, a, g, to[0], roles > 1 ? to[1] : nullptr, decays);
+  return la_launches(a, (a.V + 63) / 64, "la_state_kernel", [&](unsigned n, LaGrid g) {
+    hipLaunchKernelGGL((la_state_kernel<T, DA>), dim3(n, (unsigned)roles), dim3(256), 0, s, a, g, to[0], roles > 1 ? to[1] : nullptr, decays);
   });
 }
 
 }  // namespace
 
-#define ATK_LA_SHAPED(FN, ROWS, COLS, ...)                                                  \
-  [&]() {                                                                                   \
-    const int da = la_padded(ROWS);                                                         \
-    if (la_wide(da, COLS) == 2) return da == 128 ? FN<T, 128, 2>(__VA_ARGS__) : FN<T, 64, 2>(__VA_ARGS__); \
-    return da == 256 ? FN<T, 256, 1>(__VA_ARGS__) : da == 128 ? FN<T, 128, 1>(__VA_ARGS__) : FN<T, 64, 1>(__VA_ARGS__); \
-  }()
 template <typename T>
 int la_launch_out(const LaArgs& a, int mode, bool dots, hipStream_t s) {
-  return ATK_LA_SHAPED(la_run_out, a.role[0].AD, a.role[0].CD, a, mode, dots, s);
+  const int da = la_padded(a.role[0].AD);
+  if (la_wide(da, a.role[0].CD) == 2) return da == 128 ? la_run_out<T, 128, 2>(a, mode, dots, s) : la_run_out<T, 64, 2>(a, mode, dots, s);
+  if (da == 256) return la_run_out<T, 256, 1>(a, mode, dots, s);
+  return da == 128 ? la_run_out<T, 128, 1>(a, mode, dots, s) : la_run_out<T, 64, 1>(a, mode, dots, s);
 }
 template <typename T>
 int la_launch_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s) {
-  return ATK_LA_SHAPED(la_run_states, a.K, a.V, a, roles, to, decays, s);
+  const int da = la_padded(a.K);
+  if (da == 256) return la_run_states<T, 256>(a, roles, to, decays, s);
+  return da == 128 ? la_run_states<T, 128>(a, roles, to, decays, s) : la_run_states<T, 64>(a, roles, to, decays, s);
 }
 
 }  // namespace atk
