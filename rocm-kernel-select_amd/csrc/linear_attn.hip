@@ -288,15 +288,31 @@ struct LaPlan {
   size_t bytes;
 };
 
-// Tokens of a segment.  A workgroup goes through one chunk after the other; segments of a sequence run at
-// once, for the price of their states.
+// Tokens of a segment.  Segments of a sequence run at once, each going through its chunks one after the other,
+// for the price of their states: the length is the one with the least time by
+//   chunks of a segment x 8 us where each workgroup has a CU, 10.5 where two share one, in rounds of those
+//   + the states, written and read twice, at 3.5 TB/s,
+// or that of one segment a sequence, which has no states between.  Lengths of packed sequences are on the
+// device; there the average counts.  (bf16, 128 x 128, us a call: 2 x 2048 tokens of 16 heads with 128, 192 and 256
+// tokens a segment 62, 66 and 57; 8192 of 32 heads with 512 and 576 145 and 160; fp32, 64 x 64, 3 sequences, 1021
+// tokens of 4 heads with 64 and 256 29 and 48.)
 int64_t la_segment_tokens(const atk_linear_attn_args* p) {
-  const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
-  const double chunks = p->cu_seqlens ? (double)p->T / 64 + 1 : (double)((p->T + 63) / 64) * (double)p->N;
-  const double tiles = (p->V + 127) / 128;
-  int64_t per = (int64_t)ceil(chunks * p->Hv * tiles / (double)(2 * cus));
-  per = per < 4 ? 4 : per > 1024 ? 1024 : per;
-  return per * 64;
+  const double cus = device_cu_count() > 0 ? device_cu_count() : 256, n = (double)(p->N > 0 ? p->N : 1);
+  const double chunks = p->cu_seqlens ? (double)p->T / 64 / n : (double)((p->T + 63) / 64);
+  const double work = (double)p->Hv * ((p->V + 127) / 128) * n, state = (double)p->K * p->V * 16 / 3.5e6;  // us for 4 passes
+  const int64_t all = (p->T + 63) / 64 > 0 ? (p->T + 63) / 64 : 1;
+  int64_t best = all;
+  const auto steps = [&](double units) { return units <= cus ? 8.0 : 10.5 * ceil(units / (2 * cus)); };
+  double least = chunks * steps(work);
+  for (int64_t per = 1; per < all && per <= 4096; per += per < 16 ? 1 : per / 8) {
+    const double segs = ceil(chunks / (double)per), units = segs * work;
+    const double t = steps(units) * (double)per + units * state;
+    if (t < least) {
+      least = t;
+      best = per;
+    }
+  }
+  return best * 64;
 }
 
 // Checks a call and lays out its workspace; *rc says why where it is refused.
