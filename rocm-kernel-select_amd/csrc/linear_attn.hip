@@ -334,7 +334,7 @@ LaPlan la_plan(const atk_linear_attn_args* p, bool backward, LaArgs* a, int* rc)
   const int64_t seg = la_segment_tokens(p);
   const double slots = p->cu_seqlens ? (double)(p->T / seg) + (double)p->N
                                      : (double)(p->T > seg ? (p->T + seg - 1) / seg : 1) * (double)p->N;
-  if ((double)p->K * p->V >= (double)(1 << 29) || slots * p->Hv > 2147483000.0 || slots > 2147483000.0 || (double)p->N * (double)p->T > 1e15)
+  if ((double)p->K * p->V >= (double)(1 << 29) || slots * p->Hv > 2147483000.0 || slots > 2147483000.0 || (p->cu_seqlens ? 1.0 : (double)p->N) * (double)p->T > 1e12)
     return *rc = fail(ATK_UNSUPPORTED, "linear attention: a state of 2^29 elements or more, or too many sequences and heads"), L;
   *a = LaArgs{};
   // the kernels' loads of 64 tokens have offsets of 32 bits

@@ -244,3 +244,394 @@ def test_packed_backward(dev, cu, dk, dv, fixed, dtype):
     dout = torch.randn(1, t, hv, dv, generator=gen).to(dev, dtype)
     state, dstate = (torch.randn(n, hv, dk, dv, generator=gen).to(dev) for _ in range(2))
     check_backward(P, args, 0.3, state, cu, dout, dstate, t / 4 + dk + dv + 100)
+
+
+# ---------------------------------------------------------------------------------------------
+# layouts, values and callers out of the ordinary
+# ---------------------------------------------------------------------------------------------
+@gpu
+def test_strided_and_broadcast_inputs(dev):
+    """The same numbers in another layout run through the same kernel: equal bits."""
+    import amd_tuned_torch as P
+    b, t, hk, hv, dk, dv = 2, 300, 2, 4, 64, 72
+    q, k, v, g = make((b, t), hk, hv, dk, dv, torch.bfloat16, dev, gdtype=torch.bfloat16)
+    want = P.linear_attention(q, k, v, g)
+    fused = torch.cat([q.flatten(2), k.flatten(2), v.flatten(2), v.flatten(2)[..., :3]], -1)  # odd rows
+    q1, k1, v1 = fused.split([hk * dk, hk * dk, hv * dv, 3], -1)[:3]
+    got = P.linear_attention(q1.unflatten(2, (hk, dk)), k1.unflatten(2, (hk, dk)), v1.unflatten(2, (hv, dv)),
+                             g.transpose(1, 2).contiguous().transpose(1, 2))
+    assert torch.equal(got, want)
+    heads_first = lambda x: x.transpose(1, 2).contiguous().transpose(1, 2)  # noqa: E731
+    assert torch.equal(P.linear_attention(*(heads_first(x) for x in (q, k, v, g))), want)
+    columns_first = lambda x: x.transpose(2, 3).contiguous().transpose(2, 3)  # noqa: E731
+    assert torch.equal(P.linear_attention(columns_first(q), k, columns_first(v), g), want)
+    one = k[:, :1].expand(b, t, hk, dk)                                        # a broadcast input, and one decay a head
+    fixed = g[0, 0]
+    assert torch.equal(P.linear_attention(q, one, v, fixed),
+                       P.linear_attention(q, one.contiguous(), v, fixed.expand(b, t, hv).contiguous()))
+    # gradients: heads first, an expanded leaf, an output gradient that is not dense
+    dout = torch.randn(b, hv, t, dv, device=dev).bfloat16().transpose(1, 2)
+    outs = []
+    for f in (lambda x: x, heads_first, columns_first):
+        leaves = [x.detach().clone().requires_grad_() for x in (q, k, v)]
+        outs.append(torch.autograd.grad(P.linear_attention(*(f(x) for x in leaves), g), leaves, dout if f is heads_first else dout.contiguous()))
+    assert all(torch.equal(x, y) for other in outs[1:] for x, y in zip(outs[0], other))
+    leaf = k[:, :1].detach().clone().requires_grad_()
+    full = k[:, :1].expand(b, t, hk, dk).contiguous().requires_grad_()
+    a, = torch.autograd.grad(P.linear_attention(q, leaf.expand(b, t, hk, dk), v, g), leaf, dout)
+    c, = torch.autograd.grad(P.linear_attention(q, full, v, g), full, dout)
+    # the expanded leaf's gradient is torch's sum of t rounded rows
+    assert ((a.double() - c.double().sum(1, keepdim=True)).abs() <= 2.0 ** -7 * c.double().abs().sum(1, keepdim=True)).all()
+
+
+@gpu
+def test_offsets_beyond_32_bits(dev):
+    """Rows of a buffer whose elements lie up to 3.3e9 apart, and slots of a state as far apart."""
+    import amd_tuned_torch as P
+    t, far = 100, 1 << 25
+    q, k, v, g = make((1, t), 1, 1, 64, 64, torch.bfloat16, dev)
+    buffer = torch.empty(t * far, dtype=torch.bfloat16, device=dev)
+    rows = buffer.view(1, t, 1, far)
+    for i, x in enumerate((q, k, v)):
+        rows[..., i * 64:(i + 1) * 64] = x
+    apart = [rows[..., i * 64:(i + 1) * 64] for i in range(3)]
+    assert torch.equal(P.linear_attention(*apart, g), P.linear_attention(q, k, v, g))
+    big = torch.empty(3, 1 << 30, device=dev)
+    state = big.as_strided((3, 1, 64, 64), (1 << 30, 4096, 64, 1))
+    state.zero_()
+    idx = torch.tensor([2, 0], dtype=torch.int32, device=dev)
+    args = [x[0, :2] for x in (q, k, v, g)]
+    small = torch.zeros(3, 1, 64, 64, device=dev)
+    assert torch.equal(P.linear_attention_update(*args, state, state_indices=idx),
+                       P.linear_attention_update(*args, small, state_indices=idx))
+    assert torch.equal(state, small)
+
+
+@gpu
+def test_many_tokens(dev):
+    """A packed row of 70000 tokens: sequences of one token, of none and of most of it, against each alone."""
+    import amd_tuned_torch as P
+    t = 70000
+    q, k, v, g = make((1, t), 1, 2, 64, 64, torch.bfloat16, dev)
+    cu = [0, 1, 1, 2, 66, 69000, 69999, t]
+    off = torch.tensor(cu, dtype=torch.int32, device=dev)
+    out, final = P.linear_attention(q, k, v, g, cu_seqlens=off, return_final_state=True)
+    size, size_s, _ = forward64(*sizes(*(x[:, 66:2066] for x in (q, k, v, g))), 0.125, None, None)
+    for i, (a, b) in enumerate(zip(cu, cu[1:])):
+        alone, state = P.linear_attention(*(x[:, a:b].contiguous() for x in (q, k, v, g)), return_final_state=True)
+        # another length of segments: sums in another order, each of 2^-24 of at most `size`, then one rounding
+        lim = 2 * 2.0 ** -8 * alone.float().abs() + (2.0 ** -15 + t / 4 * 2.0 ** -24) * size.max()
+        assert ((out[:, a:b].float() - alone.float()).abs() <= lim).all(), i
+        assert ((final[i] - state[0]).abs() <= t / 4 * 2.0 ** -24 * size_s.max()).all(), i
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_decays_at_their_ends(dev, dtype):
+    """No decay, all forgotten, hardly anything left, the type's least value, growth, decays that cancel in sums."""
+    import amd_tuned_torch as P
+    q, k, v, g = make((1, 150), 1, 7, 64, 64, dtype, dev)
+    g[:, :, 0] = 0
+    g[:, ::7, 1] = float("-inf")
+    g[:, :, 2] = -40
+    g[:, :, 3] = torch.finfo(torch.float32).min
+    g[:, :, 4] = 0.05
+    g[:, 20, 5] = -119
+    g[:, 21:, 5] = -2.0 ** -12
+    g[:, 100, 6] = -1e6
+    state = torch.randn(1, 7, 64, 64, device=dev)
+    want, want_s, _ = forward64(q, k, v, g, 0.125, state, None)
+    size, size_s, _ = forward64(*sizes(q, k, v, g), 0.125, state.abs(), None)
+    got, got_s = P.linear_attention(q, k, v, g, initial_state=state, return_final_state=True)
+    for h in range(7):
+        close(got[:, :, h], want[:, :, h], size[:, :, h], 300, h)
+        close(got_s[:, h], want_s[:, h], size_s[:, h], 300, h)
+    gen = torch.Generator().manual_seed(0)
+    dout = torch.randn(1, 150, 7, 64, generator=gen).to(dev, dtype)
+    dstate = torch.randn(1, 7, 64, 64, generator=gen).to(dev)
+    _, grads = check_backward(P, (q, k, v, g), 0.125, state, None, dout, dstate, 300)
+    assert grads[3][:, ::7, 1].eq(0).all() and grads[3][:, :, 3].eq(0).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_values_that_are_not_finite(dev, bad, dtype):
+    """They spoil no token before their own, no other head and, in v, no other column."""
+    import amd_tuned_torch as P
+    t, at = 400, 301                               # in the second segment or later, and inside a chunk
+    clean = make((1, t), 1, 2, 64, 72, dtype, dev)
+    want, want_s = P.linear_attention(*clean, return_final_state=True)
+    for i, name in enumerate("qkvg"):
+        args = [x.clone() for x in clean]
+        args[i][(0, at, 0, 5) if i < 2 else (0, at, 1, 5) if i == 2 else (0, at, 1)] = bad
+        out, final = P.linear_attention(*args, return_final_state=True)
+        assert torch.equal(out[:, :at], want[:, :at]), name
+        if i == 0:                                 # a query's own token
+            assert not out[0, at].isfinite().any() and torch.equal(out[:, at + 1:], want[:, at + 1:]) and torch.equal(final, want_s)
+        elif i == 1:
+            assert not out[0, at:].isfinite().any() and not final[0, :, 5].isfinite().any()
+        elif i == 2:
+            assert not out[0, at:, 1, 5].isfinite().any() and not final[0, 1, :, 5].isfinite().any()
+            rest = [c for c in range(72) if c != 5]
+            assert torch.equal(out[..., rest], want[..., rest]) and torch.equal(out[:, :, 0], want[:, :, 0])
+            assert torch.equal(final[..., rest], want_s[..., rest])
+        elif bad != -float("inf"):
+            assert not out[0, at:, 1].isfinite().any() and torch.equal(out[:, :, 0], want[:, :, 0])
+        else:
+            assert out.isfinite().all()            # -inf forgets
+    # a batch element, or a packed sequence, of its own
+    args = [x.expand(2, *x.shape[1:]).clone() for x in clean]
+    args[2][0, 3, 0, 0] = bad
+    assert torch.equal(P.linear_attention(*args)[1:], want)
+    off = torch.tensor([0, 200, t], dtype=torch.int32, device=dev)
+    args = [x.clone() for x in clean]
+    args[1][0, 199, 0, 0] = bad
+    assert torch.equal(P.linear_attention(*args, cu_seqlens=off)[:, 200:], P.linear_attention(*clean, cu_seqlens=off)[:, 200:])
+
+
+@gpu
+def test_offsets_that_no_row_has(dev):
+    """Offsets past the row or before it are clamped to it; nothing else is read or written."""
+    import amd_tuned_torch as P
+    args = make((1, 300), 1, 2, 64, 64, torch.bfloat16, dev)
+    cu = torch.tensor([-50, 30, 1000], dtype=torch.int32, device=dev)
+    good = torch.tensor([0, 30, 300], dtype=torch.int32, device=dev)
+    for a, b in zip(P.linear_attention(*args, return_final_state=True, cu_seqlens=cu),
+                    P.linear_attention(*args, return_final_state=True, cu_seqlens=good)):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_continuing_and_decoding_agree_with_one_pass(dev):
+    """A prompt in two parts and then token by token gives what one pass gives."""
+    import amd_tuned_torch as P
+    args = make((2, 150), 2, 4, 128, 64, torch.float32, dev)
+    want, want_s = P.linear_attention(*args, return_final_state=True)
+    size, size_s, _ = forward64(*sizes(*args), 128 ** -0.5, None, None)
+    out, S = P.linear_attention(*(x[:, :80] for x in args), return_final_state=True)
+    outs = [out]
+    out, S = P.linear_attention(*(x[:, 80:145] for x in args), initial_state=S, return_final_state=True)
+    outs.append(out)
+    for t in range(145, 150):
+        outs.append(P.linear_attention_update(*(x[:, t] for x in args), S)[:, None])
+    close(torch.cat(outs, 1), want.double(), size, 600)
+    close(S, want_s.double(), size_s, 600)
+
+
+@gpu
+def test_empty_calls(dev):
+    import amd_tuned_torch as P
+    args = make((2, 70), 1, 2, 64, 64, torch.bfloat16, dev)
+    assert P.linear_attention(*(x[:0] for x in args)).shape == (0, 70, 2, 64)
+    state = torch.randn(2, 2, 64, 64, device=dev)
+    none = [x[:, :0].clone().requires_grad_() for x in args]
+    s = state.clone().requires_grad_()
+    out, S = P.linear_attention(*none, initial_state=s, return_final_state=True)
+    assert out.shape == (2, 0, 2, 64) and torch.equal(S, state)
+    grads = torch.autograd.grad(S, [*none, s], torch.ones_like(S), allow_unused=True)
+    assert grads[4].eq(1).all() and all(x.shape == y.shape for x, y in zip(grads, none))
+    fixed = torch.full((2,), -0.1, device=dev, requires_grad=True)
+    _, S = P.linear_attention(*(x[:, :0] for x in args[:3]), fixed, initial_state=state, return_final_state=True)
+    assert torch.autograd.grad(S.sum(), fixed)[0].eq(0).all()
+    cu = torch.tensor([7], dtype=torch.int32, device=dev)
+    out, S = P.linear_attention(*(x[:1] for x in args), cu_seqlens=cu, return_final_state=True)
+    assert out.eq(0).all() and S.shape == (0, 2, 64, 64)
+    cu = torch.tensor([5, 5, 5], dtype=torch.int32, device=dev)
+    leaves = [x[:1].clone().requires_grad_() for x in args]
+    out, S = P.linear_attention(*leaves, initial_state=state, cu_seqlens=cu, return_final_state=True)
+    assert out.eq(0).all() and torch.equal(S, state)
+    assert all(x.eq(0).all() for x in torch.autograd.grad(out.sum(), leaves))
+
+
+@gpu
+def test_gradients_of_some(dev):
+    """Only some inputs, only one result, and without the decays' gradient: what all together give."""
+    import amd_tuned_torch as P
+    args = make((1, 90), 2, 4, 64, 48, torch.bfloat16, dev)
+    gen = torch.Generator().manual_seed(3)
+    dout = torch.randn(1, 90, 4, 48, generator=gen).to(dev, torch.bfloat16)
+    state, dstate = (torch.randn(1, 4, 64, 48, generator=gen).to(dev) for _ in range(2))
+    _, full = run_backward(P, args, 0.2, state, None, dout, dstate)
+    want = backward64(*args, 0.2, state, None, dout, dstate)
+    size = backward64(*sizes(*args), 0.2, state.abs(), None, dout.abs(), dstate.abs(), size=True)
+    for wanted in ((0,), (1, 2), (3,), (4,), (0, 1, 2)):
+        leaves = [x.detach().clone().requires_grad_(i in wanted) for i, x in enumerate((*args, state))]
+        out, S = P.linear_attention(*leaves[:4], 0.2, initial_state=leaves[4], return_final_state=True)
+        got = torch.autograd.grad((out, S), [leaves[i] for i in wanted], (dout, dstate))
+        for i, x in zip(wanted, got):
+            close(x, want[i], size[i], 2 * 300, i)
+            if i > 1:
+                assert torch.equal(x, full[i])
+    leaves = [x.detach().clone().requires_grad_() for x in args]
+    _, S = P.linear_attention(*leaves, 0.2, return_final_state=True)
+    got = torch.autograd.grad(S, leaves, dstate, allow_unused=True)
+    zero = torch.zeros_like(dout)
+    want = backward64(*args, 0.2, None, None, zero, dstate)
+    size = backward64(*sizes(*args), 0.2, None, None, zero, dstate.abs(), size=True)
+    for x, a, b in zip(got, want, size):
+        close(x, a, b, 600)
+
+
+@gpu
+def test_gradients_against_differences(dev):
+    """The output is linear in each of q, k, v and the state, so L(x + d) - L(x - d) is twice the slope along d but
+    for rounding, of 300 2^-24 of the magnitudes; along g a step of e leaves e^2 / 6 of the third derivative,
+    which the magnitudes times (sum of |d| over a sequence, 4 at most here)^3 bound."""
+    import amd_tuned_torch as P
+    args = make((1, 100), 1, 2, 32, 40, torch.float32, dev, seed=4)
+    gen = torch.Generator().manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=gen).to(dev)  # noqa: E731
+    state, dout, dstate = r(1, 2, 32, 40), r(1, 100, 2, 40), r(1, 2, 32, 40)
+
+    def loss(a):
+        out, S = P.linear_attention(*a[:4], 0.3, initial_state=a[4], return_final_state=True)
+        return (out.double() * dout.double()).sum() + (S.double() * dstate.double()).sum()
+
+    leaves = [*args, state]
+    _, grads = run_backward(P, args, 0.3, state, None, dout, dstate)
+    for i in range(5):
+        d = r(*leaves[i].shape)
+        e = 1.0
+        if i == 3:
+            d, e = d / d.abs().sum(1, keepdim=True) * 4, 2.0 ** -6
+        ends = [loss([x + s * e * d if j == i else x for j, x in enumerate(leaves)]) for s in (1, -1)]
+        a = [x.abs() + (e * d.abs() if j == i and i != 3 else 0) if j != 3 else x for j, x in enumerate(leaves)]
+        if i == 3:
+            a[3] = a[3] + e * d.abs()
+        o, s, _ = forward64(*a[:4], 0.3, a[4], None)
+        size = (o * dout.double().abs()).sum() + (s * dstate.double().abs()).sum()
+        slope, want = (ends[0] - ends[1]) / (2 * e), (grads[i].double() * d.double()).sum()
+        lim = (2 * 300 * 2.0 ** -24 / e + (e * e / 6 * 64 if i == 3 else 0)) * size
+        assert (slope - want).abs() <= lim, (i, slope, want, lim)
+
+
+@gpu
+def test_streams_and_graphs(dev):
+    """On another stream, and captured with its backward: replayed with inputs and gradients changed between."""
+    import amd_tuned_torch as P
+    args = [x.requires_grad_() for x in make((2, 300), 1, 2, 64, 64, torch.bfloat16, dev)]
+    dout = torch.randn(2, 300, 2, 64, device=dev).bfloat16()
+    call = lambda: (lambda o: (o.detach(), *torch.autograd.grad(o, args, dout)))(P.linear_attention(*args))  # noqa: E731
+    first = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = call()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for _ in range(3):
+        with torch.no_grad():
+            args[2].normal_()
+            dout.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, call()))
+
+
+@gpu
+def test_two_graphs_side_by_side(dev):
+    """Two captured passes, replayed on two streams at once: each has a workspace of its own."""
+    import amd_tuned_torch as P
+    sets = []
+    for seed in (0, 1):
+        args = [x.requires_grad_() for x in make((1, 2000), 2, 4, 64, 64, torch.bfloat16, dev, seed=seed)]
+        dout = torch.randn(1, 2000, 4, 64, device=dev).bfloat16()
+        want = torch.autograd.grad(P.linear_attention(*args), args, dout)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(P.linear_attention(*args), args, dout)
+        sets.append((graph, got, want, args, dout, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, _, _, _, _, stream in sets:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for s in sets for a, b in zip(s[1], s[2]))
+
+
+@gpu
+def test_update_in_a_graph_and_values(dev):
+    import amd_tuned_torch as P
+    args = make((3,), 2, 4, 128, 128, torch.bfloat16, dev)
+    state = torch.randn(3, 4, 128, 128, device=dev)
+    eager = state.clone()
+    graph = torch.cuda.CUDAGraph()
+    P.linear_attention_update(*args, state.clone())
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = P.linear_attention_update(*args, state)
+    state.copy_(eager)
+    for _ in range(3):
+        graph.replay()
+        want = P.linear_attention_update(*args, eager)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(state, eager)
+    q, k, v, g = make((2,), 1, 2, 64, 64, torch.float32, dev)
+    state = torch.randn(2, 2, 64, 64, device=dev)
+    g[0] = float("-inf")
+    v[1, 0, 3] = float("nan")
+    one = [x[:, None] for x in (q, k, v, g)]
+    want, want_s, _ = forward64(*one, 0.125, state, None)
+    size, size_s, _ = forward64(*sizes(*one), 0.125, state.abs(), None)
+    out = P.linear_attention_update(q, k, v, g, state)
+    close(out[0], want[0, 0], size[0, 0], 72)
+    close(state[0], want_s[0], size_s[0], 8)
+    assert torch.equal(out[1].isnan(), want[1, 0].isnan()) and torch.equal(state[1].isnan(), want_s[1].isnan())
+
+
+@gpu
+def test_second_derivatives_and_transforms(dev):
+    import amd_tuned_torch as P
+    small = [x.requires_grad_() for x in make((1, 9), 1, 2, 8, 8, torch.float32, dev)]
+    twice = []
+    for fn in (P.linear_attention, P.linear_attention_ops.linear_attention_ref):
+        grads = torch.autograd.grad(fn(*small).square().sum(), small, create_graph=True)
+        twice.append(torch.autograd.grad(sum(x.square().sum() for x in grads), small))
+    # the statement's own operations but for the first output, 2^-20 apart
+    assert all((x - y).abs().max() <= 1e-4 * y.abs().max() for x, y in zip(*twice))
+    with torch.no_grad():
+        assert not P.linear_attention(*small).requires_grad
+        plain = [x.detach() for x in small]
+        got, tangent = torch.func.jvp(lambda v: P.linear_attention(plain[0], plain[1], v, plain[3]), (plain[2],), (plain[2],))
+        assert (got - tangent).abs().max() <= 1e-5 * got.abs().max()          # linear in v
+
+
+@gpu
+def test_refusals(dev):
+    import amd_tuned_torch as P
+    q, k, v, g = make((2, 5), 2, 4, 32, 16, torch.bfloat16, dev)
+    bad = [(q[0], k, v, g), (q, k[:, :3], v, g), (q, k.half(), v, g), (q, k, v[:, :3], g), (q, k, v[:, :, :3], g[:, :, :3]),
+           (q, k, v, g.double()), (q, k, v, g.half()), (q, k, v, g[..., :2]), (q, k, v, g[0]), (q.cpu(), k, v, g), (q, k, v, g.cpu()),
+           tuple(x.double() for x in (q, k, v, g))]
+    for a in bad:
+        with pytest.raises(RuntimeError, match="linear_attention"):
+            P.linear_attention(*a)
+    cu = torch.tensor([0, 5], dtype=torch.int32, device=dev)
+    one = [x[:1] for x in (q, k, v, g)]
+    for c, a in ((cu, (q, k, v, g)), (cu.long(), one), (cu.cpu(), one), (cu[:0], one)):
+        with pytest.raises(RuntimeError, match="cu_seqlens"):
+            P.linear_attention(*a, cu_seqlens=c)
+    for s in (torch.zeros(2, 4, 32, 16, device=dev), torch.zeros(1, 4, 32, 16, device=dev).half(), torch.zeros(1, 4, 32, 16)):
+        with pytest.raises(RuntimeError, match="initial_state"):
+            P.linear_attention(*one, initial_state=s)
+    with pytest.raises(RuntimeError, match="256"):
+        P.linear_attention(*make((1, 5), 1, 1, 257, 8, torch.bfloat16, dev))
+    q, k, v, g = make((2,), 2, 4, 32, 16, torch.bfloat16, dev)
+    state = torch.zeros(2, 4, 32, 16, device=dev)
+    idx = torch.zeros(2, dtype=torch.int32, device=dev)
+    bad = [(q[0], k, v, g, state), (q, k[:1], v, g, state), (q, k.half(), v, g, state), (q, k, v[:, :3], g[:, :3], state[:, :3]),
+           (q, k, v, g[:1], state), (q, k, v, g.double(), state), (q, k, v, g, state.bfloat16()), (q, k, v, g, state[:1]),
+           (q, k, v, g, state.transpose(2, 3)), (q.cpu(), k, v, g, state), (q, k, v, g, state.cpu())]
+    for a in bad:
+        with pytest.raises(RuntimeError, match="linear_attention_update"):
+            P.linear_attention_update(*a)
+    for i in (idx.long(), idx[:1], idx.cpu()):
+        with pytest.raises(RuntimeError, match="state_indices"):
+            P.linear_attention_update(q, k, v, g, state, state_indices=i)
+    with pytest.raises(RuntimeError, match="256"):
+        P.linear_attention_update(*make((1,), 1, 1, 257, 8, torch.bfloat16, dev), torch.zeros(1, 1, 257, 8, device=dev))
