@@ -6,7 +6,7 @@
 namespace atk {
 
 constexpr int kLaMaxK = 256;                      // key columns: a state's rows
-constexpr int kLaBlocks = 1 << 21;                // workgroups of 256 in a launch: fewer than 2^32 threads, with two roles too
+constexpr int kLaBlocks = 1 << 21;                // workgroups of 256 in a launch: fewer than 2^32 threads, with three roles too
 
 // One chunked product over the sequences, of which the forward and the gradients are four:
 //   out_i = scale sum over j of D_ij (a_i . b_j) c_j + f_i S^T a_i
@@ -35,7 +35,7 @@ struct LaRole {
 };
 
 struct LaArgs {
-  LaRole role[2];
+  LaRole role[3];
   const void* g; int64_t g_s[3];
   const int* cu;
   int64_t T, B;             // tokens of a sequence (of the packed row with cu); first axis of the tensors
@@ -89,9 +89,10 @@ __device__ __forceinline__ bool la_place(const LaArgs& a, const LaGrid& gr, int*
   return s < (uint32_t)a.slots;
 }
 
-// Launchers, each for one type: the outputs of role 0, or of roles 0 and 1 for kLaDq (dq and dk); what segments
-// add to the states, forward and, with roles 2, in reverse.
-template <typename T> int la_launch_out(const LaArgs& a, int mode, bool dots, hipStream_t s);
+// Launchers, each for one type: the outputs of role 0, or all gradients (dq, dk, dv are roles 0, 1 and 2); what
+// segments add to the states, forward and, with roles 2, in reverse.
+template <typename T> int la_launch_out(const LaArgs& a, hipStream_t s);
+template <typename T> int la_launch_grads(const LaArgs& a, bool dots, hipStream_t s);
 template <typename T> int la_launch_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s);
 
 inline int la_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }

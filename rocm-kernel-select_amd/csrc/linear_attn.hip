@@ -409,7 +409,7 @@ int la_forward(const atk_linear_attn_args* p, LaArgs& a, const LaPlan& L, hipStr
     if (int rc = la_launch_states<T>(a, 1, to, L.decays, s)) return rc;
     if (int rc = la_scan(a, L.s_fwd, nullptr, L.decays, 1, s)) return rc;
   }
-  return la_launch_out<T>(a, kLaFwd, false, s);
+  return la_launch_out<T>(a, s);
 }
 
 template <typename T, typename G>
@@ -456,9 +456,8 @@ int la_backward(const atk_linear_attn_args* p, LaArgs& a, const LaPlan& L, const
   q.parts = L.parts[0]; k.parts = L.parts[1];
   q.dots = L.dots[0]; k.dots = L.dots[1];
   q.x_last = ds1; q.x_between = L.s_rev; q.x_out = L.x;
-  if (int rc = la_launch_out<T>(a, kLaDq, dg != nullptr, s)) return rc;
-  b.role[0] = v;
-  if (int rc = la_launch_out<T>(b, kLaDv, false, s)) return rc;
+  a.role[2] = v;
+  if (int rc = la_launch_grads<T>(a, dg != nullptr, s)) return rc;
   if (L.n_parts > 1 && a.T > 0) {
     LaSumArgs m = {{L.parts[0], L.parts[1]}, {dq, dk}, a.B * a.T * a.Hk * (int64_t)a.K, L.n_parts};
     const bool vec = m.count % 4 == 0;

@@ -674,11 +674,13 @@ __global__ __launch_bounds__(256, (kLaWaves<LaLds<T, DA, NT, false>>)) void la_o
   __shared__ __align__(16) char lds[sizeof(LaLds<T, DA, NT, false>)];
   la_segment<T, DA, NT, MODE, false>(a, a.role[0], gr, lds);
 }
+// dq, dk and, where its tiles are as many, dv: a row of workgroups each.
 template <typename T, int DA, int NT, bool DOTS>
-__global__ __launch_bounds__(256, (kLaWaves<LaLds<T, DA, NT, DOTS>>)) void la_dqk_kernel(LaArgs a, LaGrid gr) {
+__global__ __launch_bounds__(256, (kLaWaves<LaLds<T, DA, NT, DOTS>>)) void la_grads_kernel(LaArgs a, LaGrid gr) {
   __shared__ __align__(16) char lds[sizeof(LaLds<T, DA, NT, DOTS>)];
   if (blockIdx.y == 0) la_segment<T, DA, NT, kLaDq, DOTS>(a, a.role[0], gr, lds);
-  else la_segment<T, DA, NT, kLaDk, DOTS>(a, a.role[1], gr, lds);
+  else if (blockIdx.y == 1) la_segment<T, DA, NT, kLaDk, DOTS>(a, a.role[1], gr, lds);
+  else la_segment<T, DA, NT, kLaDv, false>(a, a.role[2], gr, lds);
 }
 
 template <typename T, int DA>
@@ -768,15 +770,18 @@ int la_launches(const LaArgs& a, int64_t tiles, const char* what, F launch) {
   }
   return ATK_OK;
 }
+template <typename T, int DA, int NT, int MODE>
+int la_run_out(const LaArgs& a, hipStream_t s) {
+  return la_launches(a, (a.role[0].CD + 64 * NT - 1) / (64 * NT), "la_out_kernel", [&](unsigned n, LaGrid g) {
+    hipLaunchKernelGGL((la_out_kernel<T, DA, NT, MODE>), dim3(n), dim3(256), 0, s, a, g);
+  });
+}
 template <typename T, int DA, int NT>
-int la_run_out(const LaArgs& a, int mode, bool dots, hipStream_t s) {
+int la_run_grads(const LaArgs& a, bool dots, unsigned roles, hipStream_t s) {
   const LaRole& r = a.role[0];
-  const dim3 b(256);
-  return la_launches(a, (int64_t)((r.CD + 64 * NT - 1) / (64 * NT)) * r.a_tiles, "la_out_kernel", [&](unsigned n, LaGrid g) {
-    if (mode == kLaFwd) hipLaunchKernelGGL((la_out_kernel<T, DA, NT, kLaFwd>), dim3(n), b, 0, s, a, g);
-    else if (mode == kLaDv) hipLaunchKernelGGL((la_out_kernel<T, DA, NT, kLaDv>), dim3(n), b, 0, s, a, g);
-    else if (dots) hipLaunchKernelGGL((la_dqk_kernel<T, DA, NT, true>), dim3(n, 2), b, 0, s, a, g);
-    else hipLaunchKernelGGL((la_dqk_kernel<T, DA, NT, false>), dim3(n, 2), b, 0, s, a, g);
+  return la_launches(a, (int64_t)((r.CD + 64 * NT - 1) / (64 * NT)) * r.a_tiles, "la_grads_kernel", [&](unsigned n, LaGrid g) {
+    if (dots) hipLaunchKernelGGL((la_grads_kernel<T, DA, NT, true>), dim3(n, roles), dim3(256), 0, s, a, g);
+    else hipLaunchKernelGGL((la_grads_kernel<T, DA, NT, false>), dim3(n, roles), dim3(256), 0, s, a, g);
   });
 }
 template <typename T, int DA>
@@ -788,12 +793,30 @@ int la_run_states(const LaArgs& a, int roles, float* const* to, float* decays, h
 
 }  // namespace
 
+#define ATK_LA_TILED(DA, NT, FN)                                                        \
+  [&]() {                                                                              \
+    if (NT == 2) return DA == 128 ? FN(128, 2) : FN(64, 2);                            \
+    return DA == 256 ? FN(256, 1) : DA == 128 ? FN(128, 1) : FN(64, 1);                \
+  }()
 template <typename T>
-int la_launch_out(const LaArgs& a, int mode, bool dots, hipStream_t s) {
-  const int da = la_padded(a.role[0].AD);
-  if (la_wide(da, a.role[0].CD) == 2) return da == 128 ? la_run_out<T, 128, 2>(a, mode, dots, s) : la_run_out<T, 64, 2>(a, mode, dots, s);
-  if (da == 256) return la_run_out<T, 256, 1>(a, mode, dots, s);
-  return da == 128 ? la_run_out<T, 128, 1>(a, mode, dots, s) : la_run_out<T, 64, 1>(a, mode, dots, s);
+int la_launch_out(const LaArgs& a, hipStream_t s) {
+  const int da = la_padded(a.K), nt = la_wide(da, a.V);
+#define ATK_LA_OUT(DA, NT) la_run_out<T, DA, NT, kLaFwd>(a, s)
+  return ATK_LA_TILED(da, nt, ATK_LA_OUT);
+}
+template <typename T>
+int la_launch_grads(const LaArgs& a, bool dots, hipStream_t s) {
+  const int dk = la_padded(a.K), dv = la_padded(a.V), nv = la_wide(dk, a.V), nt = la_wide(dv, a.K);
+  // dv shares the launch where its workgroups are shaped as those of dq and dk, and as many
+  const bool one = dk == dv && nv == nt && (a.V + 64 * nt - 1) / (64 * nt) == (a.K + 64 * nt - 1) / (64 * nt) * a.role[0].a_tiles;
+  const unsigned roles = one ? 3 : 2;
+#define ATK_LA_GRADS(DA, NT) la_run_grads<T, DA, NT>(a, dots, roles, s)
+  if (int rc = ATK_LA_TILED(dv, nt, ATK_LA_GRADS)) return rc;
+  if (one) return ATK_OK;
+  LaArgs b = a;
+  b.role[0] = a.role[2];
+#define ATK_LA_DV(DA, NT) la_run_out<T, DA, NT, kLaDv>(b, s)
+  return ATK_LA_TILED(dk, nv, ATK_LA_DV);
 }
 template <typename T>
 int la_launch_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s) {
