@@ -352,13 +352,10 @@ struct LaLds {
 // the first n of N values, one at a time
 template <int N, typename T>
 __device__ __forceinline__ void la_tail(T* to, const float* v, int n) {
-#pragma nounroll
-  for (int i = 0; i < n; ++i) {
-    float x = v[0];
 #pragma unroll
-    for (int j = 1; j < N; ++j) x = i == j ? v[j] : x;
-    to[i] = from_f32<T>(x);
-  }
+  for (int i = 0; i < N; ++i)
+    if (i < n) to[i] = from_f32<T>(v[i]);
+  asm volatile("");  // (else the last store is shared with the whole vector's, which is then split)
 }
 
 // The outputs of one segment, and its last state.  Products that make outputs are taken transposed, so that a
@@ -510,12 +507,6 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
         for (int x = 0; x < NT; ++x) acc[x][m] *= f;
       }
     }
-    T ev[DOTS ? MT : 1][OW];
-    if constexpr (DOTS) {
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-        __builtin_memcpy(ev[m], pe + (at + (16 * m + c < rows ? 16 * m + c : 0)) * r.e_s[1], OW * sizeof(T));
-    }
 #pragma unroll
     for (int s = 0; s < HS; ++s) {
       uint4 cf[NT][NP], pf[MT][OP];
@@ -545,6 +536,12 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
                 for (int x = 0; x < NT; ++x) acc[x][m] = mma(cf[x][p], pf[m][q], acc[x][m]);
               }
             }
+    }
+    T ev[DOTS ? MT : 1][OW];
+    if constexpr (DOTS) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+        __builtin_memcpy(ev[m], pe + (at + (16 * m + c < rows ? 16 * m + c : 0)) * r.e_s[1], OW * sizeof(T));
     }
     if constexpr (MODE == kLaFwd) {
       if (L.spoilt) {  // outputs from a column's first c on that is not finite are not either
