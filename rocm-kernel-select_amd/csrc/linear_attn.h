@@ -96,7 +96,12 @@ template <typename T> int la_launch_grads(const LaArgs& a, bool dots, hipStream_
 template <typename T> int la_launch_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s);
 
 inline int la_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
-// 16 columns of c that each wave of a workgroup has, times: two where the state's rows leave the registers for it
-inline int la_wide(int rows, int cols) { return rows <= 128 && cols > 64 ? 2 : 1; }
+// 16 columns of c that each wave of a workgroup has, times: two where the state's rows leave the registers for it,
+// unless that leaves more than half of the CUs without a workgroup (bf16, 4 sequences of 37 tokens, 16 heads of
+// 128 x 128: 8.5 and 7.3 us a call; 8192 tokens of 32 heads 135 and 164).
+inline int la_wide(const LaArgs& a, int rows, int cols) {
+  const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
+  return rows <= 128 && cols > 64 && (int64_t)a.slots * a.Hv * ((cols + 127) / 128) * 2 > cus ? 2 : 1;
+}
 
 }  // namespace atk

@@ -364,7 +364,8 @@ LaPlan la_plan(const atk_linear_attn_args* p, bool backward, LaArgs* a, int* rc)
   if (backward) {
     const int da = la_padded(a->V);
     L.a_tiles = (a->V + da - 1) / da;
-    L.k_tiles = (a->K + 64 * la_wide(da, a->K) - 1) / (64 * la_wide(da, a->K));
+    const int w = 64 * la_wide(*a, da, a->K);
+    L.k_tiles = (a->K + w - 1) / w;
     L.n_parts = a->group * L.a_tiles;
     if (L.n_parts > 1)
       for (int i = 0; i < 2; ++i) L.parts[i] = take((size_t)L.n_parts * tokens * a->Hk * a->K);
