@@ -73,6 +73,18 @@ __device__ __forceinline__ int la_seq_of_slot(const LaArgs& a, int slot) {
   return lo;
 }
 
+// Tokens of a packed row that no sequence has, before the first and after the last, have results of zero: f(from,
+// to) for those among the slot's share of the row, whichever sequence has the slot, if any.
+template <typename F>
+__device__ __forceinline__ void la_outside(const LaArgs& a, int slot, F f) {
+  if (!a.cu) return;
+  const LaSeq last = la_seq(a, a.n - 1);
+  const int64_t lo = la_seq(a, 0).begin, hi = last.begin + last.len;
+  const int64_t b = (int64_t)slot * a.seg, e = b + a.seg < a.T ? b + a.seg : a.T;
+  if (b < lo) f(b, e < lo ? e : lo);
+  if (e > hi) f(b > hi ? b : hi, e);
+}
+
 // Workgroup -> (tile, value head, slot).  Workgroups are dealt to the 8 XCDs in turn; the tiles and value
 // heads of a key head get the same one, since they read the same rows through its L2.  A launch begins with
 // the first workgroup of unit `unit0`, a multiple of 8.

@@ -259,11 +259,10 @@ __global__ __launch_bounds__(256) void la_gate_kernel(LaArgs a, LaGateArgs b) {
 #pragma unroll
     for (int off = 32; off >= 1; off >>= 1) all += __shfl_xor(all, off, 64);
     if (lane == 0) b.seg_sums[(int64_t)h * a.slots + slot] = (float)all;
-  } else if (live && a.cu) {  // tokens of no sequence
-    if (n == 0 && z == 0)
-      for (int64_t t = lane; t < seq.begin; t += 64) static_cast<G*>(b.dg)[t * a.Hv + h] = from_f32<G>(0.f);
-    if (n == a.n - 1 && z == segs - 1)
-      for (int64_t t = seq.begin + seq.len + lane; t < a.T; t += 64) static_cast<G*>(b.dg)[t * a.Hv + h] = from_f32<G>(0.f);
+  } else {
+    la_outside(a, slot, [&](int64_t from, int64_t to) {
+      for (int64_t t = from + lane; t < to; t += 64) static_cast<G*>(b.dg)[t * a.Hv + h] = from_f32<G>(0.f);
+    });
   }
 }
 // one decay a head: its gradient is the sum over all segments

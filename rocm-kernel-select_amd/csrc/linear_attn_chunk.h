@@ -257,7 +257,7 @@ __device__ __forceinline__ void la_load(const LaArgs& a, const LaRole& r, bool f
 #pragma unroll
       for (int t = 0; t < RT; ++t) {
         if constexpr (SWAP) {
-          S[t][x] = *reinterpret_cast<const f32x4*>(at + 16 * t);
+          __builtin_memcpy(&S[t][x], at + 16 * t, 16);  // (a state may begin at any element)
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e) S[t][x][e] = at[(uint32_t)((16 * t + e) * a.V)];
@@ -372,16 +372,28 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
   int tile, h, slot;
   if (!la_place(a, gr, &tile, &h, &slot)) return;
   const int hk = h / a.group, c_tiles = (r.CD + W - 1) / W, c_tile = swapped ? tile % c_tiles : tile, a_tile = swapped ? tile / c_tiles : 0;
+  const int a0 = a_tile * DA, col0 = c_tile * W, col = col0 + wave * 16 * NT;
+  const int acols = r.AD - a0 < DA ? r.AD - a0 : DA, ccols = r.CD - col0 < W ? r.CD - col0 : W;
+  const bool full = acols == DA && ccols == W;
+  const int ha = swapped ? h : hk, hc = swapped ? hk : h;
+  if (a_tile == 0)
+    la_outside(a, slot, [&](int64_t from, int64_t to) {
+      for (int64_t t = from + tid / 64; t < to; t += 4)
+        for (int j = lane; j < ccols; j += 64) {
+          if (swapped && r.parts) {
+            for (int q = 0; q < r.a_tiles; ++q)
+              r.parts[((((int64_t)(h % a.group) * r.a_tiles + q) * a.B * a.T + t) * a.Hk + hk) * r.CD + col0 + j] = 0.f;
+          } else {
+            static_cast<T*>(r.out)[(t * (swapped ? a.Hk : a.Hv) + hc) * r.CD + col0 + j] = from_f32<T>(0.f);
+          }
+        }
+    });
   const int n = la_seq_of_slot(a, slot);
   const LaSeq seq = la_seq(a, n);
   const int z = slot - seq.slot;
   if (z < 0 || z >= seq.segs) return;
   const int t0 = z * a.seg, len = seq.len - t0 < a.seg ? seq.len - t0 : a.seg;  // tokens of this segment
   const int chunks = (len + CT - 1) / CT;
-  const int a0 = a_tile * DA, col0 = c_tile * W, col = col0 + wave * 16 * NT;
-  const int acols = r.AD - a0 < DA ? r.AD - a0 : DA, ccols = r.CD - col0 < W ? r.CD - col0 : W;
-  const bool full = acols == DA && ccols == W;
-  const int ha = swapped ? h : hk, hc = swapped ? hk : h;
   const int64_t first = seq.begin + t0;
   const T* __restrict__ pa = static_cast<const T*>(r.a) + seq.batch * r.a_s[0] + first * r.a_s[1] + ha * r.a_s[2] + a0;
   const T* __restrict__ pb = static_cast<const T*>(r.b) + seq.batch * r.b_s[0] + first * r.b_s[1] + ha * r.b_s[2] + a0;
@@ -643,22 +655,6 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
       __syncthreads();
       if (tid == 0)
         r.x_out[((int64_t)tile * a.slots + slot) * a.Hv + h] = (L.dots[0][0] + L.dots[1][0]) + (L.dots[2][0] + L.dots[3][0]);
-    }
-  }
-  // tokens of a packed row before its first sequence and after its last have zeros
-  if (a.cu && a_tile == 0) {
-    for (int w = 0; w < 2; ++w) {
-      if (w == 0 ? n != 0 || z != 0 : n != a.n - 1 || z != seq.segs - 1) continue;
-      const int64_t b = w == 0 ? 0 : seq.begin + seq.len, end = w == 0 ? seq.begin : a.T;
-      for (int64_t t = b; t < end; ++t)
-        for (int j = tid; j < ccols; j += 256) {
-          if (swapped && r.parts) {
-            for (int q = 0; q < r.a_tiles; ++q)
-              r.parts[((((int64_t)(h % a.group) * r.a_tiles + q) * a.B * a.T + t) * a.Hk + hk) * r.CD + col0 + j] = 0.f;
-          } else {
-            static_cast<T*>(r.out)[(t * (swapped ? a.Hk : a.Hv) + hc) * r.CD + col0 + j] = from_f32<T>(0.f);
-          }
-        }
     }
   }
 }

@@ -635,3 +635,45 @@ def test_refusals(dev):
             P.linear_attention_update(q, k, v, g, state, state_indices=i)
     with pytest.raises(RuntimeError, match="256"):
         P.linear_attention_update(*make((1,), 1, 1, 257, 8, torch.bfloat16, dev), torch.zeros(1, 1, 257, 8, device=dev))
+
+
+@gpu
+@pytest.mark.parametrize("cu", [(0, 70), (5000, 5064), (0, 0), (19999, 20000)], ids=str)
+def test_rows_mostly_outside(dev, cu):
+    """A packed row most of which belongs to no sequence: zeros there, written by the call."""
+    import amd_tuned_torch as P
+    t = 20000
+    args = make((1, t), 1, 4, 64, 40, torch.bfloat16, dev)
+    off = torch.tensor(cu, dtype=torch.int32, device=dev)
+    keep = torch.full((1, t, 4, 40), float("nan"), device=dev, dtype=torch.bfloat16)  # what fresh memory may hold
+    dout = keep.nan_to_num(1.0)
+    del keep
+    leaves = [x.requires_grad_() for x in args]
+    out = P.linear_attention(*leaves, cu_seqlens=off)
+    grads = torch.autograd.grad(out, leaves, dout)
+    a, b = cu
+    alone = [x.detach()[:, a:b].clone().requires_grad_() for x in args]
+    want = P.linear_attention(*alone)
+    want_grads = torch.autograd.grad(want, alone, dout[:, a:b])
+    for x, y in zip((out, *grads), (want, *want_grads)):
+        assert x[:, :a].eq(0).all() and x[:, b:].eq(0).all()
+        assert (x[:, a:b].float() - y.float()).abs().max() <= 2.0 ** -6 * y.float().abs().max() if b > a else True
+
+
+@gpu
+def test_states_that_begin_anywhere(dev):
+    """Initial states and their gradients whose first element has no alignment."""
+    import amd_tuned_torch as P
+    args = make((2, 700), 1, 2, 64, 64, torch.bfloat16, dev)
+    n = 2 * 2 * 64 * 64
+    base, dbase = torch.randn(n + 1, device=dev), torch.randn(n + 1, device=dev)
+    dout = torch.randn(2, 700, 2, 64, device=dev).bfloat16()
+    outs = []
+    for shift in (lambda x: x[1:].view(2, 2, 64, 64), lambda x: x[1:].clone().view(2, 2, 64, 64)):
+        state, dstate = shift(base), shift(dbase)
+        outs.append(run_backward(P, args, 0.1, None, None, dout, dstate))
+        leaves = [x.detach().requires_grad_() for x in args]
+        out, S = P.linear_attention(*leaves, 0.1, initial_state=state, return_final_state=True)
+        outs[-1] += (out.detach(), S.detach(), *torch.autograd.grad((out, S), leaves, (dout, dstate)))
+    flat = [[y for x in o for y in (x if isinstance(x, tuple) else (x,))] for o in outs]
+    assert all(torch.equal(a, b) for a, b in zip(*flat))

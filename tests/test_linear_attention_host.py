@@ -323,3 +323,24 @@ def test_traces(nat, monkeypatch):
                 want = fn(*(x.clone() for x in other))
         for a, b in zip(*(x if isinstance(x, tuple) else (x,) for x in (got, want))):
             assert torch.equal(a, b), i
+
+
+def test_launches_go_to_the_tensors_device(nat, monkeypatch):
+    """Where another device is the current one, the call runs with the tensors' made current."""
+    seen, current = [], [0]
+
+    class Switch:
+        def __init__(self, device):
+            self.to = device.index
+
+        def __enter__(self):
+            self.back, current[0] = current[0], self.to
+
+        def __exit__(self, *a):
+            current[0] = self.back
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Switch)
+    for index in (0, 3):
+        assert nat._on(torch.device("cuda", index), lambda x: seen.append((x, current[0])) or x, index) == index
+    assert seen == [(0, 0), (3, 3)] and current == [0]
