@@ -62,15 +62,32 @@ __device__ __forceinline__ LaSeq la_seq(const LaArgs& a, int n) {
   e = e < b ? b : e > T ? T : e;
   return {0, b, e - b, (int)fdiv((uint32_t)b, a.by_seg) + n, la_segments(a, e - b)};
 }
-__device__ __forceinline__ int la_seq_of_slot(const LaArgs& a, int slot) {
-  if (!a.cu) return (int)fdiv((uint32_t)slot, a.by_segs);
-  int lo = 0, hi = a.n - 1;  // the last sequence whose first slot is not after `slot`
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (la_seq(a, mid).slot <= slot) lo = mid;
-    else hi = mid - 1;
+// The last of n sequences that `before` holds for, or the first (it holds up to one, if offsets are in order): by a
+// wave, 64 at a time.
+template <typename F>
+__device__ __forceinline__ int la_last(int n, F before) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 63) / 64, at = lo + (int)(threadIdx.x & 63) * step;
+    const uint64_t in = __ballot(at < hi && before(at));
+    lo += (in ? 63 - __builtin_clzll(in) : 0) * step;
+    hi = lo + step < hi ? lo + step : hi;
   }
   return lo;
+}
+__device__ __forceinline__ int la_seq_of_slot(const LaArgs& a, int slot) {
+  if (!a.cu) return (int)fdiv((uint32_t)slot, a.by_segs);
+  return la_last(a.n, [&](int n) { return la_seq(a, n).slot <= slot; });
+}
+// Where all that is asked for is sequences of more than one segment, those are found by the tokens i seg, of which each
+// segment of `seg` tokens has one: fewer than slots where sequences are many and short.  The segment with that
+// token, or false.
+__device__ __forceinline__ bool la_segment_at(const LaArgs& a, int i, int* n, LaSeq* seq, int* z) {
+  const int token = i * a.seg;
+  *n = la_last(a.n, [&](int m) { return la_seq(a, m).begin <= token; });
+  *seq = la_seq(a, *n);
+  *z = (int)fdiv((uint32_t)(token - seq->begin), a.by_seg);
+  return token >= seq->begin && token < seq->begin + seq->len;
 }
 
 // Tokens of a packed row that no sequence has, before the first and after the last, have results of zero: f(from,
@@ -90,7 +107,7 @@ __device__ __forceinline__ void la_outside(const LaArgs& a, int slot, F f) {
 // the first workgroup of unit `unit0`, a multiple of 8.
 struct LaGrid {
   FastDiv per, tiles;  // workgroups of a unit (tiles of the value heads of a key head); tiles of a head
-  int unit0;
+  int unit0, slots;
 };
 __device__ __forceinline__ bool la_place(const LaArgs& a, const LaGrid& gr, int* tile, int* h, int* slot) {
   const uint32_t j = blockIdx.x / 8, u = fdiv(j, gr.per), unit = gr.unit0 + u * 8 + blockIdx.x % 8;
@@ -98,7 +115,7 @@ __device__ __forceinline__ bool la_place(const LaArgs& a, const LaGrid& gr, int*
   *tile = (int)(in - head * gr.tiles.d);
   *h = (int)((unit - s * a.by_hk.d) * a.group + head);
   *slot = (int)s;
-  return s < (uint32_t)a.slots;
+  return s < (uint32_t)gr.slots;
 }
 
 // Launchers, each for one type: the outputs of role 0, or all gradients (dq, dk, dv are roles 0, 1 and 2); what
@@ -115,5 +132,8 @@ inline int la_wide(const LaArgs& a, int rows, int cols) {
   const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
   return rows <= 128 && cols > 64 && (int64_t)a.slots * a.Hv * ((cols + 127) / 128) * 2 > cus ? 2 : 1;
 }
+
+// tokens i seg of a packed row (la_segment_at)
+inline int la_marks(const LaArgs& a) { return (int)((a.T + a.seg - 1) / a.seg); }
 
 }  // namespace atk

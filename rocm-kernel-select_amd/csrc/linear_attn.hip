@@ -145,18 +145,26 @@ void launch_step_typed(const LaStepArgs& a, hipStream_t s) {
 // Segments joined: what each adds to the state becomes the state after it (in reverse, the gradient of the
 // state before it), in place.  A thread has VW elements of a state, all segments of a sequence.
 template <int VW>
-__global__ __launch_bounds__(256) void la_scan_kernel(LaArgs a, float* s0, float* s1, const float* decays, FastDiv per, int first) {
-  const uint32_t unit = fdiv(blockIdx.x, per), nh = first + unit, n = fdiv(nh, a.by_hv);
-  const int h = (int)(nh - n * a.by_hv.d);
+__global__ __launch_bounds__(256) void la_scan_kernel(LaArgs a, float* s0, float* s1, const float* decays, FastDiv per, int first,
+                                                      int marks) {
+  const uint32_t unit = fdiv(blockIdx.x, per), ih = first + unit, index = fdiv(ih, a.by_hv);
+  const int h = (int)(ih - index * a.by_hv.d);
+  int n = (int)index;
+  LaSeq seq;
+  if (marks) {  // the sequence with its first token of those that la_segment_at goes by
+    int z;
+    if (!la_segment_at(a, (int)index, &n, &seq, &z) || z > 0) return;
+  } else {
+    seq = la_seq(a, n);
+  }
   const int kv = a.K * a.V, i = (int)((blockIdx.x - unit * per.d) * 256 + threadIdx.x) * VW;
   const bool rev = blockIdx.y;
   if (i >= kv) return;
-  const LaSeq seq = la_seq(a, (int)n);
   const int segs = seq.segs;
   const float* init = a.role[rev].s_first;
   float run[VW];
 #pragma unroll
-  for (int j = 0; j < VW; ++j) run[j] = init ? init[(int64_t)nh * kv + i + j] : 0.f;
+  for (int j = 0; j < VW; ++j) run[j] = init ? init[((int64_t)n * a.Hv + h) * kv + i + j] : 0.f;
   const int64_t step = (int64_t)a.Hv * kv;
   float* __restrict__ p = (rev ? s1 : s0) + (seq.slot + (rev ? segs - 1 : 0)) * step + (int64_t)h * kv + i;
   const float* __restrict__ d = decays + ((int64_t)(rev ? a.slots : 0) + seq.slot + (rev ? segs - 1 : 0)) * a.Hv + h;
@@ -215,11 +223,12 @@ __global__ __launch_bounds__(256) void la_sum_kernel(LaSumArgs a) {
 struct LaGateArgs {
   const float* qd; const float* kd; const float* x; void* dg; float* seg_sums;
   int tiles;
+  uint32_t unit0;  // segments of heads before this launch's
 };
 template <typename G>
 __global__ __launch_bounds__(256) void la_gate_kernel(LaArgs a, LaGateArgs b) {
   const int lane = threadIdx.x & 63;
-  const uint32_t unit = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const uint32_t unit = b.unit0 + blockIdx.x * 4 + (threadIdx.x >> 6);
   const int slot = (int)fdiv(unit, a.by_hv), h = (int)unit - slot * a.Hv;
   if (slot >= a.slots) return;
   const int n = la_seq_of_slot(a, slot);
@@ -292,9 +301,11 @@ struct LaPlan {
 //   chunks of a segment x 8 us where each workgroup has a CU, 10.5 where two share one, in rounds of those
 //   + the states, written and read twice, at 3.5 TB/s,
 // or that of one segment a sequence, which has no states between.  Lengths of packed sequences are on the
-// device; there the average counts.  (bf16, 128 x 128, us a call: 2 x 2048 tokens of 16 heads with 128, 192 and 256
-// tokens a segment 62, 66 and 57; 8192 of 32 heads with 512 and 576 145 and 160; fp32, 64 x 64, 3 sequences, 1021
-// tokens of 4 heads with 64 and 256 29 and 48.)
+// device; there the average counts, and a segment has at most 1024 tokens or four times the average, lest a long
+// sequence among short ones be left to a workgroup a head (bf16, 128 x 128, 16 heads: one of 8192 and 64 of 64 tokens
+// 663 -> 136 us; the launches that this adds where all are short, 64 of 192 tokens 61 -> 63).  (bf16, 128 x 128, us a
+// call: 2 x 2048 tokens of 16 heads with 128, 192 and 256 tokens a segment 62, 66 and 57; 8192 of 32 heads with 512 and
+// 576 145 and 160; fp32, 64 x 64, 3 sequences, 1021 tokens of 4 heads with 64 and 256 29 and 48.)
 int64_t la_segment_tokens(const atk_linear_attn_args* p) {
   const double cus = device_cu_count() > 0 ? device_cu_count() : 256, n = (double)(p->N > 0 ? p->N : 1);
   const double chunks = p->cu_seqlens ? (double)p->T / 64 / n : (double)((p->T + 63) / 64);
@@ -310,6 +321,10 @@ int64_t la_segment_tokens(const atk_linear_attn_args* p) {
       least = t;
       best = per;
     }
+  }
+  if (p->cu_seqlens) {
+    const int64_t most = chunks > 4 ? (int64_t)(4 * chunks) : 16;
+    if (best > most) best = most;
   }
   return best * 64;
 }
@@ -383,12 +398,14 @@ int la_scan(const LaArgs& a, float* s0, float* s1, const float* decays, int role
   const int64_t kv = (int64_t)a.K * a.V;
   bool vec = kv % 4 == 0;
   for (int i = 0; i < roles; ++i) vec = vec && aligned16(a.role[i].s_first);
-  const int64_t per = (kv + (vec ? 1023 : 255)) / (vec ? 1024 : 256), units = (int64_t)a.n * a.Hv;
+  const int64_t per = (kv + (vec ? 1023 : 255)) / (vec ? 1024 : 256);
+  const int marks = a.cu && la_marks(a) < a.n ? la_marks(a) : 0;
+  const int64_t units = (int64_t)(marks ? marks : a.n) * a.Hv;
   const int64_t most = kLaBlocks / per > 0 ? kLaBlocks / per : 1;
   for (int64_t u = 0; u < units; u += most) {
     const dim3 g((unsigned)((units - u < most ? units - u : most) * per), (unsigned)roles);
-    if (vec) hipLaunchKernelGGL((la_scan_kernel<4>), g, dim3(256), 0, s, a, s0, s1, decays, make_fastdiv((uint32_t)per), (int)u);
-    else hipLaunchKernelGGL((la_scan_kernel<1>), g, dim3(256), 0, s, a, s0, s1, decays, make_fastdiv((uint32_t)per), (int)u);
+    if (vec) hipLaunchKernelGGL((la_scan_kernel<4>), g, dim3(256), 0, s, a, s0, s1, decays, make_fastdiv((uint32_t)per), (int)u, marks);
+    else hipLaunchKernelGGL((la_scan_kernel<1>), g, dim3(256), 0, s, a, s0, s1, decays, make_fastdiv((uint32_t)per), (int)u, marks);
     if (int rc = check_launch("la_scan_kernel")) return rc;
   }
   return ATK_OK;
@@ -414,9 +431,14 @@ int la_forward(const atk_linear_attn_args* p, LaArgs& a, const LaPlan& L, hipStr
 
 template <typename T, typename G>
 int la_gates(const LaArgs& a, const LaPlan& L, void* dg, hipStream_t s) {
-  LaGateArgs b = {L.dots[0], L.dots[1], L.x, dg, L.seg_sums, L.a_tiles * L.k_tiles};
-  hipLaunchKernelGGL((la_gate_kernel<G>), dim3((unsigned)(((int64_t)a.slots * a.Hv + 3) / 4)), dim3(256), 0, s, a, b);
-  if (int rc = check_launch("la_gate_kernel")) return rc;
+  LaGateArgs b = {L.dots[0], L.dots[1], L.x, dg, L.seg_sums, L.a_tiles * L.k_tiles, 0};
+  const int64_t units = (int64_t)a.slots * a.Hv;
+  for (int64_t u = 0; u < units; u += (int64_t)kLaBlocks * 4) {
+    b.unit0 = (uint32_t)u;
+    const int64_t blocks = (units - u + 3) / 4;
+    hipLaunchKernelGGL((la_gate_kernel<G>), dim3((unsigned)(blocks < kLaBlocks ? blocks : kLaBlocks)), dim3(256), 0, s, a, b);
+    if (int rc = check_launch("la_gate_kernel")) return rc;
+  }
   if (!a.fixed) return ATK_OK;
   hipLaunchKernelGGL((la_gate_sum_kernel<G>), dim3((unsigned)a.Hv), dim3(256), 0, s, L.seg_sums, static_cast<G*>(dg), a.slots);
   return check_launch("la_gate_sum_kernel");

@@ -66,6 +66,8 @@ struct LaTile {
       __builtin_memcpy(&r[i], reinterpret_cast<const char*>(p - back) + (size_t)off, 16);  // element alignment only
     }
   }
+  // fp32 values that round up to infinity in bf16 have no parts either: raised by 2^-8 they are infinite
+  static __device__ __forceinline__ float raised(float v) { return sizeof(T) == 4 ? v * 1.00390625f : v; }
   // NaN or not zero where one of a vector's elements is not finite
   static __device__ __forceinline__ float spoilt_by(uint4 v) {
     float z = 0.f;
@@ -73,7 +75,7 @@ struct LaTile {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (sizeof(T) == 4) {
-        z = fmaf(__uint_as_float(w[j]), 0.f, z);
+        z = fmaf(raised(__uint_as_float(w[j])), 0.f, z);
       } else if constexpr (__is_same(T, __bf16)) {
         typedef __bf16 b2 __attribute__((ext_vector_type(2)));
         z = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w[j]), b2{0, 0}, z, false);
@@ -115,8 +117,7 @@ struct LaTile {
           __builtin_memcpy(e, &r[i], 16);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            const float f = to_f32(e[j]);
-            if (f * 0.f != 0.f) {
+            if (raised(to_f32(e[j])) * 0.f != 0.f) {
               atomicMin(&bad[c + j], from + row0 + i * STEP);
               *spoilt = 1;
               e[j] = from_f32<T>(0.f);
@@ -698,10 +699,18 @@ __device__ __forceinline__ void la_state(const LaArgs& a, const LaRole& r, const
   int tile, h, slot;
   if (!la_place(a, gr, &tile, &h, &slot)) return;
   const int hk = h / a.group;
-  const int n = la_seq_of_slot(a, slot);
-  const LaSeq seq = la_seq(a, n);
-  const int z = slot - seq.slot;
-  if (z < 0 || z >= seq.segs || z == (rev ? 0 : seq.segs - 1)) return;
+  int n, z;
+  LaSeq seq;
+  if (a.cu) {
+    if (!la_segment_at(a, slot, &n, &seq, &z)) return;
+  } else {
+    n = la_seq_of_slot(a, slot);
+    seq = la_seq(a, n);
+    z = slot - seq.slot;
+  }
+  if (z == seq.segs - 1) return;
+  z += rev;
+  slot = seq.slot + z;
   const int t0 = z * a.seg, len = seq.len - t0 < a.seg ? seq.len - t0 : a.seg, chunks = (len + CT - 1) / CT;
   const int col0 = tile * W, col = col0 + wave * 16 * NT;
   const int acols = r.AD, ccols = r.CD - col0 < W ? r.CD - col0 : W;
@@ -752,34 +761,34 @@ __global__ __launch_bounds__(256, 2) void la_state_kernel(LaArgs a, LaGrid gr, f
 
 // launch(grid, its place) for workgroups of all tiles, heads and segments, in as many launches as it takes
 template <typename F>
-int la_launches(const LaArgs& a, int64_t tiles, const char* what, F launch) {
-  const int64_t per = tiles * a.group, units = ((int64_t)a.slots * a.Hk + 7) / 8 * 8;
+int la_launches(const LaArgs& a, int slots, int64_t tiles, const char* what, F launch) {
+  const int64_t per = tiles * a.group, units = ((int64_t)slots * a.Hk + 7) / 8 * 8;
   if (per > kLaBlocks / 8) return fail(ATK_UNSUPPORTED, "linear attention: too many value heads and columns of a key head");
   const int64_t most = kLaBlocks / 8 / per * 8;
   for (int64_t u = 0; u < units; u += most) {
     launch((unsigned)((units - u < most ? units - u : most) * per),
-           LaGrid{make_fastdiv((uint32_t)per), make_fastdiv((uint32_t)tiles), (int)u});
+           LaGrid{make_fastdiv((uint32_t)per), make_fastdiv((uint32_t)tiles), (int)u, slots});
     if (int rc = check_launch(what)) return rc;
   }
   return ATK_OK;
 }
 template <typename T, int DA, int NT, int MODE>
 int la_run_out(const LaArgs& a, hipStream_t s) {
-  return la_launches(a, (a.role[0].CD + 64 * NT - 1) / (64 * NT), "la_out_kernel", [&](unsigned n, LaGrid g) {
+  return la_launches(a, a.slots, (a.role[0].CD + 64 * NT - 1) / (64 * NT), "la_out_kernel", [&](unsigned n, LaGrid g) {
     hipLaunchKernelGGL((la_out_kernel<T, DA, NT, MODE>), dim3(n), dim3(256), 0, s, a, g);
   });
 }
 template <typename T, int DA, int NT>
 int la_run_grads(const LaArgs& a, bool dots, unsigned roles, hipStream_t s) {
   const LaRole& r = a.role[0];
-  return la_launches(a, (int64_t)((r.CD + 64 * NT - 1) / (64 * NT)) * r.a_tiles, "la_grads_kernel", [&](unsigned n, LaGrid g) {
+  return la_launches(a, a.slots, (int64_t)((r.CD + 64 * NT - 1) / (64 * NT)) * r.a_tiles, "la_grads_kernel", [&](unsigned n, LaGrid g) {
     if (dots) hipLaunchKernelGGL((la_grads_kernel<T, DA, NT, true>), dim3(n, roles), dim3(256), 0, s, a, g);
     else hipLaunchKernelGGL((la_grads_kernel<T, DA, NT, false>), dim3(n, roles), dim3(256), 0, s, a, g);
   });
 }
 template <typename T, int DA>
 int la_run_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s) {
-  return la_launches(a, (a.V + 63) / 64, "la_state_kernel", [&](unsigned n, LaGrid g) {
+  return la_launches(a, a.cu ? la_marks(a) : a.slots, (a.V + 63) / 64, "la_state_kernel", [&](unsigned n, LaGrid g) {
     hipLaunchKernelGGL((la_state_kernel<T, DA>), dim3(n, (unsigned)roles), dim3(256), 0, s, a, g, to[0], roles > 1 ? to[1] : nullptr, decays);
   });
 }

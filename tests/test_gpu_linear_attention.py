@@ -677,3 +677,45 @@ def test_states_that_begin_anywhere(dev):
         outs[-1] += (out.detach(), S.detach(), *torch.autograd.grad((out, S), leaves, (dout, dstate)))
     flat = [[y for x in o for y in (x if isinstance(x, tuple) else (x,))] for o in outs]
     assert all(torch.equal(a, b) for a, b in zip(*flat))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_a_types_largest_values(dev, dtype):
+    """The type's lowest and largest value, as padding may hold them, spoil no token before their own either."""
+    import amd_tuned_torch as P
+    t, at = 400, 301
+    clean = make((1, t), 1, 2, 64, 72, dtype, dev)
+    want = P.linear_attention(*clean)
+    for x in (torch.finfo(dtype).min, torch.finfo(dtype).max):
+        for i in (0, 1, 2):
+            args = [y.clone() for y in clean]
+            args[i][0, at:] = x
+            assert torch.equal(P.linear_attention(*args)[:, :at], want[:, :at]), (i, x)
+        args = [y.clone() for y in clean]
+        args[2][0, at, 1, 5] = x
+        rest = [c for c in range(72) if c != 5]
+        assert torch.equal(P.linear_attention(*args)[..., rest], want[..., rest]), x
+
+
+@gpu
+def test_more_heads_than_a_launch(dev):
+    """More sequences' heads than a launch has workgroups: every kernel of the backward is launched in parts."""
+    import amd_tuned_torch as P
+    n, hv, d = 65535, 136, 8                       # 8912760 of them; a launch has 2^23 waves or 2^21 workgroups
+    torch.manual_seed(3)
+    q, k = (torch.randn(n, 1, 1, d, device=dev).bfloat16().requires_grad_() for _ in range(2))
+    v = torch.randn(n, 1, hv, d, device=dev).bfloat16().requires_grad_()
+    g = (-torch.rand(n, 1, hv, device=dev)).requires_grad_()
+    state, dout = torch.randn(n, hv, d, d, device=dev), torch.randn(n, 1, hv, d, device=dev).bfloat16()
+    out = P.linear_attention(q, k, v, g, 1.0, initial_state=state)
+    dq, dk, dv, dg = torch.autograd.grad(out, (q, k, v, g), dout)
+    steps = 1 + 2 * d + 100 + hv                   # and the sum over the heads of dq and dk
+    for at in (slice(0, 40), slice(30000, 30040), slice(n - 40, n)):
+        few, s0, do = [x.detach()[at] for x in (q, k, v, g)], state[at], dout[at]
+        want, size = forward64(*few, 1.0, s0, None)[0], forward64(*sizes(*few), 1.0, s0.abs(), None)[0]
+        close(out.detach()[at], want, size, steps, "out")
+        want = backward64(*few, 1.0, s0, None, do, None)
+        size = backward64(*sizes(*few), 1.0, s0.abs(), None, do.abs(), None, size=True)
+        for got, w, s, name in zip((dq, dk, dv, dg), want, size, ("dq", "dk", "dv", "dg")):
+            close(got[at], w, s, 2 * steps, name)
