@@ -1880,6 +1880,11 @@ def _on(device: torch.device, fn, *args):
         return fn(*args)
 
 
+def _dense_like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised tensor like t, dense (0.9 us; torch.empty of its shape, dtype and device takes 2.0)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _gated_block(x, gate, weight, eps: float, group: int, activation: str, gate_first: bool):
     """(struct, its address, x and gate as rows, weight), checked and filled but for the outputs."""
     dt = x.dtype
@@ -1916,7 +1921,7 @@ def rms_norm_gated(x: torch.Tensor, gate: torch.Tensor, weight: Optional[torch.T
     """The norm over each run of `group` columns of x's last axis (0: all of it), times weight and the gate's
     activation, which gate_first puts in front of the norm."""
     a, at, x, gate, weight = _gated_block(x, gate, weight, eps, group, activation, gate_first)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _dense_like(x)
     if a.M == 0 or a.N == 0:
         return y
     a.y = y.data_ptr()
@@ -1930,7 +1935,7 @@ def rms_norm_gated_backward(dy: torch.Tensor, x: torch.Tensor, gate: torch.Tenso
     if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
         raise RuntimeError("rms_norm_gated backward: the gradient must match the output")
     a, at, x, gate, weight = _gated_block(x, gate, weight, eps, group, activation, gate_first)
-    dx, dz = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for _ in range(2))
+    dx, dz = _dense_like(x), _dense_like(x)
     want_dw = want_dw and weight is not None
     if a.M == 0 or a.N == 0:
         return dx, dz, (torch.zeros_like(weight) if want_dw else None)
@@ -1983,8 +1988,7 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, p
         a.rot, a.freq64, a.interleaved, a.inverse = 2 * inv_freq.numel(), int(inv_freq.dtype == torch.float64), interleaved, inverse
         a.dtype, a.scale = _DTYPE_CODE[q.dtype], scale
         blk[2] = key
-    oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ok = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    oq, ok = _dense_like(q), None if k is None else _dense_like(k)
     if oq.numel() == 0 and (ok is None or ok.numel() == 0):
         return oq, ok
     a.q, a.k, a.q_out, a.k_out, a.inv_freq = q.data_ptr(), _ptr(k), oq.data_ptr(), _ptr(ok), inv_freq.data_ptr()
@@ -2041,7 +2045,7 @@ def linear_attn_update(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: tor
         a.Hk, a.Hv, a.K, a.V, a.scale = Hk, v.shape[1], K, v.shape[2], scale
         a.dtype, a.g_dtype = _DTYPE_CODE[q.dtype], _DTYPE_CODE[g.dtype]
         blk[2] = key
-    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    out = _dense_like(v)
     if a.N == 0:
         return out
     a.q, a.k, a.v, a.g = q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr()
@@ -2175,7 +2179,7 @@ def linear_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tens
         return out[..., :V].contiguous(), None if final is None else final[:, :, :K, :V].contiguous()
     blk = _linear_block(q, k, v, g, scale, initial_state, cu_seqlens)
     a, n, device = blk[0], blk[3], v.device
-    out = torch.empty(v.shape, dtype=v.dtype, device=device)
+    out = _dense_like(v)
     final = torch.empty((n, v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=device) if want_state else None
     if n == 0:
         return out.zero_(), final
@@ -2207,9 +2211,9 @@ def linear_attn_backward(q, k, v, g, scale: float, initial_state, cu_seqlens, do
                 None if ds is None else ds[:, :, :K, :V].contiguous())
     blk = _linear_block(q, k, v, g, scale, initial_state, cu_seqlens)
     a, n, device = blk[0], blk[3], v.device
-    make = torch.empty if n and v.numel() else torch.zeros
-    grads = [make(t.shape, dtype=t.dtype, device=device) for t in (q, k, v)]
-    dg = make(g.shape, dtype=g.dtype, device=device) if want_dg else None
+    make = _dense_like if n and v.numel() else lambda t: _dense_like(t).zero_()
+    grads = [make(t) for t in (q, k, v)]
+    dg = make(g) if want_dg else None
     dstate = None
     if want_dstate:
         dstate = torch.empty((n, v.shape[2], q.shape[3], v.shape[3]), dtype=torch.float32, device=device)
