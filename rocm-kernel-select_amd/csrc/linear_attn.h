@@ -26,7 +26,7 @@ struct LaRole {
   int AD, CD;                              // columns of a and b, and of c, in all
   int a_tiles;                             // tiles of a's columns, each a sum of its own
   const float* s_first;                    // state that the first segment starts from, or null (zeros)
-  const float* s_between;                  // [slot][Hv] states at the ends (in reverse: the starts) of segments, or null
+  const float* s_between;                  // [end][Hv] states where segments of a sequence meet, or null
   float* s_last;                           // where the last segment's state goes, or null
   void* out;                               // T (B, T, heads of out, CD), or
   float* parts;                            // fp32 sums [head of the group * a_tiles + a tile][B T][Hk][CD]
@@ -40,27 +40,30 @@ struct LaArgs {
   const int* cu;
   int64_t T, B;             // tokens of a sequence (of the packed row with cu); first axis of the tensors
   int n, slots, seg;        // sequences; segments (unused ones of packed sequences among them), tokens of one
+  int ends;                 // places for states where two segments meet
   int Hk, Hv, group, K, V, g_dtype, fixed;
   FastDiv by_hk, by_hv, by_seg, by_segs;  // segments of a sequence where all have as many
   float scale;
 };
 
 // Where sequence n's tokens and segments lie.  A packed sequence has the segment slots from begin / seg + n
-// on: the next one's begin at or after its end, so no prefix sum over the lengths is needed.  Offsets are
-// clamped to the row.
+// on: the next one's begin at or after its end, so no prefix sum over the lengths is needed.  The state where its
+// segments z and z + 1 meet has the place `end` + z: that of the one token i seg (la_segment_at) in segment z.
+// Offsets are clamped to the row.
 struct LaSeq {
-  int batch, begin, len, slot, segs;
+  int batch, begin, len, slot, segs, end;
 };
 __device__ __forceinline__ int la_segments(const LaArgs& a, int len) {
   return len > a.seg ? (int)fdiv((uint32_t)(len - 1), a.by_seg) + 1 : 1;
 }
 __device__ __forceinline__ LaSeq la_seq(const LaArgs& a, int n) {
   const int T = (int)a.T;
-  if (!a.cu) return {n, 0, T, n * (int)a.by_segs.d, (int)a.by_segs.d};
+  if (!a.cu) return {n, 0, T, n * (int)a.by_segs.d, (int)a.by_segs.d, n * (int)a.by_segs.d};
   int b = a.cu[n], e = a.cu[n + 1];
   b = b < 0 ? 0 : b > T ? T : b;
   e = e < b ? b : e > T ? T : e;
-  return {0, b, e - b, (int)fdiv((uint32_t)b, a.by_seg) + n, la_segments(a, e - b)};
+  const int i = (int)fdiv((uint32_t)b, a.by_seg);
+  return {0, b, e - b, i + n, la_segments(a, e - b), i + (i * a.seg < b)};
 }
 // The last of n sequences that `before` holds for, or the first (it holds up to one, if offsets are in order): by a
 // wave, 64 at a time.
@@ -132,8 +135,5 @@ inline int la_wide(const LaArgs& a, int rows, int cols) {
   const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
   return rows <= 128 && cols > 64 && (int64_t)a.slots * a.Hv * ((cols + 127) / 128) * 2 > cus ? 2 : 1;
 }
-
-// tokens i seg of a packed row (la_segment_at)
-inline int la_marks(const LaArgs& a) { return (int)((a.T + a.seg - 1) / a.seg); }
 
 }  // namespace atk

@@ -157,37 +157,38 @@ __global__ __launch_bounds__(256) void la_scan_kernel(LaArgs a, float* s0, float
   } else {
     seq = la_seq(a, n);
   }
-  const int kv = a.K * a.V, i = (int)((blockIdx.x - unit * per.d) * 256 + threadIdx.x) * VW;
+  const int kv = a.K * a.V, segs = seq.segs;
   const bool rev = blockIdx.y;
-  if (i >= kv) return;
-  const int segs = seq.segs;
-  const float* init = a.role[rev].s_first;
-  float run[VW];
+  if (segs == 1) return;
+  for (int i = (int)((blockIdx.x - unit * per.d) * 256 + threadIdx.x) * VW; i < kv; i += (int)per.d * 256 * VW) {
+    const float* init = a.role[rev].s_first;
+    float run[VW];
 #pragma unroll
-  for (int j = 0; j < VW; ++j) run[j] = init ? init[((int64_t)n * a.Hv + h) * kv + i + j] : 0.f;
-  const int64_t step = (int64_t)a.Hv * kv;
-  float* __restrict__ p = (rev ? s1 : s0) + (seq.slot + (rev ? segs - 1 : 0)) * step + (int64_t)h * kv + i;
-  const float* __restrict__ d = decays + ((int64_t)(rev ? a.slots : 0) + seq.slot + (rev ? segs - 1 : 0)) * a.Hv + h;
-  const int64_t ps = rev ? -step : step, ds = rev ? -a.Hv : a.Hv;
-  constexpr int U = 8;  // segments whose loads are in flight together
-  for (int z = 0; z + 1 < segs; z += U) {
-    float t[U][VW], f[U];
-    const int left = segs - 1 - z;
+    for (int j = 0; j < VW; ++j) run[j] = init ? init[((int64_t)n * a.Hv + h) * kv + i + j] : 0.f;
+    const int64_t step = (int64_t)a.Hv * kv;
+    float* __restrict__ p = (rev ? s1 : s0) + (seq.end + (rev ? segs - 2 : 0)) * step + (int64_t)h * kv + i;
+    const float* __restrict__ d = decays + ((int64_t)(rev ? a.ends : 0) + seq.end + (rev ? segs - 2 : 0)) * a.Hv + h;
+    const int64_t ps = rev ? -step : step, ds = rev ? -a.Hv : a.Hv;
+    constexpr int U = 8;  // segments whose loads are in flight together
+    for (int z = 0; z + 1 < segs; z += U) {
+      float t[U][VW], f[U];
+      const int left = segs - 1 - z;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int at = u < left ? u : 0;
-      __builtin_memcpy(t[u], p + at * ps, 4 * VW);
-      f[u] = d[at * ds];
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (u < left) {
-#pragma unroll
-        for (int j = 0; j < VW; ++j) run[j] = fmaf(f[u], run[j], t[u][j]);
-        __builtin_memcpy(p + u * ps, run, 4 * VW);
+      for (int u = 0; u < U; ++u) {
+        const int at = u < left ? u : 0;
+        __builtin_memcpy(t[u], p + at * ps, 4 * VW);
+        f[u] = d[at * ds];
       }
-    p += U * ps;
-    d += U * ds;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (u < left) {
+#pragma unroll
+          for (int j = 0; j < VW; ++j) run[j] = fmaf(f[u], run[j], t[u][j]);
+          __builtin_memcpy(p + u * ps, run, 4 * VW);
+        }
+      p += U * ps;
+      d += U * ds;
+    }
   }
 }
 
@@ -297,26 +298,47 @@ struct LaPlan {
 };
 
 // Tokens of a segment.  Segments of a sequence run at once, each going through its chunks one after the other,
-// for the price of their states: the length is the one with the least time by
-//   chunks of a segment x 8 us where each workgroup has a CU, 10.5 where two share one, in rounds of those
-//   + the states, written and read twice, at 3.5 TB/s,
-// or that of one segment a sequence, which has no states between.  Lengths of packed sequences are on the
-// device; there the average counts, and a segment has at most 1024 tokens or four times the average, lest a long
-// sequence among short ones be left to a workgroup a head (bf16, 128 x 128, 16 heads: one of 8192 and 64 of 64 tokens
-// 663 -> 136 us; the launches that this adds where all are short, 64 of 192 tokens 61 -> 63).  (bf16, 128 x 128, us a
-// call: 2 x 2048 tokens of 16 heads with 128, 192 and 256 tokens a segment 62, 66 and 57; 8192 of 32 heads with 512 and
-// 576 145 and 160; fp32, 64 x 64, 3 sequences, 1021 tokens of 4 heads with 64 and 256 29 and 48.)
+// for the price of their states.  The length is the one with the least time by what was measured, in us:
+//   a step of 64 tokens, states and outputs together, takes 5.5 where each CU has half a workgroup (of 128 columns), 7
+//   where it has one, 10 where it has two, whatever it holds (bf16, 128 key columns; a state of 256 has one a CU and
+//   7.5, one of 64 three and 0.65 of the time; fp16 x 1.75, fp32 x 2.4), more workgroups take turns;
+//   + the states, written and read twice, at 4.4 TB/s, and the launches, 5;
+// or that of one segment a sequence, with no states between and steps of 4, 5.8 and 8.
+//   us a call with so many 64 tokens a segment, the one taken in brackets:
+//     bf16, 128 x 128: 2 x 2048 tokens of 16 heads 2: 54  [4]: 51  8: 60; 8192 of 32 heads 4: 140  [8]: 121  16: 137
+//     16 x 1024 of 16 heads 4: 139  8: 121  [whole]: 96; 256 x 256, 4096 of 8 heads 4: 96  [8]: 87  16: 140
+//     fp32, 128 x 128, 2048 of 8 heads [1]: 41  2: 41  4: 61; fp16, 64 x 100, 7 sequences, 4099 of 16 heads 1: 57  [2]: 53  4: 65
+// Lengths of packed sequences are on the device.  The longest is taken for two and a half times the average, and
+// 0.012 us for each workgroup that finds no segment.  A segment has at most 1024 tokens or four times the average, lest a
+// long sequence among short ones be left to a workgroup a head (bf16, 128 x 128, 16 heads: one of 8192 and 64 of 64
+// tokens, whole 663, in segments 136; where all are short that costs, 300 of 64 tokens, 107 and 112).
 int64_t la_segment_tokens(const atk_linear_attn_args* p) {
   const double cus = device_cu_count() > 0 ? device_cu_count() : 256, n = (double)(p->N > 0 ? p->N : 1);
   const double chunks = p->cu_seqlens ? (double)p->T / 64 / n : (double)((p->T + 63) / 64);
-  const double work = (double)p->Hv * ((p->V + 127) / 128) * n, state = (double)p->K * p->V * 16 / 3.5e6;  // us for 4 passes
+  const double longest = p->cu_seqlens ? chunks * (n < 2.5 ? n : 2.5) : chunks;
+  const int da = la_padded(p->K), w = da <= 128 ? 128 : 64;
+  const double type = (p->dtype == ATK_BF16 ? 1 : p->dtype == ATK_F16 ? 1.75 : 2.4) * (da <= 64 ? 0.65 : 1);
+  const double work = (double)p->Hv * ((p->V + w - 1) / w) * n, states = (double)p->K * p->V * p->Hv * n * 16 / 4.4e6;
+  const auto step = [&](double units, double half, double one, double two) {
+    if (da > 128) return 0.75 * two * ceil(units / cus) * type;
+    const double turns = units / (cus * (da <= 64 ? 3 : 2));
+    return type * (units <= cus / 2 ? half : units <= cus ? one : turns <= 1 ? two : two * (ceil(turns) + turns) / 2);
+  };
   const int64_t all = (p->T + 63) / 64 > 0 ? (p->T + 63) / 64 : 1;
   int64_t best = all;
-  const auto steps = [&](double units) { return units <= cus ? 8.0 : 10.5 * ceil(units / (2 * cus)); };
-  double least = chunks * steps(work);
+  double least = chunks * step(work, 4, 5.8, 8);
+  if (p->cu_seqlens) {
+    const double slowest = longest * step(work < 2 * cus ? work : 2 * cus, 4, 5.8, 8);
+    if (least < slowest) least = slowest;
+  }
   for (int64_t per = 1; per < all && per <= 4096; per += per < 16 ? 1 : per / 8) {
-    const double segs = ceil(chunks / (double)per), units = segs * work;
-    const double t = steps(units) * (double)per + units * state;
+    const double segs = ceil(chunks / (double)per);
+    const double units = segs * work, full = units < 2 * cus ? units : 2 * cus, some = (double)per;
+    double t = step(units, 5.5, 7, 10) * (some < chunks ? some : chunks) + (segs > 1 ? segs * states : 0) + 5;
+    if (p->cu_seqlens) {
+      const double slowest = step(full, 5.5, 7, 10) * (some < longest ? some : longest);
+      t = (t > slowest ? t : slowest) + 0.012 * work * (chunks / some - (segs - 1));
+    }
     if (t < least) {
       least = t;
       best = per;
@@ -358,6 +380,7 @@ LaPlan la_plan(const atk_linear_attn_args* p, bool backward, LaArgs* a, int* rc)
   a->g = p->g; a->cu = p->cu_seqlens; a->n = (int)p->N; a->T = p->T; a->B = p->cu_seqlens ? 1 : p->N;
   for (int i = 0; i < 3; ++i) a->g_s[i] = p->g_stride[i];
   a->slots = (int)slots; a->seg = (int)seg;
+  a->ends = p->cu_seqlens ? (int)((p->T + seg - 1) / seg) : a->slots;
   a->Hk = p->Hk; a->Hv = p->Hv; a->group = p->Hv / p->Hk; a->K = p->K; a->V = p->V;
   a->g_dtype = p->g_dtype; a->fixed = p->fixed_decay; a->scale = p->scale;
   a->by_hk = make_fastdiv((uint32_t)p->Hk); a->by_hv = make_fastdiv((uint32_t)p->Hv); a->by_seg = make_fastdiv((uint32_t)seg);
@@ -369,10 +392,10 @@ LaPlan la_plan(const atk_linear_attn_args* p, bool backward, LaArgs* a, int* rc)
     L.bytes += (floats * 4 + 15) / 16 * 16;
     return q;
   };
-  const size_t state = (size_t)a->slots * a->Hv * a->K * a->V, tokens = (size_t)a->B * a->T;
+  const size_t state = (size_t)a->ends * a->Hv * a->K * a->V, tokens = (size_t)a->B * a->T;
   if (L.split) {
     L.s_fwd = take(state);
-    L.decays = take((size_t)a->slots * a->Hv * (backward ? 2 : 1));
+    L.decays = take((size_t)a->ends * a->Hv * (backward ? 2 : 1));
     if (backward) L.s_rev = take(state);
   }
   if (backward) {
@@ -398,9 +421,11 @@ int la_scan(const LaArgs& a, float* s0, float* s1, const float* decays, int role
   const int64_t kv = (int64_t)a.K * a.V;
   bool vec = kv % 4 == 0;
   for (int i = 0; i < roles; ++i) vec = vec && aligned16(a.role[i].s_first);
-  const int64_t per = (kv + (vec ? 1023 : 255)) / (vec ? 1024 : 256);
-  const int marks = a.cu && la_marks(a) < a.n ? la_marks(a) : 0;
+  int64_t per = (kv + (vec ? 1023 : 255)) / (vec ? 1024 : 256);
+  const int marks = a.cu && a.ends < a.n ? a.ends : 0;
   const int64_t units = (int64_t)(marks ? marks : a.n) * a.Hv;
+  // most sequences of many have one segment: fewer workgroups that find that out
+  if (a.cu && units * per > 8192) per = 8192 / units > 0 ? 8192 / units : 1;
   const int64_t most = kLaBlocks / per > 0 ? kLaBlocks / per : 1;
   for (int64_t u = 0; u < units; u += most) {
     const dim3 g((unsigned)((units - u < most ? units - u : most) * per), (unsigned)roles);

@@ -420,7 +420,7 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
   const float* from = (rev ? z == seq.segs - 1 : z == 0) ? r.s_first : r.s_between;
   bool have = from != nullptr;
   if (have) {
-    const int64_t at = (int64_t)((rev ? z == seq.segs - 1 : z == 0) ? n : slot + (rev ? 1 : -1)) * a.Hv + h;
+    const int64_t at = (int64_t)((rev ? z == seq.segs - 1 : z == 0) ? n : seq.end + z - (rev ? 0 : 1)) * a.Hv + h;
     la_load<RT, NT, swapped>(a, r, full, a0, col, c, g, from + at * a.K * a.V, S);
   } else {
 #pragma unroll
@@ -642,7 +642,7 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
       const float* d = z == seq.segs - 1 ? r.x_last : r.x_between;
       if (d) {
         f32x4 D[RT][NT];
-        la_load<RT, NT, true>(a, r, full, a0, col, c, g, d + ((int64_t)(z == seq.segs - 1 ? n : slot + 1) * a.Hv + h) * a.K * a.V, D);
+        la_load<RT, NT, true>(a, r, full, a0, col, c, g, d + ((int64_t)(z == seq.segs - 1 ? n : seq.end + z) * a.Hv + h) * a.K * a.V, D);
 #pragma unroll
         for (int t = 0; t < RT; ++t)
 #pragma unroll
@@ -709,8 +709,8 @@ __device__ __forceinline__ void la_state(const LaArgs& a, const LaRole& r, const
     z = slot - seq.slot;
   }
   if (z == seq.segs - 1) return;
+  const int64_t end = (int64_t)(seq.end + z) * a.Hv + h;
   z += rev;
-  slot = seq.slot + z;
   const int t0 = z * a.seg, len = seq.len - t0 < a.seg ? seq.len - t0 : a.seg, chunks = (len + CT - 1) / CT;
   const int col0 = tile * W, col = col0 + wave * 16 * NT;
   const int acols = r.AD, ccols = r.CD - col0 < W ? r.CD - col0 : W;
@@ -748,15 +748,15 @@ __device__ __forceinline__ void la_state(const LaArgs& a, const LaRole& r, const
                               rev ? L.d.grown : L.d.rest, rev ? a.scale : 1.f, L.d.all, lane, S);
     __syncthreads();
   }
-  la_store<RT, NT>(a, r, acols == DA && ccols == W, col, c, g, to + ((int64_t)slot * a.Hv + h) * a.K * a.V, S);
-  if (tile == 0 && tid == 0) decays[(int64_t)slot * a.Hv + h] = gdr_decay(total, make_float2(0.f, 0.f));
+  la_store<RT, NT>(a, r, acols == DA && ccols == W, col, c, g, to + end * a.K * a.V, S);
+  if (tile == 0 && tid == 0) decays[end] = gdr_decay(total, make_float2(0.f, 0.f));
 }
 // Roles 0 and, where there is a second row of workgroups, 1 in reverse.
 template <typename T, int DA>
 __global__ __launch_bounds__(256, 2) void la_state_kernel(LaArgs a, LaGrid gr, float* to0, float* to1, float* decays) {
   __shared__ __align__(16) char lds[sizeof(LaStateLds<T, DA>)];
   if (blockIdx.y == 0) la_state<T, DA, false>(a, a.role[0], gr, lds, to0, decays);
-  else la_state<T, DA, true>(a, a.role[1], gr, lds, to1, decays + (int64_t)a.slots * a.Hv);
+  else la_state<T, DA, true>(a, a.role[1], gr, lds, to1, decays + (int64_t)a.ends * a.Hv);
 }
 
 // launch(grid, its place) for workgroups of all tiles, heads and segments, in as many launches as it takes
@@ -788,7 +788,7 @@ int la_run_grads(const LaArgs& a, bool dots, unsigned roles, hipStream_t s) {
 }
 template <typename T, int DA>
 int la_run_states(const LaArgs& a, int roles, float* const* to, float* decays, hipStream_t s) {
-  return la_launches(a, a.cu ? la_marks(a) : a.slots, (a.V + 63) / 64, "la_state_kernel", [&](unsigned n, LaGrid g) {
+  return la_launches(a, a.ends, (a.V + 63) / 64, "la_state_kernel", [&](unsigned n, LaGrid g) {
     hipLaunchKernelGGL((la_state_kernel<T, DA>), dim3(n, (unsigned)roles), dim3(256), 0, s, a, g, to[0], roles > 1 ? to[1] : nullptr, decays);
   });
 }
