@@ -21,6 +21,7 @@ struct LaStepArgs {
 // The decode step is HBM-bound: the state is read and written once, past the caches' replacement
 // (nontemporal), since every other layer has gone through them by the next step.  A new element is stored
 // as soon as its old one is there; only o waits for a reduction over the rows.
+// 64 sequences of 32 heads of 128 x 128: 48.8 us for 270 MB, 5.5 TB/s; one of 16 heads 3.8 us, a launch's own time.
 // A workgroup has NV * VW columns of one head's state: NV threads of VW columns side by side, 256 / NV
 // groups of rows, RPT rows a thread.
 template <typename T, int VW, int NV, int RPT>
@@ -143,7 +144,8 @@ void launch_step_typed(const LaStepArgs& a, hipStream_t s) {
 }
 
 // Segments joined: what each adds to the state becomes the state after it (in reverse, the gradient of the
-// state before it), in place.  A thread has VW elements of a state, all segments of a sequence.
+// state before it), in place.  A thread has VW elements of a state, all segments of a sequence, eight of them in
+// flight.  HBM-bound: 15 states of 32 heads of 128 x 128, 12.6 us for 63 MB, 5 TB/s.
 template <int VW>
 __global__ __launch_bounds__(256) void la_scan_kernel(LaArgs a, float* s0, float* s1, const float* decays, FastDiv per, int first,
                                                       int marks) {
@@ -220,7 +222,8 @@ __global__ __launch_bounds__(256) void la_sum_kernel(LaSumArgs a) {
 
 // The gradient of a log decay: with q_t . dq_t - k_t . dk_t summed from t to the end of the segment, and the
 // inner product of the state there with its gradient.  A wave for each segment and head.  The sums cancel
-// where the decay is strong, so they are in 64 bits.
+// where the decay is strong, so they are in 64 bits.  Latency of a wave's loads and six steps of its sums for each 64
+// tokens: 2 x 2048 tokens of 16 heads, segments of 256, 6.7 us.
 struct LaGateArgs {
   const float* qd; const float* kd; const float* x; void* dg; float* seg_sums;
   int tiles;

@@ -7,6 +7,13 @@
 // 16 of them.  The state stays in the accumulators from chunk to chunk: as it is, it is the next product's
 // second operand.  Rows of a, b and c are staged in LDS in bf16 parts, the next chunk's loads in flight
 // meanwhile; products over tokens read them transposed (ds_read_tr).
+//
+// Measured, bf16: 8192 tokens, 16 and 32 heads of 128 x 128, in 16 segments: states 44 us (100 MB read, 31 written), outputs
+// 87 (134 + 31 and 67).  The matrix units are busy for 10 and 21 us of these; a third of a wave's cycles it waits for
+// memory or LDS, a third for its turn or a result, a quarter it issues vector instructions, most of them the
+// splitting of S, of P and of the decayed c in parts: two workgroups a CU, no resource full.  Without an effect:
+// loads two chunks ahead, eight waves, chunks of 32, other pitches, raised priority.  One part of S and P and two of
+// c's would take 10 % off, for errors of 2^-8 and 2^-16 of each term; they are kept.
 #pragma once
 #include <limits.h>
 
@@ -360,7 +367,7 @@ __device__ __forceinline__ void la_tail(T* to, const float* v, int n) {
 }
 
 // The outputs of one segment, and its last state.  Products that make outputs are taken transposed, so that a
-// lane has 4 NT columns of one token.
+// lane has 4 NT columns of one token.  (Gradients, 2 x 2048 tokens of 16 heads of 128 x 128: dq, dk and dv 83 us.)
 template <typename T, int DA, int NT, int MODE, bool DOTS>
 __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, const LaGrid& gr, char* lds) {
   using Lds = LaLds<T, DA, NT, DOTS>;

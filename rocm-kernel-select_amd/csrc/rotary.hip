@@ -7,7 +7,8 @@
 // HBM-bound: every element is read once and written once.  The angles are products in 64 bits, brought to
 // a part of a turn there (a position of 10^6 has an error of 0.06 in an fp32 product), and sine and cosine
 // are taken once for each token and pair, in fp32, by a workgroup that has all heads of its tokens: the
-// table lies in LDS while they stream through.
+// table lies in LDS while they stream through.  8192 tokens of 32 and 16 heads of 128 columns, bf16: 42 us for
+// 201 MB, 4.8 TB/s (a large copy reaches 5.05); 64 single tokens 3.5 us, a launch's own time.
 #include "atk_common.h"
 
 namespace atk {
