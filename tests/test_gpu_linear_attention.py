@@ -719,3 +719,48 @@ def test_more_heads_than_a_launch(dev):
         size = backward64(*sizes(*few), 1.0, s0.abs(), None, do.abs(), None, size=True)
         for got, w, s, name in zip((dq, dk, dv, dg), want, size, ("dq", "dk", "dv", "dg")):
             close(got[at], w, s, 2 * steps, name)
+
+
+def offsets(lens):
+    return torch.tensor([0] + lens).cumsum(0).tolist()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+def test_many_packed_sequences(dev, dtype):
+    """More sequences than are looked at together, most of them short, some empty; one of many segments among them,
+    one at the end."""
+    import amd_tuned_torch as P
+    torch.manual_seed(11)
+    lens = torch.randint(0, 12, (260,)).tolist()
+    lens[131], lens[-1] = 2100, 1500
+    cu = offsets(lens)
+    t, n = cu[-1] + 3, len(lens)
+    args = make((1, t), 1, 2, 64, 40, dtype, dev)
+    state, dstate = (torch.randn(n, 2, 64, 40, device=dev) for _ in range(2))
+    dout = torch.randn(1, t, 2, 40, device=dev).to(dtype)
+    check_backward(P, args, 0.125, state, cu, dout, dstate, max(lens) // 4 + 64 + 40 + 100)
+
+
+@gpu
+def test_packed_states_of_many_heads(dev):
+    """So many heads that a workgroup joins more than its share of a state: as each sequence by itself, both within
+    their rounding of `size` (here from the kernels, of magnitudes)."""
+    import amd_tuned_torch as P
+    lens = [4000, 1, 2500, 30, 0, 700, 1100, 64, 5, 200, 3, 90] + [7] * 30
+    cu = offsets(lens)
+    args = make((1, cu[-1]), 8, 64, 128, 128, torch.float32, dev)
+    off = torch.tensor(cu, dtype=torch.int32, device=dev)
+    dout, dstate = torch.randn(1, cu[-1], 64, 128, device=dev), torch.randn(len(lens), 64, 128, 128, device=dev)
+    out, grads = run_backward(P, args, 0.1, None, off, dout, dstate)
+    steps = max(lens) / 4 + 256 + 100
+    for i, (a, b) in enumerate(zip(cu, cu[1:])):
+        part = lambda x: x[:, a:b]  # noqa: E731
+        want, _ = run_backward(P, [part(x) for x in args], 0.1, None, None, part(dout), dstate[i:i + 1])
+        size = P.linear_attention(*[part(x) for x in sizes(*args)], 0.1)
+        close(part(out), want.double(), 2 * size.double(), steps, i)
+        if b - a in (1, 2500, 1100):
+            _, want = run_backward(P, [part(x) for x in args], 0.1, None, None, part(dout), dstate[i:i + 1])
+            _, size = run_backward(P, [part(x) for x in sizes(*args)], 0.1, None, None, part(dout).abs(), dstate[i:i + 1].abs())
+            for got, w, m, name in zip(grads[:3], want, size, ("dq", "dk", "dv")):
+                close(part(got), w.double(), 2 * m.double(), 2 * steps + 8, (i, name))
