@@ -404,7 +404,7 @@ LaPlan la_plan(const atk_linear_attn_args* p, bool backward, LaArgs* a, int* rc)
   if (backward) {
     const int da = la_padded(a->V);
     L.a_tiles = (a->V + da - 1) / da;
-    const int w = 64 * la_wide(*a, da, a->K);
+    const int w = 64 * la_wide(*a, da, a->K, 3);
     L.k_tiles = (a->K + w - 1) / w;
     L.n_parts = a->group * L.a_tiles;
     if (L.n_parts > 1)

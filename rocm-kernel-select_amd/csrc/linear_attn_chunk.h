@@ -809,13 +809,13 @@ int la_run_states(const LaArgs& a, int roles, float* const* to, float* decays, h
   }()
 template <typename T>
 int la_launch_out(const LaArgs& a, hipStream_t s) {
-  const int da = la_padded(a.K), nt = la_wide(a, da, a.V);
+  const int da = la_padded(a.K), nt = la_wide(a, da, a.V, 1);
 #define ATK_LA_OUT(DA, NT) la_run_out<T, DA, NT, kLaFwd>(a, s)
   return ATK_LA_TILED(da, nt, ATK_LA_OUT);
 }
 template <typename T>
 int la_launch_grads(const LaArgs& a, bool dots, hipStream_t s) {
-  const int dk = la_padded(a.K), dv = la_padded(a.V), nv = la_wide(a, dk, a.V), nt = la_wide(a, dv, a.K);
+  const int dk = la_padded(a.K), dv = la_padded(a.V), nv = la_wide(a, dk, a.V, 3), nt = la_wide(a, dv, a.K, 3);
   // dv shares the launch where its workgroups are shaped as those of dq and dk, and as many
   const bool one = dk == dv && nv == nt && (a.V + 64 * nt - 1) / (64 * nt) == (a.K + 64 * nt - 1) / (64 * nt) * a.role[0].a_tiles;
   const unsigned roles = one ? 3 : 2;
