@@ -1988,6 +1988,8 @@ def rotary(q: torch.Tensor, k: Optional[torch.Tensor], inv_freq: torch.Tensor, p
         a.rot, a.freq64, a.interleaved, a.inverse = 2 * inv_freq.numel(), int(inv_freq.dtype == torch.float64), interleaved, inverse
         a.dtype, a.scale = _DTYPE_CODE[q.dtype], scale
         blk[2] = key
+    if not tensor and not -1 << 62 <= positions < 1 << 62:  # (the struct's 64 bits would keep its low ones)
+        raise RuntimeError("rotary_embedding: positions must be within 62 bits")
     oq, ok = _dense_like(q), None if k is None else _dense_like(k)
     if oq.numel() == 0 and (ok is None or ok.numel() == 0):
         return oq, ok

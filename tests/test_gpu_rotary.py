@@ -203,3 +203,13 @@ def test_statement_on_the_cpu():
         assert (back - q).abs().max() < 1e-13
         assert torch.autograd.gradcheck(lambda x: R.rotary_embedding_ref(x, None, inv, pos, interleaved, 1.5),
                                         q.clone().requires_grad_())
+
+
+@gpu
+def test_offsets_that_no_position_has(dev):
+    import amd_tuned_torch as P
+    q, f = torch.randn(1, 2, 1, 8, device=dev), torch.ones(4, device=dev)
+    for at in (1 << 64, -(1 << 63), 1 << 62):
+        with pytest.raises(RuntimeError, match="62 bits"):
+            P.rotary_embedding(q, None, f, at)
+    assert P.rotary_embedding(q, None, f, -(1 << 40)).isfinite().all()
