@@ -12,8 +12,9 @@
 // 87 (134 + 31 and 67).  The matrix units are busy for 10 and 21 us of these; a third of a wave's cycles it waits for
 // memory or LDS, a third for its turn or a result, a quarter it issues vector instructions, most of them the
 // splitting of S, of P and of the decayed c in parts: two workgroups a CU, no resource full.  Without an effect:
-// loads two chunks ahead, eight waves, chunks of 32, other pitches, raised priority.  One part of S and P and two of
-// c's would take 10 % off, for errors of 2^-8 and 2^-16 of each term; they are kept.
+// loads two chunks ahead, eight waves, chunks of 32, other pitches, raised priority.  S, P and the decayed c keep all
+// their bits: two parts of S and P towards 16-bit outputs took a call from 143 to 133 us, and rounded results to the
+// wrong side that are within 2^-17 of half way between two values.
 #pragma once
 #include <limits.h>
 
@@ -26,8 +27,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // Tokens of a chunk: 64, or 32 where the parts of 64 rows would not fit LDS twice.
 template <typename T, int DA> inline constexpr int kLaC = kParts<T> == 1 ? 64 : 32;
-// parts of what is multiplied towards outputs of T; gradients of decays are fp32, from three
-template <typename T, bool DOTS> inline constexpr int kLaOut = DOTS || sizeof(T) == 4 ? 3 : 2;
+// parts of fp32 factors (S, P, the decayed c): all their bits, also towards 16-bit outputs
+constexpr int kLaOut = 3;
 
 // Running sum over the wave of v / ln 2 in 64 bits, as two floats each; lane 63's sum in *last.
 template <int CTRL, int ROWS>
@@ -306,7 +307,7 @@ __device__ __forceinline__ void la_update(const __bf16* b, int b_pitch, int b_pa
     for (int x = 0; x < NT; ++x) S[t][x] *= all;
 #pragma unroll
   for (int s = 0; s < HS; ++s) {
-    uint4 cw[NT][3];
+    uint4 cw[NT][kLaOut];
     f32x4 w[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) w[u] = *reinterpret_cast<const f32x4*>(f + 32 * s + 16 * u + 4 * g) * factor;
@@ -319,7 +320,7 @@ __device__ __forceinline__ void la_update(const __bf16* b, int b_pitch, int b_pa
       la_values<NP>(cf, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= w[e / 4][e & 3];
-      la_split<3>(v, cw[x]);
+      la_split<kLaOut>(v, cw[x]);
     }
 #pragma unroll
     for (int t = 0; t < RT; t += 4) {
@@ -332,7 +333,7 @@ __device__ __forceinline__ void la_update(const __bf16* b, int b_pitch, int b_pa
 #pragma unroll
         for (int x = 0; x < NT; ++x) y[u][x] = S[t + u][x];
       }
-      la_mma<4, NT, NP, 3>(bf, cw, y);
+      la_mma<4, NT, NP, kLaOut>(bf, cw, y);
 #pragma unroll
       for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -348,7 +349,7 @@ struct LaLds {
   __bf16 a[NP][CT][PA];
   __bf16 b[NP][CT][PA];
   __bf16 c[NP][CT][PC];
-  uint4 p[PF][kLaOut<T, DOTS>][64];
+  uint4 p[PF][kLaOut][64];
   LaDecays<CT> d;
   union {
     float dots[DOTS ? 4 : 1][CT];
@@ -372,7 +373,7 @@ template <typename T, int DA, int NT, int MODE, bool DOTS>
 __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, const LaGrid& gr, char* lds) {
   using Lds = LaLds<T, DA, NT, DOTS>;
   constexpr int NP = Lds::NP, CT = Lds::CT, W = Lds::W, RT = DA / 16, KS = DA / 32, MT = CT / 16, HS = CT / 32;
-  constexpr int OP = kLaOut<T, DOTS>, OW = 4 * NT;
+  constexpr int OP = kLaOut, OW = 4 * NT;
   constexpr bool rev = la_reverse(MODE), swapped = la_swapped(MODE);
   Lds& L = *reinterpret_cast<Lds*>(lds);
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
