@@ -30,8 +30,8 @@ struct LaRole {
   float* s_last;                           // where the last segment's state goes, or null
   void* out;                               // T (B, T, heads of out, CD), or
   float* parts;                            // fp32 sums [head of the group * a_tiles + a tile][B T][Hk][CD]
-  float* dots;                             // [tile][Hv][B T]: e_i . out_i over the tile's columns
-  const float* x_last; const float* x_between; float* x_out;  // [tile][slot][Hv]: sum of S and the other direction's state
+  float* dots;                             // [tile][Hv][B T]: e_i . out_i over the tile's columns, but for j = i
+  const float* x_last; const float* x_between; float* x_out;  // [tile][slot][Hv]: sum of S, but for the last token, and the other direction's state
 };
 
 struct LaArgs {

@@ -220,9 +220,10 @@ __global__ __launch_bounds__(256) void la_sum_kernel(LaSumArgs a) {
   }
 }
 
-// The gradient of a log decay: with q_t . dq_t - k_t . dk_t summed from t to the end of the segment, and the
-// inner product of the state there with its gradient.  A wave for each segment and head.  The sums cancel
-// where the decay is strong, so they are in 64 bits.  Latency of a wave's loads and six steps of its sums for each 64
+// The gradient of a log decay: q_t . dq_t - k_t . dk_t, both without the token's product with itself, which has no
+// decay, summed from t to the end of the segment, and the inner product of the state there with its gradient.  A
+// wave for each segment and head.  What is left has the decays as the sum has, but cancels where weak ones stand
+// beside strong ones, so the sums are in 64 bits.  Latency of a wave's loads and six steps of its sums for each 64
 // tokens: 2 x 2048 tokens of 16 heads, segments of 256, 6.7 us.
 struct LaGateArgs {
   const float* qd; const float* kd; const float* x; void* dg; float* seg_sums;

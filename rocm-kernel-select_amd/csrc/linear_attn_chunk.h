@@ -351,6 +351,7 @@ struct LaLds {
   __bf16 c[NP][CT][PC];
   uint4 p[PF][kLaOut][64];
   LaDecays<CT> d;
+  float self[DOTS ? CT : 1];  // each token's product with itself, scaled: P's diagonal
   union {
     float dots[DOTS ? 4 : 1][CT];
     int bad[W];  // (forward) each column's first token whose c is not finite
@@ -368,7 +369,11 @@ __device__ __forceinline__ void la_tail(T* to, const float* v, int n) {
 }
 
 // The outputs of one segment, and its last state.  Products that make outputs are taken transposed, so that a
-// lane has 4 NT columns of one token.  (Gradients, 2 x 2048 tokens of 16 heads of 128 x 128: dq, dk and dv 83 us.)
+// lane has 4 NT columns of one token.  (Gradients, 2 x 2048 tokens of 16 heads of 128 x 128: dq, dk and dv 88 us.)
+// DOTS: a token's term with itself has no decay, so it is no part of a decay's gradient.  It is in q . dq and in
+// k . dk alike, and 2^-24 of it would stay of their difference, where exp(g) leaves less of that.  So the dots
+// are taken before it is added, of the triangle without its diagonal; and of what the state at the segment's
+// end and the gradient of it have in common, without the last token's own term, the one without a decay there.
 template <typename T, int DA, int NT, int MODE, bool DOTS>
 __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, const LaGrid& gr, char* lds) {
   using Lds = LaLds<T, DA, NT, DOTS>;
@@ -446,7 +451,11 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
     ta.template put<NP>(&L.a[0][0][0], Lds::PA, CT * Lds::PA, rows, acols);
     tb.template put<NP>(&L.b[0][0][0], Lds::PA, CT * Lds::PA, rows, acols);
     tc.template put<NP, MODE == kLaFwd>(&L.c[0][0][0], Lds::PC, CT * Lds::PC, rows, ccols, at, L.bad, &L.spoilt);
-    if (wave == 3) L.d.put(gdr_gate<T>(tg, a.g_dtype), lane, rows);
+    if (wave == 3) {
+      L.d.put(gdr_gate<T>(tg, a.g_dtype), lane, rows);
+      // (here S is read once more, for that inner product)
+      if (DOTS && MODE == kLaDq && k + 1 == chunks && lane == rows - 1) L.d.rest[lane] = 0.f;
+    }
     __syncthreads();
     // scale lower(A B^T * D), or upper in reverse, as the results of its transpose: a lane has 8 of 32 columns
     // of a row, one fragment.  The fragments within the triangle are shared out to the waves.
@@ -478,7 +487,7 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
       }
       const int out = 16 * m + c;
       const float2 go = L.d.gd[out];
-      float v[8];
+      float v[8], self = 0.f;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         float4 gi[2];
@@ -490,9 +499,11 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
           float p = y[u][0][e] * gdr_decay(rev ? i : go, rev ? go : i) * a.scale;
           asm("" : "+v"(p));  // (else a branch for each)
           const int in = 32 * s + 16 * u + 4 * g + e;
-          v[4 * u + e] = (rev ? in >= out : in <= out) ? p : 0.f;
+          if (DOTS) self = in == out ? p : self;
+          v[4 * u + e] = (DOTS ? rev ? in > out : in < out : rev ? in >= out : in <= out) ? p : 0.f;
         }
       }
+      if (DOTS && s == m >> 1 && g == c >> 2) L.self[out] = self;
       uint4 w[OP];
       la_split<OP>(v, w);
 #pragma unroll
@@ -599,7 +610,19 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
         }
         dot += __shfl_xor(dot, 16, 64);
         dot += __shfl_xor(dot, 32, 64);
-        if (g == 0) L.dots[wave][row] = dot;
+        // (of the segment's last token k . dk has nothing but that term)
+        if (g == 0) L.dots[wave][row] = MODE == kLaDk && k == 0 && row == rows - 1 ? 0.f : dot;
+        const float self = L.self[row];
+        uint4 cw[NP];
+        float own[8];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+          cw[p] = make_uint4(0, 0, 0, 0);
+          __builtin_memcpy(&cw[p], __builtin_assume_aligned(&L.c[p][row][oc], 2 * OW), 2 * OW);
+        }
+        la_values<NP>(cw, own);
+#pragma unroll
+        for (int q = 0; q < OW; ++q) o[q] = fmaf(self, own[q], o[q]);
       }
       if (row < rows) {
         const int64_t tok = seq.batch * a.T + first + at + row;

@@ -1,5 +1,5 @@
 """Linear attention where fewer bits than an fp32 product's would show: results next to a border between two values
-of a 16-bit type."""
+of a 16-bit type, gradients of strong decays."""
 from __future__ import annotations
 
 import pytest
@@ -49,3 +49,102 @@ def test_results_next_to_a_border(dev, later, dtype):
         leaf = leaves[name].requires_grad_()
         got, = torch.autograd.grad(P.linear_attention(q, k, v, g, 1.0), leaf, do)
         assert got[0, later + (1 if name == "q" else 0), 0, 0].item() == up, name
+
+
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def decays64(q, k, v, g, scale, state, cu, dout, dstate, size=False):
+    """The gradient of every token's log decay (1, t, heads) by the formula, exp(g_t) <S_{t-1}, dS_t>, in 64 bits.  With
+    `size`, of magnitudes, the sum of what it is the sum of: of each token s from t on, q_s . dq_s and k_s . dk_s
+    without the token's product with itself (what they have from other tokens and states, which has decays),
+    and the end's inner product without the last token's own term."""
+    rep = v.shape[2] // q.shape[2]
+    q, k = (x.double().repeat_interleave(rep, dim=2) for x in (q, k))
+    v, dout, g = v.double(), dout.double(), g.double().expand(v.shape[:3])
+    dg = torch.zeros_like(g)
+    for i, (a, b) in enumerate(zip(cu, cu[1:])):
+        S = torch.zeros(v.shape[2], q.shape[3], v.shape[3], dtype=torch.float64, device=v.device) if state is None else state[i].double()
+        seen = []                                                # decayed states, before each token's own term
+        for t in range(a, b):
+            seen.append(S * g[0, t].exp()[:, None, None])
+            S = seen[-1] + k[0, t][..., None] * v[0, t][..., None, :]
+        dS = torch.zeros_like(S) if dstate is None else dstate[i].double()
+        total = (dS * seen[-1]).sum((-1, -2)) if seen else 0
+        for t in range(b - 1, a - 1, -1):
+            if size:
+                total = total + scale * (q[0, t][..., None] * seen[t - a] * dout[0, t][..., None, :]).sum((-1, -2))
+                total = total + ((k[0, t][..., None] * dS * v[0, t][..., None, :]).sum((-1, -2)) if t < b - 1 else 0)
+                dg[0, t] = total
+            dS = dS + scale * q[0, t][..., None] * dout[0, t][..., None, :]
+            if not size:
+                dg[0, t] = (dS * seen[t - a]).sum((-1, -2))
+            dS = dS * g[0, t].exp()[:, None, None]
+    return dg
+
+
+def decay_case(dev, dtype, cu, hk, hv, dk, dv):
+    gen = torch.Generator().manual_seed(len(cu))
+    r = lambda *s: torch.randn(*s, generator=gen).to(dev)  # noqa: E731
+    t, n = cu[-1], len(cu) - 1
+    return [r(1, t, h, d).to(dtype) for h, d in ((hk, dk), (hk, dk), (hv, dv))], r(1, t, hv, dv).to(dtype), r(n, hv, dk, dv), r(n, hv, dk, dv)
+
+
+def decay_gradient(P, qkv, g, state, cu, dout, dstate):
+    g = g.clone().requires_grad_()
+    off = torch.tensor(cu, dtype=torch.int32, device=g.device) if len(cu) > 2 else None
+    out, S = P.linear_attention(*qkv, g, 0.125, initial_state=state, return_final_state=True, cu_seqlens=off)
+    ends, grads = ([out, S], [dout, dstate]) if dstate is not None else ([out], [dout])
+    return torch.autograd.grad(ends, g, grads)[0]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("cu,hk,hv,dk,dv", [((0, 256), 2, 2, 64, 64), ((0, 1), 1, 2, 32, 32), ((0, 130, 131, 131, 700), 2, 4, 128, 100),
+                                            ((0, 150), 1, 1, 256, 264), ((0, 2100), 1, 2, 64, 128)], ids=str)
+def test_gradients_of_strong_decays(dev, cu, hk, hv, dk, dv, dtype):
+    """exp(g) is all that is left of a decay's gradient, so it is right by that measure, not by that of products
+    without a decay.  Tolerances: the roundings that follow each other, in number as for the other gradients,
+    2 (T / 4 + dim_k + dim_v + 100), of 2^-24 of the magnitudes, which have the decays too.  And against its own
+    size, in the 2-norm: a dot product of d columns and a chunk's tokens has sqrt(d_k + d_v + 64) roundings of 2^-24 by
+    chance, so at most 24 of its own size, which is a token's gradient's; from t on 2 T of these are added, so a
+    token's is off by sqrt(2 T) 24 2^-24 of it or less, 2^-13 for T up to 4096; a head's sum is off by as many T
+    times over, sqrt(T) more for terms of random sign, and so is up to sqrt(T) 2^-13, at 256 tokens 2^-9."""
+    import amd_tuned_torch as P
+    qkv, dout, state, dstate = decay_case(dev, dtype, cu, hk, hv, dk, dv)
+    t = max(b - a for a, b in zip(cu, cu[1:]))
+    steps = 2 * (t / 4 + dk + dv + 100)
+    mag = [x.abs() for x in (*qkv, dout, state, dstate)]
+    for s0, s1, m0, m1 in ((state, dstate, mag[4], mag[5]), (None, None, None, None)):
+        for rate in (-0.1, -2.0, -5.0, -10.0, -20.0, -40.0):
+            for fixed in (False, True):
+                g = torch.full((hv,) if fixed else (1, cu[-1], hv), rate, device=dev)
+                got = decay_gradient(P, qkv, g, s0, cu, dout, s1)
+                want = decays64(*qkv, g, 0.125, s0, cu, dout, s1)
+                size = decays64(*mag[:3], g, 0.125, m0, cu, mag[3], m1, size=True)
+                if fixed:
+                    want, size = want.sum((0, 1)), size.sum((0, 1))
+                assert ((got.double() - want).abs() <= steps * 2.0 ** -24 * size + 1e-37).all(), (rate, fixed)
+                if not fixed or t <= 256:
+                    near = 2.0 ** (-9 if fixed else -13) * want.norm()
+                    assert (got.double() - want).norm() <= near, (rate, fixed, ((got.double() - want).norm() / want.norm()).item())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_gradients_of_decays_of_all_strengths(dev, dtype):
+    """Weak and strong decays side by side, tokens that forget everything among them: within the roundings of the
+    terms that have decays."""
+    import amd_tuned_torch as P
+    cu = (0, 500, 770)
+    qkv, dout, state, dstate = decay_case(dev, dtype, cu, 1, 4, 64, 64)
+    gen = torch.Generator().manual_seed(9)
+    g = -40 * torch.rand(1, cu[-1], 4, generator=gen).to(dev) ** 4
+    g[:, ::90, 1] = float("-inf")
+    g[:, :, 2] = -30
+    g[:, 400:, 2] = -0.01
+    got = decay_gradient(P, qkv, g, state, cu, dout, dstate)
+    want = decays64(*qkv, g, 0.125, state, cu, dout, dstate)
+    size = decays64(*[x.abs() for x in qkv], g, 0.125, state.abs(), cu, dout.abs(), dstate.abs(), size=True)
+    assert ((got.double() - want).abs() <= 2 * (500 / 4 + 228) * 2.0 ** -24 * size + 1e-37).all()
+    assert got[:, ::90, 1].eq(0).all()
