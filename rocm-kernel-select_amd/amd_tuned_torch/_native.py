@@ -2127,8 +2127,10 @@ def _linear_block(q, k, v, g, scale, initial_state, cu_seqlens):
     blk[6] = None
     if blk[2] != key:
         n = _linear_check(q, k, v, g, initial_state, cu_seqlens)
-        fits = [t.stride(3) == 1 and t.stride(1) < 1 << 22 for t in (q, k, v)]  # (the kernels' offsets within 64 tokens)
-        if not all(fits) or (g.dim() == 3 and g.stride(1) >= 1 << 22) or not (
+        # the kernels' offsets within 64 tokens; an axis of one token may have any stride, also after a copy
+        near = lambda t: t.shape[1] == 1 or t.stride(1) < 1 << 22  # noqa: E731
+        fits = [t.stride(3) == 1 and near(t) for t in (q, k, v)]
+        if not all(fits) or (g.dim() == 3 and not near(g)) or not (
                 (initial_state is None or initial_state.is_contiguous()) and (cu_seqlens is None or cu_seqlens.is_contiguous())):
             q, k, v = (t if ok else t.contiguous() for t, ok in zip((q, k, v), fits))
             g = g.contiguous()
@@ -2140,6 +2142,8 @@ def _linear_block(q, k, v, g, scale, initial_state, cu_seqlens):
         a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
         a.fixed_decay = int(g.dim() == 1)
         a.g_stride[:] = (0, 0, g.stride(0)) if g.dim() == 1 else g.stride()
+        if q.shape[1] == 1:
+            a.q_stride[1] = a.k_stride[1] = a.v_stride[1] = a.g_stride[1] = 0
         a.N, a.T, a.Hk, a.Hv, a.K, a.V = n, q.shape[1], q.shape[2], v.shape[2], q.shape[3], v.shape[3]
         a.dtype, a.g_dtype = _DTYPE_CODE[q.dtype], _DTYPE_CODE[g.dtype]
         a.scale = scale

@@ -377,8 +377,8 @@ LaPlan la_plan(const atk_linear_attn_args* p, bool backward, LaArgs* a, int* rc)
   if ((double)p->K * p->V >= (double)(1 << 29) || slots * p->Hv > 2147483000.0 || slots > 2147483000.0 || (p->cu_seqlens ? 1.0 : (double)p->N) * (double)p->T > 1e12)
     return *rc = fail(ATK_UNSUPPORTED, "linear attention: a state of 2^29 elements or more, or too many sequences and heads"), L;
   *a = LaArgs{};
-  // the kernels' loads of 64 tokens have offsets of 32 bits
-  for (const int64_t* st : {p->q_stride, p->k_stride, p->v_stride, p->g_stride})
+  // the kernels' loads of 64 tokens have offsets of 32 bits; of one token there is no offset
+  if (p->T > 1) for (const int64_t* st : {p->q_stride, p->k_stride, p->v_stride, p->g_stride})
     if (st[1] < 0 || st[1] >= (1 << 22)) return *rc = fail(ATK_UNSUPPORTED, "linear attention: tokens of 2^22 elements or more apart"), L;
   if ((int64_t)p->Hv * p->V >= (1 << 22) && backward) return *rc = fail(ATK_UNSUPPORTED, "linear attention backward: 2^22 value columns or more"), L;
   a->g = p->g; a->cu = p->cu_seqlens; a->n = (int)p->N; a->T = p->T; a->B = p->cu_seqlens ? 1 : p->N;
