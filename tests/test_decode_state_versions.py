@@ -16,7 +16,22 @@ def linear(P, dev):
             lambda cache: P.linear_attention_update(*token, cache), r(2, 2, 16, 16))
 
 
-OPERATORS = {"linear attention": (linear, "linear_attn_update", "_linear_update_check")}
+def delta(P, dev):
+    r = lambda *s: torch.randn(*s, device=dev)  # noqa: E731
+    token = [r(2, 1, 16), torch.nn.functional.normalize(r(2, 1, 16), dim=-1), r(2, 2, 16), -r(2, 2).abs(), r(2, 2).sigmoid()]
+    return (lambda cache: P.gated_delta_rule(*[x[:, None] for x in token[:2]], token[2][:, None].requires_grad_(),
+                                             *[x[:, None] for x in token[3:]], initial_state=cache),
+            lambda cache: P.gated_delta_rule_update(*token, cache), r(2, 2, 16, 16))
+
+
+OPERATORS = {"linear attention": (linear, "_linear_update_check"), "gated delta rule": (delta, "_delta_update_check")}
+
+
+class Launches:
+    """A library of which every call succeeds and does nothing."""
+
+    def __getattr__(self, name):
+        return lambda *a: 0
 
 
 @pytest.mark.parametrize("name", OPERATORS)
@@ -24,9 +39,9 @@ def test_a_step_counts_as_an_operation_in_place(name, monkeypatch):
     """Without a GPU: the call with the launch left out.  A tensor of inference mode has no version."""
     import amd_tuned_torch as P
     from amd_tuned_torch import _native as nat
-    make, _, check = OPERATORS[name]
-    nat.load()
+    make, check = OPERATORS[name]
     monkeypatch.setattr(nat, check, lambda *a: None)
+    monkeypatch.setattr(nat, "lib", Launches)
     monkeypatch.setattr(nat, "_on", lambda device, fn, *a: 0)
     monkeypatch.setattr(nat, "_stream", lambda t: None)
     _, step, cache = make(P, "cpu")
