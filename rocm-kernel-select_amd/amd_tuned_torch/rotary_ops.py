@@ -6,7 +6,8 @@
 
 With angle = position * inv_freq[i], pair i's (a, b) become scale * (a cos - b sin, a sin + b cos).  Pair i
 is columns i and i + rot / 2, or 2 i and 2 i + 1 with `interleaved`, rot = 2 * len(inv_freq); columns from
-rot on are copied.  Angles are products in 64 bits, so far positions lose nothing.  `rotary_embedding` is
+rot on are copied.  Angles are products in 64 bits with what their rounding leaves, so far positions lose nothing:
+any in 62 bits.  `rotary_embedding` is
 differentiable in q and k any number of times: the way back is the same by the opposite angle.
 """
 from __future__ import annotations
@@ -50,12 +51,34 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[str] =
     return inv_freq.to(device), scale
 
 
+def _product(a, b):
+    """(a * b in float64, what its rounding left), both exact: by halves of 26 bits."""
+    halves = []
+    for x in (a, b):
+        high = 134217729.0 * x
+        high = high - (high - x)
+        halves += [high, x - high]
+    p = a * b
+    ah, al, bh, bl = halves
+    return p, ((ah * bh - p) + ah * bl + al * bh) + al * bl
+
+
+def _part_of_turn(positions, inv_freq):
+    """positions * inv_freq in turns, without whole ones, in float64: as the kernel takes it."""
+    low = positions & 2047
+    p, rest = _product((positions - low).double(), inv_freq)
+    turns, left = _product(p, torch.full((), 0.15915494309189535, dtype=torch.float64, device=p.device))   # 1 / (2 pi)
+    left = left + (p * -9.839338337591243e-18 + (rest + low.double() * inv_freq) * 0.15915494309189535)    # and its next 53 bits
+    part = (turns - turns.round()) + left
+    return part - part.round()
+
+
 def rotary_embedding_ref(q, k, inv_freq, positions=0, interleaved=False, scale=1.0, inverse=False):
-    """rotary_embedding in torch operations (angles in float64, the rest in float32 or wider, rounded once)."""
+    """rotary_embedding in torch operations (parts of a turn in float64, the rest in float32 or wider, rounded once)."""
     acc = torch.promote_types(q.dtype, torch.float32)
     if not isinstance(positions, torch.Tensor):
         positions = positions + torch.arange(q.shape[-3], device=q.device)
-    angle = positions.expand(q.shape[:-2])[..., None, None].double() * inv_freq.double()
+    angle = 2 * math.pi * _part_of_turn(positions.expand(q.shape[:-2])[..., None, None].long(), inv_freq.double())
     cos, sin = (scale * torch.cos(angle)).to(acc), (scale * torch.sin(angle)).to(acc)
     sin = -sin if inverse else sin
     rot = 2 * inv_freq.shape[0]

@@ -4,9 +4,9 @@
 // Pair i is columns i and i + rot / 2 (halves) or 2 i and 2 i + 1 (interleaved); columns from rot on are
 // copied.  The way back, the gradient, is the same by the opposite angle.
 //
-// HBM-bound: every element is read once and written once.  The angles are products in 64 bits, brought to
-// a part of a turn there (a position of 10^6 has an error of 0.06 in an fp32 product), and sine and cosine
-// are taken once for each token and pair, in fp32, by a workgroup that has all heads of its tokens: the
+// HBM-bound: every element is read once and written once.  The angles are products in 64 bits, with what their
+// rounding leaves, brought to a part of a turn there (a position of 10^6 has an error of 0.06 in an fp32 product, one
+// of 2^40 7e-5 in a product rounded to 64 bits), and sine and cosine are taken once for each token and pair by a workgroup that has all heads of its tokens: the
 // table lies in LDS while they stream through.  8192 tokens of 32 and 16 heads of 128 columns, bf16: 42 us for
 // 201 MB, 4.8 TB/s (a large copy reaches 5.05); 64 single tokens 3.5 us, a launch's own time.
 #include "atk_common.h"
@@ -36,6 +36,19 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   return r;
 }
 
+// position * freq in turns, without whole ones: within 2^-40 of a turn for any position and freq up to 1, 2^-52 of the turns of
+// nearer ones.  The position's last 11 bits are apart, so the rest has no rounding in 64 bits; products keep what
+// theirs leaves, and 1 / (2 pi) has 107 bits.  (Contracted, a product would be taken with that twice.)
+__device__ __forceinline__ double part_of_turn(int64_t pos, double freq) {
+#pragma clang fp contract(off)
+  constexpr double kTurn = 0.15915494309189535, kTurnRest = -9.839338337591243e-18;
+  const int64_t low = pos & 2047;
+  const double high = (double)(pos - low), p = high * freq, rest = fma(high, freq, -p) + (double)low * freq;
+  const double turns = p * kTurn, left = fma(p, kTurn, -turns) + (p * kTurnRest + rest * kTurn);
+  const double part = (turns - rint(turns)) + left;
+  return part - rint(part);
+}
+
 // V: columns of a vector of pairs (of halves: V of each), CV of one that is copied.  An item is a vector of
 // a head: pairs first, then columns to copy.  The last of either ends where they end, so it may repeat some
 // columns of the one before it, with the same values.
@@ -56,9 +69,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int64_t first
       pos = a.pos64 ? static_cast<const int64_t*>(a.pos)[at] : (int64_t)static_cast<const int*>(a.pos)[at];
     }
     const double f = a.freq64 ? static_cast<const double*>(a.freq)[j] : (double)static_cast<const float*>(a.freq)[j];
-    const double turns = (double)pos * f * 0.15915494309189535;
     float s, c;
-    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
+    sincospif(2.f * (float)part_of_turn(pos, f), &s, &c);
     table[k * 2 * a.R + j] = a.scale * c;
     table[k * 2 * a.R + a.R + j] = a.scale * (a.inverse ? -s : s);
   }
