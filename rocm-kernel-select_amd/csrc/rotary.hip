@@ -69,10 +69,11 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a, int64_t first
       pos = a.pos64 ? static_cast<const int64_t*>(a.pos)[at] : (int64_t)static_cast<const int*>(a.pos)[at];
     }
     const double f = a.freq64 ? static_cast<const double*>(a.freq)[j] : (double)static_cast<const float*>(a.freq)[j];
-    float s, c;
-    sincospif(2.f * (float)part_of_turn(pos, f), &s, &c);
-    table[k * 2 * a.R + j] = a.scale * c;
-    table[k * 2 * a.R + a.R + j] = a.scale * (a.inverse ? -s : s);
+    // (an angle rounded to fp32 is off by up to 2^-23.3, and what comes of it by more than the fp32 products that follow)
+    double s, c;
+    sincospi(2. * part_of_turn(pos, f), &s, &c);
+    table[k * 2 * a.R + j] = (float)(a.scale * c);
+    table[k * 2 * a.R + a.R + j] = (float)(a.scale * (a.inverse ? -s : s));
   }
   __syncthreads();
   const int rot = 2 * a.R, rest = a.D - rot;

@@ -59,3 +59,18 @@ def test_far_positions(dev, dtype):
         if -(1 << 62) <= p:
             got = P.rotary_embedding(q[:1], None, inv.to(dev), p)[0, 0].cpu().double()
             assert ((got - torch.cat((c, s))).abs() <= 2.0 ** -20 + (2.0 ** -8 if dtype == torch.bfloat16 else 0)).all(), p
+
+
+@gpu
+def test_sine_and_cosine_are_rounded_once(dev):
+    """A pair of (1, 0) becomes (scale cos, scale sin), whose products with 1 and 0 are exact in fp32: within half a
+    step of fp32, 2^-24 of the value, and 2 pi 2^-40 of scale where the value is small."""
+    import amd_tuned_torch as P
+    inv = freqs()
+    positions = list(range(0, 4000, 37)) + [10 ** 6 + i for i in range(50)] + FAR
+    q = torch.cat((torch.ones(len(positions), 1, 16), torch.zeros(len(positions), 1, 16)), -1).to(dev)
+    want = torch.cat(exact(positions, inv), -1)
+    for scale in (1.0, 1.25):                                               # (both exact in fp32)
+        got = P.rotary_embedding(q, None, inv.to(dev), torch.tensor(positions, device=dev), scale=scale)[:, 0].cpu().double()
+        off = (got - scale * want).abs() - 2.0 ** -24 * scale * want.abs() - scale * 2 * math.pi * 2.0 ** -40
+        assert off.max() <= 0, off.max().item()
