@@ -99,10 +99,8 @@ class RotaryFn(torch.autograd.Function):
     def forward(ctx, q, k, inv_freq, positions, interleaved, scale, inverse):
         tensor = isinstance(positions, torch.Tensor)
         ctx.how = None if tensor else positions, interleaved, scale, inverse
-        ctx.key = k is not None
         ctx.save_for_backward(inv_freq, positions if tensor else None)
         ctx.set_materialize_grads(False)
-        ctx.shapes = q.shape, None if k is None else k.shape
         oq, ok = _native.rotary(q, k, inv_freq, positions, interleaved, scale, inverse)
         return oq if k is None else (oq, ok)
 
