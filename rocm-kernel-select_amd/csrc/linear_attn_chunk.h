@@ -52,6 +52,28 @@ __device__ __forceinline__ float2 la_running(float v, float2* last) {
   return r;
 }
 
+// v[0..N) as NP parts of N bf16 each; WIDE: of any fp32 value.  Those from 3.39e38 on round up to infinity in bf16, so
+// there the first part is bf16's largest value, and the others have what is left of it.
+template <int NP, int N, bool WIDE, typename P>
+__device__ __forceinline__ void la_parts(const float* v, P (&out)[NP]) {
+  if constexpr (WIDE && NP > 1) {
+    constexpr float kMost = 3.3895313892515355e38f;
+    float rest[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const __bf16 h = (__bf16)fminf(fmaxf(v[i], -kMost), kMost);
+      out[0][i] = h;
+      rest[i] = v[i] - (float)h;
+    }
+    P more[NP - 1];
+    split_parts<NP - 1, N>(rest, more);
+#pragma unroll
+    for (int p = 1; p < NP; ++p) out[p] = more[p - 1];
+  } else {
+    split_parts<NP, N>(v, out);
+  }
+}
+
 // ROWS x W elements in registers on their way to LDS, vectors of 16 bytes: a thread's loads all in flight at
 // once, without branches.  Rows and columns that are not there are loaded from where there are some, and
 // become zeros when they are put down.
@@ -74,8 +96,6 @@ struct LaTile {
       __builtin_memcpy(&r[i], reinterpret_cast<const char*>(p - back) + (size_t)off, 16);  // element alignment only
     }
   }
-  // fp32 values that round up to infinity in bf16 have no parts either: raised by 2^-8 they are infinite
-  static __device__ __forceinline__ float raised(float v) { return sizeof(T) == 4 ? v * 1.00390625f : v; }
   // NaN or not zero where one of a vector's elements is not finite
   static __device__ __forceinline__ float spoilt_by(uint4 v) {
     float z = 0.f;
@@ -83,7 +103,7 @@ struct LaTile {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if constexpr (sizeof(T) == 4) {
-        z = fmaf(raised(__uint_as_float(w[j])), 0.f, z);
+        z = fmaf(__uint_as_float(w[j]), 0.f, z);
       } else if constexpr (__is_same(T, __bf16)) {
         typedef __bf16 b2 __attribute__((ext_vector_type(2)));
         z = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, w[j]), b2{0, 0}, z, false);
@@ -125,7 +145,7 @@ struct LaTile {
           __builtin_memcpy(e, &r[i], 16);
 #pragma unroll
           for (int j = 0; j < V; ++j) {
-            if (raised(to_f32(e[j])) * 0.f != 0.f) {
+            if (to_f32(e[j]) * 0.f != 0.f) {
               atomicMin(&bad[c + j], from + row0 + i * STEP);
               *spoilt = 1;
               e[j] = from_f32<T>(0.f);
@@ -148,7 +168,7 @@ struct LaTile {
         __builtin_memcpy(e, &r[i], 16);
 #pragma unroll
         for (int j = 0; j < V; ++j) f[j] = to_f32(e[j]);
-        split_parts<NP, V>(f, parts);
+        la_parts<NP, V, sizeof(T) == 4>(f, parts);
 #pragma unroll
         for (int q = 0; q < NP; ++q) __builtin_memcpy(to + i * STEP * pitch + q * part, &parts[q], V * 2);
       }
@@ -190,10 +210,10 @@ __device__ __forceinline__ void la_values(const uint4 (&f)[NP], float (&v)[8]) {
     }
   }
 }
-template <int NP>
+template <int NP, bool WIDE>
 __device__ __forceinline__ void la_split(const float (&v)[8], uint4 (&f)[NP]) {
   bf16x8 parts[NP];
-  split_parts<NP, 8>(v, parts);
+  la_parts<NP, 8, WIDE>(v, parts);
 #pragma unroll
   for (int p = 0; p < NP; ++p) f[p] = __builtin_bit_cast(uint4, parts[p]);
 }
@@ -320,7 +340,7 @@ __device__ __forceinline__ void la_update(const __bf16* b, int b_pitch, int b_pa
       la_values<NP>(cf, v);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] *= w[e / 4][e & 3];
-      la_split<kLaOut>(v, cw[x]);
+      la_split<kLaOut, NP == 3>(v, cw[x]);
     }
 #pragma unroll
     for (int t = 0; t < RT; t += 4) {
@@ -505,7 +525,7 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
       }
       if (DOTS && s == m >> 1 && g == c >> 2) L.self[out] = self;
       uint4 w[OP];
-      la_split<OP>(v, w);
+      la_split<OP, sizeof(T) == 4>(v, w);
 #pragma unroll
       for (int p = 0; p < OP; ++p) L.p[f][p][lane] = w[p];
     }
@@ -528,7 +548,7 @@ __device__ __forceinline__ void la_segment(const LaArgs& a, const LaRole& r, con
           float v[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[e] = S[2 * s + e / 4][x][e & 3];
-          la_split<OP>(v, sf[x]);
+          la_split<OP, sizeof(T) == 4>(v, sf[x]);
         }
         la_mma<NT, MT, OP, NP>(sf, af, acc);
       }

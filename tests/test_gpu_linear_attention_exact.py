@@ -1,5 +1,5 @@
 """Linear attention where fewer bits than an fp32 product's would show: results next to a border between two values
-of a 16-bit type, gradients of strong decays."""
+of a 16-bit type, gradients of strong decays, values beyond a part's range."""
 from __future__ import annotations
 
 import pytest
@@ -148,3 +148,32 @@ def test_gradients_of_decays_of_all_strengths(dev, dtype):
     size = decays64(*[x.abs() for x in qkv], g, 0.125, state.abs(), cu, dout.abs(), dstate.abs(), size=True)
     assert ((got.double() - want).abs() <= 2 * (500 / 4 + 228) * 2.0 ** -24 * size + 1e-37).all()
     assert got[:, ::90, 1].eq(0).all()
+
+
+@gpu
+@pytest.mark.parametrize("large", ["q", "k", "v", "state", "dout", "dstate"])
+def test_values_that_bf16_has_not(dev, large):
+    """fp32 values from bf16's largest to fp32's, in one tensor, the others so small that no result overflows."""
+    from test_gpu_linear_attention import backward64, close, forward64, sizes
+    import amd_tuned_torch as P
+    gen = torch.Generator().manual_seed(7)
+    t, most = 130, torch.finfo(torch.float32).max
+    shapes = {"q": (1, t, 1, 16), "k": (1, t, 1, 16), "v": (1, t, 2, 24), "state": (1, 2, 16, 24), "dout": (1, t, 2, 24),
+              "dstate": (1, 2, 16, 24)}
+    x = {name: torch.randn(*s, generator=gen).to(dev) * 2.0 ** -30 for name, s in shapes.items()}
+    x[large] = most * (1 - torch.rand(*shapes[large], generator=gen).to(dev) * 2.0 ** -8) * x[large].sign()
+    assert (x[large].abs() > 3.3895e38).any() and x[large].isfinite().all()
+    g = torch.full((1, t, 2), -0.1, device=dev)
+    leaves = [x[n].clone().requires_grad_() for n in ("q", "k", "v")] + [g.clone().requires_grad_(), x["state"].clone().requires_grad_()]
+    out, S = P.linear_attention(*leaves[:4], 0.25, initial_state=leaves[4], return_final_state=True)
+    grads = torch.autograd.grad((out, S), leaves, (x["dout"], x["dstate"]))
+    args = [leaf.detach() for leaf in leaves]
+    steps = t / 4 + 16 + 24 + 100
+    want, want_s, _ = forward64(*args[:4], 0.25, args[4], None)
+    size, size_s, _ = forward64(*sizes(*args[:4]), 0.25, args[4].abs(), None)
+    close(out.detach(), want, size, steps, "out")
+    close(S.detach(), want_s, size_s, steps, "state")
+    want = backward64(*args[:4], 0.25, args[4], None, x["dout"], x["dstate"])
+    size = backward64(*sizes(*args[:4]), 0.25, args[4].abs(), None, x["dout"].abs(), x["dstate"].abs(), size=True)
+    for name, a, b, c in zip(("dq", "dk", "dv", "dg", "dstate"), grads, want, size):
+        close(a, b, c, 2 * steps, name)
