@@ -538,7 +538,9 @@ extern "C" int atk_linear_attn_update(const atk_linear_attn_update_args* p) {
   if (p->K > kLaMaxK || p->Hv > 65535 || p->N > 65535 || p->V > (1 << 24))
     return fail(ATK_UNSUPPORTED, "linear attention update: more than %d key columns, or more than 65535 heads or sequences", kLaMaxK);
   if (p->N == 0) return ATK_OK;
-  if (!p->q || !p->k || !p->v || !p->g || !p->state || !p->out) return fail(ATK_EINVAL, "linear attention update: null pointer");
+  // (a cache of no slots has no memory; every sequence is padding then)
+  if (!p->q || !p->k || !p->v || !p->g || (!p->state && p->slots > 0) || !p->out)
+    return fail(ATK_EINVAL, "linear attention update: null pointer");
   if (!p->state_indices && p->slots < p->N) return fail(ATK_EINVAL, "linear attention update: fewer slots than sequences");
   LaStepArgs a = {};
   a.q = p->q; a.k = p->k; a.v = p->v; a.g = p->g;

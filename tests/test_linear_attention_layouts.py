@@ -62,3 +62,25 @@ def test_one_token_of_many_sequences(dev, dtype):
         out = P.linear_attention(*leaves)
         got.append((out.detach(), *torch.autograd.grad(out, leaves, dout)))
     assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
+@gpu
+@pytest.mark.parametrize("dv", [64, 66])
+def test_a_cache_without_slots(dev, dv):
+    """Every sequence is a row of padding: outputs of zeros."""
+    import amd_tuned_torch as P
+    r = lambda *s: torch.randn(*s, device=dev)  # noqa: E731
+    out = P.linear_attention_update(r(3, 1, 64), r(3, 1, 64), r(3, 2, dv), -r(3, 2).abs(), torch.zeros(0, 2, 64, dv, device=dev),
+                                    state_indices=torch.tensor([-1, 0, 7], dtype=torch.int32, device=dev))
+    assert out.shape == (3, 2, dv) and out.eq(0).all()
+
+
+def test_null_states_of_slots_are_refused():
+    from amd_tuned_torch import _native as nat
+    nat.load()
+    P = 1 << 20
+    a = nat._LinearUpdateArgs(q=P, k=P, v=P, g=P, out=P, state_indices=P, N=2, slots=1, Hk=2, Hv=4, K=64, V=64, dtype=nat.ATK_BF16,
+                              g_dtype=nat.ATK_BF16)
+    assert nat.lib().atk_linear_attn_update(ctypes.addressof(a)) == nat.ATK_EINVAL
+    a.slots, a.state_indices = 0, None
+    assert nat.lib().atk_linear_attn_update(ctypes.addressof(a)) == nat.ATK_EINVAL   # fewer slots than sequences
