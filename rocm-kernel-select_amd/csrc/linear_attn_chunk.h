@@ -58,12 +58,19 @@ template <int NP, int N, bool WIDE, typename P>
 __device__ __forceinline__ void la_parts(const float* v, P (&out)[NP]) {
   if constexpr (WIDE && NP > 1) {
     constexpr float kMost = 3.3895313892515355e38f;
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
     float rest[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const __bf16 h = (__bf16)fminf(fmaxf(v[i], -kMost), kMost);
-      out[0][i] = h;
-      rest[i] = v[i] - (float)h;
+    for (int i = 0; i < N; i += 2) {
+      // (a NaN becomes some value here, and stays one in what is left)
+      const b2 h = __builtin_convertvector((f2{__builtin_amdgcn_fmed3f(v[i], -kMost, kMost),
+                                               __builtin_amdgcn_fmed3f(v[i + 1], -kMost, kMost)}), b2);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        out[0][i + e] = h[e];
+        rest[i + e] = v[i + e] - (float)h[e];
+      }
     }
     P more[NP - 1];
     split_parts<NP - 1, N>(rest, more);
