@@ -129,9 +129,9 @@ template <typename T> int la_launch_states(const LaArgs& a, int roles, float* co
 
 inline int la_padded(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 // 16 columns of c that each wave of a workgroup has, times: two where the state's rows leave the registers for it,
-// unless that leaves more than half of the CUs without a workgroup (bf16, 4 sequences of 37 tokens, 16 heads of
-// 128 x 128: 8.5 and 7.3 us a call; 8192 tokens of 32 heads 135 and 164).  A launch of three roles has three times
-// as many (gradients, 512 tokens of 16 heads: 43 us with 64 columns, 38 with 128).
+// unless that leaves more than half of the CUs without a workgroup (C entry, call after call, bf16, 128 x 128: 4 sequences of
+// 37 tokens, 16 heads, 8.7 us and 7.7 with one; 8192 tokens of 32 heads 131 and 156).  A launch of three roles has three
+// times as many (gradients, 512 tokens of 16 heads: 39 us with two and 44 with one).
 inline int la_wide(const LaArgs& a, int rows, int cols, int roles) {
   const int64_t cus = device_cu_count() > 0 ? device_cu_count() : 256;
   return rows <= 128 && cols > 64 && (int64_t)a.slots * a.Hv * ((cols + 127) / 128) * 2 * roles > cus ? 2 : 1;

@@ -302,20 +302,24 @@ struct LaPlan {
 };
 
 // Tokens of a segment.  Segments of a sequence run at once, each going through its chunks one after the other,
-// for the price of their states.  The length is the one with the least time by what was measured, in us:
+// for the price of their states.  The length is the one with the least time by a model fitted to what was measured, in
+// us, whose workgroups on a CU are three for states of up to 64 rows, two for up to 128 and one above.  (Not of every
+// kernel: fp32 outputs of 128 rows and 128 columns have one, gradients of 64 rows two.  That is in the types' factors.)
 //   a step of 64 tokens, states and outputs together, takes 5.5 where each CU has half a workgroup (of 128 columns), 7
 //   where it has one, 10 where it has two, whatever it holds (bf16, 128 key columns; a state of 256 has one a CU and
 //   7.5, one of 64 three and 0.65 of the time; fp16 x 1.75, fp32 x 2.4), more workgroups take turns;
 //   + the states, written and read twice, at 4.4 TB/s, and the launches, 5;
 // or that of one segment a sequence, with no states between and steps of 4, 5.8 and 8.
-//   us a call with so many 64 tokens a segment, the one taken in brackets:
-//     bf16, 128 x 128: 2 x 2048 tokens of 16 heads 2: 54  [4]: 51  8: 60; 8192 of 32 heads 4: 140  [8]: 121  16: 137
-//     16 x 1024 of 16 heads 4: 139  8: 121  [whole]: 96; 256 x 256, 4096 of 8 heads 4: 96  [8]: 87  16: 140
-//     fp32, 128 x 128, 2048 of 8 heads [1]: 41  2: 41  4: 61; fp16, 64 x 100, 7 sequences, 4099 of 16 heads 1: 57  [2]: 53  4: 65
+//   us a call (C entry, ten calls one after the other, the best of four such) with so many 64 tokens a segment, the one
+//   taken in brackets:
+//     bf16, 128 x 128: 2 x 2048 tokens of 16 heads 2: 57  [4]: 55  8: 63; 8192 of 32 heads 4: 152  [8]: 132  16: 147
+//     16 x 1024 of 16 heads 4: 149  8: 127  [whole]: 104; 256 x 256, 4096 of 8 heads 4: 98  [8]: 90  16: 149
+//     fp32, 128 x 128, 2048 of 8 heads [1]: 43  2: 44  4: 64; fp16, 64 x 100, 7 sequences, 4099 of 16 heads 1: 57  [2]: 54  4: 67
+// The gradients take the same length: for 2 x 2048 tokens 124, with 8 117; for 2048 in fp32 108, with 2 104; else the least.
 // Lengths of packed sequences are on the device.  The longest is taken for two and a half times the average, and
 // 0.012 us for each workgroup that finds no segment.  A segment has at most 1024 tokens or four times the average, lest a
-// long sequence among short ones be left to a workgroup a head (bf16, 128 x 128, 16 heads: one of 8192 and 64 of 64
-// tokens, whole 663, in segments 136; where all are short that costs, 300 of 64 tokens, 107 and 112).
+// long sequence among short ones be left to a workgroup a head (bf16, 128 x 128, 16 heads: one of 8192 amid 64 of 64
+// tokens, whole 756, in segments 187; where all are short that costs, 300 of 64 tokens, 105 and 115).
 int64_t la_segment_tokens(const atk_linear_attn_args* p) {
   const double cus = device_cu_count() > 0 ? device_cu_count() : 256, n = (double)(p->N > 0 ? p->N : 1);
   const double chunks = p->cu_seqlens ? (double)p->T / 64 / n : (double)((p->T + 63) / 64);

@@ -9,9 +9,10 @@
 // meanwhile; products over tokens read them transposed (ds_read_tr).
 //
 // Measured, bf16: 8192 tokens, 16 and 32 heads of 128 x 128, in 16 segments: states 44 us (100 MB read, 31 written), outputs
-// 87 (134 + 31 and 67).  The matrix units are busy for 10 and 21 us of these; a third of a wave's cycles it waits for
-// memory or LDS, a third for its turn or a result, a quarter it issues vector instructions, most of them the
-// splitting of S, of P and of the decayed c in parts: two workgroups a CU, no resource full.  Without an effect:
+// 100 (134 + 31 and 67).  LDS is busy for 11 and 28 us of these, 34 and 41 % of that with bank conflicts, the matrix units
+// for 10 and 26; a third of a wave's cycles it waits for memory or LDS, a third for its turn or a result, a quarter it
+// issues vector instructions, most of them the splitting of S, of P and of the decayed c in parts.  Two workgroups a
+// CU.  Without an effect:
 // loads two chunks ahead, eight waves, chunks of 32, other pitches, raised priority.  S, P and the decayed c keep all
 // their bits: two parts of S and P towards 16-bit outputs took a call from 143 to 133 us, and rounded results to the
 // wrong side that are within 2^-17 of half way between two values.
@@ -744,7 +745,7 @@ struct LaStateLds {
 };
 
 // (64 columns a workgroup, also where there are more: it is bound by loads on their way, and twice as many
-// workgroups have more of them; 8192 tokens, 32 heads of 128 x 128: 139 us a call against 145.)
+// workgroups have more of them: 4 % off a call of 8192 tokens of 32 heads of 128 x 128.)
 // What a segment adds to the state, and its decay: b and c alone.  The last segment's (in reverse the
 // first's) nobody asks for.
 template <typename T, int DA, bool rev>

@@ -7,8 +7,8 @@
 // HBM-bound: every element is read once and written once.  The angles are products in 64 bits, with what their
 // rounding leaves, brought to a part of a turn there (a position of 10^6 has an error of 0.06 in an fp32 product, one
 // of 2^40 7e-5 in a product rounded to 64 bits), and sine and cosine are taken once for each token and pair by a workgroup that has all heads of its tokens: the
-// table lies in LDS while they stream through.  8192 tokens of 32 and 16 heads of 128 columns, bf16: 42 us for
-// 201 MB, 4.8 TB/s (a large copy reaches 5.05); 64 single tokens 3.5 us, a launch's own time.
+// table lies in LDS while they stream through.  8192 tokens of 32 and 16 heads of 128 columns, bf16: 43 us for
+// 201 MB, 4.7 TB/s (a large copy reaches 5.05); 64 single tokens 3.5 us, a launch's own time.
 #include "atk_common.h"
 
 namespace atk {
