@@ -743,7 +743,7 @@ int atk_linear_attn_update(const atk_linear_attn_update_args* a);
  * one decay a head (its strides of the first two axes 0).  The workspace (16-byte aligned, contents
  * ignored) has atk_linear_attn_workspace_bytes of the same arguments: 0 for sequences that one workgroup a
  * head goes through.  K up to 256, K and V of 16 bytes or more, K V below 2^29; up to 65535 sequences and value
- * heads, tokens of one tensor less than 2^22 elements apart; otherwise ATK_UNSUPPORTED. */
+ * heads, tokens of one tensor less than 2^22 elements apart where there is more than one; otherwise ATK_UNSUPPORTED. */
 typedef struct atk_linear_attn_args {
   const void* q; const void* k; const void* v; const void* g;
   const void* initial_state; void* final_state; void* out; const int* cu_seqlens;
@@ -757,8 +757,9 @@ size_t atk_linear_attn_workspace_bytes(const atk_linear_attn_args* a);
 int atk_linear_attn_fwd(const atk_linear_attn_args* a);
 
 /* Its backward, arguments as for atk_gated_delta_bwd.  dg (NULL: not wanted) is (N, T, Hv), or [Hv] with
- * fixed_decay; where a decay is below exp(-120) it is 0.  Sums over heads, columns and tokens have a fixed order.
- * Up to 2^22 value columns of all heads. */
+ * fixed_decay; where a decay is below exp(-120) it is 0.  It has fp32 roundings of terms that each have a decay: beside
+ * tokens of weak decays those of strong ones are right by the size of the weak ones' gradients.  Sums over heads,
+ * columns and tokens have a fixed order.  Up to 2^22 value columns of all heads. */
 size_t atk_linear_attn_bwd_workspace_bytes(const atk_linear_attn_args* a);
 int atk_linear_attn_bwd(const atk_linear_attn_args* a, const void* dout, const void* dfinal_state, void* dq, void* dk,
                         void* dv, void* dg, void* dinitial_state);

@@ -12,10 +12,9 @@
 // 100 (134 + 31 and 67).  LDS is busy for 11 and 28 us of these, 34 and 41 % of that with bank conflicts, the matrix units
 // for 10 and 26; a third of a wave's cycles it waits for memory or LDS, a third for its turn or a result, a quarter it
 // issues vector instructions, most of them the splitting of S, of P and of the decayed c in parts.  Two workgroups a
-// CU.  Without an effect:
-// loads two chunks ahead, eight waves, chunks of 32, other pitches, raised priority.  S, P and the decayed c keep all
-// their bits: two parts of S and P towards 16-bit outputs took a call from 143 to 133 us, and rounded results to the
-// wrong side that are within 2^-17 of half way between two values.
+// CU.  Without an effect: loads two chunks ahead, eight waves, chunks of 32, other pitches, raised priority.  S, P and the
+// decayed c keep all their bits: two parts of S and P towards 16-bit outputs took a call from 143 to 133 us, and
+// rounded results to the wrong side that are within 2^-17 of half way between two values.
 #pragma once
 #include <limits.h>
 

@@ -117,11 +117,11 @@ def test_gradients_of_strong_decays(dev, cu, hk, hv, dk, dv, dtype):
     mag = [x.abs() for x in (*qkv, dout, state, dstate)]
     for s0, s1, m0, m1 in ((state, dstate, mag[4], mag[5]), (None, None, None, None)):
         for rate in (-0.1, -2.0, -5.0, -10.0, -20.0, -40.0):
+            g = torch.full((1, cu[-1], hv), rate, device=dev)
+            want = decays64(*qkv, g, 0.125, s0, cu, dout, s1)
+            size = decays64(*mag[:3], g, 0.125, m0, cu, mag[3], m1, size=True)
             for fixed in (False, True):
-                g = torch.full((hv,) if fixed else (1, cu[-1], hv), rate, device=dev)
-                got = decay_gradient(P, qkv, g, s0, cu, dout, s1)
-                want = decays64(*qkv, g, 0.125, s0, cu, dout, s1)
-                size = decays64(*mag[:3], g, 0.125, m0, cu, mag[3], m1, size=True)
+                got = decay_gradient(P, qkv, g[0, 0] if fixed else g, s0, cu, dout, s1)
                 if fixed:
                     want, size = want.sum((0, 1)), size.sum((0, 1))
                 assert ((got.double() - want).abs() <= steps * 2.0 ** -24 * size + 1e-37).all(), (rate, fixed)
