@@ -31,7 +31,8 @@ struct LaRole {
   void* out;                               // T (B, T, heads of out, CD), or
   float* parts;                            // fp32 sums [head of the group * a_tiles + a tile][B T][Hk][CD]
   float* dots;                             // [tile][Hv][B T]: e_i . out_i over the tile's columns, but for j = i
-  const float* x_last; const float* x_between; float* x_out;  // [tile][slot][Hv]: sum of S, but for the last token, and the other direction's state
+  // [tile][slot][Hv]: inner product of S, without the last token's term, and the other direction's state
+  const float* x_last; const float* x_between; float* x_out;
 };
 
 struct LaArgs {

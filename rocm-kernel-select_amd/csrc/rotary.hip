@@ -6,8 +6,8 @@
 //
 // HBM-bound: every element is read once and written once.  The angles are products in 64 bits, with what their
 // rounding leaves, brought to a part of a turn there (a position of 10^6 has an error of 0.06 in an fp32 product, one
-// of 2^40 7e-5 in a product rounded to 64 bits), and sine and cosine are taken once for each token and pair by a workgroup that has all heads of its tokens: the
-// table lies in LDS while they stream through.  8192 tokens of 32 and 16 heads of 128 columns, bf16: 43 us for
+// of 2^40 7e-5 in a product rounded to 64 bits), and sine and cosine are taken once for each token and pair by a
+// workgroup that has all heads of its tokens: the table lies in LDS while they stream through.  8192 tokens of 32 and 16 heads of 128 columns, bf16: 43 us for
 // 201 MB, 4.7 TB/s (a large copy reaches 5.05); 64 single tokens 3.5 us, a launch's own time.
 #include "atk_common.h"
 
@@ -36,8 +36,8 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
   return r;
 }
 
-// position * freq in turns, without whole ones: within 2^-40 of a turn for any position and freq up to 1, 2^-52 of the turns of
-// nearer ones.  The position's last 11 bits are apart, so the rest has no rounding in 64 bits; products keep what
+// position * freq in turns, without whole ones: within 2^-40 of a turn for any position and freq up to 1, 2^-52 of the
+// turns of nearer ones.  The position's last 11 bits are apart, so the rest has no rounding in 64 bits; products keep what
 // theirs leaves, and 1 / (2 pi) has 107 bits.  (Contracted, a product would be taken with that twice.)
 __device__ __forceinline__ double part_of_turn(int64_t pos, double freq) {
 #pragma clang fp contract(off)
